@@ -337,7 +337,7 @@ def _plain_plan(s):
     slots = table_out[of, (position // b).clamp(0, width - 1)].long() * b + position % b
     table.copy_(table_out)
     free.copy_(free_out)
-    taken = torch.where(short, 0, offset + need).amax()
+    taken = torch.where(served & (need > 0), offset + need, 0).amax()
     return {"lengths": lengths.int(), "starts": starts.int(), "slots": torch.where(there, slots, -1),
             "ring": torch.stack([head + taken, tail + gives.sum(), torch.where(short, need, 0).sum(), wide.sum()]), "table": table, "free": free}
 
