@@ -30,7 +30,8 @@ BUILD = HERE / "_build"
 INCLUDE = REPO / "include"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-LIB_SOURCES = ["dk_abi.cu", "dk_gemv.cu", "dk_stream.cu", "dk_quant.cu", "dk_shard.cu"]
+LIB_SOURCES = ["dk_abi.cu", "dk_gemv.cu", "dk_stream.cu", "dk_quant.cu", "dk_shard.cu",
+               "dk_cache.cu", "dk_attend.cu", "dk_norm.cu"]
 COMMON_DEPS = [CSRC / "dk_device.cuh", CSRC / "dk_host.h", CSRC / "dk_batch.cuh", INCLUDE / "dk_w4a16.h"]
 LIB = PKG / "libdk_b200.so"
 

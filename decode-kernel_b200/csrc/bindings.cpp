@@ -10,13 +10,22 @@
 //   stream_recommended_blocks(), last_kernel_stamp()
 // and adds: w4a16_gemv_out (caller-provided y, optional PDL launch),
 // workspace_bytes, quantize_pack / unpack_to_int / dequantize on the GPU,
-// device_error.  Every C-ABI status other than DK_OK becomes a RuntimeError.
+// device_error, and the rest of a decode step: Cache8 (a paged 8-bit cache's
+// tensors, checked once), cache_plan, cache_append, cache_attention, block_norm.
+// Every C-ABI status other than DK_OK becomes a RuntimeError.
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <cmath>
 #include <cstdint>
+#include <map>
+#include <mutex>
+#include <optional>
 #include <string>
+#include <tuple>
+#include <utility>
 
 #include "dk_w4a16.h"
 
@@ -219,6 +228,321 @@ torch::Tensor dequantize(torch::Tensor packed, torch::Tensor scales) {
   return w;
 }
 
+// ---------------------------------------------------------------------------
+// The paged 8-bit cache and the norms between blocks.
+// ---------------------------------------------------------------------------
+using OptTensor = std::optional<torch::Tensor>;
+
+// A cache's four tensors and their description, checked once.
+struct Cache8 {
+  torch::Tensor k, v, k_scale, v_scale;
+  dk_cache8 c;
+
+  Cache8(torch::Tensor k_, torch::Tensor v_, torch::Tensor ks, torch::Tensor vs)
+      : k(std::move(k_)), v(std::move(v_)), k_scale(std::move(ks)), v_scale(std::move(vs)) {
+    TORCH_CHECK(k.is_cuda() && v.is_cuda() && k_scale.is_cuda() && v_scale.is_cuda(),
+                "the cache's tensors must be CUDA tensors");
+    TORCH_CHECK(k.device() == v.device() && k.device() == k_scale.device() &&
+                    k.device() == v_scale.device(),
+                "the cache's tensors must be on one device");
+    TORCH_CHECK(k.scalar_type() == v.scalar_type() &&
+                    (k.scalar_type() == torch::kInt8 || k.scalar_type() == torch::kFloat8_e4m3fn),
+                "k and v must both be int8 or both float8_e4m3fn");
+    TORCH_CHECK(k.dim() == 4 && v.sizes() == k.sizes(),
+                "k and v must be [blocks, kv_heads, block_size, head_dim]");
+    TORCH_CHECK(k.size(0) >= 1 && k.size(0) <= INT32_MAX && k.size(1) >= 1 && k.size(1) <= 65535,
+                "blocks and kv_heads out of range");
+    TORCH_CHECK(k.size(2) >= 16 && k.size(2) <= 256 && k.size(2) % 16 == 0,
+                "block_size must be a multiple of 16 in 16..256");
+    TORCH_CHECK(k.size(3) == 64 || k.size(3) == 128 || k.size(3) == 256,
+                "head_dim must be 64, 128 or 256");
+    TORCH_CHECK(k.stride(3) == 1 && v.stride(3) == 1, "head_dim must be contiguous");
+    for (int i = 0; i < 3; ++i)
+      TORCH_CHECK(k.stride(i) % 32 == 0 && v.stride(i) % 32 == 0 && k.stride(i) >= 0 &&
+                      v.stride(i) >= 0,
+                  "the cache's strides must be multiples of 32");
+    TORCH_CHECK((reinterpret_cast<uintptr_t>(k.data_ptr()) & 31u) == 0 &&
+                    (reinterpret_cast<uintptr_t>(v.data_ptr()) & 31u) == 0,
+                "k and v must be 32-byte aligned");
+    TORCH_CHECK(k_scale.scalar_type() == torch::kFloat32 && v_scale.scalar_type() == torch::kFloat32,
+                "scales must be fp32");
+    for (const torch::Tensor* s : {&k_scale, &v_scale})
+      TORCH_CHECK(s->dim() == 2 && s->size(0) == k.size(0) && s->size(1) == k.size(1) &&
+                      s->is_contiguous(),
+                  "scales must be contiguous [blocks, kv_heads]");
+    c.k = k.data_ptr();
+    c.v = v.data_ptr();
+    c.k_scale = k_scale.data_ptr<float>();
+    c.v_scale = v_scale.data_ptr<float>();
+    c.blocks = static_cast<int>(k.size(0));
+    c.kv_heads = static_cast<int>(k.size(1));
+    c.block_size = static_cast<int>(k.size(2));
+    c.head_dim = static_cast<int>(k.size(3));
+    c.code = k.scalar_type() == torch::kInt8 ? DK_INT8 : DK_E4M3;
+    c.k_block_stride = k.stride(0);
+    c.k_head_stride = k.stride(1);
+    c.k_token_stride = k.stride(2);
+    c.v_block_stride = v.stride(0);
+    c.v_head_stride = v.stride(1);
+    c.v_token_stride = v.stride(2);
+  }
+};
+
+dk_dtype half_type(const torch::Tensor& t, const char* what) {
+  if (t.scalar_type() == torch::kFloat16) return DK_FP16;
+  TORCH_CHECK(t.scalar_type() == torch::kBFloat16, what, " must be fp16 or bf16");
+  return DK_BF16;
+}
+
+void check_ints(const torch::Tensor& t, torch::ScalarType type, int64_t n, const torch::Device& device,
+                const char* what) {
+  TORCH_CHECK(t.is_cuda() && t.device() == device, what, " must be on the call's CUDA device");
+  TORCH_CHECK(t.scalar_type() == type, what, " must be ", type);
+  TORCH_CHECK(t.dim() == 1 && t.size(0) == n && t.is_contiguous(), what, " must be contiguous [" + std::to_string(n) + "]");
+}
+
+void check_table(const torch::Tensor& t, int64_t requests, const torch::Device& device) {
+  TORCH_CHECK(t.is_cuda() && t.device() == device, "block_table must be on the call's CUDA device");
+  TORCH_CHECK(t.scalar_type() == torch::kInt32 && t.dim() == 2 && t.size(0) == requests &&
+                  t.size(1) >= 1 && t.stride(1) == 1 && t.stride(0) >= t.size(1) &&
+                  t.stride(0) <= INT32_MAX,
+              "block_table must be int32 [requests, max_blocks] with contiguous rows");
+}
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> cache_plan(
+    torch::Tensor held, torch::Tensor fresh, torch::Tensor block_table, torch::Tensor free_blocks,
+    torch::Tensor ring, int64_t block_size, int64_t tokens, OptTensor lengths, OptTensor starts,
+    OptTensor slots, OptTensor ring_out) {
+  TORCH_CHECK(held.is_cuda(), "held must be a CUDA tensor");
+  TORCH_CHECK(held.dim() == 1, "held must be [requests]");
+  const torch::Device device = held.device();
+  const int64_t n = held.size(0);
+  TORCH_CHECK(n <= DK_PLAN_MAX_REQUESTS, "at most " + std::to_string(DK_PLAN_MAX_REQUESTS) + " requests");
+  TORCH_CHECK(tokens >= 0 && tokens <= INT32_MAX, "tokens out of range");
+  TORCH_CHECK(block_size >= 16 && block_size <= 256 && block_size % 16 == 0,
+              "block_size must be a multiple of 16 in 16..256");
+  check_ints(held, torch::kInt32, n, device, "held");
+  check_ints(fresh, torch::kInt32, n, device, "fresh");
+  check_table(block_table, n, device);
+  TORCH_CHECK(free_blocks.numel() <= INT32_MAX, "free_blocks is too long");
+  check_ints(free_blocks, torch::kInt32, free_blocks.numel(), device, "free_blocks");
+  check_ints(ring, torch::kInt64, 4, device, "ring");
+  const c10::cuda::CUDAGuard guard(device);
+  const auto ints = held.options();
+  const auto longs = ring.options();
+  auto given = [&](OptTensor& t, torch::ScalarType type, int64_t size, const char* what) {
+    if (t) check_ints(*t, type, size, device, what);
+    else t = torch::empty({size}, type == torch::kInt32 ? ints : longs);
+    return *t;
+  };
+  torch::Tensor l = given(lengths, torch::kInt32, n, "lengths");
+  torch::Tensor s = given(starts, torch::kInt32, n + 1, "starts");
+  torch::Tensor m = given(slots, torch::kInt64, tokens, "slots");
+  torch::Tensor r = given(ring_out, torch::kInt64, 4, "ring_out");
+  check_status(
+      dk_cache_plan(held.data_ptr<int32_t>(), fresh.data_ptr<int32_t>(), static_cast<int>(n),
+                    block_table.data_ptr<int32_t>(), static_cast<int>(block_table.size(1)),
+                    static_cast<int>(n > 1 ? block_table.stride(0) : block_table.size(1)),
+                    static_cast<int>(block_size), free_blocks.data_ptr<int32_t>(),
+                    static_cast<int>(free_blocks.numel()), ring.data_ptr<int64_t>(),
+                    r.data_ptr<int64_t>(), l.data_ptr<int32_t>(), s.data_ptr<int32_t>(),
+                    m.data_ptr<int64_t>(), static_cast<int>(tokens),
+                    at::cuda::getCurrentCUDAStream().stream()),
+      "cache_plan");
+  return {l, s, m, r};
+}
+
+void cache_append(torch::Tensor k, torch::Tensor v, torch::Tensor slots, const Cache8& cache) {
+  const torch::Device device = cache.k.device();
+  TORCH_CHECK(k.is_cuda() && v.is_cuda() && k.device() == device && v.device() == device,
+              "k and v must be CUDA tensors on the cache's device");
+  TORCH_CHECK(k.dim() == 3 && k.size(1) == cache.c.kv_heads && k.size(2) == cache.c.head_dim,
+              "k must be [tokens, kv_heads, head_dim]");
+  TORCH_CHECK(v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type(),
+              "v must have k's shape and type");
+  TORCH_CHECK(k.size(0) <= INT32_MAX, "too many tokens");
+  const dk_dtype type = half_type(k, "k and v");
+  check_ints(slots, torch::kInt64, k.size(0), device, "slots");
+  const c10::cuda::CUDAGuard guard(device);
+  // A lane reads head_dim / 32 neighbouring values at once: re-home other views.
+  const int64_t piece = cache.c.head_dim / 32;
+  auto fits = [&](const torch::Tensor& t) {
+    return t.stride(2) == 1 && t.stride(0) % piece == 0 && t.stride(1) % piece == 0 &&
+           reinterpret_cast<uintptr_t>(t.data_ptr()) % (2 * piece) == 0;
+  };
+  const torch::Tensor kc = fits(k) ? k : k.clone(at::MemoryFormat::Contiguous);
+  const torch::Tensor vc = fits(v) ? v : v.clone(at::MemoryFormat::Contiguous);
+  check_status(dk_cache_append(&cache.c, kc.data_ptr(), vc.data_ptr(), type,
+                               static_cast<int>(k.size(0)), kc.stride(0), kc.stride(1),
+                               vc.stride(0), vc.stride(1), slots.data_ptr<int64_t>(),
+                               at::cuda::getCurrentCUDAStream().stream()),
+               "cache_append");
+}
+
+// The attention workspace: one for each device, stream and head size, zeroed
+// when it is made; every call leaves it ready for the next on that stream.  A
+// call that is being captured gets one of its own with its zeroing in the
+// graph, since the graph may be replayed beside later calls of the stream.
+torch::Tensor attention_workspace(int head_dim, const at::cuda::CUDAStream& stream) {
+  const auto options = torch::TensorOptions().dtype(torch::kUInt8).device(stream.device());
+  const int64_t bytes = static_cast<int64_t>(dk_cache_attention_workspace_bytes(head_dim));
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
+    return torch::zeros({bytes}, options);
+  static std::mutex mu;
+  // Never freed: the process may end after the CUDA context.
+  static auto* kept = new std::map<std::tuple<int, cudaStream_t, int>, torch::Tensor>();
+  const std::lock_guard<std::mutex> lock(mu);
+  torch::Tensor& w = (*kept)[{stream.device_index(), stream.stream(), head_dim}];
+  if (!w.defined()) w = torch::zeros({bytes}, options);
+  return w;
+}
+
+std::tuple<torch::Tensor, OptTensor> cache_attention(torch::Tensor q, const Cache8& cache,
+                                                     torch::Tensor block_table, torch::Tensor lengths,
+                                                     OptTensor starts, std::optional<double> scale,
+                                                     bool causal, int64_t window, OptTensor out,
+                                                     bool want_lse) {
+  const torch::Device device = cache.k.device();
+  TORCH_CHECK(q.is_cuda() && q.device() == device, "q must be a CUDA tensor on the cache's device");
+  TORCH_CHECK(q.dim() == 3 && q.size(2) == cache.c.head_dim, "q must be [tokens, q_heads, head_dim]");
+  TORCH_CHECK(q.size(0) <= INT32_MAX && q.size(1) >= 1 && q.size(1) % cache.c.kv_heads == 0 &&
+                  q.size(1) <= INT32_MAX,
+              "q_heads must be a multiple of kv_heads");
+  TORCH_CHECK(window >= 0 && window <= INT32_MAX && (window == 0 || causal),
+              "window must be 0 (none) or positive, and causal");
+  const int64_t n = lengths.size(0);
+  TORCH_CHECK(n <= INT32_MAX, "too many requests");
+  check_ints(lengths, torch::kInt32, n, device, "lengths");
+  check_table(block_table, n, device);
+  if (starts) check_ints(*starts, torch::kInt32, n + 1, device, "starts");
+  else TORCH_CHECK(q.size(0) == n, "without starts q must have one token for each request");
+  const c10::cuda::CUDAGuard guard(device);
+  dk_cache_attention_args a;
+  a.dtype = half_type(q, "q");
+  const bool fits = q.stride(2) == 1 && q.stride(0) % 8 == 0 && q.stride(1) % 8 == 0 && aligned16(q);
+  const torch::Tensor qc = fits ? q : q.clone(at::MemoryFormat::Contiguous);
+  torch::Tensor o;
+  if (out) {
+    o = *out;
+    TORCH_CHECK(o.is_cuda() && o.device() == device && o.scalar_type() == q.scalar_type() &&
+                    o.sizes() == q.sizes() && o.is_contiguous() && aligned16(o),
+                "out must be contiguous, with q's shape, type and device");
+  } else {
+    o = torch::empty(q.sizes(), q.options());
+  }
+  OptTensor lse;
+  if (want_lse) lse = torch::empty({q.size(0), q.size(1)}, q.options().dtype(torch::kFloat32));
+  const at::cuda::CUDAStream stream = at::cuda::getCurrentCUDAStream();
+  const torch::Tensor ws = attention_workspace(cache.c.head_dim, stream);
+  a.cache = cache.c;
+  a.q = qc.data_ptr();
+  a.out = o.data_ptr();
+  a.lse = want_lse ? lse->data_ptr<float>() : nullptr;
+  a.q_token_stride = qc.stride(0);
+  a.q_head_stride = qc.stride(1);
+  a.block_table = block_table.data_ptr<int32_t>();
+  a.max_blocks = static_cast<int>(block_table.size(1));
+  a.table_stride = static_cast<int>(n > 1 ? block_table.stride(0) : block_table.size(1));
+  a.lengths = lengths.data_ptr<int32_t>();
+  a.starts = starts ? starts->data_ptr<int32_t>() : nullptr;
+  a.requests = static_cast<int>(n);
+  a.tokens = static_cast<int>(q.size(0));
+  a.q_heads = static_cast<int>(q.size(1));
+  a.scale = static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(cache.c.head_dim)));
+  a.causal = causal ? 1 : 0;
+  a.window = static_cast<int>(window);
+  check_status(dk_cache_attention(&a, ws.data_ptr(), static_cast<size_t>(ws.numel()), stream.stream()),
+               "cache_attention");
+  return {o, lse};
+}
+
+std::tuple<torch::Tensor, OptTensor> block_norm(torch::Tensor residual, OptTensor y, int kind,
+                                                OptTensor post_weight, OptTensor post_bias,
+                                                OptTensor gate, int act, double residual_scale,
+                                                double block_scale, OptTensor pre_weight,
+                                                OptTensor pre_bias, double eps, bool inplace) {
+  TORCH_CHECK(residual.is_cuda(), "residual must be a CUDA tensor");
+  TORCH_CHECK(residual.dim() >= 1 && residual.size(-1) >= 1 && residual.size(-1) <= 32768,
+              "residual must be [..., dim] with dim in 1..32768");
+  TORCH_CHECK(y || pre_weight, "nothing to do: neither y nor pre_weight");
+  TORCH_CHECK(y || !(gate || post_weight), "gate and post_weight belong to y");
+  TORCH_CHECK(post_weight || !post_bias, "post_bias needs post_weight");
+  TORCH_CHECK(pre_weight || !pre_bias, "pre_bias needs pre_weight");
+  const torch::Device device = residual.device();
+  const int64_t dim = residual.size(-1), rows = residual.numel() / dim;
+  TORCH_CHECK(rows <= INT32_MAX, "too many rows");
+  dk_block_norm_args a{};
+  a.dtype = half_type(y ? *y : *pre_weight, "y and the weights");
+  const torch::ScalarType type = y ? y->scalar_type() : pre_weight->scalar_type();
+  TORCH_CHECK(residual.scalar_type() == type || residual.scalar_type() == torch::kFloat32,
+              "residual must have y's type or be fp32");
+  a.residual_dtype = residual.scalar_type() == torch::kFloat32 ? DK_FP32 : a.dtype;
+  auto weight = [&](const OptTensor& t, const char* what) -> const void* {
+    if (!t) return nullptr;
+    TORCH_CHECK(t->is_cuda() && t->device() == device && t->scalar_type() == type && t->dim() == 1 &&
+                    t->size(0) == dim && t->is_contiguous(),
+                what, " must be contiguous [dim] with y's type, on residual's device");
+    return t->data_ptr();
+  };
+  const c10::cuda::CUDAGuard guard(device);
+  // Rows of any tensor: 2-D ones keep their row stride, others are contiguous.
+  auto in_rows = [&](const torch::Tensor& t) {
+    return (t.dim() == 2 && t.stride(1) == 1) || t.is_contiguous() ? t : t.contiguous();
+  };
+  auto row_stride = [&](const torch::Tensor& t) { return t.dim() == 2 ? t.stride(0) : dim; };
+  const torch::Tensor r = inplace ? residual : in_rows(residual);
+  TORCH_CHECK(!inplace || (r.dim() == 2 && r.stride(1) == 1) || r.is_contiguous(),
+              "an in-place residual must have contiguous rows");
+  a.residual = r.data_ptr();
+  a.residual_stride = row_stride(r);
+  torch::Tensor yc, gc, h, out = residual;
+  if (y) {
+    TORCH_CHECK(y->is_cuda() && y->device() == device && y->sizes() == residual.sizes(),
+                "y must have residual's shape and device");
+    yc = in_rows(*y);
+    a.y = yc.data_ptr();
+    a.y_stride = row_stride(yc);
+  }
+  if (gate) {
+    TORCH_CHECK(gate->is_cuda() && gate->device() == device && gate->scalar_type() == type,
+                "gate must have y's type and device");
+    const bool channel = gate->dim() == 1 && gate->size(0) == dim;
+    const bool full = gate->sizes() == residual.sizes();
+    bool row = !full && gate->dim() == residual.dim() && gate->size(-1) == 1;
+    for (int64_t i = 0; row && i + 1 < residual.dim(); ++i) row = gate->size(i) == residual.size(i);
+    TORCH_CHECK(channel || full || row, "gate must be [dim], [..., 1] or [..., dim]");
+    gc = full ? in_rows(*gate) : gate->contiguous();
+    a.gate = gc.data_ptr();
+    a.gate_column_stride = row ? 0 : 1;
+    a.gate_stride = full ? row_stride(gc) : row ? 1 : 0;
+  }
+  a.post_weight = weight(post_weight, "post_weight");
+  a.post_bias = weight(post_bias, "post_bias");
+  a.pre_weight = weight(pre_weight, "pre_weight");
+  a.pre_bias = weight(pre_bias, "pre_bias");
+  // Without y and with a scale of 1 the residual stays what it is.
+  if (y || residual_scale != 1.0) {
+    if (!inplace) out = torch::empty(residual.sizes(), residual.options());
+    a.residual_out = out.data_ptr();
+    a.residual_out_stride = inplace ? row_stride(r) : dim;
+  }
+  OptTensor result;
+  if (pre_weight) {
+    result = torch::empty(residual.sizes(), pre_weight->options());
+    a.h = result->data_ptr();
+    a.h_stride = dim;
+  }
+  a.rows = static_cast<int>(rows);
+  a.dim = static_cast<int>(dim);
+  a.kind = static_cast<dk_norm_kind>(kind);
+  a.act = static_cast<dk_gate_act>(act);
+  a.residual_scale = static_cast<float>(residual_scale);
+  a.block_scale = static_cast<float>(block_scale);
+  a.eps = static_cast<float>(eps);
+  check_status(dk_block_norm(&a, at::cuda::getCurrentCUDAStream().stream()), "block_norm");
+  return {out, result};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -246,5 +570,24 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("torch_cuda_scale") = false);
   m.def("unpack_to_int", &unpack_to_int, "GPU unpack_to_int", py::arg("packed"));
   m.def("dequantize", &dequantize, "GPU dequantize to fp32", py::arg("packed"), py::arg("scales"));
+  py::class_<Cache8>(m, "Cache8")
+      .def(py::init<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor>(), py::arg("k"),
+           py::arg("v"), py::arg("k_scale"), py::arg("v_scale"));
+  m.def("cache_plan", &cache_plan, "Block tables and slot maps of a step", py::arg("held"),
+        py::arg("fresh"), py::arg("block_table"), py::arg("free_blocks"), py::arg("ring"),
+        py::arg("block_size"), py::arg("tokens"), py::arg("lengths") = py::none(),
+        py::arg("starts") = py::none(), py::arg("slots") = py::none(),
+        py::arg("ring_out") = py::none());
+  m.def("cache_append", &cache_append, "New keys and values into a paged 8-bit cache", py::arg("k"),
+        py::arg("v"), py::arg("slots"), py::arg("cache"));
+  m.def("cache_attention", &cache_attention, "Attention over a paged 8-bit cache", py::arg("q"),
+        py::arg("cache"), py::arg("block_table"), py::arg("lengths"), py::arg("starts") = py::none(),
+        py::arg("scale") = py::none(), py::arg("causal") = true, py::arg("window") = 0,
+        py::arg("out") = py::none(), py::arg("lse") = false);
+  m.def("block_norm", &block_norm, "Norms, gate and residual between two blocks",
+        py::arg("residual"), py::arg("y"), py::arg("kind"), py::arg("post_weight"),
+        py::arg("post_bias"), py::arg("gate"), py::arg("act"), py::arg("residual_scale"),
+        py::arg("block_scale"), py::arg("pre_weight"), py::arg("pre_bias"), py::arg("eps"),
+        py::arg("inplace"));
   m.def("version", []() { return std::string(dk_version()); });
 }

@@ -1,0 +1,815 @@
+// dk_attend.cu -- attention of a step's queries over a paged cache held in 8
+// bits (int8 or e4m3) with one fp32 scale per page and KV head.
+//
+// For a query row q of KV head h and the cached tokens j its mask leaves,
+//   s_j = scale * ks[page(j)] * (q . Kcode_j)         out = sum_j p_j V_j
+//   p_j = exp(s_j) / sum_i exp(s_i)                   V_j = vs[page(j)] * Vcode_j
+// computed in one pass with a running maximum.  The page's V scale goes into
+// the exponent: with t_j = s_j log2(e) + log2(vs_j) and w_j = 2^(t_j - m),
+//   out = (sum_j w_j Vcode_j) / (sum_j w_j / vs_j),
+// so the codes enter the tensor core unscaled (int8 and e4m3 are exact in
+// fp16) and w_j is at most 2^8, whatever the scales.  w_j is rounded to fp16
+// (11 bits; a relative 2^-12 on each weight, the size of the rounding of an
+// fp16 output); scores, maxima, sums and outputs are fp32.
+//
+// What bounds it: the cache's bytes from HBM.  Up to 16 query rows per KV head
+// the arithmetic is 4 * rows flops per byte pair, far below the tensor cores'
+// rate, so the tiles are built for streaming: a unit of 16 tokens goes from
+// global memory straight into the registers of one warp in the layout of the
+// m16n8k16 fragments, with the tokens (then the channels) as the 16 rows and
+// the query rows as the 8 columns, so no row of the tile is padding when 8
+// query heads share a KV head.
+//   K: lane (g, c) holds 2 rows (tokens g, g + 8), channels 32c..32c+31: word s
+//      of a row is its part of the s-th k step (the sum over channels may run in
+//      any order, so q is loaded in the same one).
+//   V: lane (g, c) holds tokens 2c, 2c+1, 2c+8, 2c+9, channels 16g..16g+15: byte
+//      pairs of two tokens are interleaved with PRMT and converted.
+//   P: the score tile is [token][row]; movmatrix transposes it into the second
+//      product's operand.
+// Each warp instruction reads whole 128-byte lines, nothing passes through
+// shared memory, and the next unit's loads are issued as soon as a fragment's
+// registers are free.
+//
+// Split: the units of all (request, KV head, row tile) segments form one line,
+// which the CTAs share evenly, and each CTA's warps share its part evenly, so
+// the split follows the lengths as they are on the device; no host sync and no
+// padding to the longest.  A segment that a warp covers alone is written at
+// once; the other parts meet in shared memory, and a segment that several CTAs
+// share is joined by whichever of them arrives last, always in the same order
+// of parts.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "dk_device.cuh"
+#include "dk_host.h"
+
+namespace dk {
+namespace {
+
+constexpr int kUnit = 16;             // tokens of a unit
+constexpr int kMaxRequests = 8192;    // requests of one launch (their prefix sums are in shared memory)
+constexpr float kFarBelow = -1e30f;   // maximum of a row that has seen no token
+constexpr float kSlack = 8.f;         // a row's maximum may lag its scores by this much (log2)
+constexpr float kLeastScale = 8.4703294725430034e-22f;  // 2^-70: keeps sum w / vs finite
+
+struct AttendArgs {
+  const void* q;
+  const uint8_t* k;
+  const uint8_t* v;
+  const float* k_scale;
+  const float* v_scale;
+  const int* table;
+  const int* lengths;
+  const int* starts;
+  void* out;
+  float* lse;
+  int* counters;
+  float* partials;
+  long long q_token_stride, q_head_stride;
+  long long k_block_stride, k_head_stride, k_token_stride;
+  long long v_block_stride, v_head_stride, v_token_stride;
+  int table_stride, max_blocks, blocks, block_size;
+  int requests, tokens, kv_heads, group;
+  float scale_log2;
+  int causal, window, bf16;
+};
+
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+
+// Four codes of one word to two half2: (b0, b1) and (b2, b3).
+template <bool E4M3>
+__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (E4M3) {
+    asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n"
+        " cvt.rn.f16x2.e4m3x2 %0, l;\n cvt.rn.f16x2.e4m3x2 %1, h;\n}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
+  } else {
+    // code + 128 in the mantissa of 1024: 1152 + code, exact, less 1152.
+    const uint32_t u = w ^ 0x80808080u;
+    lo = hsub2_u32(prmt(u, 0x64646464u, 0x4140), 0x64806480u);
+    hi = hsub2_u32(prmt(u, 0x64646464u, 0x4342), 0x64806480u);
+  }
+}
+
+template <int WORDS>
+__device__ __forceinline__ void ldg_words(const uint8_t* p, uint32_t* r) {
+  static_assert(WORDS == 2 || WORDS == 4 || WORDS == 8, "");
+  if constexpr (WORDS == 8) {
+    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
+                   "=r"(r[6]), "=r"(r[7])
+                 : "l"(p));
+  } else if constexpr (WORDS == 4) {
+    asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "l"(p));
+  } else {
+    asm volatile("ld.global.nc.L1::no_allocate.v2.b32 {%0,%1}, [%2];"
+                 : "=r"(r[0]), "=r"(r[1])
+                 : "l"(p));
+  }
+}
+
+// One (request, KV head, row tile): where its rows, tokens and units are.
+struct Segment {
+  int request, head, tile;
+  int length, fresh, first_token;  // tokens held, queries, row of the first query in q
+  int unit0, units;                // its first unit among the request's, and how many
+  int begin;                       // its first unit in the line of all units
+};
+
+template <int D, int NT, bool E4M3, int W>
+struct Attend {
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kKWords = D / 16;  // words of a lane's part of a K row
+  static constexpr int kVWords = D / 32;  // words of a lane's part of a V row
+  static constexpr int kPitch = D + 4;    // floats between rows of a part in shared memory
+  static constexpr int kSlots = 2 * W;
+
+  struct Shared {
+    float o[kSlots][kRows][kPitch];
+    float m[kSlots][kRows];
+    float l[kSlots][kRows];
+    Segment seg[kSlots];
+    int used[kSlots];
+    int last[2];
+    int total[W];
+  };
+
+  __device__ static __forceinline__ int units_of(const AttendArgs& a, int length, int fresh, int& unit0) {
+    unit0 = 0;
+    if (a.window > 0) unit0 = max(0, length - fresh + 1 - a.window) / kUnit;
+    return max(1, (length + kUnit - 1) / kUnit - unit0);
+  }
+  __device__ static __forceinline__ int tiles_of(const AttendArgs& a, int fresh) {
+    return (fresh * a.group + kRows - 1) / kRows;
+  }
+  __device__ static __forceinline__ void request_of(const AttendArgs& a, int r, int& length, int& fresh, int& first) {
+    length = min(max(__ldg(a.lengths + r), 0), (int)min((long long)a.max_blocks * a.block_size, 0x7fffffffLL));
+    if (a.starts) {
+      first = __ldg(a.starts + r);
+      fresh = max(0, __ldg(a.starts + r + 1) - first);
+    } else {
+      first = r;
+      fresh = 1;
+    }
+  }
+
+  __device__ static __forceinline__ Segment segment_at(const AttendArgs& a, const int* prefix, int u) {
+    int lo = 0, hi = a.requests - 1;  // the last request whose first unit is at or before u
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (prefix[mid] <= u) lo = mid; else hi = mid - 1;
+    }
+    Segment s;
+    s.request = lo;
+    request_of(a, lo, s.length, s.fresh, s.first_token);
+    s.units = units_of(a, s.length, s.fresh, s.unit0);
+    const int tiles = tiles_of(a, s.fresh);
+    const int local = u - prefix[lo];
+    const int which = local / s.units;
+    s.begin = prefix[lo] + which * s.units;
+    s.head = which / tiles;
+    s.tile = which - s.head * tiles;
+    return s;
+  }
+
+  // Token range [low, high) that query row `row` of the segment sees, and its
+  // place in q and out; false where the tile has no such row.
+  __device__ static __forceinline__ bool row_of(const AttendArgs& a, const Segment& s, int row, int& token, int& head, int& low, int& high) {
+    const int all = s.tile * kRows + row;
+    const int i = all / a.group;
+    token = s.first_token + i;
+    head = s.head * a.group + all - i * a.group;
+    low = high = 0;
+    if (i >= s.fresh || (unsigned)token >= (unsigned)a.tokens) return false;
+    high = a.causal ? min(s.length, max(0, s.length - s.fresh + i + 1)) : s.length;
+    if (a.window > 0) low = max(0, s.length - s.fresh + i + 1 - a.window);
+    return true;
+  }
+
+  // Row `row` of q as this lane's words of the B operand, in K's order of
+  // channels; bf16 rows are scaled by a power of two into fp16's range (the
+  // return value undoes it).
+  __device__ static __forceinline__ float load_q(const AttendArgs& a, const Segment& s, int row, uint32_t (&b)[2 * kKWords]) {
+    const int c = threadIdx.x & 3;
+    int token, head, low, high;
+    const bool there = row_of(a, s, row, token, head, low, high);
+    constexpr int kSpan = D >= 128 ? 32 : 16;  // channels of a lane's contiguous piece
+#pragma unroll
+    for (int i = 0; i < 2 * kKWords; ++i) b[i] = 0;
+    if (there) {
+      const uint16_t* p = static_cast<const uint16_t*>(a.q) + token * a.q_token_stride + head * a.q_head_stride + c * kSpan;
+#pragma unroll
+      for (int i = 0; i < kKWords / 2; ++i) {  // 8 channels each
+        const int at = (i * 8) % kSpan + (i * 8) / kSpan * 128;
+        const uint4 x = __ldg(reinterpret_cast<const uint4*>(p + at));
+        b[4 * i] = x.x; b[4 * i + 1] = x.y; b[4 * i + 2] = x.z; b[4 * i + 3] = x.w;
+      }
+    }
+    if (!a.bf16) return 1.f;
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2 * kKWords; ++i)
+      top = fmaxf(top, fmaxf(fabsf(__uint_as_float(b[i] << 16)), fabsf(__uint_as_float(b[i] & 0xffff0000u))));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    // 2^-e with e the exponent of the row's largest value; 1 for a row of zeros.
+    const int e = min(max((int)(__float_as_uint(top) >> 23), 2), 252);
+    const float down = __uint_as_float((uint32_t)(254 - e) << 23), up = __uint_as_float((uint32_t)e << 23);
+#pragma unroll
+    for (int i = 0; i < 2 * kKWords; ++i)
+      b[i] = pack_half2(__uint_as_float(b[i] << 16) * down, __uint_as_float(b[i] & 0xffff0000u) * down);
+    return up;
+  }
+
+  __device__ static __forceinline__ void store_row(const AttendArgs& a, long long at, const float4& x) {
+    uint2 w;
+    if (a.bf16) {
+      const __nv_bfloat162 p = __floats2bfloat162_rn(x.x, x.y), r = __floats2bfloat162_rn(x.z, x.w);
+      w.x = *reinterpret_cast<const uint32_t*>(&p);
+      w.y = *reinterpret_cast<const uint32_t*>(&r);
+    } else {
+      w.x = pack_half2(x.x, x.y);
+      w.y = pack_half2(x.z, x.w);
+    }
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) = w;
+  }
+
+  // Units [from, to) of segment s by one warp.
+  __device__ static __forceinline__ void units(const AttendArgs& a, const Segment& s, int from, int to,
+                                               float (&o)[NT][D / 16][4], float (&m)[NT][2], float (&l)[NT][2]) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    uint32_t qb[NT][2 * kKWords];
+    float factor[NT][2];
+    int low[NT][2], high[NT][2];
+    // Tokens that every row sees are [most_low, least_high), those that some
+    // row sees are within [least_low, most_high).
+    int least_high = 0x7fffffff, most_low = 0, least_low = 0x7fffffff, most_high = 0;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const float up = load_q(a, s, n * 8 + g, qb[n]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        factor[n][i] = a.scale_log2 * __shfl_sync(0xffffffffu, up, (2 * c + i) * 4);
+        int token, head;
+        const bool there = row_of(a, s, n * 8 + 2 * c + i, token, head, low[n][i], high[n][i]);
+        least_high = min(least_high, there ? high[n][i] : 0x7fffffff);
+        least_low = min(least_low, there ? low[n][i] : 0x7fffffff);
+        most_low = max(most_low, low[n][i]);
+        most_high = max(most_high, high[n][i]);
+        m[n][i] = kFarBelow;
+        l[n][i] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[n][i][j] = 0.f;
+    }
+    least_high = __reduce_min_sync(0xffffffffu, least_high);
+    most_low = __reduce_max_sync(0xffffffffu, most_low);
+    least_low = __reduce_min_sync(0xffffffffu, least_low);
+    most_high = __reduce_max_sync(0xffffffffu, most_high);
+
+    const int upb = a.block_size / kUnit;
+    int u = s.unit0 + from;
+    const int end = s.unit0 + to;
+    const int* table = a.table + (long long)s.request * a.table_stride;
+    const int last_block = (s.length - 1) / a.block_size;
+    int block = u / upb, sub = u - block * upb;
+    auto page_of = [&](int b) { return b <= last_block && s.length > 0 ? __ldg(table + b) : -1; };
+    uint32_t kr[2][kKWords], vr[4][kVWords];
+    float ks, vs;
+    auto load_k = [&](int page, int sub_) {
+      const uint8_t* p = a.k + page * a.k_block_stride + s.head * a.k_head_stride + (sub_ * kUnit + g) * a.k_token_stride;
+      if constexpr (D == 64) {
+        ldg_words<4>(p + c * 16, kr[0]);
+        ldg_words<4>(p + 8 * a.k_token_stride + c * 16, kr[1]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < D / 128; ++i) {
+          ldg_words<8>(p + i * 128 + c * 32, kr[0] + 8 * i);
+          ldg_words<8>(p + 8 * a.k_token_stride + i * 128 + c * 32, kr[1] + 8 * i);
+        }
+      }
+      ks = __ldg(a.k_scale + (long long)page * a.kv_heads + s.head);
+    };
+    auto load_v = [&](int page, int sub_) {
+      const uint8_t* p = a.v + page * a.v_block_stride + s.head * a.v_head_stride + (sub_ * kUnit + 2 * c) * a.v_token_stride + g * (D / 8);
+      ldg_words<kVWords>(p, vr[0]);
+      ldg_words<kVWords>(p + a.v_token_stride, vr[1]);
+      ldg_words<kVWords>(p + 8 * a.v_token_stride, vr[2]);
+      ldg_words<kVWords>(p + 9 * a.v_token_stride, vr[3]);
+      vs = __ldg(a.v_scale + (long long)page * a.kv_heads + s.head);
+    };
+
+    int page = page_of(block);
+    bool good = (unsigned)page < (unsigned)a.blocks;
+    page = good ? page : 0;
+    load_k(page, sub);
+    load_v(page, sub);
+    int next_block = block, next_sub = sub + 1;
+    if (next_sub == upb) { next_sub = 0; ++next_block; }
+    int next_page = page_of(next_block);
+
+    for (; u < end; ++u) {
+      const bool more = u + 1 < end;
+      // Scores of the unit: [16 tokens][8 rows] for each tile of rows.
+      float sc[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+#pragma unroll
+      for (int w = 0; w < kKWords; ++w) {
+        uint32_t a0, a1, a2, a3;
+        codes_to_half<E4M3>(kr[0][w], a0, a2);
+        codes_to_half<E4M3>(kr[1][w], a1, a3);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma16816(sc[n], a0, a1, a2, a3, qb[n][2 * w], qb[n][2 * w + 1]);
+      }
+      const bool good_now = good;
+      const float k_now = ks, v_now = good_now ? (vs < kLeastScale ? kLeastScale : vs) : 1.f;
+      const int page_now = next_page, sub_now = next_sub;
+      if (more) {
+        good = (unsigned)page_now < (unsigned)a.blocks;
+        page = good ? page_now : 0;
+        load_k(page, sub_now);
+        if (++next_sub == upb) { next_sub = 0; ++next_block; }
+        next_page = page_of(next_block);
+      }
+      const float v_log2 = __log2f(v_now), v_inverse = __frcp_rn(v_now);
+      const int base = u * kUnit;
+      const bool edge = base + kUnit > least_high || base < most_low || !good_now;  // the same in all lanes
+      bool grow = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float t = fmaf(sc[n][i], factor[n][i & 1] * k_now, v_log2);
+          if (edge) {
+            const int at = base + g + (i >> 1) * 8;
+            if (at >= high[n][i & 1] || at < low[n][i & 1] || !good_now) t = -INFINITY;
+          }
+          sc[n][i] = t;
+        }
+        grow |= fmaxf(sc[n][0], sc[n][2]) > m[n][0] + kSlack || fmaxf(sc[n][1], sc[n][3]) > m[n][1] + kSlack;
+      }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float top = fmaxf(sc[n][i], sc[n][i + 2]);
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            top = fmaxf(top, m[n][i]);
+            const float f = exp2_approx(m[n][i] - top);
+            m[n][i] = top;
+            l[n][i] *= f;
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+              o[n][d][i] *= f;
+              o[n][d][i + 2] *= f;
+            }
+          }
+        }
+      }
+      uint32_t pb[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = exp2_approx(sc[n][i] - m[n][i & 1]);
+        l[n][0] = fmaf(w[0] + w[2], v_inverse, l[n][0]);
+        l[n][1] = fmaf(w[1] + w[3], v_inverse, l[n][1]);
+        pb[n][0] = transpose8x8(pack_half2(w[0], w[1]));
+        pb[n][1] = transpose8x8(pack_half2(w[2], w[3]));
+      }
+      if (edge) {  // bytes of tokens that no row sees may be anything, e4m3's NaN too
+        const int past = good_now ? most_high - base : 0, before = least_low - base;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int at = 2 * c + (j & 1) + (j >> 1) * 8;
+          if (at >= past || at < before)
+#pragma unroll
+            for (int w = 0; w < kVWords; ++w) vr[j][w] = 0u;
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < kVWords; ++w) {
+        uint32_t e[4], f[4];  // [channel 4w + i]: tokens (2c, 2c+1) and (2c+8, 2c+9)
+        codes_to_half<E4M3>(prmt(vr[0][w], vr[1][w], 0x5140), e[0], e[1]);
+        codes_to_half<E4M3>(prmt(vr[0][w], vr[1][w], 0x7362), e[2], e[3]);
+        codes_to_half<E4M3>(prmt(vr[2][w], vr[3][w], 0x5140), f[0], f[1]);
+        codes_to_half<E4M3>(prmt(vr[2][w], vr[3][w], 0x7362), f[2], f[3]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          mma16816(o[n][2 * w], e[0], e[1], f[0], f[1], pb[n][0], pb[n][1]);
+          mma16816(o[n][2 * w + 1], e[2], e[3], f[2], f[3], pb[n][0], pb[n][1]);
+        }
+      }
+      if (more) load_v(page, sub_now);
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], d);
+  }
+
+  // Channels of o[.][i][j] for lane row group g: 2i + (j >> 1) from g * (D / 8).
+  __device__ static __forceinline__ void write_rows(const AttendArgs& a, const Segment& s, const float (&o)[NT][D / 16][4],
+                                                    const float (&m)[NT][2], const float (&l)[NT][2]) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        int token, head, low, high;
+        if (!row_of(a, s, n * 8 + 2 * c + i, token, head, low, high)) continue;
+        const float f = l[n][i] > 0.f || l[n][i] != l[n][i] ? 1.f / l[n][i] : 0.f;
+        const long long row = (long long)token * a.kv_heads * a.group + head;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+          store_row(a, row * D + g * (D / 8) + 4 * d,
+                    make_float4(o[n][2 * d][i] * f, o[n][2 * d][i + 2] * f, o[n][2 * d + 1][i] * f, o[n][2 * d + 1][i + 2] * f));
+        if (a.lse && g == 0) a.lse[row] = l[n][i] == 0.f ? -INFINITY : (m[n][i] + log2f(l[n][i])) * 0.69314718055994531f;
+      }
+  }
+
+  // One row joined from parts: rows of `count` parts at o[i * stride_o], each
+  // with its m and l; lane has channels lane * (D / 32)...
+  __device__ static __forceinline__ void finish_row(const AttendArgs& a, const Segment& s, int row, const float (&x)[D / 32], float m, float l) {
+    const int lane = threadIdx.x & 31;
+    int token, head, low, high;
+    if (!row_of(a, s, row, token, head, low, high)) return;
+    const float f = l > 0.f || l != l ? 1.f / l : 0.f;
+    const long long at = (long long)token * a.kv_heads * a.group + head;
+    if constexpr (D == 64) {
+      uint32_t w;
+      if (a.bf16) {
+        const __nv_bfloat162 p = __floats2bfloat162_rn(x[0] * f, x[1] * f);
+        w = *reinterpret_cast<const uint32_t*>(&p);
+      } else {
+        w = pack_half2(x[0] * f, x[1] * f);
+      }
+      *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + at * D + lane * 2) = w;
+    } else {
+#pragma unroll
+      for (int d = 0; d < D / 128; ++d)
+        store_row(a, at * D + lane * (D / 32) + 4 * d, make_float4(x[4 * d] * f, x[4 * d + 1] * f, x[4 * d + 2] * f, x[4 * d + 3] * f));
+    }
+    if (a.lse && lane == 0) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+  }
+
+  static constexpr int kPartFloats = kRows * (D + 2);
+
+  __device__ static __forceinline__ int owner(int u, int grid, int all) {
+    return (int)((((long long)u + 1) * grid - 1) / all);
+  }
+
+  __device__ static void run(const AttendArgs& a, Shared& sh, int* prefix) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // Units of every request, summed up: prefix[r] = the first of request r.
+    int carry = 0;
+    for (int base = 0; base < a.requests; base += W * 32) {
+      const int r = base + tid;
+      int mine = 0;
+      if (r < a.requests) {
+        int length, fresh, first, unit0;
+        request_of(a, r, length, fresh, first);
+        mine = units_of(a, length, fresh, unit0) * tiles_of(a, fresh) * a.kv_heads;
+      }
+      int sum = mine;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, sum, d);
+        if (lane >= d) sum += x;
+      }
+      if (lane == 31) sh.total[warp] = sum;
+      __syncthreads();
+      int before = carry, all = 0;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const int x = sh.total[w];
+        if (w < warp) before += x;
+        all += x;
+      }
+      if (r < a.requests) prefix[r] = before + sum - mine;
+      carry += all;
+      __syncthreads();
+    }
+    const int all = carry;
+    if (all == 0) return;
+    // A CTA has a unit for each of its warps at least.
+    const int grid = min((int)gridDim.x, (all + W - 1) / W);
+    const int cta = blockIdx.x;
+    if (cta >= grid) return;
+    const int cta0 = (int)((long long)all * cta / grid), cta1 = (int)((long long)all * (cta + 1) / grid);
+    const int u0 = cta0 + (int)((long long)(cta1 - cta0) * warp / W), u1 = cta0 + (int)((long long)(cta1 - cta0) * (warp + 1) / W);
+    if (lane < 2) sh.used[2 * warp + lane] = 0;
+    __syncwarp();
+
+    for (int u = u0; u < u1;) {
+      const Segment s = segment_at(a, prefix, u);
+      const int from = u - s.begin, to = min(s.units, u1 - s.begin);
+      float o[NT][D / 16][4], m[NT][2], l[NT][2];
+      units(a, s, from, to, o, m, l);
+      if (from == 0 && to == s.units) {
+        write_rows(a, s, o, m, l);
+      } else {
+        const int slot = 2 * warp + (u == u0 ? 0 : 1), g = lane >> 2, c = lane & 3;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int row = n * 8 + 2 * c + i;
+            float* p = &sh.o[slot][row][g * (D / 8)];
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d)
+              *reinterpret_cast<float4*>(p + 4 * d) = make_float4(o[n][2 * d][i], o[n][2 * d][i + 2], o[n][2 * d + 1][i], o[n][2 * d + 1][i + 2]);
+            if (g == 0) {
+              sh.m[slot][row] = m[n][i];
+              sh.l[slot][row] = l[n][i];
+            }
+          }
+        if (lane == 0) {
+          sh.seg[slot] = s;
+          sh.used[slot] = 1;
+        }
+      }
+      u = s.begin + to;
+    }
+    __syncthreads();
+
+    // Parts of one segment are neighbours among the used slots.
+    const int used = lane < kSlots ? sh.used[lane] : 0;
+    const uint32_t valid = __ballot_sync(0xffffffffu, used);
+    if (valid == 0) return;
+    const int begin = used ? sh.seg[lane].begin : -1;
+    const uint32_t below = valid & ((1u << lane) - 1u);
+    const int prev = __shfl_sync(0xffffffffu, begin, below ? 31 - __clz(below) : 0);
+    const uint32_t heads = __ballot_sync(0xffffffffu, used && (below == 0 || prev != begin));
+    const int groups = __popc(heads);
+    bool shared_by_ctas = false;
+    for (int item = warp; item < groups * kRows; item += W) {
+      const int which = item / kRows, row = item - which * kRows;
+      uint32_t h = heads;
+      for (int i = 0; i < which; ++i) h &= h - 1;
+      const int first = __ffs(h) - 1;
+      h &= h - 1;
+      const uint32_t members = valid & ~((1u << first) - 1u) & (h ? (h & -h) - 1u : 0xffffffffu);
+      float top = kFarBelow;
+      for (uint32_t b = members; b; b &= b - 1) top = fmaxf(top, sh.m[__ffs(b) - 1][row]);
+      float x[D / 32], l = 0.f;
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d) x[d] = 0.f;
+      for (uint32_t b = members; b; b &= b - 1) {
+        const int slot = __ffs(b) - 1;
+        const float f = exp2_approx(sh.m[slot][row] - top);
+        l = fmaf(sh.l[slot][row], f, l);
+        const float* p = &sh.o[slot][row][lane * (D / 32)];
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) x[d] = fmaf(p[d], f, x[d]);
+      }
+      const Segment& s = sh.seg[first];
+      if (s.begin >= cta0 && s.begin + s.units <= cta1) {
+        finish_row(a, s, row, x, top, l);
+      } else {
+        const int slot = owner(s.begin, grid, all) == cta ? 1 : 0;
+        float* part = a.partials + (long long)(cta * 2 + slot) * kPartFloats;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) __stcg(part + row * D + lane * (D / 32) + d, x[d]);
+        if (lane == 0) {
+          __stcg(part + kRows * D + row, top);
+          __stcg(part + kRows * D + kRows + row, l);
+        }
+      }
+    }
+    // Which of the CTA's first and last segments other CTAs share, as every
+    // thread reads it from the slots.
+    int first_slot = __ffs(heads) - 1, last_slot = 31 - __clz(heads);
+    const Segment* ends[2] = {&sh.seg[first_slot], &sh.seg[last_slot]};
+    const int n_ends = first_slot == last_slot ? 1 : 2;
+    for (int e = 0; e < n_ends; ++e) {
+      const Segment& s = *ends[e];
+      shared_by_ctas |= !(s.begin >= cta0 && s.begin + s.units <= cta1);
+    }
+    if (!shared_by_ctas) return;
+    __threadfence();
+    __syncthreads();
+    if (tid < n_ends) {
+      const Segment& s = *ends[tid];
+      int last = 0;
+      if (!(s.begin >= cta0 && s.begin + s.units <= cta1)) {
+        const int c0 = owner(s.begin, grid, all), c1 = owner(s.begin + s.units - 1, grid, all);
+        last = atomicAdd(a.counters + c0, 1) == c1 - c0;
+        if (last) a.counters[c0] = 0;
+      }
+      sh.last[tid] = last;
+      __threadfence();
+    }
+    __syncthreads();
+    for (int e = 0; e < n_ends; ++e) {
+      if (!sh.last[e]) continue;
+      const Segment& s = *ends[e];
+      const int c0 = owner(s.begin, grid, all), c1 = owner(s.begin + s.units - 1, grid, all);
+      for (int row = warp; row < kRows; row += W) {
+        auto part = [&](int c) { return a.partials + (long long)(c * 2 + (c == c0 ? 1 : 0)) * kPartFloats; };
+        float top = kFarBelow;
+        for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, __ldcg(part(c) + kRows * D + row));
+#pragma unroll
+        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        float x[D / 32], l = 0.f;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) x[d] = 0.f;
+#pragma unroll 4
+        for (int c = c0; c <= c1; ++c) {
+          const float* p = part(c);
+          const float f = exp2_approx(__ldcg(p + kRows * D + row) - top);
+          l = fmaf(__ldcg(p + kRows * D + kRows + row), f, l);
+#pragma unroll
+          for (int d = 0; d < D / 32; ++d) x[d] = fmaf(__ldcg(p + row * D + lane * (D / 32) + d), f, x[d]);
+        }
+        finish_row(a, s, row, x, top, l);
+      }
+    }
+  }
+};
+
+template <int D, int NT, bool E4M3, int W, int MINB>
+__global__ void __launch_bounds__(W * 32, MINB) k_attend(const __grid_constant__ AttendArgs a) {
+  extern __shared__ __align__(16) unsigned char raw[];
+  using A = Attend<D, NT, E4M3, W>;
+  A::run(a, *reinterpret_cast<typename A::Shared*>(raw), reinterpret_cast<int*>(raw + sizeof(typename A::Shared)));
+}
+
+// Warps of a CTA and CTAs of an SM for each head size and number of row tiles:
+// what the registers of the fragments leave (q D/8 and o D/4 for each row
+// tile, one unit D/4).
+template <int D, int NT>
+struct Shape;
+template <> struct Shape<64, 1> { static constexpr int W = 8, MINB = 3; };
+template <> struct Shape<64, 2> { static constexpr int W = 8, MINB = 2; };
+template <> struct Shape<128, 1> { static constexpr int W = 8, MINB = 2; };
+template <> struct Shape<128, 2> { static constexpr int W = 4, MINB = 3; };
+template <> struct Shape<256, 1> { static constexpr int W = 4, MINB = 2; };
+
+template <int D, int NT, bool E4M3>
+dk_status launch(AttendArgs a, cudaStream_t stream) {
+  constexpr int W = Shape<D, NT>::W, MINB = Shape<D, NT>::MINB;
+  using A = Attend<D, NT, E4M3, W>;
+  const size_t smem = sizeof(typename A::Shared) + sizeof(int) * (size_t)std::min(a.requests, kMaxRequests);
+  auto kernel = k_attend<D, NT, E4M3, W, MINB>;
+  static thread_local unsigned long long prepared = 0;  // devices whose limit is set
+  const int device = current_device();
+  if (device >= 64 || !(prepared >> device & 1)) {
+    const size_t most = sizeof(typename A::Shared) + sizeof(int) * kMaxRequests;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e != cudaSuccess) {
+      set_cuda_error(e, "cudaFuncSetAttribute");
+      return DK_ERR_CUDA;
+    }
+    if (device < 64) prepared |= 1ull << device;
+  }
+  const int requests = a.requests;
+  const int* lengths = a.lengths;
+  const int* table = a.table;
+  const int* starts = a.starts;
+  const uint16_t* q = static_cast<const uint16_t*>(a.q);
+  uint16_t* out = static_cast<uint16_t*>(a.out);
+  float* lse = a.lse;
+  const int tokens = a.tokens;
+  for (int r = 0; r < requests; r += kMaxRequests) {
+    a.requests = std::min(kMaxRequests, requests - r);
+    a.lengths = lengths + r;
+    a.table = table + (long long)r * a.table_stride;
+    if (starts) {
+      a.starts = starts + r;
+    } else {  // one query each: the rows move with the requests
+      a.q = q + r * a.q_token_stride;
+      a.out = out + (long long)r * a.kv_heads * a.group * D;
+      a.lse = lse ? lse + (long long)r * a.kv_heads * a.group : nullptr;
+      a.tokens = tokens - r;
+    }
+    kernel<<<sm_count(device) * MINB, W * 32, smem, stream>>>(a);
+    const dk_status s = check_launch("dk_cache_attention");
+    if (s != DK_OK) return s;
+  }
+  return DK_OK;
+}
+
+// Row tiles of 16 where a KV head has more than 8 query rows: one pass over
+// the cache for 16 rows.  Heads of 256 keep tiles of 8 (the fragments of 16
+// rows do not fit the registers).
+int row_tiles(int head_dim, long long rows) { return head_dim < 256 && rows > 8 ? 2 : 1; }
+
+template <int D, int NT>
+dk_status launch_code(const AttendArgs& a, bool e4m3, cudaStream_t stream) {
+  return e4m3 ? launch<D, NT, true>(a, stream) : launch<D, NT, false>(a, stream);
+}
+
+}  // namespace
+}  // namespace dk
+
+using namespace dk;
+
+extern "C" size_t dk_cache_attention_workspace_bytes(int head_dim) {
+  // Two parts of 16 rows for each CTA that can run at once, and their counters.
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return 0;
+  const size_t ctas = (size_t)sm_count(-1) * 3;
+  const size_t counters = (ctas * sizeof(int) + 255) / 256 * 256;
+  return counters + ctas * 2 * 16 * (size_t)(head_dim + 2) * sizeof(float);
+}
+
+extern "C" dk_status dk_cache_attention(const dk_cache_attention_args* p, void* workspace,
+                                        size_t workspace_bytes, void* stream) {
+  if (!p) return DK_ERR_INVALID_ARG;
+  const dk_cache8& c = p->cache;
+  if (c.block_size < 16 || c.block_size > 256 || c.block_size % 16 || c.blocks < 1 || c.kv_heads < 1 ||
+      p->q_heads < 1 || p->q_heads % c.kv_heads || p->requests < 0 || p->tokens < 0 || p->max_blocks < 1 ||
+      p->window < 0 || (p->window > 0 && !p->causal))
+    return DK_ERR_INVALID_ARG;
+  if (c.code != DK_INT8 && c.code != DK_E4M3) return DK_ERR_INVALID_ARG;
+  if (p->dtype != DK_FP16 && p->dtype != DK_BF16) return DK_ERR_INVALID_ARG;
+  if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) return DK_ERR_UNSUPPORTED;
+  if (!p->starts && p->tokens != p->requests) return DK_ERR_INVALID_ARG;
+  if (p->requests == 0 || p->tokens == 0) return DK_OK;
+  if (!p->q || !p->out || !p->block_table || !p->lengths || !c.k || !c.v || !c.k_scale || !c.v_scale)
+    return DK_ERR_INVALID_ARG;
+  auto aligned = [](const void* x, uintptr_t n) { return reinterpret_cast<uintptr_t>(x) % n == 0; };
+  const long long strides[] = {c.k_block_stride, c.k_head_stride, c.k_token_stride,
+                               c.v_block_stride, c.v_head_stride, c.v_token_stride};
+  for (long long s : strides)
+    if (s < 0 || s % 32) return DK_ERR_INVALID_ARG;
+  if (!aligned(c.k, 32) || !aligned(c.v, 32) || !aligned(p->q, 16) || !aligned(p->out, 16) ||
+      p->q_token_stride % 8 || p->q_head_stride % 8)
+    return DK_ERR_INVALID_ARG;
+  // The line of units is counted in 32 bits.
+  const int group = p->q_heads / c.kv_heads;
+  const long long units = ((long long)p->max_blocks * c.block_size + 15) / 16;
+  const long long per_head = (long long)std::min(p->requests, kMaxRequests) + (long long)p->tokens * group / 8;
+  if (units > INT32_MAX / 16 || per_head > INT32_MAX / units / c.kv_heads) return DK_ERR_UNSUPPORTED;
+  const size_t need = dk_cache_attention_workspace_bytes(c.head_dim);
+  if (!workspace || workspace_bytes < need || !aligned(workspace, 256)) return DK_ERR_WORKSPACE;
+
+  AttendArgs a;
+  a.q = p->q;
+  a.k = static_cast<const uint8_t*>(c.k);
+  a.v = static_cast<const uint8_t*>(c.v);
+  a.k_scale = c.k_scale;
+  a.v_scale = c.v_scale;
+  a.table = p->block_table;
+  a.lengths = p->lengths;
+  a.starts = p->starts;
+  a.out = p->out;
+  a.lse = p->lse;
+  const size_t ctas = (size_t)sm_count(-1) * 3;
+  a.counters = static_cast<int*>(workspace);
+  a.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + (ctas * sizeof(int) + 255) / 256 * 256);
+  a.q_token_stride = p->q_token_stride;
+  a.q_head_stride = p->q_head_stride;
+  a.k_block_stride = c.k_block_stride;
+  a.k_head_stride = c.k_head_stride;
+  a.k_token_stride = c.k_token_stride;
+  a.v_block_stride = c.v_block_stride;
+  a.v_head_stride = c.v_head_stride;
+  a.v_token_stride = c.v_token_stride;
+  a.table_stride = p->table_stride;
+  a.max_blocks = p->max_blocks;
+  a.blocks = c.blocks;
+  a.block_size = c.block_size;
+  a.requests = p->requests;
+  a.tokens = p->tokens;
+  a.kv_heads = c.kv_heads;
+  a.group = group;
+  a.scale_log2 = p->scale * 1.4426950408889634f;
+  a.causal = p->causal;
+  a.window = p->window;
+  a.bf16 = p->dtype == DK_BF16;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool e4m3 = c.code == DK_E4M3;
+  const int nt = row_tiles(c.head_dim, ((long long)p->tokens + p->requests - 1) / p->requests * group);
+  if (c.head_dim == 64) return nt == 1 ? launch_code<64, 1>(a, e4m3, st) : launch_code<64, 2>(a, e4m3, st);
+  if (c.head_dim == 128) return nt == 1 ? launch_code<128, 1>(a, e4m3, st) : launch_code<128, 2>(a, e4m3, st);
+  return launch_code<256, 1>(a, e4m3, st);
+}

@@ -6,6 +6,10 @@ __init__.py:11-83): ``gemv``, ``w4a16_linear``, ``cuda_available``,
 repository's CUDA library (``libdk_b200.so``, C ABI in include/dk_w4a16.h)
 through the torch extension ``decode_kernel._cuda``.
 
+The rest of a decode step stands beside the products: a paged cache in 8 bits
+(``PagedCache8``, ``cache_plan``, ``cache_append``, ``cache_attention``) and the
+norms between blocks (``block_norm``).
+
 There is no CPU fallback: when the extension or a GPU is missing these
 functions raise.
 """
@@ -16,11 +20,19 @@ from typing import Optional
 
 import torch
 
+from .cache import CachePlan, PagedCache8, cache_append, cache_attention, cache_plan
+from .norm import block_norm
 from .quantize import GROUP_SIZE, dequantize, quantize_and_pack, quantize_and_pack_cuda
 
 __all__ = [
+    "CachePlan",
     "GROUP_SIZE",
+    "PagedCache8",
     "W4A16Linear",
+    "block_norm",
+    "cache_append",
+    "cache_attention",
+    "cache_plan",
     "cuda_available",
     "gemv_multi",
     "gemv_silu_mul",

@@ -30,6 +30,12 @@ DK_MAX_SEGMENTS = 4
 DK_SHARD_SLOTS = 256
 DK_PEER_HANDLE_BYTES = 64
 
+# enum dk_dtype, dk_norm_kind, dk_gate_act
+DK_FP16, DK_BF16, DK_FP32, DK_INT8, DK_E4M3 = range(5)
+DK_NORM_RMS, DK_NORM_LAYER = range(2)
+DK_GATE_NONE, DK_GATE_SIGMOID, DK_GATE_SILU = range(3)
+DK_PLAN_MAX_REQUESTS = 8192
+
 
 class GemvConfig(ctypes.Structure):
     """struct dk_gemv_config (gemv_w4a16.h:22-27 GemvLaunchConfig + flags)."""
@@ -57,8 +63,68 @@ class ShardGroup(ctypes.Structure):
     ]
 
 
+class Cache8(ctypes.Structure):
+    """struct dk_cache8: a pool of pages in 8 bits and its scales."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("blocks", ctypes.c_int),
+        ("block_size", ctypes.c_int),
+        ("kv_heads", ctypes.c_int),
+        ("head_dim", ctypes.c_int),
+        ("code", ctypes.c_int),
+        ("k_block_stride", ctypes.c_int64),
+        ("k_head_stride", ctypes.c_int64),
+        ("k_token_stride", ctypes.c_int64),
+        ("v_block_stride", ctypes.c_int64),
+        ("v_head_stride", ctypes.c_int64),
+        ("v_token_stride", ctypes.c_int64),
+    ]
+
+
+class CacheAttentionArgs(ctypes.Structure):
+    """struct dk_cache_attention_args."""
+
+    _fields_ = [
+        ("cache", Cache8),
+        ("q", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("dtype", ctypes.c_int),
+        ("q_token_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("block_table", ctypes.c_void_p),
+        ("max_blocks", ctypes.c_int),
+        ("table_stride", ctypes.c_int),
+        ("lengths", ctypes.c_void_p),
+        ("starts", ctypes.c_void_p),
+        ("requests", ctypes.c_int),
+        ("tokens", ctypes.c_int),
+        ("q_heads", ctypes.c_int),
+        ("scale", ctypes.c_float),
+        ("causal", ctypes.c_int),
+        ("window", ctypes.c_int),
+    ]
+
+
+class BlockNormArgs(ctypes.Structure):
+    """struct dk_block_norm_args."""
+
+    _fields_ = [(name, ctypes.c_void_p) for name in (
+        "residual", "y", "gate", "post_weight", "post_bias", "pre_weight", "pre_bias",
+        "residual_out", "h")] + [(name, ctypes.c_int64) for name in (
+            "residual_stride", "y_stride", "gate_stride", "gate_column_stride",
+            "residual_out_stride", "h_stride")] + [(name, ctypes.c_int) for name in (
+                "rows", "dim", "dtype", "residual_dtype", "kind", "act")] + [
+                    (name, ctypes.c_float) for name in ("residual_scale", "block_scale", "eps")]
+
+
 # name -> (restype, argtypes); every symbol include/dk_w4a16.h declares.
 _P, _I, _U, _SZ = ctypes.c_void_p, ctypes.c_int, ctypes.c_uint, ctypes.c_size_t
+_L = ctypes.c_int64
 SIGNATURES = {
     "dk_gemv_config_init": (None, [ctypes.POINTER(GemvConfig)]),
     "dk_w4a16_workspace_bytes": (_SZ, [_I, _I, _I, ctypes.POINTER(GemvConfig)]),
@@ -93,6 +159,11 @@ SIGNATURES = {
     "dk_quantize_pack": (_I, [_P, _I, _I, _P, _P, _U, _P]),
     "dk_unpack_to_int": (_I, [_P, _I, _I, _P, _P]),
     "dk_dequantize": (_I, [_P, _P, _I, _I, _P, _P]),
+    "dk_cache_plan": (_I, [_P, _P, _I, _P, _I, _I, _I, _P, _I, _P, _P, _P, _P, _P, _I, _P]),
+    "dk_cache_append": (_I, [ctypes.POINTER(Cache8), _P, _P, _I, _I, _L, _L, _L, _L, _P, _P]),
+    "dk_cache_attention_workspace_bytes": (_SZ, [_I]),
+    "dk_cache_attention": (_I, [ctypes.POINTER(CacheAttentionArgs), _P, _SZ, _P]),
+    "dk_block_norm": (_I, [ctypes.POINTER(BlockNormArgs), _P]),
     "dk_status_string": (ctypes.c_char_p, [_I]),
     "dk_last_cuda_error": (ctypes.c_char_p, []),
     "dk_version": (ctypes.c_char_p, []),

@@ -338,6 +338,154 @@ DK_API dk_status dk_unpack_to_int(const int32_t* packed, int M, int K, int32_t* 
 DK_API dk_status dk_dequantize(const int32_t* packed, const uint16_t* scales, int M, int K, float* w,
                         void* stream);
 
+/* ------------------------------------------------------------------------
+ * The rest of a decode step: a paged cache of keys and values in 8 bits, its
+ * tables, and the norms between blocks.  No counterpart in the reference.
+ * Like the calls above these are asynchronous on `stream`, allocate nothing
+ * and return a status.
+ * ------------------------------------------------------------------------ */
+typedef enum dk_dtype {
+  DK_FP16 = 0,
+  DK_BF16 = 1,
+  DK_FP32 = 2,
+  DK_INT8 = 3,
+  DK_E4M3 = 4 /* 8-bit float: 4 exponent bits, 3 mantissa bits, largest 448 */
+} dk_dtype;
+
+/* A pool of pages.  Page p holds block_size tokens of every KV head:
+ *   k[p, h, i, :], v[p, h, i, :]   head_dim codes (DK_INT8 or DK_E4M3)
+ *   k_scale[p, h], v_scale[p, h]   fp32 [blocks, kv_heads], contiguous
+ * and a value is its code times its page's and head's scale.  Strides are in
+ * codes (bytes), multiples of 32; the last dimension is contiguous; k and v
+ * are 32-byte aligned.  block_size: a multiple of 16 in 16..256.  head_dim:
+ * 64, 128 or 256. */
+typedef struct dk_cache8 {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int blocks, block_size, kv_heads, head_dim;
+  dk_dtype code;
+  int64_t k_block_stride, k_head_stride, k_token_stride;
+  int64_t v_block_stride, v_head_stride, v_token_stride;
+} dk_cache8;
+
+/* Block tables and slot maps of a step.  Request r holds held[r] tokens and
+ * brings fresh[r] new ones; fresh[r] < 0 says that it has ended.
+ *   free_blocks  int32 [free_capacity], a ring of page numbers; entry
+ *                i % free_capacity is free for ring[0] <= i < ring[1]
+ *   block_table  int32 [requests, max_blocks], rows table_stride apart
+ * Requests take their new pages from the ring's beginning in order of r, and
+ * requests that ended give theirs back at its end.  A request that the ring
+ * cannot serve, or that would pass max_blocks pages, gets none of its tokens:
+ * its length stays and its new tokens have slot -1.  The ring serves a request
+ * only if the pages asked for by all requests up to it were free.
+ * Writes
+ *   lengths  int32 [requests]      tokens held after the step (0 if ended)
+ *   starts   int32 [requests + 1]  first row of each request's new tokens
+ *   slots    int64 [tokens]        page * block_size + row in the page of each
+ *                                  row of the step, -1 past the last token
+ *   ring_out int64 [4]             the ring's beginning and end after the step,
+ *                                  pages that were missing, requests refused
+ *                                  for their width
+ * and the new entries of block_table and of the ring.  `tokens` is the
+ * capacity of slots.  lengths may be held and ring_out may be ring (as a
+ * captured step wants it); the call then runs on one SM.  At most 8192
+ * requests; the new tokens add up to less than 2^31. */
+#define DK_PLAN_MAX_REQUESTS 8192
+DK_API dk_status dk_cache_plan(const int32_t* held, const int32_t* fresh, int requests,
+                               int32_t* block_table, int max_blocks, int table_stride,
+                               int block_size, int32_t* free_blocks, int free_capacity,
+                               const int64_t* ring, int64_t* ring_out, int32_t* lengths,
+                               int32_t* starts, int64_t* slots, int tokens, void* stream);
+
+/* New keys and values into their pages: token t of k and v ([tokens, kv_heads,
+ * head_dim], DK_FP16 or DK_BF16, token and head strides in elements, last
+ * dimension contiguous) goes to slots[t] = page * block_size + row.  Slots
+ * below 0 or past the pool are skipped.  The tokens of a page are neighbours
+ * in t, with rising rows, and a page gets tokens of one request only
+ * (dk_cache_plan's slots are so).
+ * For each page and head, with Q = 127 (int8) or 448 (e4m3):
+ *   amax  = largest finite |x| of the call's tokens there
+ *   scale = max(old, max(amax, 2^-60) / Q), old = 0 if the tokens begin the page
+ *   code  = x * (1 / scale), clamped to +-Q, rounded to nearest even; NaN is 0
+ * and where scale > old the page's earlier rows (if any) are coded again as
+ * code * (old / scale).  All in fp32 with IEEE divisions. */
+DK_API dk_status dk_cache_append(const dk_cache8* cache, const void* k, const void* v,
+                                 dk_dtype dtype, int tokens, int64_t k_token_stride,
+                                 int64_t k_head_stride, int64_t v_token_stride,
+                                 int64_t v_head_stride, const int64_t* slots, void* stream);
+
+/* Attention of a step's queries over the cache.  Request r holds lengths[r]
+ * tokens, in the pages block_table[r, :] (block_size tokens each), its queries
+ * are rows starts[r] .. starts[r + 1] - 1 of q and are the last of its tokens
+ * (starts == NULL: one query each, row r).  Query i of n stands at place
+ * p = length - n + i and sees the tokens j < length with
+ *   j <= p                 if causal
+ *   j > p - window         if window > 0 (causal only)
+ *   out = softmax_j(scale * q . k_j) . v_j
+ * in fp32 and rounded once; rows that see no token are zeros.  lse (or NULL)
+ * gets log(sum_j exp(scale * q . k_j)), -inf for such rows.  q has strides in
+ * elements, multiples of 8, and is 16-byte aligned; out and lse are contiguous.
+ * V scales below 2^-70 count as 2^-70.  Entries of block_table outside the
+ * pool hide their tokens.
+ * The workspace (dk_cache_attention_workspace_bytes of the current device) is
+ * 256-byte aligned and zero before its first call, which every call leaves it
+ * ready for the next; calls that share one must be ordered on the GPU. */
+typedef struct dk_cache_attention_args {
+  dk_cache8 cache;
+  const void* q; /* [tokens, q_heads, head_dim] */
+  void* out;     /* [tokens, q_heads, head_dim], contiguous */
+  float* lse;    /* [tokens, q_heads] or NULL */
+  dk_dtype dtype;
+  int64_t q_token_stride, q_head_stride;
+  const int32_t* block_table;
+  int max_blocks, table_stride;
+  const int32_t* lengths;
+  const int32_t* starts;
+  int requests, tokens, q_heads;
+  float scale;
+  int causal, window;
+} dk_cache_attention_args;
+DK_API size_t dk_cache_attention_workspace_bytes(int head_dim);
+DK_API dk_status dk_cache_attention(const dk_cache_attention_args* args, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
+/* Between two blocks, in one pass over each row:
+ *   u  = y, or norm(y) * post_weight + post_bias if post_weight
+ *   r' = residual_scale * residual + block_scale * act(gate) * u
+ *   h  = norm(r') * pre_weight + pre_bias          if h
+ * y may be NULL (r' = residual_scale * residual), and so may gate (1), the
+ * biases, residual_out and h.  norm is x / sqrt(mean(x^2) + eps) (DK_NORM_RMS)
+ * or (x - mean) / sqrt(var + eps) (DK_NORM_LAYER).  Everything is computed in
+ * fp32 and rounded once, h from the unrounded r'.
+ * y, gate, h and the weights have type `dtype` (DK_FP16, DK_BF16), residual
+ * and residual_out `residual_dtype` (also DK_FP32).  Strides are in elements
+ * between rows; the last dimension is contiguous, except that gate is read
+ * with gate_stride between rows and gate_column_stride (0 or 1) between
+ * columns.  residual_out may be residual and h may be y.  dim: 1..32768. */
+typedef enum dk_norm_kind { DK_NORM_RMS = 0, DK_NORM_LAYER = 1 } dk_norm_kind;
+typedef enum dk_gate_act { DK_GATE_NONE = 0, DK_GATE_SIGMOID = 1, DK_GATE_SILU = 2 } dk_gate_act;
+typedef struct dk_block_norm_args {
+  const void* residual;
+  const void* y;
+  const void* gate;
+  const void* post_weight;
+  const void* post_bias;
+  const void* pre_weight;
+  const void* pre_bias;
+  void* residual_out;
+  void* h;
+  int64_t residual_stride, y_stride, gate_stride, gate_column_stride;
+  int64_t residual_out_stride, h_stride;
+  int rows, dim;
+  dk_dtype dtype, residual_dtype;
+  dk_norm_kind kind;
+  dk_gate_act act;
+  float residual_scale, block_scale, eps;
+} dk_block_norm_args;
+DK_API dk_status dk_block_norm(const dk_block_norm_args* args, void* stream);
+
 /* Human-readable text for a status; the CUDA error behind the last
  * DK_ERR_LAUNCH / DK_ERR_CUDA on this thread. */
 DK_API const char* dk_status_string(dk_status s);
