@@ -309,6 +309,16 @@ void check_table(const torch::Tensor& t, int64_t requests, const torch::Device& 
               "block_table must be int32 [requests, max_blocks] with contiguous rows");
 }
 
+// A tensor over part of another's storage, without the dispatcher's work of a
+// view (a plan makes four small tensors every step).
+torch::Tensor part_of(const torch::Tensor& whole, torch::ScalarType type, int64_t byte, int64_t n) {
+  torch::Tensor t = at::detail::make_tensor<c10::TensorImpl>(
+      c10::Storage(whole.storage()), whole.key_set(), c10::scalarTypeToTypeMeta(type));
+  t.unsafeGetTensorImpl()->set_storage_offset(byte / static_cast<int64_t>(c10::elementSize(type)));
+  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  return t;
+}
+
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> cache_plan(
     torch::Tensor held, torch::Tensor fresh, torch::Tensor block_table, torch::Tensor free_blocks,
     torch::Tensor ring, int64_t block_size, int64_t tokens, OptTensor lengths, OptTensor starts,
@@ -328,17 +338,21 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> cache_pla
   check_ints(free_blocks, torch::kInt32, free_blocks.numel(), device, "free_blocks");
   check_ints(ring, torch::kInt64, 4, device, "ring");
   const c10::cuda::CUDAGuard guard(device);
-  const auto ints = held.options();
-  const auto longs = ring.options();
-  auto given = [&](OptTensor& t, torch::ScalarType type, int64_t size, const char* what) {
-    if (t) check_ints(*t, type, size, device, what);
-    else t = torch::empty({size}, type == torch::kInt32 ? ints : longs);
+  // What is not given lies in one allocation: slots, ring, lengths, starts.
+  const int64_t ring_at = (8 * tokens + 15) / 16 * 16, lengths_at = ring_at + 32,
+                starts_at = lengths_at + 4 * n, bytes = starts_at + 4 * (n + 1);
+  torch::Tensor whole;
+  if (!lengths || !starts || !slots || !ring_out)
+    whole = torch::empty({bytes}, held.options().dtype(torch::kUInt8));
+  auto given = [&](OptTensor& t, torch::ScalarType type, int64_t at, int64_t size, const char* what) {
+    if (!t) return part_of(whole, type, at, size);
+    check_ints(*t, type, size, device, what);
     return *t;
   };
-  torch::Tensor l = given(lengths, torch::kInt32, n, "lengths");
-  torch::Tensor s = given(starts, torch::kInt32, n + 1, "starts");
-  torch::Tensor m = given(slots, torch::kInt64, tokens, "slots");
-  torch::Tensor r = given(ring_out, torch::kInt64, 4, "ring_out");
+  torch::Tensor l = given(lengths, torch::kInt32, lengths_at, n, "lengths");
+  torch::Tensor s = given(starts, torch::kInt32, starts_at, n + 1, "starts");
+  torch::Tensor m = given(slots, torch::kInt64, 0, tokens, "slots");
+  torch::Tensor r = given(ring_out, torch::kInt64, ring_at, 4, "ring_out");
   check_status(
       dk_cache_plan(held.data_ptr<int32_t>(), fresh.data_ptr<int32_t>(), static_cast<int>(n),
                     block_table.data_ptr<int32_t>(), static_cast<int>(block_table.size(1)),
@@ -364,11 +378,9 @@ void cache_append(torch::Tensor k, torch::Tensor v, torch::Tensor slots, const C
   const dk_dtype type = half_type(k, "k and v");
   check_ints(slots, torch::kInt64, k.size(0), device, "slots");
   const c10::cuda::CUDAGuard guard(device);
-  // A lane reads head_dim / 32 neighbouring values at once: re-home other views.
-  const int64_t piece = cache.c.head_dim / 32;
+  // The kernel reads 8 values at once: re-home views that do not allow it.
   auto fits = [&](const torch::Tensor& t) {
-    return t.stride(2) == 1 && t.stride(0) % piece == 0 && t.stride(1) % piece == 0 &&
-           reinterpret_cast<uintptr_t>(t.data_ptr()) % (2 * piece) == 0;
+    return t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && aligned16(t);
   };
   const torch::Tensor kc = fits(k) ? k : k.clone(at::MemoryFormat::Contiguous);
   const torch::Tensor vc = fits(v) ? v : v.clone(at::MemoryFormat::Contiguous);

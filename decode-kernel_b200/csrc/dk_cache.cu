@@ -45,13 +45,16 @@ __device__ __forceinline__ int last_at(const int* p, int n, int x) {
   return lo;
 }
 
+// VT: neighbouring slots of a thread, found with one search.
+template <int VT>
 __global__ void __launch_bounds__(kPlanThreads) k_cache_plan(const __grid_constant__ PlanArgs a) {
   extern __shared__ int raw[];
   constexpr int W = kPlanThreads / 32;
+  constexpr int PER = 4;  // neighbouring requests of a thread in one round of sums
   __shared__ int s_total[3][W];
   __shared__ int s_taken, s_wide;
   __shared__ unsigned long long s_missing;
-  int* s_tokens = raw;                    // [requests + 1] first new token
+  int* s_tokens = raw;                      // [requests + 1] first new token
   int* s_need = s_tokens + a.requests + 1;  // [requests + 1] first new page
   int* s_back = s_need + a.requests + 1;    // [requests + 1] first page given back
   int* s_held = s_back + a.requests + 1;    // [requests] tokens held, ~held if not served
@@ -60,28 +63,35 @@ __global__ void __launch_bounds__(kPlanThreads) k_cache_plan(const __grid_consta
     s_taken = s_wide = 0;
     s_missing = 0;
   }
-  const long long head = max(0LL, a.ring[0]), tail = max(0LL, a.ring[1]);
-  const int available = (int)max(0LL, min(tail - head, (long long)a.free_capacity));
   const int bs = a.block_size;
   int carry[3] = {0, 0, 0};
-  __syncthreads();
-  for (int base = 0, turn = 0; base < a.requests; base += kPlanThreads, ++turn) {
-    const int r = base + tid;
-    int c = 0, n = 0, have = 0;
+  pdl_trigger();
+  pdl_wait();
+  const long long head = max(0LL, a.ring[0]), tail = max(0LL, a.ring[1]);
+  const int available = (int)max(0LL, min(tail - head, (long long)a.free_capacity));
+  for (int base = 0, turn = 0; base < a.requests; base += kPlanThreads * PER, ++turn) {
+    const int r0 = base + tid * PER;
+    int c[PER], n[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      c[i] = r0 + i < a.requests ? a.held[r0 + i] : 0;
+      n[i] = r0 + i < a.requests ? a.fresh[r0 + i] : 0;
+    }
+    int need[PER], back[PER];
+    bool wide[PER];
     int mine[3] = {0, 0, 0};
-    bool ended = false, wide = false;
-    if (r < a.requests) {
-      c = max(a.held[r], 0);
-      n = a.fresh[r];
-      ended = n < 0;
-      n = max(n, 0);
-      have = c / bs + (c % bs != 0);
-      const long long all = (long long)c + n;
-      const long long want = (all + bs - 1) / bs;
-      wide = n > 0 && (want > a.max_blocks || all > INT_MAX);
-      mine[0] = n;
-      mine[1] = n > 0 && !wide ? (int)want - have : 0;
-      mine[2] = ended ? min(have, a.max_blocks) : 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      c[i] = max(c[i], 0);
+      const int have = c[i] / bs + (c[i] % bs != 0);
+      const unsigned all = (unsigned)c[i] + (unsigned)max(n[i], 0);
+      const unsigned want = all / (unsigned)bs + (all % (unsigned)bs != 0);
+      wide[i] = n[i] > 0 && (want > (unsigned)a.max_blocks || all > (unsigned)INT_MAX);
+      need[i] = n[i] > 0 && !wide[i] ? (int)want - have : 0;
+      back[i] = n[i] < 0 ? min(have, a.max_blocks) : 0;
+      mine[0] += max(n[i], 0);
+      mine[1] += need[i];
+      mine[2] += back[i];
     }
     int sum[3];
 #pragma unroll
@@ -104,21 +114,29 @@ __global__ void __launch_bounds__(kPlanThreads) k_cache_plan(const __grid_consta
         if (w < warp) before += x;
         carry[k] += x;
       }
-      sum[k] += before;  // up to and with request r
+      sum[k] += before - mine[k];  // up to the thread's first request
     }
-    if (r < a.requests) {
-      const bool lacking = mine[1] > 0 && (sum[1] > available || sum[1] < 0);
-      const bool served = !wide && !lacking;
-      s_tokens[r] = sum[0] - mine[0];
-      s_need[r] = sum[1] - mine[1];
-      s_back[r] = sum[2] - mine[2];
-      s_held[r] = served ? c : ~c;
-      if (lacking) atomicAdd(&s_missing, (unsigned long long)mine[1]);
-      else if (mine[1] > 0) atomicMax(&s_taken, sum[1]);
-      if (wide) atomicAdd(&s_wide, 1);
-      if (turn % (int)gridDim.x == cta) {
-        a.lengths[r] = ended ? 0 : served ? c + n : c;
-        a.starts[r] = sum[0] - mine[0];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int r = r0 + i;
+      if (r < a.requests) {
+        const int after = sum[1] + need[i];
+        const bool lacking = need[i] > 0 && (after > available || after < 0);
+        const bool served = !wide[i] && !lacking;
+        s_tokens[r] = sum[0];
+        s_need[r] = sum[1];
+        s_back[r] = sum[2];
+        s_held[r] = served ? c[i] : ~c[i];
+        if (lacking) atomicAdd(&s_missing, (unsigned long long)need[i]);
+        else if (need[i] > 0) atomicMax(&s_taken, after);
+        if (wide[i]) atomicAdd(&s_wide, 1);
+        if (turn % (int)gridDim.x == cta) {
+          a.lengths[r] = n[i] < 0 ? 0 : served ? c[i] + n[i] : c[i];
+          a.starts[r] = sum[0];
+        }
+        sum[0] += max(n[i], 0);
+        sum[1] = after;
+        sum[2] += back[i];
       }
     }
     __syncthreads();
@@ -144,6 +162,43 @@ __global__ void __launch_bounds__(kPlanThreads) k_cache_plan(const __grid_consta
     return x >= capacity || x < from ? x - capacity : x;
   };
   const int step = gridDim.x * kPlanThreads, id = cta * kPlanThreads + tid;
+  // Slots: VT neighbours a thread, in 16-byte stores.
+  const bool pairs = (reinterpret_cast<uintptr_t>(a.slots) & 15) == 0;
+  for (long long at = (long long)id * VT; at < a.tokens; at += (long long)step * VT) {
+    const int t0 = (int)at;
+    long long out[VT];
+    int r = a.requests ? last_at(s_tokens, a.requests, t0) : 0;
+    int known = -1, known_of = -1, page = 0;  // the page that the last slot is in
+#pragma unroll
+    for (int i = 0; i < VT; ++i) {
+      const int t = t0 + i;
+      out[i] = -1;
+      if (t < carry[0]) {
+        while (r + 1 < a.requests && s_tokens[r + 1] <= t) ++r;
+        const int c = s_held[r];
+        if (c >= 0) {
+          const int place = c + (t - s_tokens[r]), block = place / bs;
+          if (block != known || r != known_of) {
+            const int have = c / bs + (c % bs != 0);
+            page = block < have ? a.table[(long long)r * a.table_stride + block]
+                                : a.free_blocks[ring_at(head0, s_need[r] + block - have)];
+            known = block;
+            known_of = r;
+          }
+          out[i] = (long long)page * bs + (place - block * bs);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VT; i += 2) {
+      if (pairs && t0 + i + 1 < a.tokens) {
+        *reinterpret_cast<longlong2*>(a.slots + t0 + i) = make_longlong2(out[i], out[i + 1]);
+      } else {
+        if (t0 + i < a.tokens) a.slots[t0 + i] = out[i];
+        if (t0 + i + 1 < a.tokens) a.slots[t0 + i + 1] = out[i + 1];
+      }
+    }
+  }
   // New pages into the table.  Requests past the last served page are refused.
   for (int j = id; j < s_taken; j += step) {
     const int r = last_at(s_need, a.requests, j);
@@ -157,47 +212,30 @@ __global__ void __launch_bounds__(kPlanThreads) k_cache_plan(const __grid_consta
     const int r = last_at(s_back, a.requests, j);
     a.free_blocks[ring_at(tail0, j)] = a.table[(long long)r * a.table_stride + (j - s_back[r])];
   }
-  // Slots: two neighbours a thread, one 16-byte store.
-  const bool pairs = (reinterpret_cast<uintptr_t>(a.slots) & 15) == 0;
-  for (long long t2 = id; t2 * 2 < a.tokens; t2 += step) {
-    const int t0 = (int)(t2 * 2);
-    long long out[2] = {-1, -1};
-    int r = a.requests ? last_at(s_tokens, a.requests, t0) : 0;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int t = t0 + i;
-      if (t >= carry[0] || t < 0) break;
-      while (r + 1 < a.requests && s_tokens[r + 1] <= t) ++r;
-      const int c = s_held[r];
-      if (c < 0) continue;
-      const int at = c + (t - s_tokens[r]), block = at / bs;
-      const int have = c / bs + (c % bs != 0);
-      const int page = block < have ? a.table[(long long)r * a.table_stride + block]
-                                    : a.free_blocks[ring_at(head0, s_need[r] + block - have)];
-      out[i] = (long long)page * bs + (at - block * bs);
-    }
-    if (pairs && t0 + 1 < a.tokens) {
-      *reinterpret_cast<longlong2*>(a.slots + t0) = make_longlong2(out[0], out[1]);
-    } else {
-      a.slots[t0] = out[0];
-      if (t0 + 1 < a.tokens) a.slots[t0 + 1] = out[1];
-    }
-  }
 }
 
 // ---------------------------------------------------------------------------
-// Append.  A run is the call's tokens of one page; for each run, KV head and
-// of K and V one group of warps finds the largest magnitude, settles the
-// page's scale, codes the earlier rows again if it grew, and writes the new
-// codes.  Bound by bytes: 2 read and 1 written for each value (long runs), or
-// by the latency of the dependent steps slot -> page -> scale (single tokens).
-// A warp takes a short run alone, a lane holding D/32 neighbouring channels of
-// a row; the CTA takes a long one together, its rows dealt to the warps and
-// kept in registers between the maximum and the coding, so x is read once.
+// Append.  A run is the call's tokens of one page.  For each run, KV head and
+// of K and V: the largest magnitude, the page's scale, the earlier rows coded
+// again if it grew, the new codes.  Bound by bytes, 2 read and 1 written for
+// each value (long runs), or by latency (single tokens): slot -> scale and
+// values -> codes.
+//
+// A CTA looks for the runs that begin in its window of tokens, reading the
+// slots of the window and of the pages that may begin in it at once.  A short
+// run is a warp's, a long one the CTA's, its rows kept in registers between
+// the maximum and the coding, so the values are read once.  A lane holds 8
+// neighbouring channels (16 bytes read, 8 written).  Earlier rows that a single
+// token's larger value makes to be coded again are left to the whole CTA.
+// The largest magnitude is taken over the 16-bit patterns without their sign,
+// which order as the values do, infinities and NaN above all: only where one
+// of those turns up does a slower path look at each value.
 // ---------------------------------------------------------------------------
-constexpr int kAppendWarps = 8;
-constexpr int kShortRun = 8;   // rows that a warp takes alone
-constexpr int kKeep = 16;      // rows of a long run that a warp keeps in registers
+constexpr int kAppendWarps = 4;
+constexpr int kShortRun = 8;  // rows that a warp takes alone
+constexpr int kKeep = 8;      // pieces of 8 values that a lane keeps
+constexpr int kMaxWindow = 64;
+constexpr int kMaxBlock = 256;
 constexpr float kLeastAmax = 8.673617379884035e-19f;  // 2^-60
 
 struct AppendArgs {
@@ -207,216 +245,239 @@ struct AppendArgs {
   long long block_stride[2], head_stride[2], row_stride[2];
   long long x_token_stride[2], x_head_stride[2];
   const long long* slots;
+  unsigned long long block_magic;  // ceil(2^64 / block_size): slot / block_size is the high half of the product
   int tokens, blocks, block_size, kv_heads, window, bf16;
 };
 
-template <int N>
-struct Piece {  // N neighbouring 16-bit values
-  uint32_t w[N / 2];
-};
-
-template <int N>
-__device__ __forceinline__ Piece<N> load_piece(const uint16_t* p) {
-  Piece<N> r;
-  if constexpr (N == 8) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
-    r.w[0] = v.x; r.w[1] = v.y; r.w[2] = v.z; r.w[3] = v.w;
-  } else if constexpr (N == 4) {
-    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-    r.w[0] = v.x; r.w[1] = v.y;
-  } else {
-    r.w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
-  }
-  return r;
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
 }
 
-template <int N>
-__device__ __forceinline__ void to_float(const Piece<N>& p, int bf16, float (&x)[N]) {
+__device__ __forceinline__ void to_float8(const uint4& p, int bf16, float (&x)[8]) {
+  const uint32_t w[4] = {p.x, p.y, p.z, p.w};
 #pragma unroll
-  for (int i = 0; i < N / 2; ++i) {
+  for (int i = 0; i < 4; ++i) {
     if (bf16) {
-      x[2 * i] = __uint_as_float(p.w[i] << 16);
-      x[2 * i + 1] = __uint_as_float(p.w[i] & 0xffff0000u);
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     } else {
-      const __half2 h = *reinterpret_cast<const __half2*>(&p.w[i]);
+      const __half2 h = *reinterpret_cast<const __half2*>(&w[i]);
       x[2 * i] = __low2float(h);
       x[2 * i + 1] = __high2float(h);
     }
   }
 }
 
-template <int N>
-__device__ __forceinline__ float largest(const float (&x)[N]) {
-  float m = 0.f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float y = fabsf(x[i]);
-    m = fmaxf(m, y < INFINITY ? y : 0.f);
+// Four values to four codes.  CHECK: the values may be past the scale or NaN.
+template <bool E4M3, bool CHECK>
+__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
+  if constexpr (CHECK) {
+    constexpr float Q = E4M3 ? 448.f : 127.f;
+    a = a == a ? fminf(fmaxf(a, -Q), Q) : 0.f;
+    b = b == b ? fminf(fmaxf(b, -Q), Q) : 0.f;
+    c = c == c ? fminf(fmaxf(c, -Q), Q) : 0.f;
+    d = d == d ? fminf(fmaxf(d, -Q), Q) : 0.f;
   }
-  return m;
-}
-
-// Two values to two codes (the low byte is a's).
-template <bool E4M3>
-__device__ __forceinline__ uint32_t encode2(float a, float b) {
-  constexpr float Q = E4M3 ? 448.f : 127.f;
-  a = a == a ? fminf(fmaxf(a, -Q), Q) : 0.f;
-  b = b == b ? fminf(fmaxf(b, -Q), Q) : 0.f;
   if constexpr (E4M3) {
-    uint16_t r;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
+    uint32_t r;
+    asm("{\n .reg .b16 l, h;\n cvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\n"
+        " cvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\n mov.b32 %0, {l, h};\n}"
+        : "=r"(r)
+        : "f"(a), "f"(b), "f"(c), "f"(d));
     return r;
   } else {
-    return ((uint32_t)__float2int_rn(a) & 0xffu) | (((uint32_t)__float2int_rn(b) & 0xffu) << 8);
+    // 1.5 * 2^23 moves the rounded (to nearest even) value into the low byte.
+    constexpr float kMagic = 12582912.f;
+    const uint32_t lo = prmt(__float_as_uint(__fadd_rn(a, kMagic)), __float_as_uint(__fadd_rn(b, kMagic)), 0x0040);
+    const uint32_t hi = prmt(__float_as_uint(__fadd_rn(c, kMagic)), __float_as_uint(__fadd_rn(d, kMagic)), 0x0040);
+    return prmt(lo, hi, 0x5410);
   }
 }
 
 template <bool E4M3>
-__device__ __forceinline__ void decode2(uint32_t w, float& a, float& b) {
+__device__ __forceinline__ uint2 encode8(const uint4& p, int bf16, float by, bool check) {
+  float x[8];
+  to_float8(p, bf16, x);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(x[i], by);
+  if (check) return make_uint2(encode4<E4M3, true>(x[0], x[1], x[2], x[3]), encode4<E4M3, true>(x[4], x[5], x[6], x[7]));
+  return make_uint2(encode4<E4M3, false>(x[0], x[1], x[2], x[3]), encode4<E4M3, false>(x[4], x[5], x[6], x[7]));
+}
+
+// Four codes to the codes of a larger scale.
+template <bool E4M3>
+__device__ __forceinline__ uint32_t code_again(uint32_t w, float ratio) {
+  float x[4];
   if constexpr (E4M3) {
-    uint32_t h;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)w));
-    const __half2 x = *reinterpret_cast<const __half2*>(&h);
-    a = __low2float(x);
-    b = __high2float(x);
+    uint32_t lo, hi;
+    asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n cvt.rn.f16x2.e4m3x2 %0, l;\n cvt.rn.f16x2.e4m3x2 %1, h;\n}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
+    const __half2 a = *reinterpret_cast<const __half2*>(&lo), b = *reinterpret_cast<const __half2*>(&hi);
+    x[0] = __low2float(a); x[1] = __high2float(a);
+    x[2] = __low2float(b); x[3] = __high2float(b);
   } else {
-    a = (float)(int8_t)(w & 0xffu);
-    b = (float)(int8_t)((w >> 8) & 0xffu);
-  }
-}
-
-template <int N, bool E4M3>
-__device__ __forceinline__ void store_codes(uint8_t* p, const float (&x)[N], float by) {
-  uint32_t w[(N + 3) / 4];
 #pragma unroll
-  for (int i = 0; i < N / 2; ++i) {
-    const uint32_t two = encode2<E4M3>(__fmul_rn(x[2 * i], by), __fmul_rn(x[2 * i + 1], by));
-    if (i & 1) w[i / 2] |= two << 16; else w[i / 2] = two;
+    for (int i = 0; i < 4; ++i) x[i] = (float)((int)(w << (24 - 8 * i)) >> 24);
   }
-  if constexpr (N == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-  else if constexpr (N == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
-  else *reinterpret_cast<uint16_t*>(p) = (uint16_t)w[0];
-}
-
-template <int N, bool E4M3>
-__device__ __forceinline__ void code_again(uint8_t* p, float ratio) {
-  uint32_t w[(N + 3) / 4];
-  if constexpr (N == 8) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    w[0] = v.x; w[1] = v.y;
-  } else if constexpr (N == 4) {
-    w[0] = *reinterpret_cast<const uint32_t*>(p);
-  } else {
-    w[0] = *reinterpret_cast<const uint16_t*>(p);
-  }
-  float x[N];
 #pragma unroll
-  for (int i = 0; i < N / 2; ++i) decode2<E4M3>(w[i / 2] >> (16 * (i & 1)), x[2 * i], x[2 * i + 1]);
-  store_codes<N, E4M3>(p, x, ratio);
+  for (int i = 0; i < 4; ++i) x[i] = __fmul_rn(x[i], ratio);
+  return encode4<E4M3, E4M3>(x[0], x[1], x[2], x[3]);  // int8 codes get no larger; e4m3's may be NaN
 }
 
 template <int D, bool E4M3>
 __global__ void __launch_bounds__(kAppendWarps * 32) k_cache_append(const __grid_constant__ AppendArgs a) {
-  constexpr int N = D / 32;
   constexpr float Q = E4M3 ? 448.f : 127.f;
-  __shared__ float s_top[kAppendWarps];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int LPR = D / 8;     // lanes of a row
+  constexpr int RPW = 32 / LPR;  // rows of a warp's load
+  constexpr int kSpan = kMaxWindow + kMaxBlock;
+  struct Job {  // earlier rows to be coded again
+    uint8_t* rows;
+    int n;
+    float ratio;
+  };
+  __shared__ long long s_slot[kSpan + 1];
+  __shared__ uint32_t s_break[kSpan / 32 + 1];
+  __shared__ uint32_t s_top[2][kAppendWarps];
+  __shared__ Job s_job[kMaxWindow];
+  __shared__ int s_jobs;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int h = blockIdx.y, which = blockIdx.z, bs = a.block_size;
   const int first = blockIdx.x * a.window;
-  // The runs that begin in this CTA's window of tokens.
-  const int t = first + lane;
-  long long slot = -1;
-  bool begins = false;
-  if (lane < a.window && t < a.tokens) {
-    slot = a.slots[t];
-    begins = slot >= 0 && slot / bs < a.blocks;
-    if (begins && t > 0 && slot % bs != 0) begins = a.slots[t - 1] != slot - 1;
-  }
-  uint32_t runs = __ballot_sync(0xffffffffu, begins);
-  for (int turn = 0; runs; runs &= runs - 1, ++turn) {
-    const int src = __ffs(runs) - 1;
-    const int t0 = first + src;
-    const long long s0 = __shfl_sync(0xffffffffu, slot, src);
-    const long long page = s0 / bs;
-    const int row0 = (int)(s0 - page * bs);
-    const int most = min(bs - row0, a.tokens - t0);
-    int n = 1;  // rows of the run
-    while (n < most) {
-      const int i = n + lane;
-      const uint32_t same = __ballot_sync(0xffffffffu, i < most && a.slots[t0 + i] == s0 + i);
-      n += __ffs(~same) ? __ffs(~same) - 1 : 32;
-      if (same != 0xffffffffu) break;
+  const long long xs = a.x_token_stride[which], ps = a.row_stride[which];
+  const uint16_t* x_base = a.x[which] + h * a.x_head_stride[which] + (lane % LPR) * 8;
+  const int sub = lane / LPR;
+  pdl_trigger();
+  pdl_wait();
+  // The warp's token of a small window, while its slot is on its way.
+  uint4 ahead = make_uint4(0, 0, 0, 0);
+  if (a.window == kAppendWarps && first + warp < a.tokens && sub == 0)
+    ahead = *reinterpret_cast<const uint4*>(x_base + (long long)(first + warp) * xs);
+  // s_slot[i]: the slot of token first - 1 + i.  A token breaks the run before
+  // it if it has no slot, begins a page or does not follow its neighbour.
+  const int span = min(a.window + bs, a.tokens - first);
+  for (int i = tid; i <= span; i += kAppendWarps * 32) s_slot[i] = first - 1 + i >= 0 ? a.slots[first - 1 + i] : -1;
+  if (tid == 0) s_jobs = 0;
+  __syncthreads();
+  auto page_of = [&](long long slot) { return (long long)__umul64hi((unsigned long long)slot, a.block_magic); };
+  for (int i = tid; i < (span + 31) / 32 * 32; i += kAppendWarps * 32) {
+    bool breaks = true;
+    if (i < span) {
+      const long long slot = s_slot[i + 1];
+      breaks = slot < 0 || s_slot[i] != slot - 1 || page_of(slot) * bs == slot;
     }
+    const uint32_t bits = __ballot_sync(0xffffffffu, breaks);
+    if (lane == 0) s_break[i >> 5] = bits;
+  }
+  __syncthreads();
+  auto next_break = [&](int i) {  // the first at or after i, at most span
+    while (i < span) {
+      const uint32_t bits = s_break[i >> 5] >> (i & 31);
+      if (bits) return min(span, i + __ffs(bits) - 1);
+      i = (i | 31) + 1;
+    }
+    return span;
+  };
+  auto again = [&](uint8_t* rows, int n, float ratio, int w, int warps) {
+    constexpr int LR = D / 16, RW = 32 / LR;  // 16 codes a lane
+#pragma unroll 4
+    for (int i = w * RW + lane / LR; i < n; i += warps * RW) {
+      uint4* p = reinterpret_cast<uint4*>(rows + i * ps + lane % LR * 16);
+      const uint4 c = *p;
+      *p = make_uint4(code_again<E4M3>(c.x, ratio), code_again<E4M3>(c.y, ratio), code_again<E4M3>(c.z, ratio), code_again<E4M3>(c.w, ratio));
+    }
+  };
+  int turn = 0, big = 0;
+  for (int i0 = next_break(0); i0 < min(span, a.window); i0 = next_break(i0 + 1)) {
+    const long long slot = s_slot[i0 + 1];
+    const long long page = page_of(slot);
+    if (slot < 0 || page >= a.blocks) continue;
+    const int row0 = (int)(slot - page * bs);
+    const int n = next_break(i0 + 1) - i0;
     const bool alone = n <= kShortRun;
-    if (alone && turn % kAppendWarps != warp) continue;
-    const int w0 = alone ? 0 : warp, step = alone ? 1 : kAppendWarps;
-    const uint16_t* x = a.x[which] + (long long)t0 * a.x_token_stride[which] + h * a.x_head_stride[which] + lane * N;
-    const long long xs = a.x_token_stride[which], ps = a.row_stride[which];
-    uint8_t* pool = a.pool[which] + page * a.block_stride[which] + h * a.head_stride[which] + lane * N;
+    if (alone && turn++ % kAppendWarps != warp) continue;
+    const int w0 = alone ? sub : warp * RPW + sub, step = alone ? RPW : kAppendWarps * RPW;
+    const uint16_t* x = x_base + (long long)(first + i0) * xs;
+    uint8_t* pool = a.pool[which] + page * a.block_stride[which] + h * a.head_stride[which];
     float* scale = a.scale[which] + page * a.kv_heads + h;
     const float old = row0 > 0 ? *scale : 0.f;
 
-    Piece<N> keep[kKeep];
-    float top = 0.f;
+    uint4 keep[kKeep];
+    uint32_t top2 = 0;
+    if (a.window == kAppendWarps && n == 1 && i0 == warp) {
+      keep[0] = ahead;
+    } else {
 #pragma unroll
-    for (int k = 0; k < kKeep; ++k) {
-      const int i = w0 + k * step;
-      if (i < n) keep[k] = load_piece<N>(x + i * xs);
+      for (int k = 0; k < kKeep; ++k)
+        if (w0 + k * step < n) keep[k] = *reinterpret_cast<const uint4*>(x + (w0 + k * step) * xs);
     }
+    auto add = [&](const uint4& p) {
+      top2 = max_u16x2(max_u16x2(top2, p.x & 0x7fff7fffu), max_u16x2(p.y & 0x7fff7fffu, max_u16x2(p.z & 0x7fff7fffu, p.w & 0x7fff7fffu)));
+    };
 #pragma unroll
-    for (int k = 0; k < kKeep; ++k) {
-      if (w0 + k * step < n) {
-        float v[N];
-        to_float<N>(keep[k], a.bf16, v);
-        top = fmaxf(top, largest<N>(v));
+    for (int k = 0; k < kKeep; ++k)
+      if (w0 + k * step < n) add(keep[k]);
+    for (int i = w0 + kKeep * step; i < n; i += step) add(*reinterpret_cast<const uint4*>(x + i * xs));
+    auto over_all = [&](uint32_t v) {  // the largest of the run's warps; `old` is read before any scale changes
+      v = __reduce_max_sync(0xffffffffu, v);
+      if (!alone) {
+        if (lane == 0) s_top[big & 1][warp] = v;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kAppendWarps; ++w) v = max(v, s_top[big & 1][w]);
+        ++big;
       }
-    }
-    for (int i = w0 + kKeep * step; i < n; i += step) {
-      float v[N];
-      to_float<N>(load_piece<N>(x + i * xs), a.bf16, v);
-      top = fmaxf(top, largest<N>(v));
-    }
+      return v;
+    };
+    uint32_t top = over_all(max(top2 & 0xffffu, top2 >> 16));
+    const uint32_t infinite = a.bf16 ? 0x7f80u : 0x7c00u;
+    const bool odd = top >= infinite;  // the same in all of the run's warps
+    if (odd) {
+      uint32_t finite = 0;
+      for (int i = w0; i < n; i += step) {
+        const uint4 p = *reinterpret_cast<const uint4*>(x + i * xs);
+        const uint32_t w[4] = {p.x, p.y, p.z, p.w};
 #pragma unroll
-    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    if (!alone) {
-      if (lane == 0) s_top[warp] = top;
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < kAppendWarps; ++w) top = fmaxf(top, s_top[w]);
-      __syncthreads();  // every thread has `old` and the maxima before the scale changes
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t lo = w[k] & 0x7fffu, hi = (w[k] >> 16) & 0x7fffu;
+          if (lo < infinite) finite = max(finite, lo);
+          if (hi < infinite) finite = max(finite, hi);
+        }
+      }
+      top = over_all(finite);
     }
-    const float now = fmaxf(old, __fdiv_rn(fmaxf(top, kLeastAmax), Q));
-    if (now > old) {
-      if (lane == 0 && w0 == 0) *scale = now;
-      const float ratio = __fdiv_rn(old, now);
-#pragma unroll 4
-      for (int i = w0; i < row0; i += step) code_again<N, E4M3>(pool + i * ps, ratio);
-    }
+    const float amax = a.bf16 ? __uint_as_float(top << 16) : __half2float(__ushort_as_half((unsigned short)top));
+    const float now = fmaxf(old, __fdiv_rn(fmaxf(amax, kLeastAmax), Q));
     const float by = __frcp_rn(now);
-    uint8_t* to = pool + row0 * ps;
+    uint8_t* to = pool + row0 * ps + (lane % LPR) * 8;
 #pragma unroll
-    for (int k = 0; k < kKeep; ++k) {
-      const int i = w0 + k * step;
-      if (i < n) {
-        float v[N];
-        to_float<N>(keep[k], a.bf16, v);
-        store_codes<N, E4M3>(to + i * ps, v, by);
+    for (int k = 0; k < kKeep; ++k)
+      if (w0 + k * step < n) *reinterpret_cast<uint2*>(to + (w0 + k * step) * ps) = encode8<E4M3>(keep[k], a.bf16, by, odd);
+    for (int i = w0 + kKeep * step; i < n; i += step)
+      *reinterpret_cast<uint2*>(to + i * ps) = encode8<E4M3>(*reinterpret_cast<const uint4*>(x + i * xs), a.bf16, by, odd);
+    if (now > old) {
+      if (lane == 0 && (alone || warp == 0)) *scale = now;
+      if (row0 > 0) {
+        const float ratio = __fdiv_rn(old, now);
+        if (!alone) {
+          again(pool, row0, ratio, warp, kAppendWarps);
+        } else if (lane == 0) {
+          s_job[atomicAdd(&s_jobs, 1)] = Job{pool, row0, ratio};
+        }
       }
-    }
-    for (int i = w0 + kKeep * step; i < n; i += step) {
-      float v[N];
-      to_float<N>(load_piece<N>(x + i * xs), a.bf16, v);
-      store_codes<N, E4M3>(to + i * ps, v, by);
     }
   }
+  __syncthreads();
+  for (int j = 0; j < s_jobs; ++j) again(s_job[j].rows, s_job[j].n, s_job[j].ratio, warp, kAppendWarps);
 }
 
 template <int D>
 dk_status launch_append(const AppendArgs& a, bool e4m3, cudaStream_t stream) {
   const dim3 grid((a.tokens + a.window - 1) / a.window, a.kv_heads, 2);
-  if (e4m3) k_cache_append<D, true><<<grid, kAppendWarps * 32, 0, stream>>>(a);
-  else k_cache_append<D, false><<<grid, kAppendWarps * 32, 0, stream>>>(a);
-  return check_launch("dk_cache_append");
+  return launch_early("dk_cache_append", e4m3 ? k_cache_append<D, true> : k_cache_append<D, false>, grid,
+                      dim3(kAppendWarps * 32), 0, stream, a);
 }
 
 }  // namespace
@@ -453,21 +514,25 @@ extern "C" dk_status dk_cache_plan(const int32_t* held, const int32_t* fresh, in
   a.free_capacity = free_capacity;
   a.tokens = tokens;
   const size_t smem = sizeof(int) * (4 * (size_t)requests + 3);
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(k_cache_plan, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  // Two slots a thread are the least latency; from where those would need more
+  // threads than the GPU holds, eight share a search and their pages.
+  const bool many = tokens > 2 * kPlanThreads * sm_count(-1);
+  auto kernel = many ? k_cache_plan<8> : k_cache_plan<2>;
+  if (smem > 48 * 1024 - 512) {  // the rest of it is static
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                (int)(sizeof(int) * (4 * DK_PLAN_MAX_REQUESTS + 3)));
     if (e != cudaSuccess) {
       set_cuda_error(e, "cudaFuncSetAttribute");
       return DK_ERR_CUDA;
     }
   }
-  // CTAs enough for two tokens and one request a thread.  Where an output is
-  // an input one CTA does it all: it has read what the others would still need.
-  const int work = std::max((tokens + 1) / 2, requests);
-  int grid = std::min(sm_count(-1), std::max(1, (work + kPlanThreads - 1) / kPlanThreads));
+  // Where an output is an input one CTA does it all: it has read what the
+  // others would still need.
+  const int each = kPlanThreads * (many ? 8 : 2);
+  const int work = std::max((tokens + each - 1) / each, (requests + 4 * kPlanThreads - 1) / (4 * kPlanThreads));
+  int grid = std::min(sm_count(-1), std::max(1, work));
   if (lengths == held || ring_out == ring) grid = 1;
-  k_cache_plan<<<grid, kPlanThreads, smem, static_cast<cudaStream_t>(stream)>>>(a);
-  return check_launch("dk_cache_plan");
+  return launch_early("dk_cache_plan", kernel, dim3(grid), dim3(kPlanThreads), smem, static_cast<cudaStream_t>(stream), a);
 }
 
 extern "C" dk_status dk_cache_append(const dk_cache8* c, const void* k, const void* v,
@@ -486,12 +551,11 @@ extern "C" dk_status dk_cache_append(const dk_cache8* c, const void* k, const vo
                              c->v_block_stride, c->v_head_stride, c->v_token_stride};
   for (int64_t s : strides)
     if (s < 0 || s % 32) return DK_ERR_INVALID_ARG;
-  const int piece = c->head_dim / 32;
   const int64_t in[] = {k_token_stride, k_head_stride, v_token_stride, v_head_stride};
   for (int64_t s : in)
-    if (s % piece) return DK_ERR_INVALID_ARG;
+    if (s % 8) return DK_ERR_INVALID_ARG;
   auto aligned = [](const void* x, uintptr_t n) { return reinterpret_cast<uintptr_t>(x) % n == 0; };
-  if (!aligned(c->k, 32) || !aligned(c->v, 32) || !aligned(k, 2 * piece) || !aligned(v, 2 * piece))
+  if (!aligned(c->k, 32) || !aligned(c->v, 32) || !aligned(k, 16) || !aligned(v, 16))
     return DK_ERR_INVALID_ARG;
   AppendArgs a;
   a.pool[0] = static_cast<uint8_t*>(c->k);
@@ -516,9 +580,11 @@ extern "C" dk_status dk_cache_append(const dk_cache8* c, const void* k, const vo
   a.block_size = c->block_size;
   a.kv_heads = c->kv_heads;
   a.bf16 = dtype == DK_BF16;
-  // A window of 8 tokens gives each warp one token of a decode step; with many
-  // tokens windows of 32 leave fewer CTAs without a run's beginning.
-  a.window = (long long)tokens * c->kv_heads * 2 / 32 >= 4LL * sm_count(-1) ? 32 : 8;
+  a.block_magic = ~0ull / (unsigned long long)c->block_size + 1;
+  // The window: four tokens, one for each warp, while the GPU holds the CTAs
+  // that this makes; more where most windows would hold no run's beginning.
+  const long long each = (long long)tokens * c->kv_heads * 2, room = 20LL * sm_count(-1);
+  a.window = each / kAppendWarps <= room ? kAppendWarps : each / 16 <= room ? 16 : kMaxWindow;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool e4m3 = c->code == DK_E4M3;
   if (c->head_dim == 64) return launch_append<64>(a, e4m3, st);

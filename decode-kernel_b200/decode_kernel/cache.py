@@ -16,6 +16,18 @@ import torch
 
 __all__ = ["CachePlan", "PagedCache8", "cache_append", "cache_attention", "cache_plan"]
 
+_module = None
+
+
+def _extension():
+    """decode_kernel._cuda, imported at the first call: the package loads without it."""
+    global _module
+    if _module is None:
+        from . import _cuda
+
+        _module = _cuda
+    return _module
+
 
 class PagedCache8:
     """Pages of ``block_size`` tokens of every KV head.
@@ -45,9 +57,7 @@ class PagedCache8:
         return self
 
     def _set(self, k, v, k_scale, v_scale) -> None:
-        from . import _cuda
-
-        self._handle = _cuda.Cache8(k, v, k_scale, v_scale)
+        self._handle = _extension().Cache8(k, v, k_scale, v_scale)
         self._tensors = (k, v, k_scale, v_scale)
 
     k = property(lambda self: self._tensors[0])
@@ -96,11 +106,9 @@ def cache_plan(held: torch.Tensor, fresh: torch.Tensor, block_table: torch.Tenso
     ``out`` reuses tensors of an earlier plan; its ``lengths`` may be ``held``
     and its ``ring`` may be ``ring``.
     """
-    from . import _cuda
-
     if out is None:
-        return CachePlan(*_cuda.cache_plan(held, fresh, block_table, free_blocks, ring, block_size, tokens))
-    return CachePlan(*_cuda.cache_plan(held, fresh, block_table, free_blocks, ring, block_size, tokens, *out))
+        return CachePlan(*_extension().cache_plan(held, fresh, block_table, free_blocks, ring, block_size, tokens))
+    return CachePlan(*_extension().cache_plan(held, fresh, block_table, free_blocks, ring, block_size, tokens, *out))
 
 
 def cache_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: PagedCache8) -> None:
@@ -113,9 +121,7 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: P
     past the scale saturate, NaN becomes 0.  The rows of a page must be
     neighbours with rising slots.
     """
-    from . import _cuda
-
-    _cuda.cache_append(k, v, slots, cache._handle)
+    _extension().cache_append(k, v, slots, cache._handle)
 
 
 def cache_attention(q: torch.Tensor, cache: PagedCache8, block_table: torch.Tensor,
@@ -135,7 +141,5 @@ def cache_attention(q: torch.Tensor, cache: PagedCache8, block_table: torch.Tens
     Returns out, or (out, lse) with the fp32 [tokens, q_heads] log of the sums
     of exponentials.
     """
-    from . import _cuda
-
-    o, l = _cuda.cache_attention(q, cache._handle, block_table, lengths, starts, scale, causal, window, out, lse)
+    o, l = _extension().cache_attention(q, cache._handle, block_table, lengths, starts, scale, causal, window, out, lse)
     return (o, l) if lse else o

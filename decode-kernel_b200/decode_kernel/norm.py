@@ -6,6 +6,8 @@ from typing import Optional, Tuple
 
 import torch
 
+from .cache import _extension
+
 __all__ = ["block_norm"]
 
 _KINDS = {"rms": 0, "layer": 1}
@@ -30,9 +32,7 @@ def block_norm(residual: torch.Tensor, y: Optional[torch.Tensor] = None, *, kind
     Without y, h = norm(residual_scale * residual).  Computed in fp32 and
     rounded once, h from the unrounded r.  ``inplace`` writes r over residual.
     """
-    from . import _cuda
-
     if kind not in _KINDS or gate_act not in _ACTS:
         raise ValueError("kind is 'rms' or 'layer', gate_act 'none', 'sigmoid' or 'silu'")
-    return _cuda.block_norm(residual, y, _KINDS[kind], post_weight, post_bias, gate, _ACTS[gate_act],
+    return _extension().block_norm(residual, y, _KINDS[kind], post_weight, post_bias, gate, _ACTS[gate_act],
                             residual_scale, block_scale, pre_weight, pre_bias, eps, inplace)

@@ -400,8 +400,8 @@ DK_API dk_status dk_cache_plan(const int32_t* held, const int32_t* fresh, int re
                                int32_t* starts, int64_t* slots, int tokens, void* stream);
 
 /* New keys and values into their pages: token t of k and v ([tokens, kv_heads,
- * head_dim], DK_FP16 or DK_BF16, token and head strides in elements, last
- * dimension contiguous) goes to slots[t] = page * block_size + row.  Slots
+ * head_dim], DK_FP16 or DK_BF16, token and head strides in elements, multiples
+ * of 8, last dimension contiguous, 16-byte aligned) goes to slots[t] = page * block_size + row.  Slots
  * below 0 or past the pool are skipped.  The tokens of a page are neighbours
  * in t, with rising rows, and a page gets tokens of one request only
  * (dk_cache_plan's slots are so).
