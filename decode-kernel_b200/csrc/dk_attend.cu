@@ -108,20 +108,34 @@ __device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& lo, uint32_t
   }
 }
 
+// The kernel may start while the call before it still runs (programmatic
+// launch), so nothing is read through the non-coherent path: that data would
+// have to be constant for the kernel's whole life.
+__device__ __forceinline__ int ld_int(const int* p) {
+  int x;
+  asm volatile("ld.global.b32 %0, [%1];" : "=r"(x) : "l"(p));
+  return x;
+}
+__device__ __forceinline__ float ld_float(const float* p) {
+  float x;
+  asm volatile("ld.global.b32 %0, [%1];" : "=f"(x) : "l"(p));
+  return x;
+}
+
 template <int WORDS>
 __device__ __forceinline__ void ldg_words(const uint8_t* p, uint32_t* r) {
   static_assert(WORDS == 2 || WORDS == 4 || WORDS == 8, "");
   if constexpr (WORDS == 8) {
-    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+    asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
                    "=r"(r[6]), "=r"(r[7])
                  : "l"(p));
   } else if constexpr (WORDS == 4) {
-    asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
+    asm volatile("ld.global.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                  : "l"(p));
   } else {
-    asm volatile("ld.global.nc.L1::no_allocate.v2.b32 {%0,%1}, [%2];"
+    asm volatile("ld.global.L1::no_allocate.v2.b32 {%0,%1}, [%2];"
                  : "=r"(r[0]), "=r"(r[1])
                  : "l"(p));
   }
@@ -131,6 +145,7 @@ __device__ __forceinline__ void ldg_words(const uint8_t* p, uint32_t* r) {
 struct Segment {
   int request, head, tile;
   int length, fresh, first_token;  // tokens held, queries, row of the first query in q
+  int which, all;                  // its number among the request's segments, and how many they are
   int unit0, units;                // its first unit among the request's, and how many
   int begin;                       // its first unit in the line of all units
 };
@@ -162,40 +177,55 @@ struct Attend {
     return (fresh * a.group + kRows - 1) / kRows;
   }
   __device__ static __forceinline__ void request_of(const AttendArgs& a, int r, int& length, int& fresh, int& first) {
-    length = min(max(__ldg(a.lengths + r), 0), (int)min((long long)a.max_blocks * a.block_size, 0x7fffffffLL));
+    length = min(max(ld_int(a.lengths + r), 0), (int)min((long long)a.max_blocks * a.block_size, 0x7fffffffLL));
     if (a.starts) {
-      first = __ldg(a.starts + r);
-      fresh = max(0, __ldg(a.starts + r + 1) - first);
+      first = ld_int(a.starts + r);
+      fresh = max(0, ld_int(a.starts + r + 1) - first);
     } else {
       first = r;
       fresh = 1;
     }
   }
 
+  // Segment `which` of request r.
+  __device__ static __forceinline__ Segment segment_of(const AttendArgs& a, const int* prefix, int r, int which) {
+    Segment s;
+    s.request = r;
+    request_of(a, r, s.length, s.fresh, s.first_token);
+    s.units = units_of(a, s.length, s.fresh, s.unit0);
+    s.which = which;
+    s.begin = prefix[r] + which * s.units;
+    const int tiles = tiles_of(a, s.fresh);
+    s.all = tiles * a.kv_heads;
+    s.head = tiles == 1 ? which : which / tiles;
+    s.tile = which - s.head * tiles;
+    return s;
+  }
+  // The segment of unit u of the line.
   __device__ static __forceinline__ Segment segment_at(const AttendArgs& a, const int* prefix, int u) {
     int lo = 0, hi = a.requests - 1;  // the last request whose first unit is at or before u
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
       if (prefix[mid] <= u) lo = mid; else hi = mid - 1;
     }
-    Segment s;
-    s.request = lo;
-    request_of(a, lo, s.length, s.fresh, s.first_token);
-    s.units = units_of(a, s.length, s.fresh, s.unit0);
-    const int tiles = tiles_of(a, s.fresh);
-    const int local = u - prefix[lo];
-    const int which = local / s.units;
-    s.begin = prefix[lo] + which * s.units;
-    s.head = which / tiles;
-    s.tile = which - s.head * tiles;
-    return s;
+    Segment s = segment_of(a, prefix, lo, 0);
+    const int which = (u - s.begin) / s.units;
+    return which ? segment_of(a, prefix, lo, which) : s;
+  }
+  // The segment after s.
+  __device__ static __forceinline__ Segment segment_after(const AttendArgs& a, const int* prefix, const Segment& s) {
+    if (s.which + 1 < s.all) return segment_of(a, prefix, s.request, s.which + 1);
+    int r = s.request + 1;  // some request after it has units
+    const int u = s.begin + s.units;
+    while (r + 1 < a.requests && prefix[r + 1] <= u) ++r;
+    return segment_of(a, prefix, r, 0);
   }
 
   // Token range [low, high) that query row `row` of the segment sees, and its
   // place in q and out; false where the tile has no such row.
   __device__ static __forceinline__ bool row_of(const AttendArgs& a, const Segment& s, int row, int& token, int& head, int& low, int& high) {
     const int all = s.tile * kRows + row;
-    const int i = all / a.group;
+    const int i = s.fresh == 1 ? (all >= a.group) : all / a.group;
     token = s.first_token + i;
     head = s.head * a.group + all - i * a.group;
     low = high = 0;
@@ -206,9 +236,8 @@ struct Attend {
   }
 
   // Row `row` of q as this lane's words of the B operand, in K's order of
-  // channels; bf16 rows are scaled by a power of two into fp16's range (the
-  // return value undoes it).
-  __device__ static __forceinline__ float load_q(const AttendArgs& a, const Segment& s, int row, uint32_t (&b)[2 * kKWords]) {
+  // channels.
+  __device__ static __forceinline__ void load_q(const AttendArgs& a, const Segment& s, int row, uint32_t (&b)[2 * kKWords]) {
     const int c = threadIdx.x & 3;
     int token, head, low, high;
     const bool there = row_of(a, s, row, token, head, low, high);
@@ -220,10 +249,13 @@ struct Attend {
 #pragma unroll
       for (int i = 0; i < kKWords / 2; ++i) {  // 8 channels each
         const int at = (i * 8) % kSpan + (i * 8) / kSpan * 128;
-        const uint4 x = __ldg(reinterpret_cast<const uint4*>(p + at));
-        b[4 * i] = x.x; b[4 * i + 1] = x.y; b[4 * i + 2] = x.z; b[4 * i + 3] = x.w;
+        ldg_words<4>(reinterpret_cast<const uint8_t*>(p + at), b + 4 * i);
       }
     }
+  }
+  // bf16 rows to fp16: scaled by a power of two into its range (the return
+  // value undoes it).
+  __device__ static __forceinline__ float convert_q(const AttendArgs& a, uint32_t (&b)[2 * kKWords]) {
     if (!a.bf16) return 1.f;
     float top = 0.f;
 #pragma unroll
@@ -257,7 +289,53 @@ struct Attend {
   __device__ static __forceinline__ void units(const AttendArgs& a, const Segment& s, int from, int to,
                                                float (&o)[NT][D / 16][4], float (&m)[NT][2], float (&l)[NT][2]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const int upb = a.block_size / kUnit;
+    int u = s.unit0 + from;
+    const int end = s.unit0 + to;
+    const int* table = a.table + (long long)s.request * a.table_stride;
+    const int last_block = s.length > 0 ? (s.length - 1) / a.block_size : -1;
+    int next_block = u / upb, next_sub = u - next_block * upb;
+    auto page_of = [&](int b) { return b <= last_block ? ld_int(table + b) : -1; };
+    uint32_t kr[2][kKWords], vr[4][kVWords];
+    float ks, vs;
+    auto load_k = [&](int page, int sub) {
+      const uint8_t* p = a.k + page * a.k_block_stride + s.head * a.k_head_stride + (sub * kUnit + g) * a.k_token_stride;
+      if constexpr (D == 64) {
+        ldg_words<4>(p + c * 16, kr[0]);
+        ldg_words<4>(p + 8 * a.k_token_stride + c * 16, kr[1]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < D / 128; ++i) {
+          ldg_words<8>(p + i * 128 + c * 32, kr[0] + 8 * i);
+          ldg_words<8>(p + 8 * a.k_token_stride + i * 128 + c * 32, kr[1] + 8 * i);
+        }
+      }
+      ks = ld_float(a.k_scale + (long long)page * a.kv_heads + s.head);
+    };
+    auto load_v = [&](int page, int sub) {
+      const uint8_t* p = a.v + page * a.v_block_stride + s.head * a.v_head_stride + (sub * kUnit + 2 * c) * a.v_token_stride + g * (D / 8);
+      ldg_words<kVWords>(p, vr[0]);
+      ldg_words<kVWords>(p + a.v_token_stride, vr[1]);
+      ldg_words<kVWords>(p + 8 * a.v_token_stride, vr[2]);
+      ldg_words<kVWords>(p + 9 * a.v_token_stride, vr[3]);
+      vs = ld_float(a.v_scale + (long long)page * a.kv_heads + s.head);
+    };
+    // The first loads in the order of their latencies: the table's entries and
+    // the queries together, then the first unit; what follows from the rows'
+    // places is worked out while they are on their way.
+    int page = page_of(next_block);
+    int next_page;
+    const int sub0 = next_sub;
+    if (++next_sub == upb) { next_sub = 0; ++next_block; }
+    next_page = page_of(next_block);
     uint32_t qb[NT][2 * kKWords];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) load_q(a, s, n * 8 + g, qb[n]);
+    bool good = (unsigned)page < (unsigned)a.blocks;
+    page = good ? page : 0;
+    load_k(page, sub0);
+    load_v(page, sub0);
+
     float factor[NT][2];
     int low[NT][2], high[NT][2];
     // Tokens that every row sees are [most_low, least_high), those that some
@@ -265,10 +343,8 @@ struct Attend {
     int least_high = 0x7fffffff, most_low = 0, least_low = 0x7fffffff, most_high = 0;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const float up = load_q(a, s, n * 8 + g, qb[n]);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        factor[n][i] = a.scale_log2 * __shfl_sync(0xffffffffu, up, (2 * c + i) * 4);
         int token, head;
         const bool there = row_of(a, s, n * 8 + 2 * c + i, token, head, low[n][i], high[n][i]);
         least_high = min(least_high, there ? high[n][i] : 0x7fffffff);
@@ -287,47 +363,12 @@ struct Attend {
     most_low = __reduce_max_sync(0xffffffffu, most_low);
     least_low = __reduce_min_sync(0xffffffffu, least_low);
     most_high = __reduce_max_sync(0xffffffffu, most_high);
-
-    const int upb = a.block_size / kUnit;
-    int u = s.unit0 + from;
-    const int end = s.unit0 + to;
-    const int* table = a.table + (long long)s.request * a.table_stride;
-    const int last_block = (s.length - 1) / a.block_size;
-    int block = u / upb, sub = u - block * upb;
-    auto page_of = [&](int b) { return b <= last_block && s.length > 0 ? __ldg(table + b) : -1; };
-    uint32_t kr[2][kKWords], vr[4][kVWords];
-    float ks, vs;
-    auto load_k = [&](int page, int sub_) {
-      const uint8_t* p = a.k + page * a.k_block_stride + s.head * a.k_head_stride + (sub_ * kUnit + g) * a.k_token_stride;
-      if constexpr (D == 64) {
-        ldg_words<4>(p + c * 16, kr[0]);
-        ldg_words<4>(p + 8 * a.k_token_stride + c * 16, kr[1]);
-      } else {
 #pragma unroll
-        for (int i = 0; i < D / 128; ++i) {
-          ldg_words<8>(p + i * 128 + c * 32, kr[0] + 8 * i);
-          ldg_words<8>(p + 8 * a.k_token_stride + i * 128 + c * 32, kr[1] + 8 * i);
-        }
-      }
-      ks = __ldg(a.k_scale + (long long)page * a.kv_heads + s.head);
-    };
-    auto load_v = [&](int page, int sub_) {
-      const uint8_t* p = a.v + page * a.v_block_stride + s.head * a.v_head_stride + (sub_ * kUnit + 2 * c) * a.v_token_stride + g * (D / 8);
-      ldg_words<kVWords>(p, vr[0]);
-      ldg_words<kVWords>(p + a.v_token_stride, vr[1]);
-      ldg_words<kVWords>(p + 8 * a.v_token_stride, vr[2]);
-      ldg_words<kVWords>(p + 9 * a.v_token_stride, vr[3]);
-      vs = __ldg(a.v_scale + (long long)page * a.kv_heads + s.head);
-    };
-
-    int page = page_of(block);
-    bool good = (unsigned)page < (unsigned)a.blocks;
-    page = good ? page : 0;
-    load_k(page, sub);
-    load_v(page, sub);
-    int next_block = block, next_sub = sub + 1;
-    if (next_sub == upb) { next_sub = 0; ++next_block; }
-    int next_page = page_of(next_block);
+    for (int n = 0; n < NT; ++n) {
+      const float up = convert_q(a, qb[n]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) factor[n][i] = a.scale_log2 * __shfl_sync(0xffffffffu, up, (2 * c + i) * 4);
+    }
 
     for (; u < end; ++u) {
       const bool more = u + 1 < end;
@@ -454,8 +495,7 @@ struct Attend {
       }
   }
 
-  // One row joined from parts: rows of `count` parts at o[i * stride_o], each
-  // with its m and l; lane has channels lane * (D / 32)...
+  // A row that a warp holds, lane by lane D / 32 channels, to its place.
   __device__ static __forceinline__ void finish_row(const AttendArgs& a, const Segment& s, int row, const float (&x)[D / 32], float m, float l) {
     const int lane = threadIdx.x & 31;
     int token, head, low, high;
@@ -480,13 +520,46 @@ struct Attend {
   }
 
   static constexpr int kPartFloats = kRows * (D + 2);
+  static constexpr int kLane = D / 32;  // channels of a lane where a warp holds a row
 
-  __device__ static __forceinline__ int owner(int u, int grid, int all) {
-    return (int)((((long long)u + 1) * grid - 1) / all);
+  __device__ static __forceinline__ void store_part(float* p, const float (&x)[kLane]) {
+    if constexpr (kLane == 2) {
+      __stcg(reinterpret_cast<float2*>(p), make_float2(x[0], x[1]));
+    } else {
+#pragma unroll
+      for (int d = 0; d < kLane; d += 4) __stcg(reinterpret_cast<float4*>(p + d), make_float4(x[d], x[d + 1], x[d + 2], x[d + 3]));
+    }
+  }
+  __device__ static __forceinline__ void add_part(const float* p, float f, float (&x)[kLane], bool global) {
+    float y[kLane];
+    if constexpr (kLane == 2) {
+      const float2 v = global ? __ldcg(reinterpret_cast<const float2*>(p)) : *reinterpret_cast<const float2*>(p);
+      y[0] = v.x; y[1] = v.y;
+    } else {
+#pragma unroll
+      for (int d = 0; d < kLane; d += 4) {
+        const float4 v = global ? __ldcg(reinterpret_cast<const float4*>(p + d)) : *reinterpret_cast<const float4*>(p + d);
+        y[d] = v.x; y[d + 1] = v.y; y[d + 2] = v.z; y[d + 3] = v.w;
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < kLane; ++d) x[d] = fmaf(y[d], f, x[d]);
+  }
+  __device__ static __forceinline__ float warp_max(float x) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+    return x;
+  }
+  __device__ static __forceinline__ float warp_sum(float x) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+    return x;
   }
 
   __device__ static void run(const AttendArgs& a, Shared& sh, int* prefix) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    pdl_trigger();
+    pdl_wait();
     // Units of every request, summed up: prefix[r] = the first of request r.
     int carry = 0;
     for (int base = 0; base < a.requests; base += W * 32) {
@@ -518,48 +591,55 @@ struct Attend {
     }
     const int all = carry;
     if (all == 0) return;
-    // A CTA has a unit for each of its warps at least.
+    // Every CTA has the same number of units (the last has the rest), one for
+    // each of its warps at least; CTA u / chunk has unit u.
     const int grid = min((int)gridDim.x, (all + W - 1) / W);
+    const int chunk = (all + grid - 1) / grid;
     const int cta = blockIdx.x;
-    if (cta >= grid) return;
-    const int cta0 = (int)((long long)all * cta / grid), cta1 = (int)((long long)all * (cta + 1) / grid);
-    const int u0 = cta0 + (int)((long long)(cta1 - cta0) * warp / W), u1 = cta0 + (int)((long long)(cta1 - cta0) * (warp + 1) / W);
+    if (cta >= grid || cta * chunk >= all) return;
+    const int cta0 = cta * chunk, cta1 = min(all, cta0 + chunk);
+    const int u0 = cta0 + (cta1 - cta0) * warp / W, u1 = cta0 + (cta1 - cta0) * (warp + 1) / W;
     if (lane < 2) sh.used[2 * warp + lane] = 0;
     __syncwarp();
 
-    for (int u = u0; u < u1;) {
-      const Segment s = segment_at(a, prefix, u);
-      const int from = u - s.begin, to = min(s.units, u1 - s.begin);
-      float o[NT][D / 16][4], m[NT][2], l[NT][2];
-      units(a, s, from, to, o, m, l);
-      if (from == 0 && to == s.units) {
-        write_rows(a, s, o, m, l);
-      } else {
-        const int slot = 2 * warp + (u == u0 ? 0 : 1), g = lane >> 2, c = lane & 3;
+    if (u0 < u1) {
+      Segment s = segment_at(a, prefix, u0);
+      for (int u = u0;;) {
+        const int from = u - s.begin, to = min(s.units, u1 - s.begin);
+        float o[NT][D / 16][4], m[NT][2], l[NT][2];
+        units(a, s, from, to, o, m, l);
+        if (from == 0 && to == s.units) {
+          write_rows(a, s, o, m, l);
+        } else {
+          const int slot = 2 * warp + (u == u0 ? 0 : 1), g = lane >> 2, c = lane & 3;
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int row = n * 8 + 2 * c + i;
-            float* p = &sh.o[slot][row][g * (D / 8)];
+            for (int i = 0; i < 2; ++i) {
+              const int row = n * 8 + 2 * c + i;
+              float* p = &sh.o[slot][row][g * (D / 8)];
 #pragma unroll
-            for (int d = 0; d < D / 32; ++d)
-              *reinterpret_cast<float4*>(p + 4 * d) = make_float4(o[n][2 * d][i], o[n][2 * d][i + 2], o[n][2 * d + 1][i], o[n][2 * d + 1][i + 2]);
-            if (g == 0) {
-              sh.m[slot][row] = m[n][i];
-              sh.l[slot][row] = l[n][i];
+              for (int d = 0; d < D / 32; ++d)
+                *reinterpret_cast<float4*>(p + 4 * d) = make_float4(o[n][2 * d][i], o[n][2 * d][i + 2], o[n][2 * d + 1][i], o[n][2 * d + 1][i + 2]);
+              if (g == 0) {
+                sh.m[slot][row] = m[n][i];
+                sh.l[slot][row] = l[n][i];
+              }
             }
+          if (lane == 0) {
+            sh.seg[slot] = s;
+            sh.used[slot] = 1;
           }
-        if (lane == 0) {
-          sh.seg[slot] = s;
-          sh.used[slot] = 1;
         }
+        u = s.begin + to;
+        if (u >= u1) break;
+        s = segment_after(a, prefix, s);
       }
-      u = s.begin + to;
     }
     __syncthreads();
 
-    // Parts of one segment are neighbours among the used slots.
+    // Parts of one segment are neighbours among the used slots: a group.  Each
+    // of its rows is joined by one warp.
     const int used = lane < kSlots ? sh.used[lane] : 0;
     const uint32_t valid = __ballot_sync(0xffffffffu, used);
     if (valid == 0) return;
@@ -567,88 +647,81 @@ struct Attend {
     const uint32_t below = valid & ((1u << lane) - 1u);
     const int prev = __shfl_sync(0xffffffffu, begin, below ? 31 - __clz(below) : 0);
     const uint32_t heads = __ballot_sync(0xffffffffu, used && (below == 0 || prev != begin));
-    const int groups = __popc(heads);
-    bool shared_by_ctas = false;
-    for (int item = warp; item < groups * kRows; item += W) {
-      const int which = item / kRows, row = item - which * kRows;
+    for (int item = warp; item < __popc(heads) * kRows; item += W) {
+      const int row = item % kRows;
       uint32_t h = heads;
-      for (int i = 0; i < which; ++i) h &= h - 1;
+      for (int i = item / kRows; i; --i) h &= h - 1;
       const int first = __ffs(h) - 1;
       h &= h - 1;
       const uint32_t members = valid & ~((1u << first) - 1u) & (h ? (h & -h) - 1u : 0xffffffffu);
-      float top = kFarBelow;
-      for (uint32_t b = members; b; b &= b - 1) top = fmaxf(top, sh.m[__ffs(b) - 1][row]);
-      float x[D / 32], l = 0.f;
+      const bool mine = members >> lane & 1;
+      const float part_m = mine ? sh.m[lane][row] : kFarBelow;
+      const float top = warp_max(part_m);
+      const float f = mine ? exp2_approx(part_m - top) : 0.f;
+      const float l = warp_sum(mine ? f * sh.l[lane][row] : 0.f);
+      float x[kLane];
 #pragma unroll
-      for (int d = 0; d < D / 32; ++d) x[d] = 0.f;
-      for (uint32_t b = members; b; b &= b - 1) {
-        const int slot = __ffs(b) - 1;
-        const float f = exp2_approx(sh.m[slot][row] - top);
-        l = fmaf(sh.l[slot][row], f, l);
-        const float* p = &sh.o[slot][row][lane * (D / 32)];
+      for (int d = 0; d < kLane; ++d) x[d] = 0.f;
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d) x[d] = fmaf(p[d], f, x[d]);
-      }
+      for (int slot = 0; slot < kSlots; ++slot)
+        if (members >> slot & 1) add_part(&sh.o[slot][row][lane * kLane], __shfl_sync(0xffffffffu, f, slot), x, false);
       const Segment& s = sh.seg[first];
       if (s.begin >= cta0 && s.begin + s.units <= cta1) {
         finish_row(a, s, row, x, top, l);
       } else {
-        const int slot = owner(s.begin, grid, all) == cta ? 1 : 0;
-        float* part = a.partials + (long long)(cta * 2 + slot) * kPartFloats;
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d) __stcg(part + row * D + lane * (D / 32) + d, x[d]);
+        float* part = a.partials + (long long)(cta * 2 + (s.begin >= cta0 ? 1 : 0)) * kPartFloats;
+        store_part(part + row * D + lane * kLane, x);
         if (lane == 0) {
           __stcg(part + kRows * D + row, top);
           __stcg(part + kRows * D + kRows + row, l);
         }
       }
     }
-    // Which of the CTA's first and last segments other CTAs share, as every
-    // thread reads it from the slots.
-    int first_slot = __ffs(heads) - 1, last_slot = 31 - __clz(heads);
-    const Segment* ends[2] = {&sh.seg[first_slot], &sh.seg[last_slot]};
-    const int n_ends = first_slot == last_slot ? 1 : 2;
-    for (int e = 0; e < n_ends; ++e) {
-      const Segment& s = *ends[e];
-      shared_by_ctas |= !(s.begin >= cta0 && s.begin + s.units <= cta1);
+    // The CTA's first and last segments may be shared with others: the last CTA
+    // to arrive joins the parts in the order of the CTAs.
+    const int end_slot[2] = {__ffs(heads) - 1, 31 - __clz(heads)};
+    const int ends = end_slot[0] == end_slot[1] ? 1 : 2;
+    bool shared = false;
+    for (int e = 0; e < ends; ++e) {
+      const Segment& s = sh.seg[end_slot[e]];
+      shared |= !(s.begin >= cta0 && s.begin + s.units <= cta1);
     }
-    if (!shared_by_ctas) return;
-    __threadfence();
+    if (!shared) return;
     __syncthreads();
-    if (tid < n_ends) {
-      const Segment& s = *ends[tid];
+    if (tid < ends) {
+      const Segment& s = sh.seg[tid ? end_slot[1] : end_slot[0]];
       int last = 0;
       if (!(s.begin >= cta0 && s.begin + s.units <= cta1)) {
-        const int c0 = owner(s.begin, grid, all), c1 = owner(s.begin + s.units - 1, grid, all);
+        const int c0 = s.begin / chunk, c1 = (s.begin + s.units - 1) / chunk;
+        __threadfence();  // with the barrier: the whole CTA's parts before the count
         last = atomicAdd(a.counters + c0, 1) == c1 - c0;
         if (last) a.counters[c0] = 0;
+        __threadfence();
       }
       sh.last[tid] = last;
-      __threadfence();
     }
     __syncthreads();
-    for (int e = 0; e < n_ends; ++e) {
+    for (int e = 0; e < ends; ++e) {
       if (!sh.last[e]) continue;
-      const Segment& s = *ends[e];
-      const int c0 = owner(s.begin, grid, all), c1 = owner(s.begin + s.units - 1, grid, all);
+      const Segment& s = sh.seg[end_slot[e]];
+      const int c0 = s.begin / chunk, c1 = (s.begin + s.units - 1) / chunk;
+      auto part = [&](int c) { return a.partials + (long long)(c * 2 + (c == c0 ? 1 : 0)) * kPartFloats; };
       for (int row = warp; row < kRows; row += W) {
-        auto part = [&](int c) { return a.partials + (long long)(c * 2 + (c == c0 ? 1 : 0)) * kPartFloats; };
         float top = kFarBelow;
         for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, __ldcg(part(c) + kRows * D + row));
+        top = warp_max(top);
+        float x[kLane], l = 0.f;
 #pragma unroll
-        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        float x[D / 32], l = 0.f;
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d) x[d] = 0.f;
-#pragma unroll 4
-        for (int c = c0; c <= c1; ++c) {
-          const float* p = part(c);
-          const float f = exp2_approx(__ldcg(p + kRows * D + row) - top);
-          l = fmaf(__ldcg(p + kRows * D + kRows + row), f, l);
-#pragma unroll
-          for (int d = 0; d < D / 32; ++d) x[d] = fmaf(__ldcg(p + row * D + lane * (D / 32) + d), f, x[d]);
+        for (int d = 0; d < kLane; ++d) x[d] = 0.f;
+        for (int base = c0; base <= c1; base += 32) {
+          const int c = base + lane;
+          const float f = c <= c1 ? exp2_approx(__ldcg(part(c) + kRows * D + row) - top) : 0.f;
+          l += c <= c1 ? f * __ldcg(part(c) + kRows * D + kRows + row) : 0.f;
+          const int n = min(32, c1 - base + 1);
+#pragma unroll 8
+          for (int j = 0; j < n; ++j) add_part(part(base + j) + row * D + lane * kLane, __shfl_sync(0xffffffffu, f, j), x, true);
         }
-        finish_row(a, s, row, x, top, l);
+        finish_row(a, s, row, x, top, warp_sum(l));
       }
     }
   }
@@ -711,8 +784,11 @@ dk_status launch(AttendArgs a, cudaStream_t stream) {
       a.lse = lse ? lse + (long long)r * a.kv_heads * a.group : nullptr;
       a.tokens = tokens - r;
     }
-    kernel<<<sm_count(device) * MINB, W * 32, smem, stream>>>(a);
-    const dk_status s = check_launch("dk_cache_attention");
+    // No more CTAs than the table's width can keep busy.
+    const long long most = (((long long)a.max_blocks * a.block_size + kUnit - 1) / kUnit) * a.kv_heads *
+                           (starts ? (long long)a.requests + (long long)tokens * a.group / A::kRows : (long long)a.requests * ((a.group + A::kRows - 1) / A::kRows));
+    const int grid = (int)std::min<long long>(sm_count(device) * MINB, (most + W - 1) / W);
+    const dk_status s = launch_early("dk_cache_attention", kernel, dim3(grid), dim3(W * 32), smem, stream, a);
     if (s != DK_OK) return s;
   }
   return DK_OK;
@@ -768,7 +844,7 @@ extern "C" dk_status dk_cache_attention(const dk_cache_attention_args* p, void* 
   const int group = p->q_heads / c.kv_heads;
   const long long units = ((long long)p->max_blocks * c.block_size + 15) / 16;
   const long long per_head = (long long)std::min(p->requests, kMaxRequests) + (long long)p->tokens * group / 8;
-  if (units > INT32_MAX / 16 || per_head > INT32_MAX / units / c.kv_heads) return DK_ERR_UNSUPPORTED;
+  if (units > INT32_MAX / 16 || per_head > INT32_MAX / 2 / units / c.kv_heads) return DK_ERR_UNSUPPORTED;
   const size_t need = dk_cache_attention_workspace_bytes(c.head_dim);
   if (!workspace || workspace_bytes < need || !aligned(workspace, 256)) return DK_ERR_WORKSPACE;
 
