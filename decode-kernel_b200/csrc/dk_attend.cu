@@ -70,6 +70,7 @@ struct AttendArgs {
   long long v_block_stride, v_head_stride, v_token_stride;
   int table_stride, max_blocks, blocks, block_size;
   int requests, tokens, kv_heads, group;
+  unsigned group_magic;  // ceil(2^32 / group), 0 for a group of 1
   float scale_log2;
   int causal, window, bf16;
 };
@@ -225,7 +226,8 @@ struct Attend {
   // place in q and out; false where the tile has no such row.
   __device__ static __forceinline__ bool row_of(const AttendArgs& a, const Segment& s, int row, int& token, int& head, int& low, int& high) {
     const int all = s.tile * kRows + row;
-    const int i = s.fresh == 1 ? (all >= a.group) : all / a.group;
+    int i = a.group == 1 ? all : __umulhi(all, a.group_magic);  // all / group, or one more
+    i -= i * a.group > all;
     token = s.first_token + i;
     head = s.head * a.group + all - i * a.group;
     low = high = 0;
@@ -359,10 +361,15 @@ struct Attend {
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[n][i][j] = 0.f;
     }
-    least_high = __reduce_min_sync(0xffffffffu, least_high);
-    most_low = __reduce_max_sync(0xffffffffu, most_low);
-    least_low = __reduce_min_sync(0xffffffffu, least_low);
-    most_high = __reduce_max_sync(0xffffffffu, most_high);
+    if (s.fresh == 1) {  // all rows are one query's
+      least_high = most_high = s.length;
+      least_low = most_low = a.window > 0 ? max(0, s.length - a.window) : 0;
+    } else {
+      least_high = __reduce_min_sync(0xffffffffu, least_high);
+      most_low = __reduce_max_sync(0xffffffffu, most_low);
+      least_low = __reduce_min_sync(0xffffffffu, least_low);
+      most_high = __reduce_max_sync(0xffffffffu, most_high);
+    }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const float up = convert_q(a, qb[n]);
@@ -530,18 +537,20 @@ struct Attend {
       for (int d = 0; d < kLane; d += 4) __stcg(reinterpret_cast<float4*>(p + d), make_float4(x[d], x[d + 1], x[d + 2], x[d + 3]));
     }
   }
-  __device__ static __forceinline__ void add_part(const float* p, float f, float (&x)[kLane], bool global) {
-    float y[kLane];
+  template <bool GLOBAL>
+  __device__ static __forceinline__ void load_part(const float* p, float (&y)[kLane]) {
     if constexpr (kLane == 2) {
-      const float2 v = global ? __ldcg(reinterpret_cast<const float2*>(p)) : *reinterpret_cast<const float2*>(p);
+      const float2 v = GLOBAL ? __ldcg(reinterpret_cast<const float2*>(p)) : *reinterpret_cast<const float2*>(p);
       y[0] = v.x; y[1] = v.y;
     } else {
 #pragma unroll
       for (int d = 0; d < kLane; d += 4) {
-        const float4 v = global ? __ldcg(reinterpret_cast<const float4*>(p + d)) : *reinterpret_cast<const float4*>(p + d);
+        const float4 v = GLOBAL ? __ldcg(reinterpret_cast<const float4*>(p + d)) : *reinterpret_cast<const float4*>(p + d);
         y[d] = v.x; y[d + 1] = v.y; y[d + 2] = v.z; y[d + 3] = v.w;
       }
     }
+  }
+  __device__ static __forceinline__ void add_part(const float (&y)[kLane], float f, float (&x)[kLane]) {
 #pragma unroll
     for (int d = 0; d < kLane; ++d) x[d] = fmaf(y[d], f, x[d]);
   }
@@ -662,9 +671,15 @@ struct Attend {
       float x[kLane];
 #pragma unroll
       for (int d = 0; d < kLane; ++d) x[d] = 0.f;
-#pragma unroll
-      for (int slot = 0; slot < kSlots; ++slot)
-        if (members >> slot & 1) add_part(&sh.o[slot][row][lane * kLane], __shfl_sync(0xffffffffu, f, slot), x, false);
+      // Few instructions: this code runs once a call, and fetching it costs
+      // more than running it.
+#pragma unroll 1
+      for (uint32_t left = members; left; left &= left - 1) {
+        const int slot = __ffs(left) - 1;
+        float y[kLane];
+        load_part<false>(&sh.o[slot][row][lane * kLane], y);
+        add_part(y, __shfl_sync(0xffffffffu, f, slot), x);
+      }
       const Segment& s = sh.seg[first];
       if (s.begin >= cta0 && s.begin + s.units <= cta1) {
         finish_row(a, s, row, x, top, l);
@@ -693,10 +708,12 @@ struct Attend {
       int last = 0;
       if (!(s.begin >= cta0 && s.begin + s.units <= cta1)) {
         const int c0 = s.begin / chunk, c1 = (s.begin + s.units - 1) / chunk;
-        __threadfence();  // with the barrier: the whole CTA's parts before the count
-        last = atomicAdd(a.counters + c0, 1) == c1 - c0;
+        // With the barrier: the whole CTA's parts are seen before the count,
+        // and the others' parts by the CTA that counts last.
+        int before;
+        asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(a.counters + c0) : "memory");
+        last = before == c1 - c0;
         if (last) a.counters[c0] = 0;
-        __threadfence();
       }
       sh.last[tid] = last;
     }
@@ -706,23 +723,52 @@ struct Attend {
       const Segment& s = sh.seg[end_slot[e]];
       const int c0 = s.begin / chunk, c1 = (s.begin + s.units - 1) / chunk;
       auto part = [&](int c) { return a.partials + (long long)(c * 2 + (c == c0 ? 1 : 0)) * kPartFloats; };
-      for (int row = warp; row < kRows; row += W) {
-        float top = kFarBelow;
-        for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, __ldcg(part(c) + kRows * D + row));
-        top = warp_max(top);
-        float x[kLane], l = 0.f;
+      // A warp's rows go together and several parts at a time, so that their
+      // loads overlap: the parts are in L2, a latency away.
+      constexpr int R = kRows / W, U = 8 / R;
+      float x[R][kLane], l[R], m[R];
 #pragma unroll
-        for (int d = 0; d < kLane; ++d) x[d] = 0.f;
-        for (int base = c0; base <= c1; base += 32) {
-          const int c = base + lane;
-          const float f = c <= c1 ? exp2_approx(__ldcg(part(c) + kRows * D + row) - top) : 0.f;
-          l += c <= c1 ? f * __ldcg(part(c) + kRows * D + kRows + row) : 0.f;
-          const int n = min(32, c1 - base + 1);
-#pragma unroll 8
-          for (int j = 0; j < n; ++j) add_part(part(base + j) + row * D + lane * kLane, __shfl_sync(0xffffffffu, f, j), x, true);
-        }
-        finish_row(a, s, row, x, top, warp_sum(l));
+      for (int i = 0; i < R; ++i) {
+        m[i] = kFarBelow;
+        l[i] = 0.f;
+#pragma unroll
+        for (int d = 0; d < kLane; ++d) x[i][d] = 0.f;
       }
+#pragma unroll 1
+      for (int base = c0; base <= c1; base += 32) {
+        const int c = base + lane;
+        const float* mine = part(min(c, c1)) + kRows * D + warp * R;
+        float f[R];
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          const float part_m = __ldcg(mine + i), part_l = __ldcg(mine + kRows + i);
+          const float top = fmaxf(m[i], warp_max(part_m));
+          const float scale = exp2_approx(m[i] - top);
+          m[i] = top;
+          f[i] = exp2_approx(part_m - top);
+          l[i] = l[i] * scale + (c <= c1 ? f[i] * part_l : 0.f);
+#pragma unroll
+          for (int d = 0; d < kLane; ++d) x[i][d] *= scale;
+        }
+        const int n = min(32, c1 - base + 1);
+#pragma unroll 1
+        for (int j = 0; j < n; j += U) {
+          float y[U][R][kLane];
+#pragma unroll
+          for (int k = 0; k < U; ++k)
+#pragma unroll
+            for (int i = 0; i < R; ++i) load_part<true>(part(min(base + j + k, c1)) + (warp * R + i) * D + lane * kLane, y[k][i]);
+#pragma unroll
+          for (int k = 0; k < U; ++k)
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+              const float g = __shfl_sync(0xffffffffu, f[i], j + k);
+              add_part(y[k][i], j + k < n ? g : 0.f, x[i]);
+            }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < R; ++i) finish_row(a, s, warp * R + i, x[i], m[i], warp_sum(l[i]));
     }
   }
 };
@@ -878,6 +924,7 @@ extern "C" dk_status dk_cache_attention(const dk_cache_attention_args* p, void* 
   a.tokens = p->tokens;
   a.kv_heads = c.kv_heads;
   a.group = group;
+  a.group_magic = group > 1 ? (unsigned)(((1ull << 32) + group - 1) / group) : 0u;
   a.scale_log2 = p->scale * 1.4426950408889634f;
   a.causal = p->causal;
   a.window = p->window;
