@@ -47,7 +47,7 @@ namespace dk {
 namespace {
 
 constexpr int kUnit = 16;             // tokens of a unit
-constexpr int kMaxRequests = 8192;    // requests of one launch (their prefix sums are in shared memory)
+constexpr int kMaxRequests = 2048;    // requests of one launch (their prefix sums are in shared memory)
 constexpr float kFarBelow = -1e30f;   // maximum of a row that has seen no token
 constexpr float kSlack = 8.f;         // a row's maximum may lag its scores by this much (log2)
 constexpr float kLeastScale = 8.4703294725430034e-22f;  // 2^-70: keeps sum w / vs finite
@@ -65,6 +65,7 @@ struct AttendArgs {
   float* lse;
   int* counters;
   float* partials;
+  float* early;
   long long q_token_stride, q_head_stride;
   long long k_block_stride, k_head_stride, k_token_stride;
   long long v_block_stride, v_head_stride, v_token_stride;
@@ -123,22 +124,31 @@ __device__ __forceinline__ float ld_float(const float* p) {
   return x;
 }
 
+__device__ __forceinline__ uint4 ld_quad(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+  return r;
+}
+
+// Asynchronous copies into shared memory: 16 bytes past L1, or 4.
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
+}
+
 template <int WORDS>
-__device__ __forceinline__ void ldg_words(const uint8_t* p, uint32_t* r) {
-  static_assert(WORDS == 2 || WORDS == 4 || WORDS == 8, "");
-  if constexpr (WORDS == 8) {
-    asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
-                   "=r"(r[6]), "=r"(r[7])
-                 : "l"(p));
-  } else if constexpr (WORDS == 4) {
-    asm volatile("ld.global.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "l"(p));
+__device__ __forceinline__ void lds_words(uint32_t at, uint32_t* r) {
+  if constexpr (WORDS == 4) {
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
   } else {
-    asm volatile("ld.global.L1::no_allocate.v2.b32 {%0,%1}, [%2];"
-                 : "=r"(r[0]), "=r"(r[1])
-                 : "l"(p));
+    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(at));
   }
 }
 
@@ -151,16 +161,18 @@ struct Segment {
   int begin;                       // its first unit in the line of all units
 };
 
-template <int D, int NT, bool E4M3, int W>
+template <int D, int NT, bool E4M3, int W, int S>
 struct Attend {
   static constexpr int kRows = 8 * NT;
   static constexpr int kKWords = D / 16;  // words of a lane's part of a K row
   static constexpr int kVWords = D / 32;  // words of a lane's part of a V row
-  static constexpr int kPitch = D + 4;    // floats between rows of a part in shared memory
-  static constexpr int kSlots = 2 * W;
+  static constexpr int kSlots = 2 * W;    // a warp's parts of segments: an early one and its last
+  static constexpr int kStage = 2 * kUnit * D;  // bytes of a unit
+  static_assert(kRows * D * 4 <= S * kStage, "a part fits the warp's ring");
 
   struct Shared {
-    float o[kSlots][kRows][kPitch];
+    unsigned char ring[W][S][kStage];  // at the end the warp's last part: float [kRows][D]
+    float4 meta[W][S];                 // of a stage: K scale, V scale, whether its page is in the pool
     float m[kSlots][kRows];
     float l[kSlots][kRows];
     Segment seg[kSlots];
@@ -168,6 +180,20 @@ struct Attend {
     int last[2];
     int total[W];
   };
+
+  // Place of 16-byte piece p of a unit's row: the pieces that eight lanes read
+  // together, of K (two rows) and of V (four rows two apart), lie in different
+  // banks.
+  __device__ static __forceinline__ int place(int row, int p) {
+    if constexpr (D == 64) {
+      const int line = row >> 1;
+      return line * 128 + (((row & 1) * 4 + p) ^ ((line & 3) * 2)) * 16;
+    } else if constexpr (D == 128) {
+      return row * D + (p ^ (row & 7)) * 16;
+    } else {
+      return row * D + (p ^ (((row ^ (row >> 1)) & 1) | (row & 4))) * 16;
+    }
+  }
 
   __device__ static __forceinline__ int units_of(const AttendArgs& a, int length, int fresh, int& unit0) {
     unit0 = 0;
@@ -213,13 +239,14 @@ struct Attend {
     const int which = (u - s.begin) / s.units;
     return which ? segment_of(a, prefix, lo, which) : s;
   }
-  // The segment after s.
-  __device__ static __forceinline__ Segment segment_after(const AttendArgs& a, const int* prefix, const Segment& s) {
-    if (s.which + 1 < s.all) return segment_of(a, prefix, s.request, s.which + 1);
-    int r = s.request + 1;  // some request after it has units
-    const int u = s.begin + s.units;
-    while (r + 1 < a.requests && prefix[r + 1] <= u) ++r;
-    return segment_of(a, prefix, r, 0);
+  // The segment after segment `which` of request r, which ends before unit u.
+  __device__ static __forceinline__ void after(const AttendArgs& a, const int* prefix, int r, int which, int u, int& next_r, int& next_which) {
+    next_r = r;
+    next_which = which + 1;
+    if (u < prefix[r + 1]) return;
+    next_which = 0;
+    ++next_r;  // some request after r has units
+    while (next_r + 1 < a.requests && prefix[next_r + 1] <= u) ++next_r;
   }
 
   // Token range [low, high) that query row `row` of the segment sees, and its
@@ -251,7 +278,8 @@ struct Attend {
 #pragma unroll
       for (int i = 0; i < kKWords / 2; ++i) {  // 8 channels each
         const int at = (i * 8) % kSpan + (i * 8) / kSpan * 128;
-        ldg_words<4>(reinterpret_cast<const uint8_t*>(p + at), b + 4 * i);
+        const uint4 x = ld_quad(p + at);
+        b[4 * i] = x.x; b[4 * i + 1] = x.y; b[4 * i + 2] = x.z; b[4 * i + 3] = x.w;
       }
     }
   }
@@ -287,200 +315,272 @@ struct Attend {
     *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) = w;
   }
 
-  // Units [from, to) of segment s by one warp.
-  __device__ static __forceinline__ void units(const AttendArgs& a, const Segment& s, int from, int to,
-                                               float (&o)[NT][D / 16][4], float (&m)[NT][2], float (&l)[NT][2]) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const int upb = a.block_size / kUnit;
-    int u = s.unit0 + from;
-    const int end = s.unit0 + to;
-    const int* table = a.table + (long long)s.request * a.table_stride;
-    const int last_block = s.length > 0 ? (s.length - 1) / a.block_size : -1;
-    int next_block = u / upb, next_sub = u - next_block * upb;
-    auto page_of = [&](int b) { return b <= last_block ? ld_int(table + b) : -1; };
-    uint32_t kr[2][kKWords], vr[4][kVWords];
-    float ks, vs;
-    auto load_k = [&](int page, int sub) {
-      const uint8_t* p = a.k + page * a.k_block_stride + s.head * a.k_head_stride + (sub * kUnit + g) * a.k_token_stride;
-      if constexpr (D == 64) {
-        ldg_words<4>(p + c * 16, kr[0]);
-        ldg_words<4>(p + 8 * a.k_token_stride + c * 16, kr[1]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < D / 128; ++i) {
-          ldg_words<8>(p + i * 128 + c * 32, kr[0] + 8 * i);
-          ldg_words<8>(p + 8 * a.k_token_stride + i * 128 + c * 32, kr[1] + 8 * i);
-        }
-      }
-      ks = ld_float(a.k_scale + (long long)page * a.kv_heads + s.head);
-    };
-    auto load_v = [&](int page, int sub) {
-      const uint8_t* p = a.v + page * a.v_block_stride + s.head * a.v_head_stride + (sub * kUnit + 2 * c) * a.v_token_stride + g * (D / 8);
-      ldg_words<kVWords>(p, vr[0]);
-      ldg_words<kVWords>(p + a.v_token_stride, vr[1]);
-      ldg_words<kVWords>(p + 8 * a.v_token_stride, vr[2]);
-      ldg_words<kVWords>(p + 9 * a.v_token_stride, vr[3]);
-      vs = ld_float(a.v_scale + (long long)page * a.kv_heads + s.head);
-    };
-    // The first loads in the order of their latencies: the table's entries and
-    // the queries together, then the first unit; what follows from the rows'
-    // places is worked out while they are on their way.
-    int page = page_of(next_block);
-    int next_page;
-    const int sub0 = next_sub;
-    if (++next_sub == upb) { next_sub = 0; ++next_block; }
-    next_page = page_of(next_block);
-    uint32_t qb[NT][2 * kKWords];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) load_q(a, s, n * 8 + g, qb[n]);
-    bool good = (unsigned)page < (unsigned)a.blocks;
-    page = good ? page : 0;
-    load_k(page, sub0);
-    load_v(page, sub0);
+  // The warp's copies: its units in their order, across segments, each into
+  // the next stage of its ring.
+  struct Feed {
+    const uint8_t* k;
+    const uint8_t* v;
+    const int* table;
+    int unit, end, segment_end;  // next unit in the line, the warp's end, the segment's
+    int request, which, head;
+    int block, sub, last_block, page, next_page;
+    int stage;
 
-    float factor[NT][2];
+    __device__ __forceinline__ int page_at(int b) const { return b <= last_block ? ld_int(table + b) : -1; }
+
+    // From here units of segment s.
+    __device__ __forceinline__ void enter(const AttendArgs& a, const Segment& s) {
+      const int lane = threadIdx.x & 31;
+      constexpr int kPieces = D / 16;
+      const int row = lane / kPieces, piece = lane % kPieces;
+      request = s.request;
+      which = s.which;
+      head = s.head;
+      segment_end = s.begin + s.units;
+      k = a.k + s.head * a.k_head_stride + row * a.k_token_stride + piece * 16;
+      v = a.v + s.head * a.v_head_stride + row * a.v_token_stride + piece * 16;
+      table = a.table + (long long)s.request * a.table_stride;
+      last_block = s.length > 0 ? (s.length - 1) / a.block_size : -1;
+      const int u = s.unit0 + unit - s.begin, upb = a.block_size / kUnit;
+      block = u / upb;
+      sub = u - block * upb;
+      page = page_at(block);
+      next_page = page_at(block + 1);
+    }
+
+    // Copies the next unit, if there is one; always one group.
+    __device__ __forceinline__ void next(const AttendArgs& a, const int* prefix, uint32_t ring, uint32_t meta) {
+      if (unit < end) {
+        if (unit == segment_end) {
+          int r, w;
+          after(a, prefix, request, which, segment_end, r, w);
+          enter(a, segment_of(a, prefix, r, w));
+        }
+        const int lane = threadIdx.x & 31;
+        constexpr int kStep = 512 / D;  // rows of a warp's copy
+        const bool good = (unsigned)page < (unsigned)a.blocks;
+        const long long p = good ? page : 0;
+        const uint8_t* from_k = k + p * a.k_block_stride + (long long)(sub * kUnit) * a.k_token_stride;
+        const uint8_t* from_v = v + p * a.v_block_stride + (long long)(sub * kUnit) * a.v_token_stride;
+        const uint32_t to = ring + stage * kStage;
+        const int row = lane / (D / 16), piece = lane % (D / 16);
+#pragma unroll
+        for (int j = 0; j < kUnit / kStep; ++j) copy16(to + place(row + j * kStep, piece), from_k + (long long)(j * kStep) * a.k_token_stride);
+#pragma unroll
+        for (int j = 0; j < kUnit / kStep; ++j)
+          copy16(to + kUnit * D + place(row + j * kStep, piece), from_v + (long long)(j * kStep) * a.v_token_stride);
+        const uint32_t about = meta + stage * 16;
+        if (lane < 2) copy4(about + lane * 4, (lane ? a.v_scale : a.k_scale) + p * a.kv_heads + head);
+        if (lane == 2) asm volatile("st.shared.b32 [%0], %1;" ::"r"(about + 8), "r"((int)good) : "memory");
+        ++unit;
+        if (++sub == a.block_size / kUnit) {
+          sub = 0;
+          ++block;
+          page = next_page;
+          next_page = page_at(block + 1);
+        }
+        if (++stage == S) stage = 0;
+      }
+      copy_commit();
+    }
+  };
+
+  // A warp's running sums over the units of one segment.
+  struct Rows {
+    uint32_t q[NT][2 * kKWords];
+    float o[NT][D / 16][4], m[NT][2], l[NT][2], factor[NT][2];
     int low[NT][2], high[NT][2];
     // Tokens that every row sees are [most_low, least_high), those that some
     // row sees are within [least_low, most_high).
-    int least_high = 0x7fffffff, most_low = 0, least_low = 0x7fffffff, most_high = 0;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        int token, head;
-        const bool there = row_of(a, s, n * 8 + 2 * c + i, token, head, low[n][i], high[n][i]);
-        least_high = min(least_high, there ? high[n][i] : 0x7fffffff);
-        least_low = min(least_low, there ? low[n][i] : 0x7fffffff);
-        most_low = max(most_low, low[n][i]);
-        most_high = max(most_high, high[n][i]);
-        m[n][i] = kFarBelow;
-        l[n][i] = 0.f;
-      }
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[n][i][j] = 0.f;
-    }
-    if (s.fresh == 1) {  // all rows are one query's
-      least_high = most_high = s.length;
-      least_low = most_low = a.window > 0 ? max(0, s.length - a.window) : 0;
-    } else {
-      least_high = __reduce_min_sync(0xffffffffu, least_high);
-      most_low = __reduce_max_sync(0xffffffffu, most_low);
-      least_low = __reduce_min_sync(0xffffffffu, least_low);
-      most_high = __reduce_max_sync(0xffffffffu, most_high);
-    }
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const float up = convert_q(a, qb[n]);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) factor[n][i] = a.scale_log2 * __shfl_sync(0xffffffffu, up, (2 * c + i) * 4);
-    }
+    int least_high, most_low, least_low, most_high;
+    uint32_t unseen;  // rows (bits) of this lane's columns without a token yet, whose m is 0
+    bool settled;     // no lane has any
 
-    for (; u < end; ++u) {
-      const bool more = u + 1 < end;
-      // Scores of the unit: [16 tokens][8 rows] for each tile of rows.
-      float sc[NT][4];
+    __device__ __forceinline__ void begin(const AttendArgs& a, const Segment& s) {
+      const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
-#pragma unroll
-      for (int w = 0; w < kKWords; ++w) {
-        uint32_t a0, a1, a2, a3;
-        codes_to_half<E4M3>(kr[0][w], a0, a2);
-        codes_to_half<E4M3>(kr[1][w], a1, a3);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) mma16816(sc[n], a0, a1, a2, a3, qb[n][2 * w], qb[n][2 * w + 1]);
-      }
-      const bool good_now = good;
-      const float k_now = ks, v_now = good_now ? (vs < kLeastScale ? kLeastScale : vs) : 1.f;
-      const int page_now = next_page, sub_now = next_sub;
-      if (more) {
-        good = (unsigned)page_now < (unsigned)a.blocks;
-        page = good ? page_now : 0;
-        load_k(page, sub_now);
-        if (++next_sub == upb) { next_sub = 0; ++next_block; }
-        next_page = page_of(next_block);
-      }
-      const float v_log2 = __log2f(v_now), v_inverse = __frcp_rn(v_now);
-      const int base = u * kUnit;
-      const bool edge = base + kUnit > least_high || base < most_low || !good_now;  // the same in all lanes
-      bool grow = false;
+      for (int n = 0; n < NT; ++n) load_q(a, s, n * 8 + g, q[n]);
+      least_high = least_low = 0x7fffffff;
+      most_low = most_high = 0;
+      unseen = (1u << (2 * NT)) - 1u;
+      settled = false;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float t = fmaf(sc[n][i], factor[n][i & 1] * k_now, v_log2);
-          if (edge) {
-            const int at = base + g + (i >> 1) * 8;
-            if (at >= high[n][i & 1] || at < low[n][i & 1] || !good_now) t = -INFINITY;
-          }
-          sc[n][i] = t;
+        for (int i = 0; i < 2; ++i) {
+          int token, head;
+          const bool there = row_of(a, s, n * 8 + 2 * c + i, token, head, low[n][i], high[n][i]);
+          least_high = min(least_high, there ? high[n][i] : 0x7fffffff);
+          least_low = min(least_low, there ? low[n][i] : 0x7fffffff);
+          most_low = max(most_low, low[n][i]);
+          most_high = max(most_high, high[n][i]);
+          m[n][i] = 0.f;
+          l[n][i] = 0.f;
         }
-        grow |= fmaxf(sc[n][0], sc[n][2]) > m[n][0] + kSlack || fmaxf(sc[n][1], sc[n][3]) > m[n][1] + kSlack;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[n][i][j] = 0.f;
       }
-      if (__any_sync(0xffffffffu, grow)) {
+      if (s.fresh == 1) {  // all rows are one query's
+        least_high = most_high = s.length;
+        least_low = most_low = a.window > 0 ? max(0, s.length - a.window) : 0;
+      } else {
+        least_high = __reduce_min_sync(0xffffffffu, least_high);
+        most_low = __reduce_max_sync(0xffffffffu, most_low);
+        least_low = __reduce_min_sync(0xffffffffu, least_low);
+        most_high = __reduce_max_sync(0xffffffffu, most_high);
+      }
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
+      for (int n = 0; n < NT; ++n) {
+        const float up = convert_q(a, q[n]);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float top = fmaxf(sc[n][i], sc[n][i + 2]);
+        for (int i = 0; i < 2; ++i) factor[n][i] = a.scale_log2 * __shfl_sync(0xffffffffu, up, (2 * c + i) * 4);
+      }
+    }
+
+    // Rescales to the columns' new maxima; sc holds scores less m.
+    __device__ __forceinline__ void grow(float (&sc)[NT][4]) {
 #pragma unroll
-            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-            top = fmaxf(top, m[n][i]);
-            const float f = exp2_approx(m[n][i] - top);
-            m[n][i] = top;
-            l[n][i] *= f;
+      for (int n = 0; n < NT; ++n) {
 #pragma unroll
-            for (int d = 0; d < D / 16; ++d) {
-              o[n][d][i] *= f;
-              o[n][d][i + 2] *= f;
-            }
+        for (int i = 0; i < 2; ++i) {
+          float top = fmaxf(sc[n][i], sc[n][i + 2]);
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+          const uint32_t bit = 1u << (2 * n + i);
+          float by = fmaxf(top, 0.f), f = exp2_approx(-by);
+          if (unseen & bit) {  // its sums are zeros
+            const bool some = top > -INFINITY;
+            by = some ? top : 0.f;
+            f = 0.f;
+            if (some) unseen &= ~bit;
+          }
+          m[n][i] += by;
+          sc[n][i] -= by;
+          sc[n][i + 2] -= by;
+          l[n][i] *= f;
+#pragma unroll
+          for (int d = 0; d < D / 16; ++d) {
+            o[n][d][i] *= f;
+            o[n][d][i + 2] *= f;
           }
         }
       }
+      settled = !__any_sync(0xffffffffu, unseen);
+    }
+
+    // The unit of tokens base.. in the stage at `at`.
+    __device__ __forceinline__ void add(int base, uint32_t at, uint32_t about) {
+      const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+      float k_scale, v_scale;
+      int good;
+      asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(k_scale), "=f"(v_scale) : "r"(about));
+      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(good) : "r"(about + 8));
+      // Scores: [16 tokens][8 rows] for each tile of rows, in two chains.
+      float sc[NT][4], sd[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[n][i] = sd[n][i] = 0.f;
+#pragma unroll
+      for (int part = 0; part < kKWords / 4; ++part) {
+        uint32_t k0[4], k1[4];
+        const int piece = D == 64 ? c : 2 * c + (part & 1) + (part >> 1) * 8;
+        lds_words<4>(at + place(g, piece), k0);
+        lds_words<4>(at + place(g, piece) + 8 * D, k1);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t a0, a1, a2, a3;
+          codes_to_half<E4M3>(k0[w], a0, a2);
+          codes_to_half<E4M3>(k1[w], a1, a3);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma16816(w & 1 ? sd[n] : sc[n], a0, a1, a2, a3, q[n][8 * part + 2 * w], q[n][8 * part + 2 * w + 1]);
+        }
+      }
+      const float v_now = v_scale < kLeastScale ? kLeastScale : v_scale;
+      float v_log2, v_inverse;
+      asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(v_log2) : "f"(v_now));
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(v_inverse) : "f"(v_now));
+      bool above = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[n][i] = fmaf(sc[n][i] + sd[n][i], factor[n][i & 1] * k_scale, v_log2 - m[n][i & 1]);
+      }
+      const bool edge = base + kUnit > least_high || base < most_low || !good;  // the same in all lanes
+      if (edge) {
+        if (!good) v_inverse = 0.f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int t = base + g + (i >> 1) * 8;
+            if (t >= high[n][i & 1] || t < low[n][i & 1] || !good) sc[n][i] = -INFINITY;
+          }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) above |= fmaxf(fmaxf(sc[n][0], sc[n][2]), fmaxf(sc[n][1], sc[n][3])) > kSlack;
+      if (__any_sync(0xffffffffu, above) || !settled) grow(sc);
       uint32_t pb[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = exp2_approx(sc[n][i] - m[n][i & 1]);
+        for (int i = 0; i < 4; ++i) w[i] = exp2_approx(sc[n][i]);
         l[n][0] = fmaf(w[0] + w[2], v_inverse, l[n][0]);
         l[n][1] = fmaf(w[1] + w[3], v_inverse, l[n][1]);
         pb[n][0] = transpose8x8(pack_half2(w[0], w[1]));
         pb[n][1] = transpose8x8(pack_half2(w[2], w[3]));
       }
-      if (edge) {  // bytes of tokens that no row sees may be anything, e4m3's NaN too
-        const int past = good_now ? most_high - base : 0, before = least_low - base;
+      const uint32_t at_v = at + kUnit * D;
+      constexpr int kPart = kVWords < 4 ? kVWords : 4;  // words of a load
+#pragma unroll
+      for (int part = 0; part < kVWords / kPart; ++part) {
+        uint32_t v[4][kPart];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int at = 2 * c + (j & 1) + (j >> 1) * 8;
-          if (at >= past || at < before)
+          const int row = 2 * c + (j & 1);
+          const uint32_t from = D == 64 ? place(row, g >> 1) + (g & 1) * 8 : place(row, D == 128 ? g : 2 * g + part);
+          lds_words<kPart>(at_v + from + (j >> 1) * 8 * D, v[j]);
+        }
+        if (edge) {  // bytes of tokens that no row sees may be anything, e4m3's NaN too
+          const int past = good ? most_high - base : 0, before = least_low - base;
 #pragma unroll
-            for (int w = 0; w < kVWords; ++w) vr[j][w] = 0u;
+          for (int j = 0; j < 4; ++j) {
+            const int t = 2 * c + (j & 1) + (j >> 1) * 8;
+            if (t >= past || t < before)
+#pragma unroll
+              for (int w = 0; w < kPart; ++w) v[j][w] = 0u;
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < kPart; ++w) {
+          uint32_t e[4], f[4];  // [channel 4w + i]: tokens (2c, 2c+1) and (2c+8, 2c+9)
+          codes_to_half<E4M3>(prmt(v[0][w], v[1][w], 0x5140), e[0], e[1]);
+          codes_to_half<E4M3>(prmt(v[0][w], v[1][w], 0x7362), e[2], e[3]);
+          codes_to_half<E4M3>(prmt(v[2][w], v[3][w], 0x5140), f[0], f[1]);
+          codes_to_half<E4M3>(prmt(v[2][w], v[3][w], 0x7362), f[2], f[3]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma16816(o[n][2 * (part * kPart + w)], e[0], e[1], f[0], f[1], pb[n][0], pb[n][1]);
+            mma16816(o[n][2 * (part * kPart + w) + 1], e[2], e[3], f[2], f[3], pb[n][0], pb[n][1]);
+          }
         }
       }
-#pragma unroll
-      for (int w = 0; w < kVWords; ++w) {
-        uint32_t e[4], f[4];  // [channel 4w + i]: tokens (2c, 2c+1) and (2c+8, 2c+9)
-        codes_to_half<E4M3>(prmt(vr[0][w], vr[1][w], 0x5140), e[0], e[1]);
-        codes_to_half<E4M3>(prmt(vr[0][w], vr[1][w], 0x7362), e[2], e[3]);
-        codes_to_half<E4M3>(prmt(vr[2][w], vr[3][w], 0x5140), f[0], f[1]);
-        codes_to_half<E4M3>(prmt(vr[2][w], vr[3][w], 0x7362), f[2], f[3]);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          mma16816(o[n][2 * w], e[0], e[1], f[0], f[1], pb[n][0], pb[n][1]);
-          mma16816(o[n][2 * w + 1], e[2], e[3], f[2], f[3], pb[n][0], pb[n][1]);
-        }
-      }
-      if (more) load_v(page, sub_now);
     }
+
+    __device__ __forceinline__ void finish() {
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i) {
 #pragma unroll
-        for (int d = 4; d < 32; d <<= 1) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], d);
-  }
+          for (int d = 4; d < 32; d <<= 1) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], d);
+          if (unseen >> (2 * n + i) & 1) m[n][i] = kFarBelow;
+        }
+    }
+  };
 
   // Channels of o[.][i][j] for lane row group g: 2i + (j >> 1) from g * (D / 8).
   __device__ static __forceinline__ void write_rows(const AttendArgs& a, const Segment& s, const float (&o)[NT][D / 16][4],
@@ -600,6 +700,8 @@ struct Attend {
     }
     const int all = carry;
     if (all == 0) return;
+    if (tid == 0) prefix[a.requests] = all;
+    __syncthreads();
     // Every CTA has the same number of units (the last has the rest), one for
     // each of its warps at least; CTA u / chunk has unit u.
     const int grid = min((int)gridDim.x, (all + W - 1) / W);
@@ -612,27 +714,52 @@ struct Attend {
     __syncwarp();
 
     if (u0 < u1) {
+      const uint32_t ring = smem_u32(sh.ring[warp]), meta = smem_u32(sh.meta[warp]);
       Segment s = segment_at(a, prefix, u0);
+      Feed feed;
+      feed.unit = u0;
+      feed.end = u1;
+      feed.stage = 0;
+      feed.enter(a, s);
+#pragma unroll 1
+      for (int i = 0; i < S - 1; ++i) feed.next(a, prefix, ring, meta);
+      Rows rows;
+      int stage = 0;
       for (int u = u0;;) {
+        rows.begin(a, s);
         const int from = u - s.begin, to = min(s.units, u1 - s.begin);
-        float o[NT][D / 16][4], m[NT][2], l[NT][2];
-        units(a, s, from, to, o, m, l);
+#pragma unroll 1
+        for (int i = from; i < to; ++i) {
+          copy_wait<S - 2>();
+          __syncwarp();  // the unit is there for all lanes, and the stage before it has been read by all
+          feed.next(a, prefix, ring, meta);
+          rows.add((s.unit0 + i) * kUnit, ring + stage * kStage, meta + stage * 16);
+          if (++stage == S) stage = 0;
+        }
+        rows.finish();
+        u = s.begin + to;
         if (from == 0 && to == s.units) {
-          write_rows(a, s, o, m, l);
+          write_rows(a, s, rows.o, rows.m, rows.l);
         } else {
-          const int slot = 2 * warp + (u == u0 ? 0 : 1), g = lane >> 2, c = lane & 3;
+          // An early part, after which the warp goes on, waits in L2; the last
+          // one takes the place of the ring, where nothing is left to come.
+          const bool early = u < u1;
+          const int slot = 2 * warp + (early ? 0 : 1), g = lane >> 2, c = lane & 3;
+          float* part = early ? a.early + (long long)(cta * W + warp) * kRows * D : reinterpret_cast<float*>(sh.ring[warp]);
+          if (!early) __syncwarp();
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const int row = n * 8 + 2 * c + i;
-              float* p = &sh.o[slot][row][g * (D / 8)];
+              float* p = part + row * D + g * (D / 8);
 #pragma unroll
               for (int d = 0; d < D / 32; ++d)
-                *reinterpret_cast<float4*>(p + 4 * d) = make_float4(o[n][2 * d][i], o[n][2 * d][i + 2], o[n][2 * d + 1][i], o[n][2 * d + 1][i + 2]);
+                *reinterpret_cast<float4*>(p + 4 * d) =
+                    make_float4(rows.o[n][2 * d][i], rows.o[n][2 * d][i + 2], rows.o[n][2 * d + 1][i], rows.o[n][2 * d + 1][i + 2]);
               if (g == 0) {
-                sh.m[slot][row] = m[n][i];
-                sh.l[slot][row] = l[n][i];
+                sh.m[slot][row] = rows.m[n][i];
+                sh.l[slot][row] = rows.l[n][i];
               }
             }
           if (lane == 0) {
@@ -640,10 +767,12 @@ struct Attend {
             sh.used[slot] = 1;
           }
         }
-        u = s.begin + to;
         if (u >= u1) break;
-        s = segment_after(a, prefix, s);
+        int r, which;
+        after(a, prefix, s.request, s.which, u, r, which);
+        s = segment_of(a, prefix, r, which);
       }
+      copy_wait<0>();
     }
     __syncthreads();
 
@@ -676,8 +805,9 @@ struct Attend {
 #pragma unroll 1
       for (uint32_t left = members; left; left &= left - 1) {
         const int slot = __ffs(left) - 1;
+        const float* part = slot & 1 ? reinterpret_cast<const float*>(sh.ring[slot >> 1]) : a.early + (long long)(cta * W + (slot >> 1)) * kRows * D;
         float y[kLane];
-        load_part<false>(&sh.o[slot][row][lane * kLane], y);
+        load_part<false>(part + row * D + lane * kLane, y);
         add_part(y, __shfl_sync(0xffffffffu, f, slot), x);
       }
       const Segment& s = sh.seg[first];
@@ -773,34 +903,39 @@ struct Attend {
   }
 };
 
-template <int D, int NT, bool E4M3, int W, int MINB>
+template <int D, int NT, bool E4M3, int W, int S, int MINB>
 __global__ void __launch_bounds__(W * 32, MINB) k_attend(const __grid_constant__ AttendArgs a) {
-  extern __shared__ __align__(16) unsigned char raw[];
-  using A = Attend<D, NT, E4M3, W>;
+  extern __shared__ __align__(128) unsigned char raw[];
+  using A = Attend<D, NT, E4M3, W, S>;
   A::run(a, *reinterpret_cast<typename A::Shared*>(raw), reinterpret_cast<int*>(raw + sizeof(typename A::Shared)));
 }
 
-// Warps of a CTA and CTAs of an SM for each head size and number of row tiles:
-// what the registers of the fragments leave (q D/8 and o D/4 for each row
-// tile, one unit D/4).
+// Warps of a CTA, stages of a warp's ring and CTAs of an SM for each head size
+// and number of row tiles: what the registers of the rows leave (q D/8 and o
+// D/4 for each tile), and rings of about 190 KB an SM.
 template <int D, int NT>
 struct Shape;
-template <> struct Shape<64, 1> { static constexpr int W = 8, MINB = 3; };
-template <> struct Shape<64, 2> { static constexpr int W = 8, MINB = 2; };
-template <> struct Shape<128, 1> { static constexpr int W = 8, MINB = 2; };
-template <> struct Shape<128, 2> { static constexpr int W = 4, MINB = 3; };
-template <> struct Shape<256, 1> { static constexpr int W = 4, MINB = 2; };
+template <> struct Shape<64, 1> { static constexpr int W = 8, S = 4, MINB = 3; };
+template <> struct Shape<64, 2> { static constexpr int W = 8, S = 4, MINB = 2; };
+template <> struct Shape<128, 1> { static constexpr int W = 8, S = 3, MINB = 2; };
+template <> struct Shape<128, 2> { static constexpr int W = 4, S = 4, MINB = 3; };
+template <> struct Shape<256, 1> { static constexpr int W = 4, S = 3, MINB = 2; };
+
+template <int D, int NT>
+constexpr size_t early_bytes(int sms) {
+  return (size_t)sms * Shape<D, NT>::MINB * Shape<D, NT>::W * 8 * NT * D * sizeof(float);
+}
 
 template <int D, int NT, bool E4M3>
 dk_status launch(AttendArgs a, cudaStream_t stream) {
-  constexpr int W = Shape<D, NT>::W, MINB = Shape<D, NT>::MINB;
-  using A = Attend<D, NT, E4M3, W>;
-  const size_t smem = sizeof(typename A::Shared) + sizeof(int) * (size_t)std::min(a.requests, kMaxRequests);
-  auto kernel = k_attend<D, NT, E4M3, W, MINB>;
+  constexpr int W = Shape<D, NT>::W, MINB = Shape<D, NT>::MINB, S = Shape<D, NT>::S;
+  using A = Attend<D, NT, E4M3, W, S>;
+  const size_t smem = sizeof(typename A::Shared) + sizeof(int) * (size_t)(std::min(a.requests, kMaxRequests) + 1);
+  auto kernel = k_attend<D, NT, E4M3, W, S, MINB>;
   static thread_local unsigned long long prepared = 0;  // devices whose limit is set
   const int device = current_device();
   if (device >= 64 || !(prepared >> device & 1)) {
-    const size_t most = sizeof(typename A::Shared) + sizeof(int) * kMaxRequests;
+    const size_t most = sizeof(typename A::Shared) + sizeof(int) * (kMaxRequests + 1);
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
     if (e == cudaSuccess)
       e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
@@ -856,11 +991,16 @@ dk_status launch_code(const AttendArgs& a, bool e4m3, cudaStream_t stream) {
 using namespace dk;
 
 extern "C" size_t dk_cache_attention_workspace_bytes(int head_dim) {
-  // Two parts of 16 rows for each CTA that can run at once, and their counters.
+  // Counters, two parts of up to 16 rows for each CTA that can run at once, and
+  // an early part for each of its warps.
   if (head_dim != 64 && head_dim != 128 && head_dim != 256) return 0;
-  const size_t ctas = (size_t)sm_count(-1) * 3;
+  const int sms = sm_count(-1);
+  const size_t ctas = (size_t)sms * 3;
   const size_t counters = (ctas * sizeof(int) + 255) / 256 * 256;
-  return counters + ctas * 2 * 16 * (size_t)(head_dim + 2) * sizeof(float);
+  const size_t early = head_dim == 64    ? std::max(early_bytes<64, 1>(sms), early_bytes<64, 2>(sms))
+                       : head_dim == 128 ? std::max(early_bytes<128, 1>(sms), early_bytes<128, 2>(sms))
+                                         : early_bytes<256, 1>(sms);
+  return counters + ctas * 2 * 16 * (size_t)(head_dim + 2) * sizeof(float) + early;
 }
 
 extern "C" dk_status dk_cache_attention(const dk_cache_attention_args* p, void* workspace,
@@ -908,6 +1048,7 @@ extern "C" dk_status dk_cache_attention(const dk_cache_attention_args* p, void* 
   const size_t ctas = (size_t)sm_count(-1) * 3;
   a.counters = static_cast<int*>(workspace);
   a.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + (ctas * sizeof(int) + 255) / 256 * 256);
+  a.early = a.partials + ctas * 2 * 16 * (size_t)(c.head_dim + 2);
   a.q_token_stride = p->q_token_stride;
   a.q_head_stride = p->q_head_stride;
   a.k_block_stride = c.k_block_stride;
