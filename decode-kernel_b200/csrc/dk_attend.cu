@@ -67,9 +67,9 @@ struct AttendArgs {
   float* partials;
   float* early;
   long long q_token_stride, q_head_stride;
-  long long k_block_stride, k_head_stride, k_token_stride;
-  long long v_block_stride, v_head_stride, v_token_stride;
-  int table_stride, max_blocks, blocks, block_size;
+  long long k_head_stride, v_head_stride;
+  uint32_t k_block_stride, k_token_stride, v_block_stride, v_token_stride;
+  int table_stride, max_blocks, blocks, block_size, units_per_block;
   int requests, tokens, kv_heads, group;
   unsigned group_magic;  // ceil(2^32 / group), 0 for a group of 1
   float scale_log2;
@@ -118,11 +118,6 @@ __device__ __forceinline__ int ld_int(const int* p) {
   asm volatile("ld.global.b32 %0, [%1];" : "=r"(x) : "l"(p));
   return x;
 }
-__device__ __forceinline__ float ld_float(const float* p) {
-  float x;
-  asm volatile("ld.global.b32 %0, [%1];" : "=f"(x) : "l"(p));
-  return x;
-}
 
 __device__ __forceinline__ uint4 ld_quad(const void* p) {
   uint4 r;
@@ -159,23 +154,29 @@ struct Segment {
   int which, all;                  // its number among the request's segments, and how many they are
   int unit0, units;                // its first unit among the request's, and how many
   int begin;                       // its first unit in the line of all units
+  int blocks;                      // pages of its request
 };
 
-template <int D, int NT, bool E4M3, int W, int S>
+// PACKED: the tokens of a page's head are neighbours in memory, so the rows of
+// a unit lie at fixed offsets.
+template <int D, int NT, bool E4M3, bool PACKED, int W, int S>
 struct Attend {
   static constexpr int kRows = 8 * NT;
   static constexpr int kKWords = D / 16;  // words of a lane's part of a K row
   static constexpr int kVWords = D / 32;  // words of a lane's part of a V row
   static constexpr int kSlots = 2 * W;    // a warp's parts of segments: an early one and its last
-  static constexpr int kStage = 2 * kUnit * D;  // bytes of a unit
+  // A stage: K, V and the two scales of a unit.  Multiples of 128 bytes, so that
+  // the places of pieces differ by an exclusive or of their low bits.
+  static constexpr int kScales = 2 * kUnit * D;
+  static constexpr int kStage = kScales + 128;
   static_assert(kRows * D * 4 <= S * kStage, "a part fits the warp's ring");
 
   struct Shared {
     unsigned char ring[W][S][kStage];  // at the end the warp's last part: float [kRows][D]
-    float4 meta[W][S];                 // of a stage: K scale, V scale, whether its page is in the pool
     float m[kSlots][kRows];
     float l[kSlots][kRows];
     Segment seg[kSlots];
+    Segment fed[W], now[W];            // the segments whose units a warp copies and adds up
     int used[kSlots];
     int last[2];
     int total[W];
@@ -194,6 +195,12 @@ struct Attend {
       return row * D + (p ^ (((row ^ (row >> 1)) & 1) | (row & 4))) * 16;
     }
   }
+  // A lane's places, of which the others follow by offsets and exclusive ors:
+  // place(row + j * kStep, p) = (place(row, p) ^ copy_turn(j)) + j * 512,
+  static constexpr int kPieces = D / 16, kStep = 512 / D;  // pieces of a row, rows of a warp's copy
+  __device__ static constexpr int copy_turn(int j) { return D == 64 ? 0 : D == 128 ? (j & 1) * 64 : (j & 1) * 16 + (j & 2) * 32; }
+  // place(g, 2c + 1) = place(g, 2c) ^ 16, place(2c + 1, p) = (place(2c, p) ^ kOdd) + kOddRow.
+  static constexpr int kOdd = D == 64 ? 64 : 16, kOddRow = D == 64 ? 0 : D;
 
   __device__ static __forceinline__ int units_of(const AttendArgs& a, int length, int fresh, int& unit0) {
     unit0 = 0;
@@ -222,6 +229,7 @@ struct Attend {
     s.units = units_of(a, s.length, s.fresh, s.unit0);
     s.which = which;
     s.begin = prefix[r] + which * s.units;
+    s.blocks = (s.length + a.block_size - 1) / a.block_size;
     const int tiles = tiles_of(a, s.fresh);
     s.all = tiles * a.kv_heads;
     s.head = tiles == 1 ? which : which / tiles;
@@ -318,68 +326,68 @@ struct Attend {
   // The warp's copies: its units in their order, across segments, each into
   // the next stage of its ring.
   struct Feed {
-    const uint8_t* k;
+    const uint8_t* k;  // the lane's first piece in page 0 of the segment's head
     const uint8_t* v;
-    const int* table;
+    const float* scale;  // of K (even lanes) or V there
+    uint32_t to;         // the lane's place in the next stage
     int unit, end, segment_end;  // next unit in the line, the warp's end, the segment's
-    int request, which, head;
-    int block, sub, last_block, page, next_page;
-    int stage;
+    int block, sub, page, next_page;
+    uint32_t hidden;  // of each stage (bits): its page is outside the pool
 
-    __device__ __forceinline__ int page_at(int b) const { return b <= last_block ? ld_int(table + b) : -1; }
+    __device__ __forceinline__ int page_at(const AttendArgs& a, const Segment& s, int b) const {
+      return b < s.blocks ? ld_int(a.table + (long long)s.request * a.table_stride + b) : -1;
+    }
 
     // From here units of segment s.
     __device__ __forceinline__ void enter(const AttendArgs& a, const Segment& s) {
       const int lane = threadIdx.x & 31;
-      constexpr int kPieces = D / 16;
       const int row = lane / kPieces, piece = lane % kPieces;
-      request = s.request;
-      which = s.which;
-      head = s.head;
       segment_end = s.begin + s.units;
-      k = a.k + s.head * a.k_head_stride + row * a.k_token_stride + piece * 16;
-      v = a.v + s.head * a.v_head_stride + row * a.v_token_stride + piece * 16;
-      table = a.table + (long long)s.request * a.table_stride;
-      last_block = s.length > 0 ? (s.length - 1) / a.block_size : -1;
-      const int u = s.unit0 + unit - s.begin, upb = a.block_size / kUnit;
-      block = u / upb;
-      sub = u - block * upb;
-      page = page_at(block);
-      next_page = page_at(block + 1);
+      k = a.k + s.head * a.k_head_stride + (PACKED ? row * D : row * (long long)a.k_token_stride) + piece * 16;
+      v = a.v + s.head * a.v_head_stride + (PACKED ? row * D : row * (long long)a.v_token_stride) + piece * 16;
+      scale = (lane & 1 ? a.v_scale : a.k_scale) + s.head;
+      const int u = s.unit0 + unit - s.begin;
+      block = u / a.units_per_block;
+      sub = u - block * a.units_per_block;
+      page = page_at(a, s, block);
+      next_page = page_at(a, s, block + 1);
     }
 
-    // Copies the next unit, if there is one; always one group.
-    __device__ __forceinline__ void next(const AttendArgs& a, const int* prefix, uint32_t ring, uint32_t meta) {
+    // Copies the next unit, if there is one, into stage `at` (its number,
+    // `stage`); always one group.
+    __device__ __forceinline__ void next(const AttendArgs& a, const int* prefix, Segment& s, int offset, int stage) {
       if (unit < end) {
         if (unit == segment_end) {
-          int r, w;
-          after(a, prefix, request, which, segment_end, r, w);
-          enter(a, segment_of(a, prefix, r, w));
+          int r, which;
+          after(a, prefix, s.request, s.which, segment_end, r, which);
+          __syncwarp();  // every lane has read s
+          const Segment t = segment_of(a, prefix, r, which);
+          if ((threadIdx.x & 31) == 0) s = t;
+          __syncwarp();
+          enter(a, t);
         }
-        const int lane = threadIdx.x & 31;
-        constexpr int kStep = 512 / D;  // rows of a warp's copy
         const bool good = (unsigned)page < (unsigned)a.blocks;
-        const long long p = good ? page : 0;
-        const uint8_t* from_k = k + p * a.k_block_stride + (long long)(sub * kUnit) * a.k_token_stride;
-        const uint8_t* from_v = v + p * a.v_block_stride + (long long)(sub * kUnit) * a.v_token_stride;
-        const uint32_t to = ring + stage * kStage;
-        const int row = lane / (D / 16), piece = lane % (D / 16);
-#pragma unroll
-        for (int j = 0; j < kUnit / kStep; ++j) copy16(to + place(row + j * kStep, piece), from_k + (long long)(j * kStep) * a.k_token_stride);
+        const uint32_t p = good ? page : 0;
+        hidden = (hidden & ~(1u << stage)) | ((good ? 0u : 1u) << stage);
+        const uint32_t first = sub * kUnit;
+        const uint8_t* from_k = k + (uint64_t)p * a.k_block_stride + (PACKED ? first * D : first * a.k_token_stride);
+        const uint8_t* from_v = v + (uint64_t)p * a.v_block_stride + (PACKED ? first * D : first * a.v_token_stride);
+        const uint32_t at = to + offset;
 #pragma unroll
         for (int j = 0; j < kUnit / kStep; ++j)
-          copy16(to + kUnit * D + place(row + j * kStep, piece), from_v + (long long)(j * kStep) * a.v_token_stride);
-        const uint32_t about = meta + stage * 16;
-        if (lane < 2) copy4(about + lane * 4, (lane ? a.v_scale : a.k_scale) + p * a.kv_heads + head);
-        if (lane == 2) asm volatile("st.shared.b32 [%0], %1;" ::"r"(about + 8), "r"((int)good) : "memory");
+          copy16((at ^ copy_turn(j)) + j * 512, from_k + (PACKED ? j * 512 : (uint64_t)(j * kStep) * a.k_token_stride));
+#pragma unroll
+        for (int j = 0; j < kUnit / kStep; ++j)
+          copy16((at ^ copy_turn(j)) + kUnit * D + j * 512, from_v + (PACKED ? j * 512 : (uint64_t)(j * kStep) * a.v_token_stride));
+        const int lane = threadIdx.x & 31;
+        if (lane < 2) copy4(to - place(lane / kPieces, lane % kPieces) + offset + kScales + lane * 4, scale + (uint64_t)p * (uint32_t)a.kv_heads);
         ++unit;
-        if (++sub == a.block_size / kUnit) {
+        if (++sub == a.units_per_block) {
           sub = 0;
           ++block;
           page = next_page;
-          next_page = page_at(block + 1);
+          next_page = page_at(a, s, block + 1);
         }
-        if (++stage == S) stage = 0;
       }
       copy_commit();
     }
@@ -389,7 +397,6 @@ struct Attend {
   struct Rows {
     uint32_t q[NT][2 * kKWords];
     float o[NT][D / 16][4], m[NT][2], l[NT][2], factor[NT][2];
-    int low[NT][2], high[NT][2];
     // Tokens that every row sees are [most_low, least_high), those that some
     // row sees are within [least_low, most_high).
     int least_high, most_low, least_low, most_high;
@@ -408,12 +415,14 @@ struct Attend {
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          int token, head;
-          const bool there = row_of(a, s, n * 8 + 2 * c + i, token, head, low[n][i], high[n][i]);
-          least_high = min(least_high, there ? high[n][i] : 0x7fffffff);
-          least_low = min(least_low, there ? low[n][i] : 0x7fffffff);
-          most_low = max(most_low, low[n][i]);
-          most_high = max(most_high, high[n][i]);
+          if (s.fresh != 1) {
+            int token, head, low, high;
+            const bool there = row_of(a, s, n * 8 + 2 * c + i, token, head, low, high);
+            least_high = min(least_high, there ? high : 0x7fffffff);
+            least_low = min(least_low, there ? low : 0x7fffffff);
+            most_low = max(most_low, low);
+            most_high = max(most_high, high);
+          }
           m[n][i] = 0.f;
           l[n][i] = 0.f;
         }
@@ -470,25 +479,24 @@ struct Attend {
       settled = !__any_sync(0xffffffffu, unseen);
     }
 
-    // The unit of tokens base.. in the stage at `at`.
-    __device__ __forceinline__ void add(int base, uint32_t at, uint32_t about) {
+    // The unit of tokens base.. of segment s in the stage at `at`.
+    __device__ __forceinline__ void add(const AttendArgs& a, const Segment& s, int base, uint32_t at, bool good) {
       const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
       float k_scale, v_scale;
-      int good;
-      asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(k_scale), "=f"(v_scale) : "r"(about));
-      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(good) : "r"(about + 8));
+      asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(k_scale), "=f"(v_scale) : "r"(at + kScales));
       // Scores: [16 tokens][8 rows] for each tile of rows, in two chains.
       float sc[NT][4], sd[NT][4];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) sc[n][i] = sd[n][i] = 0.f;
+      const uint32_t at_k = at + place(g, D == 64 ? c : 2 * c);
 #pragma unroll
       for (int part = 0; part < kKWords / 4; ++part) {
         uint32_t k0[4], k1[4];
-        const int piece = D == 64 ? c : 2 * c + (part & 1) + (part >> 1) * 8;
-        lds_words<4>(at + place(g, piece), k0);
-        lds_words<4>(at + place(g, piece) + 8 * D, k1);
+        const uint32_t from = (at_k ^ (part & 1) * 16) + (part >> 1) * 128;
+        lds_words<4>(from, k0);
+        lds_words<4>(from + 8 * D, k1);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           uint32_t a0, a1, a2, a3;
@@ -514,9 +522,12 @@ struct Attend {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int t = base + g + (i >> 1) * 8;
-            if (t >= high[n][i & 1] || t < low[n][i & 1] || !good) sc[n][i] = -INFINITY;
+          for (int i = 0; i < 2; ++i) {
+            int token, head, low, high;
+            row_of(a, s, n * 8 + 2 * c + i, token, head, low, high);
+            const int t = base + g;
+            if (t >= high || t < low || !good) sc[n][i] = -INFINITY;
+            if (t + 8 >= high || t + 8 < low || !good) sc[n][i + 2] = -INFINITY;
           }
       }
 #pragma unroll
@@ -533,17 +544,14 @@ struct Attend {
         pb[n][0] = transpose8x8(pack_half2(w[0], w[1]));
         pb[n][1] = transpose8x8(pack_half2(w[2], w[3]));
       }
-      const uint32_t at_v = at + kUnit * D;
+      const uint32_t at_v = at + kUnit * D + (D == 64 ? place(2 * c, g >> 1) + (g & 1) * 8 : place(2 * c, D == 128 ? g : 2 * g));
       constexpr int kPart = kVWords < 4 ? kVWords : 4;  // words of a load
 #pragma unroll
       for (int part = 0; part < kVWords / kPart; ++part) {
         uint32_t v[4][kPart];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int row = 2 * c + (j & 1);
-          const uint32_t from = D == 64 ? place(row, g >> 1) + (g & 1) * 8 : place(row, D == 128 ? g : 2 * g + part);
-          lds_words<kPart>(at_v + from + (j >> 1) * 8 * D, v[j]);
-        }
+        for (int j = 0; j < 4; ++j)
+          lds_words<kPart>((at_v ^ ((j & 1) * kOdd) ^ (part * 16)) + (j & 1) * kOddRow + (j >> 1) * 8 * D, v[j]);
         if (edge) {  // bytes of tokens that no row sees may be anything, e4m3's NaN too
           const int past = good ? most_high - base : 0, before = least_low - base;
 #pragma unroll
@@ -714,27 +722,38 @@ struct Attend {
     __syncwarp();
 
     if (u0 < u1) {
-      const uint32_t ring = smem_u32(sh.ring[warp]), meta = smem_u32(sh.meta[warp]);
-      Segment s = segment_at(a, prefix, u0);
+      const uint32_t ring = smem_u32(sh.ring[warp]);
+      Segment& s = sh.now[warp];
+      {
+        const Segment t = segment_at(a, prefix, u0);
+        if (lane == 0) s = sh.fed[warp] = t;
+        __syncwarp();
+      }
       Feed feed;
       feed.unit = u0;
       feed.end = u1;
-      feed.stage = 0;
+      feed.to = ring + place(lane / kPieces, lane % kPieces);
+      feed.hidden = 0;
       feed.enter(a, s);
 #pragma unroll 1
-      for (int i = 0; i < S - 1; ++i) feed.next(a, prefix, ring, meta);
+      for (int i = 0; i < S - 1; ++i) feed.next(a, prefix, sh.fed[warp], i * kStage, i);
       Rows rows;
-      int stage = 0;
+      int offset = 0, stage = 0, freed = (S - 1) * kStage, freed_stage = S - 1;
       for (int u = u0;;) {
         rows.begin(a, s);
         const int from = u - s.begin, to = min(s.units, u1 - s.begin);
+        int base = (s.unit0 + from) * kUnit;
 #pragma unroll 1
         for (int i = from; i < to; ++i) {
           copy_wait<S - 2>();
           __syncwarp();  // the unit is there for all lanes, and the stage before it has been read by all
-          feed.next(a, prefix, ring, meta);
-          rows.add((s.unit0 + i) * kUnit, ring + stage * kStage, meta + stage * 16);
-          if (++stage == S) stage = 0;
+          feed.next(a, prefix, sh.fed[warp], freed, freed_stage);
+          rows.add(a, s, base, ring + offset, !(feed.hidden >> stage & 1));
+          base += kUnit;
+          freed = offset;
+          freed_stage = stage;
+          offset += kStage;
+          if (++stage == S) stage = offset = 0;
         }
         rows.finish();
         u = s.begin + to;
@@ -770,7 +789,10 @@ struct Attend {
         if (u >= u1) break;
         int r, which;
         after(a, prefix, s.request, s.which, u, r, which);
-        s = segment_of(a, prefix, r, which);
+        __syncwarp();  // every lane has read s
+        const Segment t = segment_of(a, prefix, r, which);
+        if (lane == 0) s = t;
+        __syncwarp();
       }
       copy_wait<0>();
     }
@@ -903,10 +925,10 @@ struct Attend {
   }
 };
 
-template <int D, int NT, bool E4M3, int W, int S, int MINB>
+template <int D, int NT, bool E4M3, bool PACKED, int W, int S, int MINB>
 __global__ void __launch_bounds__(W * 32, MINB) k_attend(const __grid_constant__ AttendArgs a) {
   extern __shared__ __align__(128) unsigned char raw[];
-  using A = Attend<D, NT, E4M3, W, S>;
+  using A = Attend<D, NT, E4M3, PACKED, W, S>;
   A::run(a, *reinterpret_cast<typename A::Shared*>(raw), reinterpret_cast<int*>(raw + sizeof(typename A::Shared)));
 }
 
@@ -926,12 +948,12 @@ constexpr size_t early_bytes(int sms) {
   return (size_t)sms * Shape<D, NT>::MINB * Shape<D, NT>::W * 8 * NT * D * sizeof(float);
 }
 
-template <int D, int NT, bool E4M3>
+template <int D, int NT, bool E4M3, bool PACKED>
 dk_status launch(AttendArgs a, cudaStream_t stream) {
   constexpr int W = Shape<D, NT>::W, MINB = Shape<D, NT>::MINB, S = Shape<D, NT>::S;
-  using A = Attend<D, NT, E4M3, W, S>;
+  using A = Attend<D, NT, E4M3, PACKED, W, S>;
   const size_t smem = sizeof(typename A::Shared) + sizeof(int) * (size_t)(std::min(a.requests, kMaxRequests) + 1);
-  auto kernel = k_attend<D, NT, E4M3, W, S, MINB>;
+  auto kernel = k_attend<D, NT, E4M3, PACKED, W, S, MINB>;
   static thread_local unsigned long long prepared = 0;  // devices whose limit is set
   const int device = current_device();
   if (device >= 64 || !(prepared >> device & 1)) {
@@ -982,7 +1004,9 @@ int row_tiles(int head_dim, long long rows) { return head_dim < 256 && rows > 8 
 
 template <int D, int NT>
 dk_status launch_code(const AttendArgs& a, bool e4m3, cudaStream_t stream) {
-  return e4m3 ? launch<D, NT, true>(a, stream) : launch<D, NT, false>(a, stream);
+  const bool packed = a.k_token_stride == D && a.v_token_stride == D;
+  if (e4m3) return packed ? launch<D, NT, true, true>(a, stream) : launch<D, NT, true, false>(a, stream);
+  return packed ? launch<D, NT, false, true>(a, stream) : launch<D, NT, false, false>(a, stream);
 }
 
 }  // namespace
@@ -1026,6 +1050,10 @@ extern "C" dk_status dk_cache_attention(const dk_cache_attention_args* p, void* 
   if (!aligned(c.k, 32) || !aligned(c.v, 32) || !aligned(p->q, 16) || !aligned(p->out, 16) ||
       p->q_token_stride % 8 || p->q_head_stride % 8)
     return DK_ERR_INVALID_ARG;
+  // A page's stride and the offsets within one are kept in 32 bits.
+  if (c.k_block_stride > INT32_MAX || c.v_block_stride > INT32_MAX ||
+      c.k_token_stride > INT32_MAX / c.block_size || c.v_token_stride > INT32_MAX / c.block_size)
+    return DK_ERR_UNSUPPORTED;
   // The line of units is counted in 32 bits.
   const int group = p->q_heads / c.kv_heads;
   const long long units = ((long long)p->max_blocks * c.block_size + 15) / 16;
@@ -1051,16 +1079,17 @@ extern "C" dk_status dk_cache_attention(const dk_cache_attention_args* p, void* 
   a.early = a.partials + ctas * 2 * 16 * (size_t)(c.head_dim + 2);
   a.q_token_stride = p->q_token_stride;
   a.q_head_stride = p->q_head_stride;
-  a.k_block_stride = c.k_block_stride;
+  a.k_block_stride = (uint32_t)c.k_block_stride;
   a.k_head_stride = c.k_head_stride;
-  a.k_token_stride = c.k_token_stride;
-  a.v_block_stride = c.v_block_stride;
+  a.k_token_stride = (uint32_t)c.k_token_stride;
+  a.v_block_stride = (uint32_t)c.v_block_stride;
   a.v_head_stride = c.v_head_stride;
-  a.v_token_stride = c.v_token_stride;
+  a.v_token_stride = (uint32_t)c.v_token_stride;
   a.table_stride = p->table_stride;
   a.max_blocks = p->max_blocks;
   a.blocks = c.blocks;
   a.block_size = c.block_size;
+  a.units_per_block = c.block_size / kUnit;
   a.requests = p->requests;
   a.tokens = p->tokens;
   a.kv_heads = c.kv_heads;

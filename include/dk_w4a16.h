@@ -427,7 +427,8 @@ DK_API dk_status dk_cache_append(const dk_cache8* cache, const void* k, const vo
  * in fp32 and rounded once; rows that see no token are zeros.  lse (or NULL)
  * gets log(sum_j exp(scale * q . k_j)), -inf for such rows.  q has strides in
  * elements, multiples of 8, and is 16-byte aligned; out and lse are contiguous.
- * V scales below 2^-70 count as 2^-70.  Entries of block_table outside the
+ * Block strides are below 2^31 and block_size * token stride too.  V scales
+ * below 2^-70 count as 2^-70.  Entries of block_table outside the
  * pool hide their tokens.
  * The workspace (dk_cache_attention_workspace_bytes of the current device) is
  * 256-byte aligned and zero before its first call, which every call leaves it
