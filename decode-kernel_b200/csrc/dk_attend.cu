@@ -153,7 +153,7 @@ struct Segment {
   int length, fresh, first_token;  // tokens held, queries, row of the first query in q
   int which, all;                  // its number among the request's segments, and how many they are
   int unit0, units;                // its first unit among the request's, and how many
-  int begin;                       // its first unit in the line of all units
+  int begin;                       // place of its first unit in the line of all units
   int blocks;                      // pages of its request
 };
 
@@ -165,6 +165,9 @@ struct Attend {
   static constexpr int kKWords = D / 16;  // words of a lane's part of a K row
   static constexpr int kVWords = D / 32;  // words of a lane's part of a V row
   static constexpr int kSlots = 2 * W;    // a warp's parts of segments: an early one and its last
+  // Places in the line that a segment's start counts for: its queries' latency
+  // and its rows' end take as long as this many units.
+  static constexpr int kStart = D == 64 ? 2 : 1;
   // A stage: K, V and the two scales of a unit.  Multiples of 128 bytes, so that
   // the places of pieces differ by an exclusive or of their low bits.
   static constexpr int kScales = 2 * kUnit * D;
@@ -228,7 +231,7 @@ struct Attend {
     request_of(a, r, s.length, s.fresh, s.first_token);
     s.units = units_of(a, s.length, s.fresh, s.unit0);
     s.which = which;
-    s.begin = prefix[r] + which * s.units;
+    s.begin = prefix[r] + which * (s.units + kStart) + kStart;
     s.blocks = (s.length + a.block_size - 1) / a.block_size;
     const int tiles = tiles_of(a, s.fresh);
     s.all = tiles * a.kv_heads;
@@ -236,7 +239,7 @@ struct Attend {
     s.tile = which - s.head * tiles;
     return s;
   }
-  // The segment of unit u of the line.
+  // The segment of place u of the line.
   __device__ static __forceinline__ Segment segment_at(const AttendArgs& a, const int* prefix, int u) {
     int lo = 0, hi = a.requests - 1;  // the last request whose first unit is at or before u
     while (lo < hi) {
@@ -244,10 +247,10 @@ struct Attend {
       if (prefix[mid] <= u) lo = mid; else hi = mid - 1;
     }
     Segment s = segment_of(a, prefix, lo, 0);
-    const int which = (u - s.begin) / s.units;
+    const int which = (u - (s.begin - kStart)) / (s.units + kStart);
     return which ? segment_of(a, prefix, lo, which) : s;
   }
-  // The segment after segment `which` of request r, which ends before unit u.
+  // The segment after segment `which` of request r, which ends before place u.
   __device__ static __forceinline__ void after(const AttendArgs& a, const int* prefix, int r, int which, int u, int& next_r, int& next_which) {
     next_r = r;
     next_which = which + 1;
@@ -330,7 +333,7 @@ struct Attend {
     const uint8_t* v;
     const float* scale;  // of K (even lanes) or V there
     uint32_t to;         // the lane's place in the next stage
-    int unit, end, segment_end;  // next unit in the line, the warp's end, the segment's
+    int unit, end, segment_end;  // place of the next unit in the line, the warp's end, the segment's
     int block, sub, page, next_page;
     uint32_t hidden;  // of each stage (bits): its page is outside the pool
 
@@ -346,6 +349,7 @@ struct Attend {
       k = a.k + s.head * a.k_head_stride + (PACKED ? row * D : row * (long long)a.k_token_stride) + piece * 16;
       v = a.v + s.head * a.v_head_stride + (PACKED ? row * D : row * (long long)a.v_token_stride) + piece * 16;
       scale = (lane & 1 ? a.v_scale : a.k_scale) + s.head;
+      unit = max(unit, s.begin);
       const int u = s.unit0 + unit - s.begin;
       block = u / a.units_per_block;
       sub = u - block * a.units_per_block;
@@ -356,16 +360,16 @@ struct Attend {
     // Copies the next unit, if there is one, into stage `at` (its number,
     // `stage`); always one group.
     __device__ __forceinline__ void next(const AttendArgs& a, const int* prefix, Segment& s, int offset, int stage) {
-      if (unit < end) {
-        if (unit == segment_end) {
+      if (unit == segment_end && unit < end) {
           int r, which;
-          after(a, prefix, s.request, s.which, segment_end, r, which);
-          __syncwarp();  // every lane has read s
-          const Segment t = segment_of(a, prefix, r, which);
-          if ((threadIdx.x & 31) == 0) s = t;
-          __syncwarp();
-          enter(a, t);
-        }
+        after(a, prefix, s.request, s.which, segment_end, r, which);
+        __syncwarp();  // every lane has read s
+        const Segment t = segment_of(a, prefix, r, which);
+        if ((threadIdx.x & 31) == 0) s = t;
+        __syncwarp();
+        enter(a, t);
+      }
+      if (unit < end) {
         const bool good = (unsigned)page < (unsigned)a.blocks;
         const uint32_t p = good ? page : 0;
         hidden = (hidden & ~(1u << stage)) | ((good ? 0u : 1u) << stage);
@@ -677,7 +681,8 @@ struct Attend {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_trigger();
     pdl_wait();
-    // Units of every request, summed up: prefix[r] = the first of request r.
+    // Places of every request's units in the line: prefix[r] = the first of
+    // request r.
     int carry = 0;
     for (int base = 0; base < a.requests; base += W * 32) {
       const int r = base + tid;
@@ -685,7 +690,7 @@ struct Attend {
       if (r < a.requests) {
         int length, fresh, first, unit0;
         request_of(a, r, length, fresh, first);
-        mine = units_of(a, length, fresh, unit0) * tiles_of(a, fresh) * a.kv_heads;
+        mine = (units_of(a, length, fresh, unit0) + kStart) * tiles_of(a, fresh) * a.kv_heads;
       }
       int sum = mine;
 #pragma unroll
@@ -740,8 +745,9 @@ struct Attend {
       Rows rows;
       int offset = 0, stage = 0, freed = (S - 1) * kStage, freed_stage = S - 1;
       for (int u = u0;;) {
+        const int from = max(0, u - s.begin), to = min(s.units, u1 - s.begin);
+        if (to <= 0) break;  // only the segment's start is this warp's
         rows.begin(a, s);
-        const int from = u - s.begin, to = min(s.units, u1 - s.begin);
         int base = (s.unit0 + from) * kUnit;
 #pragma unroll 1
         for (int i = from; i < to; ++i) {
@@ -825,12 +831,19 @@ struct Attend {
       // Few instructions: this code runs once a call, and fetching it costs
       // more than running it.
 #pragma unroll 1
-      for (uint32_t left = members; left; left &= left - 1) {
-        const int slot = __ffs(left) - 1;
-        const float* part = slot & 1 ? reinterpret_cast<const float*>(sh.ring[slot >> 1]) : a.early + (long long)(cta * W + (slot >> 1)) * kRows * D;
-        float y[kLane];
-        load_part<false>(part + row * D + lane * kLane, y);
-        add_part(y, __shfl_sync(0xffffffffu, f, slot), x);
+      for (uint32_t left = members; left;) {
+        float y[4][kLane], by[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {  // past the last: the first again, times 0
+          const int slot = left ? __ffs(left) - 1 : first;
+          const float* part = slot & 1 ? reinterpret_cast<const float*>(sh.ring[slot >> 1]) : a.early + (long long)(cta * W + (slot >> 1)) * kRows * D;
+          load_part<false>(part + row * D + lane * kLane, y[k]);
+          by[k] = __shfl_sync(0xffffffffu, f, slot);
+          if (!left) by[k] = 0.f;
+          left &= left - 1;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) add_part(y[k], by[k], x);
       }
       const Segment& s = sh.seg[first];
       if (s.begin >= cta0 && s.begin + s.units <= cta1) {
@@ -988,7 +1001,7 @@ dk_status launch(AttendArgs a, cudaStream_t stream) {
       a.tokens = tokens - r;
     }
     // No more CTAs than the table's width can keep busy.
-    const long long most = (((long long)a.max_blocks * a.block_size + kUnit - 1) / kUnit) * a.kv_heads *
+    const long long most = (((long long)a.max_blocks * a.block_size + kUnit - 1) / kUnit + A::kStart) * a.kv_heads *
                            (starts ? (long long)a.requests + (long long)tokens * a.group / A::kRows : (long long)a.requests * ((a.group + A::kRows - 1) / A::kRows));
     const int grid = (int)std::min<long long>(sm_count(device) * MINB, (most + W - 1) / W);
     const dk_status s = launch_early("dk_cache_attention", kernel, dim3(grid), dim3(W * 32), smem, stream, a);
@@ -1056,7 +1069,7 @@ extern "C" dk_status dk_cache_attention(const dk_cache_attention_args* p, void* 
     return DK_ERR_UNSUPPORTED;
   // The line of units is counted in 32 bits.
   const int group = p->q_heads / c.kv_heads;
-  const long long units = ((long long)p->max_blocks * c.block_size + 15) / 16;
+  const long long units = ((long long)p->max_blocks * c.block_size + 15) / 16 + 2;
   const long long per_head = (long long)std::min(p->requests, kMaxRequests) + (long long)p->tokens * group / 8;
   if (units > INT32_MAX / 16 || per_head > INT32_MAX / 2 / units / c.kv_heads) return DK_ERR_UNSUPPORTED;
   const size_t need = dk_cache_attention_workspace_bytes(c.head_dim);
