@@ -63,6 +63,7 @@ struct AttendArgs {
   const int* starts;
   void* out;
   float* lse;
+  void* workspace;
   int* counters;
   float* partials;
   float* early;
@@ -172,10 +173,15 @@ struct Attend {
   // the places of pieces differ by an exclusive or of their low bits.
   static constexpr int kScales = 2 * kUnit * D;
   static constexpr int kStage = kScales + 128;
-  static_assert(kRows * D * 4 <= S * kStage, "a part fits the warp's ring");
+  // The queries' operands stay in registers while those hold them beside the
+  // output's; from 24 rows of 128 on they are read from shared memory.
+  static constexpr bool kQShared = NT * D > 256;
+  static constexpr int kQBytes = kQShared ? NT * kKWords * 256 : 0;
+  static constexpr int kWarp = S * kStage + kQBytes;  // a warp's shared memory
+  static_assert(kRows * D * 4 <= kWarp, "a part fits it");
 
   struct Shared {
-    unsigned char ring[W][S][kStage];  // at the end the warp's last part: float [kRows][D]
+    unsigned char ring[W][kWarp];  // stages and queries; at the end the warp's last part: float [kRows][D]
     float m[kSlots][kRows];
     float l[kSlots][kRows];
     Segment seg[kSlots];
@@ -399,7 +405,7 @@ struct Attend {
 
   // A warp's running sums over the units of one segment.
   struct Rows {
-    uint32_t q[NT][2 * kKWords];
+    uint32_t q[kQShared ? 1 : NT][2 * kKWords];
     float o[NT][D / 16][4], m[NT][2], l[NT][2], factor[NT][2];
     // Tokens that every row sees are [most_low, least_high), those that some
     // row sees are within [least_low, most_high).
@@ -407,10 +413,12 @@ struct Attend {
     uint32_t unseen;  // rows (bits) of this lane's columns without a token yet, whose m is 0
     bool settled;     // no lane has any
 
-    __device__ __forceinline__ void begin(const AttendArgs& a, const Segment& s) {
+    __device__ __forceinline__ void begin(const AttendArgs& a, const Segment& s, uint32_t ring) {
       const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+      if constexpr (!kQShared) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n) load_q(a, s, n * 8 + g, q[n]);
+        for (int n = 0; n < NT; ++n) load_q(a, s, n * 8 + g, q[n]);
+      }
       least_high = least_low = 0x7fffffff;
       most_low = most_high = 0;
       unseen = (1u << (2 * NT)) - 1u;
@@ -446,7 +454,15 @@ struct Attend {
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const float up = convert_q(a, q[n]);
+        constexpr int kOne = kQShared ? 0 : NT;
+        uint32_t(&mine)[2 * kKWords] = q[n < kOne ? n : 0];
+        if constexpr (kQShared) load_q(a, s, n * 8 + g, mine);
+        const float up = convert_q(a, mine);
+        if constexpr (kQShared) {  // each lane reads what it writes
+#pragma unroll
+          for (int w = 0; w < kKWords; ++w)
+            asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(ring + S * kStage + (n * kKWords + w) * 256 + lane * 8), "r"(mine[2 * w]), "r"(mine[2 * w + 1]) : "memory");
+        }
 #pragma unroll
         for (int i = 0; i < 2; ++i) factor[n][i] = a.scale_log2 * __shfl_sync(0xffffffffu, up, (2 * c + i) * 4);
       }
@@ -484,16 +500,17 @@ struct Attend {
     }
 
     // The unit of tokens base.. of segment s in the stage at `at`.
-    __device__ __forceinline__ void add(const AttendArgs& a, const Segment& s, int base, uint32_t at, bool good) {
+    __device__ __forceinline__ void add(const AttendArgs& a, const Segment& s, int base, uint32_t at, uint32_t ring, bool good) {
       const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
       float k_scale, v_scale;
       asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(k_scale), "=f"(v_scale) : "r"(at + kScales));
-      // Scores: [16 tokens][8 rows] for each tile of rows, in two chains.
-      float sc[NT][4], sd[NT][4];
+      // Scores: [16 tokens][8 rows] for each tile of rows, one tile in two chains.
+      constexpr int kChains = NT == 1 ? 2 : 1;
+      float sc[NT][4], sd[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[n][i] = sd[n][i] = 0.f;
+        for (int i = 0; i < 4; ++i) sc[n][i] = 0.f;
       const uint32_t at_k = at + place(g, D == 64 ? c : 2 * c);
 #pragma unroll
       for (int part = 0; part < kKWords / 4; ++part) {
@@ -507,7 +524,16 @@ struct Attend {
           codes_to_half<E4M3>(k0[w], a0, a2);
           codes_to_half<E4M3>(k1[w], a1, a3);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma16816(w & 1 ? sd[n] : sc[n], a0, a1, a2, a3, q[n][8 * part + 2 * w], q[n][8 * part + 2 * w + 1]);
+          for (int n = 0; n < NT; ++n) {
+            uint32_t b[2];
+            if constexpr (kQShared) {
+              lds_words<2>(ring + S * kStage + (n * kKWords + 4 * part + w) * 256 + lane * 8, b);
+            } else {
+              b[0] = q[n][8 * part + 2 * w];
+              b[1] = q[n][8 * part + 2 * w + 1];
+            }
+            mma16816(kChains == 2 && (w & 1) ? sd : sc[n], a0, a1, a2, a3, b[0], b[1]);
+          }
         }
       }
       const float v_now = v_scale < kLeastScale ? kLeastScale : v_scale;
@@ -518,7 +544,7 @@ struct Attend {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[n][i] = fmaf(sc[n][i] + sd[n][i], factor[n][i & 1] * k_scale, v_log2 - m[n][i & 1]);
+        for (int i = 0; i < 4; ++i) sc[n][i] = fmaf(kChains == 2 ? sc[n][i] + sd[i] : sc[n][i], factor[n][i & 1] * k_scale, v_log2 - m[n][i & 1]);
       }
       const bool edge = base + kUnit > least_high || base < most_low || !good;  // the same in all lanes
       if (edge) {
@@ -747,14 +773,14 @@ struct Attend {
       for (int u = u0;;) {
         const int from = max(0, u - s.begin), to = min(s.units, u1 - s.begin);
         if (to <= 0) break;  // only the segment's start is this warp's
-        rows.begin(a, s);
+        rows.begin(a, s, ring);
         int base = (s.unit0 + from) * kUnit;
 #pragma unroll 1
         for (int i = from; i < to; ++i) {
           copy_wait<S - 2>();
           __syncwarp();  // the unit is there for all lanes, and the stage before it has been read by all
           feed.next(a, prefix, sh.fed[warp], freed, freed_stage);
-          rows.add(a, s, base, ring + offset, !(feed.hidden >> stage & 1));
+          rows.add(a, s, base, ring + offset, ring, !(feed.hidden >> stage & 1));
           base += kUnit;
           freed = offset;
           freed_stage = stage;
@@ -890,7 +916,7 @@ struct Attend {
       auto part = [&](int c) { return a.partials + (long long)(c * 2 + (c == c0 ? 1 : 0)) * kPartFloats; };
       // A warp's rows go together and several parts at a time, so that their
       // loads overlap: the parts are in L2, a latency away.
-      constexpr int R = kRows / W, U = 8 / R;
+      constexpr int R = kRows / W, U = R < 8 ? 8 / R : 1;
       float x[R][kLane], l[R], m[R];
 #pragma unroll
       for (int i = 0; i < R; ++i) {
@@ -947,18 +973,32 @@ __global__ void __launch_bounds__(W * 32, MINB) k_attend(const __grid_constant__
 
 // Warps of a CTA, stages of a warp's ring and CTAs of an SM for each head size
 // and number of row tiles: what the registers of the rows leave (q D/8 and o
-// D/4 for each tile), and rings of about 190 KB an SM.
+// D/4 for each tile), and up to 200 KB of rings an SM.
 template <int D, int NT>
 struct Shape;
 template <> struct Shape<64, 1> { static constexpr int W = 8, S = 4, MINB = 3; };
 template <> struct Shape<64, 2> { static constexpr int W = 8, S = 4, MINB = 2; };
+template <> struct Shape<64, 4> { static constexpr int W = 4, S = 4, MINB = 3; };
 template <> struct Shape<128, 1> { static constexpr int W = 8, S = 3, MINB = 2; };
 template <> struct Shape<128, 2> { static constexpr int W = 4, S = 4, MINB = 3; };
+template <> struct Shape<128, 3> { static constexpr int W = 4, S = 3, MINB = 2; };
+template <> struct Shape<128, 4> { static constexpr int W = 4, S = 3, MINB = 2; };
 template <> struct Shape<256, 1> { static constexpr int W = 4, S = 3, MINB = 2; };
+template <> struct Shape<256, 2> { static constexpr int W = 4, S = 2, MINB = 2; };
 
+// The workspace: a counter for each CTA that can run at once (in the same place
+// for every shape: they stay zero between calls), two parts of its segments,
+// and an early part for each of its warps.
+struct Workspace {
+  size_t counters, partials, early;  // bytes
+};
 template <int D, int NT>
-constexpr size_t early_bytes(int sms) {
-  return (size_t)sms * Shape<D, NT>::MINB * Shape<D, NT>::W * 8 * NT * D * sizeof(float);
+Workspace workspace_of(int sms) {
+  using P = Shape<D, NT>;
+  const size_t ctas = (size_t)sms * P::MINB, rows = 8 * NT;
+  static_assert(P::MINB <= 4, "the counters' room");
+  return {((size_t)sms * 4 * sizeof(int) + 255) / 256 * 256, (ctas * 2 * rows * (D + 2) * sizeof(float) + 255) / 256 * 256,
+          ctas * P::W * rows * D * sizeof(float)};
 }
 
 template <int D, int NT, bool E4M3, bool PACKED>
@@ -967,6 +1007,10 @@ dk_status launch(AttendArgs a, cudaStream_t stream) {
   using A = Attend<D, NT, E4M3, PACKED, W, S>;
   const size_t smem = sizeof(typename A::Shared) + sizeof(int) * (size_t)(std::min(a.requests, kMaxRequests) + 1);
   auto kernel = k_attend<D, NT, E4M3, PACKED, W, S, MINB>;
+  const Workspace w = workspace_of<D, NT>(sm_count(-1));
+  a.counters = static_cast<int*>(a.workspace);
+  a.partials = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + w.counters);
+  a.early = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + w.counters + w.partials);
   static thread_local unsigned long long prepared = 0;  // devices whose limit is set
   const int device = current_device();
   if (device >= 64 || !(prepared >> device & 1)) {
@@ -1010,10 +1054,13 @@ dk_status launch(AttendArgs a, cudaStream_t stream) {
   return DK_OK;
 }
 
-// Row tiles of 16 where a KV head has more than 8 query rows: one pass over
-// the cache for 16 rows.  Heads of 256 keep tiles of 8 (the fragments of 16
-// rows do not fit the registers).
-int row_tiles(int head_dim, long long rows) { return head_dim < 256 && rows > 8 ? 2 : 1; }
+// Tiles of eight rows that one pass over the cache serves: as many as a KV
+// head's query rows fill, within what the registers hold.
+int row_tiles(int head_dim, long long rows) {
+  if (rows <= 8) return 1;
+  if (rows <= 16 || head_dim == 256) return 2;
+  return head_dim == 128 && (rows <= 24 || (rows > 32 && rows <= 48)) ? 3 : 4;
+}
 
 template <int D, int NT>
 dk_status launch_code(const AttendArgs& a, bool e4m3, cudaStream_t stream) {
@@ -1028,16 +1075,12 @@ dk_status launch_code(const AttendArgs& a, bool e4m3, cudaStream_t stream) {
 using namespace dk;
 
 extern "C" size_t dk_cache_attention_workspace_bytes(int head_dim) {
-  // Counters, two parts of up to 16 rows for each CTA that can run at once, and
-  // an early part for each of its warps.
-  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return 0;
   const int sms = sm_count(-1);
-  const size_t ctas = (size_t)sms * 3;
-  const size_t counters = (ctas * sizeof(int) + 255) / 256 * 256;
-  const size_t early = head_dim == 64    ? std::max(early_bytes<64, 1>(sms), early_bytes<64, 2>(sms))
-                       : head_dim == 128 ? std::max(early_bytes<128, 1>(sms), early_bytes<128, 2>(sms))
-                                         : early_bytes<256, 1>(sms);
-  return counters + ctas * 2 * 16 * (size_t)(head_dim + 2) * sizeof(float) + early;
+  auto all = [](const Workspace& w) { return w.counters + w.partials + w.early; };
+  if (head_dim == 64) return std::max(all(workspace_of<64, 2>(sms)), all(workspace_of<64, 4>(sms)));
+  if (head_dim == 128) return std::max(all(workspace_of<128, 2>(sms)), all(workspace_of<128, 4>(sms)));
+  if (head_dim == 256) return all(workspace_of<256, 2>(sms));
+  return 0;
 }
 
 extern "C" dk_status dk_cache_attention(const dk_cache_attention_args* p, void* workspace,
@@ -1086,10 +1129,7 @@ extern "C" dk_status dk_cache_attention(const dk_cache_attention_args* p, void* 
   a.starts = p->starts;
   a.out = p->out;
   a.lse = p->lse;
-  const size_t ctas = (size_t)sm_count(-1) * 3;
-  a.counters = static_cast<int*>(workspace);
-  a.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + (ctas * sizeof(int) + 255) / 256 * 256);
-  a.early = a.partials + ctas * 2 * 16 * (size_t)(c.head_dim + 2);
+  a.workspace = workspace;
   a.q_token_stride = p->q_token_stride;
   a.q_head_stride = p->q_head_stride;
   a.k_block_stride = (uint32_t)c.k_block_stride;
@@ -1115,7 +1155,15 @@ extern "C" dk_status dk_cache_attention(const dk_cache_attention_args* p, void* 
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool e4m3 = c.code == DK_E4M3;
   const int nt = row_tiles(c.head_dim, ((long long)p->tokens + p->requests - 1) / p->requests * group);
-  if (c.head_dim == 64) return nt == 1 ? launch_code<64, 1>(a, e4m3, st) : launch_code<64, 2>(a, e4m3, st);
-  if (c.head_dim == 128) return nt == 1 ? launch_code<128, 1>(a, e4m3, st) : launch_code<128, 2>(a, e4m3, st);
-  return launch_code<256, 1>(a, e4m3, st);
+  switch (c.head_dim * 8 + nt) {
+    case 64 * 8 + 1: return launch_code<64, 1>(a, e4m3, st);
+    case 64 * 8 + 2: return launch_code<64, 2>(a, e4m3, st);
+    case 64 * 8 + 4: return launch_code<64, 4>(a, e4m3, st);
+    case 128 * 8 + 1: return launch_code<128, 1>(a, e4m3, st);
+    case 128 * 8 + 2: return launch_code<128, 2>(a, e4m3, st);
+    case 128 * 8 + 3: return launch_code<128, 3>(a, e4m3, st);
+    case 128 * 8 + 4: return launch_code<128, 4>(a, e4m3, st);
+    case 256 * 8 + 1: return launch_code<256, 1>(a, e4m3, st);
+    default: return launch_code<256, 2>(a, e4m3, st);
+  }
 }

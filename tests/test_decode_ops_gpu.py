@@ -434,6 +434,28 @@ def test_attention_several_queries(code, dtype, hq, kv, dim, bs):
     check_attention(attention_case(lengths, fresh, hq, kv, dim, bs, code, dtype, seed=5), causal=False)
 
 
+@pytest.mark.parametrize("hq,kv,dim", [(8, 4, 128), (8, 2, 128), (6, 1, 128), (16, 2, 128), (3, 1, 64), (12, 2, 64), (2, 1, 256), (4, 1, 256)])
+@pytest.mark.parametrize("code,dtype", [("int8", "fp16"), ("e4m3", "bf16")])
+def test_attention_drafts(hq, kv, dim, code, dtype):
+    # Five queries for each request: 10 to 40 rows for a KV head, one to several tiles of each width.
+    lengths = [5, 6, 16, 20, 21, 133, 1000, 5]
+    check_attention(attention_case(lengths, [5] * 8, hq, kv, dim, 32, code, dtype, seed=hq))
+    check_attention(attention_case(lengths, [5] * 8, hq, kv, dim, 16, code, dtype, seed=hq), window=9)
+    check_attention(attention_case([9000, 3000], [5, 5], hq, kv, dim, 64, code, dtype, seed=hq))
+
+
+def test_attention_shapes_share_a_workspace():
+    # Kernels of several row tiles take turns on one stream's workspace; what one writes must not reach another's counters.
+    one = attention_case([5000, 7000, 30], None, 8, 2, 128, 64, "int8", "fp16")
+    many = attention_case([5000, 7000, 30], [5, 5, 5], 8, 2, 128, 64, "int8", "fp16")
+    more = attention_case([5000, 7000], [40, 9], 8, 2, 128, 64, "int8", "fp16")
+    want = [run_attention(c)[0] for c in (one, many, more)]
+    for _ in range(5):
+        for c, w in zip((one, many, more), want):
+            assert torch.equal(run_attention(c)[0], w)
+    check_attention(one), check_attention(many), check_attention(more)
+
+
 @pytest.mark.parametrize("window", [1, 15, 16, 17, 100])
 def test_attention_window(window):
     check_attention(attention_case(EDGES, None, 8, 2, 128, 16, "int8", "fp16", seed=window), window=window)
