@@ -184,6 +184,7 @@ struct Attend {
     unsigned char ring[W][kWarp];  // stages and queries; at the end the warp's last part: float [kRows][D]
     float m[kSlots][kRows];
     float l[kSlots][kRows];
+    float top[kSlots][kRows];
     Segment seg[kSlots];
     Segment fed[W], now[W];            // the segments whose units a warp copies and adds up
     int used[kSlots];
@@ -640,67 +641,23 @@ struct Attend {
       }
   }
 
-  // A row that a warp holds, lane by lane D / 32 channels, to its place.
-  __device__ static __forceinline__ void finish_row(const AttendArgs& a, const Segment& s, int row, const float (&x)[D / 32], float m, float l) {
-    const int lane = threadIdx.x & 31;
+  // Channels d..d+3 of a joined row to their place.
+  __device__ static __forceinline__ void finish_row(const AttendArgs& a, const Segment& s, int row, int d, const float4& x, float m, float l) {
     int token, head, low, high;
     if (!row_of(a, s, row, token, head, low, high)) return;
     const float f = l > 0.f || l != l ? 1.f / l : 0.f;
     const long long at = (long long)token * a.kv_heads * a.group + head;
-    if constexpr (D == 64) {
-      uint32_t w;
-      if (a.bf16) {
-        const __nv_bfloat162 p = __floats2bfloat162_rn(x[0] * f, x[1] * f);
-        w = *reinterpret_cast<const uint32_t*>(&p);
-      } else {
-        w = pack_half2(x[0] * f, x[1] * f);
-      }
-      *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + at * D + lane * 2) = w;
-    } else {
-#pragma unroll
-      for (int d = 0; d < D / 128; ++d)
-        store_row(a, at * D + lane * (D / 32) + 4 * d, make_float4(x[4 * d] * f, x[4 * d + 1] * f, x[4 * d + 2] * f, x[4 * d + 3] * f));
-    }
-    if (a.lse && lane == 0) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+    store_row(a, at * D + d, make_float4(x.x * f, x.y * f, x.z * f, x.w * f));
+    if (a.lse && d == 0) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
   }
 
-  static constexpr int kPartFloats = kRows * (D + 2);
-  static constexpr int kLane = D / 32;  // channels of a lane where a warp holds a row
+  static constexpr int kPartFloats = kRows * (D + 2);  // o, m, l of a CTA's part
 
-  __device__ static __forceinline__ void store_part(float* p, const float (&x)[kLane]) {
-    if constexpr (kLane == 2) {
-      __stcg(reinterpret_cast<float2*>(p), make_float2(x[0], x[1]));
-    } else {
-#pragma unroll
-      for (int d = 0; d < kLane; d += 4) __stcg(reinterpret_cast<float4*>(p + d), make_float4(x[d], x[d + 1], x[d + 2], x[d + 3]));
-    }
-  }
-  template <bool GLOBAL>
-  __device__ static __forceinline__ void load_part(const float* p, float (&y)[kLane]) {
-    if constexpr (kLane == 2) {
-      const float2 v = GLOBAL ? __ldcg(reinterpret_cast<const float2*>(p)) : *reinterpret_cast<const float2*>(p);
-      y[0] = v.x; y[1] = v.y;
-    } else {
-#pragma unroll
-      for (int d = 0; d < kLane; d += 4) {
-        const float4 v = GLOBAL ? __ldcg(reinterpret_cast<const float4*>(p + d)) : *reinterpret_cast<const float4*>(p + d);
-        y[d] = v.x; y[d + 1] = v.y; y[d + 2] = v.z; y[d + 3] = v.w;
-      }
-    }
-  }
-  __device__ static __forceinline__ void add_part(const float (&y)[kLane], float f, float (&x)[kLane]) {
-#pragma unroll
-    for (int d = 0; d < kLane; ++d) x[d] = fmaf(y[d], f, x[d]);
-  }
-  __device__ static __forceinline__ float warp_max(float x) {
-#pragma unroll
-    for (int d = 16; d; d >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-    return x;
-  }
-  __device__ static __forceinline__ float warp_sum(float x) {
-#pragma unroll
-    for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-    return x;
+  __device__ static __forceinline__ void add_part(const float4& y, float f, float4& x) {
+    x.x = fmaf(y.x, f, x.x);
+    x.y = fmaf(y.y, f, x.y);
+    x.z = fmaf(y.z, f, x.z);
+    x.w = fmaf(y.w, f, x.w);
   }
 
   __device__ static void run(const AttendArgs& a, Shared& sh, int* prefix) {
@@ -830,8 +787,9 @@ struct Attend {
     }
     __syncthreads();
 
-    // Parts of one segment are neighbours among the used slots: a group.  Each
-    // of its rows is joined by one warp.
+    // Parts of one segment are neighbours among the used slots: a group.  This
+    // code runs once a call, and fetching it costs more than running it: loops
+    // are short and few.
     const int used = lane < kSlots ? sh.used[lane] : 0;
     const uint32_t valid = __ballot_sync(0xffffffffu, used);
     if (valid == 0) return;
@@ -839,48 +797,61 @@ struct Attend {
     const uint32_t below = valid & ((1u << lane) - 1u);
     const int prev = __shfl_sync(0xffffffffu, begin, below ? 31 - __clz(below) : 0);
     const uint32_t heads = __ballot_sync(0xffffffffu, used && (below == 0 || prev != begin));
-    for (int item = warp; item < __popc(heads) * kRows; item += W) {
-      const int row = item % kRows;
-      uint32_t h = heads;
-      for (int i = item / kRows; i; --i) h &= h - 1;
-      const int first = __ffs(h) - 1;
-      h &= h - 1;
-      const uint32_t members = valid & ~((1u << first) - 1u) & (h ? (h & -h) - 1u : 0xffffffffu);
-      const bool mine = members >> lane & 1;
-      const float part_m = mine ? sh.m[lane][row] : kFarBelow;
-      const float top = warp_max(part_m);
-      const float f = mine ? exp2_approx(part_m - top) : 0.f;
-      const float l = warp_sum(mine ? f * sh.l[lane][row] : 0.f);
-      float x[kLane];
-#pragma unroll
-      for (int d = 0; d < kLane; ++d) x[d] = 0.f;
-      // Few instructions: this code runs once a call, and fetching it costs
-      // more than running it.
+    auto members_of = [&](uint32_t left) {  // of the group of left's lowest bit
+      const uint32_t after = left & (left - 1);
+      return valid & ~((left & -left) - 1u) & (after ? (after & -after) - 1u : 0xffffffffu);
+    };
+    // Each row's maximum and sum over its group; m becomes the part's factor.
+    int turn = 0;
 #pragma unroll 1
-      for (uint32_t left = members; left;) {
-        float y[4][kLane], by[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {  // past the last: the first again, times 0
-          const int slot = left ? __ffs(left) - 1 : first;
-          const float* part = slot & 1 ? reinterpret_cast<const float*>(sh.ring[slot >> 1]) : a.early + (long long)(cta * W + (slot >> 1)) * kRows * D;
-          load_part<false>(part + row * D + lane * kLane, y[k]);
-          by[k] = __shfl_sync(0xffffffffu, f, slot);
-          if (!left) by[k] = 0.f;
-          left &= left - 1;
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) add_part(y[k], by[k], x);
+    for (uint32_t left = heads; left; left &= left - 1, ++turn) {
+      if (turn % W != warp || lane >= kRows) continue;
+      const int first = __ffs(left) - 1;
+      const uint32_t members = members_of(left);
+      float top = kFarBelow, l = 0.f;
+      for (uint32_t b = members; b; b &= b - 1) top = fmaxf(top, sh.m[__ffs(b) - 1][lane]);
+      for (uint32_t b = members; b; b &= b - 1) {
+        const int slot = __ffs(b) - 1;
+        const float f = exp2_approx(sh.m[slot][lane] - top);
+        l = fmaf(f, sh.l[slot][lane], l);
+        sh.m[slot][lane] = f;
       }
+      sh.top[first][lane] = top;
+      sh.l[first][lane] = l;
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (uint32_t left = heads; left; left &= left - 1) {
+      const int first = __ffs(left) - 1;
+      const uint32_t members = members_of(left);
       const Segment& s = sh.seg[first];
-      if (s.begin >= cta0 && s.begin + s.units <= cta1) {
-        finish_row(a, s, row, x, top, l);
-      } else {
-        float* part = a.partials + (long long)(cta * 2 + (s.begin >= cta0 ? 1 : 0)) * kPartFloats;
-        store_part(part + row * D + lane * kLane, x);
-        if (lane == 0) {
-          __stcg(part + kRows * D + row, top);
-          __stcg(part + kRows * D + kRows + row, l);
+      const bool whole = s.begin >= cta0 && s.begin + s.units <= cta1;
+      float* part = a.partials + (long long)(cta * 2 + (s.begin >= cta0 ? 1 : 0)) * kPartFloats;
+#pragma unroll 1
+      for (int e = tid; e < kRows * D / 4; e += W * 32) {
+        const int row = e / (D / 4), d = e % (D / 4) * 4;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+        for (uint32_t b = members; b;) {
+          float4 y[4];
+          float f[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {  // past the last: the first again, times 0
+            const int slot = b ? __ffs(b) - 1 : first;
+            const float* from = slot & 1 ? reinterpret_cast<const float*>(sh.ring[slot >> 1]) : a.early + (long long)(cta * W + (slot >> 1)) * kRows * D;
+            y[k] = *reinterpret_cast<const float4*>(from + row * D + d);
+            f[k] = b ? sh.m[slot][row] : 0.f;
+            b &= b - 1;
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) add_part(y[k], f[k], x);
         }
+        if (whole) finish_row(a, s, row, d, x, sh.top[first][row], sh.l[first][row]);
+        else __stcg(reinterpret_cast<float4*>(part + row * D + d), x);
+      }
+      if (!whole && tid < kRows) {
+        __stcg(part + kRows * D + tid, sh.top[first][tid]);
+        __stcg(part + kRows * D + kRows + tid, sh.l[first][tid]);
       }
     }
     // The CTA's first and last segments may be shared with others: the last CTA
@@ -909,57 +880,58 @@ struct Attend {
       sh.last[tid] = last;
     }
     __syncthreads();
-    for (int e = 0; e < ends; ++e) {
-      if (!sh.last[e]) continue;
-      const Segment& s = sh.seg[end_slot[e]];
-      const int c0 = s.begin / chunk, c1 = (s.begin + s.units - 1) / chunk;
-      auto part = [&](int c) { return a.partials + (long long)(c * 2 + (c == c0 ? 1 : 0)) * kPartFloats; };
-      // A warp's rows go together and several parts at a time, so that their
-      // loads overlap: the parts are in L2, a latency away.
-      constexpr int R = kRows / W, U = R < 8 ? 8 / R : 1;
-      float x[R][kLane], l[R], m[R];
-#pragma unroll
-      for (int i = 0; i < R; ++i) {
-        m[i] = kFarBelow;
-        l[i] = 0.f;
-#pragma unroll
-        for (int d = 0; d < kLane; ++d) x[i][d] = 0.f;
-      }
 #pragma unroll 1
-      for (int base = c0; base <= c1; base += 32) {
-        const int c = base + lane;
-        const float* mine = part(min(c, c1)) + kRows * D + warp * R;
-        float f[R];
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-          const float part_m = __ldcg(mine + i), part_l = __ldcg(mine + kRows + i);
-          const float top = fmaxf(m[i], warp_max(part_m));
-          const float scale = exp2_approx(m[i] - top);
-          m[i] = top;
-          f[i] = exp2_approx(part_m - top);
-          l[i] = l[i] * scale + (c <= c1 ? f[i] * part_l : 0.f);
-#pragma unroll
-          for (int d = 0; d < kLane; ++d) x[i][d] *= scale;
-        }
-        const int n = min(32, c1 - base + 1);
-#pragma unroll 1
-        for (int j = 0; j < n; j += U) {
-          float y[U][R][kLane];
-#pragma unroll
-          for (int k = 0; k < U; ++k)
-#pragma unroll
-            for (int i = 0; i < R; ++i) load_part<true>(part(min(base + j + k, c1)) + (warp * R + i) * D + lane * kLane, y[k][i]);
-#pragma unroll
-          for (int k = 0; k < U; ++k)
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-              const float g = __shfl_sync(0xffffffffu, f[i], j + k);
-              add_part(y[k][i], j + k < n ? g : 0.f, x[i]);
-            }
+    for (int end = 0; end < ends; ++end) {
+      if (!sh.last[end]) continue;
+      const Segment& s = sh.seg[end_slot[end]];
+      const int c0 = s.begin / chunk, n = (s.begin + s.units - 1) / chunk - c0 + 1;
+      auto part = [&](int i) { return a.partials + (long long)((c0 + i) * 2 + (i == 0 ? 1 : 0)) * kPartFloats; };
+      // The parts' factors in place of the rings: a lane has a row, and the
+      // lanes and warps beyond the rows other parts.
+      constexpr int P = 32 / kRows, G = W * P;
+      float* factor = reinterpret_cast<float*>(sh.ring);  // [n][kRows]
+      float* tops = factor + n * kRows;                   // [G][kRows]
+      float* sums = tops + G * kRows;                     // [G][kRows]
+      const int row = lane % kRows, mine = warp * P + lane / kRows;
+      const bool busy = lane < P * kRows;
+      float top = kFarBelow, l = 0.f;
+#pragma unroll 4
+      for (int i = mine; i < n; i += G)
+        if (busy) top = fmaxf(top, __ldcg(part(i) + kRows * D + row));
+      if (busy) tops[mine * kRows + row] = top;
+      __syncthreads();
+#pragma unroll 4
+      for (int i = 0; i < G; ++i) top = fmaxf(top, tops[i * kRows + row]);
+#pragma unroll 4
+      for (int i = mine; i < n; i += G) {
+        if (busy) {
+          const float f = exp2_approx(__ldcg(part(i) + kRows * D + row) - top);
+          l = fmaf(f, __ldcg(part(i) + kRows * D + kRows + row), l);
+          factor[i * kRows + row] = f;
         }
       }
+      if (busy) sums[mine * kRows + row] = l;
+      __syncthreads();
+#pragma unroll 1
+      for (int e = tid; e < kRows * D / 4; e += W * 32) {
+        const int r = e / (D / 4), d = e % (D / 4) * 4;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+        for (int i = 0; i < n; i += 8) {
+          float4 y[8];
 #pragma unroll
-      for (int i = 0; i < R; ++i) finish_row(a, s, warp * R + i, x[i], m[i], warp_sum(l[i]));
+          for (int k = 0; k < 8; ++k) y[k] = __ldcg(reinterpret_cast<const float4*>(part(min(i + k, n - 1)) + r * D + d));
+#pragma unroll
+          for (int k = 0; k < 8; ++k) add_part(y[k], i + k < n ? factor[(i + k) * kRows + r] : 0.f, x);
+        }
+        float m = kFarBelow, sum = 0.f;
+        for (int i = 0; i < G; ++i) {
+          m = fmaxf(m, tops[i * kRows + r]);
+          sum += sums[i * kRows + r];
+        }
+        finish_row(a, s, r, d, x, m, sum);
+      }
+      __syncthreads();  // before the other end takes the rings' place
     }
   }
 };
