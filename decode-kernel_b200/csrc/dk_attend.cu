@@ -950,13 +950,13 @@ template <int D, int NT>
 struct Shape;
 template <> struct Shape<64, 1> { static constexpr int W = 8, S = 4, MINB = 3; };
 template <> struct Shape<64, 2> { static constexpr int W = 8, S = 4, MINB = 2; };
-template <> struct Shape<64, 4> { static constexpr int W = 4, S = 4, MINB = 3; };
+template <> struct Shape<64, 4> { static constexpr int W = 12, S = 4, MINB = 1; };
 template <> struct Shape<128, 1> { static constexpr int W = 8, S = 3, MINB = 2; };
-template <> struct Shape<128, 2> { static constexpr int W = 4, S = 4, MINB = 3; };
-template <> struct Shape<128, 3> { static constexpr int W = 4, S = 3, MINB = 2; };
-template <> struct Shape<128, 4> { static constexpr int W = 4, S = 3, MINB = 2; };
+template <> struct Shape<128, 2> { static constexpr int W = 12, S = 4, MINB = 1; };
+template <> struct Shape<128, 3> { static constexpr int W = 8, S = 3, MINB = 1; };
+template <> struct Shape<128, 4> { static constexpr int W = 8, S = 3, MINB = 1; };
 template <> struct Shape<256, 1> { static constexpr int W = 4, S = 3, MINB = 2; };
-template <> struct Shape<256, 2> { static constexpr int W = 4, S = 2, MINB = 2; };
+template <> struct Shape<256, 2> { static constexpr int W = 8, S = 2, MINB = 1; };
 
 // The workspace: a counter for each CTA that can run at once (in the same place
 // for every shape: they stay zero between calls), two parts of its segments,
