@@ -47,7 +47,8 @@ namespace dk {
 namespace {
 
 constexpr int kUnit = 16;             // tokens of a unit
-constexpr int kMaxRequests = 2048;    // requests of one launch (their prefix sums are in shared memory)
+constexpr int kMaxRequests = 1024;    // requests of one launch (their prefix sums are in shared memory)
+constexpr int kShort = 96;             // places of segments that no two CTAs share
 constexpr float kFarBelow = -1e30f;   // maximum of a row that has seen no token
 constexpr float kSlack = 8.f;         // a row's maximum may lag its scores by this much (log2)
 constexpr float kLeastScale = 8.4703294725430034e-22f;  // 2^-70: keeps sum w / vs finite
@@ -189,7 +190,8 @@ struct Attend {
     Segment fed[W], now[W];            // the segments whose units a warp copies and adds up
     int used[kSlots];
     int last[2];
-    int total[W];
+    int total[W], longest[W];
+    int range[2];
   };
 
   // Place of 16-byte piece p of a unit's row: the pieces that eight lanes read
@@ -220,11 +222,16 @@ struct Attend {
   __device__ static __forceinline__ int tiles_of(const AttendArgs& a, int fresh) {
     return (fresh * a.group + kRows - 1) / kRows;
   }
-  __device__ static __forceinline__ void request_of(const AttendArgs& a, int r, int& length, int& fresh, int& first) {
-    length = min(max(ld_int(a.lengths + r), 0), (int)min((long long)a.max_blocks * a.block_size, 0x7fffffffLL));
+  // The requests' numbers in shared memory: prefix[r] = the place of request
+  // r's first unit in the line (one more entry than requests), then the tokens
+  // that each holds, and if there are starts those (again one more).
+  __device__ static __forceinline__ void request_of(const AttendArgs& a, const int* prefix, int r, int& length, int& fresh, int& first) {
+    const int* lengths = prefix + a.requests + 1;
+    length = lengths[r];
     if (a.starts) {
-      first = ld_int(a.starts + r);
-      fresh = max(0, ld_int(a.starts + r + 1) - first);
+      const int* starts = lengths + a.requests;
+      first = starts[r];
+      fresh = max(0, starts[r + 1] - first);
     } else {
       first = r;
       fresh = 1;
@@ -235,7 +242,7 @@ struct Attend {
   __device__ static __forceinline__ Segment segment_of(const AttendArgs& a, const int* prefix, int r, int which) {
     Segment s;
     s.request = r;
-    request_of(a, r, s.length, s.fresh, s.first_token);
+    request_of(a, prefix, r, s.length, s.fresh, s.first_token);
     s.units = units_of(a, s.length, s.fresh, s.unit0);
     s.which = which;
     s.begin = prefix[r] + which * (s.units + kStart) + kStart;
@@ -664,16 +671,28 @@ struct Attend {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_trigger();
     pdl_wait();
-    // Places of every request's units in the line: prefix[r] = the first of
-    // request r.
-    int carry = 0;
+    int* lengths = prefix + a.requests + 1;
+    int* starts = lengths + a.requests;
+    const int most = (int)min((long long)a.max_blocks * a.block_size, 0x7fffffffLL);
+    int carry = 0, longest = 0;
     for (int base = 0; base < a.requests; base += W * 32) {
       const int r = base + tid;
       int mine = 0;
       if (r < a.requests) {
-        int length, fresh, first, unit0;
-        request_of(a, r, length, fresh, first);
-        mine = (units_of(a, length, fresh, unit0) + kStart) * tiles_of(a, fresh) * a.kv_heads;
+        const int length = min(max(ld_int(a.lengths + r), 0), most);
+        int fresh = 1, unit0;
+        if (a.starts) {
+          const int first = ld_int(a.starts + r), next = ld_int(a.starts + r + 1);
+          fresh = max(0, next - first);
+          starts[r] = first;
+          if (r == a.requests - 1) starts[r + 1] = next;
+        }
+        lengths[r] = length;
+        if (fresh > 0) {
+          const int one = units_of(a, length, fresh, unit0) + kStart;
+          longest = max(longest, one);
+          mine = one * tiles_of(a, fresh) * a.kv_heads;
+        }
       }
       int sum = mine;
 #pragma unroll
@@ -681,7 +700,11 @@ struct Attend {
         const int x = __shfl_up_sync(0xffffffffu, sum, d);
         if (lane >= d) sum += x;
       }
-      if (lane == 31) sh.total[warp] = sum;
+      longest = __reduce_max_sync(0xffffffffu, longest);
+      if (lane == 31) {
+        sh.total[warp] = sum;
+        sh.longest[warp] = longest;
+      }
       __syncthreads();
       int before = carry, all = 0;
 #pragma unroll
@@ -689,6 +712,7 @@ struct Attend {
         const int x = sh.total[w];
         if (w < warp) before += x;
         all += x;
+        longest = max(longest, sh.longest[w]);
       }
       if (r < a.requests) prefix[r] = before + sum - mine;
       carry += all;
@@ -698,13 +722,33 @@ struct Attend {
     if (all == 0) return;
     if (tid == 0) prefix[a.requests] = all;
     __syncthreads();
-    // Every CTA has the same number of units (the last has the rest), one for
-    // each of its warps at least; CTA u / chunk has unit u.
+    // Every CTA has the same number of places (the last has the rest), one for
+    // each of its warps at least; CTA u / chunk has place u.  Where segments
+    // are short the borders move to the nearest segment's, so that no segment
+    // is shared between CTAs: joining one costs about as long as the units do
+    // that a CTA gets too many.  (64 requests of up to 200 tokens 15.6 -> 12.0
+    // us, of up to 1000 24.8 -> 21.6; from 2000 tokens on it makes no odds.)
     const int grid = min((int)gridDim.x, (all + W - 1) / W);
     const int chunk = (all + grid - 1) / grid;
     const int cta = blockIdx.x;
     if (cta >= grid || cta * chunk >= all) return;
-    const int cta0 = cta * chunk, cta1 = min(all, cta0 + chunk);
+    const bool snap = longest <= kShort;
+    int cta0 = cta * chunk, cta1 = min(all, cta0 + chunk);
+    if (snap) {
+      if (warp < 2) {
+        int x = warp ? cta1 : cta0;
+        if (x > 0 && x < all) {
+          const Segment s = segment_at(a, prefix, x);
+          const int from = s.begin - kStart, to = s.begin + s.units;
+          x = x - from <= to - x ? from : to;
+        }
+        if (lane == 0) sh.range[warp] = x;
+      }
+      __syncthreads();
+      cta0 = sh.range[0];
+      cta1 = sh.range[1];
+      if (cta0 >= cta1) return;
+    }
     const int u0 = cta0 + (cta1 - cta0) * warp / W, u1 = cta0 + (cta1 - cta0) * (warp + 1) / W;
     if (lane < 2) sh.used[2 * warp + lane] = 0;
     __syncwarp();
@@ -948,14 +992,14 @@ __global__ void __launch_bounds__(W * 32, MINB) k_attend(const __grid_constant__
 // D/4 for each tile), and up to 200 KB of rings an SM.
 template <int D, int NT>
 struct Shape;
-template <> struct Shape<64, 1> { static constexpr int W = 8, S = 4, MINB = 3; };
+template <> struct Shape<64, 1> { static constexpr int W = 8, S = 6, MINB = 2; };
 template <> struct Shape<64, 2> { static constexpr int W = 8, S = 4, MINB = 2; };
-template <> struct Shape<64, 4> { static constexpr int W = 12, S = 4, MINB = 1; };
-template <> struct Shape<128, 1> { static constexpr int W = 8, S = 3, MINB = 2; };
-template <> struct Shape<128, 2> { static constexpr int W = 12, S = 4, MINB = 1; };
+template <> struct Shape<64, 4> { static constexpr int W = 8, S = 4, MINB = 1; };
+template <> struct Shape<128, 1> { static constexpr int W = 8, S = 2, MINB = 2; };
+template <> struct Shape<128, 2> { static constexpr int W = 8, S = 3, MINB = 1; };
 template <> struct Shape<128, 3> { static constexpr int W = 8, S = 3, MINB = 1; };
 template <> struct Shape<128, 4> { static constexpr int W = 8, S = 3, MINB = 1; };
-template <> struct Shape<256, 1> { static constexpr int W = 4, S = 3, MINB = 2; };
+template <> struct Shape<256, 1> { static constexpr int W = 8, S = 2, MINB = 1; };
 template <> struct Shape<256, 2> { static constexpr int W = 8, S = 2, MINB = 1; };
 
 // The workspace: a counter for each CTA that can run at once (in the same place
@@ -977,7 +1021,10 @@ template <int D, int NT, bool E4M3, bool PACKED>
 dk_status launch(AttendArgs a, cudaStream_t stream) {
   constexpr int W = Shape<D, NT>::W, MINB = Shape<D, NT>::MINB, S = Shape<D, NT>::S;
   using A = Attend<D, NT, E4M3, PACKED, W, S>;
-  const size_t smem = sizeof(typename A::Shared) + sizeof(int) * (size_t)(std::min(a.requests, kMaxRequests) + 1);
+  const size_t per = (a.starts ? 3 : 2) * sizeof(int);  // of a request in shared memory
+  const size_t smem = sizeof(typename A::Shared) + per * (size_t)(std::min(a.requests, kMaxRequests) + 1);
+  static_assert(sizeof(typename A::Shared) + 3 * sizeof(int) * (kMaxRequests + 1) <= 227 * 1024,
+                "a CTA fits the shared memory");
   auto kernel = k_attend<D, NT, E4M3, PACKED, W, S, MINB>;
   const Workspace w = workspace_of<D, NT>(sm_count(-1));
   a.counters = static_cast<int*>(a.workspace);
@@ -986,7 +1033,7 @@ dk_status launch(AttendArgs a, cudaStream_t stream) {
   static thread_local unsigned long long prepared = 0;  // devices whose limit is set
   const int device = current_device();
   if (device >= 64 || !(prepared >> device & 1)) {
-    const size_t most = sizeof(typename A::Shared) + sizeof(int) * (kMaxRequests + 1);
+    const size_t most = sizeof(typename A::Shared) + 3 * sizeof(int) * (kMaxRequests + 1);
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
     if (e == cudaSuccess)
       e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
