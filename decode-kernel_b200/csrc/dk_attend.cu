@@ -185,7 +185,13 @@ struct Attend {
     unsigned char ring[W][kWarp];  // stages and queries; at the end the warp's last part: float [kRows][D]
     float m[kSlots][kRows];
     float l[kSlots][kRows];
-    float top[kSlots][kRows];
+    // Of the joins: a used slot's part and factors, a group's first part and the
+    // places of its rows.
+    const float* part[kSlots];
+    float factor[kSlots][kRows];
+    float by[kSlots][kRows];
+    int place[kSlots][kRows];
+    int group[kSlots + 1];
     Segment seg[kSlots];
     Segment fed[W], now[W];            // the segments whose units a warp copies and adds up
     int used[kSlots];
@@ -423,10 +429,9 @@ struct Attend {
 
     __device__ __forceinline__ void begin(const AttendArgs& a, const Segment& s, uint32_t ring) {
       const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-      if constexpr (!kQShared) {
+      uint32_t mine[NT][2 * kKWords];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) load_q(a, s, n * 8 + g, q[n]);
-      }
+      for (int n = 0; n < NT; ++n) load_q(a, s, n * 8 + g, mine[n]);
       least_high = least_low = 0x7fffffff;
       most_low = most_high = 0;
       unseen = (1u << (2 * NT)) - 1u;
@@ -446,10 +451,6 @@ struct Attend {
           m[n][i] = 0.f;
           l[n][i] = 0.f;
         }
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) o[n][i][j] = 0.f;
       }
       if (s.fresh == 1) {  // all rows are one query's
         least_high = most_high = s.length;
@@ -462,18 +463,25 @@ struct Attend {
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        constexpr int kOne = kQShared ? 0 : NT;
-        uint32_t(&mine)[2 * kKWords] = q[n < kOne ? n : 0];
-        if constexpr (kQShared) load_q(a, s, n * 8 + g, mine);
-        const float up = convert_q(a, mine);
-        if constexpr (kQShared) {  // each lane reads what it writes
+        const float up = convert_q(a, mine[n]);
 #pragma unroll
-          for (int w = 0; w < kKWords; ++w)
-            asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(ring + S * kStage + (n * kKWords + w) * 256 + lane * 8), "r"(mine[2 * w]), "r"(mine[2 * w + 1]) : "memory");
+        for (int w = 0; w < kKWords; ++w) {
+          if constexpr (kQShared) {  // each lane reads what it writes
+            asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(ring + S * kStage + (n * kKWords + w) * 256 + lane * 8), "r"(mine[n][2 * w]), "r"(mine[n][2 * w + 1]) : "memory");
+          } else {
+            q[n][2 * w] = mine[n][2 * w];
+            q[n][2 * w + 1] = mine[n][2 * w + 1];
+          }
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) factor[n][i] = a.scale_log2 * __shfl_sync(0xffffffffu, up, (2 * c + i) * 4);
       }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[n][i][j] = 0.f;
     }
 
     // Rescales to the columns' new maxima; sc holds scores less m.
@@ -648,14 +656,18 @@ struct Attend {
       }
   }
 
-  // Channels d..d+3 of a joined row to their place.
-  __device__ static __forceinline__ void finish_row(const AttendArgs& a, const Segment& s, int row, int d, const float4& x, float m, float l) {
+  // Where a joined row goes: its place among the rows of out (-1: the tile has
+  // no such row), and what its sums are multiplied by.
+  __device__ static __forceinline__ int row_place(const AttendArgs& a, const Segment& s, int row, float m, float l, float& by) {
+    by = l > 0.f || l != l ? 1.f / l : 0.f;
     int token, head, low, high;
-    if (!row_of(a, s, row, token, head, low, high)) return;
-    const float f = l > 0.f || l != l ? 1.f / l : 0.f;
-    const long long at = (long long)token * a.kv_heads * a.group + head;
-    store_row(a, at * D + d, make_float4(x.x * f, x.y * f, x.z * f, x.w * f));
-    if (a.lse && d == 0) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+    if (!row_of(a, s, row, token, head, low, high)) return -1;
+    const int at = token * a.kv_heads * a.group + head;
+    if (a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+    return at;
+  }
+  __device__ static __forceinline__ void store_joined(const AttendArgs& a, int place, int d, const float4& x, float by) {
+    if (place >= 0) store_row(a, (long long)place * D + d, make_float4(x.x * by, x.y * by, x.z * by, x.w * by));
   }
 
   static constexpr int kPartFloats = kRows * (D + 2);  // o, m, l of a CTA's part
@@ -841,141 +853,143 @@ struct Attend {
     const uint32_t below = valid & ((1u << lane) - 1u);
     const int prev = __shfl_sync(0xffffffffu, begin, below ? 31 - __clz(below) : 0);
     const uint32_t heads = __ballot_sync(0xffffffffu, used && (below == 0 || prev != begin));
-    auto members_of = [&](uint32_t left) {  // of the group of left's lowest bit
-      const uint32_t after = left & (left - 1);
-      return valid & ~((left & -left) - 1u) & (after ? (after & -after) - 1u : 0xffffffffu);
-    };
-    // Each row's maximum and sum over its group; m becomes the part's factor.
-    int turn = 0;
+    const int groups = __popc(heads), parts = __popc(valid);
+    auto numbered = [&](int slot) { return __popc(valid & ((1u << slot) - 1u)); };  // among the used
+    if (warp == 0 && used) {
+      sh.part[__popc(below)] =
+          lane & 1 ? reinterpret_cast<const float*>(sh.ring[lane >> 1]) : a.early + (long long)(cta * W + (lane >> 1)) * kRows * D;
+      if (heads >> lane & 1) sh.group[__popc(heads & ((1u << lane) - 1u))] = __popc(below);
+      if (lane == 31 - __clz(valid)) sh.group[groups] = parts;
+    }
+    // A group's rows, one a lane: their maxima, sums and parts' factors, and
+    // where they go.
+    uint32_t left = heads;
 #pragma unroll 1
-    for (uint32_t left = heads; left; left &= left - 1, ++turn) {
-      if (turn % W != warp || lane >= kRows) continue;
+    for (int i = 0; i < groups; ++i, left &= left - 1) {
+      if (i % W != warp || lane >= kRows) continue;
       const int first = __ffs(left) - 1;
-      const uint32_t members = members_of(left);
+      const uint32_t after = left & (left - 1);
+      const uint32_t members = valid & ~((left & -left) - 1u) & (after ? (after & -after) - 1u : 0xffffffffu);
       float top = kFarBelow, l = 0.f;
       for (uint32_t b = members; b; b &= b - 1) top = fmaxf(top, sh.m[__ffs(b) - 1][lane]);
       for (uint32_t b = members; b; b &= b - 1) {
         const int slot = __ffs(b) - 1;
         const float f = exp2_approx(sh.m[slot][lane] - top);
         l = fmaf(f, sh.l[slot][lane], l);
-        sh.m[slot][lane] = f;
+        sh.factor[numbered(slot)][lane] = f;
       }
-      sh.top[first][lane] = top;
-      sh.l[first][lane] = l;
+      const Segment& s = sh.seg[first];
+      if (s.begin >= cta0 && s.begin + s.units <= cta1) {
+        sh.place[i][lane] = row_place(a, s, lane, top, l, sh.by[i][lane]);
+      } else {  // a part of what several CTAs share
+        const int which = cta * 2 + (s.begin >= cta0 ? 1 : 0);
+        float* part = a.partials + (long long)which * kPartFloats;
+        __stcg(part + kRows * D + lane, top);
+        __stcg(part + kRows * D + kRows + lane, l);
+        sh.place[i][lane] = -2 - which;
+      }
     }
     __syncthreads();
+    constexpr int kQuads = kRows * D / 4;
 #pragma unroll 1
-    for (uint32_t left = heads; left; left &= left - 1) {
-      const int first = __ffs(left) - 1;
-      const uint32_t members = members_of(left);
-      const Segment& s = sh.seg[first];
-      const bool whole = s.begin >= cta0 && s.begin + s.units <= cta1;
-      float* part = a.partials + (long long)(cta * 2 + (s.begin >= cta0 ? 1 : 0)) * kPartFloats;
-#pragma unroll 1
-      for (int e = tid; e < kRows * D / 4; e += W * 32) {
-        const int row = e / (D / 4), d = e % (D / 4) * 4;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-        for (uint32_t b = members; b;) {
-          float4 y[4];
-          float f[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {  // past the last: the first again, times 0
-            const int slot = b ? __ffs(b) - 1 : first;
-            const float* from = slot & 1 ? reinterpret_cast<const float*>(sh.ring[slot >> 1]) : a.early + (long long)(cta * W + (slot >> 1)) * kRows * D;
-            y[k] = *reinterpret_cast<const float4*>(from + row * D + d);
-            f[k] = b ? sh.m[slot][row] : 0.f;
-            b &= b - 1;
-          }
-#pragma unroll
-          for (int k = 0; k < 4; ++k) add_part(y[k], f[k], x);
-        }
-        if (whole) finish_row(a, s, row, d, x, sh.top[first][row], sh.l[first][row]);
-        else __stcg(reinterpret_cast<float4*>(part + row * D + d), x);
-      }
-      if (!whole && tid < kRows) {
-        __stcg(part + kRows * D + tid, sh.top[first][tid]);
-        __stcg(part + kRows * D + kRows + tid, sh.l[first][tid]);
-      }
+    for (int e = tid; e < groups * kQuads; e += W * 32) {
+      const int i = e / kQuads, row = e % kQuads / (D / 4), d = e % (D / 4) * 4;
+      const int end = sh.group[i + 1];
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int k = sh.group[i]; k < end; ++k) add_part(*reinterpret_cast<const float4*>(sh.part[k] + row * D + d), sh.factor[k][row], x);
+      const int place = sh.place[i][row];
+      if (place >= -1) store_joined(a, place, d, x, sh.by[i][row]);
+      else __stcg(reinterpret_cast<float4*>(a.partials + (long long)(-2 - place) * kPartFloats + row * D + d), x);
     }
     // The CTA's first and last segments may be shared with others: the last CTA
     // to arrive joins the parts in the order of the CTAs.
+    if (snap) return;
     const int end_slot[2] = {__ffs(heads) - 1, 31 - __clz(heads)};
-    const int ends = end_slot[0] == end_slot[1] ? 1 : 2;
-    bool shared = false;
-    for (int e = 0; e < ends; ++e) {
-      const Segment& s = sh.seg[end_slot[e]];
-      shared |= !(s.begin >= cta0 && s.begin + s.units <= cta1);
-    }
-    if (!shared) return;
+    const int ends = groups == 1 ? 1 : 2;
     __syncthreads();
-    if (tid < ends) {
+    if (tid < 2) {
       const Segment& s = sh.seg[tid ? end_slot[1] : end_slot[0]];
       int last = 0;
-      if (!(s.begin >= cta0 && s.begin + s.units <= cta1)) {
+      if (tid < ends && !(s.begin >= cta0 && s.begin + s.units <= cta1)) {
         const int c0 = s.begin / chunk, c1 = (s.begin + s.units - 1) / chunk;
         // With the barrier: the whole CTA's parts are seen before the count,
         // and the others' parts by the CTA that counts last.
         int before;
         asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(a.counters + c0) : "memory");
-        last = before == c1 - c0;
-        if (last) a.counters[c0] = 0;
+        if (before == c1 - c0) {
+          last = c1 - c0 + 1;
+          a.counters[c0] = 0;
+        }
+        sh.range[tid] = c0;
       }
       sh.last[tid] = last;
     }
     __syncthreads();
+    const int n0 = sh.last[0], n1 = sh.last[1];  // parts to join, of the first and of the last segment
+    if (n0 + n1 == 0) return;
+    auto part = [&](int end, int i) { return a.partials + (long long)((sh.range[end] + i) * 2 + (i == 0 ? 1 : 0)) * kPartFloats; };
+    // The parts' factors in place of the rings: a lane has a row, and the lanes
+    // and warps beyond the rows other parts; then the rows' elements, of both
+    // segments together.
+    constexpr int P = 32 / kRows, G = W * P;
+    float* tops = reinterpret_cast<float*>(sh.ring);  // [2][G][kRows]
+    float* sums = tops + 2 * G * kRows;               // [2][G][kRows]
+    float* factor = sums + 2 * G * kRows;             // [n0 + n1][kRows]
+    const int row = lane % kRows, mine = warp * P + lane / kRows;
+    const bool busy = lane < P * kRows;
 #pragma unroll 1
-    for (int end = 0; end < ends; ++end) {
-      if (!sh.last[end]) continue;
-      const Segment& s = sh.seg[end_slot[end]];
-      const int c0 = s.begin / chunk, n = (s.begin + s.units - 1) / chunk - c0 + 1;
-      auto part = [&](int i) { return a.partials + (long long)((c0 + i) * 2 + (i == 0 ? 1 : 0)) * kPartFloats; };
-      // The parts' factors in place of the rings: a lane has a row, and the
-      // lanes and warps beyond the rows other parts.
-      constexpr int P = 32 / kRows, G = W * P;
-      float* factor = reinterpret_cast<float*>(sh.ring);  // [n][kRows]
-      float* tops = factor + n * kRows;                   // [G][kRows]
-      float* sums = tops + G * kRows;                     // [G][kRows]
-      const int row = lane % kRows, mine = warp * P + lane / kRows;
-      const bool busy = lane < P * kRows;
-      float top = kFarBelow, l = 0.f;
+    for (int i = mine; i < n0 + n1; i += G) {
+      const int end = i >= n0;
+      if (busy) factor[i * kRows + row] = __ldcg(part(end, end ? i - n0 : i) + kRows * D + row);
+    }
+    __syncthreads();
+    float top[2] = {kFarBelow, kFarBelow};
 #pragma unroll 4
-      for (int i = mine; i < n; i += G)
-        if (busy) top = fmaxf(top, __ldcg(part(i) + kRows * D + row));
-      if (busy) tops[mine * kRows + row] = top;
-      __syncthreads();
-#pragma unroll 4
-      for (int i = 0; i < G; ++i) top = fmaxf(top, tops[i * kRows + row]);
-#pragma unroll 4
-      for (int i = mine; i < n; i += G) {
-        if (busy) {
-          const float f = exp2_approx(__ldcg(part(i) + kRows * D + row) - top);
-          l = fmaf(f, __ldcg(part(i) + kRows * D + kRows + row), l);
-          factor[i * kRows + row] = f;
-        }
+    for (int i = 0; i < n0 + n1; ++i) {
+      const float m = factor[i * kRows + row];
+      if (i < n0) top[0] = fmaxf(top[0], m); else top[1] = fmaxf(top[1], m);
+    }
+    __syncthreads();
+    float l[2] = {0.f, 0.f};
+#pragma unroll 1
+    for (int i = mine; i < n0 + n1; i += G) {
+      const int end = i >= n0;
+      if (busy) {
+        const float f = exp2_approx(factor[i * kRows + row] - (end ? top[1] : top[0]));
+        const float add = f * __ldcg(part(end, end ? i - n0 : i) + kRows * D + kRows + row);
+        if (end) l[1] += add; else l[0] += add;
+        factor[i * kRows + row] = f;
       }
-      if (busy) sums[mine * kRows + row] = l;
-      __syncthreads();
+    }
+    if (busy) {
+      sums[mine * kRows + row] = l[0];
+      sums[(G + mine) * kRows + row] = l[1];
+    }
+    __syncthreads();
+    if (warp < 2 && lane < kRows) {
+      float sum = 0.f;
+#pragma unroll 4
+      for (int i = 0; i < G; ++i) sum += sums[(warp * G + i) * kRows + lane];
+      if (sh.last[warp]) sh.place[warp][lane] = row_place(a, sh.seg[warp ? end_slot[1] : end_slot[0]], lane, warp ? top[1] : top[0], sum, sh.by[warp][lane]);
+    }
+    __syncthreads();
 #pragma unroll 1
-      for (int e = tid; e < kRows * D / 4; e += W * 32) {
-        const int r = e / (D / 4), d = e % (D / 4) * 4;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int e = tid + (n0 ? 0 : kQuads); e < (n1 ? 2 : 1) * kQuads; e += W * 32) {
+      const int end = e >= kQuads, r = e % kQuads / (D / 4), d = e % (D / 4) * 4, n = end ? n1 : n0;
+      const float* f = factor + (end ? n0 : 0) * kRows + r;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-        for (int i = 0; i < n; i += 8) {
-          float4 y[8];
+      for (int i = 0; i < n; i += 8) {
+        float4 y[8];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) y[k] = __ldcg(reinterpret_cast<const float4*>(part(min(i + k, n - 1)) + r * D + d));
+        for (int k = 0; k < 8; ++k)
+          if (i + k < n) y[k] = __ldcg(reinterpret_cast<const float4*>(part(end, i + k) + r * D + d));
 #pragma unroll
-          for (int k = 0; k < 8; ++k) add_part(y[k], i + k < n ? factor[(i + k) * kRows + r] : 0.f, x);
-        }
-        float m = kFarBelow, sum = 0.f;
-        for (int i = 0; i < G; ++i) {
-          m = fmaxf(m, tops[i * kRows + r]);
-          sum += sums[i * kRows + r];
-        }
-        finish_row(a, s, r, d, x, m, sum);
+        for (int k = 0; k < 8; ++k)
+          if (i + k < n) add_part(y[k], f[(i + k) * kRows], x);
       }
-      __syncthreads();  // before the other end takes the rings' place
+      store_joined(a, sh.place[end][r], d, x, sh.by[end][r]);
     }
   }
 };
@@ -992,7 +1006,7 @@ __global__ void __launch_bounds__(W * 32, MINB) k_attend(const __grid_constant__
 // D/4 for each tile), and up to 200 KB of rings an SM.
 template <int D, int NT>
 struct Shape;
-template <> struct Shape<64, 1> { static constexpr int W = 8, S = 6, MINB = 2; };
+template <> struct Shape<64, 1> { static constexpr int W = 4, S = 4, MINB = 4; };
 template <> struct Shape<64, 2> { static constexpr int W = 8, S = 4, MINB = 2; };
 template <> struct Shape<64, 4> { static constexpr int W = 8, S = 4, MINB = 1; };
 template <> struct Shape<128, 1> { static constexpr int W = 8, S = 2, MINB = 2; };
