@@ -46,9 +46,9 @@
 namespace dk {
 namespace {
 
-constexpr int kUnit = 16;             // tokens of a unit
+constexpr int kTile = 16;             // tokens of a tile: of one page, one matrix instruction's rows
 constexpr int kMaxRequests = 1024;    // requests of one launch (their prefix sums are in shared memory)
-constexpr int kShort = 96;             // places of segments that no two CTAs share
+constexpr int kShort = 96;            // tiles of segments that no two CTAs share
 constexpr float kFarBelow = -1e30f;   // maximum of a row that has seen no token
 constexpr float kSlack = 8.f;         // a row's maximum may lag its scores by this much (log2)
 constexpr float kLeastScale = 8.4703294725430034e-22f;  // 2^-70: keeps sum w / vs finite
@@ -71,7 +71,7 @@ struct AttendArgs {
   long long q_token_stride, q_head_stride;
   long long k_head_stride, v_head_stride;
   uint32_t k_block_stride, k_token_stride, v_block_stride, v_token_stride;
-  int table_stride, max_blocks, blocks, block_size, units_per_block;
+  int table_stride, max_blocks, blocks, block_size, tiles_per_block;
   int requests, tokens, kv_heads, group;
   unsigned group_magic;  // ceil(2^32 / group), 0 for a group of 1
   float scale_log2;
@@ -161,7 +161,8 @@ struct Segment {
 
 // PACKED: the tokens of a page's head are neighbours in memory, so the rows of
 // a unit lie at fixed offsets.
-template <int D, int NT, bool E4M3, bool PACKED, int W, int S>
+// MT: tiles of a unit, which a warp adds up side by side.
+template <int D, int NT, int MT, bool E4M3, bool PACKED, int W, int S>
 struct Attend {
   static constexpr int kRows = 8 * NT;
   static constexpr int kKWords = D / 16;  // words of a lane's part of a K row
@@ -169,10 +170,11 @@ struct Attend {
   static constexpr int kSlots = 2 * W;    // a warp's parts of segments: an early one and its last
   // Places in the line that a segment's start counts for: its queries' latency
   // and its rows' end take as long as this many units.
-  static constexpr int kStart = D == 64 ? 2 : 1;
-  // A stage: K, V and the two scales of a unit.  Multiples of 128 bytes, so that
-  // the places of pieces differ by an exclusive or of their low bits.
-  static constexpr int kScales = 2 * kUnit * D;
+  static constexpr int kStart = 1;
+  static constexpr int kUnit = MT * kTile;  // tokens of a unit
+  // A stage: each tile's K and V, and their scales.  Multiples of 128 bytes, so
+  // that the places of pieces differ by an exclusive or of their low bits.
+  static constexpr int kTileBytes = 2 * kTile * D, kScales = MT * kTileBytes;
   static constexpr int kStage = kScales + 128;
   // The queries' operands stay in registers while those hold them beside the
   // output's; from 24 rows of 128 on they are read from shared memory.
@@ -355,7 +357,7 @@ struct Attend {
     uint32_t to;         // the lane's place in the next stage
     int unit, end, segment_end;  // place of the next unit in the line, the warp's end, the segment's
     int block, sub, page, next_page;
-    uint32_t hidden;  // of each stage (bits): its page is outside the pool
+    uint32_t hidden;  // of each stage's tiles (bits): the page is outside the pool
 
     __device__ __forceinline__ int page_at(const AttendArgs& a, const Segment& s, int b) const {
       return b < s.blocks ? ld_int(a.table + (long long)s.request * a.table_stride + b) : -1;
@@ -370,9 +372,9 @@ struct Attend {
       v = a.v + s.head * a.v_head_stride + (PACKED ? row * D : row * (long long)a.v_token_stride) + piece * 16;
       scale = (lane & 1 ? a.v_scale : a.k_scale) + s.head;
       unit = max(unit, s.begin);
-      const int u = s.unit0 + unit - s.begin;
-      block = u / a.units_per_block;
-      sub = u - block * a.units_per_block;
+      const int t = (s.unit0 + unit - s.begin) * MT;
+      block = t / a.tiles_per_block;
+      sub = t - block * a.tiles_per_block;
       page = page_at(a, s, block);
       next_page = page_at(a, s, block + 1);
     }
@@ -390,28 +392,32 @@ struct Attend {
         enter(a, t);
       }
       if (unit < end) {
-        const bool good = (unsigned)page < (unsigned)a.blocks;
-        const uint32_t p = good ? page : 0;
-        hidden = (hidden & ~(1u << stage)) | ((good ? 0u : 1u) << stage);
-        const uint32_t first = sub * kUnit;
-        const uint8_t* from_k = k + (uint64_t)p * a.k_block_stride + (PACKED ? first * D : first * a.k_token_stride);
-        const uint8_t* from_v = v + (uint64_t)p * a.v_block_stride + (PACKED ? first * D : first * a.v_token_stride);
-        const uint32_t at = to + offset;
-#pragma unroll
-        for (int j = 0; j < kUnit / kStep; ++j)
-          copy16((at ^ copy_turn(j)) + j * 512, from_k + (PACKED ? j * 512 : (uint64_t)(j * kStep) * a.k_token_stride));
-#pragma unroll
-        for (int j = 0; j < kUnit / kStep; ++j)
-          copy16((at ^ copy_turn(j)) + kUnit * D + j * 512, from_v + (PACKED ? j * 512 : (uint64_t)(j * kStep) * a.v_token_stride));
         const int lane = threadIdx.x & 31;
-        if (lane < 2) copy4(to - place(lane / kPieces, lane % kPieces) + offset + kScales + lane * 4, scale + (uint64_t)p * (uint32_t)a.kv_heads);
-        ++unit;
-        if (++sub == a.units_per_block) {
-          sub = 0;
-          ++block;
-          page = next_page;
-          next_page = page_at(a, s, block + 1);
+        const uint32_t scales = to - place(lane / kPieces, lane % kPieces) + offset + kScales + lane * 4;
+#pragma unroll
+        for (int h = 0; h < MT; ++h) {
+          const bool good = (unsigned)page < (unsigned)a.blocks;
+          const uint32_t p = good ? page : 0, bit = stage * MT + h;
+          hidden = (hidden & ~(1u << bit)) | ((good ? 0u : 1u) << bit);
+          const uint32_t first = sub * kTile;
+          const uint8_t* from_k = k + (uint64_t)p * a.k_block_stride + (PACKED ? first * D : first * a.k_token_stride);
+          const uint8_t* from_v = v + (uint64_t)p * a.v_block_stride + (PACKED ? first * D : first * a.v_token_stride);
+          const uint32_t at = to + offset + h * kTileBytes;
+#pragma unroll
+          for (int j = 0; j < kTile / kStep; ++j)
+            copy16((at ^ copy_turn(j)) + j * 512, from_k + (PACKED ? j * 512 : (uint64_t)(j * kStep) * a.k_token_stride));
+#pragma unroll
+          for (int j = 0; j < kTile / kStep; ++j)
+            copy16((at ^ copy_turn(j)) + kTile * D + j * 512, from_v + (PACKED ? j * 512 : (uint64_t)(j * kStep) * a.v_token_stride));
+          if (lane < 2) copy4(scales + h * 8, scale + (uint64_t)p * (uint32_t)a.kv_heads);
+          if (++sub == a.tiles_per_block) {
+            sub = 0;
+            ++block;
+            page = next_page;
+            next_page = page_at(a, s, block + 1);
+          }
         }
+        ++unit;
       }
       copy_commit();
     }
@@ -485,12 +491,14 @@ struct Attend {
     }
 
     // Rescales to the columns' new maxima; sc holds scores less m.
-    __device__ __forceinline__ void grow(float (&sc)[NT][4]) {
+    __device__ __forceinline__ void grow(float (&sc)[MT][NT][4]) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float top = fmaxf(sc[n][i], sc[n][i + 2]);
+          float top = -INFINITY;
+#pragma unroll
+          for (int h = 0; h < MT; ++h) top = fmaxf(top, fmaxf(sc[h][n][i], sc[h][n][i + 2]));
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
           const uint32_t bit = 1u << (2 * n + i);
@@ -502,8 +510,11 @@ struct Attend {
             if (some) unseen &= ~bit;
           }
           m[n][i] += by;
-          sc[n][i] -= by;
-          sc[n][i + 2] -= by;
+#pragma unroll
+          for (int h = 0; h < MT; ++h) {
+            sc[h][n][i] -= by;
+            sc[h][n][i + 2] -= by;
+          }
           l[n][i] *= f;
 #pragma unroll
           for (int d = 0; d < D / 16; ++d) {
@@ -515,110 +526,126 @@ struct Attend {
       settled = !__any_sync(0xffffffffu, unseen);
     }
 
-    // The unit of tokens base.. of segment s in the stage at `at`.
-    __device__ __forceinline__ void add(const AttendArgs& a, const Segment& s, int base, uint32_t at, uint32_t ring, bool good) {
+    // The unit of tokens base.. of segment s in the stage at `at`; hidden: its
+    // tiles (bits) whose pages are outside the pool.
+    __device__ __forceinline__ void add(const AttendArgs& a, const Segment& s, int base, uint32_t at, uint32_t ring, uint32_t hidden) {
       const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-      float k_scale, v_scale;
-      asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(k_scale), "=f"(v_scale) : "r"(at + kScales));
-      // Scores: [16 tokens][8 rows] for each tile of rows, one tile in two chains.
-      constexpr int kChains = NT == 1 ? 2 : 1;
-      float sc[NT][4], sd[4] = {0.f, 0.f, 0.f, 0.f};
+      // Scores: [16 tokens][8 rows] for each tile of tokens and of rows, one tile
+      // alone in two chains.
+      constexpr int kChains = NT * MT == 1 ? 2 : 1;
+      float sc[MT][NT][4], sd[4] = {0.f, 0.f, 0.f, 0.f}, v_inverse[MT];
+      bool edge[MT], above = false;
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sc[n][i] = 0.f;
-      const uint32_t at_k = at + place(g, D == 64 ? c : 2 * c);
-#pragma unroll
-      for (int part = 0; part < kKWords / 4; ++part) {
-        uint32_t k0[4], k1[4];
-        const uint32_t from = (at_k ^ (part & 1) * 16) + (part >> 1) * 128;
-        lds_words<4>(from, k0);
-        lds_words<4>(from + 8 * D, k1);
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint32_t a0, a1, a2, a3;
-          codes_to_half<E4M3>(k0[w], a0, a2);
-          codes_to_half<E4M3>(k1[w], a1, a3);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            uint32_t b[2];
-            if constexpr (kQShared) {
-              lds_words<2>(ring + S * kStage + (n * kKWords + 4 * part + w) * 256 + lane * 8, b);
-            } else {
-              b[0] = q[n][8 * part + 2 * w];
-              b[1] = q[n][8 * part + 2 * w + 1];
-            }
-            mma16816(kChains == 2 && (w & 1) ? sd : sc[n], a0, a1, a2, a3, b[0], b[1]);
-          }
-        }
-      }
-      const float v_now = v_scale < kLeastScale ? kLeastScale : v_scale;
-      float v_log2, v_inverse;
-      asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(v_log2) : "f"(v_now));
-      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(v_inverse) : "f"(v_now));
-      bool above = false;
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sc[n][i] = fmaf(kChains == 2 ? sc[n][i] + sd[i] : sc[n][i], factor[n][i & 1] * k_scale, v_log2 - m[n][i & 1]);
-      }
-      const bool edge = base + kUnit > least_high || base < most_low || !good;  // the same in all lanes
-      if (edge) {
-        if (!good) v_inverse = 0.f;
+      for (int h = 0; h < MT; ++h) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            int token, head, low, high;
-            row_of(a, s, n * 8 + 2 * c + i, token, head, low, high);
-            const int t = base + g;
-            if (t >= high || t < low || !good) sc[n][i] = -INFINITY;
-            if (t + 8 >= high || t + 8 < low || !good) sc[n][i + 2] = -INFINITY;
-          }
-      }
+          for (int i = 0; i < 4; ++i) sc[h][n][i] = 0.f;
+        const uint32_t at_k = at + h * kTileBytes + place(g, D == 64 ? c : 2 * c);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) above |= fmaxf(fmaxf(sc[n][0], sc[n][2]), fmaxf(sc[n][1], sc[n][3])) > kSlack;
-      if (__any_sync(0xffffffffu, above) || !settled) grow(sc);
-      uint32_t pb[NT][2];
+        for (int part = 0; part < kKWords / 4; ++part) {
+          uint32_t k0[4], k1[4];
+          const uint32_t from = (at_k ^ (part & 1) * 16) + (part >> 1) * 128;
+          lds_words<4>(from, k0);
+          lds_words<4>(from + 8 * D, k1);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float w[4];
+          for (int w = 0; w < 4; ++w) {
+            uint32_t a0, a1, a2, a3;
+            codes_to_half<E4M3>(k0[w], a0, a2);
+            codes_to_half<E4M3>(k1[w], a1, a3);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = exp2_approx(sc[n][i]);
-        l[n][0] = fmaf(w[0] + w[2], v_inverse, l[n][0]);
-        l[n][1] = fmaf(w[1] + w[3], v_inverse, l[n][1]);
-        pb[n][0] = transpose8x8(pack_half2(w[0], w[1]));
-        pb[n][1] = transpose8x8(pack_half2(w[2], w[3]));
-      }
-      const uint32_t at_v = at + kUnit * D + (D == 64 ? place(2 * c, g >> 1) + (g & 1) * 8 : place(2 * c, D == 128 ? g : 2 * g));
-      constexpr int kPart = kVWords < 4 ? kVWords : 4;  // words of a load
-#pragma unroll
-      for (int part = 0; part < kVWords / kPart; ++part) {
-        uint32_t v[4][kPart];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          lds_words<kPart>((at_v ^ ((j & 1) * kOdd) ^ (part * 16)) + (j & 1) * kOddRow + (j >> 1) * 8 * D, v[j]);
-        if (edge) {  // bytes of tokens that no row sees may be anything, e4m3's NaN too
-          const int past = good ? most_high - base : 0, before = least_low - base;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int t = 2 * c + (j & 1) + (j >> 1) * 8;
-            if (t >= past || t < before)
-#pragma unroll
-              for (int w = 0; w < kPart; ++w) v[j][w] = 0u;
+            for (int n = 0; n < NT; ++n) {
+              uint32_t b[2];
+              if constexpr (kQShared) {
+                lds_words<2>(ring + S * kStage + (n * kKWords + 4 * part + w) * 256 + lane * 8, b);
+              } else {
+                b[0] = q[n][8 * part + 2 * w];
+                b[1] = q[n][8 * part + 2 * w + 1];
+              }
+              mma16816(kChains == 2 && (w & 1) ? sd : sc[h][n], a0, a1, a2, a3, b[0], b[1]);
+            }
           }
         }
+      }
 #pragma unroll
-        for (int w = 0; w < kPart; ++w) {
-          uint32_t e[4], f[4];  // [channel 4w + i]: tokens (2c, 2c+1) and (2c+8, 2c+9)
-          codes_to_half<E4M3>(prmt(v[0][w], v[1][w], 0x5140), e[0], e[1]);
-          codes_to_half<E4M3>(prmt(v[0][w], v[1][w], 0x7362), e[2], e[3]);
-          codes_to_half<E4M3>(prmt(v[2][w], v[3][w], 0x5140), f[0], f[1]);
-          codes_to_half<E4M3>(prmt(v[2][w], v[3][w], 0x7362), f[2], f[3]);
+      for (int h = 0; h < MT; ++h) {
+        const bool good = !(hidden >> h & 1);
+        float k_scale, v_scale, v_log2;
+        asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(k_scale), "=f"(v_scale) : "r"(at + kScales + h * 8));
+        if (v_scale < kLeastScale) v_scale = kLeastScale;
+        asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(v_log2) : "f"(v_scale));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(v_inverse[h]) : "f"(v_scale));
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            mma16816(o[n][2 * (part * kPart + w)], e[0], e[1], f[0], f[1], pb[n][0], pb[n][1]);
-            mma16816(o[n][2 * (part * kPart + w) + 1], e[2], e[3], f[2], f[3], pb[n][0], pb[n][1]);
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            sc[h][n][i] = fmaf(kChains == 2 ? sc[h][n][i] + sd[i] : sc[h][n][i], factor[n][i & 1] * k_scale, v_log2 - m[n][i & 1]);
+        }
+        const int first = base + h * kTile;
+        edge[h] = first + kTile > least_high || first < most_low || !good;  // the same in all lanes
+        if (edge[h]) {
+          if (!good) v_inverse[h] = 0.f;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              int token, head, low, high;
+              row_of(a, s, n * 8 + 2 * c + i, token, head, low, high);
+              const int t = first + g;
+              if (t >= high || t < low || !good) sc[h][n][i] = -INFINITY;
+              if (t + 8 >= high || t + 8 < low || !good) sc[h][n][i + 2] = -INFINITY;
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          above |= fmaxf(fmaxf(sc[h][n][0], sc[h][n][2]), fmaxf(sc[h][n][1], sc[h][n][3])) > kSlack;
+      }
+      if (__any_sync(0xffffffffu, above) || !settled) grow(sc);
+      uint32_t pb[MT][NT][2];
+#pragma unroll
+      for (int h = 0; h < MT; ++h)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = exp2_approx(sc[h][n][i]);
+          l[n][0] = fmaf(w[0] + w[2], v_inverse[h], l[n][0]);
+          l[n][1] = fmaf(w[1] + w[3], v_inverse[h], l[n][1]);
+          pb[h][n][0] = transpose8x8(pack_half2(w[0], w[1]));
+          pb[h][n][1] = transpose8x8(pack_half2(w[2], w[3]));
+        }
+      constexpr int kPart = kVWords < 4 ? kVWords : 4;  // words of a load
+#pragma unroll
+      for (int h = 0; h < MT; ++h) {
+        const uint32_t at_v = at + h * kTileBytes + kTile * D + (D == 64 ? place(2 * c, g >> 1) + (g & 1) * 8 : place(2 * c, D == 128 ? g : 2 * g));
+#pragma unroll
+        for (int part = 0; part < kVWords / kPart; ++part) {
+          uint32_t v[4][kPart];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            lds_words<kPart>((at_v ^ ((j & 1) * kOdd) ^ (part * 16)) + (j & 1) * kOddRow + (j >> 1) * 8 * D, v[j]);
+          if (edge[h]) {  // bytes of tokens that no row sees may be anything, e4m3's NaN too
+            const int first = base + h * kTile, past = hidden >> h & 1 ? 0 : most_high - first, before = least_low - first;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int t = 2 * c + (j & 1) + (j >> 1) * 8;
+              if (t >= past || t < before)
+#pragma unroll
+                for (int w = 0; w < kPart; ++w) v[j][w] = 0u;
+            }
+          }
+#pragma unroll
+          for (int w = 0; w < kPart; ++w) {
+            uint32_t e[4], f[4];  // [channel 4w + i]: tokens (2c, 2c+1) and (2c+8, 2c+9)
+            codes_to_half<E4M3>(prmt(v[0][w], v[1][w], 0x5140), e[0], e[1]);
+            codes_to_half<E4M3>(prmt(v[0][w], v[1][w], 0x7362), e[2], e[3]);
+            codes_to_half<E4M3>(prmt(v[2][w], v[3][w], 0x5140), f[0], f[1]);
+            codes_to_half<E4M3>(prmt(v[2][w], v[3][w], 0x7362), f[2], f[3]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              mma16816(o[n][2 * (part * kPart + w)], e[0], e[1], f[0], f[1], pb[h][n][0], pb[h][n][1]);
+              mma16816(o[n][2 * (part * kPart + w) + 1], e[2], e[3], f[2], f[3], pb[h][n][0], pb[h][n][1]);
+            }
           }
         }
       }
@@ -744,7 +771,7 @@ struct Attend {
     const int chunk = (all + grid - 1) / grid;
     const int cta = blockIdx.x;
     if (cta >= grid || cta * chunk >= all) return;
-    const bool snap = longest <= kShort;
+    const bool snap = longest <= kShort / MT;
     int cta0 = cta * chunk, cta1 = min(all, cta0 + chunk);
     if (snap) {
       if (warp < 2) {
@@ -793,7 +820,7 @@ struct Attend {
           copy_wait<S - 2>();
           __syncwarp();  // the unit is there for all lanes, and the stage before it has been read by all
           feed.next(a, prefix, sh.fed[warp], freed, freed_stage);
-          rows.add(a, s, base, ring + offset, ring, !(feed.hidden >> stage & 1));
+          rows.add(a, s, base, ring + offset, ring, feed.hidden >> (stage * MT));
           base += kUnit;
           freed = offset;
           freed_stage = stage;
@@ -994,27 +1021,27 @@ struct Attend {
   }
 };
 
-template <int D, int NT, bool E4M3, bool PACKED, int W, int S, int MINB>
+template <int D, int NT, int MT, bool E4M3, bool PACKED, int W, int S, int MINB>
 __global__ void __launch_bounds__(W * 32, MINB) k_attend(const __grid_constant__ AttendArgs a) {
   extern __shared__ __align__(128) unsigned char raw[];
-  using A = Attend<D, NT, E4M3, PACKED, W, S>;
+  using A = Attend<D, NT, MT, E4M3, PACKED, W, S>;
   A::run(a, *reinterpret_cast<typename A::Shared*>(raw), reinterpret_cast<int*>(raw + sizeof(typename A::Shared)));
 }
 
-// Warps of a CTA, stages of a warp's ring and CTAs of an SM for each head size
-// and number of row tiles: what the registers of the rows leave (q D/8 and o
+// Warps of a CTA, stages of a warp's ring, CTAs of an SM and tiles of a unit for
+// each head size and number of row tiles: what the registers of the rows leave (q D/8 and o
 // D/4 for each tile), and up to 200 KB of rings an SM.
 template <int D, int NT>
 struct Shape;
-template <> struct Shape<64, 1> { static constexpr int W = 4, S = 4, MINB = 4; };
-template <> struct Shape<64, 2> { static constexpr int W = 8, S = 4, MINB = 2; };
-template <> struct Shape<64, 4> { static constexpr int W = 8, S = 4, MINB = 1; };
-template <> struct Shape<128, 1> { static constexpr int W = 8, S = 2, MINB = 2; };
-template <> struct Shape<128, 2> { static constexpr int W = 8, S = 3, MINB = 1; };
-template <> struct Shape<128, 3> { static constexpr int W = 8, S = 3, MINB = 1; };
-template <> struct Shape<128, 4> { static constexpr int W = 8, S = 3, MINB = 1; };
-template <> struct Shape<256, 1> { static constexpr int W = 8, S = 2, MINB = 1; };
-template <> struct Shape<256, 2> { static constexpr int W = 8, S = 2, MINB = 1; };
+template <> struct Shape<64, 1> { static constexpr int W = 8, S = 2, MINB = 2, MT = 2; };
+template <> struct Shape<64, 2> { static constexpr int W = 12, S = 3, MINB = 1, MT = 2; };
+template <> struct Shape<64, 4> { static constexpr int W = 8, S = 3, MINB = 1, MT = 2; };
+template <> struct Shape<128, 1> { static constexpr int W = 8, S = 2, MINB = 2, MT = 1; };
+template <> struct Shape<128, 2> { static constexpr int W = 8, S = 3, MINB = 1, MT = 1; };
+template <> struct Shape<128, 3> { static constexpr int W = 8, S = 3, MINB = 1, MT = 1; };
+template <> struct Shape<128, 4> { static constexpr int W = 8, S = 3, MINB = 1, MT = 1; };
+template <> struct Shape<256, 1> { static constexpr int W = 8, S = 2, MINB = 1, MT = 1; };
+template <> struct Shape<256, 2> { static constexpr int W = 8, S = 2, MINB = 1, MT = 1; };
 
 // The workspace: a counter for each CTA that can run at once (in the same place
 // for every shape: they stay zero between calls), two parts of its segments,
@@ -1033,13 +1060,13 @@ Workspace workspace_of(int sms) {
 
 template <int D, int NT, bool E4M3, bool PACKED>
 dk_status launch(AttendArgs a, cudaStream_t stream) {
-  constexpr int W = Shape<D, NT>::W, MINB = Shape<D, NT>::MINB, S = Shape<D, NT>::S;
-  using A = Attend<D, NT, E4M3, PACKED, W, S>;
+  constexpr int W = Shape<D, NT>::W, MINB = Shape<D, NT>::MINB, S = Shape<D, NT>::S, MT = Shape<D, NT>::MT;
+  using A = Attend<D, NT, MT, E4M3, PACKED, W, S>;
   const size_t per = (a.starts ? 3 : 2) * sizeof(int);  // of a request in shared memory
   const size_t smem = sizeof(typename A::Shared) + per * (size_t)(std::min(a.requests, kMaxRequests) + 1);
   static_assert(sizeof(typename A::Shared) + 3 * sizeof(int) * (kMaxRequests + 1) <= 227 * 1024,
                 "a CTA fits the shared memory");
-  auto kernel = k_attend<D, NT, E4M3, PACKED, W, S, MINB>;
+  auto kernel = k_attend<D, NT, MT, E4M3, PACKED, W, S, MINB>;
   const Workspace w = workspace_of<D, NT>(sm_count(-1));
   a.counters = static_cast<int*>(a.workspace);
   a.partials = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + w.counters);
@@ -1078,7 +1105,7 @@ dk_status launch(AttendArgs a, cudaStream_t stream) {
       a.tokens = tokens - r;
     }
     // No more CTAs than the table's width can keep busy.
-    const long long most = (((long long)a.max_blocks * a.block_size + kUnit - 1) / kUnit + A::kStart) * a.kv_heads *
+    const long long most = (((long long)a.max_blocks * a.block_size + A::kUnit - 1) / A::kUnit + A::kStart) * a.kv_heads *
                            (starts ? (long long)a.requests + (long long)tokens * a.group / A::kRows : (long long)a.requests * ((a.group + A::kRows - 1) / A::kRows));
     const int grid = (int)std::min<long long>(sm_count(device) * MINB, (most + W - 1) / W);
     const dk_status s = launch_early("dk_cache_attention", kernel, dim3(grid), dim3(W * 32), smem, stream, a);
@@ -1175,7 +1202,7 @@ extern "C" dk_status dk_cache_attention(const dk_cache_attention_args* p, void* 
   a.max_blocks = p->max_blocks;
   a.blocks = c.blocks;
   a.block_size = c.block_size;
-  a.units_per_block = c.block_size / kUnit;
+  a.tiles_per_block = c.block_size / kTile;
   a.requests = p->requests;
   a.tokens = p->tokens;
   a.kv_heads = c.kv_heads;
