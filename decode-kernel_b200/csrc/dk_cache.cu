@@ -33,6 +33,7 @@ struct PlanArgs {
   int* starts;
   long long* slots;
   int requests, max_blocks, table_stride, block_size, free_capacity, tokens;
+  unsigned block_magic;  // ceil(2^32 / block_size)
 };
 
 // The last i in [0, n) with p[i] <= x (p rises, p[0] <= x).
@@ -157,6 +158,14 @@ __global__ void __launch_bounds__(kPlanThreads) k_cache_plan(const __grid_consta
 
   const int capacity = a.free_capacity;
   const int head0 = capacity ? (int)(head % capacity) : 0, tail0 = capacity ? (int)(tail % capacity) : 0;
+  auto over_block = [&](int x) {  // x / block_size, x >= 0
+    const int q = __umulhi(x, a.block_magic);  // that, or one more
+    return q - (q * (long long)bs > x);
+  };
+  auto blocks_of = [&](int x) {
+    const int q = over_block(x);
+    return q + (q * bs != x);
+  };
   auto ring_at = [&](int from, int i) {  // i < capacity
     const int x = from + i;
     return x >= capacity || x < from ? x - capacity : x;
@@ -168,26 +177,36 @@ __global__ void __launch_bounds__(kPlanThreads) k_cache_plan(const __grid_consta
     const int t0 = (int)at;
     long long out[VT];
     int r = a.requests ? last_at(s_tokens, a.requests, t0) : 0;
-    int known = -1, known_of = -1, page = 0;  // the page that the last slot is in
+    // The request's end, and where its next token goes: row `row` of block
+    // `block`, whose page is looked up when it begins.
+    int ends = -1, c = 0, block = 0, row = 0, page = 0;
+    bool known = false;
 #pragma unroll
     for (int i = 0; i < VT; ++i) {
       const int t = t0 + i;
       out[i] = -1;
-      if (t < carry[0]) {
+      if (t >= carry[0]) continue;
+      if (t >= ends) {
         while (r + 1 < a.requests && s_tokens[r + 1] <= t) ++r;
-        const int c = s_held[r];
-        if (c >= 0) {
-          const int place = c + (t - s_tokens[r]), block = place / bs;
-          if (block != known || r != known_of) {
-            const int have = c / bs + (c % bs != 0);
-            page = block < have ? a.table[(long long)r * a.table_stride + block]
-                                : a.free_blocks[ring_at(head0, s_need[r] + block - have)];
-            known = block;
-            known_of = r;
-          }
-          out[i] = (long long)page * bs + (place - block * bs);
-        }
+        ends = s_tokens[r + 1];
+        c = s_held[r];
+        const int place = max(c, 0) + (t - s_tokens[r]);
+        block = over_block(place);
+        row = place - block * bs;
+        known = false;
+      } else if (++row == bs) {
+        row = 0;
+        ++block;
+        known = false;
       }
+      if (c < 0) continue;
+      if (!known) {
+        const int have = blocks_of(c);
+        page = block < have ? a.table[(long long)r * a.table_stride + block]
+                            : a.free_blocks[ring_at(head0, s_need[r] + block - have)];
+        known = true;
+      }
+      out[i] = (long long)page * bs + row;
     }
 #pragma unroll
     for (int i = 0; i < VT; i += 2) {
@@ -204,7 +223,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_cache_plan(const __grid_consta
     const int r = last_at(s_need, a.requests, j);
     const int c = s_held[r];
     if (c < 0) continue;
-    const int have = c / bs + (c % bs != 0);
+    const int have = blocks_of(c);
     a.table[(long long)r * a.table_stride + have + (j - s_need[r])] = a.free_blocks[ring_at(head0, j)];
   }
   // Pages of ended requests to the ring's end, where nothing is read.
@@ -223,9 +242,9 @@ __global__ void __launch_bounds__(kPlanThreads) k_cache_plan(const __grid_consta
 //
 // A CTA looks for the runs that begin in its window of tokens, reading the
 // slots of the window and of the pages that may begin in it at once.  A short
-// run is a warp's, a long one the CTA's, its rows kept in registers between
-// the maximum and the coding, so the values are read once.  A lane holds 8
-// neighbouring channels (16 bytes read, 8 written).  Earlier rows that a single
+// run is a warp's, a long one the CTA's, its rows kept (in registers, in shared
+// memory) between the maximum and the coding, so the values are read once.  A
+// lane holds 8 neighbouring channels (16 bytes read, 8 written).  Earlier rows that a single
 // token's larger value makes to be coded again are left to the whole CTA.
 // The largest magnitude is taken over the 16-bit patterns without their sign,
 // which order as the values do, infinities and NaN above all: only where one
@@ -233,8 +252,10 @@ __global__ void __launch_bounds__(kPlanThreads) k_cache_plan(const __grid_consta
 // ---------------------------------------------------------------------------
 constexpr int kAppendWarps = 4;
 constexpr int kShortRun = 8;  // rows that a warp takes alone
-constexpr int kKeep = 8;      // pieces of 8 values that a lane keeps
+constexpr int kPieces = 8;    // pieces of 8 values of a long run that a thread keeps in shared memory
 constexpr int kMaxWindow = 64;
+constexpr int kMaxItems = 4;  // heads' K or V that a CTA takes one after the other
+constexpr int kMaxJobs = kMaxWindow * kMaxItems;
 constexpr int kMaxBlock = 256;
 constexpr float kLeastAmax = 8.673617379884035e-19f;  // 2^-60
 
@@ -246,7 +267,7 @@ struct AppendArgs {
   long long x_token_stride[2], x_head_stride[2];
   const long long* slots;
   unsigned long long block_magic;  // ceil(2^64 / block_size): slot / block_size is the high half of the product
-  int tokens, blocks, block_size, kv_heads, window, bf16;
+  int tokens, blocks, block_size, kv_heads, window, items, bf16;
 };
 
 __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
@@ -327,34 +348,59 @@ __device__ __forceinline__ uint32_t code_again(uint32_t w, float ratio) {
   return encode4<E4M3, E4M3>(x[0], x[1], x[2], x[3]);  // int8 codes get no larger; e4m3's may be NaN
 }
 
+// The largest of a warp's values by their 16-bit patterns without the sign.
+__device__ __forceinline__ uint32_t add_largest(uint32_t top2, const uint4& p) {
+  return max_u16x2(max_u16x2(top2, p.x & 0x7fff7fffu),
+                   max_u16x2(p.y & 0x7fff7fffu, max_u16x2(p.z & 0x7fff7fffu, p.w & 0x7fff7fffu)));
+}
+// The same over the finite ones.
+__device__ __forceinline__ uint32_t add_largest_finite(uint32_t top, const uint4& p, uint32_t infinite) {
+  const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t lo = w[k] & 0x7fffu, hi = (w[k] >> 16) & 0x7fffu;
+    if (lo < infinite) top = max(top, lo);
+    if (hi < infinite) top = max(top, hi);
+  }
+  return top;
+}
+
 template <int D, bool E4M3>
-__global__ void __launch_bounds__(kAppendWarps * 32) k_cache_append(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(kAppendWarps * 32, 5) k_cache_append(const __grid_constant__ AppendArgs a) {
   constexpr float Q = E4M3 ? 448.f : 127.f;
   constexpr int LPR = D / 8;     // lanes of a row
   constexpr int RPW = 32 / LPR;  // rows of a warp's load
+  constexpr int kStep = kAppendWarps * RPW;         // rows of the CTA's load
+  constexpr int kAlone = kShortRun / RPW;           // a warp's loads of a short run
   constexpr int kSpan = kMaxWindow + kMaxBlock;
   struct Job {  // earlier rows to be coded again
     uint8_t* rows;
+    long long stride;
     int n;
     float ratio;
   };
+  extern __shared__ uint4 s_rows[];  // [2][kPieces][threads], if there are long runs
   __shared__ long long s_slot[kSpan + 1];
   __shared__ uint32_t s_break[kSpan / 32 + 1];
   __shared__ uint32_t s_top[2][kAppendWarps];
-  __shared__ Job s_job[kMaxWindow];
+  __shared__ Job s_job[kMaxJobs];
   __shared__ int s_jobs;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int h = blockIdx.y, which = blockIdx.z, bs = a.block_size;
+  const int bs = a.block_size;
   const int first = blockIdx.x * a.window;
-  const long long xs = a.x_token_stride[which], ps = a.row_stride[which];
-  const uint16_t* x_base = a.x[which] + h * a.x_head_stride[which] + (lane % LPR) * 8;
   const int sub = lane / LPR;
+  // The CTA's items: K and V of neighbouring heads.
+  const int item0 = blockIdx.y * a.items, item1 = min(item0 + a.items, 2 * a.kv_heads);
+  auto rows_of = [&](int item) {  // the lane's first values of token 0
+    return a.x[item & 1] + (item >> 1) * a.x_head_stride[item & 1] + lane % LPR * 8;
+  };
   pdl_trigger();
   pdl_wait();
   // The warp's token of a small window, while its slot is on its way.
   uint4 ahead = make_uint4(0, 0, 0, 0);
-  if (a.window == kAppendWarps && first + warp < a.tokens && sub == 0)
-    ahead = *reinterpret_cast<const uint4*>(x_base + (long long)(first + warp) * xs);
+  const bool small = a.window == kAppendWarps && a.items == 1;
+  if (small && first + warp < a.tokens && sub == 0)
+    ahead = *reinterpret_cast<const uint4*>(rows_of(item0) + (long long)(first + warp) * a.x_token_stride[item0 & 1]);
   // s_slot[i]: the slot of token first - 1 + i.  A token breaks the run before
   // it if it has no slot, begins a page or does not follow its neighbour.
   const int span = min(a.window + bs, a.tokens - first);
@@ -380,7 +426,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32) k_cache_append(const __grid
     }
     return span;
   };
-  auto again = [&](uint8_t* rows, int n, float ratio, int w, int warps) {
+  auto again = [&](uint8_t* rows, long long ps, int n, float ratio, int w, int warps) {
     constexpr int LR = D / 16, RW = 32 / LR;  // 16 codes a lane
 #pragma unroll 4
     for (int i = w * RW + lane / LR; i < n; i += warps * RW) {
@@ -389,6 +435,11 @@ __global__ void __launch_bounds__(kAppendWarps * 32) k_cache_append(const __grid
       *p = make_uint4(code_again<E4M3>(c.x, ratio), code_again<E4M3>(c.y, ratio), code_again<E4M3>(c.z, ratio), code_again<E4M3>(c.w, ratio));
     }
   };
+  const uint32_t infinite = a.bf16 ? 0x7f80u : 0x7c00u;
+  auto value = [&](uint32_t pattern) {
+    return a.bf16 ? __uint_as_float(pattern << 16) : __half2float(__ushort_as_half((unsigned short)pattern));
+  };
+  auto scale_for = [&](float old, uint32_t top) { return fmaxf(old, __fdiv_rn(fmaxf(value(top), kLeastAmax), Q)); };
   int turn = 0, big = 0;
   for (int i0 = next_break(0); i0 < min(span, a.window); i0 = next_break(i0 + 1)) {
     const long long slot = s_slot[i0 + 1];
@@ -396,88 +447,128 @@ __global__ void __launch_bounds__(kAppendWarps * 32) k_cache_append(const __grid
     if (slot < 0 || page >= a.blocks) continue;
     const int row0 = (int)(slot - page * bs);
     const int n = next_break(i0 + 1) - i0;
-    const bool alone = n <= kShortRun;
-    if (alone && turn++ % kAppendWarps != warp) continue;
-    const int w0 = alone ? sub : warp * RPW + sub, step = alone ? RPW : kAppendWarps * RPW;
-    const uint16_t* x = x_base + (long long)(first + i0) * xs;
-    uint8_t* pool = a.pool[which] + page * a.block_stride[which] + h * a.head_stride[which];
-    float* scale = a.scale[which] + page * a.kv_heads + h;
-    const float old = row0 > 0 ? *scale : 0.f;
-
-    uint4 keep[kKeep];
-    uint32_t top2 = 0;
-    if (a.window == kAppendWarps && n == 1 && i0 == warp) {
-      keep[0] = ahead;
-    } else {
+    auto scale_at = [&](int item) { return a.scale[item & 1] + page * a.kv_heads + (item >> 1); };
+    auto pool_at = [&](int item) { return a.pool[item & 1] + page * a.block_stride[item & 1] + (item >> 1) * a.head_stride[item & 1]; };
+    if (n <= kShortRun) {
+#pragma unroll 1
+      for (int item = item0; item < item1; ++item) {
+        if (turn++ % kAppendWarps != warp) continue;
+        const long long xs = a.x_token_stride[item & 1], ps = a.row_stride[item & 1];
+        const uint16_t* x = rows_of(item) + (first + i0 + sub) * xs;
+        float* scale = scale_at(item);
+        const float old = row0 > 0 ? *scale : 0.f;
+        uint4 keep[kAlone];
+        if (small && n == 1 && i0 == warp) {
+          keep[0] = ahead;
+        } else {
 #pragma unroll
-      for (int k = 0; k < kKeep; ++k)
-        if (w0 + k * step < n) keep[k] = *reinterpret_cast<const uint4*>(x + (w0 + k * step) * xs);
+          for (int k = 0; k < kAlone; ++k)
+            if (sub + k * RPW < n) keep[k] = *reinterpret_cast<const uint4*>(x + k * RPW * xs);
+        }
+        uint32_t top = 0;
+#pragma unroll
+        for (int k = 0; k < kAlone; ++k)
+          if (sub + k * RPW < n) top = add_largest(top, keep[k]);
+        top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
+        const bool odd = top >= infinite;
+        if (odd) {
+          top = 0;
+#pragma unroll
+          for (int k = 0; k < kAlone; ++k)
+            if (sub + k * RPW < n) top = add_largest_finite(top, keep[k], infinite);
+          top = __reduce_max_sync(0xffffffffu, top);
+        }
+        const float now = scale_for(old, top), by = __frcp_rn(now);
+        uint8_t* pool = pool_at(item);
+        uint8_t* to = pool + (row0 + sub) * ps + lane % LPR * 8;
+#pragma unroll
+        for (int k = 0; k < kAlone; ++k)
+          if (sub + k * RPW < n) *reinterpret_cast<uint2*>(to + k * RPW * ps) = encode8<E4M3>(keep[k], a.bf16, by, odd);
+        if (now > old && lane == 0) {
+          *scale = now;
+          if (row0 > 0) s_job[atomicAdd(&s_jobs, 1)] = Job{pool, ps, row0, __fdiv_rn(old, now)};
+        }
+      }
+      continue;
     }
-    auto add = [&](const uint4& p) {
-      top2 = max_u16x2(max_u16x2(top2, p.x & 0x7fff7fffu), max_u16x2(p.y & 0x7fff7fffu, max_u16x2(p.z & 0x7fff7fffu, p.w & 0x7fff7fffu)));
-    };
+    // A long run, item after item: the next one's rows are copied into shared
+    // memory while this one's are coded.  Each thread reads what it copied;
+    // rows past the kept ones are read from global memory, twice.
+    const int w0 = warp * RPW + sub, kept = kPieces * kStep;
+    auto source = [&](int item) { return rows_of(item) + (first + i0 + w0) * a.x_token_stride[item & 1]; };
+    auto fetch = [&](int item, int buffer) {
+      const uint16_t* x = source(item);
+      const long long step = kStep * a.x_token_stride[item & 1];
+      const uint32_t to = smem_u32(s_rows + buffer * kPieces * kAppendWarps * 32 + tid);
 #pragma unroll
-    for (int k = 0; k < kKeep; ++k)
-      if (w0 + k * step < n) add(keep[k]);
-    for (int i = w0 + kKeep * step; i < n; i += step) add(*reinterpret_cast<const uint4*>(x + i * xs));
-    auto over_all = [&](uint32_t v) {  // the largest of the run's warps; `old` is read before any scale changes
-      v = __reduce_max_sync(0xffffffffu, v);
-      if (!alone) {
+      for (int k = 0; k < kPieces; ++k, x += step)
+        if (w0 + k * kStep < n) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + k * kAppendWarps * 512), "l"(x) : "memory");
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    fetch(item0, 0);
+#pragma unroll 1
+    for (int item = item0; item < item1; ++item) {
+      const int buffer = (item - item0) & 1;
+      if (item + 1 < item1) {
+        fetch(item + 1, buffer ^ 1);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+      } else {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+      }
+      const uint4* rows = s_rows + buffer * kPieces * kAppendWarps * 32 + tid;
+      const uint16_t* x = source(item) + kept * a.x_token_stride[item & 1];
+      const long long ps = a.row_stride[item & 1], x_step = kStep * a.x_token_stride[item & 1], to_step = kStep * ps;
+      float* scale = scale_at(item);
+      const float old = row0 > 0 ? *scale : 0.f;
+      uint32_t top2 = 0;
+#pragma unroll
+      for (int k = 0; k < kPieces; ++k)
+        if (w0 + k * kStep < n) top2 = add_largest(top2, rows[k * kAppendWarps * 32]);
+      for (int i = w0 + kept, k = 0; i < n; i += kStep, ++k) top2 = add_largest(top2, *reinterpret_cast<const uint4*>(x + k * x_step));
+      auto over_all = [&](uint32_t v) {  // `old` is read by all before any scale changes
+        v = __reduce_max_sync(0xffffffffu, v);
         if (lane == 0) s_top[big & 1][warp] = v;
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < kAppendWarps; ++w) v = max(v, s_top[big & 1][w]);
         ++big;
+        return v;
+      };
+      uint32_t top = over_all(max(top2 & 0xffffu, top2 >> 16));
+      const bool odd = top >= infinite;  // the same in all warps
+      if (odd) {
+        uint32_t finite = 0;
+        for (int k = 0; k < kPieces; ++k)
+          if (w0 + k * kStep < n) finite = add_largest_finite(finite, rows[k * kAppendWarps * 32], infinite);
+        for (int i = w0 + kept, k = 0; i < n; i += kStep, ++k) finite = add_largest_finite(finite, *reinterpret_cast<const uint4*>(x + k * x_step), infinite);
+        top = over_all(finite);
       }
-      return v;
-    };
-    uint32_t top = over_all(max(top2 & 0xffffu, top2 >> 16));
-    const uint32_t infinite = a.bf16 ? 0x7f80u : 0x7c00u;
-    const bool odd = top >= infinite;  // the same in all of the run's warps
-    if (odd) {
-      uint32_t finite = 0;
-      for (int i = w0; i < n; i += step) {
-        const uint4 p = *reinterpret_cast<const uint4*>(x + i * xs);
-        const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+      const float now = scale_for(old, top), by = __frcp_rn(now);
+      uint8_t* pool = pool_at(item);
+      uint8_t* to = pool + (row0 + w0) * ps + lane % LPR * 8;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t lo = w[k] & 0x7fffu, hi = (w[k] >> 16) & 0x7fffu;
-          if (lo < infinite) finite = max(finite, lo);
-          if (hi < infinite) finite = max(finite, hi);
-        }
-      }
-      top = over_all(finite);
-    }
-    const float amax = a.bf16 ? __uint_as_float(top << 16) : __half2float(__ushort_as_half((unsigned short)top));
-    const float now = fmaxf(old, __fdiv_rn(fmaxf(amax, kLeastAmax), Q));
-    const float by = __frcp_rn(now);
-    uint8_t* to = pool + row0 * ps + (lane % LPR) * 8;
-#pragma unroll
-    for (int k = 0; k < kKeep; ++k)
-      if (w0 + k * step < n) *reinterpret_cast<uint2*>(to + (w0 + k * step) * ps) = encode8<E4M3>(keep[k], a.bf16, by, odd);
-    for (int i = w0 + kKeep * step; i < n; i += step)
-      *reinterpret_cast<uint2*>(to + i * ps) = encode8<E4M3>(*reinterpret_cast<const uint4*>(x + i * xs), a.bf16, by, odd);
-    if (now > old) {
-      if (lane == 0 && (alone || warp == 0)) *scale = now;
-      if (row0 > 0) {
-        const float ratio = __fdiv_rn(old, now);
-        if (!alone) {
-          again(pool, row0, ratio, warp, kAppendWarps);
-        } else if (lane == 0) {
-          s_job[atomicAdd(&s_jobs, 1)] = Job{pool, row0, ratio};
-        }
+      for (int k = 0; k < kPieces; ++k, to += to_step)
+        if (w0 + k * kStep < n) *reinterpret_cast<uint2*>(to) = encode8<E4M3>(rows[k * kAppendWarps * 32], a.bf16, by, odd);
+      for (int i = w0 + kept, k = 0; i < n; i += kStep, ++k, to += to_step)
+        *reinterpret_cast<uint2*>(to) = encode8<E4M3>(*reinterpret_cast<const uint4*>(x + k * x_step), a.bf16, by, odd);
+      if (now > old) {
+        if (tid == 0) *scale = now;
+        if (row0 > 0) again(pool, ps, row0, __fdiv_rn(old, now), warp, kAppendWarps);
       }
     }
   }
   __syncthreads();
-  for (int j = 0; j < s_jobs; ++j) again(s_job[j].rows, s_job[j].n, s_job[j].ratio, warp, kAppendWarps);
+  for (int j = 0; j < s_jobs; ++j) again(s_job[j].rows, s_job[j].stride, s_job[j].n, s_job[j].ratio, warp, kAppendWarps);
 }
 
 template <int D>
 dk_status launch_append(const AppendArgs& a, bool e4m3, cudaStream_t stream) {
-  const dim3 grid((a.tokens + a.window - 1) / a.window, a.kv_heads, 2);
+  const dim3 grid((a.tokens + a.window - 1) / a.window, (2 * a.kv_heads + a.items - 1) / a.items);
+  // Runs are as long as the call has tokens, or a page.
+  const bool long_runs = std::min(a.tokens, a.block_size) > kShortRun;
+  const size_t smem = long_runs ? (a.items > 1 ? 2 : 1) * kPieces * kAppendWarps * 32 * sizeof(uint4) : 0;
   return launch_early("dk_cache_append", e4m3 ? k_cache_append<D, true> : k_cache_append<D, false>, grid,
-                      dim3(kAppendWarps * 32), 0, stream, a);
+                      dim3(kAppendWarps * 32), smem, stream, a);
 }
 
 }  // namespace
@@ -513,6 +604,7 @@ extern "C" dk_status dk_cache_plan(const int32_t* held, const int32_t* fresh, in
   a.block_size = block_size;
   a.free_capacity = free_capacity;
   a.tokens = tokens;
+  a.block_magic = (unsigned)(((1ull << 32) + block_size - 1) / block_size);
   const size_t smem = sizeof(int) * (4 * (size_t)requests + 3);
   // Two slots a thread are the least latency; from where those would need more
   // threads than the GPU holds, eight share a search and their pages.
@@ -583,8 +675,12 @@ extern "C" dk_status dk_cache_append(const dk_cache8* c, const void* k, const vo
   a.block_magic = ~0ull / (unsigned long long)c->block_size + 1;
   // The window: four tokens, one for each warp, while the GPU holds the CTAs
   // that this makes; more where most windows would hold no run's beginning.
+  // With large windows a CTA takes several heads, as long as there are two CTAs
+  // for each that the GPU holds: it reads the slots once for all of them.
   const long long each = (long long)tokens * c->kv_heads * 2, room = 20LL * sm_count(-1);
   a.window = each / kAppendWarps <= room ? kAppendWarps : each / 16 <= room ? 16 : kMaxWindow;
+  a.items = 1;
+  while (a.window == kMaxWindow && a.items < kMaxItems && each / kMaxWindow / (2 * a.items) >= 10LL * sm_count(-1)) a.items *= 2;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool e4m3 = c->code == DK_E4M3;
   if (c->head_dim == 64) return launch_append<64>(a, e4m3, st);
