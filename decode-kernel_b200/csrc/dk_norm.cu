@@ -31,9 +31,11 @@ struct NormArgs {
   long long residual_stride, y_stride, gate_stride, residual_out_stride, h_stride;
   int gate_columns;  // 1: one gate a value, 0: one a row
   int rows, dim;
-  int layer, act;
+  int layer, act, row_threads;
   float residual_scale, block_scale, eps, inverse_dim;
 };
+
+enum Fit { kAligned, kShifted, kLoose };  // how the rows lie in memory
 
 // VEC neighbouring values of a row, kept in the words that they are loaded in.
 template <typename T, int VEC>
@@ -69,6 +71,14 @@ struct Pack {
       for (int i = 0; i < kWords / 4; ++i) static_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
     }
   }
+  __device__ __forceinline__ void load_one(int j, const void* p) {
+    if constexpr (sizeof(T) == 4) w[j] = *static_cast<const uint32_t*>(p);
+    else w[j / 2] |= (uint32_t)*static_cast<const uint16_t*>(p) << (16 * (j & 1));
+  }
+  __device__ __forceinline__ void store_one(int j, void* p) const {
+    if constexpr (sizeof(T) == 4) *static_cast<uint32_t*>(p) = w[j];
+    else *static_cast<uint16_t*>(p) = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
+  }
   __device__ __forceinline__ float get(int j) const {
     if constexpr (sizeof(T) == 4) {
       return __uint_as_float(w[j]);
@@ -99,22 +109,28 @@ struct Pack {
   }
 };
 
-// Sum over the threads of one row (TPR of them, whole warps).  `turn` counts
+// Sum over the threads of one row (W warps; 0: `warps` of them).  `turn` counts
 // the kernel's sums: neighbours use different scratch, so one barrier each is
 // enough.
-template <int TPR, int ROWS>
-__device__ __forceinline__ float row_sum(float x, float (*scratch)[TPR * ROWS / 32], int& turn) {
+template <int W>
+__device__ __forceinline__ float row_sum(float x, int warps, float (*scratch)[32], int& turn) {
 #pragma unroll
   for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-  if constexpr (TPR > 32) {
-    constexpr int W = TPR / 32;
+  if (W ? W > 1 : warps > 1) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     float* mine = scratch[turn++ & 1];
     if (lane == 0) mine[warp] = x;
     __syncthreads();
-    x = mine[warp / W * W + lane % W];
+    if constexpr (W && (W & (W - 1)) == 0) {
+      x = mine[warp / W * W + lane % W];
 #pragma unroll
-    for (int d = W / 2; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+      for (int d = W / 2; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+    } else {
+      const int w = W ? W : warps;
+      x = lane < w ? mine[warp - warp % w + lane] : 0.f;
+#pragma unroll
+      for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+    }
   }
   return x;
 }
@@ -127,27 +143,86 @@ __device__ __forceinline__ float sigmoid(float x) {
   return y;
 }
 
-// VEC neighbouring values, NV times; TPR threads a row, ROWS rows a CTA.  What
-// comes from HBM (residual, y, a full gate) is loaded before anything is used,
-// so that one latency is waited for and not one for each norm; the weights too
-// where the registers allow it (NV == 1).
-template <typename T, typename R, int VEC, int NV, int TPR, int ROWS>
-__global__ void __launch_bounds__(TPR* ROWS) k_block_norm(const __grid_constant__ NormArgs a) {
+// VEC neighbouring values, NV times; TPR threads a row (0: a.row_threads), as
+// many rows a CTA as its threads serve.  What comes from HBM (residual, y, a full gate) is
+// loaded before anything is used, so that one latency is waited for and not one
+// for each norm; the weights too where the registers allow it (NV == 1).
+//
+// SHIFT: rows that do not begin on a 16-byte boundary (an odd dim).  All of
+// them lie the same way in memory, so a row is cut where its addresses are
+// multiples of eight values: pieces in the middle are whole accesses, the first
+// and the last are read and written value by value, and the weights, which
+// begin where their array does, are put together from 4-byte words.
+template <typename T, typename R, int VEC, int NV, bool SHIFT, int TPR, int THREADS>
+__global__ void __launch_bounds__(THREADS) k_block_norm(const __grid_constant__ NormArgs a) {
+  static_assert(!SHIFT || VEC == 8, "");
   constexpr bool kEarlyGate = NV * VEC <= 16, kEarlyWeights = NV == 1;
-  __shared__ float scratch[2][TPR * ROWS / 32];
+  __shared__ float scratch[2][32];
   int turn = 0;
-  const int tid = threadIdx.x % TPR;
-  const long long row = (long long)blockIdx.x * ROWS + threadIdx.x / TPR;
+  const int threads = TPR ? TPR : a.row_threads, warps = threads >> 5;
+  const int tid = threadIdx.x % threads;
+  const long long row = (long long)blockIdx.x * (TPR ? THREADS / TPR : blockDim.x / threads) + threadIdx.x / threads;
   const bool live = row < a.rows;
+  const int shift = SHIFT ? (int)(((unsigned)row * (unsigned)a.residual_stride) & 7u) : 0;
   using PT = Pack<T, VEC>;
   using PR = Pack<R, VEC>;
-  auto at = [&](int i) { return (i * TPR + tid) * VEC; };
+  auto at = [&](int i) { return (i * threads + tid) * VEC - shift; };  // may be below 0
   auto in = [&](int i) { return live && at(i) < a.dim; };
-  // Values past the row's end are zeros.
+  auto whole = [&](int i) { return !SHIFT || (at(i) >= 0 && at(i) + VEC <= a.dim); };
+  auto there = [&](int i, int j) { return !SHIFT || (at(i) + j >= 0 && at(i) + j < a.dim); };
+  // Values outside the row are zeros.
+  auto fetch_row = [&](auto pack, const auto* base, int i) {
+    pack.clear();
+    if (in(i)) {
+      if (whole(i)) {
+        pack.load(base + at(i));
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          if (there(i, j)) pack.load_one(j, base + at(i) + j);
+      }
+    }
+    return pack;
+  };
+  auto store_row = [&](const auto& pack, auto* base, int i) {
+    if (!in(i)) return;
+    if (whole(i)) {
+      pack.store(base + at(i));
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (there(i, j)) pack.store_one(j, base + at(i) + j);
+    }
+  };
+  // A weight's values for piece i.
   auto fetch = [&](const void* base, int i) {
     PT w;
-    w.clear();
-    if (in(i)) w.load(static_cast<const T*>(base) + at(i));
+    const T* p = static_cast<const T*>(base);
+    if constexpr (!SHIFT) {
+      w = fetch_row(PT{}, p, i);
+    } else if (in(i) && at(i) >= 1 && at(i) + VEC < a.dim) {  // the words around it are within the array
+      const uintptr_t from = reinterpret_cast<uintptr_t>(p + at(i));
+      const uint32_t* q = reinterpret_cast<const uint32_t*>(from & ~uintptr_t(3));
+      if (from & 2) {
+        uint32_t word = q[0];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t next = q[k + 1];
+          w.w[k] = prmt(word, next, 0x5432);
+          word = next;
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w.w[k] = q[k];
+      }
+    } else {
+      w.clear();
+      if (in(i)) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          if (there(i, j)) w.load_one(j, p + at(i) + j);
+      }
+    }
     return w;
   };
   pdl_trigger();
@@ -155,22 +230,22 @@ __global__ void __launch_bounds__(TPR* ROWS) k_block_norm(const __grid_constant_
   PR pr[NV];
   PT py[NV], pg[NV], pw[NV], ph[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    pr[i].clear();
-    if (in(i)) pr[i].load(static_cast<const R*>(a.residual) + row * a.residual_stride + at(i));
-  }
+  for (int i = 0; i < NV; ++i) pr[i] = fetch_row(PR{}, static_cast<const R*>(a.residual) + row * a.residual_stride, i);
   if (a.y) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) py[i] = fetch(static_cast<const T*>(a.y) + row * a.y_stride, i);
+    for (int i = 0; i < NV; ++i) py[i] = fetch_row(PT{}, static_cast<const T*>(a.y) + row * a.y_stride, i);
   }
+  // A gate of a row's own lies as the row does, one gate for all rows as a weight.
   const T* gate = static_cast<const T*>(a.gate) + row * a.gate_stride;
+  auto fetch_gate = [&](int i) { return a.gate_stride ? fetch_row(PT{}, gate, i) : fetch(a.gate, i); };
   Pack<T, 1> row_gate;
+  row_gate.clear();
   if (a.gate) {
     if (!a.gate_columns) {
       if (live) row_gate.load(gate);
     } else if (kEarlyGate) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) pg[i] = fetch(gate, i);
+      for (int i = 0; i < NV; ++i) pg[i] = fetch_gate(i);
     }
   }
   if (kEarlyWeights && a.post_weight) {
@@ -190,17 +265,17 @@ __global__ void __launch_bounds__(TPR* ROWS) k_block_norm(const __grid_constant_
       for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int j = 0; j < VEC; ++j) s += x[i][j];
-      mean = row_sum<TPR, ROWS>(s, scratch, turn) * a.inverse_dim;
+      mean = row_sum<TPR / 32>(s, warps, scratch, turn) * a.inverse_dim;
     }
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        if (a.layer) x[i][j] = in(i) ? x[i][j] - mean : 0.f;
+        if (a.layer) x[i][j] = in(i) && there(i, j) ? x[i][j] - mean : 0.f;
         s = fmaf(x[i][j], x[i][j], s);
       }
-    const float f = rsqrtf(row_sum<TPR, ROWS>(s, scratch, turn) * a.inverse_dim + a.eps);
+    const float f = rsqrtf(row_sum<TPR / 32>(s, warps, scratch, turn) * a.inverse_dim + a.eps);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const PT w = kEarlyWeights ? early[i] : fetch(weight, i);
@@ -232,7 +307,7 @@ __global__ void __launch_bounds__(TPR* ROWS) k_block_norm(const __grid_constant_
       if (a.gate_columns) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-          const PT g = kEarlyGate ? pg[i] : fetch(gate, i);
+          const PT g = kEarlyGate ? pg[i] : fetch_gate(i);
 #pragma unroll
           for (int j = 0; j < VEC; ++j) x[i][j] *= open_gate(g.get(j));
         }
@@ -255,52 +330,68 @@ __global__ void __launch_bounds__(TPR* ROWS) k_block_norm(const __grid_constant_
       for (int j = 0; j < VEC; ++j) x[i][j] = a.residual_scale * pr[i].get(j);
   }
   if (a.residual_out) {
-    R* p = static_cast<R*>(a.residual_out) + row * a.residual_out_stride;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       PR o;
       o.put(x[i]);
-      if (in(i)) o.store(p + at(i));
+      store_row(o, static_cast<R*>(a.residual_out) + row * a.residual_out_stride, i);
     }
   }
   if (a.h) {
     norm(x, ph, a.pre_weight, a.pre_bias);
-    T* p = static_cast<T*>(a.h) + row * a.h_stride;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       PT o;
       o.put(x[i]);
-      if (in(i)) o.store(p + at(i));
+      store_row(o, static_cast<T*>(a.h) + row * a.h_stride, i);
     }
   }
 }
 
-template <typename T, typename R, int VEC, int NV, int TPR, int ROWS>
-dk_status launch_shape(const NormArgs& a, cudaStream_t stream) {
-  return launch_early("dk_block_norm", k_block_norm<T, R, VEC, NV, TPR, ROWS>, dim3((a.rows + ROWS - 1) / ROWS),
-                      dim3(TPR * ROWS), 0, stream, a);
+// TPR threads a row, THREADS a CTA.
+template <typename T, typename R, int NV, int TPR, int THREADS = TPR>
+dk_status launch_fixed(const NormArgs& a, cudaStream_t stream) {
+  constexpr int kRows = THREADS / TPR;
+  return launch_early("dk_block_norm", k_block_norm<T, R, 8, NV, false, TPR, THREADS>, dim3((a.rows + kRows - 1) / kRows),
+                      dim3(THREADS), 0, stream, a);
+}
+// As many threads as the row's pieces want.
+template <typename T, typename R, int VEC, int NV, bool SHIFT, int THREADS>
+dk_status launch_any(NormArgs a, int pieces, cudaStream_t stream) {
+  a.row_threads = (pieces + NV * 32 - 1) / (NV * 32) * 32;
+  const int rows = std::max(1, 128 / a.row_threads);  // short rows share a CTA of 128 threads
+  return launch_early("dk_block_norm", k_block_norm<T, R, VEC, NV, SHIFT, 0, THREADS>, dim3((a.rows + rows - 1) / rows),
+                      dim3(a.row_threads * rows), 0, stream, a);
 }
 
-// 8 values a thread while a CTA has the threads, which is the least latency;
-// with rows for every SM 16 a thread, which keeps more bytes in flight.
+// Eight values a thread while a CTA has the threads, which is the least
+// latency; with rows for every SM 16 a thread from rows of 2048 on, which keeps
+// more bytes in flight (8192x8192 with a full gate: 16 a thread 117 us, 32 121,
+// 8 192).  Threads a row are fixed where rows are aligned: with a number of the
+// call's the same case takes 140 us.
 template <typename T, typename R>
-dk_status launch_norm(const NormArgs& a, bool packed, cudaStream_t stream) {
-  if (packed) {
-    const int packs = a.dim / 8;
-    const bool many = a.rows >= 2 * sm_count(-1);
-    if (packs <= 32) return launch_shape<T, R, 8, 1, 32, 4>(a, stream);
-    if (packs <= 64) return launch_shape<T, R, 8, 1, 64, 2>(a, stream);
-    if (packs <= 128) return launch_shape<T, R, 8, 1, 128, 1>(a, stream);
-    if (packs <= 256) return launch_shape<T, R, 8, 1, 256, 1>(a, stream);
-    if (packs <= 512) return many ? launch_shape<T, R, 8, 2, 256, 1>(a, stream) : launch_shape<T, R, 8, 1, 512, 1>(a, stream);
-    if (packs <= 1024) return many ? launch_shape<T, R, 8, 2, 512, 1>(a, stream) : launch_shape<T, R, 8, 1, 1024, 1>(a, stream);
-    if (packs <= 2048) return launch_shape<T, R, 8, 4, 512, 1>(a, stream);
-    return launch_shape<T, R, 8, 8, 512, 1>(a, stream);
+dk_status launch_norm(const NormArgs& a, Fit fit, cudaStream_t stream) {
+  const bool many = a.rows >= 2 * sm_count(-1);
+  const int pieces = (a.dim + 7) / 8;
+  if (fit == kAligned) {
+    if (pieces <= 32) return launch_fixed<T, R, 1, 32, 128>(a, stream);
+    if (pieces <= 64) return launch_fixed<T, R, 1, 64, 128>(a, stream);
+    if (pieces <= 128) return launch_fixed<T, R, 1, 128>(a, stream);
+    if (pieces <= 256) return launch_fixed<T, R, 1, 256>(a, stream);
+    if (pieces <= 512) return many ? launch_fixed<T, R, 2, 256>(a, stream) : launch_fixed<T, R, 1, 512>(a, stream);
+    if (pieces <= 768) return many ? launch_fixed<T, R, 2, 384>(a, stream) : launch_fixed<T, R, 1, 1024>(a, stream);
+    if (pieces <= 1024) return many ? launch_fixed<T, R, 2, 512>(a, stream) : launch_fixed<T, R, 1, 1024>(a, stream);
+    if (pieces <= 2048) return launch_fixed<T, R, 4, 512>(a, stream);
+    return launch_fixed<T, R, 8, 512>(a, stream);
   }
-  if (a.dim <= 256) return launch_shape<T, R, 1, 8, 32, 4>(a, stream);
-  if (a.dim <= 2048) return launch_shape<T, R, 1, 8, 256, 1>(a, stream);
-  if (a.dim <= 8192) return launch_shape<T, R, 1, 16, 512, 1>(a, stream);
-  return launch_shape<T, R, 1, 64, 512, 1>(a, stream);
+  if (fit == kShifted) {  // a row may lie over one more piece
+    if (pieces < (many ? 256 : 1024)) return launch_any<T, R, 8, 1, true, 1024>(a, pieces + 1, stream);
+    if (pieces < 1024) return launch_any<T, R, 8, 2, true, 512>(a, pieces + 1, stream);
+    if (pieces < 2048) return launch_any<T, R, 8, 4, true, 512>(a, pieces + 1, stream);
+    return launch_any<T, R, 8, 8, true, 544>(a, pieces + 1, stream);
+  }
+  if (a.dim <= 8192) return launch_any<T, R, 1, 8, false, 1024>(a, a.dim, stream);
+  return launch_any<T, R, 1, 64, false, 512>(a, a.dim, stream);
 }
 
 }  // namespace
@@ -346,19 +437,29 @@ extern "C" dk_status dk_block_norm(const dk_block_norm_args* p, void* stream) {
   a.block_scale = p->block_scale;
   a.eps = p->eps;
   a.inverse_dim = 1.f / (float)p->dim;
-  // 16-byte accesses need every row of every operand on such a boundary.
-  auto fits = [&](const void* x, int64_t stride) {
-    return !x || (aligned16(x) && (p->rows == 1 || stride % 8 == 0));
+  // Rows that all begin on a 16-byte boundary are read in whole pieces; rows
+  // that do not, but all in the same way (strides alike to multiples of eight
+  // values), in pieces that are cut at the boundaries; others value by value.
+  bool bases = true, aligned = p->dim % 8 == 0, alike = true;
+  auto rows_of = [&](const void* x, int64_t stride) {
+    if (!x) return;
+    bases = bases && aligned16(x);
+    aligned = aligned && (p->rows == 1 || stride % 8 == 0);
+    alike = alike && (p->rows == 1 || (stride - p->residual_stride) % 8 == 0);
   };
-  const bool packed = p->dim % 8 == 0 && fits(p->residual, p->residual_stride) &&
-                      fits(p->y, p->y_stride) && fits(p->residual_out, p->residual_out_stride) &&
-                      fits(p->h, p->h_stride) && fits(p->post_weight, 0) && fits(p->post_bias, 0) &&
-                      fits(p->pre_weight, 0) && fits(p->pre_bias, 0) &&
-                      (!a.gate_columns || fits(p->gate, p->gate_stride));
+  rows_of(p->residual, p->residual_stride);
+  rows_of(p->y, p->y_stride);
+  rows_of(p->residual_out, p->residual_out_stride);
+  rows_of(p->h, p->h_stride);
+  if (a.gate_columns && p->gate_stride) rows_of(p->gate, p->gate_stride);
+  bool weights = true;  // and what is the same for all rows, from a boundary
+  for (const void* w : {p->post_weight, p->post_bias, p->pre_weight, p->pre_bias}) weights = weights && aligned16(w);
+  if (p->gate && a.gate_columns && !p->gate_stride) weights = weights && aligned16(p->gate);
+  const Fit fit = bases && aligned && weights ? kAligned : bases && alike ? kShifted : kLoose;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool wide = p->residual_dtype == DK_FP32;
   if (p->dtype == DK_FP16)
-    return wide ? launch_norm<__half, float>(a, packed, st) : launch_norm<__half, __half>(a, packed, st);
-  return wide ? launch_norm<__nv_bfloat16, float>(a, packed, st)
-              : launch_norm<__nv_bfloat16, __nv_bfloat16>(a, packed, st);
+    return wide ? launch_norm<__half, float>(a, fit, st) : launch_norm<__half, __half>(a, fit, st);
+  return wide ? launch_norm<__nv_bfloat16, float>(a, fit, st)
+              : launch_norm<__nv_bfloat16, __nv_bfloat16>(a, fit, st);
 }

@@ -745,6 +745,34 @@ def test_norm_strided_rows():
     assert torch.equal(big[:, 8:520], dk.block_norm(keep[:, 8:520], keep[:, 512:1024])[0])
 
 
+@pytest.mark.parametrize("residual", [torch.float16, torch.float32])
+@pytest.mark.parametrize("dim,width", [(65, 73), (65, 70), (1001, 1009), (1001, 1002), (7, 7), (2049, 2049), (9001, 9009)])
+def test_norm_rows_off_the_boundary(residual, dim, width):
+    """Rows that begin anywhere: alike (strides equal to multiples of 8) and not; weights on odd places too."""
+    g = gen(dim + width)
+    rows = 37
+    r = torch.randn(rows, width, generator=g).to(residual)
+    y = torch.randn(rows, dim, generator=g).half()
+    gate = torch.randn(rows, dim, generator=g).half()
+    w = torch.randn(4 * dim + 1, generator=g).half()
+    pw, pb, hw, hb = (w[i * dim + 1:(i + 1) * dim + 1] for i in range(4))
+    d = w.cuda()
+    dpw, dpb, dhw, dhb = (d[i * dim + 1:(i + 1) * dim + 1] for i in range(4))
+    keep = r.cuda()
+    for kind in ("rms", "layer"):
+        want_r, want_h = norm_reference(r[:, :dim], y, kind, pw, pb, gate, "sigmoid", 0.9, 1.3, hw, hb, 1e-5)
+        for inplace in (False, True):
+            rd = keep.clone()
+            got_r, got_h = dk.block_norm(rd[:, :dim], y.cuda(), kind=kind, post_weight=dpw, post_bias=dpb, gate=gate.cuda(), gate_act="sigmoid",
+                                         residual_scale=0.9, block_scale=1.3, pre_weight=dhw, pre_bias=dhb, eps=1e-5, inplace=inplace)
+            assert torch.equal(rd[:, dim:], keep[:, dim:])
+            unit = 2.0 ** -11 if residual == torch.float16 else 2.0 ** -24
+            f32 = 64 * 2.0 ** -24
+            size = r[:, :dim].double().abs() + want_r.abs() + 4 * pb.double().abs()
+            assert ((got_r.double().cpu() - want_r).abs() <= unit * want_r.abs() + f32 * (size + 4)).all()
+            assert ((got_h.double().cpu() - want_h).abs() <= 2.0 ** -11 * want_h.abs() + f32 * (want_h.abs() + 16 * hw.double().abs() + hb.double().abs()) + 1e-7).all()
+
+
 def test_norm_of_nothing_zeros_and_odd_values():
     w = torch.ones(64, dtype=torch.float16, device="cuda")
     e = torch.empty(0, 64, dtype=torch.float16, device="cuda")
