@@ -311,11 +311,11 @@ void check_table(const torch::Tensor& t, int64_t requests, const torch::Device& 
 
 // A tensor over part of another's storage, without the dispatcher's work of a
 // view (a plan makes four small tensors every step).
-torch::Tensor part_of(const torch::Tensor& whole, torch::ScalarType type, int64_t byte, int64_t n) {
+torch::Tensor part_of(const torch::Tensor& whole, torch::ScalarType type, int64_t byte, c10::IntArrayRef sizes) {
   torch::Tensor t = at::detail::make_tensor<c10::TensorImpl>(
       c10::Storage(whole.storage()), whole.key_set(), c10::scalarTypeToTypeMeta(type));
   t.unsafeGetTensorImpl()->set_storage_offset(byte / static_cast<int64_t>(c10::elementSize(type)));
-  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
   return t;
 }
 
@@ -345,7 +345,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> cache_pla
   if (!lengths || !starts || !slots || !ring_out)
     whole = torch::empty({bytes}, held.options().dtype(torch::kUInt8));
   auto given = [&](OptTensor& t, torch::ScalarType type, int64_t at, int64_t size, const char* what) {
-    if (!t) return part_of(whole, type, at, size);
+    if (!t) return part_of(whole, type, at, {size});
     check_ints(*t, type, size, device, what);
     return *t;
   };
@@ -533,14 +533,22 @@ std::tuple<torch::Tensor, OptTensor> block_norm(torch::Tensor residual, OptTenso
   a.pre_weight = weight(pre_weight, "pre_weight");
   a.pre_bias = weight(pre_bias, "pre_bias");
   // Without y and with a scale of 1 the residual stays what it is.
+  // Two small outputs of one type come from one allocation.
+  OptTensor result;
+  const int64_t bytes = (residual.numel() * 2 + 15) / 16 * 16;
+  if ((y || residual_scale != 1.0) && !inplace && pre_weight && residual.scalar_type() == type &&
+      bytes <= (1 << 18)) {
+    const torch::Tensor whole = torch::empty({2 * bytes}, residual.options().dtype(torch::kUInt8));
+    out = part_of(whole, type, 0, residual.sizes());
+    result = part_of(whole, type, bytes, residual.sizes());
+  }
   if (y || residual_scale != 1.0) {
-    if (!inplace) out = torch::empty(residual.sizes(), residual.options());
+    if (!inplace && !result) out = torch::empty(residual.sizes(), residual.options());
     a.residual_out = out.data_ptr();
     a.residual_out_stride = inplace ? row_stride(r) : dim;
   }
-  OptTensor result;
   if (pre_weight) {
-    result = torch::empty(residual.sizes(), pre_weight->options());
+    if (!result) result = torch::empty(residual.sizes(), pre_weight->options());
     a.h = result->data_ptr();
     a.h_stride = dim;
   }

@@ -196,6 +196,7 @@ struct Attend {
     int group[kSlots + 1];
     Segment seg[kSlots];
     Segment fed[W], now[W];            // the segments whose units a warp copies and adds up
+    int4 rows[W][kRows];               // of the latter's rows: token (-1: no such row), head, low, high
     int used[kSlots];
     int last[2];
     int total[W], longest[W];
@@ -297,17 +298,14 @@ struct Attend {
     return true;
   }
 
-  // Row `row` of q as this lane's words of the B operand, in K's order of
-  // channels.
-  __device__ static __forceinline__ void load_q(const AttendArgs& a, const Segment& s, int row, uint32_t (&b)[2 * kKWords]) {
+  // A row of q as this lane's words of the B operand, in K's order of channels.
+  __device__ static __forceinline__ void load_q(const AttendArgs& a, const int4& row, uint32_t (&b)[2 * kKWords]) {
     const int c = threadIdx.x & 3;
-    int token, head, low, high;
-    const bool there = row_of(a, s, row, token, head, low, high);
     constexpr int kSpan = D >= 128 ? 32 : 16;  // channels of a lane's contiguous piece
 #pragma unroll
     for (int i = 0; i < 2 * kKWords; ++i) b[i] = 0;
-    if (there) {
-      const uint16_t* p = static_cast<const uint16_t*>(a.q) + token * a.q_token_stride + head * a.q_head_stride + c * kSpan;
+    if (row.x >= 0) {
+      const uint16_t* p = static_cast<const uint16_t*>(a.q) + row.x * a.q_token_stride + row.y * a.q_head_stride + c * kSpan;
 #pragma unroll
       for (int i = 0; i < kKWords / 2; ++i) {  // 8 channels each
         const int at = (i * 8) % kSpan + (i * 8) / kSpan * 128;
@@ -433,40 +431,31 @@ struct Attend {
     uint32_t unseen;  // rows (bits) of this lane's columns without a token yet, whose m is 0
     bool settled;     // no lane has any
 
-    __device__ __forceinline__ void begin(const AttendArgs& a, const Segment& s, uint32_t ring) {
+    // `table` gets the segment's rows.
+    __device__ __forceinline__ void begin(const AttendArgs& a, const Segment& s, uint32_t ring, int4* table) {
       const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+      int token, head, low = 0, high = 0;
+      const bool there = lane < kRows && row_of(a, s, lane, token, head, low, high);
+      if (lane < kRows) table[lane] = make_int4(there ? token : -1, head, low, high);
+      __syncwarp();
       uint32_t mine[NT][2 * kKWords];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) load_q(a, s, n * 8 + g, mine[n]);
-      least_high = least_low = 0x7fffffff;
-      most_low = most_high = 0;
-      unseen = (1u << (2 * NT)) - 1u;
-      settled = false;
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (s.fresh != 1) {
-            int token, head, low, high;
-            const bool there = row_of(a, s, n * 8 + 2 * c + i, token, head, low, high);
-            least_high = min(least_high, there ? high : 0x7fffffff);
-            least_low = min(least_low, there ? low : 0x7fffffff);
-            most_low = max(most_low, low);
-            most_high = max(most_high, high);
-          }
-          m[n][i] = 0.f;
-          l[n][i] = 0.f;
-        }
-      }
+      for (int n = 0; n < NT; ++n) load_q(a, table[n * 8 + g], mine[n]);
       if (s.fresh == 1) {  // all rows are one query's
         least_high = most_high = s.length;
         least_low = most_low = a.window > 0 ? max(0, s.length - a.window) : 0;
       } else {
-        least_high = __reduce_min_sync(0xffffffffu, least_high);
-        most_low = __reduce_max_sync(0xffffffffu, most_low);
-        least_low = __reduce_min_sync(0xffffffffu, least_low);
-        most_high = __reduce_max_sync(0xffffffffu, most_high);
+        least_high = __reduce_min_sync(0xffffffffu, there ? high : 0x7fffffff);
+        least_low = __reduce_min_sync(0xffffffffu, there ? low : 0x7fffffff);
+        most_low = __reduce_max_sync(0xffffffffu, low);
+        most_high = __reduce_max_sync(0xffffffffu, high);
       }
+      unseen = (1u << (2 * NT)) - 1u;
+      settled = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) m[n][i] = l[n][i] = 0.f;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const float up = convert_q(a, mine[n]);
@@ -526,9 +515,9 @@ struct Attend {
       settled = !__any_sync(0xffffffffu, unseen);
     }
 
-    // The unit of tokens base.. of segment s in the stage at `at`; hidden: its
+    // The unit of tokens base.. of the segment in the stage at `at`; hidden: its
     // tiles (bits) whose pages are outside the pool.
-    __device__ __forceinline__ void add(const AttendArgs& a, const Segment& s, int base, uint32_t at, uint32_t ring, uint32_t hidden) {
+    __device__ __forceinline__ void add(const int4* table, int base, uint32_t at, uint32_t ring, uint32_t hidden) {
       const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
       // Scores: [16 tokens][8 rows] for each tile of tokens and of rows, one tile
       // alone in two chains.
@@ -589,9 +578,8 @@ struct Attend {
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              int token, head, low, high;
-              row_of(a, s, n * 8 + 2 * c + i, token, head, low, high);
-              const int t = first + g;
+              const int2 sees = *reinterpret_cast<const int2*>(&table[n * 8 + 2 * c + i].z);
+              const int low = sees.x, high = sees.y, t = first + g;
               if (t >= high || t < low || !good) sc[h][n][i] = -INFINITY;
               if (t + 8 >= high || t + 8 < low || !good) sc[h][n][i + 2] = -INFINITY;
             }
@@ -664,17 +652,17 @@ struct Attend {
   };
 
   // Channels of o[.][i][j] for lane row group g: 2i + (j >> 1) from g * (D / 8).
-  __device__ static __forceinline__ void write_rows(const AttendArgs& a, const Segment& s, const float (&o)[NT][D / 16][4],
+  __device__ static __forceinline__ void write_rows(const AttendArgs& a, const int4* table, const float (&o)[NT][D / 16][4],
                                                     const float (&m)[NT][2], const float (&l)[NT][2]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        int token, head, low, high;
-        if (!row_of(a, s, n * 8 + 2 * c + i, token, head, low, high)) continue;
+        const int2 at = *reinterpret_cast<const int2*>(&table[n * 8 + 2 * c + i]);
+        if (at.x < 0) continue;
         const float f = l[n][i] > 0.f || l[n][i] != l[n][i] ? 1.f / l[n][i] : 0.f;
-        const long long row = (long long)token * a.kv_heads * a.group + head;
+        const long long row = (long long)at.x * a.kv_heads * a.group + at.y;
 #pragma unroll
         for (int d = 0; d < D / 32; ++d)
           store_row(a, row * D + g * (D / 8) + 4 * d,
@@ -762,12 +750,16 @@ struct Attend {
     if (tid == 0) prefix[a.requests] = all;
     __syncthreads();
     // Every CTA has the same number of places (the last has the rest), one for
-    // each of its warps at least; CTA u / chunk has place u.  Where segments
+    // each of its warps at least; CTA u / chunk has place u.  Nor is a segment
+    // of n units cut in more than about sqrt(2 n) parts: one CTA joins them, at
+    // a time for each that a warp needs for half a unit.  (Three requests of up
+    // to 36 thousand tokens and one KV head: 30.7 -> 20.9 us.)  Where segments
     // are short the borders move to the nearest segment's, so that no segment
     // is shared between CTAs: joining one costs about as long as the units do
     // that a CTA gets too many.  (64 requests of up to 200 tokens 15.6 -> 12.0
     // us, of up to 1000 24.8 -> 21.6; from 2000 tokens on it makes no odds.)
-    const int grid = min((int)gridDim.x, (all + W - 1) / W);
+    const int least = max(W, (int)sqrtf(0.5f * longest));
+    const int grid = min((int)gridDim.x, (all + least - 1) / least);
     const int chunk = (all + grid - 1) / grid;
     const int cta = blockIdx.x;
     if (cta >= grid || cta * chunk >= all) return;
@@ -813,14 +805,14 @@ struct Attend {
       for (int u = u0;;) {
         const int from = max(0, u - s.begin), to = min(s.units, u1 - s.begin);
         if (to <= 0) break;  // only the segment's start is this warp's
-        rows.begin(a, s, ring);
+        rows.begin(a, s, ring, sh.rows[warp]);
         int base = (s.unit0 + from) * kUnit;
 #pragma unroll 1
         for (int i = from; i < to; ++i) {
           copy_wait<S - 2>();
           __syncwarp();  // the unit is there for all lanes, and the stage before it has been read by all
           feed.next(a, prefix, sh.fed[warp], freed, freed_stage);
-          rows.add(a, s, base, ring + offset, ring, feed.hidden >> (stage * MT));
+          rows.add(sh.rows[warp], base, ring + offset, ring, feed.hidden >> (stage * MT));
           base += kUnit;
           freed = offset;
           freed_stage = stage;
@@ -830,7 +822,7 @@ struct Attend {
         rows.finish();
         u = s.begin + to;
         if (from == 0 && to == s.units) {
-          write_rows(a, s, rows.o, rows.m, rows.l);
+          write_rows(a, sh.rows[warp], rows.o, rows.m, rows.l);
         } else {
           // An early part, after which the warp goes on, waits in L2; the last
           // one takes the place of the ring, where nothing is left to come.
@@ -1007,13 +999,13 @@ struct Attend {
       const float* f = factor + (end ? n0 : 0) * kRows + r;
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-      for (int i = 0; i < n; i += 8) {
-        float4 y[8];
+      for (int i = 0; i < n; i += 16) {
+        float4 y[16];
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
+        for (int k = 0; k < 16; ++k)
           if (i + k < n) y[k] = __ldcg(reinterpret_cast<const float4*>(part(end, i + k) + r * D + d));
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
+        for (int k = 0; k < 16; ++k)
           if (i + k < n) add_part(y[k], f[(i + k) * kRows], x);
       }
       store_joined(a, sh.place[end][r], d, x, sh.by[end][r]);
