@@ -909,17 +909,32 @@ struct Attend {
       }
     }
     __syncthreads();
-    constexpr int kQuads = kRows * D / 4;
+    // A thread has U elements of four channels of each joined tile.
+    constexpr int kQuads = kRows * D / 4, T = W * 32, U = kQuads > T ? kQuads / T : 1;
+    static_assert(kQuads <= T || kQuads % T == 0, "");
+    auto row_at = [&](int u) { return (tid + u * T) / (D / 4); };
+    const int d = tid % (D / 4) * 4;
+    static_assert(T % (D / 4) == 0, "a thread's elements lie in the same channels");
+    const bool mine_too = tid < kQuads;
 #pragma unroll 1
-    for (int e = tid; e < groups * kQuads; e += W * 32) {
-      const int i = e / kQuads, row = e % kQuads / (D / 4), d = e % (D / 4) * 4;
+    for (int i = 0; i < groups; ++i) {
+      if (!mine_too) break;
       const int end = sh.group[i + 1];
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (int k = sh.group[i]; k < end; ++k) add_part(*reinterpret_cast<const float4*>(sh.part[k] + row * D + d), sh.factor[k][row], x);
-      const int place = sh.place[i][row];
-      if (place >= -1) store_joined(a, place, d, x, sh.by[i][row]);
-      else __stcg(reinterpret_cast<float4*>(a.partials + (long long)(-2 - place) * kPartFloats + row * D + d), x);
+      float4 x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+      for (int k = sh.group[i]; k < end; ++k) {
+        const float* from = sh.part[k] + d;
+#pragma unroll
+        for (int u = 0; u < U; ++u) add_part(*reinterpret_cast<const float4*>(from + row_at(u) * D), sh.factor[k][row_at(u)], x[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int row = row_at(u), place = sh.place[i][row];
+        if (place >= -1) store_joined(a, place, d, x[u], sh.by[i][row]);
+        else __stcg(reinterpret_cast<float4*>(a.partials + (long long)(-2 - place) * kPartFloats + row * D + d), x[u]);
+      }
     }
     // The CTA's first and last segments may be shared with others: the last CTA
     // to arrive joins the parts in the order of the CTAs.
@@ -993,22 +1008,31 @@ struct Attend {
       if (sh.last[warp]) sh.place[warp][lane] = row_place(a, sh.seg[warp ? end_slot[1] : end_slot[0]], lane, warp ? top[1] : top[0], sum, sh.by[warp][lane]);
     }
     __syncthreads();
+    constexpr int kBatch = 16 / U;  // parts that a thread has on their way at once
 #pragma unroll 1
-    for (int e = tid + (n0 ? 0 : kQuads); e < (n1 ? 2 : 1) * kQuads; e += W * 32) {
-      const int end = e >= kQuads, r = e % kQuads / (D / 4), d = e % (D / 4) * 4, n = end ? n1 : n0;
-      const float* f = factor + (end ? n0 : 0) * kRows + r;
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int end = 0; end < 2; ++end) {
+      const int n = end ? n1 : n0;
+      if (n == 0 || !mine_too) continue;
+      const float* f = factor + (end ? n0 : 0) * kRows;
+      float4 x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-      for (int i = 0; i < n; i += 16) {
-        float4 y[16];
+      for (int i = 0; i < n; i += kBatch) {
+        float4 y[kBatch][U];
 #pragma unroll
-        for (int k = 0; k < 16; ++k)
-          if (i + k < n) y[k] = __ldcg(reinterpret_cast<const float4*>(part(end, i + k) + r * D + d));
+        for (int k = 0; k < kBatch; ++k)
 #pragma unroll
-        for (int k = 0; k < 16; ++k)
-          if (i + k < n) add_part(y[k], f[(i + k) * kRows], x);
+          for (int u = 0; u < U; ++u)
+            if (i + k < n) y[k][u] = __ldcg(reinterpret_cast<const float4*>(part(end, i + k) + row_at(u) * D + d));
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (i + k < n) add_part(y[k][u], f[(i + k) * kRows + row_at(u)], x[u]);
       }
-      store_joined(a, sh.place[end][r], d, x, sh.by[end][r]);
+#pragma unroll
+      for (int u = 0; u < U; ++u) store_joined(a, sh.place[end][row_at(u)], d, x[u], sh.by[end][row_at(u)]);
     }
   }
 };
