@@ -170,7 +170,7 @@ struct Attend {
   static constexpr int kSlots = 2 * W;    // a warp's parts of segments: an early one and its last
   // Places in the line that a segment's start counts for: its queries' latency
   // and its rows' end take as long as this many units.
-  static constexpr int kStart = 1;
+  static constexpr int kStart = NT >= 3 ? 2 : 1;
   static constexpr int kUnit = MT * kTile;  // tokens of a unit
   // A stage: each tile's K and V, and their scales.  Multiples of 128 bytes, so
   // that the places of pieces differ by an exclusive or of their low bits.
@@ -240,7 +240,7 @@ struct Attend {
     if (a.starts) {
       const int* starts = lengths + a.requests;
       first = starts[r];
-      fresh = max(0, starts[r + 1] - first);
+      fresh = min(max(0, starts[r + 1] - first), a.tokens);
     } else {
       first = r;
       fresh = 1;
@@ -710,7 +710,7 @@ struct Attend {
         int fresh = 1, unit0;
         if (a.starts) {
           const int first = ld_int(a.starts + r), next = ld_int(a.starts + r + 1);
-          fresh = max(0, next - first);
+          fresh = min(max(0, next - first), a.tokens);
           starts[r] = first;
           if (r == a.requests - 1) starts[r + 1] = next;
         }
@@ -820,6 +820,7 @@ struct Attend {
           if (++stage == S) stage = offset = 0;
         }
         rows.finish();
+        const int before = u;
         u = s.begin + to;
         if (from == 0 && to == s.units) {
           write_rows(a, sh.rows[warp], rows.o, rows.m, rows.l);
@@ -850,7 +851,7 @@ struct Attend {
             sh.used[slot] = 1;
           }
         }
-        if (u >= u1) break;
+        if (u >= u1 || u <= before) break;  // (the second: starts that do not rise)
         int r, which;
         after(a, prefix, s.request, s.which, u, r, which);
         __syncwarp();  // every lane has read s
@@ -1188,7 +1189,7 @@ extern "C" dk_status dk_cache_attention(const dk_cache_attention_args* p, void* 
     return DK_ERR_UNSUPPORTED;
   // The line of units is counted in 32 bits.
   const int group = p->q_heads / c.kv_heads;
-  const long long units = ((long long)p->max_blocks * c.block_size + 15) / 16 + 2;
+  const long long units = ((long long)p->max_blocks * c.block_size + 15) / 16 + 2;  // and a start's places
   const long long per_head = (long long)std::min(p->requests, kMaxRequests) + (long long)p->tokens * group / 8;
   if (units > INT32_MAX / 16 || per_head > INT32_MAX / 2 / units / c.kv_heads) return DK_ERR_UNSUPPORTED;
   const size_t need = dk_cache_attention_workspace_bytes(c.head_dim);

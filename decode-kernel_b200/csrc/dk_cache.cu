@@ -223,13 +223,14 @@ __global__ void __launch_bounds__(kPlanThreads) k_cache_plan(const __grid_consta
     const int r = last_at(s_need, a.requests, j);
     const int c = s_held[r];
     if (c < 0) continue;
-    const int have = blocks_of(c);
-    a.table[(long long)r * a.table_stride + have + (j - s_need[r])] = a.free_blocks[ring_at(head0, j)];
+    const int block = blocks_of(c) + (j - s_need[r]);
+    if (block < a.max_blocks) a.table[(long long)r * a.table_stride + block] = a.free_blocks[ring_at(head0, j)];
   }
   // Pages of ended requests to the ring's end, where nothing is read.
   for (int j = id; j < carry[2] && j < capacity; j += step) {
     const int r = last_at(s_back, a.requests, j);
-    a.free_blocks[ring_at(tail0, j)] = a.table[(long long)r * a.table_stride + (j - s_back[r])];
+    const int block = j - s_back[r];
+    if (block < a.max_blocks) a.free_blocks[ring_at(tail0, j)] = a.table[(long long)r * a.table_stride + block];
   }
 }
 
