@@ -73,7 +73,7 @@ struct AttendArgs {
   uint32_t k_block_stride, k_token_stride, v_block_stride, v_token_stride;
   int table_stride, max_blocks, blocks, block_size, tiles_per_block;
   int requests, tokens, kv_heads, group;
-  unsigned group_magic;  // ceil(2^32 / group), 0 for a group of 1
+  unsigned group_magic, block_magic;  // for over()
   float scale_log2;
   int causal, window, bf16;
 };
@@ -147,6 +147,13 @@ __device__ __forceinline__ void lds_words(uint32_t at, uint32_t* r) {
   } else {
     asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(at));
   }
+}
+
+// x / by for 0 <= x < 2^31, with magic = ceil(2^32 / by) (0 for by = 1).
+__device__ __forceinline__ int over(int x, int by, unsigned magic) {
+  if (magic == 0) return x;
+  const int q = __umulhi(x, magic);  // the quotient or one more
+  return q - ((long long)q * by > x);
 }
 
 // One (request, KV head, row tile): where its rows, tokens and units are.
@@ -255,7 +262,7 @@ struct Attend {
     s.units = units_of(a, s.length, s.fresh, s.unit0);
     s.which = which;
     s.begin = prefix[r] + which * (s.units + kStart) + kStart;
-    s.blocks = (s.length + a.block_size - 1) / a.block_size;
+    s.blocks = over((s.length + kTile - 1) / kTile + a.tiles_per_block - 1, a.tiles_per_block, a.block_magic);
     const int tiles = tiles_of(a, s.fresh);
     s.all = tiles * a.kv_heads;
     s.head = tiles == 1 ? which : which / tiles;
@@ -264,10 +271,15 @@ struct Attend {
   }
   // The segment of place u of the line.
   __device__ static __forceinline__ Segment segment_at(const AttendArgs& a, const int* prefix, int u) {
-    int lo = 0, hi = a.requests - 1;  // the last request whose first unit is at or before u
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (prefix[mid] <= u) lo = mid; else hi = mid - 1;
+    // The last request whose first unit is at or before u, 32 candidates at a time.
+    const int lane = threadIdx.x & 31;
+    int lo = 0;
+    for (int n = a.requests; n > 1;) {
+      const int step = (n + 31) >> 5, at = lane * step;
+      const uint32_t before = __ballot_sync(0xffffffffu, at < n && prefix[lo + at] <= u);
+      const int skip = (31 - __clz(before | 1u)) * step;
+      lo += skip;
+      n = min(step, n - skip);
     }
     Segment s = segment_of(a, prefix, lo, 0);
     const int which = (u - (s.begin - kStart)) / (s.units + kStart);
@@ -287,8 +299,7 @@ struct Attend {
   // place in q and out; false where the tile has no such row.
   __device__ static __forceinline__ bool row_of(const AttendArgs& a, const Segment& s, int row, int& token, int& head, int& low, int& high) {
     const int all = s.tile * kRows + row;
-    int i = a.group == 1 ? all : __umulhi(all, a.group_magic);  // all / group, or one more
-    i -= i * a.group > all;
+    const int i = over(all, a.group, a.group_magic);
     token = s.first_token + i;
     head = s.head * a.group + all - i * a.group;
     low = high = 0;
@@ -371,7 +382,7 @@ struct Attend {
       scale = (lane & 1 ? a.v_scale : a.k_scale) + s.head;
       unit = max(unit, s.begin);
       const int t = (s.unit0 + unit - s.begin) * MT;
-      block = t / a.tiles_per_block;
+      block = over(t, a.tiles_per_block, a.block_magic);
       sub = t - block * a.tiles_per_block;
       page = page_at(a, s, block);
       next_page = page_at(a, s, block + 1);
@@ -886,18 +897,34 @@ struct Attend {
     uint32_t left = heads;
 #pragma unroll 1
     for (int i = 0; i < groups; ++i, left &= left - 1) {
-      if (i % W != warp || lane >= kRows) continue;
+      if (i % W != warp) continue;
       const int first = __ffs(left) - 1;
       const uint32_t after = left & (left - 1);
       const uint32_t members = valid & ~((left & -left) - 1u) & (after ? (after & -after) - 1u : 0xffffffffu);
-      float top = kFarBelow, l = 0.f;
-      for (uint32_t b = members; b; b &= b - 1) top = fmaxf(top, sh.m[__ffs(b) - 1][lane]);
-      for (uint32_t b = members; b; b &= b - 1) {
-        const int slot = __ffs(b) - 1;
-        const float f = exp2_approx(sh.m[slot][lane] - top);
-        l = fmaf(f, sh.l[slot][lane], l);
-        sh.factor[numbered(slot)][lane] = f;
+      // Lanes beyond the rows take other slots of the same rows.
+      constexpr int P = 32 / kRows, N = (kSlots + P - 1) / P;
+      const int row = lane % kRows, own = lane / kRows;
+      float m[N], top = kFarBelow, l = 0.f;
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const int slot = k * P + own;
+        m[k] = own < P && slot < kSlots && (members >> slot & 1) ? sh.m[slot][row] : -INFINITY;
+        top = fmaxf(top, m[k]);
       }
+#pragma unroll
+      for (int d = kRows; P > 1 && d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const int slot = k * P + own;
+        if (m[k] > -INFINITY) {
+          const float f = exp2_approx(m[k] - top);
+          l = fmaf(f, sh.l[slot][row], l);
+          sh.factor[numbered(slot)][row] = f;
+        }
+      }
+#pragma unroll
+      for (int d = kRows; P > 1 && d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+      if (lane >= kRows) continue;
       const Segment& s = sh.seg[first];
       if (s.begin >= cta0 && s.begin + s.units <= cta1) {
         sh.place[i][lane] = row_place(a, s, lane, top, l, sh.by[i][lane]);
@@ -1224,7 +1251,9 @@ extern "C" dk_status dk_cache_attention(const dk_cache_attention_args* p, void* 
   a.tokens = p->tokens;
   a.kv_heads = c.kv_heads;
   a.group = group;
-  a.group_magic = group > 1 ? (unsigned)(((1ull << 32) + group - 1) / group) : 0u;
+  auto magic = [](int by) { return by > 1 ? (unsigned)(((1ull << 32) + by - 1) / by) : 0u; };
+  a.group_magic = magic(group);
+  a.block_magic = magic(a.tiles_per_block);
   a.scale_log2 = p->scale * 1.4426950408889634f;
   a.causal = p->causal;
   a.window = p->window;
