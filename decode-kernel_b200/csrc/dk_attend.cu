@@ -754,12 +754,11 @@ struct Attend {
       }
       if (r < a.requests) prefix[r] = before + sum - mine;
       carry += all;
+      if (tid == 0) prefix[a.requests] = carry;  // the last round's is the whole
       __syncthreads();
     }
     const int all = carry;
     if (all == 0) return;
-    if (tid == 0) prefix[a.requests] = all;
-    __syncthreads();
     // Every CTA has the same number of places (the last has the rest), one for
     // each of its warps at least; CTA u / chunk has place u.  Nor is a segment
     // of n units cut in more than about sqrt(2 n) parts: one CTA joins them, at

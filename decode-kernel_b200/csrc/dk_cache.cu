@@ -252,7 +252,9 @@ __global__ void __launch_bounds__(kPlanThreads) k_cache_plan(const __grid_consta
 // of those turns up does a slower path look at each value.
 // ---------------------------------------------------------------------------
 constexpr int kAppendWarps = 4;
-constexpr int kShortRun = 8;  // rows that a warp takes alone
+// Rows that a warp takes alone: eight loads a lane at most.
+template <int D>
+constexpr int kShortRun = D == 256 ? 8 : 16;
 constexpr int kPieces = 8;    // pieces of 8 values of a long run that a thread keeps in shared memory
 constexpr int kMaxWindow = 64;
 constexpr int kMaxItems = 4;  // heads' K or V that a CTA takes one after the other
@@ -367,12 +369,12 @@ __device__ __forceinline__ uint32_t add_largest_finite(uint32_t top, const uint4
 }
 
 template <int D, bool E4M3>
-__global__ void __launch_bounds__(kAppendWarps * 32, 5) k_cache_append(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(kAppendWarps * 32, D == 64 ? 6 : 5) k_cache_append(const __grid_constant__ AppendArgs a) {
   constexpr float Q = E4M3 ? 448.f : 127.f;
   constexpr int LPR = D / 8;     // lanes of a row
   constexpr int RPW = 32 / LPR;  // rows of a warp's load
   constexpr int kStep = kAppendWarps * RPW;         // rows of the CTA's load
-  constexpr int kAlone = kShortRun / RPW;           // a warp's loads of a short run
+  constexpr int kAlone = kShortRun<D> / RPW;           // a warp's loads of a short run
   constexpr int kSpan = kMaxWindow + kMaxBlock;
   struct Job {  // earlier rows to be coded again
     uint8_t* rows;
@@ -450,7 +452,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 5) k_cache_append(const __g
     const int n = next_break(i0 + 1) - i0;
     auto scale_at = [&](int item) { return a.scale[item & 1] + page * a.kv_heads + (item >> 1); };
     auto pool_at = [&](int item) { return a.pool[item & 1] + page * a.block_stride[item & 1] + (item >> 1) * a.head_stride[item & 1]; };
-    if (n <= kShortRun) {
+    if (n <= kShortRun<D>) {
 #pragma unroll 1
       for (int item = item0; item < item1; ++item) {
         if (turn++ % kAppendWarps != warp) continue;
@@ -566,7 +568,7 @@ template <int D>
 dk_status launch_append(const AppendArgs& a, bool e4m3, cudaStream_t stream) {
   const dim3 grid((a.tokens + a.window - 1) / a.window, (2 * a.kv_heads + a.items - 1) / a.items);
   // Runs are as long as the call has tokens, or a page.
-  const bool long_runs = std::min(a.tokens, a.block_size) > kShortRun;
+  const bool long_runs = std::min(a.tokens, a.block_size) > kShortRun<D>;
   const size_t smem = long_runs ? (a.items > 1 ? 2 : 1) * kPieces * kAppendWarps * 32 * sizeof(uint4) : 0;
   return launch_early("dk_cache_append", e4m3 ? k_cache_append<D, true> : k_cache_append<D, false>, grid,
                       dim3(kAppendWarps * 32), smem, stream, a);
