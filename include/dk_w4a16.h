@@ -429,7 +429,10 @@ DK_API dk_status dk_cache_append(const dk_cache8* cache, const void* k, const vo
  * elements, multiples of 8, and is 16-byte aligned; out and lse are contiguous.
  * Block strides are below 2^31 and block_size * token stride too.  V scales
  * below 2^-70 count as 2^-70.  Entries of block_table outside the
- * pool hide their tokens.
+ * pool hide their tokens.  What stands in the cache where no query of a request
+ * may look is not looked at, NaN codes and scales included; an e4m3 NaN code of
+ * V that one of a request's queries sees may reach its other queries too.
+ * starts rise.
  * The workspace (dk_cache_attention_workspace_bytes of the current device) is
  * 256-byte aligned and zero before its first call, which every call leaves it
  * ready for the next; calls that share one must be ordered on the GPU. */
