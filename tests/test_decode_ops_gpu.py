@@ -473,6 +473,28 @@ def test_attention_many_requests():
     check_attention(attention_case(lengths, None, 2, 1, 64, 16, "int8", "fp16"))
 
 
+def test_attention_many_requests_of_several_queries():
+    g = gen(22)
+    fresh = torch.randint(0, 4, (2500,), generator=g).tolist()
+    lengths = [n + int(x) for n, x in zip(fresh, torch.randint(0, 40, (2500,), generator=g).tolist())]
+    check_attention(attention_case(lengths, fresh, 4, 2, 64, 16, "e4m3", "fp16"), window=11)
+
+
+def test_attention_and_append_of_nothing():
+    q, k, v, ks, vs, table, _, _ = attention_case([20], None, 8, 2, 128, 16, "int8", "fp16")
+    cache = dk.PagedCache8.from_tensors(k.cuda(), v.cuda(), ks.cuda(), vs.cuda())
+    o, l = dk.cache_attention(q.cuda()[:0], cache, table.cuda()[:0], ints([]), lse=True)
+    assert o.shape == (0, 8, 128) and l.shape == (0, 8)
+    o = dk.cache_attention(q.cuda()[:0], cache, table.cuda(), ints([20]), ints([0, 0]))
+    assert o.shape == (0, 8, 128)
+    dk.cache_append(q.cuda()[:0, :2], q.cuda()[:0, :2], ints([], torch.int64), cache)
+    assert torch.equal(cache.k.cpu(), k)
+    # Rows of q beyond the last request's are left alone.
+    out = torch.full((3, 8, 128), 7.0, dtype=torch.float16, device="cuda")
+    dk.cache_attention(q.cuda().expand(3, 8, 128), cache, table.cuda(), ints([20]), ints([1, 2]), out=out)
+    assert (out[0] == 7).all() and (out[2] == 7).all() and not (out[1] == 7).any()
+
+
 def test_attention_scale_and_large_scores():
     case = attention_case([300, 40], None, 8, 2, 128, 64, "int8", "bf16", spread=0.3)
     check_attention(case, scale=0.02)
@@ -725,6 +747,13 @@ def test_norm_leading_dims_rows_and_inplace():
         check_norm(0, 256, lead=lead, inplace=True)
     check_norm(1000, 128, gate="row", inplace=True, residual="fp32")
     check_norm(4, 4096, kind="layer", post=True, bias=True, mean=30.0)
+
+
+@pytest.mark.parametrize("dim", [2056, 4104, 5120, 5128, 6152, 7168, 8000, 8192, 16000])
+def test_norm_many_rows(dim):
+    # Enough rows for the shapes that keep every SM busy.
+    check_norm(333, dim, kind="layer", post=True, gate="row", act="silu", seed=dim)
+    check_norm(333, dim, dtype="bf16", residual="fp32", post=True, seed=dim)
 
 
 def test_norm_strided_rows():
