@@ -624,11 +624,15 @@ extern "C" dk_status dk_cache_plan(const int32_t* held, const int32_t* fresh, in
       return DK_ERR_CUDA;
     }
   }
+  // Enough CTAs for the slots, the sums and, should every request end, four
+  // pages a thread given back (545 requests, 181 of which give back up to 187
+  // pages each: 27 us by one CTA).
+  const long long slots_of = kPlanThreads * (many ? 8 : 2), pages_of = kPlanThreads * 4;
+  const long long work = std::max(((long long)tokens + slots_of - 1) / slots_of,
+                                  ((long long)requests * max_blocks + pages_of - 1) / pages_of);
+  int grid = (int)std::min<long long>(sm_count(-1), std::max(1LL, work));
   // Where an output is an input one CTA does it all: it has read what the
   // others would still need.
-  const int each = kPlanThreads * (many ? 8 : 2);
-  const int work = std::max((tokens + each - 1) / each, (requests + 4 * kPlanThreads - 1) / (4 * kPlanThreads));
-  int grid = std::min(sm_count(-1), std::max(1, work));
   if (lengths == held || ring_out == ring) grid = 1;
   return launch_early("dk_cache_plan", kernel, dim3(grid), dim3(kPlanThreads), smem, static_cast<cudaStream_t>(stream), a);
 }
