@@ -1005,8 +1005,7 @@ struct Attend {
     // and warps beyond the rows other parts; then the rows' elements, of both
     // segments together.
     constexpr int P = 32 / kRows, G = W * P;
-    float* tops = reinterpret_cast<float*>(sh.ring);  // [2][G][kRows]
-    float* sums = tops + 2 * G * kRows;               // [2][G][kRows]
+    float* sums = reinterpret_cast<float*>(sh.ring);  // [2][G][kRows]
     float* factor = sums + 2 * G * kRows;             // [n0 + n1][kRows]
     const int row = lane % kRows, mine = warp * P + lane / kRows;
     const bool busy = lane < P * kRows;
