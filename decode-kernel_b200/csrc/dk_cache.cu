@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_cache_plan(const __grid_consta
 // again if it grew, the new codes.  Bound by bytes, 2 read and 1 written for
 // each value (long runs), or by latency (single tokens): slot -> scale and
 // values -> codes.  Measured: 16 requests of up to 2047 tokens, 8 heads of 128,
-// e4m3 25.3 us (4.0 TB/s), 37 ragged pieces, 5 heads of 64, int8 9.7 us, a step
+// e4m3 25.3 us (4.0 TB/s), 37 ragged pieces, 5 heads of 64, int8 8.7 us, a step
 // of 96 tokens 5.3 us through Python.
 //
 // A CTA looks for the runs that begin in its window of tokens, reading the
@@ -683,14 +683,17 @@ extern "C" dk_status dk_cache_append(const dk_cache8* c, const void* k, const vo
   a.kv_heads = c->kv_heads;
   a.bf16 = dtype == DK_BF16;
   a.block_magic = ~0ull / (unsigned long long)c->block_size + 1;
-  // The window: four tokens, one for each warp, while the GPU holds the CTAs
-  // that this makes; more where most windows would hold no run's beginning.
-  // With large windows a CTA takes several heads, as long as there are two CTAs
-  // for each that the GPU holds: it reads the slots once for all of them.
-  const long long each = (long long)tokens * c->kv_heads * 2, room = 20LL * sm_count(-1);
-  a.window = each / kAppendWarps <= room ? kAppendWarps : each / 16 <= room ? 16 : kMaxWindow;
+  // The window: four tokens, one for each warp, up to 20 CTAs an SM (400 single
+  // tokens, 8 heads: 11.7 us, with windows of 16 13.8), then 16 up to 14 CTAs an
+  // SM (1510 tokens in runs of 15: 10.6 us, with windows of 64 13.9), then 64,
+  // since most windows would hold no run's beginning (3930 tokens in runs of 48
+  // and 5 heads: 8.7 us, with windows of 16 9.7).  With the largest windows a CTA
+  // takes several heads, as long as there are ten CTAs an SM: it reads the slots
+  // once for all of them.
+  const long long each = (long long)tokens * c->kv_heads * 2, sms = sm_count(-1);
+  a.window = each / kAppendWarps <= 20 * sms ? kAppendWarps : each / 16 <= 14 * sms ? 16 : kMaxWindow;
   a.items = 1;
-  while (a.window == kMaxWindow && a.items < kMaxItems && each / kMaxWindow / (2 * a.items) >= 10LL * sm_count(-1)) a.items *= 2;
+  while (a.window == kMaxWindow && a.items < kMaxItems && each / kMaxWindow / (2 * a.items) >= 10 * sms) a.items *= 2;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool e4m3 = c->code == DK_E4M3;
   if (c->head_dim == 64) return launch_append<64>(a, e4m3, st);
