@@ -241,9 +241,14 @@ struct Attend {
   // place(g, 2c + 1) = place(g, 2c) ^ 16, place(2c + 1, p) = (place(2c, p) ^ kOdd) + kOddRow.
   static constexpr int kOdd = D == 64 ? 64 : 16, kOddRow = D == 64 ? 0 : D;
 
+  // The first token that query i of a request sees with a window.  The maximum
+  // inside keeps the sum within 32 bits for any window and more queries than tokens.
+  __device__ static __forceinline__ int window_from(const AttendArgs& a, int length, int fresh, int i) {
+    return max(0, max(0, length - a.window) - (fresh - 1 - i));
+  }
   __device__ static __forceinline__ int units_of(const AttendArgs& a, int length, int fresh, int& unit0) {
     unit0 = 0;
-    if (a.window > 0) unit0 = max(0, length - fresh + 1 - a.window) / kUnit;
+    if (a.window > 0) unit0 = window_from(a, length, fresh, 0) / kUnit;
     return max(1, (length + kUnit - 1) / kUnit - unit0);
   }
   __device__ static __forceinline__ int tiles_of(const AttendArgs& a, int fresh) {
@@ -316,7 +321,7 @@ struct Attend {
     low = high = 0;
     if (i >= s.fresh || (unsigned)token >= (unsigned)a.tokens) return false;
     high = a.causal ? min(s.length, max(0, s.length - s.fresh + i + 1)) : s.length;
-    if (a.window > 0) low = max(0, s.length - s.fresh + i + 1 - a.window);
+    if (a.window > 0) low = window_from(a, s.length, s.fresh, i);
     return true;
   }
 

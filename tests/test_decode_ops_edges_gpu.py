@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import decode_kernel as dk
-from test_decode_ops_gpu import attention_case, run_attention
+from test_decode_ops_gpu import attention_case, check_attention, run_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -39,3 +39,10 @@ def test_attention_ignores_hidden_pages_scales(code, kv, dim, bs, fresh):
     assert hidden
     dirty = run_attention((q, kb.view(k.dtype), vb.view(v.dtype), ks, vs, table, lengths, starts), window=window)
     assert torch.equal(clean[0], dirty[0]) and torch.equal(clean[1], dirty[1])
+
+
+@pytest.mark.parametrize("hq,kv,dim", [(8, 2, 128), (4, 4, 64)])
+@pytest.mark.parametrize("window", [0, 2, 2 ** 31 - 100, 2 ** 31 - 1])
+def test_attention_of_more_queries_than_tokens_and_the_largest_windows(hq, kv, dim, window):
+    """Queries that stand before a request's first token see none; a window of any size hides no more than it says."""
+    check_attention(attention_case([2, 40, 3, 0, 0, 70], [5, 3, 9, 2, 3, 1], hq, kv, dim, 16, "int8", "fp16", seed=dim), window=window)
