@@ -390,7 +390,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32, D == 64 ? 6 : 5) k_cache_ap
   __shared__ uint32_t s_break[kSpan / 32 + 1];
   __shared__ uint32_t s_top[2][kAppendWarps];
   __shared__ Job s_job[kMaxJobs];
-  __shared__ int s_jobs;
+  __shared__ int s_jobs, s_gaps;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int bs = a.block_size;
   const int first = blockIdx.x * a.window;
@@ -411,14 +411,15 @@ __global__ void __launch_bounds__(kAppendWarps * 32, D == 64 ? 6 : 5) k_cache_ap
   // it if it has no slot, begins a page or does not follow its neighbour.
   const int span = min(a.window + bs, a.tokens - first);
   for (int i = tid; i <= span; i += kAppendWarps * 32) s_slot[i] = first - 1 + i >= 0 ? a.slots[first - 1 + i] : -1;
-  if (tid == 0) s_jobs = 0;
+  if (tid == 0) s_jobs = s_gaps = 0;
   __syncthreads();
   auto page_of = [&](long long slot) { return (long long)__umul64hi((unsigned long long)slot, a.block_magic); };
   for (int i = tid; i < (span + 31) / 32 * 32; i += kAppendWarps * 32) {
     bool breaks = true;
     if (i < span) {
-      const long long slot = s_slot[i + 1];
-      breaks = slot < 0 || s_slot[i] != slot - 1 || page_of(slot) * bs == slot;
+      const long long slot = s_slot[i + 1], before = s_slot[i], begin = page_of(slot) * bs;
+      breaks = slot < 0 || before != slot - 1 || begin == slot;
+      if (breaks && before < slot && before >= begin && slot >= 0) s_gaps = 1;  // an earlier row of the page
     }
     const uint32_t bits = __ballot_sync(0xffffffffu, breaks);
     if (lane == 0) s_break[i >> 5] = bits;
@@ -446,6 +447,44 @@ __global__ void __launch_bounds__(kAppendWarps * 32, D == 64 ? 6 : 5) k_cache_ap
     return a.bf16 ? __uint_as_float(pattern << 16) : __half2float(__ushort_as_half((unsigned short)pattern));
   };
   auto scale_for = [&](float old, uint32_t top) { return fmaxf(old, __fdiv_rn(fmaxf(value(top), kLeastAmax), Q)); };
+  // Rows of a page that rise with gaps between them (nothing that cache_plan
+  // makes): a warp takes a page's tokens, reads them twice and places each.  Rows
+  // in the gaps keep what they hold.
+  if (s_gaps) {
+    auto follows = [&](int i) { return s_slot[i] >= page_of(s_slot[i + 1]) * bs && s_slot[i] < s_slot[i + 1] && s_slot[i] >= 0; };
+    int turn = 0;
+#pragma unroll 1
+    for (int i0 = 0, n; i0 < min(span, a.window); i0 += n) {
+      n = 1;
+      const long long slot = s_slot[i0 + 1], page = page_of(slot);
+      if (slot < 0 || page >= a.blocks || follows(i0)) continue;
+      while (i0 + n < span && follows(i0 + n)) ++n;
+      const int row0 = (int)(slot - page * bs);
+#pragma unroll 1
+      for (int item = item0; item < item1; ++item) {
+        if (turn++ % kAppendWarps != warp) continue;
+        const long long xs = a.x_token_stride[item & 1], ps = a.row_stride[item & 1];
+        const uint16_t* x = rows_of(item) + (first + i0) * xs;
+        uint8_t* pool = a.pool[item & 1] + page * a.block_stride[item & 1] + (item >> 1) * a.head_stride[item & 1];
+        float* scale = a.scale[item & 1] + page * a.kv_heads + (item >> 1);
+        const float old = row0 > 0 ? *scale : 0.f;
+        uint32_t top = 0;
+#pragma unroll 1
+        for (int i = sub; i < n; i += RPW) top = add_largest_finite(top, *reinterpret_cast<const uint4*>(x + i * xs), infinite);
+        top = __reduce_max_sync(0xffffffffu, top);
+        const float now = scale_for(old, top), by = __frcp_rn(now);
+#pragma unroll 1
+        for (int i = sub; i < n; i += RPW)
+          *reinterpret_cast<uint2*>(pool + (s_slot[i0 + 1 + i] - page * bs) * ps + lane % LPR * 8) =
+              encode8<E4M3>(*reinterpret_cast<const uint4*>(x + i * xs), a.bf16, by, true);
+        if (now > old) {
+          if (lane == 0) *scale = now;
+          if (row0 > 0) again(pool, ps, row0, __fdiv_rn(old, now), 0, 1);
+        }
+      }
+    }
+    return;
+  }
   int turn = 0, big = 0;
   for (int i0 = next_break(0); i0 < min(span, a.window); i0 = next_break(i0 + 1)) {
     const long long slot = s_slot[i0 + 1];

@@ -119,7 +119,8 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: P
     (e4m3) and grows with later tokens, when the page's earlier codes are
     rounded to the new scale; tokens that begin a page begin its scale.  Values
     past the scale saturate, NaN becomes 0.  The rows of a page must be
-    neighbours with rising slots.
+    neighbours (none skipped between them) with rising slots; rows of the page
+    between them keep their codes.
     """
     _extension().cache_append(k, v, slots, cache._handle)
 

@@ -403,14 +403,15 @@ DK_API dk_status dk_cache_plan(const int32_t* held, const int32_t* fresh, int re
  * head_dim], DK_FP16 or DK_BF16, token and head strides in elements, multiples
  * of 8, last dimension contiguous, 16-byte aligned) goes to slots[t] = page * block_size + row.  Slots
  * below 0 or past the pool are skipped.  The tokens of a page are neighbours
- * in t, with rising rows, and a page gets tokens of one request only
- * (dk_cache_plan's slots are so).
+ * in t (none skipped between them), with rising rows, and a page gets tokens of
+ * one request only (dk_cache_plan's slots are so).
  * For each page and head, with Q = 127 (int8) or 448 (e4m3):
  *   amax  = largest finite |x| of the call's tokens there
  *   scale = max(old, max(amax, 2^-60) / Q), old = 0 if the tokens begin the page
  *   code  = x * (1 / scale), clamped to +-Q, rounded to nearest even; NaN is 0
- * and where scale > old the page's earlier rows (if any) are coded again as
- * code * (old / scale).  All in fp32 with IEEE divisions. */
+ * and where scale > old the page's rows before the call's first (if any) are
+ * coded again as code * (old / scale).  Rows between the call's keep their codes.
+ * All in fp32 with IEEE divisions. */
 DK_API dk_status dk_cache_append(const dk_cache8* cache, const void* k, const void* v,
                                  dk_dtype dtype, int tokens, int64_t k_token_stride,
                                  int64_t k_head_stride, int64_t v_token_stride,

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import decode_kernel as dk
-from test_decode_ops_gpu import attention_case, check_attention, run_attention
+from test_decode_ops_gpu import CODES, HALF, attention_case, check_attention, encode, gen, random_pools, raw, run_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -46,3 +46,70 @@ def test_attention_ignores_hidden_pages_scales(code, kv, dim, bs, fresh):
 def test_attention_of_more_queries_than_tokens_and_the_largest_windows(hq, kv, dim, window):
     """Queries that stand before a request's first token see none; a window of any size hides no more than it says."""
     check_attention(attention_case([2, 40, 3, 0, 0, 70], [5, 3, 9, 2, 3, 1], hq, kv, dim, 16, "int8", "fp16", seed=dim), window=window)
+
+
+# ---------------------------------------------------------------------------
+# Append
+# ---------------------------------------------------------------------------
+
+
+def pages_reference(pool, scale, x, slots, code):
+    """dk_cache_append's rule in fp32 on the CPU, page by page: a page's tokens have one maximum and one scale."""
+    bs, q = pool.shape[2], CODES[code][1]
+    pool, scale, x = pool.clone(), scale.clone(), x.float()
+    there = (slots >= 0) & (slots < pool.shape[0] * bs)
+    for page in (slots[there] // bs).unique().tolist():
+        mine = there & (slots // bs == page)
+        rows, y = slots[mine] % bs, x[mine]
+        amax = torch.where(y.isfinite(), y.abs(), torch.zeros_like(y)).amax(dim=(0, 2))
+        new = amax.clamp(min=2.0 ** -60) / torch.full_like(amax, q)
+        first = int(rows.min())
+        if first:
+            old = scale[page].clone()
+            new = torch.maximum(old, new)
+            for h in (new > old).nonzero().flatten().tolist():
+                pool[page, h, :first] = encode(pool[page, h, :first].float() * (old[h] / new[h]), code)
+        scale[page] = new
+        raw_pool = pool.view(torch.uint8)  # indexed writes of e4m3
+        raw_pool[page][:, rows] = encode(y * (torch.ones_like(new) / new)[None, :, None], code).transpose(0, 1).contiguous().view(torch.uint8)
+    return pool, scale
+
+
+def check_pages(k, v, slots, pools, code):
+    dev = [t.cuda() for t in pools]
+    dk.cache_append(k.cuda(), v.cuda(), slots.cuda(), dk.PagedCache8.from_tensors(*dev))
+    for i, x in ((0, k), (1, v)):
+        want, scale = pages_reference(pools[i], pools[2 + i], x, slots, code)
+        assert torch.equal(dev[2 + i].cpu(), scale), "scales"
+        assert torch.equal(raw(dev[i].cpu()), raw(want)), "codes"
+
+
+def rows_with_gaps(pages, bs, most, g, whole=0.2):
+    """Slots of `pages` pages: in most pages some rows, rising; in a share of them neighbouring rows only."""
+    out = []
+    for page in torch.randperm(pages, generator=g).tolist():
+        n = int(torch.randint(1, min(most, bs) + 1, (1,), generator=g))
+        if torch.rand(1, generator=g) < whole:
+            at = int(torch.randint(0, bs - n + 1, (1,), generator=g))
+            rows = torch.arange(at, at + n)
+        else:
+            rows = torch.randperm(bs, generator=g)[:n].sort().values
+        out.append(page * bs + rows)
+        if torch.rand(1, generator=g) < 0.1:
+            out.append(torch.tensor([-1]))
+    return torch.cat(out)
+
+
+@pytest.mark.parametrize("dtype,code", [("fp16", "int8"), ("bf16", "e4m3")])
+@pytest.mark.parametrize("dim,heads,bs,pages,most", [
+    (128, 2, 16, 3, 3), (128, 8, 64, 9, 64), (64, 3, 48, 40, 48), (256, 2, 256, 3, 250), (64, 12, 16, 300, 9), (128, 8, 64, 150, 40),
+])
+def test_append_rows_with_gaps(dtype, code, dim, heads, bs, pages, most):
+    """Rows of a page may rise with gaps: they are one run with one scale, whichever windows and warps they fall to."""
+    g = gen(dim + pages)
+    slots = rows_with_gaps(pages, bs, most, g)
+    pools = random_pools(pages, heads, bs, dim, code, g)
+    k, v = ((torch.randn(len(slots), heads, dim, generator=g) * torch.rand(len(slots), heads, 1, generator=g) * 5).to(HALF[dtype][0]) for _ in range(2))
+    k[::7, :, 3] = float("inf")
+    v[::5, :, 1] = float("nan")
+    check_pages(k, v, slots, pools, code)
