@@ -251,8 +251,9 @@ struct Attend {
     if (a.window > 0) unit0 = window_from(a, length, fresh, 0) / kUnit;
     return max(1, (length + kUnit - 1) / kUnit - unit0);
   }
-  __device__ static __forceinline__ int tiles_of(const AttendArgs& a, int fresh) {
-    return (fresh * a.group + kRows - 1) / kRows;
+  // Row tiles of a request: of those of its queries that the call has rows for.
+  __device__ static __forceinline__ int tiles_of(const AttendArgs& a, int first, int fresh) {
+    return (min(fresh, max(0, a.tokens - max(0, first))) * a.group + kRows - 1) / kRows;
   }
   // The requests' numbers in shared memory: prefix[r] = the place of request
   // r's first unit in the line (one more entry than requests), then the tokens
@@ -263,7 +264,7 @@ struct Attend {
     if (a.starts) {
       const int* starts = lengths + a.requests;
       first = starts[r];
-      fresh = min(max(0, starts[r + 1] - first), a.tokens);
+      fresh = max(0, starts[r + 1] - first);
     } else {
       first = r;
       fresh = 1;
@@ -279,7 +280,7 @@ struct Attend {
     s.which = which;
     s.begin = prefix[r] + which * (s.units + kStart) + kStart;
     s.blocks = over((s.length + kTile - 1) / kTile + a.tiles_per_block - 1, a.tiles_per_block, a.block_magic);
-    const int tiles = tiles_of(a, s.fresh);
+    const int tiles = tiles_of(a, s.first_token, s.fresh);
     s.all = tiles * a.kv_heads;
     s.head = tiles == 1 ? which : which / tiles;
     s.tile = which - s.head * tiles;
@@ -736,18 +737,20 @@ struct Attend {
       int mine = 0;
       if (r < a.requests) {
         const int length = min(max(ld_int(a.lengths + r), 0), most);
-        int fresh = 1, unit0;
+        int first = r, fresh = 1, unit0;
         if (a.starts) {
-          const int first = ld_int(a.starts + r), next = ld_int(a.starts + r + 1);
-          fresh = min(max(0, next - first), a.tokens);
+          first = ld_int(a.starts + r);
+          const int next = ld_int(a.starts + r + 1);
+          fresh = max(0, next - first);
           starts[r] = first;
           if (r == a.requests - 1) starts[r + 1] = next;
         }
         lengths[r] = length;
-        if (fresh > 0) {
+        const int tiles = tiles_of(a, first, fresh);
+        if (tiles > 0) {
           const int one = units_of(a, length, fresh, unit0) + kStart;
           longest = max(longest, one);
-          mine = one * tiles_of(a, fresh) * a.kv_heads;
+          mine = one * tiles * a.kv_heads;
         }
       }
       int sum = mine;

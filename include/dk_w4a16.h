@@ -433,7 +433,8 @@ DK_API dk_status dk_cache_append(const dk_cache8* cache, const void* k, const vo
  * pool hide their tokens.  What stands in the cache where no query of a request
  * may look is not looked at, NaN codes and scales included; an e4m3 NaN code of
  * V that one of a request's queries sees may reach its other queries too.
- * starts rise.
+ * starts rise; where they pass `tokens` the rows that q has are served, in their
+ * places.
  * The workspace (dk_cache_attention_workspace_bytes of the current device) is
  * 256-byte aligned and zero before its first call, which every call leaves it
  * ready for the next; calls that share one must be ordered on the GPU. */

@@ -48,6 +48,18 @@ def test_attention_of_more_queries_than_tokens_and_the_largest_windows(hq, kv, d
     check_attention(attention_case([2, 40, 3, 0, 0, 70], [5, 3, 9, 2, 3, 1], hq, kv, dim, 16, "int8", "fp16", seed=dim), window=window)
 
 
+@pytest.mark.parametrize("hq,kv,dim,window", [(8, 2, 128, 0), (4, 4, 64, 30), (16, 1, 128, 0)])
+def test_attention_of_fewer_rows_than_starts(hq, kv, dim, window):
+    """Rows that q lacks are left out; the others keep their places before the request's last token."""
+    for lengths, fresh, rows in (([130], [100], 97), ([130, 60], [100, 20], 60), ([9, 130, 60], [1, 100, 20], 104)):
+        case = attention_case(lengths, fresh, hq, kv, dim, 16, "int8", "fp16", seed=rows)
+        whole, lse = run_attention(case, window=window)
+        some, some_lse = run_attention((case[0][:rows].contiguous(), *case[1:]), window=window)
+        # Another split of the same sums: fp16 weights and outputs.
+        torch.testing.assert_close(some, whole[:rows], rtol=2.0 ** -9, atol=2.0 ** -9 * float(whole.abs().max()))
+        torch.testing.assert_close(some_lse, lse[:rows], rtol=1e-5, atol=1e-5)
+
+
 # ---------------------------------------------------------------------------
 # Append
 # ---------------------------------------------------------------------------
