@@ -84,6 +84,7 @@ struct AttendArgs {
   uint32_t k_block_stride, k_token_stride, v_block_stride, v_token_stride;
   int table_stride, max_blocks, blocks, block_size, tiles_per_block;
   int requests, tokens, kv_heads, group;
+  int heads;                          // KV heads of the launch, from the pointers' on
   unsigned group_magic, block_magic;  // for over()
   float scale_log2;
   int causal, window, bf16;
@@ -281,7 +282,7 @@ struct Attend {
     s.begin = prefix[r] + which * (s.units + kStart) + kStart;
     s.blocks = over((s.length + kTile - 1) / kTile + a.tiles_per_block - 1, a.tiles_per_block, a.block_magic);
     const int tiles = tiles_of(a, s.first_token, s.fresh);
-    s.all = tiles * a.kv_heads;
+    s.all = tiles * a.heads;
     s.head = tiles == 1 ? which : which / tiles;
     s.tile = which - s.head * tiles;
     return s;
@@ -750,7 +751,7 @@ struct Attend {
         if (tiles > 0) {
           const int one = units_of(a, length, fresh, unit0) + kStart;
           longest = max(longest, one);
-          mine = one * tiles * a.kv_heads;
+          mine = one * tiles * a.heads;
         }
       }
       int sum = mine;
@@ -1100,17 +1101,18 @@ __global__ void __launch_bounds__(W * 32, MINB) k_attend(const __grid_constant__
 //   64, one row tile: two tiles of tokens side by side 51 us for the window case,
 //     one 58 to 61
 //   more row tiles: one CTA of 8 warps (drafts 44 us, two of 4 47.6 at that time)
+constexpr int unit_tiles(int head_dim) { return head_dim == 64 ? 2 : 1; }
 template <int D, int NT>
 struct Shape;
-template <> struct Shape<64, 1> { static constexpr int W = 8, S = 2, MINB = 2, MT = 2; };
-template <> struct Shape<64, 2> { static constexpr int W = 12, S = 3, MINB = 1, MT = 2; };
-template <> struct Shape<64, 4> { static constexpr int W = 8, S = 3, MINB = 1, MT = 2; };
-template <> struct Shape<128, 1> { static constexpr int W = 8, S = 2, MINB = 2, MT = 1; };
-template <> struct Shape<128, 2> { static constexpr int W = 8, S = 3, MINB = 1, MT = 1; };
-template <> struct Shape<128, 3> { static constexpr int W = 8, S = 3, MINB = 1, MT = 1; };
-template <> struct Shape<128, 4> { static constexpr int W = 8, S = 3, MINB = 1, MT = 1; };
-template <> struct Shape<256, 1> { static constexpr int W = 8, S = 2, MINB = 1, MT = 1; };
-template <> struct Shape<256, 2> { static constexpr int W = 8, S = 2, MINB = 1, MT = 1; };
+template <> struct Shape<64, 1> { static constexpr int W = 8, S = 2, MINB = 2; };
+template <> struct Shape<64, 2> { static constexpr int W = 12, S = 3, MINB = 1; };
+template <> struct Shape<64, 4> { static constexpr int W = 8, S = 3, MINB = 1; };
+template <> struct Shape<128, 1> { static constexpr int W = 8, S = 2, MINB = 2; };
+template <> struct Shape<128, 2> { static constexpr int W = 8, S = 3, MINB = 1; };
+template <> struct Shape<128, 3> { static constexpr int W = 8, S = 3, MINB = 1; };
+template <> struct Shape<128, 4> { static constexpr int W = 8, S = 3, MINB = 1; };
+template <> struct Shape<256, 1> { static constexpr int W = 8, S = 2, MINB = 1; };
+template <> struct Shape<256, 2> { static constexpr int W = 8, S = 2, MINB = 1; };
 
 // The workspace: a counter for each CTA that can run at once (in the same place
 // for every shape: they stay zero between calls), two parts of its segments,
@@ -1128,8 +1130,9 @@ Workspace workspace_of(int sms) {
 }
 
 template <int D, int NT, bool E4M3, bool PACKED>
-dk_status launch(AttendArgs a, cudaStream_t stream) {
-  constexpr int W = Shape<D, NT>::W, MINB = Shape<D, NT>::MINB, S = Shape<D, NT>::S, MT = Shape<D, NT>::MT;
+dk_status launch(const AttendArgs& call, cudaStream_t stream) {
+  AttendArgs a = call;
+  constexpr int W = Shape<D, NT>::W, MINB = Shape<D, NT>::MINB, S = Shape<D, NT>::S, MT = unit_tiles(D);
   using A = Attend<D, NT, MT, E4M3, PACKED, W, S>;
   const size_t per = (a.starts ? 3 : 2) * sizeof(int);  // of a request in shared memory
   const size_t smem = sizeof(typename A::Shared) + per * (size_t)(std::min(a.requests, kMaxRequests) + 1);
@@ -1153,32 +1156,35 @@ dk_status launch(AttendArgs a, cudaStream_t stream) {
     }
     if (device < 64) prepared |= 1ull << device;
   }
-  const int requests = a.requests;
-  const int* lengths = a.lengths;
-  const int* table = a.table;
-  const int* starts = a.starts;
-  const uint16_t* q = static_cast<const uint16_t*>(a.q);
-  uint16_t* out = static_cast<uint16_t*>(a.out);
-  float* lse = a.lse;
-  const int tokens = a.tokens;
-  for (int r = 0; r < requests; r += kMaxRequests) {
-    a.requests = std::min(kMaxRequests, requests - r);
-    a.lengths = lengths + r;
-    a.table = table + (long long)r * a.table_stride;
-    if (starts) {
-      a.starts = starts + r;
+  const int heads = call.heads;  // of a launch
+  for (int r = 0; r < call.requests; r += kMaxRequests) {
+    a.requests = std::min(kMaxRequests, call.requests - r);
+    a.lengths = call.lengths + r;
+    a.table = call.table + (long long)r * a.table_stride;
+    long long row = 0;  // the launch's first in q
+    if (call.starts) {
+      a.starts = call.starts + r;
     } else {  // one query each: the rows move with the requests
-      a.q = q + r * a.q_token_stride;
-      a.out = out + (long long)r * a.kv_heads * a.group * D;
-      a.lse = lse ? lse + (long long)r * a.kv_heads * a.group : nullptr;
-      a.tokens = tokens - r;
+      row = r;
+      a.tokens = call.tokens - r;
     }
-    // No more CTAs than the table's width can keep busy.
-    const long long most = (((long long)a.max_blocks * a.block_size + A::kUnit - 1) / A::kUnit + A::kStart) * a.kv_heads *
-                           (starts ? (long long)a.requests + (long long)tokens * a.group / A::kRows : (long long)a.requests * ((a.group + A::kRows - 1) / A::kRows));
-    const int grid = (int)std::min<long long>(sm_count(device) * MINB, (most + W - 1) / W);
-    const dk_status s = launch_early("dk_cache_attention", kernel, dim3(grid), dim3(W * 32), smem, stream, a);
-    if (s != DK_OK) return s;
+    for (int h = 0; h < a.kv_heads; h += heads) {
+      a.heads = std::min(heads, a.kv_heads - h);
+      const long long at = (row * a.kv_heads + h) * a.group;  // among the rows of out
+      a.q = static_cast<const uint16_t*>(call.q) + row * a.q_token_stride + (long long)h * a.group * a.q_head_stride;
+      a.out = static_cast<uint16_t*>(call.out) + at * D;
+      a.lse = call.lse ? call.lse + at : nullptr;
+      a.k = call.k + h * a.k_head_stride;
+      a.v = call.v + h * a.v_head_stride;
+      a.k_scale = call.k_scale + h;
+      a.v_scale = call.v_scale + h;
+      // No more CTAs than the table's width can keep busy.
+      const long long most = (((long long)a.max_blocks * a.block_size + A::kUnit - 1) / A::kUnit + A::kStart) * a.heads *
+                             (call.starts ? (long long)a.requests + (long long)call.tokens * a.group / A::kRows : (long long)a.requests * ((a.group + A::kRows - 1) / A::kRows));
+      const int grid = (int)std::min<long long>(sm_count(device) * MINB, (most + W - 1) / W);
+      const dk_status s = launch_early("dk_cache_attention", kernel, dim3(grid), dim3(W * 32), smem, stream, a);
+      if (s != DK_OK) return s;
+    }
   }
   return DK_OK;
 }
@@ -1239,11 +1245,14 @@ extern "C" dk_status dk_cache_attention(const dk_cache_attention_args* p, void* 
   if (c.k_block_stride > INT32_MAX || c.v_block_stride > INT32_MAX ||
       c.k_token_stride > INT32_MAX / c.block_size || c.v_token_stride > INT32_MAX / c.block_size)
     return DK_ERR_UNSUPPORTED;
-  // The line of units is counted in 32 bits.
+  // The line of units is counted in 32 bits, whatever the lengths turn out to be:
+  // a launch takes as many KV heads as fit it.
   const int group = p->q_heads / c.kv_heads;
-  const long long units = ((long long)p->max_blocks * c.block_size + 15) / 16 + 2;  // and a start's places
-  const long long per_head = (long long)std::min(p->requests, kMaxRequests) + (long long)p->tokens * group / 8;
-  if (units > INT32_MAX / 16 || per_head > INT32_MAX / 2 / units / c.kv_heads) return DK_ERR_UNSUPPORTED;
+  const int nt = row_tiles(c.head_dim, ((long long)p->tokens + p->requests - 1) / p->requests * group);
+  const int unit = kTile * unit_tiles(c.head_dim);
+  const long long width = (long long)p->max_blocks * c.block_size, units = (width + unit - 1) / unit + 2;  // and a start's places
+  const long long tiles = (long long)std::min(p->requests, kMaxRequests) + (long long)p->tokens * group / (8 * nt);
+  if (width > INT32_MAX - 64 || (long long)p->tokens * p->q_heads > INT32_MAX || tiles > INT32_MAX / 2 / units) return DK_ERR_UNSUPPORTED;
   const size_t need = dk_cache_attention_workspace_bytes(c.head_dim);
   if (!workspace || workspace_bytes < need || !aligned(workspace, 256)) return DK_ERR_WORKSPACE;
 
@@ -1275,6 +1284,7 @@ extern "C" dk_status dk_cache_attention(const dk_cache_attention_args* p, void* 
   a.requests = p->requests;
   a.tokens = p->tokens;
   a.kv_heads = c.kv_heads;
+  a.heads = (int)std::min<long long>(c.kv_heads, INT32_MAX / 2 / units / tiles);
   a.group = group;
   auto magic = [](int by) { return by > 1 ? (unsigned)(((1ull << 32) + by - 1) / by) : 0u; };
   a.group_magic = magic(group);
@@ -1285,7 +1295,6 @@ extern "C" dk_status dk_cache_attention(const dk_cache_attention_args* p, void* 
   a.bf16 = p->dtype == DK_BF16;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool e4m3 = c.code == DK_E4M3;
-  const int nt = row_tiles(c.head_dim, ((long long)p->tokens + p->requests - 1) / p->requests * group);
   switch (c.head_dim * 8 + nt) {
     case 64 * 8 + 1: return launch_code<64, 1>(a, e4m3, st);
     case 64 * 8 + 2: return launch_code<64, 2>(a, e4m3, st);

@@ -428,7 +428,10 @@ DK_API dk_status dk_cache_append(const dk_cache8* cache, const void* k, const vo
  * in fp32 and rounded once; rows that see no token are zeros.  lse (or NULL)
  * gets log(sum_j exp(scale * q . k_j)), -inf for such rows.  q has strides in
  * elements, multiples of 8, and is 16-byte aligned; out and lse are contiguous.
- * Block strides are below 2^31 and block_size * token stride too.  V scales
+ * Block strides are below 2^31 and block_size * token stride too.  Calls are
+ * served as long as max_blocks * block_size (the table's width in tokens) times
+ * min(requests, 1024) + tokens * q_heads / kv_heads / 8 is below 2^33, and
+ * tokens * q_heads below 2^31; past that DK_ERR_UNSUPPORTED may come back.  V scales
  * below 2^-70 count as 2^-70.  Entries of block_table outside the
  * pool hide their tokens.  What stands in the cache where no query of a request
  * may look is not looked at, NaN codes and scales included; an e4m3 NaN code of

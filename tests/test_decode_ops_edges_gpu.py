@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import decode_kernel as dk
-from test_decode_ops_gpu import CODES, HALF, attention_case, check_attention, encode, gen, random_pools, raw, run_attention
+from test_decode_ops_gpu import CODES, HALF, attention_case, check_attention, encode, gen, ints, random_pools, raw, run_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -58,6 +58,31 @@ def test_attention_of_fewer_rows_than_starts(hq, kv, dim, window):
         # Another split of the same sums: fp16 weights and outputs.
         torch.testing.assert_close(some, whole[:rows], rtol=2.0 ** -9, atol=2.0 ** -9 * float(whole.abs().max()))
         torch.testing.assert_close(some_lse, lse[:rows], rtol=1e-5, atol=1e-5)
+
+
+def test_attention_over_a_wide_table():
+    """A table for 131072 tokens and 16384 rows in q, of which short requests use a few."""
+    lengths, fresh = [300, 290, 17, 1000], [256, 1, 17, 100]
+    q, k, v, ks, vs, table, lengths, starts = attention_case(lengths, fresh, 64, 8, 128, 64, "int8", "bf16", seed=3)
+    cache = dk.PagedCache8.from_tensors(k.cuda(), v.cuda(), ks.cuda(), vs.cuda())
+    wide = torch.full((4, 2048), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table.cuda()
+    many = torch.zeros(16384, 64, 128, dtype=torch.bfloat16, device="cuda")
+    many[:starts[-1]] = q.cuda()
+    want = dk.cache_attention(q.cuda(), cache, table.cuda(), ints(lengths), ints(starts))
+    got = dk.cache_attention(many, cache, wide, ints(lengths), ints(starts))[:starts[-1]]
+    torch.testing.assert_close(got.float(), want.float(), rtol=2.0 ** -7, atol=2.0 ** -9 * float(want.abs().max()))
+
+
+@pytest.mark.parametrize("fresh", [None, [3, 20]])
+@pytest.mark.parametrize("dim,code,dtype", [(64, "e4m3", "fp16"), (128, "int8", "bf16")])
+def test_attention_takes_kv_heads_in_several_launches(dim, code, dtype, fresh):
+    """The widest table leaves a launch's line of units room for a few KV heads only."""
+    case = attention_case([700, 33], fresh, 80, 40, dim, 256, code, dtype, seed=dim)
+    q, k, v, ks, vs, table, lengths, starts = case
+    wide = torch.full((2, (1 << 30) // 256), -1, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    check_attention((q, k, v, ks, vs, wide, lengths, starts))
 
 
 # ---------------------------------------------------------------------------
