@@ -391,21 +391,25 @@ void cache_append(torch::Tensor k, torch::Tensor v, torch::Tensor slots, const C
                "cache_append");
 }
 
-// The attention workspace: one for each device, stream and head size, zeroed
-// when it is made; every call leaves it ready for the next on that stream.  A
-// call that is being captured gets one of its own with its zeroing in the
-// graph, since the graph may be replayed beside later calls of the stream.
+// The attention workspace: one for each device, stream and head size, its
+// counters zeroed when it is made; every call leaves it ready for the next on that
+// stream.  A call that is being captured gets one of its own with the counters'
+// zeroing (a few KB of some 24 MB) in the graph, since the graph may be replayed
+// beside later calls of the stream.
 torch::Tensor attention_workspace(int head_dim, const at::cuda::CUDAStream& stream) {
-  const auto options = torch::TensorOptions().dtype(torch::kUInt8).device(stream.device());
-  const int64_t bytes = static_cast<int64_t>(dk_cache_attention_workspace_bytes(head_dim));
-  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
-    return torch::zeros({bytes}, options);
+  auto make = [&] {
+    const auto options = torch::TensorOptions().dtype(torch::kUInt8).device(stream.device());
+    const torch::Tensor w = torch::empty({static_cast<int64_t>(dk_cache_attention_workspace_bytes(head_dim))}, options);
+    C10_CUDA_CHECK(cudaMemsetAsync(w.data_ptr(), 0, dk_cache_attention_counter_bytes(), stream.stream()));
+    return w;
+  };
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return make();
   static std::mutex mu;
   // Never freed: the process may end after the CUDA context.
   static auto* kept = new std::map<std::tuple<int, cudaStream_t, int>, torch::Tensor>();
   const std::lock_guard<std::mutex> lock(mu);
   torch::Tensor& w = (*kept)[{stream.device_index(), stream.stream(), head_dim}];
-  if (!w.defined()) w = torch::zeros({bytes}, options);
+  if (!w.defined()) w = make();
   return w;
 }
 

@@ -1116,16 +1116,17 @@ template <> struct Shape<256, 2> { static constexpr int W = 8, S = 2, MINB = 1; 
 
 // The workspace: a counter for each CTA that can run at once (in the same place
 // for every shape: they stay zero between calls), two parts of its segments,
-// and an early part for each of its warps.
+// and an early part for each of its warps.  Parts are written before they are read.
 struct Workspace {
   size_t counters, partials, early;  // bytes
 };
+size_t counter_bytes(int sms) { return ((size_t)sms * 4 * sizeof(int) + 255) / 256 * 256; }
 template <int D, int NT>
 Workspace workspace_of(int sms) {
   using P = Shape<D, NT>;
   const size_t ctas = (size_t)sms * P::MINB, rows = 8 * NT;
   static_assert(P::MINB <= 4, "the counters' room");
-  return {((size_t)sms * 4 * sizeof(int) + 255) / 256 * 256, (ctas * 2 * rows * (D + 2) * sizeof(float) + 255) / 256 * 256,
+  return {counter_bytes(sms), (ctas * 2 * rows * (D + 2) * sizeof(float) + 255) / 256 * 256,
           ctas * P::W * rows * D * sizeof(float)};
 }
 
@@ -1217,6 +1218,8 @@ extern "C" size_t dk_cache_attention_workspace_bytes(int head_dim) {
   if (head_dim == 256) return all(workspace_of<256, 2>(sms));
   return 0;
 }
+
+extern "C" size_t dk_cache_attention_counter_bytes(void) { return counter_bytes(sm_count(-1)); }
 
 extern "C" dk_status dk_cache_attention(const dk_cache_attention_args* p, void* workspace,
                                         size_t workspace_bytes, void* stream) {

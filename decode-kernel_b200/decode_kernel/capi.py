@@ -162,6 +162,7 @@ SIGNATURES = {
     "dk_cache_plan": (_I, [_P, _P, _I, _P, _I, _I, _I, _P, _I, _P, _P, _P, _P, _P, _I, _P]),
     "dk_cache_append": (_I, [ctypes.POINTER(Cache8), _P, _P, _I, _I, _L, _L, _L, _L, _P, _P]),
     "dk_cache_attention_workspace_bytes": (_SZ, [_I]),
+    "dk_cache_attention_counter_bytes": (_SZ, []),
     "dk_cache_attention": (_I, [ctypes.POINTER(CacheAttentionArgs), _P, _SZ, _P]),
     "dk_block_norm": (_I, [ctypes.POINTER(BlockNormArgs), _P]),
     "dk_status_string": (ctypes.c_char_p, [_I]),

@@ -431,16 +431,17 @@ DK_API dk_status dk_cache_append(const dk_cache8* cache, const void* k, const vo
  * Block strides are below 2^31 and block_size * token stride too.  Calls are
  * served as long as max_blocks * block_size (the table's width in tokens) times
  * min(requests, 1024) + tokens * q_heads / kv_heads / 8 is below 2^33, and
- * tokens * q_heads below 2^31; past that DK_ERR_UNSUPPORTED may come back.  V scales
- * below 2^-70 count as 2^-70.  Entries of block_table outside the
- * pool hide their tokens.  What stands in the cache where no query of a request
- * may look is not looked at, NaN codes and scales included; an e4m3 NaN code of
- * V that one of a request's queries sees may reach its other queries too.
- * starts rise; where they pass `tokens` the rows that q has are served, in their
- * places.
+ * tokens * q_heads below 2^31; past that DK_ERR_UNSUPPORTED may come back.
+ * V scales below 2^-70 count as 2^-70.  Entries of block_table outside the pool
+ * hide their tokens.  What stands in the cache where no query of a request may
+ * look is not looked at, NaN codes and scales included; an e4m3 NaN code of V
+ * that one of a request's queries sees may reach its other queries too.
+ * starts rise; where they pass `tokens` the rows that q has are served, in
+ * their places.
  * The workspace (dk_cache_attention_workspace_bytes of the current device) is
- * 256-byte aligned and zero before its first call, which every call leaves it
- * ready for the next; calls that share one must be ordered on the GPU. */
+ * 256-byte aligned.  Its first dk_cache_attention_counter_bytes are zero before
+ * its first call, and every call leaves them so for the next; the rest may hold
+ * anything.  Calls that share a workspace must be ordered on the GPU. */
 typedef struct dk_cache_attention_args {
   dk_cache8 cache;
   const void* q; /* [tokens, q_heads, head_dim] */
@@ -457,6 +458,7 @@ typedef struct dk_cache_attention_args {
   int causal, window;
 } dk_cache_attention_args;
 DK_API size_t dk_cache_attention_workspace_bytes(int head_dim);
+DK_API size_t dk_cache_attention_counter_bytes(void);
 DK_API dk_status dk_cache_attention(const dk_cache_attention_args* args, void* workspace,
                                     size_t workspace_bytes, void* stream);
 

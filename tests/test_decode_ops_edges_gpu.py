@@ -4,10 +4,13 @@ place, captured calls, and the sizes at which a launch takes another form."""
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
 import decode_kernel as dk
+from decode_kernel import capi
 from test_decode_ops_gpu import CODES, HALF, attention_case, check_attention, encode, gen, ints, random_pools, raw, run_attention
 
 pytestmark = pytest.mark.gpu
@@ -83,6 +86,62 @@ def test_attention_takes_kv_heads_in_several_launches(dim, code, dtype, fresh):
     wide = torch.full((2, (1 << 30) // 256), -1, dtype=torch.int32)
     wide[:, :table.shape[1]] = table
     check_attention((q, k, v, ks, vs, wide, lengths, starts))
+
+
+def c_attention(q, cache, table, lengths, out, workspace):
+    """dk_cache_attention of one query a request on the current stream."""
+    k, v = cache.k, cache.v
+    c = capi.Cache8(k=k.data_ptr(), v=v.data_ptr(), k_scale=cache.k_scale.data_ptr(), v_scale=cache.v_scale.data_ptr(), blocks=cache.blocks,
+                    block_size=cache.block_size, kv_heads=cache.kv_heads, head_dim=cache.head_dim, code=capi.DK_INT8, k_block_stride=k.stride(0),
+                    k_head_stride=k.stride(1), k_token_stride=k.stride(2), v_block_stride=v.stride(0), v_head_stride=v.stride(1), v_token_stride=v.stride(2))
+    a = capi.CacheAttentionArgs(cache=c, q=q.data_ptr(), out=out.data_ptr(), lse=None, dtype=capi.DK_FP16, q_token_stride=q.stride(0),
+                                q_head_stride=q.stride(1), block_table=table.data_ptr(), max_blocks=table.shape[1], table_stride=table.stride(0),
+                                lengths=lengths.data_ptr(), starts=None, requests=len(lengths), tokens=len(q), q_heads=q.shape[1],
+                                scale=q.shape[2] ** -0.5, causal=1, window=0)
+    return capi.load().dk_cache_attention(ctypes.byref(a), workspace.data_ptr(), workspace.numel(), torch.cuda.current_stream().cuda_stream)
+
+
+@pytest.mark.parametrize("dim,hq,kv", [(64, 8, 2), (128, 32, 8), (128, 32, 1), (256, 4, 2)])
+def test_attention_workspace_needs_only_its_counters_zero(dim, hq, kv):
+    # Long requests, so that warps and CTAs leave parts of segments in the workspace.
+    q, k, v, ks, vs, table, lengths, _ = attention_case([9000, 40, 2500, 700], None, hq, kv, dim, 64, "int8", "fp16", seed=dim)
+    cache = dk.PagedCache8.from_tensors(k.cuda(), v.cuda(), ks.cuda(), vs.cuda())
+    q, table, lengths = q.cuda(), table.cuda(), ints(lengths)
+    want = dk.cache_attention(q, cache, table, lengths)
+    workspace = torch.full((capi.load().dk_cache_attention_workspace_bytes(dim),), 0xFF, dtype=torch.uint8, device="cuda")  # NaN
+    counters = capi.load().dk_cache_attention_counter_bytes()
+    assert 0 < counters <= 1 << 16
+    workspace[:counters] = 0
+    for _ in range(3):
+        out = torch.full_like(want, float("nan"))
+        assert c_attention(q, cache, table, lengths, out, workspace) == capi.DK_OK
+        assert torch.equal(out, want)
+        assert not workspace[:counters].any()
+
+
+def test_attention_captured_zeroes_only_its_counters():
+    runtime = pytest.importorskip("cuda.bindings.runtime")
+    q, k, v, ks, vs, table, lengths, _ = attention_case([3000], None, 8, 2, 128, 64, "int8", "fp16")
+    cache = dk.PagedCache8.from_tensors(k.cuda(), v.cuda(), ks.cuda(), vs.cuda())
+    args = (q.cuda(), cache, table.cuda(), ints(lengths))
+    want = dk.cache_attention(*args)
+    out = torch.empty_like(want)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        dk.cache_attention(*args, out=out)
+    count = runtime.cudaGraphGetNodes(graph.raw_cuda_graph(), 0)[2]
+    nodes = runtime.cudaGraphGetNodes(graph.raw_cuda_graph(), count)[1][:count]
+    types = [runtime.cudaGraphNodeGetType(n)[1] for n in nodes]
+    kind = runtime.cudaGraphNodeType
+    assert sorted(types, key=int) == sorted([kind.cudaGraphNodeTypeKernel, kind.cudaGraphNodeTypeMemset], key=int)
+    zeroed = runtime.cudaGraphMemsetNodeGetParams(nodes[types.index(kind.cudaGraphNodeTypeMemset)])[1]
+    assert zeroed.width * zeroed.height * zeroed.elementSize == capi.load().dk_cache_attention_counter_bytes()
+    graph.instantiate()
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, want)
 
 
 # ---------------------------------------------------------------------------
