@@ -391,26 +391,41 @@ void cache_append(torch::Tensor k, torch::Tensor v, torch::Tensor slots, const C
                "cache_append");
 }
 
-// The attention workspace: one for each device, stream and head size, its
-// counters zeroed when it is made; every call leaves it ready for the next on that
-// stream.  A call that is being captured gets one of its own with the counters'
+// The attention workspaces: one for each device and stream, of the largest head
+// size that the stream has asked for (the counters lie in the same place for all),
+// its counters zeroed when it is made; every call leaves it ready for the next on
+// that stream.  They stay until release_workspaces(): a dropped one goes back to
+// the caching allocator, which gives it out again in its stream's order.  A call that is being captured gets one of its own with the counters'
 // zeroing (a few KB of some 24 MB) in the graph, since the graph may be replayed
 // beside later calls of the stream.
+struct Workspaces {
+  std::mutex mu;
+  std::map<std::pair<int, cudaStream_t>, torch::Tensor> of;
+};
+Workspaces& workspaces() {
+  static auto* w = new Workspaces();  // never destroyed: the process may end after the CUDA context
+  return *w;
+}
+
 torch::Tensor attention_workspace(int head_dim, const at::cuda::CUDAStream& stream) {
+  const int64_t bytes = static_cast<int64_t>(dk_cache_attention_workspace_bytes(head_dim));
   auto make = [&] {
-    const auto options = torch::TensorOptions().dtype(torch::kUInt8).device(stream.device());
-    const torch::Tensor w = torch::empty({static_cast<int64_t>(dk_cache_attention_workspace_bytes(head_dim))}, options);
+    const torch::Tensor w = torch::empty({bytes}, torch::TensorOptions().dtype(torch::kUInt8).device(stream.device()));
     C10_CUDA_CHECK(cudaMemsetAsync(w.data_ptr(), 0, dk_cache_attention_counter_bytes(), stream.stream()));
     return w;
   };
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return make();
-  static std::mutex mu;
-  // Never freed: the process may end after the CUDA context.
-  static auto* kept = new std::map<std::tuple<int, cudaStream_t, int>, torch::Tensor>();
-  const std::lock_guard<std::mutex> lock(mu);
-  torch::Tensor& w = (*kept)[{stream.device_index(), stream.stream(), head_dim}];
-  if (!w.defined()) w = make();
+  Workspaces& kept = workspaces();
+  const std::lock_guard<std::mutex> lock(kept.mu);
+  torch::Tensor& w = kept.of[{stream.device_index(), stream.stream()}];
+  if (!w.defined() || w.numel() < bytes) w = make();
   return w;
+}
+
+void release_workspaces() {
+  Workspaces& kept = workspaces();
+  const std::lock_guard<std::mutex> lock(kept.mu);
+  kept.of.clear();
 }
 
 std::tuple<torch::Tensor, OptTensor> cache_attention(torch::Tensor q, const Cache8& cache,
@@ -608,6 +623,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("cache"), py::arg("block_table"), py::arg("lengths"), py::arg("starts") = py::none(),
         py::arg("scale") = py::none(), py::arg("causal") = true, py::arg("window") = 0,
         py::arg("out") = py::none(), py::arg("lse") = false);
+  m.def("release_workspaces", &release_workspaces, "Drop the kept attention workspaces");
   m.def("block_norm", &block_norm, "Norms, gate and residual between two blocks",
         py::arg("residual"), py::arg("y"), py::arg("kind"), py::arg("post_weight"),
         py::arg("post_bias"), py::arg("gate"), py::arg("act"), py::arg("residual_scale"),

@@ -20,7 +20,7 @@ from typing import Optional
 
 import torch
 
-from .cache import CachePlan, PagedCache8, cache_append, cache_attention, cache_plan
+from .cache import CachePlan, PagedCache8, cache_append, cache_attention, cache_plan, release_workspaces
 from .norm import block_norm
 from .quantize import GROUP_SIZE, dequantize, quantize_and_pack, quantize_and_pack_cuda
 
@@ -41,6 +41,7 @@ __all__ = [
     "gemv_out",
     "quantize_and_pack",
     "quantize_and_pack_cuda",
+    "release_workspaces",
     "w4a16_linear",
 ]
 

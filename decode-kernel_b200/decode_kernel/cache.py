@@ -14,7 +14,7 @@ from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
 
-__all__ = ["CachePlan", "PagedCache8", "cache_append", "cache_attention", "cache_plan"]
+__all__ = ["CachePlan", "PagedCache8", "cache_append", "cache_attention", "cache_plan", "release_workspaces"]
 
 _module = None
 
@@ -144,3 +144,14 @@ def cache_attention(q: torch.Tensor, cache: PagedCache8, block_table: torch.Tens
     """
     o, l = _extension().cache_attention(q, cache._handle, block_table, lengths, starts, scale, causal, window, out, lse)
     return (o, l) if lse else o
+
+
+def release_workspaces() -> None:
+    """Give the memory that ``cache_attention`` keeps back to torch's allocator.
+
+    It keeps one workspace (24 MB; 12 MB for heads of 64) for each device and
+    stream that it was called on outside a capture.  Call this after a change of
+    streams, and before a stream of one's own is destroyed: a new stream could
+    get its handle.  The next call on a stream makes a new workspace.
+    """
+    _extension().release_workspaces()

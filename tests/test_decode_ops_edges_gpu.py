@@ -144,6 +144,36 @@ def test_attention_captured_zeroes_only_its_counters():
         assert torch.equal(out, want)
 
 
+def test_attention_workspaces_are_shared_by_head_sizes_and_given_back():
+    cases = []
+    for dim, hq, kv in ((64, 8, 2), (256, 4, 2), (128, 32, 8)):
+        q, k, v, ks, vs, table, lengths, _ = attention_case([5000, 40], None, hq, kv, dim, 64, "int8", "fp16", seed=dim)
+        args = (q.cuda(), dk.PagedCache8.from_tensors(k.cuda(), v.cuda(), ks.cuda(), vs.cuda()), table.cuda(), ints(lengths))
+        cases.append((args, dk.cache_attention(*args)))
+    torch.cuda.synchronize()
+    dk.release_workspaces()
+    most = capi.load().dk_cache_attention_workspace_bytes(128)
+    assert most >= capi.load().dk_cache_attention_workspace_bytes(256)
+    kept = torch.cuda.memory_allocated()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for s in streams:
+        with torch.cuda.stream(s):
+            for args, want in cases * 2:
+                assert torch.equal(dk.cache_attention(*args), want)
+    torch.cuda.synchronize()
+    assert 3 * most <= torch.cuda.memory_allocated() - kept < 3 * most + (8 << 20)
+    # Given back between calls that are still on their way.
+    outs = []
+    for i in range(6):
+        with torch.cuda.stream(streams[i % 3]):
+            outs += [(dk.cache_attention(*args), want) for args, want in cases]
+        dk.release_workspaces()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o, want in outs)
+    del outs
+    assert torch.cuda.memory_allocated() - kept < 4 << 20
+
+
 # ---------------------------------------------------------------------------
 # Append
 # ---------------------------------------------------------------------------
