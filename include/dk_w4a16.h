@@ -380,6 +380,10 @@ typedef struct dk_cache8 {
  * cannot serve, or that would pass max_blocks pages, gets none of its tokens:
  * its length stays and its new tokens have slot -1.  The ring serves a request
  * only if the pages asked for by all requests up to it were free.
+ * A request's pages are the first ceil(held / block_size) entries of its row.
+ * All of them are its own until it ends, when each goes to the ring as it stands:
+ * a page that was given to others before, or an entry that was overwritten,
+ * would be handed out twice or lost.
  * Writes
  *   lengths  int32 [requests]      tokens held after the step (0 if ended)
  *   starts   int32 [requests + 1]  first row of each request's new tokens
