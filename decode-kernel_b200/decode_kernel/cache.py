@@ -98,7 +98,9 @@ def cache_plan(held: torch.Tensor, fresh: torch.Tensor, block_table: torch.Tenso
     ring ``free_blocks`` (entries ``ring[0] <= i < ring[1]``, modulo its
     length) into ``block_table`` [requests, max_blocks], which is updated in
     place like the ring's entries; ended requests' pages go to its end: all
-    ceil(held / block_size) of them, so none may be released before.
+    ceil(held / block_size) of them, so none may be released before.  ``held``
+    may be lowered between calls (drafts taken back); pages that it leaves have
+    to be put at the ring's end by the caller, or they are lost.
     ``tokens`` is the number of rows of the step, padding included.  A request
     that the free pages or the table's width cannot serve keeps its length, its
     rows have slot -1, and the returned ring's entries 2 and 3 say how many

@@ -383,7 +383,10 @@ typedef struct dk_cache8 {
  * A request's pages are the first ceil(held / block_size) entries of its row.
  * All of them are its own until it ends, when each goes to the ring as it stands:
  * a page that was given to others before, or an entry that was overwritten,
- * would be handed out twice or lost.
+ * would be handed out twice or lost.  The caller may lower held[r] between calls
+ * (drafts taken back) while the number of its pages stays; of the pages that a
+ * lower length leaves it has to put each at the ring's end first
+ * (free_blocks[ring[1]++ % free_capacity] = page), or they are lost.
  * Writes
  *   lengths  int32 [requests]      tokens held after the step (0 if ended)
  *   starts   int32 [requests + 1]  first row of each request's new tokens

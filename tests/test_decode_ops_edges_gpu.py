@@ -17,6 +17,42 @@ pytestmark = pytest.mark.gpu
 
 
 # ---------------------------------------------------------------------------
+# Plan
+# ---------------------------------------------------------------------------
+
+
+def test_plan_with_drafts_taken_back_loses_no_page():
+    """Steps of five tokens of which some are taken back: the pages that a lower length leaves go to the ring's end."""
+    requests, bs, width, blocks = 40, 16, 12, 300
+    g = gen(1)
+    held = torch.zeros(requests, dtype=torch.int32, device="cuda")
+    table = torch.full((requests, width), -1, dtype=torch.int32, device="cuda")
+    free = torch.arange(blocks, dtype=torch.int32, device="cuda")
+    ring = ints([0, blocks, 0, 0], torch.int64)
+    column = torch.arange(width, device="cuda")
+    most = 0
+    for step in range(60):
+        fresh = torch.full((requests,), 5, dtype=torch.int32)
+        fresh[torch.rand(requests, generator=g) < 0.03] = -1
+        plan = dk.cache_plan(held, fresh.cuda(), table, free, ring, bs, 5 * requests)
+        held, ring = plan.lengths, plan.ring
+        assert ring[2:].tolist() == [0, 0]
+        # Up to 21 tokens back, past a page's border now and then.
+        back = torch.where(torch.rand(requests, generator=g) < 0.1, 21, torch.randint(0, 5, (requests,), generator=g)).int().cuda()
+        kept = (held - back).clamp(min=0).clamp(max=width * bs - 10)
+        left = table[(column >= -(-kept // bs)[:, None]) & (column < -(-held // bs)[:, None])]
+        free[(ring[1] + torch.arange(len(left), device="cuda")) % len(free)] = left
+        ring[1] += len(left)
+        most = max(most, len(left))
+        held = kept
+        mine = table[column < -(-held // bs)[:, None]].tolist()
+        head, tail = ring[:2].tolist()
+        spare = free[torch.arange(head, tail, device="cuda") % blocks].tolist()
+        assert sorted(mine + spare) == list(range(blocks)), step
+    assert most > 0 and held.max() > 4 * bs
+
+
+# ---------------------------------------------------------------------------
 # Attention
 # ---------------------------------------------------------------------------
 
