@@ -8,9 +8,12 @@
 // the exponent: with t_j = s_j log2(e) + log2(vs_j) and w_j = 2^(t_j - m),
 //   out = (sum_j w_j Vcode_j) / (sum_j w_j / vs_j),
 // so the codes enter the tensor core unscaled (int8 and e4m3 are exact in
-// fp16) and w_j is at most 2^8, whatever the scales.  w_j is rounded to fp16
+// fp16) and w_j is at most 2^15, whatever the scales.  w_j is rounded to fp16
 // (11 bits; a relative 2^-12 on each weight, the size of the rounding of an
-// fp16 output); scores, maxima, sums and outputs are fp32.
+// fp16 output); scores, maxima, sums and outputs are fp32.  m puts the largest
+// weight at 2^7 or above, so that weights keep their 11 bits down to 2^-21 of it
+// and something down to 2^-32 (with the largest at 1, a token of large score and
+// little V would wipe out all that come to 2^-25 of it, in any number).
 //
 // What bounds it: the cache's bytes from HBM, up to about 16 query rows per KV
 // head; beyond, the matrix instructions.  A tile of 16 tokens and 8 query rows
@@ -61,7 +64,8 @@ constexpr int kTile = 16;             // tokens of a tile: of one page, one matr
 constexpr int kMaxRequests = 1024;    // requests of one launch (their prefix sums are in shared memory)
 constexpr int kShort = 96;            // tiles of segments that no two CTAs share
 constexpr float kFarBelow = -1e30f;   // maximum of a row that has seen no token
-constexpr float kSlack = 8.f;         // a row's maximum may lag its scores by this much (log2)
+constexpr float kTop = 7.f;           // log2 of the largest weight where a row's maximum is up to date
+constexpr float kSlack = 8.f;         // it may lag its scores by this much (log2)
 constexpr float kLeastScale = 8.4703294725430034e-22f;  // 2^-70: keeps sum w / vs finite
 
 struct AttendArgs {
@@ -520,10 +524,10 @@ struct Attend {
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
           const uint32_t bit = 1u << (2 * n + i);
-          float by = fmaxf(top, 0.f), f = exp2_approx(-by);
+          float by = fmaxf(top - kTop, 0.f), f = exp2_approx(-by);
           if (unseen & bit) {  // its sums are zeros
             const bool some = top > -INFINITY;
-            by = some ? top : 0.f;
+            by = some ? top - kTop : 0.f;
             f = 0.f;
             if (some) unseen &= ~bit;
           }
@@ -617,7 +621,7 @@ struct Attend {
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n)
-          above |= fmaxf(fmaxf(sc[h][n][0], sc[h][n][2]), fmaxf(sc[h][n][1], sc[h][n][3])) > kSlack;
+          above |= fmaxf(fmaxf(sc[h][n][0], sc[h][n][2]), fmaxf(sc[h][n][1], sc[h][n][3])) > kTop + kSlack;
       }
       if (__any_sync(0xffffffffu, above) || !settled) grow(sc);
       uint32_t pb[MT][NT][2];

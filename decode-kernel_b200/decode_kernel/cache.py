@@ -142,6 +142,9 @@ def cache_attention(q: torch.Tensor, cache: PagedCache8, block_table: torch.Tens
     ``window`` or more before it.  A query that sees no token gets zeros.
     ``scale`` defaults to head_dim ** -0.5.
 
+    Scores and sums are fp32; the softmax's weights are rounded to fp16 for the
+    product with V (2^-12 of each).
+
     Returns out, or (out, lse) with the fp32 [tokens, q_heads] log of the sums
     of exponentials.
     """

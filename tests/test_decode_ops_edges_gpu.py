@@ -5,6 +5,7 @@ place, captured calls, and the sizes at which a launch takes another form."""
 from __future__ import annotations
 
 import ctypes
+import math
 
 import pytest
 import torch
@@ -97,6 +98,26 @@ def test_attention_of_fewer_rows_than_starts(hq, kv, dim, window):
         # Another split of the same sums: fp16 weights and outputs.
         torch.testing.assert_close(some, whole[:rows], rtol=2.0 ** -9, atol=2.0 ** -9 * float(whole.abs().max()))
         torch.testing.assert_close(some_lse, lse[:rows], rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.parametrize("dim,fresh", [(128, None), (64, None), (128, 5), (256, None)])
+def test_attention_of_many_small_weights_behind_a_large_one(dim, fresh):
+    """The first token has all the weight and no V; what the others leave, each 2^-25.3 of it, is the output."""
+    requests, kv, n = 300, 8, 1024  # more segments than warps: one warp adds up a whole one
+    k = torch.zeros(n // 64, kv, 64, dim, dtype=torch.int8)
+    v = torch.full_like(k, 100)
+    k[0, :, 0, 0], v[0, :, 0] = 127, 0
+    cache = dk.PagedCache8.from_tensors(k.cuda(), v.cuda(), *(torch.ones(n // 64, kv, device="cuda") for _ in range(2)))
+    each = fresh or 1
+    q = torch.zeros(requests * each, kv, dim, dtype=torch.float16, device="cuda")
+    q[:, :, 0] = 1
+    starts = ints([each * r for r in range(requests + 1)]) if fresh else None
+    table = torch.arange(n // 64, dtype=torch.int32, device="cuda").expand(requests, -1).contiguous()
+    out = dk.cache_attention(q, cache, table, ints([n] * requests), starts, scale=25.3 * math.log(2) / 127).double().cpu()
+    others = torch.arange(n - each, n, dtype=torch.float64).repeat(requests) * 2.0 ** -25.3
+    want = (100 * others / (1 + others))[:, None, None]
+    # A weight is 2^-18.3 of fp16's 1 and rounded to a multiple of 2^-24; the score's and the output's own rounding.
+    assert ((out - want).abs() <= (2.0 ** -6.7 + 2.0 ** -10) * want).all()
 
 
 def test_attention_over_a_wide_table():
