@@ -347,8 +347,9 @@ struct Attend {
       }
     }
   }
-  // bf16 rows to fp16: scaled by a power of two into its range (the return
-  // value undoes it).
+  // bf16 rows to fp16: scaled by a power of two, which the return value undoes,
+  // to 2^14 and above, so that values keep their 8 bits down to 2^-31 of the row's
+  // largest (and 2^-39 of it is still not 0).
   __device__ static __forceinline__ float convert_q(const AttendArgs& a, uint32_t (&b)[2 * kKWords]) {
     if (!a.bf16) return 1.f;
     float top = 0.f;
@@ -357,9 +358,9 @@ struct Attend {
       top = fmaxf(top, fmaxf(fabsf(__uint_as_float(b[i] << 16)), fabsf(__uint_as_float(b[i] & 0xffff0000u))));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    // 2^-e with e the exponent of the row's largest value; 1 for a row of zeros.
-    const int e = min(max((int)(__float_as_uint(top) >> 23), 2), 252);
-    const float down = __uint_as_float((uint32_t)(254 - e) << 23), up = __uint_as_float((uint32_t)e << 23);
+    // 2^(14 - e) with e the exponent of the row's largest value, within fp32's range.
+    const int e = min(max((int)(__float_as_uint(top) >> 23), 15), 254);
+    const float down = __uint_as_float((uint32_t)(254 + 14 - e) << 23), up = __uint_as_float((uint32_t)(e - 14) << 23);
 #pragma unroll
     for (int i = 0; i < 2 * kKWords; ++i)
       b[i] = pack_half2(__uint_as_float(b[i] << 16) * down, __uint_as_float(b[i] & 0xffff0000u) * down);

@@ -143,7 +143,8 @@ def cache_attention(q: torch.Tensor, cache: PagedCache8, block_table: torch.Tens
     ``scale`` defaults to head_dim ** -0.5.
 
     Scores and sums are fp32; the softmax's weights are rounded to fp16 for the
-    product with V (2^-12 of each).
+    product with V (2^-12 of each), and bf16 queries scaled by a power of two
+    into fp16 (which values below 2^-31 of their row's largest lose bits by).
 
     Returns out, or (out, lse) with the fp32 [tokens, q_heads] log of the sums
     of exponentials.

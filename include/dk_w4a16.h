@@ -435,7 +435,8 @@ DK_API dk_status dk_cache_append(const dk_cache8* cache, const void* k, const vo
  * rounded once from fp32; scores, maxima, sums and lse are fp32, but the
  * softmax's weights are rounded to fp16 for the product with V (2^-12 of each,
  * more below 2^-21 of the largest, and those below 2^-32 of it count as 0
- * there).  Rows that see no token are zeros.  lse (or NULL)
+ * there), and bf16 queries are scaled by a power of two into fp16 (values below
+ * 2^-31 of their row's largest lose bits).  Rows that see no token are zeros.  lse (or NULL)
  * gets log(sum_j exp(scale * q . k_j)), -inf for such rows.  q has strides in
  * elements, multiples of 8, and is 16-byte aligned; out and lse are contiguous.
  * Block strides are below 2^31 and block_size * token stride too.  Calls are

@@ -120,6 +120,18 @@ def test_attention_of_many_small_weights_behind_a_large_one(dim, fresh):
     assert ((out - want).abs() <= (2.0 ** -6.7 + 2.0 ** -10) * want).all()
 
 
+@pytest.mark.parametrize("dim,hq,kv,fresh", [(64, 8, 2, None), (128, 8, 2, None), (128, 8, 2, [3, 1, 9]), (256, 4, 2, None)])
+def test_attention_of_queries_with_one_large_channel(dim, hq, kv, fresh):
+    """A channel of bf16 queries 2^22 times the others, in which the keys hold nothing: the others make the scores."""
+    q, k, v, ks, vs, table, lengths, starts = attention_case([70, 130, 400], fresh, hq, kv, dim, 32, "int8", "bf16", seed=dim)
+    q[..., 5] = 2.0 ** 22
+    k[..., 5] = 0
+    check_attention((q, k, v, ks, vs, table, lengths, starts))
+    q[..., 5] = 0
+    for size in (2.0 ** 123, 2.0 ** -120):  # near the ends of bf16's range
+        check_attention((q * size, k, v, ks, vs, table, lengths, starts), scale=dim ** -0.5 / size)
+
+
 def test_attention_over_a_wide_table():
     """A table for 131072 tokens and 16384 rows in q, of which short requests use a few."""
     lengths, fresh = [300, 290, 17, 1000], [256, 1, 17, 100]
