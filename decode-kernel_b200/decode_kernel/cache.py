@@ -142,6 +142,10 @@ def cache_attention(q: torch.Tensor, cache: PagedCache8, block_table: torch.Tens
     ``window`` or more before it.  A query that sees no token gets zeros.
     ``scale`` defaults to head_dim ** -0.5.
 
+    Rows past ``starts[-1]`` are not written (a new ``out`` holds anything there),
+    and rows of a request that ``cache_plan`` could not serve (slot -1) mean
+    nothing: its last old tokens are taken for theirs.
+
     Scores and sums are fp32; the softmax's weights are rounded to fp16 for the
     product with V (2^-12 of each), and bf16 queries scaled by a power of two
     into fp16 (which values below 2^-31 of their row's largest lose bits by).

@@ -448,7 +448,9 @@ DK_API dk_status dk_cache_append(const dk_cache8* cache, const void* k, const vo
  * look is not looked at, NaN codes and scales included; an e4m3 NaN code of V
  * that one of a request's queries sees may reach its other queries too.
  * starts rise; where they pass `tokens` the rows that q has are served, in
- * their places.
+ * their places, and rows of q past the last start get no output.  Rows of a
+ * request that dk_cache_plan could not serve (slot -1) are answered as if its old
+ * tokens were theirs: their output means nothing.
  * The workspace (dk_cache_attention_workspace_bytes of the current device) is
  * 256-byte aligned.  Its first dk_cache_attention_counter_bytes are zero before
  * its first call, and every call leaves them so for the next; the rest may hold
