@@ -34,7 +34,8 @@ class PagedCache8:
 
     ``k``, ``v``: int8 or float8_e4m3fn [blocks, kv_heads, block_size, head_dim];
     ``k_scale``, ``v_scale``: fp32 [blocks, kv_heads].  A value is its code
-    times its page's and head's scale.  block_size is a multiple of 16 up to
+    times its page's and head's scale; scales are positive (V's below 2^-70,
+    negative ones too, count as 2^-70).  block_size is a multiple of 16 up to
     256, head_dim 64, 128 or 256.
     """
 

@@ -355,7 +355,8 @@ typedef enum dk_dtype {
 /* A pool of pages.  Page p holds block_size tokens of every KV head:
  *   k[p, h, i, :], v[p, h, i, :]   head_dim codes (DK_INT8 or DK_E4M3)
  *   k_scale[p, h], v_scale[p, h]   fp32 [blocks, kv_heads], contiguous
- * and a value is its code times its page's and head's scale.  Strides are in
+ * and a value is its code times its page's and head's scale; V's scales are
+ * positive (below 2^-70, negative ones too, they count as 2^-70).  Strides are in
  * codes (bytes), multiples of 32; the last dimension is contiguous; k and v
  * are 32-byte aligned.  block_size: a multiple of 16 in 16..256.  head_dim:
  * 64, 128 or 256. */
@@ -443,8 +444,7 @@ DK_API dk_status dk_cache_append(const dk_cache8* cache, const void* k, const vo
  * served as long as max_blocks * block_size (the table's width in tokens) times
  * min(requests, 1024) + tokens * q_heads / kv_heads / 8 is below 2^33, and
  * tokens * q_heads below 2^31; past that DK_ERR_UNSUPPORTED may come back.
- * V scales below 2^-70 count as 2^-70.  Entries of block_table outside the pool
- * hide their tokens.  What stands in the cache where no query of a request may
+ * Entries of block_table outside the pool hide their tokens.  What stands in the cache where no query of a request may
  * look is not looked at, NaN codes and scales included; an e4m3 NaN code of V
  * that one of a request's queries sees may reach its other queries too.
  * starts rise; where they pass `tokens` the rows that q has are served, in
