@@ -12,7 +12,8 @@ import torch
 
 import decode_kernel as dk
 from decode_kernel import capi
-from test_decode_ops_gpu import CODES, HALF, attention_case, check_attention, encode, gen, ints, random_pools, raw, run_attention
+from test_decode_ops_gpu import (CODES, HALF, attention_case, check_append, check_attention, encode, gen, ints, plan_reference, random_pools, raw,
+                                 run_attention, slots_of)
 
 pytestmark = pytest.mark.gpu
 
@@ -51,6 +52,33 @@ def test_plan_with_drafts_taken_back_loses_no_page():
         spare = free[torch.arange(head, tail, device="cuda") % blocks].tolist()
         assert sorted(mine + spare) == list(range(blocks)), step
     assert most > 0 and held.max() > 4 * bs
+
+
+@pytest.mark.parametrize("inplace", [False, True])
+@pytest.mark.parametrize("requests,bs,longest,new", [(300, 16, 900, 1300), (2048, 48, 200, 400)])
+def test_plan_of_many_slots(requests, bs, longest, new, inplace):
+    """Hundreds of thousands of slots, which threads take eight at a time; empty, ended, refused and too wide requests among them."""
+    g = gen(requests)
+    held = torch.randint(0, longest, (requests,), generator=g).tolist()
+    fresh = torch.randint(0, new, (requests,), generator=g).tolist()
+    width = -(-(longest + new) // bs) + 1
+    for r in range(0, requests, 7):
+        fresh[r] = (0, -1, 1, width * bs + 5)[r // 7 % 4]
+    need = sum(-(-(h + max(n, 0)) // bs) - -(-h // bs) for h, n in zip(held, fresh) if h + max(n, 0) <= width * bs)
+    order = torch.randperm(2 * requests * width + need + 64, generator=g)
+    table, free = order[:requests * width].view(requests, width).tolist(), order[requests * width:].tolist()
+    ring = [len(free) - 50, len(free) - 50 + need - 40, 0, 0]  # wraps, and the last requests find too few pages
+    total = sum(max(n, 0) for n in fresh)
+    assert total > 160000
+    for tokens in (total, total + 13, total - 3):
+        want = plan_reference(held, fresh, table, free, ring, bs, tokens)
+        assert want[3][2] > 0 and want[3][3] > 0
+        dt, df, dr, dh = ints(table), ints(free), ints(ring, torch.int64), ints(held)
+        out = dk.CachePlan(dh, torch.empty(requests + 1, dtype=torch.int32, device="cuda"), torch.empty(tokens, dtype=torch.int64, device="cuda"), dr)
+        p = dk.cache_plan(dh, ints(fresh), dt, df, dr, bs, tokens, out=out if inplace else None)
+        got = [p.lengths.tolist(), p.starts.tolist(), p.slots.tolist(), p.ring.tolist(), dt.tolist(), df.tolist()]
+        for name, a, b in zip(("lengths", "starts", "slots", "ring", "table", "free"), got, want):
+            assert a == b, name
 
 
 # ---------------------------------------------------------------------------
@@ -155,6 +183,14 @@ def test_attention_takes_kv_heads_in_several_launches(dim, code, dtype, fresh):
     wide = torch.full((2, (1 << 30) // 256), -1, dtype=torch.int32)
     wide[:, :table.shape[1]] = table
     check_attention((q, k, v, ks, vs, wide, lengths, starts))
+
+
+@pytest.mark.parametrize("dim,hq,kv,code,dtype", [(128, 8, 2, "int8", "bf16"), (64, 3, 3, "e4m3", "fp16"), (256, 4, 2, "int8", "fp16")])
+def test_attention_of_prompts(dim, hq, kv, code, dtype):
+    """A prompt of a thousand tokens, one behind kept tokens, and single tokens beside them."""
+    lengths, fresh = [1000, 1, 900, 333, 77], [1000, 1, 300, 1, 1]
+    for window in (0, 130):
+        check_attention(attention_case(lengths, fresh, hq, kv, dim, 64, code, dtype, seed=window + dim), window=window)
 
 
 def c_attention(q, cache, table, lengths, out, workspace):
@@ -308,3 +344,27 @@ def test_append_rows_with_gaps(dtype, code, dim, heads, bs, pages, most):
     k[::7, :, 3] = float("inf")
     v[::5, :, 1] = float("nan")
     check_pages(k, v, slots, pools, code)
+
+
+@pytest.mark.parametrize("dtype,code", [("fp16", "e4m3"), ("bf16", "int8")])
+@pytest.mark.parametrize("dim,heads,bs,tokens", [
+    # Token-heads of K and V in the hundreds of thousands: a CTA takes two, then four heads' K or V, fewer in the last one.
+    (64, 5, 48, 20000), (64, 5, 256, 40000), (128, 9, 64, 12000), (128, 7, 16, 30000), (256, 3, 256, 33000), (256, 3, 48, 65000),
+    # Long runs in windows of 16 and of 64 tokens.
+    (128, 8, 64, 1000), (64, 3, 256, 4000), (128, 8, 64, 2500), (256, 2, 48, 9000),
+])
+def test_append_in_wide_windows(dtype, code, dim, heads, bs, tokens):
+    """Every form that the number of tokens and heads chooses, with pages begun before, short and long runs and values that are not finite."""
+    g = gen(dim + tokens)
+    held, new, left = [], [], tokens
+    while left > 0:
+        n = min(left, int(torch.randint(1, 7 * bs, (1,), generator=g)))
+        held.append(int(torch.randint(0, 2 * bs, (1,), generator=g)))
+        new.append(n)
+        left -= n
+    slots, pages = slots_of(held, new, bs, g)
+    slots = torch.where(torch.rand(len(slots), generator=g) < 0.001, torch.where(slots % bs == 0, -1, slots), slots)  # rows that begin a page left out
+    pools = random_pools(pages, heads, bs, dim, code, g)
+    k, v = ((torch.randn(tokens, heads, dim, generator=g) * torch.rand(tokens, heads, 1, generator=g) * 5).to(HALF[dtype][0]) for _ in range(2))
+    k[::501, :, 3], v[::701, 0, 7], v[::333, -1, 1] = float("inf"), float("-inf"), float("nan")
+    check_append(k, v, slots, pools, code)
