@@ -722,15 +722,22 @@ extern "C" dk_status dk_cache_append(const dk_cache8* c, const void* k, const vo
   a.kv_heads = c->kv_heads;
   a.bf16 = dtype == DK_BF16;
   a.block_magic = ~0ull / (unsigned long long)c->block_size + 1;
-  // The window: four tokens, one for each warp, up to 20 CTAs an SM (400 single
-  // tokens, 8 heads: 11.7 us, with windows of 16 13.8), then 16 up to 14 CTAs an
-  // SM (1510 tokens in runs of 15: 10.6 us, with windows of 64 13.9), then 64,
-  // since most windows would hold no run's beginning (3930 tokens in runs of 48
-  // and 5 heads: 8.7 us, with windows of 16 9.7).  With the largest windows a CTA
+  // The window: four tokens, one for each warp, as long as single tokens gain by
+  // it, up to 16 CTAs an SM; then 16 tokens up to 14 CTAs an SM; then 64, since most
+  // windows would hold no run's beginning.  The length of the runs is the device's
+  // to know.  Measured with 8 heads of 128, int8, us by windows of 4 / 16 (first
+  // two lines) and of 16 / 64 for runs of
+  //                      1 token    4          8          16         48        256
+  //    296 tokens, 8 CTAs    9/15     6.1/5.6    5.8/4.5    5.2/4.1   5.4/4.5   12/12
+  //    590 tokens, 16       15/15      11/5.7    8.8/4.6    8.1/4.3   7.5/4.7   15/13
+  //   1480 tokens, 10       33/54      12/16      10/10     7.5/6.0   6.8/6.9   16/15
+  //   2070 tokens, 14       42/54      14/16      11/10      10/7.1   8.5/7.8   18/15
+  //   2960 tokens, 20       57/64      19/19      15/13      14/9.3    11/7.9   20/16
+  // and the same turns with 5 heads of 64 and 4 of 256.  With the largest windows a CTA
   // takes several heads, as long as there are ten CTAs an SM: it reads the slots
   // once for all of them.
   const long long each = (long long)tokens * c->kv_heads * 2, sms = sm_count(-1);
-  a.window = each / kAppendWarps <= 20 * sms ? kAppendWarps : each / 16 <= 14 * sms ? 16 : kMaxWindow;
+  a.window = each / kAppendWarps <= 16 * sms ? kAppendWarps : each / 16 <= 14 * sms ? 16 : kMaxWindow;
   a.items = 1;
   while (a.window == kMaxWindow && a.items < kMaxItems && each / kMaxWindow / (2 * a.items) >= 10 * sms) a.items *= 2;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
