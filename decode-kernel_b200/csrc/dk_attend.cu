@@ -62,7 +62,8 @@ namespace {
 
 constexpr int kTile = 16;             // tokens of a tile: of one page, one matrix instruction's rows
 constexpr int kMaxRequests = 1024;    // requests of one launch (their prefix sums are in shared memory)
-constexpr int kShort = 96;            // tiles of segments that no two CTAs share
+constexpr int kShort = 96;            // tiles of segments that no two CTAs share, where there are many
+constexpr int kVeryShort = 36;        // places of segments that no two CTAs share, however few
 constexpr float kFarBelow = -1e30f;   // maximum of a row that has seen no token
 constexpr float kTop = 7.f;           // log2 of the largest weight where a row's maximum is up to date
 constexpr float kSlack = 8.f;         // it may lag its scores by this much (log2)
@@ -222,7 +223,7 @@ struct Attend {
     int4 rows[W][kRows];               // of the latter's rows: token (-1: no such row), head, low, high
     int used[kSlots];
     int last[2];
-    int total[W], longest[W];
+    int total[W], longest[W], segments[W];
     int range[2];
   };
 
@@ -737,10 +738,10 @@ struct Attend {
     int* lengths = prefix + a.requests + 1;
     int* starts = lengths + a.requests;
     const int most = (int)min((long long)a.max_blocks * a.block_size, 0x7fffffffLL);
-    int carry = 0, longest = 0;
+    int carry = 0, longest = 0, segments = 0;
     for (int base = 0; base < a.requests; base += W * 32) {
       const int r = base + tid;
-      int mine = 0;
+      int mine = 0, count = 0;
       if (r < a.requests) {
         const int length = min(max(ld_int(a.lengths + r), 0), most);
         int first = r, fresh = 1, unit0;
@@ -756,7 +757,8 @@ struct Attend {
         if (tiles > 0) {
           const int one = units_of(a, length, fresh, unit0) + kStart;
           longest = max(longest, one);
-          mine = one * tiles * a.heads;
+          count = tiles * a.heads;
+          mine = one * count;
         }
       }
       int sum = mine;
@@ -766,9 +768,11 @@ struct Attend {
         if (lane >= d) sum += x;
       }
       longest = __reduce_max_sync(0xffffffffu, longest);
+      count = __reduce_add_sync(0xffffffffu, count);
       if (lane == 31) {
         sh.total[warp] = sum;
         sh.longest[warp] = longest;
+        sh.segments[warp] = count;
       }
       __syncthreads();
       int before = carry, all = 0;
@@ -778,6 +782,7 @@ struct Attend {
         if (w < warp) before += x;
         all += x;
         longest = max(longest, sh.longest[w]);
+        segments += sh.segments[w];
       }
       if (r < a.requests) prefix[r] = before + sum - mine;
       carry += all;
@@ -794,13 +799,21 @@ struct Attend {
     // are short the borders move to the nearest segment's, so that no segment
     // is shared between CTAs: joining one costs about as long as the units do
     // that a CTA gets too many.  (64 requests of up to 200 tokens 15.6 -> 12.0
-    // us, of up to 1000 tokens 24.8 -> 21.6; from 2000 on it makes no odds.)
+    // us, of up to 1000 tokens 24.8 -> 21.6; from 2000 on it makes no odds.)  Few
+    // segments would leave CTAs idle, though, and from 36 units on that costs more
+    // than the joins: 8 KV heads of 128, us with moved borders / without, requests of
+    //                 300 tokens  700        1000       1500
+    //    1 (8 segments)  7.9/9.6   10.0/9.9  11.9/10.2  14.5/10.9
+    //    8 (64)          9.5/11    13.2/12.4 15.9/13.2  20.4/15.1
+    //   24 (192)         9.8/13    13.5/14.9 16.3/17.9  20.9/20.7
+    //   64 (512)          13/17    21.0/24.4 28.6/32.7  39.1/42.2
+    // so borders move there only if there are segments for half the CTAs.
     const int least = max(W, (int)sqrtf(0.5f * longest));
     const int grid = min((int)gridDim.x, (all + least - 1) / least);
     const int chunk = (all + grid - 1) / grid;
     const int cta = blockIdx.x;
     if (cta >= grid || cta * chunk >= all) return;
-    const bool snap = longest <= kShort / MT;
+    const bool snap = longest <= kVeryShort || (longest <= kShort / MT && 2 * segments >= (int)gridDim.x);
     int cta0 = cta * chunk, cta1 = min(all, cta0 + chunk);
     if (snap) {
       if (warp < 2) {
