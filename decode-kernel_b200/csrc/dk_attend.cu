@@ -608,9 +608,9 @@ struct Attend {
         const int first = base + h * kTile;
         edge[h] = first + kTile > least_high || first < most_low || !good;  // the same in all lanes
         if (edge[h]) {
-          // No row sees any of the tile's tokens: its page may be hidden wholly,
-          // scales of NaN and all (a unit of two tiles begins at a whole unit).
-          if (!good || first + kTile <= least_low || first >= most_high) v_inverse[h] = 0.f;
+          // A unit of two tiles begins at a whole unit, so that its first may be a
+          // page that the window hides wholly, scales of NaN and all.
+          if (!good || (MT > 1 && (first + kTile <= least_low || first >= most_high))) v_inverse[h] = 0.f;
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
