@@ -17,9 +17,10 @@ namespace {
 // writes its share of the table's new entries, the ring's and the slots;
 // nothing is exchanged between CTAs and one launch does it all.  A small step
 // (a decode step's one token a request) is one CTA and bound by latency: the
-// launch, two dependent loads and the sums; a call of 64 requests takes 8.3 us
+// launch, two dependent loads and the sums; a call of 64 requests takes 8.7 us
 // through Python, which is the host's.  A large one (2048 requests, half a
-// million slots: 9.3 us) adds the sums' rounds and the slots' 8 bytes, 0.6 us.
+// million slots: 9.2 us) adds the sums' rounds and the slots' 8 bytes, 0.6 us.
+// With outputs in place of inputs one CTA does it all (that one: 370 us).
 // ---------------------------------------------------------------------------
 constexpr int kPlanThreads = 512;
 
@@ -241,8 +242,8 @@ __global__ void __launch_bounds__(kPlanThreads) k_cache_plan(const __grid_consta
 // again if it grew, the new codes.  Bound by bytes, 2 read and 1 written for
 // each value (long runs), or by latency (single tokens): slot -> scale and
 // values -> codes.  Measured: 16 requests of up to 2047 tokens, 8 heads of 128,
-// e4m3 25.3 us (4.0 TB/s), 37 ragged pieces, 5 heads of 64, int8 8.7 us, a step
-// of 96 tokens 5.3 us through Python.
+// e4m3 27 us (3.8 TB/s), 37 ragged pieces, 5 heads of 64, int8 8.6 us, a step
+// of 96 tokens 5.5 us through Python.
 //
 // A CTA looks for the runs that begin in its window of tokens, reading the
 // slots of the window and of the pages that may begin in it at once.  A short
@@ -371,9 +372,74 @@ __device__ __forceinline__ uint32_t add_largest_finite(uint32_t top, const uint4
   return top;
 }
 
+// A warp's share (w of `warps`) of n rows coded again.
+template <int D, bool E4M3>
+__device__ __forceinline__ void rows_again(uint8_t* rows, long long ps, int n, float ratio, int w, int warps) {
+  constexpr int LR = D / 16, RW = 32 / LR;  // 16 codes a lane
+  const int lane = threadIdx.x & 31;
+#pragma unroll 4
+  for (int i = w * RW + lane / LR; i < n; i += warps * RW) {
+    uint4* p = reinterpret_cast<uint4*>(rows + i * ps + lane % LR * 16);
+    const uint4 c = *p;
+    *p = make_uint4(code_again<E4M3>(c.x, ratio), code_again<E4M3>(c.y, ratio), code_again<E4M3>(c.z, ratio), code_again<E4M3>(c.w, ratio));
+  }
+}
+
+// The scale of a page whose was `old`, with values up to that of the pattern `top`.
+template <bool E4M3>
+__device__ __forceinline__ float scale_of(float old, uint32_t top, int bf16) {
+  const float x = bf16 ? __uint_as_float(top << 16) : __half2float(__ushort_as_half((unsigned short)top));
+  return fmaxf(old, __fdiv_rn(fmaxf(x, kLeastAmax), E4M3 ? 448.f : 127.f));
+}
+
+// The runs of a window where rows of a page rise with gaps between them (nothing
+// that cache_plan makes): a warp takes a page's tokens, reads them twice and places
+// each.  Rows in the gaps keep what they hold.  slots[i]: of the window's token i;
+// slots[-1] is its neighbour's.  A function of its own, called: in line its
+// instructions lie among the kernel's, 30 -> 34 us for a first call of 16 prompts.
+template <int D, bool E4M3>
+__device__ __noinline__ void append_gapped(const AppendArgs& a, const long long* slots, int window, int span, int item0, int item1) {
+  constexpr int LPR = D / 8, RPW = 32 / LPR;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LPR;
+  const int bs = a.block_size;
+  const long long first = (long long)blockIdx.x * a.window;
+  auto page_of = [&](long long slot) { return (long long)__umul64hi((unsigned long long)slot, a.block_magic); };
+  auto follows = [&](int i) { return slots[i - 1] >= page_of(slots[i]) * bs && slots[i - 1] < slots[i] && slots[i - 1] >= 0; };
+  int turn = 0;
+#pragma unroll 1
+  for (int i0 = 0, n; i0 < window; i0 += n) {
+    n = 1;
+    const long long page = page_of(slots[i0]);
+    if (slots[i0] < 0 || page >= a.blocks || follows(i0)) continue;
+    while (i0 + n < span && follows(i0 + n)) ++n;
+    const int row0 = (int)(slots[i0] - page * bs);
+#pragma unroll 1
+    for (int item = item0; item < item1; ++item) {
+      if (turn++ % kAppendWarps != warp) continue;
+      const long long xs = a.x_token_stride[item & 1], ps = a.row_stride[item & 1];
+      const uint16_t* x = a.x[item & 1] + (item >> 1) * a.x_head_stride[item & 1] + lane % LPR * 8 + (first + i0) * xs;
+      uint8_t* pool = a.pool[item & 1] + page * a.block_stride[item & 1] + (item >> 1) * a.head_stride[item & 1];
+      float* scale = a.scale[item & 1] + page * a.kv_heads + (item >> 1);
+      const float old = row0 > 0 ? *scale : 0.f;
+      uint32_t top = 0;
+#pragma unroll 1
+      for (int i = sub; i < n; i += RPW) top = add_largest_finite(top, *reinterpret_cast<const uint4*>(x + i * xs), a.bf16 ? 0x7f80u : 0x7c00u);
+      top = __reduce_max_sync(0xffffffffu, top);
+      const float now = scale_of<E4M3>(old, top, a.bf16), by = __frcp_rn(now);
+#pragma unroll 1
+      for (int i = sub; i < n; i += RPW)
+        *reinterpret_cast<uint2*>(pool + (slots[i0 + i] - page * bs) * ps + lane % LPR * 8) =
+            encode8<E4M3>(*reinterpret_cast<const uint4*>(x + i * xs), a.bf16, by, true);
+      if (now > old) {
+        if (lane == 0) *scale = now;
+        if (row0 > 0) rows_again<D, E4M3>(pool, ps, row0, __fdiv_rn(old, now), 0, 1);
+      }
+    }
+  }
+}
+
 template <int D, bool E4M3>
 __global__ void __launch_bounds__(kAppendWarps * 32, D == 64 ? 6 : 5) k_cache_append(const __grid_constant__ AppendArgs a) {
-  constexpr float Q = E4M3 ? 448.f : 127.f;
   constexpr int LPR = D / 8;     // lanes of a row
   constexpr int RPW = 32 / LPR;  // rows of a warp's load
   constexpr int kStep = kAppendWarps * RPW;         // rows of the CTA's load
@@ -433,56 +499,11 @@ __global__ void __launch_bounds__(kAppendWarps * 32, D == 64 ? 6 : 5) k_cache_ap
     }
     return span;
   };
-  auto again = [&](uint8_t* rows, long long ps, int n, float ratio, int w, int warps) {
-    constexpr int LR = D / 16, RW = 32 / LR;  // 16 codes a lane
-#pragma unroll 4
-    for (int i = w * RW + lane / LR; i < n; i += warps * RW) {
-      uint4* p = reinterpret_cast<uint4*>(rows + i * ps + lane % LR * 16);
-      const uint4 c = *p;
-      *p = make_uint4(code_again<E4M3>(c.x, ratio), code_again<E4M3>(c.y, ratio), code_again<E4M3>(c.z, ratio), code_again<E4M3>(c.w, ratio));
-    }
-  };
+  auto again = [&](uint8_t* rows, long long ps, int n, float ratio, int w, int warps) { rows_again<D, E4M3>(rows, ps, n, ratio, w, warps); };
   const uint32_t infinite = a.bf16 ? 0x7f80u : 0x7c00u;
-  auto value = [&](uint32_t pattern) {
-    return a.bf16 ? __uint_as_float(pattern << 16) : __half2float(__ushort_as_half((unsigned short)pattern));
-  };
-  auto scale_for = [&](float old, uint32_t top) { return fmaxf(old, __fdiv_rn(fmaxf(value(top), kLeastAmax), Q)); };
-  // Rows of a page that rise with gaps between them (nothing that cache_plan
-  // makes): a warp takes a page's tokens, reads them twice and places each.  Rows
-  // in the gaps keep what they hold.
+  auto scale_for = [&](float old, uint32_t top) { return scale_of<E4M3>(old, top, a.bf16); };
   if (s_gaps) {
-    auto follows = [&](int i) { return s_slot[i] >= page_of(s_slot[i + 1]) * bs && s_slot[i] < s_slot[i + 1] && s_slot[i] >= 0; };
-    int turn = 0;
-#pragma unroll 1
-    for (int i0 = 0, n; i0 < min(span, a.window); i0 += n) {
-      n = 1;
-      const long long slot = s_slot[i0 + 1], page = page_of(slot);
-      if (slot < 0 || page >= a.blocks || follows(i0)) continue;
-      while (i0 + n < span && follows(i0 + n)) ++n;
-      const int row0 = (int)(slot - page * bs);
-#pragma unroll 1
-      for (int item = item0; item < item1; ++item) {
-        if (turn++ % kAppendWarps != warp) continue;
-        const long long xs = a.x_token_stride[item & 1], ps = a.row_stride[item & 1];
-        const uint16_t* x = rows_of(item) + (first + i0) * xs;
-        uint8_t* pool = a.pool[item & 1] + page * a.block_stride[item & 1] + (item >> 1) * a.head_stride[item & 1];
-        float* scale = a.scale[item & 1] + page * a.kv_heads + (item >> 1);
-        const float old = row0 > 0 ? *scale : 0.f;
-        uint32_t top = 0;
-#pragma unroll 1
-        for (int i = sub; i < n; i += RPW) top = add_largest_finite(top, *reinterpret_cast<const uint4*>(x + i * xs), infinite);
-        top = __reduce_max_sync(0xffffffffu, top);
-        const float now = scale_for(old, top), by = __frcp_rn(now);
-#pragma unroll 1
-        for (int i = sub; i < n; i += RPW)
-          *reinterpret_cast<uint2*>(pool + (s_slot[i0 + 1 + i] - page * bs) * ps + lane % LPR * 8) =
-              encode8<E4M3>(*reinterpret_cast<const uint4*>(x + i * xs), a.bf16, by, true);
-        if (now > old) {
-          if (lane == 0) *scale = now;
-          if (row0 > 0) again(pool, ps, row0, __fdiv_rn(old, now), 0, 1);
-        }
-      }
-    }
+    append_gapped<D, E4M3>(a, s_slot + 1, min(span, a.window), span, item0, item1);
     return;
   }
   int turn = 0, big = 0;
