@@ -19,9 +19,10 @@
 // head; beyond, the matrix instructions.  A tile of 16 tokens and 8 query rows
 // takes 16 m16n8k16 instructions for heads of 128, in which the tokens (then
 // the channels) are the 16 rows and the query rows the 8 columns, so no row is
-// padding when 8 query heads share a KV head.  (tcgen05 works on 128 rows: with
-// 8 it would spend 16 times the operations, and the tokens' codes would have to
-// go to shared memory once more, as fp16.)
+// padding when 8 query heads share a KV head.  (tcgen05 would take the same
+// arrangement, 128 tokens by 16 to 256 query rows, but with the codes converted
+// and stored to shared or tensor memory once more, as fp16; for the rows past 16
+// that is not measured.)
 //   K: lane (g, c) takes tokens g and g + 8, channels 32c..32c+31: word s of a
 //      row is its part of the s-th k step (the sum over channels may run in any
 //      order, so q is loaded in the same one).
@@ -46,11 +47,11 @@
 //
 // Measured on one B200 (6550 GB/s copied): four contexts of 131 thousand tokens,
 // 64 query heads over 8 of 128, e4m3: 167 us, 6.2 TB/s; 32 requests of 0 to 8192
-// tokens, 32 over 8 heads, int8: 55 us, 5.0 TB/s, of which 40 us stream and the
+// tokens, 32 over 8 heads, int8: 56 us, 5.0 TB/s, of which 40 us stream and the
 // rest is the call's start, the slowest warps and the joins; 200 requests of up
-// to 1900 tokens, a window of 1000, 12 heads of 64, e4m3: 51 us, 4.5 TB/s; 17
-// requests of five queries (20 rows a KV head), 0.8 to 4 thousand tokens: 35 us;
-// one request of 700 tokens 10.6 us.
+// to 1900 tokens, a window of 1000, 12 heads of 64, e4m3: 52 us, 4.4 TB/s; 17
+// requests of five queries (20 rows a KV head), 0.8 to 4 thousand tokens: 36 us;
+// one request of 700 tokens 11.1 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -1112,13 +1113,14 @@ __global__ void __launch_bounds__(W * 32, MINB) k_attend(const __grid_constant__
 
 // Warps of a CTA, stages of a warp's ring, CTAs of an SM and tiles of a unit for
 // each head size and number of row tiles, as the registers allow (q D/8 and o
-// D/4 for each row tile) and as measured:
+// D/4 for each row tile) and as measured, each against its alternative:
 //   128, one row tile: 16 warps with 2 stages 167 us for the longest case above,
 //     with 3 stages 175, one CTA of 16 warps 167 (but 15.7 instead of 13.4 for
 //     four requests of 3000 tokens), four CTAs of 4 172
-//   64, one row tile: two tiles of tokens side by side 51 us for the window case,
+//   64, one row tile: two tiles of tokens side by side 52 us for the window case,
 //     one 58 to 61
-//   more row tiles: one CTA of 8 warps (drafts 44 us, two of 4 47.6 at that time)
+//   more row tiles: one CTA of 8 warps (drafts 44 us, two of 4 47.6, when both
+//     were slower)
 constexpr int unit_tiles(int head_dim) { return head_dim == 64 ? 2 : 1; }
 template <int D, int NT>
 struct Shape;

@@ -6,7 +6,7 @@
 // there, and r' and h are written: the floor's bytes and no others.  A norm by
 // mean and variance takes the mean first and then the squares about it, which
 // costs one more reduction and no accuracy.  Many rows are bound by HBM (8192 x
-// 8192, both norms and a full gate: 117 to 122 us, 5.6 TB/s), one by the
+// 8192, both norms and a full gate: 122 us, 5.5 TB/s), one by the
 // latency of a load, the reductions and a store (3.1 us on the GPU, 7.0 us a
 // call through Python).
 #include <cuda_bf16.h>

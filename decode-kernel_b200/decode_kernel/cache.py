@@ -108,7 +108,8 @@ def cache_plan(held: torch.Tensor, fresh: torch.Tensor, block_table: torch.Tenso
     pages were missing and how many requests were too wide.
 
     ``out`` reuses tensors of an earlier plan; its ``lengths`` may be ``held``
-    and its ``ring`` may be ``ring``.
+    and its ``ring`` may be ``ring`` (the call then runs on one SM, which steps
+    of many thousand tokens feel).
     """
     if out is None:
         return CachePlan(*_extension().cache_plan(held, fresh, block_table, free_blocks, ring, block_size, tokens))
