@@ -26,6 +26,7 @@
 #include <string>
 #include <tuple>
 #include <utility>
+#include <vector>
 
 #include "dk_w4a16.h"
 
@@ -582,6 +583,298 @@ std::tuple<torch::Tensor, OptTensor> block_norm(torch::Tensor residual, OptTenso
   return {out, result};
 }
 
+// ---------------------------------------------------------------------------
+// A prompt's step: products of many rows, their gradients, rotary positions, the
+// cache read back.
+// ---------------------------------------------------------------------------
+// Rows of `width` values of a tensor of any shape: a 2-D one whose rows the
+// kernels can read where they lie, else a copy of it (its rows a multiple of 8
+// values apart).
+torch::Tensor in_rows(const torch::Tensor& t, int64_t width) {
+  const int64_t rows = t.numel() / std::max<int64_t>(width, 1);
+  torch::Tensor r = t.dim() == 2 ? t : t.reshape({rows, width});
+  if (aligned16(r) && (width == 1 || r.stride(1) == 1) && (rows <= 1 || (r.stride(0) % 8 == 0 && r.stride(0) >= width))) return r;
+  const torch::Tensor home = torch::empty({rows, (width + 7) / 8 * 8}, t.options()).narrow(1, 0, width);
+  home.copy_(r);
+  return home;
+}
+
+int64_t row_stride(const torch::Tensor& r) { return r.size(0) > 1 ? r.stride(0) : (r.size(1) + 7) / 8 * 8; }
+
+// A pair of weights, checked; re-homed where it does not begin on 16 bytes.
+struct Weights {
+  torch::Tensor packed, scales;
+  int64_t M, K;
+
+  Weights(const torch::Tensor& p, const torch::Tensor& s, const torch::Tensor& x) : packed(p), scales(s) {
+    TORCH_CHECK(p.is_cuda() && s.is_cuda() && x.is_cuda(), "packed, scales, and x must be CUDA tensors");
+    TORCH_CHECK(p.scalar_type() == torch::kInt32, "packed must be int32 (uint32 bit pattern)");
+    TORCH_CHECK(s.scalar_type() == torch::kFloat16, "scales must be fp16");
+    TORCH_CHECK(p.dim() == 2 && s.dim() == 2, "packed [M,K/8], scales [M,K/128]");
+    TORCH_CHECK(p.is_contiguous() && s.is_contiguous(), "packed and scales must be contiguous");
+    TORCH_CHECK(p.device() == x.device() && s.device() == x.device(), "packed, scales, and x must be on the same device");
+    M = p.size(0);
+    K = p.size(1) * DK_NIBBLES_PER_WORD;
+    TORCH_CHECK(K >= DK_GROUP_SIZE && K % DK_GROUP_SIZE == 0, "K must be divisible by group size 128");
+    TORCH_CHECK(s.size(0) == M && s.size(1) == K / DK_GROUP_SIZE, "scales shape must be [M, K/128]");
+    TORCH_CHECK(M <= INT32_MAX && K <= INT32_MAX, "dimensions must fit in int32");
+    if (!aligned16(packed)) packed = packed.clone();
+  }
+  const int32_t* words() const { return packed.data_ptr<int32_t>(); }
+  const uint16_t* factors() const { return reinterpret_cast<const uint16_t*>(scales.data_ptr<at::Half>()); }
+};
+
+// x of [..., width]: its other dimensions, with `last` behind them.
+std::vector<int64_t> shape_with(const torch::Tensor& x, int64_t last) {
+  std::vector<int64_t> shape = x.sizes().vec();
+  shape.back() = last;
+  return shape;
+}
+
+void check_rows(const torch::Tensor& x, int64_t width, const char* what) {
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) == width, what, " must be [..., " + std::to_string(width) + "]");
+  TORCH_CHECK(x.numel() / std::max<int64_t>(width, 1) <= INT32_MAX, what, " has too many rows");
+}
+
+dk_mlp_act mlp_act(int act) {
+  TORCH_CHECK(act == DK_MLP_SILU || act == DK_MLP_GELU, "unknown activation");
+  return static_cast<dk_mlp_act>(act);
+}
+
+// An output given by the caller: contiguous rows of any stride, or a new one.
+torch::Tensor output(const OptTensor& out, const std::vector<int64_t>& shape, const torch::Tensor& x) {
+  if (!out) return torch::empty(shape, x.options());
+  TORCH_CHECK(out->device() == x.device() && out->scalar_type() == x.scalar_type() && out->sizes() == c10::IntArrayRef(shape),
+              "out must have the product's shape and x's type and device");
+  TORCH_CHECK(out->is_contiguous() || (out->dim() == 2 && out->stride(1) == 1 && out->stride(0) >= out->size(1)),
+              "out must have contiguous rows");
+  return *out;
+}
+
+std::tuple<torch::Tensor, OptTensor, OptTensor> w4a16_gemm(torch::Tensor packed, torch::Tensor scales, OptTensor packed2,
+                                                           OptTensor scales2, torch::Tensor x, int act, bool keep,
+                                                           OptTensor out) {
+  const Weights w(packed, scales, x);
+  dk_gemm_args a{};
+  a.dtype = half_type(x, "x");
+  a.act = mlp_act(act);
+  check_rows(x, w.K, "x");
+  const c10::cuda::CUDAGuard guard(x.device());
+  std::optional<Weights> w2;
+  if (packed2) {
+    w2.emplace(*packed2, *scales2, x);
+    TORCH_CHECK(w2->M == w.M && w2->K == w.K, "gate and up must have the same shape");
+    a.packed2 = w2->words();
+    a.scales2 = w2->factors();
+  }
+  const torch::Tensor xr = in_rows(x, w.K);
+  const std::vector<int64_t> shape = shape_with(x, w.M);
+  torch::Tensor y = output(out, shape, x);
+  OptTensor g, u;
+  if (keep) {  // kept for the gradient, whose product wants rows a multiple of 8 apart
+    const int64_t wide = (w.M + 7) / 8 * 8;
+    const torch::Tensor whole = torch::empty({2, xr.size(0), wide}, x.options());
+    g = whole[0].narrow(1, 0, w.M);
+    u = whole[1].narrow(1, 0, w.M);
+    a.gate_out = g->data_ptr();
+    a.up_out = u->data_ptr();
+    a.ldk = wide;
+  }
+  a.packed = w.words();
+  a.scales = w.factors();
+  a.x = xr.data_ptr();
+  a.ldx = row_stride(xr);
+  a.y = y.data_ptr();
+  a.ldy = y.dim() == 2 && y.size(0) > 1 ? y.stride(0) : w.M;
+  a.rows = static_cast<int>(xr.size(0));
+  a.M = static_cast<int>(w.M);
+  a.K = static_cast<int>(w.K);
+  check_status(dk_w4a16_gemm(&a, at::cuda::getCurrentCUDAStream().stream()), "w4a16_gemm");
+  return {y, g, u};
+}
+
+torch::Tensor w4a16_gemm_t(torch::Tensor packed, torch::Tensor scales, OptTensor packed2, OptTensor scales2,
+                           torch::Tensor g, OptTensor g2, OptTensor out) {
+  const Weights w(packed, scales, g);
+  dk_gemm_t_args a{};
+  a.dtype = half_type(g, "g");
+  check_rows(g, w.M, "g");
+  const c10::cuda::CUDAGuard guard(g.device());
+  if (w.M == 0) return output(out, shape_with(g, w.K), g).zero_();
+  torch::Tensor gr = in_rows(g, w.M), gr2;
+  std::optional<Weights> w2;
+  if (packed2) {
+    w2.emplace(*packed2, *scales2, g);
+    TORCH_CHECK(w2->M == w.M && w2->K == w.K, "gate and up must have the same shape");
+    TORCH_CHECK(g2 && g2->sizes() == g.sizes() && g2->scalar_type() == g.scalar_type() && g2->device() == g.device(),
+                "g2 must have g's shape, type and device");
+    gr2 = in_rows(*g2, w.M);
+    if (row_stride(gr2) != row_stride(gr)) {
+      gr = in_rows(gr.contiguous(), w.M);
+      gr2 = in_rows(gr2.contiguous(), w.M);
+    }
+    a.packed2 = w2->words();
+    a.scales2 = w2->factors();
+    a.g2 = gr2.data_ptr();
+  }
+  torch::Tensor dx = output(out, shape_with(g, w.K), g);
+  a.packed = w.words();
+  a.scales = w.factors();
+  a.g = gr.data_ptr();
+  a.ldg = row_stride(gr);
+  a.dx = dx.data_ptr();
+  a.lddx = dx.dim() == 2 && dx.size(0) > 1 ? dx.stride(0) : w.K;
+  a.rows = static_cast<int>(gr.size(0));
+  a.M = static_cast<int>(w.M);
+  a.K = static_cast<int>(w.K);
+  check_status(dk_w4a16_gemm_t(&a, at::cuda::getCurrentCUDAStream().stream()), "w4a16_gemm_t");
+  return dx;
+}
+
+std::tuple<torch::Tensor, torch::Tensor> gated_grad(torch::Tensor dh, torch::Tensor g, torch::Tensor u, int act) {
+  TORCH_CHECK(dh.is_cuda() && g.is_cuda() && u.is_cuda() && g.device() == dh.device() && u.device() == dh.device(),
+              "dh, g and u must be CUDA tensors of one device");
+  const dk_dtype type = half_type(dh, "dh");
+  TORCH_CHECK(g.dim() == 2 && u.sizes() == g.sizes() && g.scalar_type() == dh.scalar_type() &&
+                  u.scalar_type() == dh.scalar_type() && dh.numel() == g.numel(),
+              "g and u must be [rows, M] with dh's type");
+  TORCH_CHECK(g.stride(1) == 1 && u.strides() == g.strides(), "g and u must have contiguous rows and the same strides");
+  const int64_t rows = g.size(0), M = g.size(1);
+  TORCH_CHECK(rows <= INT32_MAX && M <= INT32_MAX, "dimensions must fit in int32");
+  const c10::cuda::CUDAGuard guard(dh.device());
+  const torch::Tensor d = in_rows(dh, M);
+  const int64_t wide = (M + 7) / 8 * 8;
+  const torch::Tensor whole = torch::empty({2, rows, wide}, dh.options());
+  const torch::Tensor dg = whole[0].narrow(1, 0, M), du = whole[1].narrow(1, 0, M);
+  check_status(dk_gated_grad(d.data_ptr(), g.data_ptr(), u.data_ptr(), dg.data_ptr(), du.data_ptr(), static_cast<int>(rows),
+                             static_cast<int>(M), row_stride(d), row_stride(g), wide, type, mlp_act(act),
+                             at::cuda::getCurrentCUDAStream().stream()),
+               "gated_grad");
+  return {dg, du};
+}
+
+std::tuple<torch::Tensor, OptTensor> rotary(torch::Tensor q, OptTensor k, torch::Tensor positions, torch::Tensor frequency,
+                                            std::optional<std::vector<int64_t>> sections, bool paired, bool inverse,
+                                            bool inplace) {
+  TORCH_CHECK(q.is_cuda(), "q must be a CUDA tensor");
+  TORCH_CHECK(q.dim() == 3, "q must be [tokens, q_heads, head_dim]");
+  const torch::Device device = q.device();
+  const int64_t tokens = q.size(0), dim = q.size(2);
+  TORCH_CHECK(q.scalar_type() == torch::kFloat16 || q.scalar_type() == torch::kBFloat16 || q.scalar_type() == torch::kFloat32,
+              "q must be fp16, bf16 or fp32");
+  TORCH_CHECK(tokens <= INT32_MAX && q.size(1) >= 1 && q.size(1) < (1 << 20), "q must have 1 to 2^20 heads and less than 2^31 tokens");
+  TORCH_CHECK(dim >= 2 && dim <= DK_ROTARY_MAX_DIM, "head_dim must be 2 to " + std::to_string(DK_ROTARY_MAX_DIM));
+  if (k) {
+    TORCH_CHECK(k->is_cuda() && k->device() == device && k->scalar_type() == q.scalar_type(), "k must have q's type and device");
+    TORCH_CHECK(k->dim() == 3 && k->size(0) == tokens && k->size(2) == dim && k->size(1) >= 1 && k->size(1) < (1 << 20),
+                "k must be [tokens, kv_heads, head_dim]");
+  }
+  TORCH_CHECK(frequency.is_cuda() && frequency.device() == device && frequency.scalar_type() == torch::kFloat32 &&
+                  frequency.dim() == 1 && frequency.is_contiguous(),
+              "frequency must be contiguous fp32 [pairs] on q's device");
+  const int64_t pairs = frequency.size(0);
+  TORCH_CHECK(pairs >= 1 && 2 * pairs <= dim, "frequency must have 1 to head_dim / 2 values");
+  TORCH_CHECK(positions.is_cuda() && positions.device() == device, "positions must be on q's device");
+  TORCH_CHECK(positions.scalar_type() == torch::kInt32 || positions.scalar_type() == torch::kInt64, "positions must be int32 or int64");
+  TORCH_CHECK((positions.dim() == 1 || positions.dim() == 2) && positions.size(-1) == tokens,
+              "positions must be [tokens] or [axes, tokens]");
+  dk_rotary_args a{};
+  const int64_t axes = positions.dim() == 2 ? positions.size(0) : 1;
+  TORCH_CHECK(axes >= 1 && axes <= DK_ROTARY_MAX_AXES, "positions must have 1 to " + std::to_string(DK_ROTARY_MAX_AXES) + " axes");
+  TORCH_CHECK(sections || axes == 1, "several axes need sections");
+  if (sections) {
+    TORCH_CHECK(static_cast<int64_t>(sections->size()) == axes, "sections must have a number of pairs for each axis");
+    int64_t end = 0;
+    for (int64_t i = 0; i < axes; ++i) {
+      TORCH_CHECK((*sections)[i] >= 0 && (*sections)[i] <= pairs, "sections must be numbers of pairs");
+      a.section_end[i] = static_cast<int>(end += (*sections)[i]);
+    }
+    TORCH_CHECK(end == pairs, "sections must add up to frequency's length");
+  } else {
+    a.section_end[0] = static_cast<int>(pairs);
+  }
+  const c10::cuda::CUDAGuard guard(device);
+  const torch::Tensor at = positions.stride(-1) == 1 || tokens <= 1 ? positions : positions.contiguous();
+  auto place = [&](const torch::Tensor& t, const void*& in, void*& out, int64_t& it, int64_t& ih, int64_t& ot, int64_t& oh) {
+    if (inplace) {
+      TORCH_CHECK(t.stride(2) == 1, "q and k that are turned in place must have contiguous heads");
+      for (int64_t i = 0; i < 2; ++i)
+        TORCH_CHECK(t.size(i) == 1 || t.stride(i) >= dim, "q and k that are turned in place may not overlap themselves");
+      TORCH_CHECK(t.size(0) <= 1 || t.size(1) == 1 || t.stride(0) >= t.size(1) * t.stride(1) || t.stride(1) >= t.size(0) * t.stride(0),
+                  "q and k that are turned in place may not overlap themselves");
+    }
+    const torch::Tensor from = t.stride(2) == 1 ? t : t.contiguous();
+    const torch::Tensor to = inplace ? t : torch::empty(t.sizes(), t.options());
+    in = from.data_ptr();
+    out = to.data_ptr();
+    it = from.stride(0), ih = from.stride(1), ot = to.stride(0), oh = to.stride(1);
+    return std::make_pair(from, to);
+  };
+  const auto qs = place(q, a.q, a.q_out, a.q_token_stride, a.q_head_stride, a.q_out_token_stride, a.q_out_head_stride);
+  std::pair<torch::Tensor, torch::Tensor> ks;
+  if (k) {
+    ks = place(*k, a.k, a.k_out, a.k_token_stride, a.k_head_stride, a.k_out_token_stride, a.k_out_head_stride);
+    TORCH_CHECK(!inplace || k->data_ptr() != q.data_ptr() || tokens == 0, "q and k that are turned in place must be two tensors");
+    a.kv_heads = static_cast<int>(k->size(1));
+  }
+  a.positions = at.data_ptr();
+  a.positions_64 = at.scalar_type() == torch::kInt64;
+  a.position_stride = at.dim() == 2 ? at.stride(0) : 0;
+  a.frequency = frequency.data_ptr<float>();
+  a.tokens = static_cast<int>(tokens);
+  a.q_heads = static_cast<int>(q.size(1));
+  a.head_dim = static_cast<int>(dim);
+  a.pairs = static_cast<int>(pairs);
+  a.axes = static_cast<int>(axes);
+  a.paired = paired;
+  a.inverse = inverse;
+  a.dtype = q.scalar_type() == torch::kFloat32 ? DK_FP32 : half_type(q, "q");
+  check_status(dk_rotary(&a, at::cuda::getCurrentCUDAStream().stream()), "rotary");
+  return {qs.second, k ? OptTensor(ks.second) : OptTensor()};
+}
+
+std::tuple<torch::Tensor, torch::Tensor> cache_read(const Cache8& cache, torch::Tensor block_table, torch::Tensor lengths,
+                                                    torch::Tensor starts, int64_t tokens, torch::ScalarType type, OptTensor k,
+                                                    OptTensor v) {
+  const torch::Device device = cache.k.device();
+  TORCH_CHECK(lengths.dim() == 1, "lengths must be [requests]");
+  const int64_t n = lengths.size(0);
+  TORCH_CHECK(n <= INT32_MAX - 1, "too many requests");
+  TORCH_CHECK(tokens >= 0 && tokens <= INT32_MAX, "tokens out of range");
+  check_ints(lengths, torch::kInt32, n, device, "lengths");
+  check_ints(starts, torch::kInt32, n + 1, device, "starts");
+  check_table(block_table, n, device);
+  TORCH_CHECK(type == torch::kFloat16 || type == torch::kBFloat16, "dtype must be fp16 or bf16");
+  const c10::cuda::CUDAGuard guard(device);
+  const std::vector<int64_t> shape = {tokens, cache.c.kv_heads, cache.c.head_dim};
+  auto given = [&](const OptTensor& t, const char* what) {
+    if (!t) return torch::empty(shape, cache.k.options().dtype(type));
+    TORCH_CHECK(t->is_cuda() && t->device() == device && t->scalar_type() == type && t->sizes() == c10::IntArrayRef(shape),
+                what, " must be [tokens, kv_heads, head_dim] of dtype on the cache's device");
+    TORCH_CHECK(t->stride(2) == 1 && (t->size(1) == 1 || t->stride(1) == t->size(2)) &&
+                    (tokens <= 1 || (t->stride(0) % 8 == 0 && t->stride(0) >= t->size(1) * t->size(2))) && aligned16(*t),
+                what, " must have contiguous rows, a multiple of 8 values apart and 16-byte aligned");
+    return *t;
+  };
+  const torch::Tensor ko = given(k, "k"), vo = given(v, "v");
+  dk_cache_read_args a{};
+  a.cache = cache.c;
+  a.block_table = block_table.data_ptr<int32_t>();
+  a.max_blocks = static_cast<int>(block_table.size(1));
+  a.table_stride = static_cast<int>(n > 1 ? block_table.stride(0) : block_table.size(1));
+  a.lengths = lengths.data_ptr<int32_t>();
+  a.starts = starts.data_ptr<int32_t>();
+  a.requests = static_cast<int>(n);
+  a.tokens = static_cast<int>(tokens);
+  a.k = ko.data_ptr();
+  a.v = vo.data_ptr();
+  a.k_token_stride = tokens > 1 ? ko.stride(0) : 0;
+  a.v_token_stride = tokens > 1 ? vo.stride(0) : 0;
+  a.dtype = type == torch::kFloat16 ? DK_FP16 : DK_BF16;
+  check_status(dk_cache_read(&a, at::cuda::getCurrentCUDAStream().stream()), "cache_read");
+  return {ko, vo};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -629,5 +922,17 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("post_bias"), py::arg("gate"), py::arg("act"), py::arg("residual_scale"),
         py::arg("block_scale"), py::arg("pre_weight"), py::arg("pre_bias"), py::arg("eps"),
         py::arg("inplace"));
+  m.def("w4a16_gemm", &w4a16_gemm, "Many rows through 4-bit weights, or through a gated pair", py::arg("packed"),
+        py::arg("scales"), py::arg("packed2"), py::arg("scales2"), py::arg("x"), py::arg("act") = 0, py::arg("keep") = false,
+        py::arg("out") = py::none());
+  m.def("w4a16_gemm_t", &w4a16_gemm_t, "The transposed product", py::arg("packed"), py::arg("scales"), py::arg("packed2"),
+        py::arg("scales2"), py::arg("g"), py::arg("g2") = py::none(), py::arg("out") = py::none());
+  m.def("gated_grad", &gated_grad, "Gradients of a gated block's pre-activations", py::arg("dh"), py::arg("g"), py::arg("u"),
+        py::arg("act"));
+  m.def("rotary", &rotary, "Rotary positions of queries and keys", py::arg("q"), py::arg("k"), py::arg("positions"),
+        py::arg("frequency"), py::arg("sections"), py::arg("paired"), py::arg("inverse"), py::arg("inplace"));
+  m.def("cache_read", &cache_read, "Keys and values of a paged 8-bit cache as rows", py::arg("cache"), py::arg("block_table"),
+        py::arg("lengths"), py::arg("starts"), py::arg("tokens"), py::arg("dtype"), py::arg("k") = py::none(),
+        py::arg("v") = py::none());
   m.def("version", []() { return std::string(dk_version()); });
 }

@@ -7,8 +7,10 @@ repository's CUDA library (``libdk_b200.so``, C ABI in include/dk_w4a16.h)
 through the torch extension ``decode_kernel._cuda``.
 
 The rest of a decode step stands beside the products: a paged cache in 8 bits
-(``PagedCache8``, ``cache_plan``, ``cache_append``, ``cache_attention``) and the
-norms between blocks (``block_norm``).
+(``PagedCache8``, ``cache_plan``, ``cache_append``, ``cache_attention``,
+``cache_read``), rotary positions (``rotary``) and the norms between blocks
+(``block_norm``).  Prompts take the products of many rows (``gemm``,
+``gemm_gated``), which carry gradients through the frozen weights (``gemm_t``).
 
 There is no CPU fallback: when the extension or a GPU is missing these
 functions raise.
@@ -20,28 +22,36 @@ from typing import Optional
 
 import torch
 
-from .cache import CachePlan, PagedCache8, cache_append, cache_attention, cache_plan, release_workspaces
+from .cache import CachePlan, PagedCache8, cache_append, cache_attention, cache_plan, cache_read, release_workspaces
+from .gemm import gemm, gemm_gated, gemm_t
 from .norm import block_norm
 from .quantize import GROUP_SIZE, dequantize, quantize_and_pack, quantize_and_pack_cuda
+from .rotary import rotary
 
 __all__ = [
     "CachePlan",
     "GROUP_SIZE",
     "PagedCache8",
+    "W4A16GatedMLP",
     "W4A16Linear",
     "block_norm",
     "cache_append",
     "cache_attention",
     "cache_plan",
+    "cache_read",
     "cuda_available",
     "gemv_multi",
     "gemv_silu_mul",
     "dequantize",
+    "gemm",
+    "gemm_gated",
+    "gemm_t",
     "gemv",
     "gemv_out",
     "quantize_and_pack",
     "quantize_and_pack_cuda",
     "release_workspaces",
+    "rotary",
     "w4a16_linear",
 ]
 
@@ -215,4 +225,4 @@ def w4a16_linear(
     )
 
 
-from .ops import W4A16Linear  # noqa: E402  (registers torch.ops.decode_kernel.w4a16_linear)
+from .ops import W4A16GatedMLP, W4A16Linear  # noqa: E402  (registers torch.ops.decode_kernel.w4a16_linear)

@@ -4,7 +4,8 @@
 tables, slot maps and lengths on the GPU from the requests' lengths;
 ``cache_append`` quantises the step's keys and values into their pages (one
 fp32 scale per page and KV head, int8 or float8_e4m3fn codes);
-``cache_attention`` attends over the pages.  Nothing waits for the GPU, so a
+``cache_attention`` attends over the pages; ``cache_read`` gives them back as
+rows of keys and values.  Nothing waits for the GPU, so a
 whole step can be captured in a CUDA graph.  There is no CPU fallback.
 """
 
@@ -14,7 +15,7 @@ from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
 
-__all__ = ["CachePlan", "PagedCache8", "cache_append", "cache_attention", "cache_plan", "release_workspaces"]
+__all__ = ["CachePlan", "PagedCache8", "cache_append", "cache_attention", "cache_plan", "cache_read", "release_workspaces"]
 
 _module = None
 
@@ -157,6 +158,25 @@ def cache_attention(q: torch.Tensor, cache: PagedCache8, block_table: torch.Tens
     """
     o, l = _extension().cache_attention(q, cache._handle, block_table, lengths, starts, scale, causal, window, out, lse)
     return (o, l) if lse else o
+
+
+def cache_read(cache: PagedCache8, block_table: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor,
+               tokens: int, *, dtype: torch.dtype = torch.float16,
+               out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The cache's keys and values as rows: (k, v), fp16 or bf16 [tokens, kv_heads, head_dim].
+
+    Request r's rows are ``starts[r]:starts[r + 1]`` and the last of its
+    ``lengths[r]`` tokens, as ``cache_attention`` takes its queries; with
+    ``starts`` the running sum of ``lengths`` they are all of them.  ``tokens``
+    is the number of rows, padding included.  A value is its code times its
+    page's and head's scale in fp32, rounded once (past fp16's range to
+    infinity).  Rows without a token (more rows than tokens, table entries
+    outside the pool) are zeros; rows from ``starts[-1]`` on are not written.
+
+    ``out``: (k, v) of an earlier call, or views with contiguous rows a multiple
+    of 8 values apart.
+    """
+    return _extension().cache_read(cache._handle, block_table, lengths, starts, tokens, dtype, *(out or (None, None)))
 
 
 def release_workspaces() -> None:

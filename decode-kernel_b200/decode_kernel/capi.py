@@ -122,6 +122,61 @@ class BlockNormArgs(ctypes.Structure):
                     (name, ctypes.c_float) for name in ("residual_scale", "block_scale", "eps")]
 
 
+class GemmArgs(ctypes.Structure):
+    """struct dk_gemm_args."""
+
+    _fields_ = [(name, ctypes.c_void_p) for name in (
+        "packed", "scales", "packed2", "scales2", "x", "y", "gate_out", "up_out")] + [
+            (name, ctypes.c_int64) for name in ("ldx", "ldy", "ldk")] + [
+                (name, ctypes.c_int) for name in ("rows", "M", "K", "dtype", "act")]
+
+
+class GemmTArgs(ctypes.Structure):
+    """struct dk_gemm_t_args."""
+
+    _fields_ = [(name, ctypes.c_void_p) for name in (
+        "packed", "scales", "packed2", "scales2", "g", "g2", "dx")] + [
+            (name, ctypes.c_int64) for name in ("ldg", "lddx")] + [
+                (name, ctypes.c_int) for name in ("rows", "M", "K", "dtype")]
+
+
+DK_ROTARY_MAX_AXES = 4
+
+
+class RotaryArgs(ctypes.Structure):
+    """struct dk_rotary_args."""
+
+    _fields_ = [(name, ctypes.c_void_p) for name in ("q", "k", "q_out", "k_out")] + [
+        (name, ctypes.c_int64) for name in (
+            "q_token_stride", "q_head_stride", "k_token_stride", "k_head_stride",
+            "q_out_token_stride", "q_out_head_stride", "k_out_token_stride", "k_out_head_stride")] + [
+                ("positions", ctypes.c_void_p), ("frequency", ctypes.c_void_p), ("position_stride", ctypes.c_int64)] + [
+                    (name, ctypes.c_int) for name in (
+                        "positions_64", "tokens", "q_heads", "kv_heads", "head_dim", "pairs", "axes")] + [
+                            ("section_end", ctypes.c_int * DK_ROTARY_MAX_AXES)] + [
+                                (name, ctypes.c_int) for name in ("paired", "inverse", "dtype")]
+
+
+class CacheReadArgs(ctypes.Structure):
+    """struct dk_cache_read_args."""
+
+    _fields_ = [
+        ("cache", Cache8),
+        ("block_table", ctypes.c_void_p),
+        ("max_blocks", ctypes.c_int),
+        ("table_stride", ctypes.c_int),
+        ("lengths", ctypes.c_void_p),
+        ("starts", ctypes.c_void_p),
+        ("requests", ctypes.c_int),
+        ("tokens", ctypes.c_int),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_token_stride", ctypes.c_int64),
+        ("v_token_stride", ctypes.c_int64),
+        ("dtype", ctypes.c_int),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/dk_w4a16.h declares.
 _P, _I, _U, _SZ = ctypes.c_void_p, ctypes.c_int, ctypes.c_uint, ctypes.c_size_t
 _L = ctypes.c_int64
@@ -165,6 +220,11 @@ SIGNATURES = {
     "dk_cache_attention_counter_bytes": (_SZ, []),
     "dk_cache_attention": (_I, [ctypes.POINTER(CacheAttentionArgs), _P, _SZ, _P]),
     "dk_block_norm": (_I, [ctypes.POINTER(BlockNormArgs), _P]),
+    "dk_w4a16_gemm": (_I, [ctypes.POINTER(GemmArgs), _P]),
+    "dk_w4a16_gemm_t": (_I, [ctypes.POINTER(GemmTArgs), _P]),
+    "dk_gated_grad": (_I, [_P, _P, _P, _P, _P, _I, _I, _L, _L, _L, _I, _I, _P]),
+    "dk_rotary": (_I, [ctypes.POINTER(RotaryArgs), _P]),
+    "dk_cache_read": (_I, [ctypes.POINTER(CacheReadArgs), _P]),
     "dk_status_string": (ctypes.c_char_p, [_I]),
     "dk_last_cuda_error": (ctypes.c_char_p, []),
     "dk_version": (ctypes.c_char_p, []),

@@ -1,0 +1,121 @@
+"""Many rows through 4-bit weights, with gradients through the frozen weights.
+
+``gemm`` is a layer's product for prompts and batches, ``gemm_gated`` the two
+projections, activation and product of a gated block in one launch, ``gemm_t``
+the transposed product.  The weights are frozen: gradients reach the rows, not
+the packed weights or their scales.  There is no CPU fallback.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .cache import _extension
+
+__all__ = ["gemm", "gemm_gated", "gemm_t"]
+
+_ACTS = {"silu": 0, "gelu": 1}
+
+
+def _wants_grad(x: torch.Tensor, *scales: torch.Tensor) -> bool:
+    if not torch.is_grad_enabled():
+        return False
+    if any(s.requires_grad for s in scales):
+        raise RuntimeError("the weights are frozen: scales must not require a gradient")
+    return x.requires_grad
+
+
+class _Gemm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, packed, scales):
+        ctx.save_for_backward(packed, scales)
+        return _extension().w4a16_gemm(packed, scales, None, None, x)[0]
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        return _extension().w4a16_gemm_t(*ctx.saved_tensors, None, None, dy), None, None
+
+
+class _GemmT(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, g, packed, scales):
+        ctx.save_for_backward(packed, scales)
+        return _extension().w4a16_gemm_t(packed, scales, None, None, g)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dx):
+        packed, scales = ctx.saved_tensors
+        return _extension().w4a16_gemm(packed, scales, None, None, dx)[0], None, None
+
+
+class _GemmGated(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, gate_scales, up, up_scales, act):
+        h, g, u = _extension().w4a16_gemm(gate, gate_scales, up, up_scales, x, act, True)
+        ctx.save_for_backward(gate, gate_scales, up, up_scales, g, u)
+        ctx.act = act
+        return h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh):
+        gate, gate_scales, up, up_scales, g, u = ctx.saved_tensors
+        dg, du = _extension().gated_grad(dh, g, u, ctx.act)
+        dx = _extension().w4a16_gemm_t(gate, gate_scales, up, up_scales, dg, du)
+        return dx.view(*dh.shape[:-1], dx.shape[-1]), None, None, None, None, None
+
+
+def _no_out(out: Optional[torch.Tensor]) -> None:
+    if out is not None:
+        raise RuntimeError("out takes no part in a gradient: call without it or under torch.no_grad()")
+
+
+def gemm(packed: torch.Tensor, scales: torch.Tensor, x: torch.Tensor, *,
+         out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x . dequant(W)^T for any number of rows: fp16 or bf16 [..., K] -> [..., M].
+
+    packed: int32 [M, K/8]; scales: fp16 [M, K/128].  A weight q * scale is
+    rounded once to x's type (past its range to infinity); products and sums are
+    fp32, and so is the result until it is rounded once.  x may be any view;
+    rows that do not begin on 16-byte boundaries are copied first.  ``out`` is
+    contiguous or has contiguous rows.  Differentiable in x.
+    """
+    if _wants_grad(x, scales):
+        _no_out(out)
+        return _Gemm.apply(x, packed, scales)
+    return _extension().w4a16_gemm(packed, scales, None, None, x, 0, False, out)[0]
+
+
+def gemm_t(packed: torch.Tensor, scales: torch.Tensor, g: torch.Tensor, *,
+           out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """g . dequant(W): fp16 or bf16 [..., M] -> [..., K], the gradient of ``gemm``'s x.
+
+    The same types and roundings as ``gemm``.  Differentiable in g.
+    """
+    if _wants_grad(g, scales):
+        _no_out(out)
+        return _GemmT.apply(g, packed, scales)
+    return _extension().w4a16_gemm_t(packed, scales, None, None, g, None, out)
+
+
+def gemm_gated(gate: Tuple[torch.Tensor, torch.Tensor], up: Tuple[torch.Tensor, torch.Tensor], x: torch.Tensor, *,
+               act: str = "silu", out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """act(x . Wg^T) * (x . Wu^T) in one launch: fp16 or bf16 [..., K] -> [..., M].
+
+    ``gate`` and ``up``: ``(packed, scales)`` of two [M, K] matrices; ``act``:
+    "silu" or "gelu" (its tanh form).  Everything between the products' fp32
+    sums and the result is fp32, rounded once (``gemv_silu_mul`` rounds as the
+    unfused fp16 sequence does).  Differentiable in x: the two projections are
+    kept in x's type for that.
+    """
+    if act not in _ACTS:
+        raise ValueError("act is 'silu' or 'gelu'")
+    if _wants_grad(x, gate[1], up[1]):
+        _no_out(out)
+        return _GemmGated.apply(x, *gate, *up, _ACTS[act])
+    return _extension().w4a16_gemm(*gate, *up, x, _ACTS[act], False, out)[0]

@@ -9,7 +9,9 @@ proper operator with a known output shape instead of an opaque Python call.
 ``W4A16Linear`` is a bias-free ``nn.Linear`` replacement holding the packed
 weights and scales as buffers.  ``torch.ops.decode_kernel.w4a16_silu_mul(x,
 packed_gate, scales_gate, packed_up, scales_up)`` is a gated MLP's gate/up
-pair with its SiLU-mul epilogue in one launch.
+pair with its SiLU-mul epilogue in one launch.  ``w4a16_linear`` has a gradient
+for x, the transposed product with the frozen weights.  ``W4A16GatedMLP`` is a
+gated feed-forward block over the many-row products, for prompts and training.
 
 There is no CPU implementation: the op raises on CPU tensors, like the rest of
 the package.
@@ -23,7 +25,7 @@ import torch
 
 from .quantize import GROUP_SIZE, quantize_and_pack_cuda
 
-__all__ = ["W4A16Linear", "w4a16_linear_op", "w4a16_silu_mul_op"]
+__all__ = ["W4A16GatedMLP", "W4A16Linear", "w4a16_linear_op", "w4a16_silu_mul_op"]
 
 
 @torch.library.custom_op("decode_kernel::w4a16_linear", mutates_args=())
@@ -44,6 +46,22 @@ def _(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor) -> torch.Tens
     torch._check(x.shape[-1] == packed.shape[1] * 8, lambda: "x.shape[-1] must equal K")
     torch._check(x.dtype == torch.float16, lambda: "x must be fp16")
     return x.new_empty((*x.shape[:-1], packed.shape[0]), dtype=torch.float16)
+
+
+def _linear_context(ctx, inputs, output) -> None:
+    _, packed, scales = inputs
+    ctx.save_for_backward(packed, scales)
+
+
+def _linear_backward(ctx, dy: torch.Tensor):
+    from . import gemm_t
+
+    if ctx.needs_input_grad[2]:
+        raise RuntimeError("the weights are frozen: scales must not require a gradient")
+    return (gemm_t(*ctx.saved_tensors, dy) if ctx.needs_input_grad[0] else None), None, None
+
+
+w4a16_linear_op.register_autograd(_linear_backward, setup_context=_linear_context)
 
 
 @torch.library.custom_op("decode_kernel::w4a16_silu_mul", mutates_args=())
@@ -116,3 +134,26 @@ class W4A16Linear(torch.nn.Module):
 
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, bits=4, group={GROUP_SIZE}"
+
+
+class W4A16GatedMLP(torch.nn.Module):
+    """A gated feed-forward block with frozen 4-bit weights: down(act(gate(x)) * up(x)).
+
+    ``gate``, ``up`` and ``down`` are ``W4A16Linear`` layers; ``act`` is "silu"
+    or "gelu" (its tanh form).  Two launches for any number of rows, and
+    gradients for x.
+    """
+
+    def __init__(self, gate: W4A16Linear, up: W4A16Linear, down: W4A16Linear, act: str = "silu"):
+        super().__init__()
+        if gate.packed.shape != up.packed.shape or down.in_features != gate.out_features:
+            raise ValueError("gate and up must have the same shape, and down their rows as its input")
+        if act not in ("silu", "gelu"):
+            raise ValueError("act is 'silu' or 'gelu'")
+        self.gate, self.up, self.down, self.act = gate, up, down, act
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        from . import gemm, gemm_gated
+
+        h = gemm_gated((self.gate.packed, self.gate.scales), (self.up.packed, self.up.scales), x, act=self.act)
+        return gemm(self.down.packed, self.down.scales, h)

@@ -510,6 +510,118 @@ typedef struct dk_block_norm_args {
 } dk_block_norm_args;
 DK_API dk_status dk_block_norm(const dk_block_norm_args* args, void* stream);
 
+/* ------------------------------------------------------------------------
+ * What a prompt's step needs besides: products of many rows with 4-bit
+ * weights, the gated pair of a feed-forward block, their gradients through
+ * the frozen weights, rotary positions, and the cache read back as rows.
+ * ------------------------------------------------------------------------ */
+
+/* y[rows, M] = x[rows, K] . dequant(W)[M, K]^T for any number of rows, or, with
+ * packed2 and scales2 (a second matrix of the same shape), a gated block's
+ *   g = x . dequant(W)^T, u = x . dequant(W2)^T, y = act(g) * u
+ *   act(g) = g * sigmoid(p(g)); DK_MLP_SILU: p = g; DK_MLP_GELU (its tanh
+ *   form): p = 2 sqrt(2 / pi) (g + 0.044715 g^3)
+ * of which gate_out and up_out (both or neither) keep g and u, rounded.
+ * x and the outputs are DK_FP16 or DK_BF16; each weight q * scale is rounded
+ * once to that type (past its range to infinity), products and sums are fp32,
+ * outputs are rounded once.  Rows are ldx (x), ldy (y) and ldk (gate_out and
+ * up_out) values apart; x and packed are 16-byte aligned and ldx is a multiple
+ * of 8 (where rows > 1).  Outputs may not overlap the inputs. */
+typedef enum dk_mlp_act { DK_MLP_SILU = 0, DK_MLP_GELU = 1 } dk_mlp_act;
+typedef struct dk_gemm_args {
+  const int32_t* packed;   /* [M, K/8] */
+  const uint16_t* scales;  /* fp16 [M, K/128] */
+  const int32_t* packed2;  /* or NULL */
+  const uint16_t* scales2;
+  const void* x;
+  void* y;
+  void* gate_out; /* or NULL */
+  void* up_out;
+  int64_t ldx, ldy, ldk;
+  int rows, M, K;
+  dk_dtype dtype;
+  dk_mlp_act act;
+} dk_gemm_args;
+DK_API dk_status dk_w4a16_gemm(const dk_gemm_args* args, void* stream);
+
+/* The transposed product, which is the gradient of x in the one above:
+ *   dx[rows, K] = g[rows, M] . dequant(W)[M, K] (+ g2[rows, M] . dequant(W2)[M, K])
+ * with the same types and roundings.  g and g2 are 16-byte aligned, their rows
+ * ldg values apart (a multiple of 8, where rows > 1). */
+typedef struct dk_gemm_t_args {
+  const int32_t* packed;
+  const uint16_t* scales;
+  const int32_t* packed2; /* or NULL */
+  const uint16_t* scales2;
+  const void* g;
+  const void* g2;
+  void* dx;
+  int64_t ldg, lddx;
+  int rows, M, K;
+  dk_dtype dtype;
+} dk_gemm_t_args;
+DK_API dk_status dk_w4a16_gemm_t(const dk_gemm_t_args* args, void* stream);
+
+/* From dh, the gradient of h = act(g) * u, those of g and u:
+ *   dg = dh * u * act'(g), du = dh * act(g)
+ * over [rows, M] tensors whose rows are lddh (dh), ldk (g and u) and ldd (dg
+ * and du) values apart; computed in fp32, rounded once. */
+DK_API dk_status dk_gated_grad(const void* dh, const void* g, const void* u, void* dg, void* du,
+                               int rows, int M, int64_t lddh, int64_t ldk, int64_t ldd,
+                               dk_dtype dtype, dk_mlp_act act, void* stream);
+
+/* Rotary positions: value pairs of every head of q and k turned by angles
+ *   a_i = positions[axis(i), token] * frequency[i], i < pairs
+ *   (x, y) -> (x cos a - y sin a, x sin a + y cos a)
+ * with the pair of values i and i + pairs, or 2i and 2i + 1 if `paired`; the
+ * values past 2 * pairs are copied.  Axis a has the pairs up to section_end[a]
+ * that the axes before it do not have.  `inverse` turns back (the gradient).
+ * Angles are fp64, sines, cosines and the turning fp32, results rounded once.
+ * q and k have strides in values, the last dimension contiguous; k may be NULL.
+ * positions are int32 or int64, axes position_stride apart.  q_out may be q and
+ * k_out k (with the same strides). */
+#define DK_ROTARY_MAX_AXES 4
+#define DK_ROTARY_MAX_DIM 1024
+typedef struct dk_rotary_args {
+  const void* q; /* [tokens, q_heads, head_dim] */
+  const void* k; /* [tokens, kv_heads, head_dim] or NULL */
+  void* q_out;
+  void* k_out;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride;
+  int64_t q_out_token_stride, q_out_head_stride, k_out_token_stride, k_out_head_stride;
+  const void* positions;
+  const float* frequency; /* [pairs], radians a position */
+  int64_t position_stride;
+  int positions_64; /* int64 instead of int32 */
+  int tokens, q_heads, kv_heads, head_dim, pairs, axes;
+  int section_end[DK_ROTARY_MAX_AXES]; /* rising, the last is pairs */
+  int paired, inverse;
+  dk_dtype dtype; /* DK_FP16, DK_BF16 or DK_FP32 */
+} dk_rotary_args;
+DK_API dk_status dk_rotary(const dk_rotary_args* args, void* stream);
+
+/* Keys and values of a paged cache as rows: row starts[r] + i of k and v
+ * ([tokens, kv_heads, head_dim], DK_FP16 or DK_BF16, code * scale in fp32
+ * rounded once) is token lengths[r] - n + i of request r, of whose n =
+ * starts[r + 1] - starts[r] rows the last is its last token.  Rows without a
+ * token (n > lengths[r], tokens past the table's width or in entries outside
+ * the pool) are zeros; rows from starts[requests] on are not written.  starts
+ * rise.  Outputs are 16-byte aligned, their rows a multiple of 8 values apart
+ * and heads head_dim apart. */
+typedef struct dk_cache_read_args {
+  dk_cache8 cache;
+  const int32_t* block_table;
+  int max_blocks, table_stride;
+  const int32_t* lengths;
+  const int32_t* starts; /* [requests + 1] */
+  int requests, tokens;
+  void* k;
+  void* v;
+  int64_t k_token_stride, v_token_stride;
+  dk_dtype dtype;
+} dk_cache_read_args;
+DK_API dk_status dk_cache_read(const dk_cache_read_args* args, void* stream);
+
 /* Human-readable text for a status; the CUDA error behind the last
  * DK_ERR_LAUNCH / DK_ERR_CUDA on this thread. */
 DK_API const char* dk_status_string(dk_status s);
