@@ -87,6 +87,34 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatil
   }
 }
 
+// The same without suspending the thread, for the one that issues the MMAs.
+__device__ __forceinline__ bool spin_bar(uint64_t* bar, uint32_t parity, volatile int* give_up, int* error) {
+  auto test = [&] {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n"
+        " mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+  };
+  if (test()) return true;
+  const uint64_t t0 = globaltimer_ns();
+  for (int i = 0;; ++i) {
+    if (test()) return true;
+    if ((i & 255) == 255) {
+      if (*give_up) return false;
+      if (globaltimer_ns() - t0 > kWaitLimitNs) {
+        if (error) atomicExch(error, kDevWaitTimeout);
+        *give_up = 1;
+        return false;
+      }
+    }
+  }
+}
+
 __device__ __forceinline__ void tma_2d(uint32_t dst, const void* map, int c0, int c1, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
@@ -132,6 +160,35 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
         "r"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
         : "memory");
 }
+// The same with A in shared memory.
+template <int CG>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  if constexpr (CG == 1)
+    umma_f16(d, a, b, idesc, accumulate);
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+        : "memory");
+}
+// A stage of A with the lanes innermost, in the 128-byte swizzle: rows of 64
+// lanes (128 bytes), one for each depth, eight in an atom of 1024 bytes; the
+// other 64 lanes are half a stage (8192 bytes) away.
+__device__ __forceinline__ uint64_t desc_lanes_inner(uint32_t addr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((addr >> 4) & 0x3FFFu);
+  d |= (uint64_t)(8192 >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(yes));
+  return yes != 0;
+}
 // Arrive on the barrier (of both CTAs of a pair) once the MMAs issued so far are done.
 template <int CG>
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
@@ -150,13 +207,46 @@ __device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&v)[32]) 
       "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]),
       "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
       : "memory");
-  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void tmem_ld16_wait(uint32_t at, float (&f)[16]) {
-  uint32_t v[16];
-  tmem_ld16(at, v);
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// 32 columns of this thread's lane.
+__device__ __forceinline__ void tmem_ld32(uint32_t at, float (&f)[32]) {
+  uint32_t v[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,"
+      "%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+        "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]),
+        "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]),
+        "=r"(v[31])
+      : "r"(at));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-  for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(v[i]);
+  for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]);
+}
+// A box of shared memory to global memory; parts outside the tensor are left out.
+__device__ __forceinline__ void tma_store_2d(const void* map, int c0, int c1, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(c0),
+               "r"(c1), "r"(src)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(LEFT) : "memory"); }
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+// Whether all `threads` that meet at the barrier say so.
+__device__ __forceinline__ bool barrier_all(int id, int threads, bool mine) {
+  uint32_t all;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n"
+      " barrier.cta.red.and.aligned.pred q, %2, %3, p;\n selp.u32 %0, 1, 0, q;\n}"
+      : "=r"(all)
+      : "r"(mine ? 1u : 0u), "r"(id), "r"(threads)
+      : "memory");
+  return all != 0;
+}
+__device__ __forceinline__ void sts16(uint32_t addr, uint16_t v) {
+  asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(v) : "memory");
 }
 __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
   uint32_t v;
@@ -229,7 +319,11 @@ __device__ __forceinline__ float gate_of(float g, int act, float& slope) {
     p = c * (g + 0.044715f * g * g * g);
     slope = c * (1.f + 0.134145f * g * g);
   }
-  return 1.f / (1.f + __expf(-p));
+  // 1 / (1 + 2^(-p log2 e)); the two approximations are 2^-22 right.
+  float e, y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-1.4426950408889634f * p));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(1.f + e));
+  return y;
 }
 
 // ---------------------------------------------------------------------------
@@ -244,9 +338,10 @@ constexpr int kLanes = 128;                // lanes a CTA
 constexpr int kStepDepth = 128;            // depth of a step: a group
 constexpr int kHalfDepth = 64;             // depth of a stage of A and B
 constexpr int kRawBytes = 128 * 64;        // packed weights of a step
-constexpr int kAStages = 8;                // stages of A in tensor memory, 32 columns each
+constexpr int kStages = 8;                 // of A in tensor memory, 32 columns each, with their stages of B
 constexpr int kAColumn = 256;              // A begins behind the sums
-constexpr int kMaxBStages = 16, kMaxRaw = 16;
+constexpr int kABytes = 128 * kHalfDepth * 2;  // a stage of A in shared memory
+constexpr int kMaxStages = 8, kMaxRaw = 16;
 constexpr int kMaxTokens = 256;
 constexpr int kSmemMost = 227 * 1024;
 // A CTA takes all of its SM's tensor memory, so two CTAs of these kernels must
@@ -256,7 +351,7 @@ constexpr int kSmemMost = 227 * 1024;
 constexpr int kSmemLeast = 116 * 1024;
 
 struct alignas(64) TileArgs {
-  CUtensorMap w[2], b[2];
+  CUtensorMap w[2], b[2], out[3];  // out: y, g, u
   const __half* scales[2];
   void* y;
   void* keep[2];
@@ -265,19 +360,25 @@ struct alignas(64) TileArgs {
   int rows, M, K, groups, act;
   int lane_tiles, token_tiles, tokens;  // tokens: of a tile
   int steps, matrix_steps;              // all steps, those of one matrix (transposed: the second's follow)
-  int b_stages, raw_stages, split;
+  int stages, raw_stages, split, boxes;  // boxes: results leave by TMA
 };
 
+// Results on their way out: 32 tokens of a tile's outputs, twice.
+constexpr int kBoxTokens = 32;
+constexpr int kBoxBytes = 3 * kBoxTokens * 64 * 2;  // h, g and u of 64 outputs; or y of 128
+
 struct GemmSmem {
-  int b, raw, scratch, bars, total;
+  int stage_bytes, raw, scratch, box, bars, total;
 };
-__host__ __device__ inline GemmSmem gemm_smem(int b_rows, int b_stages, int raw_stages) {
+// Stages (A where it goes through shared memory, then B) from 0 on.
+__host__ __device__ inline GemmSmem gemm_smem(int a_bytes, int b_rows, int stages, int raw_stages) {
   GemmSmem l;
-  l.b = 0;
-  l.raw = l.b + b_stages * b_rows * 128;
+  l.stage_bytes = a_bytes + b_rows * 128;
+  l.raw = stages * l.stage_bytes;
   l.scratch = l.raw + raw_stages * kRawBytes;
-  l.bars = l.scratch + kDqWarps * 256;
-  l.total = l.bars + (2 * kMaxBStages + 2 * kMaxRaw + 2 * kAStages + 4) * 8 + 16;
+  l.box = l.scratch + kDqWarps * 256;
+  l.bars = l.box + 2 * kBoxBytes;
+  l.total = l.bars + (2 * kMaxStages + 2 * kMaxRaw + 6) * 8 + 16;
   return l;
 }
 
@@ -288,6 +389,14 @@ template <bool BF16>
 __device__ __forceinline__ Value<BF16> rounded(float x) {
   if constexpr (BF16) return __float2bfloat16_rn(x);
   else return __float2half_rn(x);
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t rounded2(float lo, float hi) {
+  uint32_t d;
+  if constexpr (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
 }
 
 // Two columns (tokens t, t + 1) of this thread's lane: to y.
@@ -321,10 +430,10 @@ __device__ __forceinline__ void finish(const TileArgs& a, int lane_row, int out,
 }
 
 // The output that lane `lane` of a tile's 128 holds.
-template <int MODE>
+template <int MODE, bool TURNED>
 __device__ __forceinline__ int output_of(int tile, int lane) {
   const int warp = lane >> 5, l = lane & 31;
-  if constexpr (MODE == kPlain) return tile * 128 + lane;
+  if constexpr (MODE == kPlain || (MODE == kTransposed && !TURNED)) return tile * 128 + lane;
   else if constexpr (MODE == kGated) return tile * 64 + warp * 16 + (l & 15);
   else return tile * 128 + warp * 32 + 8 * (l & 3) + (l >> 2);  // as the transposition of nibbles leaves them
 }
@@ -334,40 +443,38 @@ __device__ __forceinline__ int output_of(int tile, int lane) {
 template <bool BF16, int MODE, int CG>
 __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant__ TileArgs a) {
   extern __shared__ __align__(1024) uint8_t smem[];
+  constexpr bool kATmem = CG == 1;           // where A lies
+  constexpr int kABase = kATmem ? 0 : kABytes;  // of B in its stage
   const int b_rows = a.tokens / CG;
-  const GemmSmem L = gemm_smem(b_rows, a.b_stages, a.raw_stages);
-  uint64_t* b_full = reinterpret_cast<uint64_t*>(smem + L.bars);  // tokens landed (the pair's, in its first CTA)
-  uint64_t* b_free = b_full + kMaxBStages;   // MMAs have read them
-  uint64_t* raw_full = b_free + kMaxBStages; // packed weights landed
+  const GemmSmem L = gemm_smem(kABase, b_rows, a.stages, a.raw_stages);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L.bars);  // A stored and B landed (the pair's, in its first CTA)
+  uint64_t* free_ = full + kMaxStages;       // MMAs have read them
+  uint64_t* raw_full = free_ + kMaxStages;   // packed weights landed
   uint64_t* raw_free = raw_full + kMaxRaw;   // unpacked
-  uint64_t* a_full = raw_free + kMaxRaw;     // A stored (the pair's, in its first CTA)
-  uint64_t* a_free = a_full + kAStages;      // MMAs have read it
-  uint64_t* sums_full = a_free + kAStages;   // a tile's MMAs are done
-  uint64_t* sums_free = sums_full + 1;       // and its sums read (the pair's)
-  uint64_t* drained = sums_free + 1;         // at the end: every MMA is done
+  uint64_t* sums_full = raw_free + kMaxRaw;  // a tile's MMAs are done; two places of sums for pairs
+  uint64_t* sums_free = sums_full + 2;       // and its sums read (the pair's)
+  uint64_t* drained = sums_free + 2;         // at the end: every MMA is done
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 2);
   volatile int* give_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const bool first = CG == 1 || rank == 0;
   const uint32_t base = smem_u32(smem);
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kMaxBStages; ++i) {
-      mbar_init(&b_full[i], 1);
-      mbar_init(&b_free[i], 1);
+    for (int i = 0; i < kMaxStages; ++i) {
+      mbar_init(&full[i], kDqWarps / 2 * CG + 1);
+      mbar_init(&free_[i], 1);
     }
     for (int i = 0; i < kMaxRaw; ++i) {
       mbar_init(&raw_full[i], 1);
       mbar_init(&raw_free[i], kDqWarps);
     }
-    for (int i = 0; i < kAStages; ++i) {
-      mbar_init(&a_full[i], kDqWarps / 2 * CG);
-      mbar_init(&a_free[i], 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sums_full[i], 1);
+      mbar_init(&sums_free[i], kSumWarps * CG);
     }
-    mbar_init(sums_full, 1);
-    mbar_init(sums_free, kSumWarps * CG);
     mbar_init(drained, 1);
     *give_up = 0;
     fence_barrier_init();
@@ -391,65 +498,118 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
   if (warp < kDqWarps) {
     // ---------------- unpacking ----------------
     const int half = warp >> 2, quad = warp & 3, tile_lane = quad * 32 + lane;
-    const uint32_t a_leader = mapa(smem_u32(a_full), 0);
+    const uint32_t full_leader = mapa(smem_u32(full), 0);
     const uint32_t scratch = base + L.scratch + warp * 256;
     int raw = 0, raw_phase = 0, slot = half, phase = 0;
-    bool fresh = true, going = true;  // fresh: the stages of A have not been used yet
-    for (int item = item0; item < items && going; item += item_step) {
-      const int tile = item / a.token_tiles * CG + (CG == 2 ? (int)rank : 0);
-      // Where this lane's packed row lies in a step's copy, and its scales.
-      int row, matrix = 0;
-      const __half* scale_row = nullptr;
-      if constexpr (MODE == kPlain) {
-        row = tile_lane;
-        if (tile * 128 + row < a.M) scale_row = a.scales[0] + (long long)(tile * 128 + row) * a.groups;
-      } else if constexpr (MODE == kGated) {
-        matrix = lane >> 4;
-        row = matrix * 64 + quad * 16 + (lane & 15);
-        const int m = tile * 64 + quad * 16 + (lane & 15);
-        if (m < a.M) scale_row = a.scales[matrix] + (long long)m * a.groups;
-      } else {
-        row = half * 64 + (lane >> 2);  // and every eighth after it
+    bool fresh = true;  // the stages have not been used yet
+    int pending = -1;   // the stage that is on its way into tensor memory
+    auto arrive = [&] {
+      tmem_st_wait();
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&full[pending]);
       }
-      for (int s = begin; s < end; ++s) {
-        ScalePair<BF16> pair;
+    };
+    // Where this lane's packed row lies in a step's copy, and of its four pieces
+    // of 32 values the first of two.
+    const int row = MODE == kPlain ? tile_lane
+                    : MODE == kGated ? (lane >> 4) * 64 + quad * 16 + (lane & 15)
+                    : kATmem ? half * 64 + (lane >> 2)  // and every eighth after it
+                             : half * 64 + (tile_lane & 63);
+    const int piece = MODE == kTransposed ? 2 * (tile_lane >> 6) : 2 * half;
+    // A's row in shared memory: 64 values of the depth for each lane; transposed,
+    // 64 lanes for each depth, the tile's second 64 lanes behind the first.
+    const int a_row = MODE == kTransposed ? tile_lane & 63 : tile_lane;
+    const uint32_t a_at = base + (MODE == kTransposed ? (tile_lane >> 6) * (kABytes / 2) : 0) + a_row * 128;
+    // Scales are asked for three steps before they are needed.
+    int f_item = item0, f_step = begin;
+    long long f_at;  // where the item's scales begin, -1 where it has none
+    auto scales_at = [&](int item) -> long long {
+      const int tile = item / a.token_tiles * CG + (CG == 2 ? (int)rank : 0);
+      if constexpr (MODE == kTransposed) return tile < a.groups ? tile : -1;
+      const int m = MODE == kPlain ? tile * 128 + tile_lane : tile * 64 + quad * 16 + (lane & 15);
+      return m < a.M ? (long long)m * a.groups : -1;
+    };
+    f_at = scales_at(item0);
+    const unsigned short* scales[2] = {reinterpret_cast<const unsigned short*>(a.scales[MODE == kGated ? lane >> 4 : 0]),
+                                       reinterpret_cast<const unsigned short*>(a.scales[1])};
+    auto fetch = [&]() -> uint32_t {
+      uint32_t two = 0;
+      if (f_item < items) {
         if constexpr (MODE != kTransposed) {
-          const __half sc = scale_row ? __ldg(scale_row + s) : __half(0.f);
-          pair = scale_pair<BF16>(sc, sc);
+          if (f_at >= 0) two = __ldg(scales[0] + f_at + f_step);
         } else {
-          // Lane l brings the scales of depths 2 l and 2 l + 1.
-          const int seg = s >= a.matrix_steps, m = (s - seg * a.matrix_steps) * kStepDepth + half * 64 + 2 * lane;
-          const __half* p = a.scales[seg] + (long long)m * a.groups + tile;
-          const bool in = tile < a.groups;
-          const __half lo = in && m < a.M ? __ldg(p) : __half(0.f), hi = in && m + 1 < a.M ? __ldg(p + a.groups) : __half(0.f);
-          const ScalePair<BF16> mine = scale_pair<BF16>(lo, hi);
-          __syncwarp();
-          asm volatile("st.shared.u32 [%0], %1;" ::"r"(scratch + lane * 4), "r"(mine.first) : "memory");
-          if constexpr (BF16) asm volatile("st.shared.u32 [%0], %1;" ::"r"(scratch + 128 + lane * 4), "r"(mine.rest) : "memory");
-          __syncwarp();
-        }
-        going = __all_sync(0xffffffffu, wait_bar(&raw_full[raw], raw_phase, give_up, a.error));
-        if (!going) break;
-        uint32_t w[8];
-        const uint32_t from = base + L.raw + raw * kRawBytes;
-        if constexpr (MODE != kTransposed) {
-          // 32 bytes of the row: pieces 2 half and 2 half + 1 of four, swizzled.
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint4 v = lds128(from + row * 64 + (((2 * half + i) ^ ((row >> 1) & 3)) << 4));
-            w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int r = row + 8 * i;
-            w[i] = lds32(from + r * 64 + ((quad ^ ((r >> 1) & 3)) << 4) + (lane & 3) * 4);
+          // A in tensor memory: lane l brings the scales of depths 2 l and 2 l + 1; else its row's.
+          const int seg = f_step >= a.matrix_steps;
+          const int m = (f_step - seg * a.matrix_steps) * kStepDepth + half * 64 + (kATmem ? 2 * lane : tile_lane & 63);
+          if (f_at >= 0) {
+            const unsigned short* p = scales[seg] + f_at + (long long)m * a.groups;
+            if (m < a.M) two = __ldg(p);
+            if (kATmem && m + 1 < a.M) two |= (uint32_t)__ldg(p + a.groups) << 16;
           }
         }
+        if (++f_step == end) {
+          f_step = begin;
+          f_item += item_step;
+          if (f_item < items) f_at = scales_at(f_item);
+        }
+      }
+      return two;
+    };
+    uint32_t scale0 = fetch(), scale1 = fetch(), scale2 = fetch();
+    const int todo = (items - item0 + item_step - 1) / item_step * (end - begin);
+    for (int step = 0; step < todo; ++step) {
+      constexpr bool kTurn = MODE == kTransposed && kATmem;  // columns of W become lanes
+      ScalePair<BF16> pair;
+      const __half2 both = *reinterpret_cast<const __half2*>(&scale0);
+      if constexpr (!kTurn) {
+        pair = scale_pair<BF16>(__low2half(both), __low2half(both));
+      } else {
+        const ScalePair<BF16> mine = scale_pair<BF16>(__low2half(both), __high2half(both));
         __syncwarp();
-        if (lane == 0) mbar_arrive(&raw_free[raw]);
-        if (++raw == a.raw_stages) raw = 0, raw_phase ^= 1;
-        if constexpr (MODE == kTransposed) {
+        asm volatile("st.shared.u32 [%0], %1;" ::"r"(scratch + lane * 4), "r"(mine.first) : "memory");
+        if constexpr (BF16) asm volatile("st.shared.u32 [%0], %1;" ::"r"(scratch + 128 + lane * 4), "r"(mine.rest) : "memory");
+        __syncwarp();
+      }
+      scale0 = scale1;
+      scale1 = scale2;
+      scale2 = fetch();
+      if (!__all_sync(0xffffffffu, wait_bar(&raw_full[raw], raw_phase, give_up, a.error))) break;
+      uint32_t w[8];
+      const uint32_t from = base + L.raw + raw * kRawBytes;
+      if constexpr (!kTurn) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint4 v = lds128(from + row * 64 + (((piece + i) ^ ((row >> 1) & 3)) << 4));
+          w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = row + 8 * i;
+          w[i] = lds32(from + r * 64 + ((quad ^ ((r >> 1) & 3)) << 4) + (lane & 3) * 4);
+        }
+      }
+      if constexpr (!kATmem) {
+        if (!fresh && !__all_sync(0xffffffffu, wait_bar(&free_[slot], phase ^ 1, give_up, a.error))) break;
+        const uint32_t at = a_at + slot * L.stage_bytes;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t w4 = BF16 ? w[i] >> 4 : 0;
+          uint32_t o[4];
+#pragma unroll
+          for (int b = 0; b < 4; ++b) o[b] = scaled<BF16>(exact_pair<BF16>(w[i], w4, b), pair);
+          sts128(at + ((i ^ (a_row & 7)) << 4), o);
+        }
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) {
+          arrive_cluster(full_leader + slot * 8);
+          mbar_arrive(&raw_free[raw]);
+        }
+      } else {
+        if constexpr (kTurn) {
           // An 8 x 8 transposition of nibbles over the lanes l, l ^ 4, l ^ 8, ..:
           // row r's word with columns 0..7 becomes column r's with rows 0..7.
           const bool b2 = lane & 16, b1 = lane & 8, b0 = lane & 4;
@@ -468,67 +628,116 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           uint4 first4, rest4;
-          if constexpr (MODE == kTransposed) {
+          if constexpr (kTurn) {
             first4 = lds128(scratch + i * 16);
             if constexpr (BF16) rest4 = lds128(scratch + 128 + i * 16);
           }
           const uint32_t w4 = BF16 ? w[i] >> 4 : 0;
 #pragma unroll
           for (int b = 0; b < 4; ++b) {
-            if constexpr (MODE == kTransposed) {
+            if constexpr (kTurn) {
               pair.first = b == 0 ? first4.x : b == 1 ? first4.y : b == 2 ? first4.z : first4.w;
               if constexpr (BF16) pair.rest = b == 0 ? rest4.x : b == 1 ? rest4.y : b == 2 ? rest4.z : rest4.w;
             }
             o[4 * i + b] = scaled<BF16>(exact_pair<BF16>(w[i], w4, b), pair);
           }
         }
-        if (!fresh) {
-          going = __all_sync(0xffffffffu, wait_bar(&a_free[slot], phase ^ 1, give_up, a.error));
-          if (!going) break;
-        }
+        if (pending >= 0) arrive();  // the stage before, whose storing went on beside this one's unpacking
+        pending = -1;
+        if (!fresh && !__all_sync(0xffffffffu, wait_bar(&free_[slot], phase ^ 1, give_up, a.error))) break;
         tcgen05_fence_after();
         tmem_st32(tmem + ((uint32_t)(quad * 32) << 16) + kAColumn + slot * 32, o);
-        tcgen05_fence_before();
+        pending = slot;
         __syncwarp();
-        if (lane == 0) {
-          if constexpr (CG == 1) mbar_arrive(&a_full[slot]);
-          else arrive_cluster(a_leader + slot * 8);
-        }
-        slot += 2;
-        if (slot >= kAStages) slot -= kAStages, phase ^= 1, fresh = false;
+        if (lane == 0) mbar_arrive(&raw_free[raw]);
       }
+      // The packed words were given back only after what was made of them had
+      // been stored: a load whose value nobody has used yet may still be on its
+      // way when the next copy lands.
+      if (++raw == a.raw_stages) raw = 0, raw_phase ^= 1;
+      slot += 2;
+      if (slot >= a.stages) slot -= a.stages, phase ^= 1, fresh = false;
     }
+    if (pending >= 0) arrive();
   } else if (warp < kDqWarps + kSumWarps) {
     // ---------------- the sums ----------------
     const int quad = warp & 3, tile_lane = quad * 32 + lane;
-    const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16);
     const uint32_t free_leader = mapa(smem_u32(sums_free), 0);
-    int phase = 0;
+    const bool issuer = threadIdx.x == kDqWarps * 32;
+    constexpr int kOuts = MODE == kGated ? 64 : 128;  // of a tile
+    const uint32_t column = (uint32_t)output_of<MODE, kATmem>(0, tile_lane) * 2;
+    int phase = 0, turn = 0, place = 0;
     for (int item = item0; item < items; item += item_step) {
-      if (!__all_sync(0xffffffffu, wait_bar(sums_full, phase, give_up, a.error))) break;
-      phase ^= 1;
+      // All four warps go on or none does: they meet at barriers.
+      if (!barrier_all(1, kSumWarps * 32, wait_bar(&sums_full[place], phase, give_up, a.error))) break;
       tcgen05_fence_after();
+      const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + place * kMaxTokens;
       const int tile = item / a.token_tiles * CG + (CG == 2 ? (int)rank : 0);
-      const int t0 = item % a.token_tiles * a.tokens, out = output_of<MODE>(tile, tile_lane);
-      for (int c = 0; c < a.tokens; c += 16) {
-        float v[16];
-        tmem_ld16_wait(from + c, v);
+      const int t0 = item % a.token_tiles * a.tokens, out = output_of<MODE, kATmem>(tile, tile_lane);
+      for (int c = 0; c < a.tokens; c += kBoxTokens) {
+        float v[32];
+        tmem_ld32(from + c, v);
+        if (c + kBoxTokens >= a.tokens) {  // the last of the tile's sums are in registers
+          tcgen05_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (CG == 1) mbar_arrive(sums_free);
+            else arrive_cluster(free_leader + place * 8);
+          }
+        }
         if (CG == 1 && a.split > 1) {
           float* red = reinterpret_cast<float*>(smem);  // over the rings: every copy has been read
 #pragma unroll
-          for (int j = 0; j < 16; ++j) red[(c + j) * kLanes + tile_lane] = v[j];
-        } else {
+          for (int j = 0; j < 32; ++j) red[(c + j) * kLanes + tile_lane] = v[j];
+        } else if (!a.boxes) {
 #pragma unroll
-          for (int j = 0; j < 16; j += 2) finish<BF16, MODE>(a, tile_lane, out, t0 + c + j, v[j], v[j + 1]);
+          for (int j = 0; j < 32; j += 2) finish<BF16, MODE>(a, tile_lane, out, t0 + c + j, v[j], v[j + 1]);
+        } else {
+          const uint32_t box = base + L.box + turn * kBoxBytes;
+          turn ^= 1;
+          if (issuer) bulk_wait_read<1>();  // the store before last has read this box
+          named_barrier(1, kSumWarps * 32);
+          if constexpr (MODE != kGated) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              const uint32_t two = rounded2<BF16>(v[j], v[j + 1]);
+              sts16(box + j * kOuts * 2 + column, (uint16_t)two);
+              sts16(box + (j + 1) * kOuts * 2 + column, (uint16_t)(two >> 16));
+            }
+          } else {
+            // Lanes 0..15 of a warp hold g, lanes 16..31 u of the same outputs:
+            // each takes every second token.
+            const bool gate = lane < 16;
+            const uint32_t at = box + column + (gate ? 0 : kOuts * 2);
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              const float other = __shfl_xor_sync(0xffffffffu, gate ? v[j + 1] : v[j], 16);
+              const float g = gate ? v[j] : other, u = gate ? other : v[j + 1];
+              float slope;
+              const float h = g * gate_of(g, a.act, slope) * u;
+              const uint32_t two = rounded2<BF16>(h, g);
+              sts16(at + j * kOuts * 2, (uint16_t)two);
+              if (a.keep[0]) {
+                sts16(at + kBoxTokens * kOuts * 2 + j * kOuts * 2, (uint16_t)(two >> 16));
+                sts16(at + 2 * kBoxTokens * kOuts * 2 + j * kOuts * 2, (uint16_t)rounded2<BF16>(u, u));
+              }
+            }
+          }
+          fence_async_shared();
+          named_barrier(1, kSumWarps * 32);
+          if (issuer && tile * kOuts < (MODE == kTransposed ? a.K : a.M) && t0 + c < a.rows) {
+            tma_store_2d(&a.out[0], tile * kOuts, t0 + c, box);
+            if (MODE == kGated && a.keep[0]) {
+              tma_store_2d(&a.out[1], tile * kOuts, t0 + c, box + kBoxTokens * kOuts * 2);
+              tma_store_2d(&a.out[2], tile * kOuts, t0 + c, box + 2 * kBoxTokens * kOuts * 2);
+            }
+            bulk_commit();
+          }
         }
       }
-      tcgen05_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if constexpr (CG == 1) mbar_arrive(sums_free);
-        else arrive_cluster(free_leader);
-      }
+      if (CG == 1 || (place ^= 1) == 0) phase ^= 1;
     }
+    if (issuer) bulk_wait_all();
     // The pair's second CTA stays until the first one's last signal is here.
     if (!first && warp == kDqWarps && lane == 0) wait_bar(drained, 0, give_up, a.error);
     __syncwarp();
@@ -538,32 +747,33 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
       int slot = 0, phase = 0, issued = 0;
       bool going = true;
       const uint32_t bytes = (uint32_t)b_rows * 128;
-      const uint32_t full_leader = mapa(smem_u32(b_full), 0);
+      const uint32_t full_leader = mapa(smem_u32(full), 0);
       for (int item = item0; item < items && going; item += item_step) {
         const int t0 = item % a.token_tiles * a.tokens + (CG == 2 ? (int)rank * b_rows : 0);
         for (int n = 2 * begin; n < 2 * end; ++n) {
-          if (issued >= a.b_stages && !wait_bar(&b_free[slot], phase ^ 1, give_up, a.error)) {
+          if (issued >= a.stages && !wait_bar(&free_[slot], phase ^ 1, give_up, a.error)) {
             going = false;
             break;
           }
           const int seg = MODE == kTransposed && (n >> 1) >= a.matrix_steps;
           const int d = (n - 2 * seg * a.matrix_steps) * kHalfDepth;
-          const uint32_t dst = base + L.b + slot * bytes;
+          const uint32_t dst = base + slot * L.stage_bytes + kABase;
           if constexpr (CG == 1) {
-            mbar_arrive_expect_tx(&b_full[slot], bytes);
-            tma_2d(dst, &a.b[seg], d, t0, smem_u32(&b_full[slot]));
+            mbar_arrive_expect_tx(&full[slot], bytes);
+            tma_2d(dst, &a.b[seg], d, t0, smem_u32(&full[slot]));
           } else {
-            if (first) mbar_arrive_expect_tx(&b_full[slot], 2 * bytes);
+            if (first) mbar_arrive_expect_tx(&full[slot], 2 * bytes);
             tma_2d_pair(dst, &a.b[seg], d, t0, full_leader + slot * 8);
           }
           ++issued;
-          if (++slot == a.b_stages) slot = 0, phase ^= 1;
+          if (++slot == a.stages) slot = 0, phase ^= 1;
         }
       }
-      if (!going && first) {  // what was asked for lands before the CTA ends
+      if (!going) {
+        // What was asked for lands before the CTA ends; a stage whose A never
+        // came cannot say so, its wait ends by the clock.
         volatile int none = 0;
-        for (int i = max(0, issued - a.b_stages); i < issued; ++i)
-          wait_bar(&b_full[i % a.b_stages], (i / a.b_stages) & 1, &none, a.error);
+        for (int i = max(0, issued - a.stages); i < issued && first; ++i) wait_bar(&full[i % a.stages], (i / a.stages) & 1, &none, a.error);
       }
     }
     __syncwarp();
@@ -603,36 +813,51 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
     __syncwarp();
   } else if (warp == kMmaWarp) {
     // ---------------- the MMAs ----------------
-    if (lane == 0 && first) {
-      // fp32 sums, A and B fp16 (0) or bf16 (1), both with the depth innermost.
-      const uint32_t idesc = (1u << 4) | ((BF16 ? 1u : 0u) << 7) | ((BF16 ? 1u : 0u) << 10) | ((uint32_t)(a.tokens >> 3) << 17) |
+    // The whole warp goes along, so that the operands stay in uniform registers;
+    // one thread issues.
+    if (first) {
+      // fp32 sums, A and B fp16 (0) or bf16 (1), B with the depth innermost, A
+      // too but for the transposed product's, whose lanes are innermost.
+      const uint32_t idesc = (1u << 4) | ((BF16 ? 1u : 0u) << 7) | ((BF16 ? 1u : 0u) << 10) |
+                             ((MODE == kTransposed && !kATmem ? 1u : 0u) << 15) | ((uint32_t)(a.tokens >> 3) << 17) |
                              ((uint32_t)(kLanes * CG >> 4) << 24);
-      int slot = 0, phase = 0, a_slot = 0, a_phase = 0, tile_phase = 0;
-      bool going = true, again = false;
-      for (int item = item0; item < items && going; item += item_step) {
-        if (again) {
-          if (!wait_bar(sums_free, tile_phase, give_up, a.error)) break;
-          tile_phase ^= 1;
-        }
-        again = true;
+      int slot = 0, phase = 0, tile = 0;
+      bool going = true;
+      for (int item = item0; item < items && going; item += item_step, ++tile) {
+        const int place = CG == 1 ? 0 : tile & 1;
+        if (CG == 2 && tile >= 2 && !__all_sync(0xffffffffu, spin_bar(&sums_free[place], ((tile >> 1) & 1) ^ 1, give_up, a.error))) break;
         tcgen05_fence_after();
+        const uint32_t d = tmem + place * kMaxTokens;
         for (int n = 2 * begin; n < 2 * end; ++n) {
-          going = wait_bar(&a_full[a_slot], a_phase, give_up, a.error) && wait_bar(&b_full[slot], phase, give_up, a.error);
-          if (!going) break;
+          going = spin_bar(&full[slot], phase, give_up, a.error);
+          if (!__all_sync(0xffffffffu, going)) {
+            going = false;
+            break;
+          }
           tcgen05_fence_after();
-          const uint32_t at = tmem + kAColumn + a_slot * 32, bt = base + L.b + slot * (uint32_t)b_rows * 128;
+          const uint32_t at = base + slot * L.stage_bytes;
+          const uint64_t b0 = umma_desc_k_sw128(at + kABase);
+          if (elect_one()) {
+            if constexpr (kATmem) {
+              const uint32_t a0 = tmem + kAColumn + slot * 32;
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            mma_ts<CG>(tmem, at + k * 8, umma_desc_k_sw128(bt + k * 32), idesc, n > 2 * begin || k > 0);
-          mma_commit<CG>(&a_free[a_slot]);
-          mma_commit<CG>(&b_free[slot]);
-          if (++a_slot == kAStages) a_slot = 0, a_phase ^= 1;
-          if (++slot == a.b_stages) slot = 0, phase ^= 1;
+              for (int k = 0; k < 4; ++k) mma_ts<CG>(d, a0 + k * 8, b0 + k * 2, idesc, n > 2 * begin || k > 0);
+            } else {
+              // 16 of the depth: 32 bytes on in a row, or 16 rows on.
+              const uint64_t a0 = MODE == kTransposed ? desc_lanes_inner(at) : umma_desc_k_sw128(at);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) mma_ss<CG>(d, a0 + k * (MODE == kTransposed ? 128 : 2), b0 + k * 2, idesc, n > 2 * begin || k > 0);
+            }
+            mma_commit<CG>(&free_[slot]);
+            if (n + 1 == 2 * end) mma_commit<CG>(&sums_full[place]);
+          }
+          __syncwarp();
+          if (++slot == a.stages) slot = 0, phase ^= 1;
         }
-        if (going) mma_commit<CG>(sums_full);
       }
       // Every MMA is done before the tensor memory is given back.
-      mma_commit<CG>(drained);
+      if (elect_one()) mma_commit<CG>(drained);
+      __syncwarp();
       volatile int none = 0;
       wait_bar(drained, 0, &none, a.error);
     }
@@ -647,7 +872,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
     // The cluster's sums, added in the order of the depth, two tokens a thread.
     if (warp < 12 && !*give_up) {
       const int quad = warp & 3, tile_lane = quad * 32 + lane, item = item0;
-      const int out = output_of<MODE>(item / a.token_tiles, tile_lane), t0 = item % a.token_tiles * a.tokens;
+      const int out = output_of<MODE, kATmem>(item / a.token_tiles, tile_lane), t0 = item % a.token_tiles * a.tokens;
       for (int p = (int)rank * 3 + (warp >> 2); p < a.tokens / 2; p += a.split * 3) {
         if (t0 + 2 * p >= a.rows) break;
         float v0 = 0.f, v1 = 0.f;
@@ -780,7 +1005,7 @@ dk_status product(const Product& p, cudaStream_t stream) {
     cluster = 2;
     grid = 2 * std::min((int64_t)pairs, (int64_t)a.lane_tiles * a.token_tiles);
     a.split = 1;
-    a.raw_stages = 4;
+    a.raw_stages = 3;
   } else {
     a.lane_tiles = tiles;
     a.tokens = std::max(16, ceil_div(p.rows, 16) * 16);
@@ -793,12 +1018,10 @@ dk_status product(const Product& p, cudaStream_t stream) {
     a.raw_stages = 8;
   }
   if ((int64_t)a.lane_tiles * a.token_tiles > INT32_MAX / 4) return DK_ERR_UNSUPPORTED;
-  const int b_rows = a.tokens / (pair ? 2 : 1);
-  a.b_stages = std::min(pair ? 8 : 12, (kSmemMost - 4096 - a.raw_stages * kRawBytes) / (b_rows * 128));
-  a.b_stages = std::min(a.b_stages, kMaxBStages);
-  GemmSmem l = gemm_smem(b_rows, a.b_stages, a.raw_stages);
-  size_t smem = std::max<size_t>(l.total, kSmemLeast);
-  if (!pair && a.split > 1) smem = std::max<size_t>(smem, (size_t)a.tokens * kLanes * 4);
+  const int b_rows = a.tokens / (pair ? 2 : 1), a_bytes = pair ? kABytes : 0;
+  a.stages = pair ? std::min(kMaxStages, (kSmemMost - gemm_smem(0, 0, 0, a.raw_stages).total) / (a_bytes + b_rows * 128)) : kStages;
+  const GemmSmem l = gemm_smem(a_bytes, b_rows, a.stages, a.raw_stages);
+  const size_t smem = std::max<size_t>(l.total, kSmemLeast);
 
   for (int i = 0; i < p.matrices; ++i) {
     const uint32_t box = MODE == kGated ? 64 : 128;
@@ -809,6 +1032,18 @@ dk_status product(const Product& p, cudaStream_t stream) {
     const uint64_t stride = p.rows > 1 ? (uint64_t)p.ldx * 2 : (uint64_t)ceil_div(depth, 8) * 16;
     if (!tensor_map(&a.b[i], p.x[i], p.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, depth, p.rows, stride,
                     kHalfDepth, b_rows, CU_TENSOR_MAP_SWIZZLE_128B))
+      return DK_ERR_UNSUPPORTED;
+  }
+  // Results leave in boxes where the tensors' addresses and strides allow it.
+  const int outs = MODE == kTransposed ? p.K : p.M;
+  auto boxed = [&](const void* at, int64_t ld) { return aligned16(at) && (p.rows == 1 || ld % 8 == 0); };
+  a.boxes = a.split == 1 && boxed(p.y, p.ldy) && (!p.keep[0] || (boxed(p.keep[0], p.ldk) && boxed(p.keep[1], p.ldk)));
+  for (int i = 0; i < 3 && a.boxes; ++i) {
+    void* at = i ? p.keep[i - 1] : p.y;
+    if (!at) continue;
+    const uint64_t stride = p.rows > 1 ? (uint64_t)(i ? p.ldk : p.ldy) * 2 : (uint64_t)ceil_div(outs, 8) * 16;
+    if (!tensor_map(&a.out[i], at, p.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, outs, p.rows, stride,
+                    MODE == kGated ? 64 : 128, kBoxTokens, CU_TENSOR_MAP_SWIZZLE_NONE))
       return DK_ERR_UNSUPPORTED;
   }
   if (pair) return p.bf16 ? launch_tiles<true, MODE, 2>(a, smem, grid, cluster, stream) : launch_tiles<false, MODE, 2>(a, smem, grid, cluster, stream);
