@@ -56,26 +56,15 @@ __device__ __forceinline__ float ld_cluster(uint32_t addr) {
   return v;
 }
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n .reg .pred p;\n"
-      " mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
-      " selp.u32 %0, 1, 0, p;\n}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // Every wait ends: after the library's limit the device's error word is set and
 // the CTA gives up.
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* give_up, int* error) {
-  if (try_wait_cluster(bar, parity)) return true;
+  if (mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = globaltimer_ns();
   for (int i = 0;; ++i) {
-    if (try_wait_cluster(bar, parity)) return true;
+    if (mbar_try_wait(bar, parity)) return true;
     if ((i & 15) == 15) {
       if (*give_up) return false;
       if (globaltimer_ns() - t0 > kWaitLimitNs) {
@@ -89,21 +78,10 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatil
 
 // The same without suspending the thread, for the one that issues the MMAs.
 __device__ __forceinline__ bool spin_bar(uint64_t* bar, uint32_t parity, volatile int* give_up, int* error) {
-  auto test = [&] {
-    uint32_t ok;
-    asm volatile(
-        "{\n .reg .pred p;\n"
-        " mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
-        " selp.u32 %0, 1, 0, p;\n}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
-  };
-  if (test()) return true;
+  if (mbar_test_wait(bar, parity)) return true;
   const uint64_t t0 = globaltimer_ns();
   for (int i = 0;; ++i) {
-    if (test()) return true;
+    if (mbar_test_wait(bar, parity)) return true;
     if ((i & 255) == 255) {
       if (*give_up) return false;
       if (globaltimer_ns() - t0 > kWaitLimitNs) {
@@ -331,9 +309,10 @@ __device__ __forceinline__ float gate_of(float g, int act, float& slope) {
 // ---------------------------------------------------------------------------
 enum Mode { kPlain, kGated, kTransposed };
 
-constexpr int kDqWarps = 8, kSumWarps = 4;
-constexpr int kCopyB = 12, kMmaWarp = 13, kCopyW = 14;
-constexpr int kGemmThreads = 15 * 32;
+constexpr int kDqGroups = 4, kDqWarps = 4 * kDqGroups, kSumWarps = 4;
+constexpr int kCopyB = kDqWarps + kSumWarps, kMmaWarp = kCopyB + 1, kCopyW = kCopyB + 2;
+constexpr int kGemmThreads = (kDqWarps + kSumWarps + 3) * 32;
+constexpr int kStepStride = kDqGroups / 2;  // of the steps that a warp unpacks
 constexpr int kLanes = 128;                // lanes a CTA
 constexpr int kStepDepth = 128;            // depth of a step: a group
 constexpr int kHalfDepth = 64;             // depth of a stage of A and B
@@ -464,12 +443,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kMaxStages; ++i) {
-      mbar_init(&full[i], kDqWarps / 2 * CG + 1);
+      mbar_init(&full[i], 4 * CG + 1);
       mbar_init(&free_[i], 1);
     }
     for (int i = 0; i < kMaxRaw; ++i) {
       mbar_init(&raw_full[i], 1);
-      mbar_init(&raw_free[i], kDqWarps);
+      mbar_init(&raw_free[i], 8);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sums_full[i], 1);
@@ -497,10 +476,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
 
   if (warp < kDqWarps) {
     // ---------------- unpacking ----------------
-    const int half = warp >> 2, quad = warp & 3, tile_lane = quad * 32 + lane;
+    const int half = warp >> 2 & 1, offset = warp >> 3, quad = warp & 3, tile_lane = quad * 32 + lane;
     const uint32_t full_leader = mapa(smem_u32(full), 0);
     const uint32_t scratch = base + L.scratch + warp * 256;
-    int raw = 0, raw_phase = 0, slot = half, phase = 0;
+    int raw = offset, raw_phase = 0, slot = 2 * offset + half, phase = 0;
     bool fresh = true;  // the stages have not been used yet
     int pending = -1;   // the stage that is on its way into tensor memory
     auto arrive = [&] {
@@ -522,8 +501,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
     // 64 lanes for each depth, the tile's second 64 lanes behind the first.
     const int a_row = MODE == kTransposed ? tile_lane & 63 : tile_lane;
     const uint32_t a_at = base + (MODE == kTransposed ? (tile_lane >> 6) * (kABytes / 2) : 0) + a_row * 128;
-    // Scales are asked for three steps before they are needed.
-    int f_item = item0, f_step = begin;
+    // Scales are asked for two turns before they are needed.
+    int f_item = item0, f_step = begin - kStepStride + offset;
     long long f_at;  // where the item's scales begin, -1 where it has none
     auto scales_at = [&](int item) -> long long {
       const int tile = item / a.token_tiles * CG + (CG == 2 ? (int)rank : 0);
@@ -532,10 +511,19 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
       return m < a.M ? (long long)m * a.groups : -1;
     };
     f_at = scales_at(item0);
+    auto ahead = [&] {
+      f_step += kStepStride;
+      while (f_step >= end && f_item < items) {
+        f_step -= end - begin;
+        f_item += item_step;
+        if (f_item < items) f_at = scales_at(f_item);
+      }
+    };
     const unsigned short* scales[2] = {reinterpret_cast<const unsigned short*>(a.scales[MODE == kGated ? lane >> 4 : 0]),
                                        reinterpret_cast<const unsigned short*>(a.scales[1])};
     auto fetch = [&]() -> uint32_t {
       uint32_t two = 0;
+      ahead();
       if (f_item < items) {
         if constexpr (MODE != kTransposed) {
           if (f_at >= 0) two = __ldg(scales[0] + f_at + f_step);
@@ -549,17 +537,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
             if (kATmem && m + 1 < a.M) two |= (uint32_t)__ldg(p + a.groups) << 16;
           }
         }
-        if (++f_step == end) {
-          f_step = begin;
-          f_item += item_step;
-          if (f_item < items) f_at = scales_at(f_item);
-        }
       }
       return two;
     };
-    uint32_t scale0 = fetch(), scale1 = fetch(), scale2 = fetch();
+    uint32_t scale0 = fetch(), scale1 = fetch();
     const int todo = (items - item0 + item_step - 1) / item_step * (end - begin);
-    for (int step = 0; step < todo; ++step) {
+    for (int step = offset; step < todo; step += kStepStride) {
       constexpr bool kTurn = MODE == kTransposed && kATmem;  // columns of W become lanes
       ScalePair<BF16> pair;
       const __half2 both = *reinterpret_cast<const __half2*>(&scale0);
@@ -573,8 +556,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
         __syncwarp();
       }
       scale0 = scale1;
-      scale1 = scale2;
-      scale2 = fetch();
+      scale1 = fetch();
       if (!__all_sync(0xffffffffu, wait_bar(&raw_full[raw], raw_phase, give_up, a.error))) break;
       uint32_t w[8];
       const uint32_t from = base + L.raw + raw * kRawBytes;
@@ -654,8 +636,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
       // The packed words were given back only after what was made of them had
       // been stored: a load whose value nobody has used yet may still be on its
       // way when the next copy lands.
-      if (++raw == a.raw_stages) raw = 0, raw_phase ^= 1;
-      slot += 2;
+      raw += kStepStride;
+      if (raw >= a.raw_stages) raw -= a.raw_stages, raw_phase ^= 1;
+      slot += 2 * kStepStride;
       if (slot >= a.stages) slot -= a.stages, phase ^= 1, fresh = false;
     }
     if (pending >= 0) arrive();
@@ -870,10 +853,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
   tcgen05_fence_after();
   if (CG == 1 && a.split > 1) {
     // The cluster's sums, added in the order of the depth, two tokens a thread.
-    if (warp < 12 && !*give_up) {
+    if (warp < kDqWarps + kSumWarps && !*give_up) {
       const int quad = warp & 3, tile_lane = quad * 32 + lane, item = item0;
       const int out = output_of<MODE, kATmem>(item / a.token_tiles, tile_lane), t0 = item % a.token_tiles * a.tokens;
-      for (int p = (int)rank * 3 + (warp >> 2); p < a.tokens / 2; p += a.split * 3) {
+      constexpr int kTeams = kDqGroups + 1;
+      for (int p = (int)rank * kTeams + (warp >> 2); p < a.tokens / 2; p += a.split * kTeams) {
         if (t0 + 2 * p >= a.rows) break;
         float v0 = 0.f, v1 = 0.f;
         const uint32_t at = base + (uint32_t)(2 * p * kLanes + tile_lane) * 4;
@@ -1005,7 +989,7 @@ dk_status product(const Product& p, cudaStream_t stream) {
     cluster = 2;
     grid = 2 * std::min((int64_t)pairs, (int64_t)a.lane_tiles * a.token_tiles);
     a.split = 1;
-    a.raw_stages = 3;
+    a.raw_stages = 4;
   } else {
     a.lane_tiles = tiles;
     a.tokens = std::max(16, ceil_div(p.rows, 16) * 16);
