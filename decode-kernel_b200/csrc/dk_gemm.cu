@@ -152,11 +152,11 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint3
 }
 // A stage of A with the lanes innermost, in the 128-byte swizzle: rows of 64
 // lanes (128 bytes), one for each depth, eight in an atom of 1024 bytes; the
-// other 64 lanes are half a stage (8192 bytes) away.
+// other 64 lanes are half a stage away.
 __device__ __forceinline__ uint64_t desc_lanes_inner(uint32_t addr) {
   uint64_t d = 0;
   d |= (uint64_t)((addr >> 4) & 0x3FFFu);
-  d |= (uint64_t)(8192 >> 4) << 16;
+  d |= (uint64_t)(16384 >> 4) << 16;
   d |= (uint64_t)(1024 >> 4) << 32;
   d |= (uint64_t)1 << 46;
   d |= (uint64_t)2 << 61;
@@ -315,12 +315,11 @@ constexpr int kGemmThreads = (kDqWarps + kSumWarps + 3) * 32;
 constexpr int kStepStride = kDqGroups / 2;  // of the steps that a warp unpacks
 constexpr int kLanes = 128;                // lanes a CTA
 constexpr int kStepDepth = 128;            // depth of a step: a group
-constexpr int kHalfDepth = 64;             // depth of a stage of A and B
+constexpr int kHalfDepth = 64;             // what a 128-byte row of A or B holds of it
 constexpr int kRawBytes = 128 * 64;        // packed weights of a step
-constexpr int kStages = 8;                 // of A in tensor memory, 32 columns each, with their stages of B
-constexpr int kAColumn = 256;              // A begins behind the sums
-constexpr int kABytes = 128 * kHalfDepth * 2;  // a stage of A in shared memory
-constexpr int kMaxStages = 8, kMaxRaw = 16;
+constexpr int kAColumn = 256;              // A in tensor memory: behind the sums, 64 columns a step
+constexpr int kABytes = kLanes * kStepDepth * 2;  // A of a step in shared memory
+constexpr int kMaxA = 4, kMaxB = 16, kMaxRaw = 16;
 constexpr int kMaxTokens = 256;
 constexpr int kSmemMost = 227 * 1024;
 // A CTA takes all of its SM's tensor memory, so two CTAs of these kernels must
@@ -339,7 +338,7 @@ struct alignas(64) TileArgs {
   int rows, M, K, groups, act;
   int lane_tiles, token_tiles, tokens;  // tokens: of a tile
   int steps, matrix_steps;              // all steps, those of one matrix (transposed: the second's follow)
-  int stages, raw_stages, split, boxes;  // boxes: results leave by TMA
+  int a_stages, b_stages, raw_stages, split, boxes;  // boxes: results leave by TMA
 };
 
 // Results on their way out: 32 tokens of a tile's outputs, twice.
@@ -347,17 +346,17 @@ constexpr int kBoxTokens = 32;
 constexpr int kBoxBytes = 3 * kBoxTokens * 64 * 2;  // h, g and u of 64 outputs; or y of 128
 
 struct GemmSmem {
-  int stage_bytes, raw, scratch, box, bars, total;
+  int b, raw, scratch, box, bars, total;
 };
-// Stages (A where it goes through shared memory, then B) from 0 on.
-__host__ __device__ inline GemmSmem gemm_smem(int a_bytes, int b_rows, int stages, int raw_stages) {
+// A's stages first, where it goes through shared memory.
+__host__ __device__ inline GemmSmem gemm_smem(int a_bytes, int b_rows, int b_stages, int raw_stages) {
   GemmSmem l;
-  l.stage_bytes = a_bytes + b_rows * 128;
-  l.raw = stages * l.stage_bytes;
+  l.b = a_bytes;
+  l.raw = l.b + b_stages * b_rows * 256;
   l.scratch = l.raw + raw_stages * kRawBytes;
   l.box = l.scratch + kDqWarps * 256;
   l.bars = l.box + 2 * kBoxBytes;
-  l.total = l.bars + (2 * kMaxStages + 2 * kMaxRaw + 6) * 8 + 16;
+  l.total = l.bars + (2 * kMaxA + 2 * kMaxB + 2 * kMaxRaw + 6) * 8 + 16;
   return l;
 }
 
@@ -422,13 +421,14 @@ __device__ __forceinline__ int output_of(int tile, int lane) {
 template <bool BF16, int MODE, int CG>
 __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant__ TileArgs a) {
   extern __shared__ __align__(1024) uint8_t smem[];
-  constexpr bool kATmem = CG == 1;           // where A lies
-  constexpr int kABase = kATmem ? 0 : kABytes;  // of B in its stage
+  constexpr bool kATmem = CG == 1;  // where A lies
   const int b_rows = a.tokens / CG;
-  const GemmSmem L = gemm_smem(kABase, b_rows, a.stages, a.raw_stages);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L.bars);  // A stored and B landed (the pair's, in its first CTA)
-  uint64_t* free_ = full + kMaxStages;       // MMAs have read them
-  uint64_t* raw_full = free_ + kMaxStages;   // packed weights landed
+  const GemmSmem L = gemm_smem(kATmem ? 0 : a.a_stages * kABytes, b_rows, a.b_stages, a.raw_stages);
+  uint64_t* a_full = reinterpret_cast<uint64_t*>(smem + L.bars);  // A stored (the pair's, in its first CTA)
+  uint64_t* a_free = a_full + kMaxA;         // MMAs have read it
+  uint64_t* b_full = a_free + kMaxA;         // tokens landed (the pair's, in its first CTA)
+  uint64_t* b_free = b_full + kMaxB;         // MMAs have read them
+  uint64_t* raw_full = b_free + kMaxB;       // packed weights landed
   uint64_t* raw_free = raw_full + kMaxRaw;   // unpacked
   uint64_t* sums_full = raw_free + kMaxRaw;  // a tile's MMAs are done; two places of sums for pairs
   uint64_t* sums_free = sums_full + 2;       // and its sums read (the pair's)
@@ -442,9 +442,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
   const uint32_t base = smem_u32(smem);
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kMaxStages; ++i) {
-      mbar_init(&full[i], 4 * CG + 1);
-      mbar_init(&free_[i], 1);
+    for (int i = 0; i < kMaxA; ++i) {
+      mbar_init(&a_full[i], 8 * CG);
+      mbar_init(&a_free[i], 1);
+    }
+    for (int i = 0; i < kMaxB; ++i) {
+      mbar_init(&b_full[i], 1);
+      mbar_init(&b_free[i], 1);
     }
     for (int i = 0; i < kMaxRaw; ++i) {
       mbar_init(&raw_full[i], 1);
@@ -477,19 +481,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
   if (warp < kDqWarps) {
     // ---------------- unpacking ----------------
     const int half = warp >> 2 & 1, offset = warp >> 3, quad = warp & 3, tile_lane = quad * 32 + lane;
-    const uint32_t full_leader = mapa(smem_u32(full), 0);
+    const uint32_t full_leader = mapa(smem_u32(a_full), 0);
     const uint32_t scratch = base + L.scratch + warp * 256;
-    int raw = offset, raw_phase = 0, slot = 2 * offset + half, phase = 0;
+    int raw = offset, raw_phase = 0, slot = offset, phase = 0;
     bool fresh = true;  // the stages have not been used yet
-    int pending = -1;   // the stage that is on its way into tensor memory
-    auto arrive = [&] {
-      tmem_st_wait();
-      tcgen05_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&full[pending]);
-      }
-    };
     // Where this lane's packed row lies in a step's copy, and of its four pieces
     // of 32 values the first of two.
     const int row = MODE == kPlain ? tile_lane
@@ -497,10 +492,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
                     : kATmem ? half * 64 + (lane >> 2)  // and every eighth after it
                              : half * 64 + (tile_lane & 63);
     const int piece = MODE == kTransposed ? 2 * (tile_lane >> 6) : 2 * half;
-    // A's row in shared memory: 64 values of the depth for each lane; transposed,
-    // 64 lanes for each depth, the tile's second 64 lanes behind the first.
-    const int a_row = MODE == kTransposed ? tile_lane & 63 : tile_lane;
-    const uint32_t a_at = base + (MODE == kTransposed ? (tile_lane >> 6) * (kABytes / 2) : 0) + a_row * 128;
+    // A in shared memory: rows of 64 of the depth for each lane, the step's other
+    // 64 behind them; transposed, rows of 64 lanes for each depth, the tile's
+    // other 64 lanes behind them.
+    const int a_row = MODE == kTransposed ? half * 64 + (tile_lane & 63) : tile_lane;
+    const uint32_t a_at = base + (MODE == kTransposed ? tile_lane >> 6 : half) * (kABytes / 2) + a_row * 128;
     // Scales are asked for two turns before they are needed.
     int f_item = item0, f_step = begin - kStepStride + offset;
     long long f_at;  // where the item's scales begin, -1 where it has none
@@ -573,75 +569,68 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
           w[i] = lds32(from + r * 64 + ((quad ^ ((r >> 1) & 3)) << 4) + (lane & 3) * 4);
         }
       }
-      if constexpr (!kATmem) {
-        if (!fresh && !__all_sync(0xffffffffu, wait_bar(&free_[slot], phase ^ 1, give_up, a.error))) break;
-        const uint32_t at = a_at + slot * L.stage_bytes;
+      if constexpr (kTurn) {
+        // An 8 x 8 transposition of nibbles over the lanes l, l ^ 4, l ^ 8, ..:
+        // row r's word with columns 0..7 becomes column r's with rows 0..7.
+        const bool b2 = lane & 16, b1 = lane & 8, b0 = lane & 4;
+        const uint32_t sel2 = b2 ? 0x3276u : 0x5410u, sel1 = b1 ? 0x3715u : 0x6240u, keep = b0 ? 0xF0F0F0F0u : 0x0F0F0F0Fu;
+        const uint32_t turn = b0 ? 28 : 4;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const uint32_t w4 = BF16 ? w[i] >> 4 : 0;
-          uint32_t o[4];
+          uint32_t x = w[i];
+          x = prmt(x, __shfl_xor_sync(0xffffffffu, x, 16), sel2);
+          x = prmt(x, __shfl_xor_sync(0xffffffffu, x, 8), sel1);
+          const uint32_t o = __shfl_xor_sync(0xffffffffu, x, 4);
+          w[i] = (x & keep) | (__funnelshift_l(o, o, turn) & ~keep);
+        }
+      }
+      uint32_t o[32];
 #pragma unroll
-          for (int b = 0; b < 4; ++b) o[b] = scaled<BF16>(exact_pair<BF16>(w[i], w4, b), pair);
-          sts128(at + ((i ^ (a_row & 7)) << 4), o);
+      for (int i = 0; i < 8; ++i) {
+        uint4 first4, rest4;
+        if constexpr (kTurn) {
+          first4 = lds128(scratch + i * 16);
+          if constexpr (BF16) rest4 = lds128(scratch + 128 + i * 16);
+        }
+        const uint32_t w4 = BF16 ? w[i] >> 4 : 0;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          if constexpr (kTurn) {
+            pair.first = b == 0 ? first4.x : b == 1 ? first4.y : b == 2 ? first4.z : first4.w;
+            if constexpr (BF16) pair.rest = b == 0 ? rest4.x : b == 1 ? rest4.y : b == 2 ? rest4.z : rest4.w;
+          }
+          o[4 * i + b] = scaled<BF16>(exact_pair<BF16>(w[i], w4, b), pair);
+        }
+      }
+      if (!fresh && !__all_sync(0xffffffffu, wait_bar(&a_free[slot], phase ^ 1, give_up, a.error))) break;
+      if constexpr (kATmem) {
+        tcgen05_fence_after();
+        tmem_st32(tmem + ((uint32_t)(quad * 32) << 16) + kAColumn + slot * 64 + half * 32, o);
+        tmem_st_wait();
+        tcgen05_fence_before();
+      } else {
+        const uint32_t at = a_at + slot * kABytes;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t q[4] = {o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]};
+          sts128(at + ((i ^ (a_row & 7)) << 4), q);
         }
         fence_async_shared();
-        __syncwarp();
-        if (lane == 0) {
-          arrive_cluster(full_leader + slot * 8);
-          mbar_arrive(&raw_free[raw]);
-        }
-      } else {
-        if constexpr (kTurn) {
-          // An 8 x 8 transposition of nibbles over the lanes l, l ^ 4, l ^ 8, ..:
-          // row r's word with columns 0..7 becomes column r's with rows 0..7.
-          const bool b2 = lane & 16, b1 = lane & 8, b0 = lane & 4;
-          const uint32_t sel2 = b2 ? 0x3276u : 0x5410u, sel1 = b1 ? 0x3715u : 0x6240u, keep = b0 ? 0xF0F0F0F0u : 0x0F0F0F0Fu;
-          const uint32_t turn = b0 ? 28 : 4;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            uint32_t x = w[i];
-            x = prmt(x, __shfl_xor_sync(0xffffffffu, x, 16), sel2);
-            x = prmt(x, __shfl_xor_sync(0xffffffffu, x, 8), sel1);
-            const uint32_t o = __shfl_xor_sync(0xffffffffu, x, 4);
-            w[i] = (x & keep) | (__funnelshift_l(o, o, turn) & ~keep);
-          }
-        }
-        uint32_t o[32];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          uint4 first4, rest4;
-          if constexpr (kTurn) {
-            first4 = lds128(scratch + i * 16);
-            if constexpr (BF16) rest4 = lds128(scratch + 128 + i * 16);
-          }
-          const uint32_t w4 = BF16 ? w[i] >> 4 : 0;
-#pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            if constexpr (kTurn) {
-              pair.first = b == 0 ? first4.x : b == 1 ? first4.y : b == 2 ? first4.z : first4.w;
-              if constexpr (BF16) pair.rest = b == 0 ? rest4.x : b == 1 ? rest4.y : b == 2 ? rest4.z : rest4.w;
-            }
-            o[4 * i + b] = scaled<BF16>(exact_pair<BF16>(w[i], w4, b), pair);
-          }
-        }
-        if (pending >= 0) arrive();  // the stage before, whose storing went on beside this one's unpacking
-        pending = -1;
-        if (!fresh && !__all_sync(0xffffffffu, wait_bar(&free_[slot], phase ^ 1, give_up, a.error))) break;
-        tcgen05_fence_after();
-        tmem_st32(tmem + ((uint32_t)(quad * 32) << 16) + kAColumn + slot * 32, o);
-        pending = slot;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&raw_free[raw]);
       }
-      // The packed words were given back only after what was made of them had
+      __syncwarp();
+      // The packed words are given back only now that what was made of them has
       // been stored: a load whose value nobody has used yet may still be on its
       // way when the next copy lands.
+      if (lane == 0) {
+        if constexpr (CG == 1) mbar_arrive(&a_full[slot]);
+        else arrive_cluster(full_leader + slot * 8);
+        mbar_arrive(&raw_free[raw]);
+      }
       raw += kStepStride;
       if (raw >= a.raw_stages) raw -= a.raw_stages, raw_phase ^= 1;
-      slot += 2 * kStepStride;
-      if (slot >= a.stages) slot -= a.stages, phase ^= 1, fresh = false;
+      slot += kStepStride;
+      if (slot >= a.a_stages) slot -= a.a_stages, phase ^= 1, fresh = false;
     }
-    if (pending >= 0) arrive();
   } else if (warp < kDqWarps + kSumWarps) {
     // ---------------- the sums ----------------
     const int quad = warp & 3, tile_lane = quad * 32 + lane;
@@ -729,34 +718,34 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
     if (lane == 0) {
       int slot = 0, phase = 0, issued = 0;
       bool going = true;
-      const uint32_t bytes = (uint32_t)b_rows * 128;
-      const uint32_t full_leader = mapa(smem_u32(full), 0);
+      const uint32_t bytes = (uint32_t)b_rows * 256;  // two boxes
+      const uint32_t full_leader = mapa(smem_u32(b_full), 0);
       for (int item = item0; item < items && going; item += item_step) {
         const int t0 = item % a.token_tiles * a.tokens + (CG == 2 ? (int)rank * b_rows : 0);
-        for (int n = 2 * begin; n < 2 * end; ++n) {
-          if (issued >= a.stages && !wait_bar(&free_[slot], phase ^ 1, give_up, a.error)) {
+        for (int s = begin; s < end; ++s) {
+          if (issued >= a.b_stages && !wait_bar(&b_free[slot], phase ^ 1, give_up, a.error)) {
             going = false;
             break;
           }
-          const int seg = MODE == kTransposed && (n >> 1) >= a.matrix_steps;
-          const int d = (n - 2 * seg * a.matrix_steps) * kHalfDepth;
-          const uint32_t dst = base + slot * L.stage_bytes + kABase;
+          const int seg = MODE == kTransposed && s >= a.matrix_steps;
+          const int d = (s - seg * a.matrix_steps) * kStepDepth;
+          const uint32_t dst = base + L.b + slot * bytes;
           if constexpr (CG == 1) {
-            mbar_arrive_expect_tx(&full[slot], bytes);
-            tma_2d(dst, &a.b[seg], d, t0, smem_u32(&full[slot]));
+            mbar_arrive_expect_tx(&b_full[slot], bytes);
+            tma_2d(dst, &a.b[seg], d, t0, smem_u32(&b_full[slot]));
+            tma_2d(dst + bytes / 2, &a.b[seg], d + kHalfDepth, t0, smem_u32(&b_full[slot]));
           } else {
-            if (first) mbar_arrive_expect_tx(&full[slot], 2 * bytes);
+            if (first) mbar_arrive_expect_tx(&b_full[slot], 2 * bytes);
             tma_2d_pair(dst, &a.b[seg], d, t0, full_leader + slot * 8);
+            tma_2d_pair(dst + bytes / 2, &a.b[seg], d + kHalfDepth, t0, full_leader + slot * 8);
           }
           ++issued;
-          if (++slot == a.stages) slot = 0, phase ^= 1;
+          if (++slot == a.b_stages) slot = 0, phase ^= 1;
         }
       }
-      if (!going) {
-        // What was asked for lands before the CTA ends; a stage whose A never
-        // came cannot say so, its wait ends by the clock.
+      if (!going && first) {  // what was asked for lands before the CTA ends
         volatile int none = 0;
-        for (int i = max(0, issued - a.stages); i < issued && first; ++i) wait_bar(&full[i % a.stages], (i / a.stages) & 1, &none, a.error);
+        for (int i = max(0, issued - a.b_stages); i < issued; ++i) wait_bar(&b_full[i % a.b_stages], (i / a.b_stages) & 1, &none, a.error);
       }
     }
     __syncwarp();
@@ -804,38 +793,43 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
       const uint32_t idesc = (1u << 4) | ((BF16 ? 1u : 0u) << 7) | ((BF16 ? 1u : 0u) << 10) |
                              ((MODE == kTransposed && !kATmem ? 1u : 0u) << 15) | ((uint32_t)(a.tokens >> 3) << 17) |
                              ((uint32_t)(kLanes * CG >> 4) << 24);
-      int slot = 0, phase = 0, tile = 0;
+      int slot = 0, phase = 0, a_slot = 0, a_phase = 0, tile = 0;
       bool going = true;
+      const uint32_t b_half = (uint32_t)b_rows * 128 >> 4;  // in the descriptors' units of 16 bytes
       for (int item = item0; item < items && going; item += item_step, ++tile) {
         const int place = CG == 1 ? 0 : tile & 1;
         if (CG == 2 && tile >= 2 && !__all_sync(0xffffffffu, spin_bar(&sums_free[place], ((tile >> 1) & 1) ^ 1, give_up, a.error))) break;
         tcgen05_fence_after();
         const uint32_t d = tmem + place * kMaxTokens;
-        for (int n = 2 * begin; n < 2 * end; ++n) {
-          going = spin_bar(&full[slot], phase, give_up, a.error);
+        for (int s = begin; s < end; ++s) {
+          going = spin_bar(&b_full[slot], phase, give_up, a.error) && spin_bar(&a_full[a_slot], a_phase, give_up, a.error);
           if (!__all_sync(0xffffffffu, going)) {
             going = false;
             break;
           }
           tcgen05_fence_after();
-          const uint32_t at = base + slot * L.stage_bytes;
-          const uint64_t b0 = umma_desc_k_sw128(at + kABase);
+          const uint64_t b0 = umma_desc_k_sw128(base + L.b + slot * (uint32_t)b_rows * 256);
           if (elect_one()) {
             if constexpr (kATmem) {
-              const uint32_t a0 = tmem + kAColumn + slot * 32;
+              const uint32_t a0 = tmem + kAColumn + a_slot * 64;
 #pragma unroll
-              for (int k = 0; k < 4; ++k) mma_ts<CG>(d, a0 + k * 8, b0 + k * 2, idesc, n > 2 * begin || k > 0);
+              for (int k = 0; k < 8; ++k) mma_ts<CG>(d, a0 + k * 8, b0 + (k >> 2) * b_half + (k & 3) * 2, idesc, s > begin || k > 0);
             } else {
               // 16 of the depth: 32 bytes on in a row, or 16 rows on.
+              const uint32_t at = base + a_slot * kABytes;
               const uint64_t a0 = MODE == kTransposed ? desc_lanes_inner(at) : umma_desc_k_sw128(at);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) mma_ss<CG>(d, a0 + k * (MODE == kTransposed ? 128 : 2), b0 + k * 2, idesc, n > 2 * begin || k > 0);
+              for (int k = 0; k < 8; ++k)
+                mma_ss<CG>(d, a0 + (MODE == kTransposed ? k * 128 : (k >> 2) * (kABytes / 2 >> 4) + (k & 3) * 2), b0 + (k >> 2) * b_half + (k & 3) * 2,
+                           idesc, s > begin || k > 0);
             }
-            mma_commit<CG>(&free_[slot]);
-            if (n + 1 == 2 * end) mma_commit<CG>(&sums_full[place]);
+            mma_commit<CG>(&a_free[a_slot]);
+            mma_commit<CG>(&b_free[slot]);
+            if (s + 1 == end) mma_commit<CG>(&sums_full[place]);
           }
           __syncwarp();
-          if (++slot == a.stages) slot = 0, phase ^= 1;
+          if (++a_slot == a.a_stages) a_slot = 0, a_phase ^= 1;
+          if (++slot == a.b_stages) slot = 0, phase ^= 1;
         }
       }
       // Every MMA is done before the tensor memory is given back.
@@ -1002,9 +996,11 @@ dk_status product(const Product& p, cudaStream_t stream) {
     a.raw_stages = 8;
   }
   if ((int64_t)a.lane_tiles * a.token_tiles > INT32_MAX / 4) return DK_ERR_UNSUPPORTED;
-  const int b_rows = a.tokens / (pair ? 2 : 1), a_bytes = pair ? kABytes : 0;
-  a.stages = pair ? std::min(kMaxStages, (kSmemMost - gemm_smem(0, 0, 0, a.raw_stages).total) / (a_bytes + b_rows * 128)) : kStages;
-  const GemmSmem l = gemm_smem(a_bytes, b_rows, a.stages, a.raw_stages);
+  const int b_rows = a.tokens / (pair ? 2 : 1);
+  a.a_stages = pair ? 2 : kMaxA;
+  const int a_bytes = pair ? a.a_stages * kABytes : 0;
+  a.b_stages = std::min(pair ? 8 : kMaxB, (kSmemMost - gemm_smem(a_bytes, 0, 0, a.raw_stages).total) / (b_rows * 256));
+  const GemmSmem l = gemm_smem(a_bytes, b_rows, a.b_stages, a.raw_stages);
   const size_t smem = std::max<size_t>(l.total, kSmemLeast);
 
   for (int i = 0; i < p.matrices; ++i) {
