@@ -75,22 +75,27 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatil
     }
   }
 }
-
-// The same without suspending the thread, for the one that issues the MMAs.
-__device__ __forceinline__ bool spin_bar(uint64_t* bar, uint32_t parity, volatile int* give_up, int* error) {
-  if (mbar_test_wait(bar, parity)) return true;
-  const uint64_t t0 = globaltimer_ns();
-  for (int i = 0;; ++i) {
-    if (mbar_test_wait(bar, parity)) return true;
-    if ((i & 255) == 255) {
-      if (*give_up) return false;
+// A warp's wait.  All lanes ask (one that asks for all costs the others a vote
+// more: 1.4 times the time of whole products).
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* give_up, int* error) {
+  return __all_sync(0xffffffffu, wait_bar(bar, parity, give_up, error));
+}
+// The same without suspending, for the warp that issues the MMAs.
+__device__ __forceinline__ bool warp_spin(uint64_t* bar, uint32_t parity, volatile int* give_up, int* error) {
+  bool ok = mbar_test_wait(bar, parity);
+  if (!ok) {
+    const uint64_t t0 = globaltimer_ns();
+    for (int i = 0; !(ok = mbar_test_wait(bar, parity)); ++i) {
+      if ((i & 255) != 255) continue;
+      if (*give_up) break;
       if (globaltimer_ns() - t0 > kWaitLimitNs) {
         if (error) atomicExch(error, kDevWaitTimeout);
         *give_up = 1;
-        return false;
+        break;
       }
     }
   }
+  return __all_sync(0xffffffffu, ok);
 }
 
 __device__ __forceinline__ void tma_2d(uint32_t dst, const void* map, int c0, int c1, uint32_t bar) {
@@ -150,9 +155,9 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint3
         "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
         : "memory");
 }
-// A stage of A with the lanes innermost, in the 128-byte swizzle: rows of 64
-// lanes (128 bytes), one for each depth, eight in an atom of 1024 bytes; the
-// other 64 lanes are half a stage away.
+// A of a step with the lanes innermost, in the 128-byte swizzle: rows of 64 lanes
+// (128 bytes), one for each depth, eight in an atom of 1024 bytes; the other 64
+// lanes are 16 KB away.
 __device__ __forceinline__ uint64_t desc_lanes_inner(uint32_t addr) {
   uint64_t d = 0;
   d |= (uint64_t)((addr >> 4) & 0x3FFFu);
@@ -317,10 +322,25 @@ constexpr int kLanes = 128;                // lanes a CTA
 constexpr int kStepDepth = 128;            // depth of a step: a group
 constexpr int kHalfDepth = 64;             // what a 128-byte row of A or B holds of it
 constexpr int kRawBytes = 128 * 64;        // packed weights of a step
-constexpr int kAColumn = 256;              // A in tensor memory: behind the sums, 64 columns a step
+// Where a step's A goes, and how tensor memory's 512 columns are shared.
+// A in tensor memory: a pair's sums twice, so that one tile's are read while the
+// next one's grow (or once, of wider tiles), then A of two steps, 64 columns
+// each; a single CTA's sums, then A of four.
+// The transposed product of pairs has A in shared memory, where it may lie with
+// the lanes innermost, as it was packed: 1.05 thousand cycles a step against 1.4
+// thousand where warps turn it for tensor memory.  The others gain by tensor
+// memory, since shared memory's bandwidth (128 bytes a cycle) then has to carry B
+// and the packed words only: 650 cycles a step of 160 tokens instead of 870.
+template <int MODE, int CG>
+struct Place {
+  static constexpr bool kATmem = CG == 1 || MODE != kTransposed;
+  static constexpr int kSums = CG == 2 && kATmem ? 192 : 256;  // columns of a tile's sums
+  static constexpr int kA = CG == 1 ? 256 : 384;
+  static constexpr int kABits = CG == 1 ? 2 : 1;
+};
 constexpr int kABytes = kLanes * kStepDepth * 2;  // A of a step in shared memory
-constexpr int kMaxA = 4, kMaxB = 16, kMaxRaw = 16;
-constexpr int kMaxTokens = 256;
+constexpr int kMaxA = 4, kMaxB = 16, kMaxRaw = 8;
+constexpr int kDone = 16;                  // steps whose end is remembered: no fewer than B's stages
 constexpr int kSmemMost = 227 * 1024;
 // A CTA takes all of its SM's tensor memory, so two CTAs of these kernels must
 // not share an SM: one would wait for the other's columns, and where clusters do
@@ -338,17 +358,18 @@ struct alignas(64) TileArgs {
   int rows, M, K, groups, act;
   int lane_tiles, token_tiles, tokens;  // tokens: of a tile
   int steps, matrix_steps;              // all steps, those of one matrix (transposed: the second's follow)
-  int a_stages, b_stages, raw_stages, split, boxes;  // boxes: results leave by TMA
+  int places;                           // of sums
+  int b_stages, raw_stages, split, boxes;  // boxes: results leave by TMA
 };
 
 // Results on their way out: 32 tokens of a tile's outputs, twice.
 constexpr int kBoxTokens = 32;
 constexpr int kBoxBytes = 3 * kBoxTokens * 64 * 2;  // h, g and u of 64 outputs; or y of 128
 
+// A's stages first, where it has any.
 struct GemmSmem {
   int b, raw, scratch, box, bars, total;
 };
-// A's stages first, where it goes through shared memory.
 __host__ __device__ inline GemmSmem gemm_smem(int a_bytes, int b_rows, int b_stages, int raw_stages) {
   GemmSmem l;
   l.b = a_bytes;
@@ -356,7 +377,7 @@ __host__ __device__ inline GemmSmem gemm_smem(int a_bytes, int b_rows, int b_sta
   l.scratch = l.raw + raw_stages * kRawBytes;
   l.box = l.scratch + kDqWarps * 256;
   l.bars = l.box + 2 * kBoxBytes;
-  l.total = l.bars + (2 * kMaxA + 2 * kMaxB + 2 * kMaxRaw + 6) * 8 + 16;
+  l.total = l.bars + (kMaxA + kMaxB + 2 * kMaxRaw + kDone + 6) * 8 + 16;
   return l;
 }
 
@@ -421,14 +442,15 @@ __device__ __forceinline__ int output_of(int tile, int lane) {
 template <bool BF16, int MODE, int CG>
 __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant__ TileArgs a) {
   extern __shared__ __align__(1024) uint8_t smem[];
-  constexpr bool kATmem = CG == 1;  // where A lies
+  using At = Place<MODE, CG>;
+  constexpr bool kATmem = At::kATmem;
   const int b_rows = a.tokens / CG;
-  const GemmSmem L = gemm_smem(kATmem ? 0 : a.a_stages * kABytes, b_rows, a.b_stages, a.raw_stages);
+  const GemmSmem L = gemm_smem(kATmem ? 0 : 2 * kABytes, b_rows, a.b_stages, a.raw_stages);
+  // Step t of this CTA's line uses place t modulo the ring's size of each ring.
   uint64_t* a_full = reinterpret_cast<uint64_t*>(smem + L.bars);  // A stored (the pair's, in its first CTA)
-  uint64_t* a_free = a_full + kMaxA;         // MMAs have read it
-  uint64_t* b_full = a_free + kMaxA;         // tokens landed (the pair's, in its first CTA)
-  uint64_t* b_free = b_full + kMaxB;         // MMAs have read them
-  uint64_t* raw_full = b_free + kMaxB;       // packed weights landed
+  uint64_t* b_full = a_full + kMaxA;         // tokens landed (the pair's, in its first CTA)
+  uint64_t* done = b_full + kMaxB;           // the step's MMAs are done: A and B have been read
+  uint64_t* raw_full = done + kDone;         // packed weights landed
   uint64_t* raw_free = raw_full + kMaxRaw;   // unpacked
   uint64_t* sums_full = raw_free + kMaxRaw;  // a tile's MMAs are done; two places of sums for pairs
   uint64_t* sums_free = sums_full + 2;       // and its sums read (the pair's)
@@ -441,27 +463,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
   const bool first = CG == 1 || rank == 0;
   const uint32_t base = smem_u32(smem);
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < kMaxA; ++i) {
-      mbar_init(&a_full[i], 8 * CG);
-      mbar_init(&a_free[i], 1);
-    }
-    for (int i = 0; i < kMaxB; ++i) {
-      mbar_init(&b_full[i], 1);
-      mbar_init(&b_free[i], 1);
-    }
-    for (int i = 0; i < kMaxRaw; ++i) {
-      mbar_init(&raw_full[i], 1);
-      mbar_init(&raw_free[i], 8);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&sums_full[i], 1);
-      mbar_init(&sums_free[i], kSumWarps * CG);
-    }
-    mbar_init(drained, 1);
-    *give_up = 0;
+  constexpr int kBars = kMaxA + kMaxB + kDone + 2 * kMaxRaw + 5;
+  if (threadIdx.x < kBars) {
+    uint64_t* bar = a_full + threadIdx.x;
+    const int count = bar < b_full ? 8 * CG : bar < raw_free ? 1 : bar < sums_full ? 8 : bar < sums_free ? 1 : bar < drained ? kSumWarps * CG : 1;
+    mbar_init(bar, count);
     fence_barrier_init();
   }
+  if (threadIdx.x == 0) *give_up = 0;
   if (warp == kMmaWarp) tmem_take<CG>(smem_u32(tmem_slot));
   tcgen05_fence_before();
   __syncthreads();
@@ -483,8 +492,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
     const int half = warp >> 2 & 1, offset = warp >> 3, quad = warp & 3, tile_lane = quad * 32 + lane;
     const uint32_t full_leader = mapa(smem_u32(a_full), 0);
     const uint32_t scratch = base + L.scratch + warp * 256;
-    int raw = offset, raw_phase = 0, slot = offset, phase = 0;
-    bool fresh = true;  // the stages have not been used yet
+    constexpr int kRawBits = CG == 1 ? 3 : 2, kABits = At::kABits;
     // Where this lane's packed row lies in a step's copy, and of its four pieces
     // of 32 values the first of two.
     const int row = MODE == kPlain ? tile_lane
@@ -492,11 +500,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
                     : kATmem ? half * 64 + (lane >> 2)  // and every eighth after it
                              : half * 64 + (tile_lane & 63);
     const int piece = MODE == kTransposed ? 2 * (tile_lane >> 6) : 2 * half;
-    // A in shared memory: rows of 64 of the depth for each lane, the step's other
-    // 64 behind them; transposed, rows of 64 lanes for each depth, the tile's
+    // Transposed A in shared memory: rows of 64 lanes for each depth, the tile's
     // other 64 lanes behind them.
-    const int a_row = MODE == kTransposed ? half * 64 + (tile_lane & 63) : tile_lane;
-    const uint32_t a_at = base + (MODE == kTransposed ? tile_lane >> 6 : half) * (kABytes / 2) + a_row * 128;
+    const uint32_t a_at = base + (tile_lane >> 6) * (kABytes / 2) + row * 128;
     // Scales are asked for two turns before they are needed.
     int f_item = item0, f_step = begin - kStepStride + offset;
     long long f_at;  // where the item's scales begin, -1 where it has none
@@ -539,6 +545,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
     uint32_t scale0 = fetch(), scale1 = fetch();
     const int todo = (items - item0 + item_step - 1) / item_step * (end - begin);
     for (int step = offset; step < todo; step += kStepStride) {
+      const int raw = step & ((1 << kRawBits) - 1), slot = step & ((1 << kABits) - 1);
       constexpr bool kTurn = MODE == kTransposed && kATmem;  // columns of W become lanes
       ScalePair<BF16> pair;
       const __half2 both = *reinterpret_cast<const __half2*>(&scale0);
@@ -553,7 +560,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
       }
       scale0 = scale1;
       scale1 = fetch();
-      if (!__all_sync(0xffffffffu, wait_bar(&raw_full[raw], raw_phase, give_up, a.error))) break;
+      if (!warp_wait(&raw_full[raw], step >> kRawBits & 1, give_up, a.error)) break;
       uint32_t w[8];
       const uint32_t from = base + L.raw + raw * kRawBytes;
       if constexpr (!kTurn) {
@@ -602,10 +609,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
           o[4 * i + b] = scaled<BF16>(exact_pair<BF16>(w[i], w4, b), pair);
         }
       }
-      if (!fresh && !__all_sync(0xffffffffu, wait_bar(&a_free[slot], phase ^ 1, give_up, a.error))) break;
+      const int before = step - (1 << kABits);  // the step whose place in the ring this one takes
+      if (before >= 0 && !warp_wait(&done[before % kDone], before / kDone & 1, give_up, a.error)) break;
       if constexpr (kATmem) {
         tcgen05_fence_after();
-        tmem_st32(tmem + ((uint32_t)(quad * 32) << 16) + kAColumn + slot * 64 + half * 32, o);
+        tmem_st32(tmem + ((uint32_t)(quad * 32) << 16) + At::kA + slot * 64 + half * 32, o);
         tmem_st_wait();
         tcgen05_fence_before();
       } else {
@@ -613,7 +621,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const uint32_t q[4] = {o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]};
-          sts128(at + ((i ^ (a_row & 7)) << 4), q);
+          sts128(at + ((i ^ (row & 7)) << 4), q);
         }
         fence_async_shared();
       }
@@ -626,10 +634,6 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
         else arrive_cluster(full_leader + slot * 8);
         mbar_arrive(&raw_free[raw]);
       }
-      raw += kStepStride;
-      if (raw >= a.raw_stages) raw -= a.raw_stages, raw_phase ^= 1;
-      slot += kStepStride;
-      if (slot >= a.a_stages) slot -= a.a_stages, phase ^= 1, fresh = false;
     }
   } else if (warp < kDqWarps + kSumWarps) {
     // ---------------- the sums ----------------
@@ -641,9 +645,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
     int phase = 0, turn = 0, place = 0;
     for (int item = item0; item < items; item += item_step) {
       // All four warps go on or none does: they meet at barriers.
-      if (!barrier_all(1, kSumWarps * 32, wait_bar(&sums_full[place], phase, give_up, a.error))) break;
+      if (!barrier_all(1, kSumWarps * 32, warp_wait(&sums_full[place], phase, give_up, a.error))) break;
       tcgen05_fence_after();
-      const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + place * kMaxTokens;
+      const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + place * At::kSums;
       const int tile = item / a.token_tiles * CG + (CG == 2 ? (int)rank : 0);
       const int t0 = item % a.token_tiles * a.tokens, out = output_of<MODE, kATmem>(tile, tile_lane);
       for (int c = 0; c < a.tokens; c += kBoxTokens) {
@@ -707,7 +711,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
           }
         }
       }
-      if (CG == 1 || (place ^= 1) == 0) phase ^= 1;
+      if (a.places == 1 || (place ^= 1) == 0) phase ^= 1;
     }
     if (issuer) bulk_wait_all();
     // The pair's second CTA stays until the first one's last signal is here.
@@ -716,14 +720,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
   } else if (warp == kCopyB) {
     // ---------------- copies of the tokens ----------------
     if (lane == 0) {
-      int slot = 0, phase = 0, issued = 0;
+      int slot = 0, issued = 0;
       bool going = true;
       const uint32_t bytes = (uint32_t)b_rows * 256;  // two boxes
       const uint32_t full_leader = mapa(smem_u32(b_full), 0);
       for (int item = item0; item < items && going; item += item_step) {
         const int t0 = item % a.token_tiles * a.tokens + (CG == 2 ? (int)rank * b_rows : 0);
         for (int s = begin; s < end; ++s) {
-          if (issued >= a.b_stages && !wait_bar(&b_free[slot], phase ^ 1, give_up, a.error)) {
+          const int before = issued - a.b_stages;
+          if (before >= 0 && !wait_bar(&done[before % kDone], before / kDone & 1, give_up, a.error)) {
             going = false;
             break;
           }
@@ -740,7 +745,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
             tma_2d_pair(dst + bytes / 2, &a.b[seg], d + kHalfDepth, t0, full_leader + slot * 8);
           }
           ++issued;
-          if (++slot == a.b_stages) slot = 0, phase ^= 1;
+          if (++slot == a.b_stages) slot = 0;
         }
       }
       if (!going && first) {  // what was asked for lands before the CTA ends
@@ -788,47 +793,40 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
     // The whole warp goes along, so that the operands stay in uniform registers;
     // one thread issues.
     if (first) {
-      // fp32 sums, A and B fp16 (0) or bf16 (1), B with the depth innermost, A
-      // too but for the transposed product's, whose lanes are innermost.
-      const uint32_t idesc = (1u << 4) | ((BF16 ? 1u : 0u) << 7) | ((BF16 ? 1u : 0u) << 10) |
-                             ((MODE == kTransposed && !kATmem ? 1u : 0u) << 15) | ((uint32_t)(a.tokens >> 3) << 17) |
+      // fp32 sums, A and B fp16 (0) or bf16 (1), the depth innermost but for an A
+      // in shared memory.
+      const uint32_t idesc = (1u << 4) | ((BF16 ? 1u : 0u) << 7) | ((BF16 ? 1u : 0u) << 10) | ((kATmem ? 0u : 1u) << 15) | ((uint32_t)(a.tokens >> 3) << 17) |
                              ((uint32_t)(kLanes * CG >> 4) << 24);
-      int slot = 0, phase = 0, a_slot = 0, a_phase = 0, tile = 0;
+      int slot = 0, phase = 0, step = 0, tile = 0;
+      constexpr int kABits = At::kABits;
       bool going = true;
       const uint32_t b_half = (uint32_t)b_rows * 128 >> 4;  // in the descriptors' units of 16 bytes
       for (int item = item0; item < items && going; item += item_step, ++tile) {
-        const int place = CG == 1 ? 0 : tile & 1;
-        if (CG == 2 && tile >= 2 && !__all_sync(0xffffffffu, spin_bar(&sums_free[place], ((tile >> 1) & 1) ^ 1, give_up, a.error))) break;
+        const int place = a.places == 2 ? tile & 1 : 0, before = tile - a.places;  // the tile whose sums were there
+        if (before >= 0 && !warp_wait(&sums_free[place], (a.places == 2 ? before >> 1 : before) & 1, give_up, a.error)) break;
         tcgen05_fence_after();
-        const uint32_t d = tmem + place * kMaxTokens;
+        const uint32_t d = tmem + place * At::kSums;
         for (int s = begin; s < end; ++s) {
-          going = spin_bar(&b_full[slot], phase, give_up, a.error) && spin_bar(&a_full[a_slot], a_phase, give_up, a.error);
-          if (!__all_sync(0xffffffffu, going)) {
-            going = false;
-            break;
-          }
+          const int a_slot = step & ((1 << kABits) - 1);
+          going = warp_spin(&b_full[slot], phase, give_up, a.error) && warp_spin(&a_full[a_slot], step >> kABits & 1, give_up, a.error);
+          if (!going) break;
           tcgen05_fence_after();
           const uint64_t b0 = umma_desc_k_sw128(base + L.b + slot * (uint32_t)b_rows * 256);
           if (elect_one()) {
             if constexpr (kATmem) {
-              const uint32_t a0 = tmem + kAColumn + a_slot * 64;
+              const uint32_t a0 = tmem + At::kA + a_slot * 64;
 #pragma unroll
               for (int k = 0; k < 8; ++k) mma_ts<CG>(d, a0 + k * 8, b0 + (k >> 2) * b_half + (k & 3) * 2, idesc, s > begin || k > 0);
             } else {
-              // 16 of the depth: 32 bytes on in a row, or 16 rows on.
-              const uint32_t at = base + a_slot * kABytes;
-              const uint64_t a0 = MODE == kTransposed ? desc_lanes_inner(at) : umma_desc_k_sw128(at);
+              const uint64_t a0 = desc_lanes_inner(base + a_slot * kABytes);  // 16 rows further each
 #pragma unroll
-              for (int k = 0; k < 8; ++k)
-                mma_ss<CG>(d, a0 + (MODE == kTransposed ? k * 128 : (k >> 2) * (kABytes / 2 >> 4) + (k & 3) * 2), b0 + (k >> 2) * b_half + (k & 3) * 2,
-                           idesc, s > begin || k > 0);
+              for (int k = 0; k < 8; ++k) mma_ss<CG>(d, a0 + k * 128, b0 + (k >> 2) * b_half + (k & 3) * 2, idesc, s > begin || k > 0);
             }
-            mma_commit<CG>(&a_free[a_slot]);
-            mma_commit<CG>(&b_free[slot]);
+            mma_commit<CG>(&done[step % kDone]);
             if (s + 1 == end) mma_commit<CG>(&sums_full[place]);
           }
           __syncwarp();
-          if (++a_slot == a.a_stages) a_slot = 0, a_phase ^= 1;
+          ++step;
           if (++slot == a.b_stages) slot = 0, phase ^= 1;
         }
       }
@@ -971,14 +969,20 @@ dk_status product(const Product& p, cudaStream_t stream) {
   if (pair) {
     a.lane_tiles = (tiles + 1) / 2;
     const int pairs = sms / 2;
-    // The width of the token tiles (a multiple of 32 up to 256) that leaves the
-    // least to do for the busiest pair.
+    // The width of the token tiles (a multiple of 32) that leaves the least to do
+    // for the busiest pair.  In cycles, as measured: a step takes 4 a token, and no
+    // less than its unpacking or its way through shared memory; where the sums
+    // have one place only, the next tile waits until they are read.
+    using At = Place<MODE, 2>;
     long long best = 0;
-    for (int n = ceil_div(p.rows, kMaxTokens); n <= ceil_div(p.rows, 128); ++n) {
-      const int width = std::min(kMaxTokens, ceil_div(ceil_div(p.rows, n), 32) * 32);
-      const long long cost = (long long)ceil_div((int64_t)a.lane_tiles * ceil_div(p.rows, width), pairs) * (width + 16);
-      if (!best || cost < best) best = cost, a.tokens = width;
+    for (int width = 64; width <= 256; width += 32) {
+      const long long tiles_each = ceil_div((int64_t)a.lane_tiles * ceil_div(p.rows, width), pairs);
+      const int step = At::kATmem ? std::max(4 * width, 650) : std::max(4 * width, 640 + 2 * width);
+      const int read = 20 * width, wait = width > At::kSums ? read : 0;
+      const long long cost = tiles_each * ((long long)a.steps * step + wait) + read;
+      if (!best || cost <= best) best = cost, a.tokens = width;
     }
+    a.places = a.tokens > At::kSums ? 1 : 2;
     a.token_tiles = ceil_div(p.rows, a.tokens);
     cluster = 2;
     grid = 2 * std::min((int64_t)pairs, (int64_t)a.lane_tiles * a.token_tiles);
@@ -994,11 +998,11 @@ dk_status product(const Product& p, cudaStream_t stream) {
     if ((int64_t)tiles * a.split > INT32_MAX) return DK_ERR_UNSUPPORTED;
     grid = (unsigned)tiles * a.split;
     a.raw_stages = 8;
+    a.places = 1;
   }
   if ((int64_t)a.lane_tiles * a.token_tiles > INT32_MAX / 4) return DK_ERR_UNSUPPORTED;
   const int b_rows = a.tokens / (pair ? 2 : 1);
-  a.a_stages = pair ? 2 : kMaxA;
-  const int a_bytes = pair ? a.a_stages * kABytes : 0;
+  const int a_bytes = !pair || Place<MODE, 2>::kATmem ? 0 : 2 * kABytes;
   a.b_stages = std::min(pair ? 8 : kMaxB, (kSmemMost - gemm_smem(a_bytes, 0, 0, a.raw_stages).total) / (b_rows * 256));
   const GemmSmem l = gemm_smem(a_bytes, b_rows, a.b_stages, a.raw_stages);
   const size_t smem = std::max<size_t>(l.total, kSmemLeast);
