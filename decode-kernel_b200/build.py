@@ -32,7 +32,7 @@ INCLUDE = REPO / "include"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 LIB_SOURCES = ["dk_abi.cu", "dk_gemv.cu", "dk_stream.cu", "dk_quant.cu", "dk_shard.cu",
                "dk_cache.cu", "dk_attend.cu", "dk_norm.cu", "dk_gemm.cu", "dk_rotary.cu", "dk_read.cu"]
-COMMON_DEPS = [CSRC / "dk_device.cuh", CSRC / "dk_host.h", CSRC / "dk_batch.cuh", INCLUDE / "dk_w4a16.h"]
+COMMON_DEPS = [CSRC / "dk_device.cuh", CSRC / "dk_host.h", CSRC / "dk_batch.cuh", CSRC / "dk_few.cuh", INCLUDE / "dk_w4a16.h"]
 LIB = PKG / "libdk_b200.so"
 
 

@@ -689,6 +689,12 @@ std::tuple<torch::Tensor, OptTensor, OptTensor> w4a16_gemm(torch::Tensor packed,
   a.rows = static_cast<int>(xr.size(0));
   a.M = static_cast<int>(w.M);
   a.K = static_cast<int>(w.K);
+  torch::Tensor workspace;
+  if (const size_t need = dk_w4a16_gemm_workspace_bytes(a.rows, a.K, a.dtype)) {
+    workspace = torch::empty({static_cast<int64_t>(need)}, x.options().dtype(torch::kUInt8));
+    a.workspace = workspace.data_ptr();
+    a.workspace_bytes = need;
+  }
   check_status(dk_w4a16_gemm(&a, at::cuda::getCurrentCUDAStream().stream()), "w4a16_gemm");
   return {y, g, u};
 }

@@ -399,8 +399,8 @@ __device__ __forceinline__ uint32_t rounded2(float lo, float hi) {
 }
 
 // Two columns (tokens t, t + 1) of this thread's lane: to y.
-template <bool BF16, int MODE>
-__device__ __forceinline__ void finish(const TileArgs& a, int lane_row, int out, int t, float v0, float v1) {
+template <bool BF16, int MODE, typename Args>
+__device__ __forceinline__ void finish(const Args& a, int lane_row, int out, int t, float v0, float v1) {
   using V = Value<BF16>;
   V* y = static_cast<V*>(a.y);
   if constexpr (MODE == kGated) {
@@ -528,15 +528,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
       ahead();
       if (f_item < items) {
         if constexpr (MODE != kTransposed) {
-          if (f_at >= 0) two = __ldg(scales[0] + f_at + f_step);
+          if (f_at >= 0) two = scales[0][f_at + f_step];
         } else {
           // A in tensor memory: lane l brings the scales of depths 2 l and 2 l + 1; else its row's.
           const int seg = f_step >= a.matrix_steps;
           const int m = (f_step - seg * a.matrix_steps) * kStepDepth + half * 64 + (kATmem ? 2 * lane : tile_lane & 63);
           if (f_at >= 0) {
             const unsigned short* p = scales[seg] + f_at + (long long)m * a.groups;
-            if (m < a.M) two = __ldg(p);
-            if (kATmem && m + 1 < a.M) two |= (uint32_t)__ldg(p + a.groups) << 16;
+            if (m < a.M) two = *p;
+            if (kATmem && m + 1 < a.M) two |= (uint32_t)p[a.groups] << 16;
           }
         }
       }
@@ -866,6 +866,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
   if (warp == kMmaWarp) tmem_give<CG>(tmem);
 }
 
+#include "dk_few.cuh"
+
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
@@ -900,21 +902,27 @@ struct Product {
   int64_t ldx, ldy, ldk;
   int rows, M, K, matrices, act;
   bool bf16;
+  void* workspace;
 };
 
-template <bool BF16, int MODE, int CG>
-dk_status launch_tiles(TileArgs& a, size_t smem, unsigned grid, int cluster, cudaStream_t stream) {
-  auto kernel = k_gemm<BF16, MODE, CG>;
-  static std::atomic<unsigned long long> done{0};  // devices on which the kernel may use the shared memory
+// A kernel's first use on a device: its shared memory.
+template <typename Kernel>
+dk_status allow_smem(Kernel kernel, std::atomic<unsigned long long>& done) {
   const unsigned long long bit = 1ull << (current_device() & 63);
-  if (!(done.load(std::memory_order_acquire) & bit)) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
-    if (e != cudaSuccess) {
-      set_cuda_error(e, "cudaFuncSetAttribute");
-      return DK_ERR_CUDA;
-    }
-    done.fetch_or(bit, std::memory_order_acq_rel);
+  if (done.load(std::memory_order_acquire) & bit) return DK_OK;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
+  if (e != cudaSuccess) {
+    set_cuda_error(e, "cudaFuncSetAttribute");
+    return DK_ERR_CUDA;
   }
+  done.fetch_or(bit, std::memory_order_acq_rel);
+  return DK_OK;
+}
+
+inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+template <typename Args>
+dk_status launch_cluster(const char* name, void (*kernel)(Args), const Args& a, int threads, size_t smem, unsigned grid, int cluster, cudaStream_t stream) {
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -923,7 +931,7 @@ dk_status launch_tiles(TileArgs& a, size_t smem, unsigned grid, int cluster, cud
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kGemmThreads);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cfg.attrs = attr;
@@ -931,16 +939,108 @@ dk_status launch_tiles(TileArgs& a, size_t smem, unsigned grid, int cluster, cud
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
   if (e != cudaSuccess) {
     (void)cudaGetLastError();
-    set_cuda_error(e, "k_gemm");
+    set_cuda_error(e, name);
     return DK_ERR_LAUNCH;
   }
   return DK_OK;
 }
 
-inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+// ---- few rows ----
+constexpr int kFewRows = 64;
+
+inline int few_form(int rows) { return rows <= 4 ? 4 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+inline size_t few_pieces(int rows, int groups, bool bf16) {
+  return (size_t)groups * (((bf16 ? 2 : 3) * few_form(rows) + 15) / 16 * 16) * 128;
+}
+inline size_t few_bytes(int rows, int groups, bool bf16) { return few_pieces(rows, groups, bf16) + (size_t)groups * few_form(rows) * sizeof(float2); }
+
+template <bool BF16, int MODE, int TT>
+dk_status few_product(const Product& p, cudaStream_t stream) {
+  using F = few::Form<BF16, TT>;
+  auto kernel = few::k_few<BF16, MODE, TT>;
+  static std::atomic<unsigned long long> done{0};
+  dk_status st = allow_smem(kernel, done);
+  if (st != DK_OK) return st;
+  few::Args a{};
+  a.groups = p.K / kGroup;
+  a.scales[0] = reinterpret_cast<const __half*>(p.scales[0]);
+  a.scales[1] = reinterpret_cast<const __half*>(p.scales[1]);
+  uint8_t* pieces = static_cast<uint8_t*>(p.workspace);
+  float2* factors = reinterpret_cast<float2*>(pieces + few_pieces(p.rows, a.groups, BF16));
+  a.factors = factors;
+  a.y = p.y;
+  a.keep[0] = p.keep[0];
+  a.keep[1] = p.keep[1];
+  a.ldy = p.ldy;
+  a.ldk = p.ldk;
+  a.error = device_error_address();
+  a.rows = p.rows;
+  a.M = p.M;
+  a.K = p.K;
+  a.act = p.act;
+  a.tiles = ceil_div(p.M, MODE == kGated ? 64 : 128);
+  // The cluster's size that leaves the fewest steps to its busiest CTA.  How
+  // many clusters of a size run at once is the device's property.
+  static std::atomic<int> at_once[64][4];
+  const int device = current_device() & 63;
+  int best = 0;
+  for (int i = 0; i < 4; ++i) {
+    const int size = 1 << i;
+    int most = at_once[device][i].load(std::memory_order_relaxed);
+    if (!most) {
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = size;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(size * sm_count(-1));
+      cfg.blockDim = dim3(F::kThreads);
+      cfg.dynamicSmemBytes = F::kSmem;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&most, kernel, &cfg) != cudaSuccess || most < 1) {
+        (void)cudaGetLastError();
+        most = std::max(1, sm_count(-1) / size);
+      }
+      at_once[device][i].store(most, std::memory_order_relaxed);
+    }
+    const int clusters = std::min(a.tiles, most);
+    const int steps = ceil_div((int64_t)ceil_div(a.tiles, clusters) * a.groups, size);
+    if (!best || steps < best) best = steps, a.cluster = size, a.clusters = clusters;
+  }
+  for (int i = 0; i < p.matrices; ++i)
+    if (!tensor_map(&a.w[i], p.packed[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, p.K / 2, p.M, p.K / 2, 64, MODE == kGated ? 64 : 128, CU_TENSOR_MAP_SWIZZLE_64B))
+      return DK_ERR_UNSUPPORTED;
+  if (!tensor_map(&a.b, pieces, CU_TENSOR_MAP_DATA_TYPE_UINT8, 128, (uint64_t)a.groups * F::kN, 128, 128, F::kN, CU_TENSOR_MAP_SWIZZLE_128B))
+    return DK_ERR_UNSUPPORTED;
+  few::SplitArgs split{p.x[0], pieces, factors, p.rows > 1 ? p.ldx : 0, p.rows, a.groups};
+  st = launch_early("k_split", few::k_split<BF16, TT>, dim3(ceil_div((int64_t)p.rows * a.groups, 4)), dim3(128), 0, stream, split);
+  if (st != DK_OK) return st;
+  return launch_cluster("k_few", kernel, a, F::kThreads, F::kSmem, (unsigned)(a.clusters * a.cluster), a.cluster, stream);
+}
+
+template <bool BF16, int MODE>
+dk_status few_product(const Product& p, cudaStream_t stream) {
+  switch (few_form(p.rows)) {
+    case 4: return few_product<BF16, MODE, 4>(p, stream);
+    case 16: return few_product<BF16, MODE, 16>(p, stream);
+    case 32: return few_product<BF16, MODE, 32>(p, stream);
+    default: return few_product<BF16, MODE, 64>(p, stream);
+  }
+}
+
+// ---- many rows ----
+template <bool BF16, int MODE, int CG>
+dk_status launch_tiles(const TileArgs& a, size_t smem, unsigned grid, int cluster, cudaStream_t stream) {
+  static std::atomic<unsigned long long> done{0};
+  const dk_status st = allow_smem(k_gemm<BF16, MODE, CG>, done);
+  return st != DK_OK ? st : launch_cluster("k_gemm", k_gemm<BF16, MODE, CG>, a, kGemmThreads, smem, grid, cluster, stream);
+}
 
 template <int MODE>
 dk_status product(const Product& p, cudaStream_t stream) {
+  if constexpr (MODE != kTransposed)
+    if (p.rows <= kFewRows) return p.bf16 ? few_product<true, MODE>(p, stream) : few_product<false, MODE>(p, stream);
   TileArgs a{};
   a.scales[0] = reinterpret_cast<const __half*>(p.scales[0]);
   a.scales[1] = reinterpret_cast<const __half*>(p.scales[1]);
@@ -1065,6 +1165,11 @@ __global__ void __launch_bounds__(256) k_gated_grad(const __grid_constant__ Grad
 
 using namespace dk;
 
+extern "C" size_t dk_w4a16_gemm_workspace_bytes(int rows, int K, dk_dtype dtype) {
+  if (rows < 1 || rows > kFewRows || K < DK_GROUP_SIZE || K % DK_GROUP_SIZE || (dtype != DK_FP16 && dtype != DK_BF16)) return 0;
+  return few_bytes(rows, K / DK_GROUP_SIZE, dtype == DK_BF16);
+}
+
 extern "C" dk_status dk_w4a16_gemm(const dk_gemm_args* p, void* stream) {
   if (!p || p->rows < 0 || p->M < 0 || p->K < 1 || p->K % DK_GROUP_SIZE) return DK_ERR_INVALID_ARG;
   if (p->dtype != DK_FP16 && p->dtype != DK_BF16) return DK_ERR_INVALID_ARG;
@@ -1077,7 +1182,10 @@ extern "C" dk_status dk_w4a16_gemm(const dk_gemm_args* p, void* stream) {
   if (!aligned16(p->packed) || !aligned16(p->packed2) || !aligned16(p->x)) return DK_ERR_INVALID_ARG;
   if (p->rows > 1 && (p->ldx < p->K || p->ldx % 8 || p->ldy < p->M || (p->gate_out && p->ldk < p->M)))
     return DK_ERR_INVALID_ARG;
+  const size_t need = dk_w4a16_gemm_workspace_bytes(p->rows, p->K, p->dtype);
+  if (need && (!p->workspace || p->workspace_bytes < need || (reinterpret_cast<uintptr_t>(p->workspace) & 127u))) return DK_ERR_WORKSPACE;
   Product a{};
+  a.workspace = p->workspace;
   a.packed[0] = p->packed;
   a.packed[1] = p->packed2;
   a.scales[0] = p->scales;

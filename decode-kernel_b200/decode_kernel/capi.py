@@ -128,7 +128,8 @@ class GemmArgs(ctypes.Structure):
     _fields_ = [(name, ctypes.c_void_p) for name in (
         "packed", "scales", "packed2", "scales2", "x", "y", "gate_out", "up_out")] + [
             (name, ctypes.c_int64) for name in ("ldx", "ldy", "ldk")] + [
-                (name, ctypes.c_int) for name in ("rows", "M", "K", "dtype", "act")]
+                (name, ctypes.c_int) for name in ("rows", "M", "K", "dtype", "act")] + [
+                    ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
 
 
 class GemmTArgs(ctypes.Structure):
@@ -220,6 +221,7 @@ SIGNATURES = {
     "dk_cache_attention_counter_bytes": (_SZ, []),
     "dk_cache_attention": (_I, [ctypes.POINTER(CacheAttentionArgs), _P, _SZ, _P]),
     "dk_block_norm": (_I, [ctypes.POINTER(BlockNormArgs), _P]),
+    "dk_w4a16_gemm_workspace_bytes": (_SZ, [_I, _I, _I]),
     "dk_w4a16_gemm": (_I, [ctypes.POINTER(GemmArgs), _P]),
     "dk_w4a16_gemm_t": (_I, [ctypes.POINTER(GemmTArgs), _P]),
     "dk_gated_grad": (_I, [_P, _P, _P, _P, _P, _I, _I, _L, _L, _L, _I, _I, _P]),
