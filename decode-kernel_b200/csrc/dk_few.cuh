@@ -26,7 +26,7 @@ namespace few {
 
 constexpr int kCopyB = 0, kMma = 1, kCopyW = 2;  // behind the unpacking and the summing warps
 
-// TT: rows of a call, rounded up to 4, 16, 32 or 64.
+// TT: rows of a call, rounded up to 4, 16 or 32.
 template <bool BF16, int TT>
 struct Form {
   static constexpr int kPieces = BF16 ? 2 : 3;
@@ -34,14 +34,15 @@ struct Form {
   static constexpr int kRing = TT <= 16 ? 8 : 4;            // steps of A (32 columns each) and B
   static constexpr int kRoom = (512 - kRing * 32) / kN;
   static constexpr int kPlaces = kRoom >= 8 && kRing >= 8 ? 8 : kRoom >= 4 ? 4 : 2;  // of sums
-  static constexpr int kRaw = TT <= 32 ? 16 : 4;            // steps of packed words: a power of two
+  static constexpr int kRaw = TT <= 16 ? 16 : 8;            // steps of packed words: a power of two
   static constexpr int kGroups = TT <= 16 ? 4 : 2;          // of four unpacking warps
-  static constexpr int kDq = 4 * kGroups, kSum = kDq, kRest = kDq + 4;
+  static constexpr int kTeams = 2;                          // of four summing warps, a step each in turn
+  static constexpr int kDq = 4 * kGroups, kRest = kDq + 4 * kTeams;
   static constexpr int kThreads = (kRest + 3) * 32;
   static constexpr int kFactors = 2 * kRing;                // steps of the rows' factors
   // Shared memory.
   static constexpr int kB = 0, kRawAt = kB + kRing * kN * 128, kPart = kRawAt + kRaw * kRawBytes;
-  static constexpr int kPartBytes = TT * kLanes * 4, kFactorAt = kPart + 2 * kPartBytes;
+  static constexpr int kPartBytes = TT * kLanes * 4, kFactorAt = kPart + 2 * kTeams * kPartBytes;
   static constexpr int kBars = kFactorAt + kFactors * TT * 8;
   static constexpr int kTotal = kBars + (kRing + 16 + 2 * kRaw + 1) * 8 + 16;
   static constexpr int kSmem = kTotal > kSmemLeast ? kTotal : kSmemLeast;
@@ -212,7 +213,7 @@ __global__ void __launch_bounds__(Form<BF16, TT>::kThreads, 1) k_few(const __gri
     const int row = MODE == kPlain ? quad * 32 + lane : (lane >> 4) * 64 + quad * 16 + (lane & 15);
     for (int step = offset; step < todo; step += F::kGroups / 2) {
       const int raw = step % F::kRaw, slot = step % F::kRing;
-      if (!warp_wait(&raw_full[raw], step / F::kRaw & 1, give_up, a.error)) break;
+      warp_wait(&raw_full[raw], step / F::kRaw & 1, give_up, a.error);
       const uint32_t from = base + F::kRawAt + raw * kRawBytes + row * 64;
       uint32_t o[16];
 #pragma unroll
@@ -226,7 +227,7 @@ __global__ void __launch_bounds__(Form<BF16, TT>::kThreads, 1) k_few(const __gri
         }
       }
       const int before = step - F::kRing;
-      if (before >= 0 && !warp_wait(&done[before % 16], before / 16 & 1, give_up, a.error)) break;
+      if (before >= 0) warp_wait(&done[before % 16], before / 16 & 1, give_up, a.error);
       tcgen05_fence_after();
       tmem_st16(tmem + ((uint32_t)(quad * 32) << 16) + kAColumn + slot * 32 + half * 16, o);
       tmem_st_wait();
@@ -239,78 +240,87 @@ __global__ void __launch_bounds__(Form<BF16, TT>::kThreads, 1) k_few(const __gri
     }
   } else if (warp < F::kRest) {
     // ---------------- sums to fp32 ----------------
-    const int quad = warp & 3, tile_lane = quad * 32 + lane;
+    const int quad = warp & 3, team = (warp - F::kDq) >> 2, tile_lane = quad * 32 + lane;
     // A place is free for the first steps.
-    if (lane == 0)
+    if (team == 0 && lane == 0)
       for (int s = 0; s < F::kPlaces; ++s) mbar_arrive(&full[s % F::kRing]);
-    const unsigned short* scales = reinterpret_cast<const unsigned short*>(a.scales[MODE == kGated ? lane >> 4 : 0]);
-    int f_tile = tile, f_group = group, f_left = todo;
-    auto fetch = [&]() -> unsigned short {
-      unsigned short v = 0;
-      if (f_left > 0) {
-        const int m = MODE == kPlain ? f_tile * 128 + tile_lane : f_tile * 64 + quad * 16 + (lane & 15);
-        if (m < a.M) v = __ldg(scales + (long long)m * steps + f_group);
-        if (++f_group == steps) f_group = 0, ++f_tile;
-        --f_left;
-      }
-      return v;
+    const __half* scales = a.scales[MODE == kGated ? lane >> 4 : 0];
+    auto scale_of = [&](int tile, int group) {
+      const int m = MODE == kPlain ? tile * 128 + tile_lane : tile * 64 + quad * 16 + (lane & 15);
+      return m < a.M ? scales[(long long)m * steps + group] : __half(0.f);
     };
-    unsigned short scale0 = fetch(), scale1 = fetch(), scale2 = fetch();
     float acc[TT];
 #pragma unroll
     for (int t = 0; t < TT; ++t) acc[t] = 0.f;
     int first = group;  // of the tile's groups that are added here
-    pdl_wait();         // y may be read by what came before
+    // This team's next step's scale is on its way while the step before is added.
+    auto after = [&](int by) {
+      int t = tile, g = group + by;
+      if (g >= steps) g -= steps, ++t;  // steps > by, or the tile is past the line's end or has one step only
+      while (g >= steps) g -= steps, ++t;
+      return t < tile1 ? scale_of(t, g) : __half(0.f);
+    };
+    __half scale = after(team), scale_next = __half(0.f);
+    pdl_wait();  // y may be read by what came before
     for (int step = 0; step < todo; ++step) {
-      const float scale = __half2float(__ushort_as_half(scale0));
-      scale0 = scale1;
-      scale1 = scale2;
-      scale2 = fetch();
-      if (!warp_wait(&done[step % 16], step / 16 & 1, give_up, a.error)) break;
-      tcgen05_fence_after();
-      const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + (step % F::kPlaces) * F::kN;
-      const uint32_t factors = base + F::kFactorAt + (step % F::kFactors) * TT * 8;
-      constexpr int C = TT < 16 ? 4 : TT == 16 ? 8 : 16;
+      if (step % F::kTeams == team) {
+        scale_next = after(F::kTeams);
+        warp_wait(&done[step % 16], step / 16 & 1, give_up, a.error);
+        tcgen05_fence_after();
+        const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + (step % F::kPlaces) * F::kN;
+        const uint32_t factors = base + F::kFactorAt + (step % F::kFactors) * TT * 8;
+        constexpr int C = TT < 16 ? 4 : 8;
+        float s = __half2float(scale);
 #pragma unroll
-      for (int t0 = 0; t0 < TT; t0 += C) {
-        float p1[C], p2[C], p3[C];
-        tmem_ld(from + t0, p1);
-        tmem_ld(from + TT + t0, p2);
-        if constexpr (!BF16) tmem_ld(from + 2 * TT + t0, p3);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        for (int t0 = 0; t0 < TT; t0 += C) {
+          float p1[C], p2[C], p3[C];
+          tmem_ld(from + t0, p1);
+          tmem_ld(from + TT + t0, p2);
+          if constexpr (!BF16) tmem_ld(from + 2 * TT + t0, p3);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-        for (int t = 0; t < C; t += 2) {
-          const uint4 two = lds128(factors + (t0 + t) * 8);
-          const float down[2] = {__uint_as_float(two.x), __uint_as_float(two.z)}, off[2] = {__uint_as_float(two.y), __uint_as_float(two.w)};
+          for (int t = 0; t < C; t += 2) {
+            const uint4 two = lds128(factors + (t0 + t) * 8);
+            const float down[2] = {__uint_as_float(two.x), __uint_as_float(two.z)}, off[2] = {__uint_as_float(two.y), __uint_as_float(two.w)};
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            // The pieces' sums are whole multiples of 2^-18 and 2^-9 below 2^20:
-            // two roundings at most, 2^-24 of the sum each.
-            float v = p2[t + j];
-            if constexpr (!BF16) v = fmaf(p3[t + j], 0.0625f, v);
-            v = fmaf(fmaf(v, 0.0625f, p1[t + j]), 512.f, -off[j]);
-            acc[t0 + t + j] = fmaf(v * scale, down[j], acc[t0 + t + j]);
+            for (int j = 0; j < 2; ++j) {
+              // The pieces' sums are whole multiples of 2^-18 and 2^-9 below 2^20:
+              // two roundings at most, 2^-24 of the sum each.
+              float v = p2[t + j];
+              if constexpr (!BF16) v = fmaf(p3[t + j], 0.0625f, v);
+              v = fmaf(fmaf(v, 0.0625f, p1[t + j]), 512.f, -off[j]);
+              acc[t0 + t + j] = fmaf(v * s, down[j], acc[t0 + t + j]);
+            }
           }
         }
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0 && step + F::kPlaces < todo) mbar_arrive(&full[(step + F::kPlaces) % F::kRing]);
+        scale = scale_next;
       }
-      tcgen05_fence_before();
-      __syncwarp();
-      if (lane == 0 && step + F::kPlaces < todo) mbar_arrive(&full[(step + F::kPlaces) % F::kRing]);
       if (group == steps - 1 || step == todo - 1) {
-        // Begun before this CTA's part: place 0; else place 1, from where a whole
-        // tile goes on at once (by this thread itself, in a loop that needs no
-        // registers for all rows).
+        // The teams' sums.  Begun before this CTA's part of the line: place 0; else
+        // place 1, from where a whole tile goes on at once.
         const uint32_t to = base + F::kPart + (first ? 0 : F::kPartBytes) + tile_lane * 4;
 #pragma unroll
-        for (int t = 0; t < TT; ++t) asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + t * kLanes * 4), "f"(acc[t]) : "memory");
+        for (int t = 0; t < TT; ++t) {
+          asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + team * 2 * F::kPartBytes + t * kLanes * 4), "f"(acc[t]) : "memory");
+          acc[t] = 0.f;
+        }
         if (first == 0 && group == steps - 1) {
+          named_barrier(1, F::kTeams * 128);
           const int out = output_of<MODE, false>(tile, tile_lane);
 #pragma unroll 1
-          for (int t = 0; t < a.rows; t += 2)
-            finish<BF16, MODE>(a, tile_lane, out, t, __uint_as_float(lds32(to + t * kLanes * 4)), __uint_as_float(lds32(to + (t + 1) * kLanes * 4)));
-        }
+          for (int t = 2 * team; t < a.rows; t += 2 * F::kTeams) {
+            float v[2] = {0.f, 0.f};
 #pragma unroll
-        for (int t = 0; t < TT; ++t) acc[t] = 0.f;
+            for (int i = 0; i < F::kTeams; ++i)
+#pragma unroll
+              for (int j = 0; j < 2; ++j) v[j] += __uint_as_float(lds32(to + i * 2 * F::kPartBytes + (t + j) * kLanes * 4));
+            finish<BF16, MODE>(a, tile_lane, out, t, v[0], v[1]);
+          }
+          named_barrier(1, F::kTeams * 128);
+        }
         first = 0;
       }
       next();
@@ -376,7 +386,7 @@ __global__ void __launch_bounds__(Form<BF16, TT>::kThreads, 1) k_few(const __gri
     int step = 0;
     for (; step < todo; ++step) {
       const int slot = step % F::kRing;
-      if (!warp_spin(&full[slot], step / F::kRing & 1, give_up, a.error)) break;
+      warp_wait<true>(&full[slot], step / F::kRing & 1, give_up, a.error);
       tcgen05_fence_after();
       const uint32_t at = tmem + kAColumn + slot * 32, d = tmem + (step % F::kPlaces) * F::kN;
       const uint64_t b0 = umma_desc_k_sw128(base + F::kB + slot * F::kN * 128);
@@ -409,13 +419,16 @@ __global__ void __launch_bounds__(Form<BF16, TT>::kThreads, 1) k_few(const __gri
       if (low >= high || rank < low || rank > high) continue;
       const int share = high - low + 1, out = output_of<MODE, false>(tile0 + n, tile_lane);
 #pragma unroll 1
-      for (int p = (rank - low) + share * (warp >> 2); p < (a.rows + 1) / 2; p += share * (F::kGroups + 1)) {
+      for (int p = (rank - low) + share * (warp >> 2); p < (a.rows + 1) / 2; p += share * (F::kGroups + F::kTeams)) {
         float v0 = 0.f, v1 = 0.f;
         for (int r = low; r <= high; ++r) {
           if (border(r) == border(r + 1)) continue;
           const uint32_t far = mapa(base + F::kPart + (border(r) > from ? 0 : F::kPartBytes) + (2 * p * kLanes + tile_lane) * 4, r);
-          v0 += ld_cluster(far);
-          v1 += ld_cluster(far + kLanes * 4);
+#pragma unroll
+          for (int i = 0; i < F::kTeams; ++i) {
+            v0 += ld_cluster(far + i * 2 * F::kPartBytes);
+            v1 += ld_cluster(far + i * 2 * F::kPartBytes + kLanes * 4);
+          }
         }
         finish<BF16, MODE>(a, tile_lane, out, 2 * p, v0, v1);
       }

@@ -75,27 +75,28 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatil
     }
   }
 }
-// A warp's wait.  All lanes ask (one that asks for all costs the others a vote
-// more: 1.4 times the time of whole products).
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* give_up, int* error) {
-  return __all_sync(0xffffffffu, wait_bar(bar, parity, give_up, error));
-}
-// The same without suspending, for the warp that issues the MMAs.
-__device__ __forceinline__ bool warp_spin(uint64_t* bar, uint32_t parity, volatile int* give_up, int* error) {
-  bool ok = mbar_test_wait(bar, parity);
-  if (!ok) {
-    const uint64_t t0 = globaltimer_ns();
-    for (int i = 0; !(ok = mbar_test_wait(bar, parity)); ++i) {
-      if ((i & 255) != 255) continue;
-      if (*give_up) break;
-      if (globaltimer_ns() - t0 > kWaitLimitNs) {
-        if (error) atomicExch(error, kDevWaitTimeout);
-        *give_up = 1;
-        break;
+// A warp's wait, without an answer: after the limit every wait ends at once and
+// the loops run out over whatever is there, without MMAs or results.  Nothing to
+// vote on keeps a wait that need not wait short.
+template <bool SPIN = false>
+__device__ __forceinline__ void warp_wait(uint64_t* bar, uint32_t parity, volatile int* give_up, int* error) {
+  if (!mbar_test_wait(bar, parity)) {
+    if constexpr (SPIN) {  // without suspending
+      const uint64_t t0 = globaltimer_ns();
+      for (int i = 1; !mbar_test_wait(bar, parity); ++i) {
+        if (i & 255) continue;
+        if (*give_up) break;
+        if (globaltimer_ns() - t0 > kWaitLimitNs) {
+          if (error) atomicExch(error, kDevWaitTimeout);
+          *give_up = 1;
+          break;
+        }
       }
+    } else {
+      wait_bar(bar, parity, give_up, error);
     }
   }
-  return __all_sync(0xffffffffu, ok);
+  __syncwarp();
 }
 
 __device__ __forceinline__ void tma_2d(uint32_t dst, const void* map, int c0, int c1, uint32_t bar) {
@@ -217,17 +218,6 @@ __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.comm
 template <int LEFT>
 __device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(LEFT) : "memory"); }
 __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
-// Whether all `threads` that meet at the barrier say so.
-__device__ __forceinline__ bool barrier_all(int id, int threads, bool mine) {
-  uint32_t all;
-  asm volatile(
-      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n"
-      " barrier.cta.red.and.aligned.pred q, %2, %3, p;\n selp.u32 %0, 1, 0, q;\n}"
-      : "=r"(all)
-      : "r"(mine ? 1u : 0u), "r"(id), "r"(threads)
-      : "memory");
-  return all != 0;
-}
 __device__ __forceinline__ void sts16(uint32_t addr, uint16_t v) {
   asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(v) : "memory");
 }
@@ -560,7 +550,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
       }
       scale0 = scale1;
       scale1 = fetch();
-      if (!warp_wait(&raw_full[raw], step >> kRawBits & 1, give_up, a.error)) break;
+      warp_wait(&raw_full[raw], step >> kRawBits & 1, give_up, a.error);
       uint32_t w[8];
       const uint32_t from = base + L.raw + raw * kRawBytes;
       if constexpr (!kTurn) {
@@ -610,7 +600,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
         }
       }
       const int before = step - (1 << kABits);  // the step whose place in the ring this one takes
-      if (before >= 0 && !warp_wait(&done[before % kDone], before / kDone & 1, give_up, a.error)) break;
+      if (before >= 0) warp_wait(&done[before % kDone], before / kDone & 1, give_up, a.error);
       if constexpr (kATmem) {
         tcgen05_fence_after();
         tmem_st32(tmem + ((uint32_t)(quad * 32) << 16) + At::kA + slot * 64 + half * 32, o);
@@ -644,8 +634,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
     const uint32_t column = (uint32_t)output_of<MODE, kATmem>(0, tile_lane) * 2;
     int phase = 0, turn = 0, place = 0;
     for (int item = item0; item < items; item += item_step) {
-      // All four warps go on or none does: they meet at barriers.
-      if (!barrier_all(1, kSumWarps * 32, warp_wait(&sums_full[place], phase, give_up, a.error))) break;
+      warp_wait(&sums_full[place], phase, give_up, a.error);
       tcgen05_fence_after();
       const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + place * At::kSums;
       const int tile = item / a.token_tiles * CG + (CG == 2 ? (int)rank : 0);
@@ -798,18 +787,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
       const uint32_t idesc = (1u << 4) | ((BF16 ? 1u : 0u) << 7) | ((BF16 ? 1u : 0u) << 10) | ((kATmem ? 0u : 1u) << 15) | ((uint32_t)(a.tokens >> 3) << 17) |
                              ((uint32_t)(kLanes * CG >> 4) << 24);
       int slot = 0, phase = 0, step = 0, tile = 0;
-      constexpr int kABits = At::kABits;
-      bool going = true;
       const uint32_t b_half = (uint32_t)b_rows * 128 >> 4;  // in the descriptors' units of 16 bytes
-      for (int item = item0; item < items && going; item += item_step, ++tile) {
+      for (int item = item0; item < items; item += item_step, ++tile) {
         const int place = a.places == 2 ? tile & 1 : 0, before = tile - a.places;  // the tile whose sums were there
-        if (before >= 0 && !warp_wait(&sums_free[place], (a.places == 2 ? before >> 1 : before) & 1, give_up, a.error)) break;
+        if (before >= 0) warp_wait<true>(&sums_free[place], (a.places == 2 ? before >> 1 : before) & 1, give_up, a.error);
         tcgen05_fence_after();
         const uint32_t d = tmem + place * At::kSums;
         for (int s = begin; s < end; ++s) {
-          const int a_slot = step & ((1 << kABits) - 1);
-          going = warp_spin(&b_full[slot], phase, give_up, a.error) && warp_spin(&a_full[a_slot], step >> kABits & 1, give_up, a.error);
-          if (!going) break;
+          const int a_slot = step & ((1 << At::kABits) - 1);
+          warp_wait<true>(&b_full[slot], phase, give_up, a.error);
+          warp_wait<true>(&a_full[a_slot], step >> At::kABits & 1, give_up, a.error);
           tcgen05_fence_after();
           const uint64_t b0 = umma_desc_k_sw128(base + L.b + slot * (uint32_t)b_rows * 256);
           if (elect_one()) {
@@ -946,9 +933,9 @@ dk_status launch_cluster(const char* name, void (*kernel)(Args), const Args& a, 
 }
 
 // ---- few rows ----
-constexpr int kFewRows = 64;
+constexpr int kFewRows = 32;
 
-inline int few_form(int rows) { return rows <= 4 ? 4 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+inline int few_form(int rows) { return rows <= 4 ? 4 : rows <= 16 ? 16 : 32; }
 inline size_t few_pieces(int rows, int groups, bool bf16) {
   return (size_t)groups * (((bf16 ? 2 : 3) * few_form(rows) + 15) / 16 * 16) * 128;
 }
@@ -1024,8 +1011,7 @@ dk_status few_product(const Product& p, cudaStream_t stream) {
   switch (few_form(p.rows)) {
     case 4: return few_product<BF16, MODE, 4>(p, stream);
     case 16: return few_product<BF16, MODE, 16>(p, stream);
-    case 32: return few_product<BF16, MODE, 32>(p, stream);
-    default: return few_product<BF16, MODE, 64>(p, stream);
+    default: return few_product<BF16, MODE, 32>(p, stream);
   }
 }
 

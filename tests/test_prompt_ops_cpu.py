@@ -50,8 +50,8 @@ def test_gemm_t_rejects(kw):
 
 def test_few_rows_need_a_workspace():
     need = capi.load().dk_w4a16_gemm_workspace_bytes
-    assert need(1, 256, capi.DK_FP16) > 0 and need(64, 256, capi.DK_BF16) > 0
-    assert need(65, 256, capi.DK_FP16) == need(0, 256, capi.DK_FP16) == need(1, 200, capi.DK_FP16) == need(1, 256, capi.DK_FP32) == 0
+    assert need(1, 256, capi.DK_FP16) > 0 and need(32, 256, capi.DK_BF16) > 0
+    assert need(33, 256, capi.DK_FP16) == need(0, 256, capi.DK_FP16) == need(1, 200, capi.DK_FP16) == need(1, 256, capi.DK_FP32) == 0
     size = need(4, 256, capi.DK_FP16)
     for kw in (dict(), dict(workspace=1024, workspace_bytes=size - 1), dict(workspace=1088, workspace_bytes=size)):
         assert capi.load().dk_w4a16_gemm(ctypes.byref(gemm_args(**kw)), None) == capi.DK_ERR_WORKSPACE

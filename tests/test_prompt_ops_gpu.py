@@ -28,7 +28,7 @@ def weights(M, K, seed):
     return packed, scales.half()
 
 
-FEW = 64  # rows up to which the products take the weights as they are
+FEW = 32  # rows up to which the products take the weights as they are
 
 
 def values(w, dtype, rows=FEW + 1):
