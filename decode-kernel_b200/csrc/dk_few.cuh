@@ -245,32 +245,29 @@ __global__ void __launch_bounds__(Form<BF16, TT>::kThreads, 1) k_few(const __gri
     if (team == 0 && lane == 0)
       for (int s = 0; s < F::kPlaces; ++s) mbar_arrive(&full[s % F::kRing]);
     const __half* scales = a.scales[MODE == kGated ? lane >> 4 : 0];
-    auto scale_of = [&](int tile, int group) {
+    auto row_of = [&](int tile) -> const __half* {  // of the lane's scales; null where it has none
       const int m = MODE == kPlain ? tile * 128 + tile_lane : tile * 64 + quad * 16 + (lane & 15);
-      return m < a.M ? scales[(long long)m * steps + group] : __half(0.f);
+      return m < a.M && tile < tile1 ? scales + (long long)m * steps : nullptr;
     };
     float acc[TT];
 #pragma unroll
     for (int t = 0; t < TT; ++t) acc[t] = 0.f;
-    int first = group;  // of the tile's groups that are added here
-    // This team's next step's scale is on its way while the step before is added.
-    auto after = [&](int by) {
-      int t = tile, g = group + by;
-      if (g >= steps) g -= steps, ++t;  // steps > by, or the tile is past the line's end or has one step only
-      while (g >= steps) g -= steps, ++t;
-      return t < tile1 ? scale_of(t, g) : __half(0.f);
-    };
-    __half scale = after(team), scale_next = __half(0.f);
+    // The line tile by tile: groups first .. end - 1 of each.  A team takes every
+    // kTeams-th step of the line; its next scale is on its way meanwhile.
+    const __half* row = row_of(tile);
     pdl_wait();  // y may be read by what came before
-    for (int step = 0; step < todo; ++step) {
-      if (step % F::kTeams == team) {
-        scale_next = after(F::kTeams);
-        warp_wait(&done[step % 16], step / 16 & 1, give_up, a.error);
+    for (int step = 0; step < todo;) {
+      const int first = group, end = min(steps, group + todo - step);
+      int g = first + (team - step % F::kTeams + F::kTeams) % F::kTeams;
+      __half scale = row && g < end ? row[g] : __half(0.f);
+      for (int at = step + g - first; g < end; g += F::kTeams, at += F::kTeams) {
+        const float s = __half2float(scale);
+        if (row && g + F::kTeams < end) scale = row[g + F::kTeams];
+        warp_wait(&done[at % 16], at / 16 & 1, give_up, a.error);
         tcgen05_fence_after();
-        const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + (step % F::kPlaces) * F::kN;
-        const uint32_t factors = base + F::kFactorAt + (step % F::kFactors) * TT * 8;
+        const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + (at % F::kPlaces) * F::kN;
+        const uint32_t factors = base + F::kFactorAt + (at % F::kFactors) * TT * 8;
         constexpr int C = TT < 16 ? 4 : 8;
-        float s = __half2float(scale);
 #pragma unroll
         for (int t0 = 0; t0 < TT; t0 += C) {
           float p1[C], p2[C], p3[C];
@@ -295,35 +292,33 @@ __global__ void __launch_bounds__(Form<BF16, TT>::kThreads, 1) k_few(const __gri
         }
         tcgen05_fence_before();
         __syncwarp();
-        if (lane == 0 && step + F::kPlaces < todo) mbar_arrive(&full[(step + F::kPlaces) % F::kRing]);
-        scale = scale_next;
+        if (lane == 0 && at + F::kPlaces < todo) mbar_arrive(&full[(at + F::kPlaces) % F::kRing]);
       }
-      if (group == steps - 1 || step == todo - 1) {
-        // The teams' sums.  Begun before this CTA's part of the line: place 0; else
-        // place 1, from where a whole tile goes on at once.
-        const uint32_t to = base + F::kPart + (first ? 0 : F::kPartBytes) + tile_lane * 4;
+      // The teams' sums.  Begun before this CTA's part of the line: place 0; else
+      // place 1, from where a whole tile goes on at once.
+      const uint32_t to = base + F::kPart + (first ? 0 : F::kPartBytes) + tile_lane * 4;
 #pragma unroll
-        for (int t = 0; t < TT; ++t) {
-          asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + team * 2 * F::kPartBytes + t * kLanes * 4), "f"(acc[t]) : "memory");
-          acc[t] = 0.f;
-        }
-        if (first == 0 && group == steps - 1) {
-          named_barrier(1, F::kTeams * 128);
-          const int out = output_of<MODE, false>(tile, tile_lane);
+      for (int t = 0; t < TT; ++t) {
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + team * 2 * F::kPartBytes + t * kLanes * 4), "f"(acc[t]) : "memory");
+        acc[t] = 0.f;
+      }
+      if (first == 0 && end == steps) {
+        named_barrier(1, F::kTeams * 128);
+        const int out = output_of<MODE, false>(tile, tile_lane);
 #pragma unroll 1
-          for (int t = 2 * team; t < a.rows; t += 2 * F::kTeams) {
-            float v[2] = {0.f, 0.f};
+        for (int t = 2 * team; t < a.rows; t += 2 * F::kTeams) {
+          float v[2] = {0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < F::kTeams; ++i)
+          for (int i = 0; i < F::kTeams; ++i)
 #pragma unroll
-              for (int j = 0; j < 2; ++j) v[j] += __uint_as_float(lds32(to + i * 2 * F::kPartBytes + (t + j) * kLanes * 4));
-            finish<BF16, MODE>(a, tile_lane, out, t, v[0], v[1]);
-          }
-          named_barrier(1, F::kTeams * 128);
+            for (int j = 0; j < 2; ++j) v[j] += __uint_as_float(lds32(to + i * 2 * F::kPartBytes + (t + j) * kLanes * 4));
+          finish<BF16, MODE>(a, tile_lane, out, t, v[0], v[1]);
         }
-        first = 0;
+        named_barrier(1, F::kTeams * 128);
       }
-      next();
+      step += end - first;
+      group = 0;
+      row = row_of(++tile);
     }
   } else if (warp == F::kRest + kCopyB) {
     if (lane == 0) {
