@@ -321,44 +321,45 @@ __global__ void __launch_bounds__(Form<BF16, TT>::kThreads, 1) k_few(const __gri
       row = row_of(++tile);
     }
   } else if (warp == F::kRest + kCopyB) {
-    if (lane == 0) {
-      pdl_wait();  // for the pieces
-      int issued = 0;
-      bool going = true;
-      for (; issued < todo; ++issued) {
-        const int before = issued - F::kRing, slot = issued % F::kRing;
-        if (before >= 0 && !wait_bar(&done[before % 16], before / 16 & 1, give_up, a.error)) {
-          going = false;
-          break;
-        }
+    // ---------------- copies of the pieces ----------------
+    // (Whole warps go along here and below, so that operands stay in uniform
+    // registers: a step of one diverged thread took 600 cycles and held up the
+    // rest.)
+    pdl_wait();  // for the pieces
+    int issued = 0;
+    for (; issued < todo; ++issued) {
+      const int before = issued - F::kRing, slot = issued % F::kRing;
+      if (before >= 0) warp_wait<true>(&done[before % 16], before / 16 & 1, give_up, a.error);
+      if (__any_sync(0xffffffffu, *give_up)) break;
+      if (elect_one()) {
+        const uint32_t bar = smem_u32(&full[slot]);
         mbar_arrive_expect_tx(&full[slot], F::kN * 128 + TT * 8);
-        tma_2d(base + F::kB + slot * F::kN * 128, &a.b, 0, group * F::kN, smem_u32(&full[slot]));
+        tma_2d(base + F::kB + slot * F::kN * 128, &a.b, 0, group * F::kN, bar);
         // The factors are read after the step's MMAs are done, so their ring is
         // longer by what the sums may be behind.
         asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
                          base + F::kFactorAt + (issued % F::kFactors) * TT * 8),
-                     "l"(a.factors + (long long)group * TT), "r"(TT * 8), "r"(smem_u32(&full[slot]))
+                     "l"(a.factors + (long long)group * TT), "r"(TT * 8), "r"(bar)
                      : "memory");
-        next();
       }
-      if (!going) {  // what was asked for lands before the CTA ends
-        volatile int none = 0;
-        for (int i = max(0, issued - F::kRing); i < issued; ++i) wait_bar(&full[i % F::kRing], i / F::kRing & 1, &none, a.error);
-      }
+      __syncwarp();
+      next();
+    }
+    if (issued < todo && lane == 0) {  // what was asked for lands before the CTA ends
+      volatile int none = 0;
+      for (int i = max(0, issued - F::kRing); i < issued; ++i) wait_bar(&full[i % F::kRing], i / F::kRing & 1, &none, a.error);
     }
     __syncwarp();
   } else if (warp == F::kRest + kCopyW) {
-    if (lane == 0) {
-      // The weights are older than the kernel before, which waited for what
-      // wrote them: no wait here.
-      int issued = 0;
-      bool going = true;
-      for (; issued < todo; ++issued) {
-        const int slot = issued % F::kRaw, round = issued / F::kRaw;
-        if (round && !wait_bar(&raw_free[slot], (round - 1) & 1, give_up, a.error)) {
-          going = false;
-          break;
-        }
+    // ---------------- copies of the packed weights ----------------
+    // The weights are older than the kernel before, which waited for what wrote
+    // them: no wait here.
+    int issued = 0;
+    for (; issued < todo; ++issued) {
+      const int slot = issued % F::kRaw, round = issued / F::kRaw;
+      if (round) warp_wait<true>(&raw_free[slot], (round - 1) & 1, give_up, a.error);
+      if (__any_sync(0xffffffffu, *give_up)) break;
+      if (elect_one()) {
         const uint32_t dst = base + F::kRawAt + slot * kRawBytes, bar = smem_u32(&raw_full[slot]);
         mbar_arrive_expect_tx(&raw_full[slot], kRawBytes);
         if constexpr (MODE == kPlain) {
@@ -367,12 +368,13 @@ __global__ void __launch_bounds__(Form<BF16, TT>::kThreads, 1) k_few(const __gri
           tma_2d(dst, &a.w[0], group * 64, tile * 64, bar);
           tma_2d(dst + kRawBytes / 2, &a.w[1], group * 64, tile * 64, bar);
         }
-        next();
       }
-      if (!going) {
-        volatile int none = 0;
-        for (int i = max(0, issued - F::kRaw); i < issued; ++i) wait_bar(&raw_full[i % F::kRaw], i / F::kRaw & 1, &none, a.error);
-      }
+      __syncwarp();
+      next();
+    }
+    if (issued < todo && lane == 0) {
+      volatile int none = 0;
+      for (int i = max(0, issued - F::kRaw); i < issued; ++i) wait_bar(&raw_full[i % F::kRaw], i / F::kRaw & 1, &none, a.error);
     }
     __syncwarp();
   } else {

@@ -708,22 +708,25 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
     __syncwarp();
   } else if (warp == kCopyB) {
     // ---------------- copies of the tokens ----------------
-    if (lane == 0) {
-      int slot = 0, issued = 0;
-      bool going = true;
-      const uint32_t bytes = (uint32_t)b_rows * 256;  // two boxes
-      const uint32_t full_leader = mapa(smem_u32(b_full), 0);
-      for (int item = item0; item < items && going; item += item_step) {
-        const int t0 = item % a.token_tiles * a.tokens + (CG == 2 ? (int)rank * b_rows : 0);
-        for (int s = begin; s < end; ++s) {
-          const int before = issued - a.b_stages;
-          if (before >= 0 && !wait_bar(&done[before % kDone], before / kDone & 1, give_up, a.error)) {
-            going = false;
-            break;
-          }
-          const int seg = MODE == kTransposed && s >= a.matrix_steps;
-          const int d = (s - seg * a.matrix_steps) * kStepDepth;
-          const uint32_t dst = base + L.b + slot * bytes;
+    // Whole warps go along here and below, so that the operands stay in uniform
+    // registers; one thread issues.
+    int slot = 0, issued = 0;
+    bool going = true;
+    const uint32_t bytes = (uint32_t)b_rows * 256;  // two boxes
+    const uint32_t full_leader = mapa(smem_u32(b_full), 0);
+    for (int item = item0; item < items && going; item += item_step) {
+      const int t0 = item % a.token_tiles * a.tokens + (CG == 2 ? (int)rank * b_rows : 0);
+      for (int s = begin; s < end; ++s) {
+        const int before = issued - a.b_stages;
+        if (before >= 0) warp_wait<true>(&done[before % kDone], before / kDone & 1, give_up, a.error);
+        if (__any_sync(0xffffffffu, *give_up)) {
+          going = false;
+          break;
+        }
+        const int seg = MODE == kTransposed && s >= a.matrix_steps;
+        const int d = (s - seg * a.matrix_steps) * kStepDepth;
+        const uint32_t dst = base + L.b + slot * bytes;
+        if (elect_one()) {
           if constexpr (CG == 1) {
             mbar_arrive_expect_tx(&b_full[slot], bytes);
             tma_2d(dst, &a.b[seg], d, t0, smem_u32(&b_full[slot]));
@@ -733,28 +736,30 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
             tma_2d_pair(dst, &a.b[seg], d, t0, full_leader + slot * 8);
             tma_2d_pair(dst + bytes / 2, &a.b[seg], d + kHalfDepth, t0, full_leader + slot * 8);
           }
-          ++issued;
-          if (++slot == a.b_stages) slot = 0;
         }
+        __syncwarp();
+        ++issued;
+        if (++slot == a.b_stages) slot = 0;
       }
-      if (!going && first) {  // what was asked for lands before the CTA ends
-        volatile int none = 0;
-        for (int i = max(0, issued - a.b_stages); i < issued; ++i) wait_bar(&b_full[i % a.b_stages], (i / a.b_stages) & 1, &none, a.error);
-      }
+    }
+    if (!going && first && lane == 0) {  // what was asked for lands before the CTA ends
+      volatile int none = 0;
+      for (int i = max(0, issued - a.b_stages); i < issued; ++i) wait_bar(&b_full[i % a.b_stages], (i / a.b_stages) & 1, &none, a.error);
     }
     __syncwarp();
   } else if (warp == kCopyW) {
     // ---------------- copies of the packed weights ----------------
-    if (lane == 0) {
-      int slot = 0, phase = 0, issued = 0;
-      bool going = true;
-      for (int item = item0; item < items && going; item += item_step) {
-        const int tile = item / a.token_tiles * CG + (CG == 2 ? (int)rank : 0);
-        for (int s = begin; s < end; ++s) {
-          if (issued >= a.raw_stages && !wait_bar(&raw_free[slot], phase ^ 1, give_up, a.error)) {
-            going = false;
-            break;
-          }
+    int slot = 0, phase = 0, issued = 0;
+    bool going = true;
+    for (int item = item0; item < items && going; item += item_step) {
+      const int tile = item / a.token_tiles * CG + (CG == 2 ? (int)rank : 0);
+      for (int s = begin; s < end; ++s) {
+        if (issued >= a.raw_stages) warp_wait<true>(&raw_free[slot], phase ^ 1, give_up, a.error);
+        if (__any_sync(0xffffffffu, *give_up)) {
+          going = false;
+          break;
+        }
+        if (elect_one()) {
           const uint32_t dst = base + L.raw + slot * kRawBytes, bar = smem_u32(&raw_full[slot]);
           mbar_arrive_expect_tx(&raw_full[slot], kRawBytes);
           if constexpr (MODE == kPlain) {
@@ -766,21 +771,20 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
             const int seg = s >= a.matrix_steps;
             tma_2d(dst, &a.w[seg], tile * 64, (s - seg * a.matrix_steps) * kStepDepth, bar);
           }
-          ++issued;
-          if (++slot == a.raw_stages) slot = 0, phase ^= 1;
         }
+        __syncwarp();
+        ++issued;
+        if (++slot == a.raw_stages) slot = 0, phase ^= 1;
       }
-      if (!going) {
-        volatile int none = 0;
-        for (int i = max(0, issued - a.raw_stages); i < issued; ++i)
-          wait_bar(&raw_full[i % a.raw_stages], (i / a.raw_stages) & 1, &none, a.error);
-      }
+    }
+    if (!going && lane == 0) {
+      volatile int none = 0;
+      for (int i = max(0, issued - a.raw_stages); i < issued; ++i)
+        wait_bar(&raw_full[i % a.raw_stages], (i / a.raw_stages) & 1, &none, a.error);
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
     // ---------------- the MMAs ----------------
-    // The whole warp goes along, so that the operands stay in uniform registers;
-    // one thread issues.
     if (first) {
       // fp32 sums, A and B fp16 (0) or bf16 (1), the depth innermost but for an A
       // in shared memory.
