@@ -1029,8 +1029,21 @@ dk_status launch_tiles(const TileArgs& a, size_t smem, unsigned grid, int cluste
 
 template <int MODE>
 dk_status product(const Product& p, cudaStream_t stream) {
-  if constexpr (MODE != kTransposed)
+  if constexpr (MODE != kTransposed) {
+    // Up to 8 contiguous fp16 rows the GEMV's streaming kernel, whose groups' sums
+    // are fp32 too: one launch instead of two.  us a call in a chain, it and the
+    // 8-bit form, one row / eight: 4096 x 4096 6.2 / 8.2, 10.7 / 12.2; 28672 x 8192
+    // 28 / 37, 42 / 46; pairs of 11008 x 4096 15 / 18, 21 / 24.
+    if (p.rows <= 8 && !p.bf16 && (p.rows == 1 || (p.ldx == p.K && p.ldy == p.M)) && !p.keep[0]) {
+      const dk_status st =
+          MODE == kGated
+              ? stream_gated(p.packed, p.scales, p.x[0], p.y, p.M, p.K, p.rows, (dk_mlp_act)p.act, stream)
+              : dk_w4a16_gemv(p.packed[0], p.scales[0], static_cast<const uint16_t*>(p.x[0]), static_cast<uint16_t*>(p.y), p.M, p.K, p.rows,
+                              nullptr, nullptr, 0, stream);
+      if (st != DK_ERR_UNSUPPORTED) return st;
+    }
     if (p.rows <= kFewRows) return p.bf16 ? few_product<true, MODE>(p, stream) : few_product<false, MODE>(p, stream);
+  }
   TileArgs a{};
   a.scales[0] = reinterpret_cast<const __half*>(p.scales[0]);
   a.scales[1] = reinterpret_cast<const __half*>(p.scales[1]);
@@ -1127,27 +1140,48 @@ dk_status product(const Product& p, cudaStream_t stream) {
 struct GradArgs {
   const void *dh, *g, *u;
   void *dg, *du;
-  long long lddh, ldk, ldd;
-  int rows, M, act;
+  long long lddh, ldk, ldd, pieces;  // pieces: rows * pieces a row
+  int M, row_pieces, act;
 };
 
-template <typename T>
-__device__ __forceinline__ float get(const void* p, long long i) {
-  return (float)static_cast<const T*>(p)[i];
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) Values {
+  T v[VEC];
+};
+
+// dg = dh * u * act'(g), du = dh * act(g), VEC neighbouring values a thread:
+// three loads and two stores of 16 bytes where rows allow it, bound by HBM.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) k_gated_grad(const __grid_constant__ GradArgs a) {
+  using P = Values<T, VEC>;
+  pdl_wait();
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= a.pieces) return;
+  const long long r = i / a.row_pieces;
+  const int c = (int)(i - r * a.row_pieces) * VEC;
+  const P dh = *reinterpret_cast<const P*>(static_cast<const T*>(a.dh) + r * a.lddh + c);
+  const P g = *reinterpret_cast<const P*>(static_cast<const T*>(a.g) + r * a.ldk + c);
+  const P u = *reinterpret_cast<const P*>(static_cast<const T*>(a.u) + r * a.ldk + c);
+  P dg, du;
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) {
+    const float d = (float)dh.v[j], gv = (float)g.v[j];
+    float slope;
+    const float s = gate_of(gv, a.act, slope);
+    dg.v[j] = (T)(d * (float)u.v[j] * (s + gv * s * (1.f - s) * slope));
+    du.v[j] = (T)(d * gv * s);
+  }
+  *reinterpret_cast<P*>(static_cast<T*>(a.dg) + r * a.ldd + c) = dg;
+  *reinterpret_cast<P*>(static_cast<T*>(a.du) + r * a.ldd + c) = du;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) k_gated_grad(const __grid_constant__ GradArgs a) {
-  pdl_wait();
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= a.M) return;
-  for (long long r = blockIdx.y; r < a.rows; r += gridDim.y) {
-    const float dh = get<T>(a.dh, r * a.lddh + c), g = get<T>(a.g, r * a.ldk + c), u = get<T>(a.u, r * a.ldk + c);
-    float slope;
-    const float s = gate_of(g, a.act, slope);
-    static_cast<T*>(a.dg)[r * a.ldd + c] = (T)(dh * u * (s + g * s * (1.f - s) * slope));
-    static_cast<T*>(a.du)[r * a.ldd + c] = (T)(dh * g * s);
-  }
+dk_status launch_grad(GradArgs& a, int rows, bool wide, cudaStream_t st) {
+  a.row_pieces = wide ? a.M / 8 : a.M;
+  a.pieces = (long long)rows * a.row_pieces;
+  const long long grid = (a.pieces + 255) / 256;
+  if (grid > INT32_MAX) return DK_ERR_UNSUPPORTED;
+  return launch_early("dk_gated_grad", wide ? k_gated_grad<T, 8> : k_gated_grad<T, 1>, dim3((unsigned)grid), dim3(256), 0, st, a);
 }
 
 }  // namespace
@@ -1231,8 +1265,9 @@ extern "C" dk_status dk_gated_grad(const void* dh, const void* g, const void* u,
   if (rows == 0 || M == 0) return DK_OK;
   if (!dh || !g || !u || !dg || !du) return DK_ERR_INVALID_ARG;
   if (rows > 1 && (lddh < M || ldk < M || ldd < M)) return DK_ERR_INVALID_ARG;
-  GradArgs a{dh, g, u, dg, du, lddh, ldk, ldd, rows, M, (int)act};
-  const dim3 grid((M + 255) / 256, std::min(rows, 32768));
-  return launch_early("dk_gated_grad", dtype == DK_FP16 ? k_gated_grad<__half> : k_gated_grad<__nv_bfloat16>, grid, dim3(256), 0,
-                      static_cast<cudaStream_t>(stream), a);
+  GradArgs a{dh, g, u, dg, du, lddh, ldk, ldd, 0, M, 0, (int)act};
+  bool wide = M % 8 == 0 && (rows == 1 || (lddh % 8 == 0 && ldk % 8 == 0 && ldd % 8 == 0));
+  for (const void* p : {dh, g, u, static_cast<const void*>(dg), static_cast<const void*>(du)}) wide = wide && aligned16(p);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == DK_FP16 ? launch_grad<__half>(a, rows, wide, st) : launch_grad<__nv_bfloat16>(a, rows, wide, st);
 }

@@ -82,6 +82,7 @@ struct OutSpec {
 // their concatenated rows (q/k/v, gate/up).  Segment s owns the global 16-row
 // tiles [tile0, tile0 + ceil(rows / 16)); its last tile may be partial.
 constexpr int kMaxSeg = DK_MAX_SEGMENTS;
+constexpr int kPairedUnfused = 1, kPairedOnce = 2;  // h's roundings: those of an unfused fp16 sequence, or one
 struct Segment {
   const uint32_t* packed;  // [rows, K/8]
   const __half* scales;    // [rows, K/128]
@@ -90,10 +91,10 @@ struct Segment {
 };
 // Paired (gate/up SiLU-mul) mode: n == 2 with equal rows; the tiles run as
 // (gate tile j, up tile j) pairs, CTAs own whole pairs, and only s[0].y --
-// h = silu(gate) * up -- is written.
+// h = act(gate) * up -- is written.
 struct SegList {
   int n;       // 2..kMaxSeg
-  int paired;  // 1: gate/up SiLU-mul pairs
+  int paired;  // gate/up pairs: kPairedUnfused, or kPairedOnce + dk_mlp_act
   Segment s[kMaxSeg];
   __host__ __device__ int pairs() const { return (s[0].rows + 15) / 16; }
   __host__ __device__ int tiles() const {
@@ -1140,11 +1141,20 @@ __global__ void __launch_bounds__(NCW * 32 + 64, NCW == 8 ? 2 : 1)
             float gsum = 0.f;
 #pragma unroll
             for (int w = 0; w < kClasses; ++w) gsum = __fadd_rn(gsum, gsrc[w * 16 * nbp]);
+            const Segment& s0 = a.segs.s[0];
+            __half* h = &s0.y[(size_t)b * s0.rows + trow + r];
+            if (a.segs.paired >= kPairedOnce) {
+              // h = g * sigmoid(p(g)) * u in fp32, rounded once; p as dk_w4a16_gemm has it.
+              const float arg = a.segs.paired == kPairedOnce + DK_MLP_GELU
+                                    ? 1.5957691216057308f * (gsum + 0.044715f * gsum * gsum * gsum)
+                                    : gsum;
+              *h = __float2half_rn(gsum / (1.0f + expf(-arg)) * sum);
+              continue;
+            }
             const float gv = __half2float(__float2half_rn(gsum));
             const float sg = __half2float(__float2half_rn(gv / (1.0f + expf(-gv))));
             const float u = __half2float(__float2half_rn(sum));
-            const Segment& s0 = a.segs.s[0];
-            s0.y[(size_t)b * s0.rows + trow + r] = __float2half_rn(__fmul_rn(sg, u));
+            *h = __float2half_rn(__fmul_rn(sg, u));
           } else {
             const Segment& sg = a.segs.s[tr.seg];
             sg.y[(size_t)b * sg.rows + trow + r] = __float2half_rn(sum);
@@ -2025,7 +2035,7 @@ extern "C" dk_status dk_w4a16_gemv_silu_mul(const int32_t* packed_gate,
     SegList segs;
     std::memset(&segs, 0, sizeof(segs));
     segs.n = 2;
-    segs.paired = 1;
+    segs.paired = kPairedUnfused;
     segs.s[0] = Segment{reinterpret_cast<const uint32_t*>(packed_gate),
                         reinterpret_cast<const __half*>(scales_gate), p.y, M, 0};
     segs.s[1] = Segment{reinterpret_cast<const uint32_t*>(packed_up),
@@ -2035,6 +2045,32 @@ extern "C" dk_status dk_w4a16_gemv_silu_mul(const int32_t* packed_gate,
     if (s != DK_OK) return s;
   }
   return DK_OK;
+}
+
+// The pair for at most 8 rows with h rounded once, for dk_w4a16_gemm (which has
+// checked its arguments).
+dk_status dk::stream_gated(const int32_t* const (&packed)[2], const uint16_t* const (&scales)[2], const void* x, void* h, int M, int K,
+                           int rows, dk_mlp_act act, cudaStream_t stream) {
+  stamp_begin_call();
+  if (2ll * M > (1ll << 30)) return DK_ERR_UNSUPPORTED;
+  GemvParams p;
+  p.packed = reinterpret_cast<const uint32_t*>(packed[0]);
+  p.scales = reinterpret_cast<const __half*>(scales[0]);
+  p.x = static_cast<const __half*>(x);
+  p.y = static_cast<__half*>(h);
+  p.M = 2 * M;  // rows streamed
+  p.K = K;
+  p.ldx = K;
+  p.B = rows;
+  p.ws = nullptr;
+  p.counters = nullptr;
+  SegList segs;
+  std::memset(&segs, 0, sizeof(segs));
+  segs.n = 2;
+  segs.paired = kPairedOnce + (int)act;
+  segs.s[0] = Segment{reinterpret_cast<const uint32_t*>(packed[0]), reinterpret_cast<const __half*>(scales[0]), p.y, M, 0};
+  segs.s[1] = Segment{reinterpret_cast<const uint32_t*>(packed[1]), reinterpret_cast<const __half*>(scales[1]), nullptr, M, 0};
+  return launch_stream_nt<5>(p, stream, false, &segs);
 }
 
 // ---------------------------------------------------------------------------

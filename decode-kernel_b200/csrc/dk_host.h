@@ -24,6 +24,11 @@ int current_device();
 // dk_gemv.cu), for kernels of other translation units; nullptr on failure.
 int* device_error_address();
 
+// A gated pair of GEMVs for at most 8 contiguous fp16 rows, h rounded once
+// (defined in dk_gemv.cu).
+dk_status stream_gated(const int32_t* const (&packed)[2], const uint16_t* const (&scales)[2], const void* x, void* h, int M, int K,
+                       int rows, dk_mlp_act act, cudaStream_t stream);
+
 inline dk_status check_launch(const char* where) {
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) {
