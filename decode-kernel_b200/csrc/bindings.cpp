@@ -690,7 +690,7 @@ std::tuple<torch::Tensor, OptTensor, OptTensor> w4a16_gemm(torch::Tensor packed,
   a.M = static_cast<int>(w.M);
   a.K = static_cast<int>(w.K);
   torch::Tensor workspace;
-  if (const size_t need = dk_w4a16_gemm_workspace_bytes(a.rows, a.K, a.dtype)) {
+  if (const size_t need = dk_w4a16_gemm_workspace_bytes(a.rows, a.K, packed2 ? 2 : 1, a.dtype)) {
     workspace = torch::empty({static_cast<int64_t>(need)}, x.options().dtype(torch::kUInt8));
     a.workspace = workspace.data_ptr();
     a.workspace_bytes = need;
@@ -881,6 +881,80 @@ std::tuple<torch::Tensor, torch::Tensor> cache_read(const Cache8& cache, torch::
   return {ko, vo};
 }
 
+// ---------------------------------------------------------------------------
+// Gradients.  The linear operators are each other's gradients (a turning's is the
+// turning back), so they may be differentiated any number of times.
+// ---------------------------------------------------------------------------
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+bool wants_grad(const torch::Tensor& x, const torch::Tensor& scales) {
+  if (!torch::GradMode::is_enabled()) return false;
+  TORCH_CHECK(!scales.requires_grad(), "the weights are frozen: scales must not require a gradient");
+  return x.requires_grad();
+}
+
+torch::Tensor linear(bool transposed, const torch::Tensor& packed, const torch::Tensor& scales, const torch::Tensor& x, OptTensor out);
+
+struct Linear : torch::autograd::Function<Linear> {
+  static torch::Tensor forward(AutogradContext* ctx, torch::Tensor x, torch::Tensor packed, torch::Tensor scales, bool transposed) {
+    ctx->save_for_backward({packed, scales});
+    ctx->saved_data["transposed"] = transposed;
+    const at::AutoDispatchBelowADInplaceOrView below;
+    return transposed ? w4a16_gemm_t(packed, scales, {}, {}, x, {}, {}) : std::get<0>(w4a16_gemm(packed, scales, {}, {}, x, 0, false, {}));
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    return {linear(!ctx->saved_data["transposed"].toBool(), saved[0], saved[1], grads[0], {}), {}, {}, {}};
+  }
+};
+
+torch::Tensor linear(bool transposed, const torch::Tensor& packed, const torch::Tensor& scales, const torch::Tensor& x, OptTensor out) {
+  if (wants_grad(x, scales)) {
+    TORCH_CHECK(!out, "out takes no part in a gradient: call without it or under torch.no_grad()");
+    return Linear::apply(x, packed, scales, transposed);
+  }
+  return transposed ? w4a16_gemm_t(packed, scales, {}, {}, x, {}, out) : std::get<0>(w4a16_gemm(packed, scales, {}, {}, x, 0, false, out));
+}
+
+using Pair = std::tuple<torch::Tensor, OptTensor>;
+Pair turn(torch::Tensor q, OptTensor k, torch::Tensor positions, torch::Tensor frequency, std::optional<std::vector<int64_t>> sections,
+          bool paired, bool inverse, bool inplace);
+
+struct Turn : torch::autograd::Function<Turn> {
+  static variable_list forward(AutogradContext* ctx, torch::Tensor q, OptTensor k, torch::Tensor positions, torch::Tensor frequency,
+                               std::optional<std::vector<int64_t>> sections, bool paired, bool inverse) {
+    ctx->save_for_backward({positions, frequency});
+    ctx->saved_data["sections"] = sections;
+    ctx->saved_data["paired"] = paired;
+    ctx->saved_data["inverse"] = inverse;
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const Pair both = rotary(q, k, positions, frequency, sections, paired, inverse, false);
+    return k ? variable_list{std::get<0>(both), *std::get<1>(both)} : variable_list{std::get<0>(both)};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    std::optional<std::vector<int64_t>> sections;
+    if (!ctx->saved_data["sections"].isNone()) sections = ctx->saved_data["sections"].toIntVector();
+    const Pair both = turn(grads[0], grads.size() > 1 ? OptTensor(grads[1]) : OptTensor(), saved[0], saved[1], sections,
+                           ctx->saved_data["paired"].toBool(), !ctx->saved_data["inverse"].toBool(), false);
+    return {std::get<0>(both), grads.size() > 1 ? *std::get<1>(both) : torch::Tensor(), {}, {}, {}, {}, {}};
+  }
+};
+
+Pair turn(torch::Tensor q, OptTensor k, torch::Tensor positions, torch::Tensor frequency, std::optional<std::vector<int64_t>> sections,
+          bool paired, bool inverse, bool inplace) {
+  if (torch::GradMode::is_enabled()) {
+    TORCH_CHECK(!frequency.requires_grad(), "frequency must not require a gradient");
+    if (q.requires_grad() || (k && k->requires_grad())) {
+      TORCH_CHECK(!inplace, "q and k that require a gradient are not turned in place");
+      const variable_list out = Turn::apply(q, k, positions, frequency, sections, paired, inverse);
+      return {out[0], k ? OptTensor(out[1]) : OptTensor()};
+    }
+  }
+  return rotary(q, k, positions, frequency, sections, paired, inverse, inplace);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -928,6 +1002,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("post_bias"), py::arg("gate"), py::arg("act"), py::arg("residual_scale"),
         py::arg("block_scale"), py::arg("pre_weight"), py::arg("pre_bias"), py::arg("eps"),
         py::arg("inplace"));
+  m.def("linear", &linear, "A product of rows, or the transposed one; differentiable", py::arg("transposed"), py::arg("packed"), py::arg("scales"),
+        py::arg("x"), py::arg("out") = py::none());
   m.def("w4a16_gemm", &w4a16_gemm, "Many rows through 4-bit weights, or through a gated pair", py::arg("packed"),
         py::arg("scales"), py::arg("packed2"), py::arg("scales2"), py::arg("x"), py::arg("act") = 0, py::arg("keep") = false,
         py::arg("out") = py::none());
@@ -935,7 +1011,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("scales2"), py::arg("g"), py::arg("g2") = py::none(), py::arg("out") = py::none());
   m.def("gated_grad", &gated_grad, "Gradients of a gated block's pre-activations", py::arg("dh"), py::arg("g"), py::arg("u"),
         py::arg("act"));
-  m.def("rotary", &rotary, "Rotary positions of queries and keys", py::arg("q"), py::arg("k"), py::arg("positions"),
+  m.def("rotary", &turn, "Rotary positions of queries and keys", py::arg("q"), py::arg("k"), py::arg("positions"),
         py::arg("frequency"), py::arg("sections"), py::arg("paired"), py::arg("inverse"), py::arg("inplace"));
   m.def("cache_read", &cache_read, "Keys and values of a paged 8-bit cache as rows", py::arg("cache"), py::arg("block_table"),
         py::arg("lengths"), py::arg("starts"), py::arg("tokens"), py::arg("dtype"), py::arg("k") = py::none(),

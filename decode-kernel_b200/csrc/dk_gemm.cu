@@ -937,7 +937,10 @@ dk_status launch_cluster(const char* name, void (*kernel)(Args), const Args& a, 
 }
 
 // ---- few rows ----
-constexpr int kFewRows = 32;
+// Up to 16 rows, 32 of a pair: us a call in a chain by it and by the fp16 form,
+// 16 rows, 4096 x 4096 12 / 11, 11008 x 4096 19 / 18, 28672 x 8192 46 / 60; 32 rows
+// 13 / 11, 23 / 19, 60 / 62; pairs with 32 rows 16 / 15, 29 / 37, 97 / 125.
+inline int few_limit(bool pair) { return pair ? 32 : 16; }
 
 inline int few_form(int rows) { return rows <= 4 ? 4 : rows <= 16 ? 16 : 32; }
 inline size_t few_pieces(int rows, int groups, bool bf16) {
@@ -1042,7 +1045,7 @@ dk_status product(const Product& p, cudaStream_t stream) {
                               nullptr, nullptr, 0, stream);
       if (st != DK_ERR_UNSUPPORTED) return st;
     }
-    if (p.rows <= kFewRows) return p.bf16 ? few_product<true, MODE>(p, stream) : few_product<false, MODE>(p, stream);
+    if (p.rows <= few_limit(MODE == kGated)) return p.bf16 ? few_product<true, MODE>(p, stream) : few_product<false, MODE>(p, stream);
   }
   TileArgs a{};
   a.scales[0] = reinterpret_cast<const __half*>(p.scales[0]);
@@ -1189,8 +1192,8 @@ dk_status launch_grad(GradArgs& a, int rows, bool wide, cudaStream_t st) {
 
 using namespace dk;
 
-extern "C" size_t dk_w4a16_gemm_workspace_bytes(int rows, int K, dk_dtype dtype) {
-  if (rows < 1 || rows > kFewRows || K < DK_GROUP_SIZE || K % DK_GROUP_SIZE || (dtype != DK_FP16 && dtype != DK_BF16)) return 0;
+extern "C" size_t dk_w4a16_gemm_workspace_bytes(int rows, int K, int matrices, dk_dtype dtype) {
+  if (matrices < 1 || matrices > 2 || rows < 1 || rows > few_limit(matrices == 2) || K < DK_GROUP_SIZE || K % DK_GROUP_SIZE || (dtype != DK_FP16 && dtype != DK_BF16)) return 0;
   return few_bytes(rows, K / DK_GROUP_SIZE, dtype == DK_BF16);
 }
 
@@ -1206,7 +1209,7 @@ extern "C" dk_status dk_w4a16_gemm(const dk_gemm_args* p, void* stream) {
   if (!aligned16(p->packed) || !aligned16(p->packed2) || !aligned16(p->x)) return DK_ERR_INVALID_ARG;
   if (p->rows > 1 && (p->ldx < p->K || p->ldx % 8 || p->ldy < p->M || (p->gate_out && p->ldk < p->M)))
     return DK_ERR_INVALID_ARG;
-  const size_t need = dk_w4a16_gemm_workspace_bytes(p->rows, p->K, p->dtype);
+  const size_t need = dk_w4a16_gemm_workspace_bytes(p->rows, p->K, p->packed2 ? 2 : 1, p->dtype);
   if (need && (!p->workspace || p->workspace_bytes < need || (reinterpret_cast<uintptr_t>(p->workspace) & 127u))) return DK_ERR_WORKSPACE;
   Product a{};
   a.workspace = p->workspace;

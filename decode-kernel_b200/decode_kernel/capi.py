@@ -221,7 +221,7 @@ SIGNATURES = {
     "dk_cache_attention_counter_bytes": (_SZ, []),
     "dk_cache_attention": (_I, [ctypes.POINTER(CacheAttentionArgs), _P, _SZ, _P]),
     "dk_block_norm": (_I, [ctypes.POINTER(BlockNormArgs), _P]),
-    "dk_w4a16_gemm_workspace_bytes": (_SZ, [_I, _I, _I]),
+    "dk_w4a16_gemm_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
     "dk_w4a16_gemm": (_I, [ctypes.POINTER(GemmArgs), _P]),
     "dk_w4a16_gemm_t": (_I, [ctypes.POINTER(GemmTArgs), _P]),
     "dk_gated_grad": (_I, [_P, _P, _P, _P, _P, _I, _I, _L, _L, _L, _I, _I, _P]),

@@ -20,39 +20,6 @@ __all__ = ["gemm", "gemm_gated", "gemm_t"]
 _ACTS = {"silu": 0, "gelu": 1}
 
 
-def _wants_grad(x: torch.Tensor, *scales: torch.Tensor) -> bool:
-    if not torch.is_grad_enabled():
-        return False
-    if any(s.requires_grad for s in scales):
-        raise RuntimeError("the weights are frozen: scales must not require a gradient")
-    return x.requires_grad
-
-
-class _Gemm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, packed, scales):
-        ctx.save_for_backward(packed, scales)
-        return _extension().w4a16_gemm(packed, scales, None, None, x)[0]
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        return _extension().w4a16_gemm_t(*ctx.saved_tensors, None, None, dy), None, None
-
-
-class _GemmT(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, g, packed, scales):
-        ctx.save_for_backward(packed, scales)
-        return _extension().w4a16_gemm_t(packed, scales, None, None, g)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dx):
-        packed, scales = ctx.saved_tensors
-        return _extension().w4a16_gemm(packed, scales, None, None, dx)[0], None, None
-
-
 class _GemmGated(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate, gate_scales, up, up_scales, act):
@@ -70,11 +37,6 @@ class _GemmGated(torch.autograd.Function):
         return dx.view(*dh.shape[:-1], dx.shape[-1]), None, None, None, None, None
 
 
-def _no_out(out: Optional[torch.Tensor]) -> None:
-    if out is not None:
-        raise RuntimeError("out takes no part in a gradient: call without it or under torch.no_grad()")
-
-
 def gemm(packed: torch.Tensor, scales: torch.Tensor, x: torch.Tensor, *,
          out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x . dequant(W)^T for any number of rows: fp16 or bf16 [..., K] -> [..., M].
@@ -85,10 +47,7 @@ def gemm(packed: torch.Tensor, scales: torch.Tensor, x: torch.Tensor, *,
     rows that do not begin on 16-byte boundaries are copied first.  ``out`` is
     contiguous or has contiguous rows.  Differentiable in x.
     """
-    if _wants_grad(x, scales):
-        _no_out(out)
-        return _Gemm.apply(x, packed, scales)
-    return _extension().w4a16_gemm(packed, scales, None, None, x, 0, False, out)[0]
+    return _extension().linear(False, packed, scales, x, out)
 
 
 def gemm_t(packed: torch.Tensor, scales: torch.Tensor, g: torch.Tensor, *,
@@ -97,10 +56,7 @@ def gemm_t(packed: torch.Tensor, scales: torch.Tensor, g: torch.Tensor, *,
 
     The same types and roundings as ``gemm``.  Differentiable in g.
     """
-    if _wants_grad(g, scales):
-        _no_out(out)
-        return _GemmT.apply(g, packed, scales)
-    return _extension().w4a16_gemm_t(packed, scales, None, None, g, None, out)
+    return _extension().linear(True, packed, scales, g, out)
 
 
 def gemm_gated(gate: Tuple[torch.Tensor, torch.Tensor], up: Tuple[torch.Tensor, torch.Tensor], x: torch.Tensor, *,
@@ -115,7 +71,10 @@ def gemm_gated(gate: Tuple[torch.Tensor, torch.Tensor], up: Tuple[torch.Tensor, 
     """
     if act not in _ACTS:
         raise ValueError("act is 'silu' or 'gelu'")
-    if _wants_grad(x, gate[1], up[1]):
-        _no_out(out)
+    if torch.is_grad_enabled() and (x.requires_grad or gate[1].requires_grad or up[1].requires_grad):
+        if gate[1].requires_grad or up[1].requires_grad:
+            raise RuntimeError("the weights are frozen: scales must not require a gradient")
+        if out is not None:
+            raise RuntimeError("out takes no part in a gradient: call without it or under torch.no_grad()")
         return _GemmGated.apply(x, *gate, *up, _ACTS[act])
     return _extension().w4a16_gemm(*gate, *up, x, _ACTS[act], False, out)[0]

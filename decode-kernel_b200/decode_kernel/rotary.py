@@ -5,27 +5,10 @@ from __future__ import annotations
 from typing import Optional, Sequence, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .cache import _extension
 
 __all__ = ["rotary"]
-
-
-class _Rotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, positions, frequency, sections, paired, inverse):
-        ctx.save_for_backward(positions, frequency)
-        ctx.form = sections, paired, inverse
-        q, k = _extension().rotary(q, k, positions, frequency, sections, paired, inverse, False)
-        return q, k
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dq, dk):
-        sections, paired, inverse = ctx.form
-        dq, dk = _extension().rotary(dq, dk, *ctx.saved_tensors, sections, paired, not inverse, False)
-        return dq, dk, None, None, None, None, None
 
 
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, frequency: torch.Tensor, *,
@@ -48,10 +31,4 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     turning are fp32, rounded once.  ``inverse`` turns back.  ``inplace`` writes
     over q and k.  Differentiable in q and k (not in place).
     """
-    if frequency.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("frequency must not require a gradient")
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        if inplace:
-            raise RuntimeError("q and k that require a gradient are not turned in place")
-        return _Rotary.apply(q, k, positions, frequency, sections, paired, inverse)
     return _extension().rotary(q, k, positions, frequency, sections, paired, inverse, inplace)

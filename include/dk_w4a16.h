@@ -522,15 +522,15 @@ DK_API dk_status dk_block_norm(const dk_block_norm_args* args, void* stream);
  *   act(g) = g * sigmoid(p(g)); DK_MLP_SILU: p = g; DK_MLP_GELU (its tanh
  *   form): p = 2 sqrt(2 / pi) (g + 0.044715 g^3)
  * of which gate_out and up_out (both or neither) keep g and u, rounded.
- * x and the outputs are DK_FP16 or DK_BF16.  Up to 32 rows the sums of a group's
- * 128 products q * x are exact (of x what is above 2^-25 (fp16) or 2^-21 (bf16)
- * of its row's largest in the group) and are added in fp32 with their scales;
- * with more rows each weight q * scale is rounded once to x's type (past its range
- * to infinity) and products and sums are fp32.  Outputs are rounded once.  Up to
- * 32 rows need a workspace of dk_w4a16_gemm_workspace_bytes (0 with more), 128-byte
- * aligned, which may hold anything; calls that share one must be ordered on the
- * GPU, and so the kernel before a call on the stream may write packed and scales.
- * Rows are ldx (x), ldy (y) and ldk (gate_out and
+ * x and the outputs are DK_FP16 or DK_BF16.  Up to 16 rows, 32 of a pair, the
+ * sums of a group's 128 products q * x are exact to fp32 (of x what is above 2^-25
+ * (fp16) or 2^-21 (bf16) of its row's largest in the group) and are added in fp32
+ * with their scales; with more rows each weight q * scale is rounded once to x's
+ * type (past its range to infinity) and products and sums are fp32.  Outputs are
+ * rounded once.  The first form needs a workspace of dk_w4a16_gemm_workspace_bytes
+ * (matrices: 1, or 2 for a pair; 0 bytes for more rows), 128-byte aligned, which
+ * may hold anything; calls that share one must be ordered on the GPU.
+ *  * Rows are ldx (x), ldy (y) and ldk (gate_out and
  * up_out) values apart; x and packed are 16-byte aligned and ldx is a multiple
  * of 8 (where rows > 1).  Outputs may not overlap the inputs. */
 typedef enum dk_mlp_act { DK_MLP_SILU = 0, DK_MLP_GELU = 1 } dk_mlp_act;
@@ -550,7 +550,7 @@ typedef struct dk_gemm_args {
   void* workspace;
   size_t workspace_bytes;
 } dk_gemm_args;
-DK_API size_t dk_w4a16_gemm_workspace_bytes(int rows, int K, dk_dtype dtype);
+DK_API size_t dk_w4a16_gemm_workspace_bytes(int rows, int K, int matrices, dk_dtype dtype);
 DK_API dk_status dk_w4a16_gemm(const dk_gemm_args* args, void* stream);
 
 /* The transposed product, which is the gradient of x in the one above:

@@ -50,9 +50,11 @@ def test_gemm_t_rejects(kw):
 
 def test_few_rows_need_a_workspace():
     need = capi.load().dk_w4a16_gemm_workspace_bytes
-    assert need(1, 256, capi.DK_FP16) > 0 and need(32, 256, capi.DK_BF16) > 0
-    assert need(33, 256, capi.DK_FP16) == need(0, 256, capi.DK_FP16) == need(1, 200, capi.DK_FP16) == need(1, 256, capi.DK_FP32) == 0
-    size = need(4, 256, capi.DK_FP16)
+    assert need(1, 256, 1, capi.DK_FP16) > 0 and need(16, 256, 1, capi.DK_BF16) > 0 and need(32, 256, 2, capi.DK_BF16) > 0
+    for bad in ((17, 256, 1, capi.DK_FP16), (33, 256, 2, capi.DK_FP16), (0, 256, 1, capi.DK_FP16), (1, 200, 1, capi.DK_FP16), (1, 256, 1, capi.DK_FP32),
+                (1, 256, 0, capi.DK_FP16), (1, 256, 3, capi.DK_FP16)):
+        assert need(*bad) == 0
+    size = need(4, 256, 1, capi.DK_FP16)
     for kw in (dict(), dict(workspace=1024, workspace_bytes=size - 1), dict(workspace=1088, workspace_bytes=size)):
         assert capi.load().dk_w4a16_gemm(ctypes.byref(gemm_args(**kw)), None) == capi.DK_ERR_WORKSPACE
 

@@ -28,15 +28,15 @@ def weights(M, K, seed):
     return packed, scales.half()
 
 
-FEW = 32  # rows up to which the products take the weights as they are
+FEW, FEW_OF_PAIR = 16, 32  # rows up to which the products take the weights as they are
 
 
-def values(w, dtype, rows=FEW + 1):
+def values(w, dtype, rows=1000, few=FEW):
     """The weights as the products use them: q * scale, rounded once to the rows' type where there are many."""
     packed, scales = w
     q = torch.stack([(packed << (28 - 4 * i)) >> 28 for i in range(8)], -1).reshape(packed.shape[0], -1)
     v = q.float() * scales.float().repeat_interleave(128, 1)
-    return (v.to(dtype) if rows > FEW else v).double()
+    return (v.to(dtype) if rows > few else v).double()
 
 
 def rows_of(T, n, dtype, seed):
@@ -56,9 +56,9 @@ def sum_error(total, depth):
     return total * (depth / 16 + 16) * 2.0 ** -23
 
 
-def lost(x, w):
+def lost(x, w, few=FEW):
     """What few rows lose of values that are small beside their row's largest in the group: 2^-25 of that (fp16) or 2^-21 (bf16)."""
-    if x.shape[0] > FEW or x.shape[1] % 128:
+    if x.shape[0] > few or x.shape[1] % 128:
         return 0.0
     most = x.double().abs().unflatten(1, (-1, 128)).amax(-1, keepdim=True).expand(-1, -1, 128).flatten(1)
     return most @ w.abs() * (2.0 ** -25 if x.dtype == torch.float16 else 2.0 ** -21)
@@ -110,7 +110,7 @@ def check_gated(h, x, wg, wu, act, depth):
     """|act'| <= 1.13 for both forms; the sigmoid's exponential is 2^-21 off times its argument."""
     xd = x.double()
     g, u = xd @ wg.t(), xd @ wu.t()
-    eg, eu = (sum_error(xd.abs() @ w.abs().t(), depth) + lost(x, w.t()) for w in (wg, wu))
+    eg, eu = (sum_error(xd.abs() @ w.abs().t(), depth) + lost(x, w.t(), FEW_OF_PAIR) for w in (wg, wu))
     a, _, p = act_parts(g, act)
     want = a * u
     bound = want.abs() * (half_step(h.dtype) + (2 + p.abs()) * 2.0 ** -21) + 1.2 * eg * (u.abs() + eu) + a.abs() * eu + 2.0 ** -25
@@ -124,7 +124,7 @@ def check_gated(h, x, wg, wu, act, depth):
 def test_gemm_gated(T, M, K, dtype, act):
     wg, wu = weights(M, K, T + M + 2), weights(M, K, T + M + 3)
     x = rows_of(T, K, HALF[dtype], K + T + 2)
-    check_gated(dk.gemm_gated(wg, wu, x, act=act), x, values(wg, x.dtype, T), values(wu, x.dtype, T), act, K)
+    check_gated(dk.gemm_gated(wg, wu, x, act=act), x, values(wg, x.dtype, T, FEW_OF_PAIR), values(wu, x.dtype, T, FEW_OF_PAIR), act, K)
 
 
 def gated_gradient(x, dh, wg, wu, act, depth, M):
@@ -134,8 +134,8 @@ def gated_gradient(x, dh, wg, wu, act, depth, M):
     e = half_step(x.dtype)
     xd, d = x.double(), dh.double()
     g, u = xd @ wg.t(), xd @ wu.t()
-    few = e if len(x) <= FEW else 0.0
-    eg, eu = (p.abs() * e + few * (xd.abs() @ w.abs().t()) + sum_error(xd.abs() @ w.abs().t(), depth) + lost(x, w.t()) for p, w in ((g, wg), (u, wu)))
+    few = e if len(x) <= FEW_OF_PAIR else 0.0
+    eg, eu = (p.abs() * e + few * (xd.abs() @ w.abs().t()) + sum_error(xd.abs() @ w.abs().t(), depth) + lost(x, w.t(), FEW_OF_PAIR) for p, w in ((g, wg), (u, wu)))
     a, slope, p = act_parts(g, act)
     dg, du = d * u * slope, d * a
     more = (2 + p.abs()) * 2.0 ** -20 + e
@@ -155,7 +155,7 @@ def test_gemm_gated_gradient(T, M, K, dtype, act):
     h = dk.gemm_gated(wg, wu, x, act=act)
     dx, = torch.autograd.grad(h, x, dh)
     vg, vu = values(wg, x.dtype), values(wu, x.dtype)
-    check_gated(h.detach(), x.detach(), values(wg, x.dtype, T), values(wu, x.dtype, T), act, K)
+    check_gated(h.detach(), x.detach(), values(wg, x.dtype, T, FEW_OF_PAIR), values(wu, x.dtype, T, FEW_OF_PAIR), act, K)
     want, bound = gated_gradient(x.detach(), dh, vg, vu, act, K, M)
     off = (dx.double() - want).abs()
     assert (off <= bound).all(), float((off / bound).max())
@@ -180,6 +180,11 @@ def test_gradient_of_gemm_and_linear(dtype):
     g = dy.clone().requires_grad_()
     back, = torch.autograd.grad(dk.gemm_t(*w, g), g, x.detach())
     check_product(back, x.detach(), values(w, x.dtype, T).t(), depth=K)
+    # The operators are linear: a gradient's gradient is the product itself.
+    seed = dy.clone().requires_grad_()
+    once, = torch.autograd.grad(dk.gemm(*w, x), x, seed, create_graph=True)
+    twice, = torch.autograd.grad(once, seed, x.detach())
+    assert torch.equal(twice, dk.gemm(*w, x.detach()))
     if dtype == "fp16":
         layer = dk.W4A16Linear(*w)
         y = layer(x)
