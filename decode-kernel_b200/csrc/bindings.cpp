@@ -13,6 +13,7 @@
 // device_error, and the rest of a decode step: Cache8 (a paged 8-bit cache's
 // tensors, checked once), cache_plan, cache_append, cache_attention, block_norm.
 // Every C-ABI status other than DK_OK becomes a RuntimeError.
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -648,6 +649,7 @@ torch::Tensor output(const OptTensor& out, const std::vector<int64_t>& shape, co
               "out must have the product's shape and x's type and device");
   TORCH_CHECK(out->is_contiguous() || (out->dim() == 2 && out->stride(1) == 1 && out->stride(0) >= out->size(1)),
               "out must have contiguous rows");
+  at::assert_no_overlap(*out, x);
   return *out;
 }
 
@@ -820,7 +822,10 @@ std::tuple<torch::Tensor, OptTensor> rotary(torch::Tensor q, OptTensor k, torch:
   std::pair<torch::Tensor, torch::Tensor> ks;
   if (k) {
     ks = place(*k, a.k, a.k_out, a.k_token_stride, a.k_head_stride, a.k_out_token_stride, a.k_out_head_stride);
-    TORCH_CHECK(!inplace || k->data_ptr() != q.data_ptr() || tokens == 0, "q and k that are turned in place must be two tensors");
+    const at::MemOverlapStatus both = at::get_overlap_status(q, *k);
+    TORCH_CHECK(!inplace || tokens == 0 ||
+                    (k->data_ptr() != q.data_ptr() && both != at::MemOverlapStatus::Full && both != at::MemOverlapStatus::Partial),
+                "q and k that are turned in place must be two tensors");
     a.kv_heads = static_cast<int>(k->size(1));
   }
   a.positions = at.data_ptr();
@@ -863,6 +868,7 @@ std::tuple<torch::Tensor, torch::Tensor> cache_read(const Cache8& cache, torch::
     return *t;
   };
   const torch::Tensor ko = given(k, "k"), vo = given(v, "v");
+  TORCH_CHECK(tokens == 0 || ko.data_ptr() != vo.data_ptr(), "k and v must be two tensors");
   dk_cache_read_args a{};
   a.cache = cache.c;
   a.block_table = block_table.data_ptr<int32_t>();

@@ -325,7 +325,7 @@ template <int MODE, int CG>
 struct Place {
   static constexpr bool kATmem = CG == 1 || MODE != kTransposed;
   static constexpr int kSums = CG == 2 && kATmem ? 192 : 256;  // columns of a tile's sums
-  static constexpr int kA = CG == 1 ? 256 : 384;
+  static constexpr int kA = !kATmem ? 512 : CG == 1 ? 256 : 384;  // its first column
   static constexpr int kABits = CG == 1 ? 2 : 1;
 };
 constexpr int kABytes = kLanes * kStepDepth * 2;  // A of a step in shared memory
@@ -936,6 +936,32 @@ dk_status launch_cluster(const char* name, void (*kernel)(Args), const Args& a, 
   return DK_OK;
 }
 
+// How many clusters of `size` CTAs, one to an SM, run at once: the device's
+// property (its SMs are not a multiple of eight in every part), asked for once.
+template <typename Args>
+int clusters_at_once(void (*kernel)(Args), int threads, size_t smem, int size) {
+  static std::atomic<int> known[64][9];
+  std::atomic<int>& at = known[current_device() & 63][size];
+  int most = at.load(std::memory_order_relaxed);
+  if (most) return most;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = size;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(size * sm_count(-1));
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&most, kernel, &cfg) != cudaSuccess || most < 1) {
+    (void)cudaGetLastError();
+    most = std::max(1, sm_count(-1) / size - (size > 2));
+  }
+  at.store(most, std::memory_order_relaxed);
+  return most;
+}
+
 // ---- few rows ----
 // Up to 16 rows, 32 of a pair: us a call in a chain by it and by the fp16 form,
 // 16 rows, 4096 x 4096 12 / 11, 11008 x 4096 19 / 18, 28672 x 8192 46 / 60; 32 rows
@@ -973,31 +999,10 @@ dk_status few_product(const Product& p, cudaStream_t stream) {
   a.K = p.K;
   a.act = p.act;
   a.tiles = ceil_div(p.M, MODE == kGated ? 64 : 128);
-  // The cluster's size that leaves the fewest steps to its busiest CTA.  How
-  // many clusters of a size run at once is the device's property.
-  static std::atomic<int> at_once[64][4];
-  const int device = current_device() & 63;
+  // The cluster's size that leaves the fewest steps to its busiest CTA.
   int best = 0;
-  for (int i = 0; i < 4; ++i) {
-    const int size = 1 << i;
-    int most = at_once[device][i].load(std::memory_order_relaxed);
-    if (!most) {
-      cudaLaunchAttribute attr[1];
-      attr[0].id = cudaLaunchAttributeClusterDimension;
-      attr[0].val.clusterDim.x = size;
-      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-      cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3(size * sm_count(-1));
-      cfg.blockDim = dim3(F::kThreads);
-      cfg.dynamicSmemBytes = F::kSmem;
-      cfg.attrs = attr;
-      cfg.numAttrs = 1;
-      if (cudaOccupancyMaxActiveClusters(&most, kernel, &cfg) != cudaSuccess || most < 1) {
-        (void)cudaGetLastError();
-        most = std::max(1, sm_count(-1) / size);
-      }
-      at_once[device][i].store(most, std::memory_order_relaxed);
-    }
+  for (int size = 1; size <= 8; size *= 2) {
+    const int most = clusters_at_once(kernel, F::kThreads, F::kSmem, size);
     const int clusters = std::min(a.tiles, most);
     const int steps = ceil_div((int64_t)ceil_div(a.tiles, clusters) * a.groups, size);
     if (!best || steps < best) best = steps, a.cluster = size, a.clusters = clusters;
@@ -1066,47 +1071,52 @@ dk_status product(const Product& p, cudaStream_t stream) {
   a.steps = a.matrix_steps * (MODE == kTransposed ? p.matrices : 1);
   const int tiles = MODE == kPlain ? ceil_div(p.M, 128) : MODE == kGated ? ceil_div(p.M, 64) : a.groups;
   const int sms = sm_count(-1);
+  static std::atomic<unsigned long long> asked{0};
+  const dk_status allowed = allow_smem(k_gemm<false, MODE, 1>, asked);  // before it is asked about
+  if (allowed != DK_OK) return allowed;
 
-  // Few rows: one tile of tokens a CTA, the depth over the CTAs of a cluster so
-  // that all SMs work.  Many: pairs.
-  const bool pair = p.rows > 128;
-  int cluster;
-  unsigned grid;
-  if (pair) {
-    a.lane_tiles = (tiles + 1) / 2;
-    const int pairs = sms / 2;
-    // The width of the token tiles (a multiple of 32) that leaves the least to do
-    // for the busiest pair.  In cycles, as measured: a step takes 4 a token, and no
-    // less than its unpacking or its way through shared memory; where the sums
-    // have one place only, the next tile waits until they are read.
-    using At = Place<MODE, 2>;
-    long long best = 0;
-    for (int width = 64; width <= 256; width += 32) {
-      const long long tiles_each = ceil_div((int64_t)a.lane_tiles * ceil_div(p.rows, width), pairs);
-      const int step = At::kATmem ? std::max(4 * width, 650) : std::max(4 * width, 640 + 2 * width);
-      const int read = 20 * width, wait = width > At::kSums ? read : 0;
-      const long long cost = tiles_each * ((long long)a.steps * step + wait) + read;
-      if (!best || cost <= best) best = cost, a.tokens = width;
-    }
-    a.places = a.tokens > At::kSums ? 1 : 2;
-    a.token_tiles = ceil_div(p.rows, a.tokens);
-    cluster = 2;
-    grid = 2 * std::min((int64_t)pairs, (int64_t)a.lane_tiles * a.token_tiles);
-    a.split = 1;
-    a.raw_stages = 4;
-  } else {
-    a.lane_tiles = tiles;
-    a.tokens = std::max(16, ceil_div(p.rows, 16) * 16);
-    a.token_tiles = 1;
-    a.split = std::max(1, std::min({8, a.steps, sms / std::max(1, tiles)}));
-    while (tiles * (int64_t)a.split > sms && a.split > 1) --a.split;
-    cluster = a.split;
-    if ((int64_t)tiles * a.split > INT32_MAX) return DK_ERR_UNSUPPORTED;
-    grid = (unsigned)tiles * a.split;
-    a.raw_stages = 8;
-    a.places = 1;
+  // The form and the width of the token tiles that leave the least to do for the
+  // busiest CTA, in cycles as measured.  A step takes 4 cycles a token, and no less
+  // than its unpacking (850 cycles for the 128 lanes of a CTA alone, 1400 where it
+  // turns nibbles, 650 beside a pair's other half) or its way through shared
+  // memory; a CTA's beginning and end 7500, reading a tile's sums 20 a
+  // token, adding those of a split 4000.
+  //   Pairs go from tile to tile; where the sums have one place only, the next
+  // tile waits until they are read.
+  //   CTAs alone take a tile each with the depth over up to eight of them.
+  // us by pairs and by CTAs alone: 333 rows, 1000 x 2816 12.9 / 10.8; 129 rows,
+  // 4096 x 4096 16.5 / 14.9; 128 rows, 14336 x 4096 17.8 / 20.6; 64 rows, 28672 x
+  // 8192 59.6 / 61.9; 700 rows, 1024 x 1024 8.0 / 9.8.
+  using At = Place<MODE, 2>;
+  const int pairs = sms / 2;
+  long long best = 0;
+  bool pair = true;
+  for (int width = 64; width <= 256; width += 32) {
+    const long long each = ceil_div((int64_t)(tiles + 1) / 2 * ceil_div(p.rows, width), pairs);
+    const int step = At::kATmem ? std::max(4 * width, 650) : std::max(4 * width, 640 + 2 * width);
+    const int read = 20 * width, wait = width > At::kSums ? read : 0;
+    const long long cost = each * ((long long)a.steps * step + wait) + read + 7500;
+    if (!best || cost <= best) best = cost, a.tokens = width;
   }
-  if ((int64_t)a.lane_tiles * a.token_tiles > INT32_MAX / 4) return DK_ERR_UNSUPPORTED;
+  for (int width = 16; width <= 128; width += 16) {
+    const int of_tokens = ceil_div(p.rows, width);
+    if (of_tokens > 1 && width % kBoxTokens) continue;  // sums are read 32 tokens at a time: no further than the last tile's end
+    const long long items = (int64_t)tiles * of_tokens;
+    const int split = (int)std::max<long long>(1, std::min<long long>({8, a.steps, sms / items}));
+    const int at_once = clusters_at_once(k_gemm<false, MODE, 1>, kGemmThreads, kSmemLeast, split);
+    const long long cost = ceil_div(items, at_once) *
+                           ((long long)ceil_div(a.steps, split) * std::max(4 * width, MODE == kTransposed ? 1400 : 850) + 20 * width + 7500 + (split > 1 ? 4000 : 0));
+    if (cost <= best) best = cost, pair = false, a.tokens = width, a.split = split;
+  }
+  a.token_tiles = ceil_div(p.rows, a.tokens);
+  a.lane_tiles = pair ? (tiles + 1) / 2 : tiles;
+  const int64_t items = (int64_t)a.lane_tiles * a.token_tiles;
+  if (items > INT32_MAX / 8) return DK_ERR_UNSUPPORTED;
+  if (pair) a.split = 1;
+  a.places = pair && a.tokens <= At::kSums ? 2 : 1;
+  a.raw_stages = pair ? 4 : 8;
+  const int cluster = pair ? 2 : a.split;
+  const unsigned grid = (unsigned)(pair ? 2 * std::min<int64_t>(pairs, items) : items * a.split);
   const int b_rows = a.tokens / (pair ? 2 : 1);
   const int a_bytes = !pair || Place<MODE, 2>::kATmem ? 0 : 2 * kABytes;
   a.b_stages = std::min(pair ? 8 : kMaxB, (kSmemMost - gemm_smem(a_bytes, 0, 0, a.raw_stages).total) / (b_rows * 256));

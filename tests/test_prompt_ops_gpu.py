@@ -10,6 +10,7 @@ import pytest
 import torch
 
 import decode_kernel as dk
+from decode_kernel import capi
 
 pytestmark = pytest.mark.gpu
 
@@ -193,6 +194,27 @@ def test_gradient_of_gemm_and_linear(dtype):
         assert torch.equal(dx, dx2)
 
 
+def test_gradients_of_any_layout():
+    """Gradients that come broadcast, transposed or with more dimensions, of inputs that are views."""
+    M, K, T = 120, 256, 24
+    w, w2 = weights(M, K, 14), weights(M, K, 15)
+    base = rows_of(T, 2 * K, torch.float16, 16)
+    for view in (lambda b: b[:, :K], lambda b: b[:, 8:K + 8].reshape(2, T // 2, K), lambda b: b[:1, :K].expand(T, K)):
+        for call in (lambda x: dk.gemm(*w, x), lambda x: dk.gemm_gated(w, w2, x)):
+            leaf = base.clone().requires_grad_()
+            x = view(leaf)
+            call(x).float().sum().backward()  # the gradient of the output is one number, broadcast
+            alone = x.detach().clone().requires_grad_()
+            dx, = torch.autograd.grad(call(alone), alone, torch.ones(*alone.shape[:-1], M, dtype=torch.float16, device="cuda"))
+            want = base.clone().requires_grad_()
+            view(want).backward(dx)
+            assert torch.equal(leaf.grad, want.grad)
+    g = rows_of(M, T, torch.float16, 17).t()
+    x = rows_of(T, K, torch.float16, 18).requires_grad_()
+    dx, = torch.autograd.grad(dk.gemm(*w, x), x, g)
+    assert torch.equal(dx, dk.gemm_t(*w, g.contiguous()))
+
+
 def test_gated_mlp_module_runs_and_trains():
     dim, hidden = 256, 384
     g = gen(10)
@@ -249,7 +271,7 @@ def test_packed_that_begins_off_16_bytes():
     assert torch.equal(dk.gemm(shifted, scales, x), dk.gemm(packed, scales, x))
 
 
-@pytest.mark.parametrize("T", [3, 40, 300])
+@pytest.mark.parametrize("T", [3, 12, 24, 40, 300])
 def test_rows_with_infinities_and_nan_stay_to_themselves(T):
     M, K = 300, 512
     w, w2 = weights(M, K, 40), weights(M, K, 41)
@@ -351,6 +373,8 @@ def test_product_refusals():
         lambda: dk.gemm_gated((packed, scales), (packed[:32], scales[:32]), x), lambda: dk.gemm_t(packed, scales, x),
         lambda: dk.gemm(packed, scales, x.clone().requires_grad_(), out=torch.empty(4, M, dtype=torch.float16, device="cuda")),
         lambda: dk.gemm(packed, scales, torch.zeros((), dtype=torch.float16, device="cuda")),
+        lambda: dk.gemm(packed, scales, x, out=x.view(-1)[:4 * M].view(4, M)),
+        lambda: dk.gemm(packed, scales.clone().requires_grad_(), x), lambda: dk.gemm_gated((packed, scales), (packed, scales.clone().requires_grad_()), x),
     ]
     for i, call in enumerate(bad):
         with pytest.raises(RuntimeError):
@@ -474,6 +498,18 @@ def test_rotary_of_far_positions():
     assert torch.equal(dk.rotary(odd, None, positions, frequency)[0], out)
 
 
+def test_rotary_gradient_of_a_gradient():
+    """Turning is linear: the gradient's gradient is the turning itself."""
+    q, k, positions, frequency = rotary_case(9, 4, 2, 64, [20, 12], False, "fp32")
+    dq = torch.randn_like(q).requires_grad_()
+    q.requires_grad_()
+    out, _ = dk.rotary(q, k, positions, frequency, sections=[20, 12])
+    once, = torch.autograd.grad(out, q, dq, create_graph=True)
+    v = torch.randn_like(q)
+    twice, = torch.autograd.grad(once, dq, v)
+    assert torch.equal(twice, dk.rotary(v, None, positions, frequency, sections=[20, 12])[0])
+
+
 def test_rotary_refusals():
     q, k, positions, frequency = rotary_case(6, 4, 2, 64, [20, 12], False, "fp16")
     good = dict(sections=[20, 12])
@@ -486,6 +522,7 @@ def test_rotary_refusals():
         lambda: dk.rotary(q.cpu(), None, positions, frequency, **good), lambda: dk.rotary(q[..., :63], None, positions, torch.ones(32, device="cuda"), **good),
         lambda: dk.rotary(q, q, positions, frequency, inplace=True, **good), lambda: dk.rotary(q[0], None, positions, frequency, **good),
         lambda: dk.rotary(q[:, :1].expand(6, 4, 64), None, positions, frequency, inplace=True, **good),
+        lambda: dk.rotary(q.view(-1)[:768].view(6, 2, 64), q.view(-1)[64:832].view(6, 2, 64), positions, frequency, inplace=True, **good),
         lambda: dk.rotary(q.double(), None, positions, frequency, **good), lambda: dk.rotary(q, k, positions.repeat(3, 1), frequency, **good),
         lambda: dk.rotary(q.transpose(1, 2), None, positions, frequency[:2], sections=[1, 1], inplace=True),
     ]
@@ -566,7 +603,7 @@ def test_cache_read_of_other_layouts_and_bad_pages():
         assert torch.equal(o[:16], (p[2].float() * s[2][:, None]).half()) and torch.equal(o[48:64], (p[4].float() * s[4][:, None]).half())
         assert (o[16:48] == 0).all() and (o[64:] == 0).all()  # outside the pool; past the table
     assert (wide[:, heads * dim:2 * heads * dim] == 0).all()
-    for bad in (dict(out=(k, v[:, :1])), dict(dtype=torch.float32), dict(out=(wide[:, 1:129].unflatten(1, (2, 64)), v))):
+    for bad in (dict(out=(k, k)), dict(out=(k, v[:, :1])), dict(dtype=torch.float32), dict(out=(wide[:, 1:129].unflatten(1, (2, 64)), v))):
         with pytest.raises(RuntimeError):
             dk.cache_read(cache, table, lengths, starts, 80, **bad)
     with pytest.raises(RuntimeError):
@@ -637,3 +674,39 @@ def test_a_prompt_step(code):
     h = dk.gemm_gated(w["gate"], w["up"], y)
     check_gated(h, y, values(w["gate"], torch.float16), values(w["up"], torch.float16), "silu", dim)
     check_product(dk.gemm(*w["down"], h), h, values(w["down"], torch.float16).t(), depth=hidden)
+
+
+def test_first_call_of_a_process_may_be_captured():
+    """Nothing that a first call sets up stands in a capture's way."""
+    code = """
+import torch, sys
+sys.path.insert(0, "decode-kernel_b200")
+import decode_kernel as dk
+from decode_kernel import _cuda
+packed, scales = torch.zeros(256, 64, dtype=torch.int32, device="cuda"), torch.ones(256, 4, dtype=torch.float16, device="cuda")
+packed += 0x11111111
+xs = [torch.ones(T, 512, dtype=torch.float16, device="cuda") for T in (1, 12, 40, 300)]
+q, pos, freq = torch.ones(5, 2, 64, device="cuda"), torch.zeros(5, dtype=torch.int32, device="cuda"), torch.ones(32, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    ys = [dk.gemm(packed, scales, x) for x in xs]
+    back = [dk.gemm_t(packed, scales, y) for y in ys]
+    hs = [dk.gemm_gated((packed, scales), (packed, scales), x) for x in xs]
+    turned = dk.rotary(q, None, pos, freq)[0]
+graph.replay()
+torch.cuda.synchronize()
+assert all((y == 512).all() for y in ys) and all((b == torch.inf).all() for b in back) and torch.equal(turned, q)
+assert all((h == torch.inf).all() for h in hs)
+"""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=240, cwd=Path(__file__).resolve().parent.parent)
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
+def test_no_wait_ran_out():
+    torch.cuda.synchronize()
+    assert capi.load().dk_device_error(-1, 0) == 0
