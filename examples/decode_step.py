@@ -2,10 +2,12 @@
 
     PYTHONPATH=decode-kernel_b200 python examples/decode_step.py [--steps 64] [--code int8|e4m3]
 
-Ragged prompts go in as one step, then every request decodes token by token
-with the whole step -- plan, norms, W4A16 products, append, attention --
-replayed as one CUDA graph: nothing in it waits for the host.  Between steps
-requests end and their pages go back to the free ring.
+Ragged prompts go in as one step (the products of many rows, the gated block in
+one launch), then every request decodes token by token with the whole step --
+plan, norms, W4A16 products, rotary positions, append, attention -- replayed as
+one CUDA graph: nothing in it waits for the host.  Half-way the requests move to
+a second server with other pages: their cache is read back and written into its.
+At the end requests end and their pages go back to the free ring.
 """
 
 from __future__ import annotations
@@ -40,23 +42,25 @@ class Decoder:
         self.frequency = 10000.0 ** (-torch.arange(0, head_dim, 2, device="cuda").float() / head_dim)
 
     def rotate(self, x, positions):
-        angle = positions[:, None, None].float() * self.frequency
-        a, b = x.float().chunk(2, -1)
-        return torch.cat([a * angle.cos() - b * angle.sin(), a * angle.sin() + b * angle.cos()], -1).half()
+        return dk.rotary(x, None, positions, self.frequency)[0]
 
     def step(self, tokens, positions, attend):
         """Logits of every row; attend(layer, q, k, v) keeps k and v and returns the attention's output."""
         n = tokens.shape[0]
         r = self.embedding[tokens]
         _, h = dk.block_norm(r, pre_weight=self.layers[0]["norm1"])
+        many = n > 8  # prompts and batches; a few rows go by the GEMV's launches of several matrices
+        product = dk.gemm if many else dk.gemv
         for i, w in enumerate(self.layers):
-            q, k, v = (x.view(n, -1, self.head_dim) for x in dk.gemv_multi([w["q"], w["k"], w["v"]], h))
-            a = attend(i, self.rotate(q, positions), self.rotate(k, positions), v)
-            r, h = dk.block_norm(r, dk.gemv(*w["o"], a.reshape(n, -1)), pre_weight=w["norm2"])
-            y = dk.gemv(*w["down"], dk.gemv_silu_mul(w["gate"], w["up"], h))
+            parts = [w["q"], w["k"], w["v"]]
+            q, k, v = (x.view(n, -1, self.head_dim) for x in ([dk.gemm(*p, h) for p in parts] if many else dk.gemv_multi(parts, h)))
+            dk.rotary(q, k, positions, self.frequency, inplace=True)
+            a = attend(i, q, k, v)
+            r, h = dk.block_norm(r, product(*w["o"], a.reshape(n, -1)), pre_weight=w["norm2"])
+            y = product(*w["down"], (dk.gemm_gated if many else dk.gemv_silu_mul)(w["gate"], w["up"], h))
             after = self.layers[i + 1]["norm1"] if i + 1 < len(self.layers) else self.norm
             r, h = dk.block_norm(r, y, pre_weight=after)
-        return dk.gemv(*self.head, h)
+        return product(*self.head, h)
 
 
 class Server:
@@ -96,6 +100,20 @@ class Server:
         logits = self.step(tokens, fresh, single=False)
         return logits[self.starts[1:].long() - 1]
 
+    def take_over(self, other):
+        """The other server's requests: their keys and values read back from its pages and written into this one's, of
+        whatever size and type those are.  This server holds none yet, and serves as many."""
+        lengths = other.held.clone()
+        starts = torch.cat([lengths.new_zeros(1), lengths.cumsum(0, dtype=torch.int32)])
+        tokens = int(starts[-1])  # waits for the GPU
+        slots = torch.empty(tokens, dtype=torch.int64, device="cuda")
+        plan = dk.cache_plan(self.held, lengths, self.table, self.free, self.ring, self.block_size, tokens,
+                             out=dk.CachePlan(self.held, self.starts, slots, self.ring))
+        for mine, theirs in zip(self.caches, other.caches):
+            k, v = dk.cache_read(theirs, other.table, lengths, starts, tokens)
+            dk.cache_append(k, v, plan.slots, mine)
+        self.tokens.copy_(other.tokens)
+
     def decode(self):
         """One token for every request, from self.tokens; the step is captured once and replayed."""
         if self.graph is None:
@@ -131,13 +149,17 @@ def main():
     prompts = [[(7 * r + 13 * t) % 4096 for t in range(5 + 37 * r)] for r in range(a.requests)]
     server.tokens.copy_(server.prefill(prompts).argmax(-1))
     server.decode()
+    moved = Server(model, a.requests, blocks=a.requests * 24, block_size=32, code=torch.float8_e4m3fn if code == torch.int8 else torch.int8, max_blocks=64)
+    moved.take_over(server)
+    server = moved
+    server.decode()
     torch.cuda.synchronize()
     began = time.perf_counter()
     for _ in range(a.steps):
         server.decode()
     torch.cuda.synchronize()
     took = (time.perf_counter() - began) / a.steps
-    print(f"{a.requests} requests, {sum(len(p) for p in prompts)} prompt tokens, then {a.steps + 1} steps: {took * 1e6:.0f} us a step "
+    print(f"{a.requests} requests, {sum(len(p) for p in prompts)} prompt tokens, then {a.steps + 2} steps: {took * 1e6:.0f} us a step "
           f"of {len(model.layers)} layers; lengths {server.held.tolist()}, pages missing {int(server.ring[2])}")
     server.fresh.fill_(-1)  # every request ends
     dk.cache_plan(server.held, server.fresh, server.table, server.free, server.ring, server.block_size, 0,
