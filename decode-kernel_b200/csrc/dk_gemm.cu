@@ -1,24 +1,37 @@
 // dk_gemm.cu -- many rows through 4-bit weights: y = x . dequant(W)^T, a gated
-// block's act(x Wg^T) * (x Wu^T), and the transposed product dx = g . dequant(W).
+// block's act(x Wg^T) * (x Wu^T), and the transposed product dx = g . dequant(W),
+// the gradient of the others.  (Few rows: dk_few.cuh.)
 //
 // All three are one tile product on the 5th-generation tensor cores,
 //   D[lane][token] = sum_d A[lane][d] . B[token][d],
 // with the weights as A and the rows as B: a tile has 128 lanes a CTA (outputs
-// of W; 64 of Wg beside 64 of Wu; or columns k of W) and up to 256 tokens.  The
-// packed weights come into shared memory by TMA; warps unpack them, fold the
-// group's scale in (one rounding to the rows' type) and store them straight into
-// tensor memory, where the MMA reads A: no second trip of the weights through
-// shared memory, whose bandwidth B needs.  B tiles come by TMA in the 128-byte
-// swizzle, the fp32 sums stay in tensor memory until the tile is done.
-//   warps 0..7    unpack: 128 deep a step, four warps for each 64 of them
-//   warps 8..11   the sums: tensor memory -> activation -> y
-//   warp 12       copies of B, warp 13 the MMAs (one thread), warp 14 copies of W
-// For many rows two CTAs of a cluster work as a pair (cta_group::2) on 256 lanes:
-// each unpacks its own 128 lanes and loads half of the tokens, which halves B's
-// traffic and footprint; pairs go on from tile to tile while the sums of the
-// last one are read.  For few rows the depth is split over a cluster's CTAs,
-// whose sums are added in order through distributed shared memory: no workspace
-// and no atomics, the same bits in every run.
+// of W; 64 of Wg beside 64 of Wu, sixteen of each in turn, so that a warp holds
+// both halves of its outputs; or columns k of W) and up to 256 tokens.  The
+// packed weights come into shared memory by TMA; warps unpack them and fold the
+// group's scale in (one rounding to the rows' type: 2^-12 of a weight on average in
+// fp16, 2^-9 in bf16, which moves a product as much as rounding the result does and
+// a gated result or its gradient up to twice as much; scaling each group's fp32 sums
+// instead, as few rows do, would read the sums 32 times a tile of 4096), and store
+// them as A.  B tiles come by TMA in the 128-byte swizzle, the fp32 sums stay in
+// tensor memory until the tile is done.
+//   warps 0..15   unpack, a step (128 of the depth, one group) by eight of them in turn
+//   warps 16..19  the sums: tensor memory -> activation -> boxes in shared memory -> y by TMA
+//   warp 20       copies of B, warp 21 the MMAs, warp 22 copies of W
+// Mostly two CTAs of a cluster work as a pair (cta_group::2) on 256 lanes: each
+// unpacks its own 128 lanes and loads half of the tokens, which halves B's traffic
+// and footprint; pairs go on from tile to tile while the sums of the last one are
+// read.  Where there are few tiles, CTAs work alone with the depth split over a
+// cluster, whose sums are added in order through distributed shared memory: no
+// workspace and no atomics, the same bits in every run.
+//   What bounds it: the tensor cores, 84 (plain) to 88 % (gated) busy over whole
+// kernels of 2048 rows, 69 % in the transposed product, and the power they draw: the
+// SM clock falls to 1.2..1.5 GHz in them, so that 4096 rows of a 7B-shaped gated
+// block take 500..580 us (1.27..1.47 PFLOP/s) by the box and its temperature, at
+// 1.09 thousand cycles a step of 256 x 256 x 128 or less (1024 at best).
+//   What that took, each step measured: no fences of cluster scope in the barriers
+// (an arrival with one took 1.4 thousand cycles), sixteen unpacking warps instead
+// of eight, A through tensor memory where possible, whole warps with uniform
+// operands around single-thread instructions (34 cycles an MMA instead of 80).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
