@@ -18,7 +18,8 @@
 // The pieces are made once a call by k_split, in the order of k in which the
 // nibbles come out.  k_few streams the packed words: TMA to shared memory, words
 // to codes in tensor memory (A), pieces by TMA (B), one group a step, its sums in
-// a ring of places in tensor memory, from where four warps take them to fp32.
+// a ring of places in tensor memory, from where two teams of four warps, a step
+// each in turn, take them to fp32.
 // The tiles of a cluster are one line of steps that its CTAs share evenly; the
 // sums of tiles that several of them work on are added in order over distributed
 // shared memory.
