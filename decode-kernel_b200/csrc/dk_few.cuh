@@ -331,24 +331,28 @@ __global__ void __launch_bounds__(Form<BF16, TT>::kThreads, 1) k_few(const __gri
     // registers: a step of one diverged thread took 600 cycles and held up the
     // rest.)
     pdl_wait();  // for the pieces
+    constexpr int kBatch = F::kRing / 2;  // copies after one wait
     int issued = 0;
-    for (; issued < todo; ++issued) {
-      const int before = issued - F::kRing, slot = issued % F::kRing;
-      if (before >= 0) warp_wait<true>(&done[before % 16], before / 16 & 1, give_up, a.error);
+    while (issued < todo) {
+      const int end = min(todo, issued + kBatch), before = end - 1 - F::kRing;
+      if (before >= 0) warp_wait(&done[before % 16], before / 16 & 1, give_up, a.error);
       if (__any_sync(0xffffffffu, *give_up)) break;
-      if (elect_one()) {
-        const uint32_t bar = smem_u32(&full[slot]);
-        mbar_arrive_expect_tx(&full[slot], F::kN * 128 + TT * 8);
-        tma_2d(base + F::kB + slot * F::kN * 128, &a.b, 0, group * F::kN, bar);
-        // The factors are read after the step's MMAs are done, so their ring is
-        // longer by what the sums may be behind.
-        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                         base + F::kFactorAt + (issued % F::kFactors) * TT * 8),
-                     "l"(a.factors + (long long)group * TT), "r"(TT * 8), "r"(bar)
-                     : "memory");
+      for (; issued < end; ++issued) {
+        const int slot = issued % F::kRing;
+        if (elect_one()) {
+          const uint32_t bar = smem_u32(&full[slot]);
+          mbar_arrive_expect_tx(&full[slot], F::kN * 128 + TT * 8);
+          tma_2d(base + F::kB + slot * F::kN * 128, &a.b, 0, group * F::kN, bar);
+          // The factors are read after the step's MMAs are done, so their ring is
+          // longer by what the sums may be behind.
+          asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                           base + F::kFactorAt + (issued % F::kFactors) * TT * 8),
+                       "l"(a.factors + (long long)group * TT), "r"(TT * 8), "r"(bar)
+                       : "memory");
+        }
+        __syncwarp();
+        next();
       }
-      __syncwarp();
-      next();
     }
     if (issued < todo && lane == 0) {  // what was asked for lands before the CTA ends
       volatile int none = 0;
@@ -359,23 +363,30 @@ __global__ void __launch_bounds__(Form<BF16, TT>::kThreads, 1) k_few(const __gri
     // ---------------- copies of the packed weights ----------------
     // The weights are older than the kernel before, which waited for what wrote
     // them: no wait here.
+    constexpr int kBatch = 4;  // copies after the waits for the last two: teams of warps give back every other step in order
     int issued = 0;
-    for (; issued < todo; ++issued) {
-      const int slot = issued % F::kRaw, round = issued / F::kRaw;
-      if (round) warp_wait<true>(&raw_free[slot], (round - 1) & 1, give_up, a.error);
-      if (__any_sync(0xffffffffu, *give_up)) break;
-      if (elect_one()) {
-        const uint32_t dst = base + F::kRawAt + slot * kRawBytes, bar = smem_u32(&raw_full[slot]);
-        mbar_arrive_expect_tx(&raw_full[slot], kRawBytes);
-        if constexpr (MODE == kPlain) {
-          tma_2d(dst, &a.w[0], group * 64, tile * 128, bar);
-        } else {
-          tma_2d(dst, &a.w[0], group * 64, tile * 64, bar);
-          tma_2d(dst + kRawBytes / 2, &a.w[1], group * 64, tile * 64, bar);
-        }
+    while (issued < todo) {
+      const int end = min(todo, issued + kBatch), round = issued / F::kRaw;  // of the whole batch: kRaw is a multiple of it
+      if (round) {
+        warp_wait(&raw_free[(end - 1) % F::kRaw], (round - 1) & 1, give_up, a.error);
+        if (end - issued > 1) warp_wait(&raw_free[(end - 2) % F::kRaw], (round - 1) & 1, give_up, a.error);
       }
-      __syncwarp();
-      next();
+      if (__any_sync(0xffffffffu, *give_up)) break;
+      for (; issued < end; ++issued) {
+        const int slot = issued % F::kRaw;
+        if (elect_one()) {
+          const uint32_t dst = base + F::kRawAt + slot * kRawBytes, bar = smem_u32(&raw_full[slot]);
+          mbar_arrive_expect_tx(&raw_full[slot], kRawBytes);
+          if constexpr (MODE == kPlain) {
+            tma_2d(dst, &a.w[0], group * 64, tile * 128, bar);
+          } else {
+            tma_2d(dst, &a.w[0], group * 64, tile * 64, bar);
+            tma_2d(dst + kRawBytes / 2, &a.w[1], group * 64, tile * 64, bar);
+          }
+        }
+        __syncwarp();
+        next();
+      }
     }
     if (issued < todo && lane == 0) {
       volatile int none = 0;
