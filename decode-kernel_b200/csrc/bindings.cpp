@@ -803,7 +803,12 @@ std::tuple<torch::Tensor, OptTensor> rotary(torch::Tensor q, OptTensor k, torch:
   }
   const c10::cuda::CUDAGuard guard(device);
   const torch::Tensor at = positions.stride(-1) == 1 || tokens <= 1 ? positions : positions.contiguous();
-  auto place = [&](const torch::Tensor& t, const void*& in, void*& out, int64_t& it, int64_t& ih, int64_t& ot, int64_t& oh) {
+  // Two small outputs come from one allocation.
+  torch::Tensor whole;
+  const int64_t size = static_cast<int64_t>(q.element_size()), q_bytes = (q.numel() * size + 15) / 16 * 16;
+  if (k && !inplace && q_bytes + k->numel() * size <= (1 << 22))
+    whole = torch::empty({q_bytes + k->numel() * size}, q.options().dtype(torch::kUInt8));
+  auto place = [&](const torch::Tensor& t, int64_t byte, const void*& in, void*& out, int64_t& it, int64_t& ih, int64_t& ot, int64_t& oh) {
     if (inplace) {
       TORCH_CHECK(t.stride(2) == 1, "q and k that are turned in place must have contiguous heads");
       for (int64_t i = 0; i < 2; ++i)
@@ -812,16 +817,16 @@ std::tuple<torch::Tensor, OptTensor> rotary(torch::Tensor q, OptTensor k, torch:
                   "q and k that are turned in place may not overlap themselves");
     }
     const torch::Tensor from = t.stride(2) == 1 ? t : t.contiguous();
-    const torch::Tensor to = inplace ? t : torch::empty(t.sizes(), t.options());
+    const torch::Tensor to = inplace ? t : whole.defined() ? part_of(whole, t.scalar_type(), byte, t.sizes()) : torch::empty(t.sizes(), t.options());
     in = from.data_ptr();
     out = to.data_ptr();
     it = from.stride(0), ih = from.stride(1), ot = to.stride(0), oh = to.stride(1);
     return std::make_pair(from, to);
   };
-  const auto qs = place(q, a.q, a.q_out, a.q_token_stride, a.q_head_stride, a.q_out_token_stride, a.q_out_head_stride);
+  const auto qs = place(q, 0, a.q, a.q_out, a.q_token_stride, a.q_head_stride, a.q_out_token_stride, a.q_out_head_stride);
   std::pair<torch::Tensor, torch::Tensor> ks;
   if (k) {
-    ks = place(*k, a.k, a.k_out, a.k_token_stride, a.k_head_stride, a.k_out_token_stride, a.k_out_head_stride);
+    ks = place(*k, q_bytes, a.k, a.k_out, a.k_token_stride, a.k_head_stride, a.k_out_token_stride, a.k_out_head_stride);
     const at::MemOverlapStatus both = at::get_overlap_status(q, *k);
     TORCH_CHECK(!inplace || tokens == 0 ||
                     (k->data_ptr() != q.data_ptr() && both != at::MemOverlapStatus::Full && both != at::MemOverlapStatus::Partial),
@@ -858,7 +863,12 @@ std::tuple<torch::Tensor, torch::Tensor> cache_read(const Cache8& cache, torch::
   TORCH_CHECK(type == torch::kFloat16 || type == torch::kBFloat16, "dtype must be fp16 or bf16");
   const c10::cuda::CUDAGuard guard(device);
   const std::vector<int64_t> shape = {tokens, cache.c.kv_heads, cache.c.head_dim};
+  // Two small outputs come from one allocation.
+  torch::Tensor whole;
+  const int64_t bytes = tokens * cache.c.kv_heads * cache.c.head_dim * 2;  // a multiple of 16
+  if (!k && !v && bytes <= (1 << 21)) whole = torch::empty({2 * bytes}, cache.k.options().dtype(torch::kUInt8));
   auto given = [&](const OptTensor& t, const char* what) {
+    if (!t && whole.defined()) return part_of(whole, type, *what == 'v' ? bytes : 0, shape);
     if (!t) return torch::empty(shape, cache.k.options().dtype(type));
     TORCH_CHECK(t->is_cuda() && t->device() == device && t->scalar_type() == type && t->sizes() == c10::IntArrayRef(shape),
                 what, " must be [tokens, kv_heads, head_dim] of dtype on the cache's device");

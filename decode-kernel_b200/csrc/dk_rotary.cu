@@ -8,7 +8,7 @@
 // has 29 bits before the point, and the fraction of a turn is what counts), so
 // far positions lose nothing; the sines and cosines of the fraction are fp32.
 //   Bound by HBM in fp32 (8192 tokens of 40 heads of 128: 54 us, 6.2 TB/s) and
-// nearly so in bf16 (30 us, 5.6 TB/s); one token by the call (8 us).  One piece a
+// nearly so in bf16 (30 us, 5.6 TB/s); one token by the call (7.5 us).  One piece a
 // thread at a time with 40 registers: four pieces' loads at once cost the occupancy
 // that hides them (56 us instead of 33).
 #include <cuda_bf16.h>
