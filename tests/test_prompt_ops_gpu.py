@@ -710,3 +710,70 @@ assert all((h == torch.inf).all() for h in hs)
 def test_no_wait_ran_out():
     torch.cuda.synchronize()
     assert capi.load().dk_device_error(-1, 0) == 0
+
+
+@pytest.mark.parametrize("T", [1, 12, 24, 60, 300])
+def test_weights_that_change_between_calls(T):
+    """New weights written into the same tensors just before a call: no form reads what stood there before."""
+    M, K = 700, 1024
+    sets = [(weights(M, K, 300 + i), weights(M, K, 310 + i)) for i in range(2)]
+    x, g = rows_of(T, K, torch.float16, 320), rows_of(T, M, torch.float16, 321)
+    call = lambda a, b: (dk.gemm(*a, x), dk.gemm_gated(a, b, x), dk.gemm_t(*a, g))  # noqa: E731
+    want = [call(a, b) for a, b in sets]
+    held = [tuple(t.clone() for t in w) for w in sets[0]]
+    for i in range(60):
+        for mine, given in zip(held, sets[i % 2]):
+            for t, n in zip(mine, given):
+                t.copy_(n)
+        assert all(torch.equal(p, q) for p, q in zip(call(*held), want[i % 2])), i
+
+
+def test_few_rows_on_several_streams_at_once():
+    M, K = 1500, 1024
+    w, w2 = weights(M, K, 330), weights(M, K, 331)
+    xs = [rows_of(T, K, dtype, 332 + T) for T, dtype in ((3, torch.bfloat16), (9, torch.float16), (16, torch.float16), (24, torch.bfloat16), (32, torch.float16))]
+    call = lambda x: (dk.gemm(*w, x), dk.gemm_gated(w, w2, x), dk.gemm_t(*w, dk.gemm(*w, x)))  # noqa: E731
+    want = [call(x) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = [[] for _ in xs]
+    for _ in range(10):
+        for s, x, out in zip(streams, xs, got):
+            with torch.cuda.stream(s):
+                out.append(call(x))
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(p, q) for out in b for p, q in zip(a, out))
+    held = [x.clone() for x in xs]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = [call(x) for x in held]
+    for scale in (1.0, -0.5):
+        for x, h in zip(xs, held):
+            h.copy_(x * scale)
+        graph.replay()
+        for h, b in zip(held, out):
+            assert all(torch.equal(p, q) for p, q in zip(call(h), b))
+
+
+def test_keys_and_values_read_on_another_stream_and_in_a_graph():
+    cache = dk.PagedCache8(20, 16, 2, 64)
+    for pool, scale in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
+        pool.copy_(torch.randint(-127, 128, pool.shape, generator=gen(1), device="cuda"))
+        scale.uniform_(0.01, 0.02)
+    ints = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    table, lengths, starts = ints([[3, 5, 7], [11, 13, 2]]), ints([40, 20]), ints([0, 40, 60])
+    want = dk.cache_read(cache, table, lengths, starts, 60)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = dk.cache_read(cache, table, lengths, starts, 60)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = dk.cache_read(cache, table, lengths, starts, 60)
+    lengths.copy_(ints([33, 44]))  # rows that a request does not hold become zeros
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(dk.cache_read(cache, table, lengths, starts, 60), got))
+    assert (got[0][:7] == 0).all() and torch.equal(got[0][7:40], want[0][:33])
