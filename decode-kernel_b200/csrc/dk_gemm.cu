@@ -1230,6 +1230,9 @@ extern "C" dk_status dk_w4a16_gemm(const dk_gemm_args* p, void* stream) {
       (p->gate_out && !p->packed2))
     return DK_ERR_INVALID_ARG;
   if (!aligned16(p->packed) || !aligned16(p->packed2) || !aligned16(p->x)) return DK_ERR_INVALID_ARG;
+  for (const void* at : {static_cast<const void*>(p->scales), static_cast<const void*>(p->scales2), static_cast<const void*>(p->y),
+                         static_cast<const void*>(p->gate_out), static_cast<const void*>(p->up_out)})
+    if (!aligned_to(at, 2)) return DK_ERR_INVALID_ARG;
   if (p->rows > 1 && (p->ldx < p->K || p->ldx % 8 || p->ldy < p->M || (p->gate_out && p->ldk < p->M)))
     return DK_ERR_INVALID_ARG;
   const size_t need = dk_w4a16_gemm_workspace_bytes(p->rows, p->K, p->packed2 ? 2 : 1, p->dtype);
@@ -1265,6 +1268,7 @@ extern "C" dk_status dk_w4a16_gemm_t(const dk_gemm_t_args* p, void* stream) {
   if ((p->packed2 == nullptr) != (p->scales2 == nullptr) || (p->packed2 == nullptr) != (p->g2 == nullptr))
     return DK_ERR_INVALID_ARG;
   if (!aligned16(p->packed) || !aligned16(p->packed2) || !aligned16(p->g) || !aligned16(p->g2)) return DK_ERR_INVALID_ARG;
+  if (!aligned_to(p->scales, 2) || !aligned_to(p->scales2, 2) || !aligned_to(p->dx, 2)) return DK_ERR_INVALID_ARG;
   if (p->rows > 1 && (p->ldg < p->M || p->ldg % 8 || p->lddx < p->K)) return DK_ERR_INVALID_ARG;
   Product a{};
   a.packed[0] = p->packed;
@@ -1293,7 +1297,10 @@ extern "C" dk_status dk_gated_grad(const void* dh, const void* g, const void* u,
   if (rows > 1 && (lddh < M || ldk < M || ldd < M)) return DK_ERR_INVALID_ARG;
   GradArgs a{dh, g, u, dg, du, lddh, ldk, ldd, 0, M, 0, (int)act};
   bool wide = M % 8 == 0 && (rows == 1 || (lddh % 8 == 0 && ldk % 8 == 0 && ldd % 8 == 0));
-  for (const void* p : {dh, g, u, static_cast<const void*>(dg), static_cast<const void*>(du)}) wide = wide && aligned16(p);
+  for (const void* p : {dh, g, u, static_cast<const void*>(dg), static_cast<const void*>(du)}) {
+    if (!aligned_to(p, 2)) return DK_ERR_INVALID_ARG;
+    wide = wide && aligned16(p);
+  }
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   return dtype == DK_FP16 ? launch_grad<__half>(a, rows, wide, st) : launch_grad<__nv_bfloat16>(a, rows, wide, st);
 }

@@ -64,6 +64,9 @@ dk_status launch_early(const char* name, void (*kernel)(Args), dim3 grid, dim3 b
   return DK_OK;
 }
 
+inline bool aligned_to(const void* p, uintptr_t bytes) {
+  return reinterpret_cast<uintptr_t>(p) % bytes == 0;
+}
 inline bool aligned16(const void* p) {
   return (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
 }

@@ -158,8 +158,10 @@ extern "C" dk_status dk_cache_read(const dk_cache_read_args* p, void* stream) {
                              c.v_block_stride, c.v_head_stride, c.v_token_stride};
   for (int64_t s : strides)
     if (s < 0 || s % 32) return DK_ERR_INVALID_ARG;
-  auto aligned = [](const void* x, uintptr_t n) { return reinterpret_cast<uintptr_t>(x) % n == 0; };
-  if (!aligned(c.k, 32) || !aligned(c.v, 32) || !aligned(p->k, 16) || !aligned(p->v, 16) ||
+  for (const void* at : {static_cast<const void*>(c.k_scale), static_cast<const void*>(c.v_scale), static_cast<const void*>(p->block_table),
+                         static_cast<const void*>(p->lengths), static_cast<const void*>(p->starts)})
+    if (!aligned_to(at, 4)) return DK_ERR_INVALID_ARG;
+  if (!aligned_to(c.k, 32) || !aligned_to(c.v, 32) || !aligned16(p->k) || !aligned16(p->v) ||
       p->k_token_stride % 8 || p->v_token_stride % 8)
     return DK_ERR_INVALID_ARG;
   ReadArgs a;

@@ -201,6 +201,7 @@ extern "C" dk_status dk_rotary(const dk_rotary_args* p, void* stream) {
   if (p->tokens == 0) return DK_OK;
   const int kv_heads = p->k ? p->kv_heads : 0;
   if (!p->q || !p->q_out || !p->positions || !p->frequency || (kv_heads && !p->k_out)) return DK_ERR_INVALID_ARG;
+  if (!aligned_to(p->positions, p->positions_64 ? 8 : 4) || !aligned_to(p->frequency, 4)) return DK_ERR_INVALID_ARG;
   const int size = p->dtype == DK_FP32 ? 4 : 2;
   RotaryArgs a;
   a.in[0] = p->q;

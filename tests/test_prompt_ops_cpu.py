@@ -162,3 +162,19 @@ def test_bad_arguments_raise_before_the_device():
         dk.W4A16GatedMLP(lin(128, 256), lin(256, 256), lin(256, 128))
     with pytest.raises(ValueError):
         dk.W4A16GatedMLP(lin(128, 256), lin(128, 256), lin(256, 128), act="relu")
+
+
+@pytest.mark.parametrize("call", [
+    *(lambda kw=kw: capi.load().dk_w4a16_gemm(ctypes.byref(gemm_args(rows=40, **kw)), None) for kw in (
+        dict(scales=65), dict(y=1025), dict(packed2=1024, scales2=65), dict(packed2=1024, scales2=64, gate_out=65, up_out=64),
+        dict(packed2=1024, scales2=64, gate_out=64, up_out=65))),
+    *(lambda kw=kw: capi.load().dk_w4a16_gemm_t(ctypes.byref(gemm_t_args(**kw)), None) for kw in (
+        dict(scales=65), dict(dx=1025), dict(packed2=1024, scales2=65, g2=1024))),
+    *(lambda kw=kw: gated_grad(**kw) for kw in (dict(dh=65), dict(g=65), dict(u=65), dict(dg=65), dict(du=65))),
+    *(lambda kw=kw: capi.load().dk_rotary(ctypes.byref(rotary_args(**kw)), None) for kw in (
+        dict(positions=66), dict(positions=68, positions_64=1), dict(frequency=66))),
+    *(lambda kw=kw: capi.load().dk_cache_read(ctypes.byref(read_args(**kw)), None) for kw in (
+        dict(block_table=66), dict(lengths=66), dict(starts=66), dict(cache=cache(k_scale=66)), dict(cache=cache(v_scale=66)))),
+])
+def test_addresses_between_values_are_refused(call):
+    assert call() == capi.DK_ERR_INVALID_ARG
