@@ -642,6 +642,12 @@ dk_mlp_act mlp_act(int act) {
   return static_cast<dk_mlp_act>(act);
 }
 
+// A kernel wrote over a tensor of the caller's: a graph that saved what stood there
+// learns of it.
+void written(const torch::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // An output given by the caller: contiguous rows of any stride, or a new one.
 torch::Tensor output(const OptTensor& out, const std::vector<int64_t>& shape, const torch::Tensor& x) {
   if (!out) return torch::empty(shape, x.options());
@@ -698,6 +704,7 @@ std::tuple<torch::Tensor, OptTensor, OptTensor> w4a16_gemm(torch::Tensor packed,
     a.workspace_bytes = need;
   }
   check_status(dk_w4a16_gemm(&a, at::cuda::getCurrentCUDAStream().stream()), "w4a16_gemm");
+  if (out) written(y);
   return {y, g, u};
 }
 
@@ -736,6 +743,7 @@ torch::Tensor w4a16_gemm_t(torch::Tensor packed, torch::Tensor scales, OptTensor
   a.M = static_cast<int>(w.M);
   a.K = static_cast<int>(w.K);
   check_status(dk_w4a16_gemm_t(&a, at::cuda::getCurrentCUDAStream().stream()), "w4a16_gemm_t");
+  if (out) written(dx);
   return dx;
 }
 
@@ -846,6 +854,10 @@ std::tuple<torch::Tensor, OptTensor> rotary(torch::Tensor q, OptTensor k, torch:
   a.inverse = inverse;
   a.dtype = q.scalar_type() == torch::kFloat32 ? DK_FP32 : half_type(q, "q");
   check_status(dk_rotary(&a, at::cuda::getCurrentCUDAStream().stream()), "rotary");
+  if (inplace) {
+    written(q);
+    if (k) written(*k);
+  }
   return {qs.second, k ? OptTensor(ks.second) : OptTensor()};
 }
 
@@ -894,6 +906,8 @@ std::tuple<torch::Tensor, torch::Tensor> cache_read(const Cache8& cache, torch::
   a.v_token_stride = tokens > 1 ? vo.stride(0) : 0;
   a.dtype = type == torch::kFloat16 ? DK_FP16 : DK_BF16;
   check_status(dk_cache_read(&a, at::cuda::getCurrentCUDAStream().stream()), "cache_read");
+  if (k) written(*k);
+  if (v) written(*v);
   return {ko, vo};
 }
 

@@ -777,3 +777,42 @@ def test_keys_and_values_read_on_another_stream_and_in_a_graph():
     graph.replay()
     assert all(torch.equal(a, b) for a, b in zip(dk.cache_read(cache, table, lengths, starts, 60), got))
     assert (got[0][:7] == 0).all() and torch.equal(got[0][7:40], want[0][:33])
+
+
+@pytest.mark.parametrize("which", ["gemm", "few", "gated", "gemm_t", "rotary q", "rotary k", "cache_read"])
+def test_a_graph_learns_that_what_it_saved_was_written_over(which):
+    M, K = 256, 256
+    w, T = weights(M, K, 340), 4 if which == "few" else 40
+    x = rows_of(T, K, torch.float16, 341)
+    out = torch.zeros(T, M, dtype=torch.float16, device="cuda")
+    q, k = (torch.randn(6, h, 64, device="cuda") for h in (4, 2))
+    frequency = torch.rand(32, device="cuda")
+    cache = dk.PagedCache8(4, 16, 2, 64)
+    kv = tuple(torch.zeros(6, 2, 64, dtype=torch.float16, device="cuda") for _ in range(2))
+    ints = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    saved = {"rotary q": q, "rotary k": k, "cache_read": kv[1]}.get(which, out)
+    factor = torch.ones_like(saved, requires_grad=True)
+    loss = (factor * saved).sum()
+    if which in ("gemm", "few"):
+        dk.gemm(*w, x, out=out)
+    elif which == "gated":
+        dk.gemm_gated(w, w, x, out=out)
+    elif which == "gemm_t":
+        dk.gemm_t(*w, x, out=out)
+    elif which == "cache_read":
+        dk.cache_read(cache, ints([[0]]), ints([6]), ints([0, 6]), 6, out=kv)
+    else:
+        dk.rotary(q, k, torch.arange(6, device="cuda"), frequency, inplace=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_outputs_are_written_under_inference_mode():
+    w = weights(256, 256, 342)
+    with torch.inference_mode():
+        x = rows_of(40, 256, torch.float16, 343)
+        out = torch.zeros(40, 256, dtype=torch.float16, device="cuda")
+        dk.gemm(*w, x, out=out)
+        assert torch.equal(out, dk.gemm(*w, x))
+    dk.gemm(*w, x, out=out)  # inference tensors outside of it
+    assert torch.equal(out, dk.gemm(*w, x))
