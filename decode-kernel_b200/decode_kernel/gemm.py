@@ -41,9 +41,12 @@ def gemm(packed: torch.Tensor, scales: torch.Tensor, x: torch.Tensor, *,
          out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x . dequant(W)^T for any number of rows: fp16 or bf16 [..., K] -> [..., M].
 
-    packed: int32 [M, K/8]; scales: fp16 [M, K/128].  A weight q * scale is
-    rounded once to x's type (past its range to infinity); products and sums are
-    fp32, and so is the result until it is rounded once.  x may be any view;
+    packed: int32 [M, K/8]; scales: fp16 [M, K/128].  Past 16 rows (32 of a
+    gated pair) a weight q * scale is rounded once to x's type (past its range to
+    infinity), for fewer it is not; products and sums are fp32, and so is the
+    result until it is rounded once.  A row with an infinity or a NaN gives
+    results that are not finite; which of the two is the formula's answer for a
+    single infinity in a group of 128.  x may be any view;
     rows that do not begin on 16-byte boundaries are copied first.  ``out`` is
     contiguous or has contiguous rows.  Differentiable in x.
     """
@@ -54,7 +57,8 @@ def gemm_t(packed: torch.Tensor, scales: torch.Tensor, g: torch.Tensor, *,
            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """g . dequant(W): fp16 or bf16 [..., M] -> [..., K], the gradient of ``gemm``'s x.
 
-    The same types and roundings as ``gemm``.  Differentiable in g.
+    The types of ``gemm``; weights are rounded as for its many rows.  Differentiable
+    in g.
     """
     return _extension().linear(True, packed, scales, g, out)
 

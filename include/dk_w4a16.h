@@ -529,8 +529,10 @@ DK_API dk_status dk_block_norm(const dk_block_norm_args* args, void* stream);
  * type (past its range to infinity) and products and sums are fp32.  Outputs are
  * rounded once.  The first form needs a workspace of dk_w4a16_gemm_workspace_bytes
  * (matrices: 1, or 2 for a pair; 0 bytes for more rows), 128-byte aligned, which
- * may hold anything; calls that share one must be ordered on the GPU.
- *  * Rows are ldx (x), ldy (y) and ldk (gate_out and
+ * may hold anything; calls that share one must be ordered on the GPU.  There, of
+ * several infinities in a row's group only their sum with the weights counts: inf
+ * or NaN, where the formula may say the other.
+ *   Rows are ldx (x), ldy (y) and ldk (gate_out and
  * up_out) values apart; x and packed are 16-byte aligned and ldx is a multiple
  * of 8 (where rows > 1).  Outputs may not overlap the inputs. */
 typedef enum dk_mlp_act { DK_MLP_SILU = 0, DK_MLP_GELU = 1 } dk_mlp_act;
@@ -555,7 +557,7 @@ DK_API dk_status dk_w4a16_gemm(const dk_gemm_args* args, void* stream);
 
 /* The transposed product, which is the gradient of x in the one above:
  *   dx[rows, K] = g[rows, M] . dequant(W)[M, K] (+ g2[rows, M] . dequant(W2)[M, K])
- * with the same types and roundings.  g and g2 are 16-byte aligned, their rows
+ * with the same types, and the roundings of many rows.  g and g2 are 16-byte aligned, their rows
  * ldg values apart (a multiple of 8, where rows > 1). */
 typedef struct dk_gemm_t_args {
   const int32_t* packed;
