@@ -652,17 +652,23 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
       const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + place * At::kSums;
       const int tile = item / a.token_tiles * CG + (CG == 2 ? (int)rank : 0);
       const int t0 = item % a.token_tiles * a.tokens, out = output_of<MODE, kATmem>(tile, tile_lane);
-      for (int c = 0; c < a.tokens; c += kBoxTokens) {
+      // Only sums of the call's rows and outputs are read.  Every turn of a box
+      // then has its store, which is what the wait for the store before last
+      // counts on.
+      const int sums = tile * kOuts < (MODE == kTransposed ? a.K : a.M) ? min(a.tokens, a.rows - t0) : 0;
+      auto give_back = [&] {  // the last of the tile's sums are in registers
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (CG == 1) mbar_arrive(sums_free);
+          else arrive_cluster(free_leader + place * 8);
+        }
+      };
+      if (sums == 0) give_back();
+      for (int c = 0; c < sums; c += kBoxTokens) {
         float v[32];
         tmem_ld32(from + c, v);
-        if (c + kBoxTokens >= a.tokens) {  // the last of the tile's sums are in registers
-          tcgen05_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            if constexpr (CG == 1) mbar_arrive(sums_free);
-            else arrive_cluster(free_leader + place * 8);
-          }
-        }
+        if (c + kBoxTokens >= sums) give_back();
         if (CG == 1 && a.split > 1) {
           float* red = reinterpret_cast<float*>(smem);  // over the rings: every copy has been read
 #pragma unroll
@@ -703,7 +709,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
           }
           fence_async_shared();
           named_barrier(1, kSumWarps * 32);
-          if (issuer && tile * kOuts < (MODE == kTransposed ? a.K : a.M) && t0 + c < a.rows) {
+          if (issuer) {
             tma_store_2d(&a.out[0], tile * kOuts, t0 + c, box);
             if (MODE == kGated && a.keep[0]) {
               tma_store_2d(&a.out[1], tile * kOuts, t0 + c, box + kBoxTokens * kOuts * 2);
