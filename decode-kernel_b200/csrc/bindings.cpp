@@ -13,12 +13,13 @@
 // device_error, and the rest of a decode step: Cache8 (a paged 8-bit cache's
 // tensors, checked once), cache_plan, cache_append, cache_attention, block_norm.
 // Every C-ABI status other than DK_OK becomes a RuntimeError.
-#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
+#include <array>
 #include <cmath>
 #include <cstdint>
 #include <map>
@@ -648,14 +649,80 @@ void written(const torch::Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// Whether two tensors have a byte in common, for any strides.  With D the distance
+// of a value of a from a value of b they do where -size_a < D < size_b for some choice
+// of indices: D is a sum of index * stride, tried from the largest stride on with
+// only those indices from which the smaller ones can still reach.  Strides that nest,
+// as those of slices do, leave an index or two each; a search that would go on for
+// long counts as a byte in common.
+struct Strides {
+  std::vector<std::array<int64_t, 5>> of;  // stride, its lowest and highest index, what it and the smaller ones reach
+  int64_t low, high;                       // of D
+  int tries = 1 << 14;
+
+  // A tensor's values, contiguous ones taken as one; returns their bytes.
+  int64_t add(const torch::Tensor& t, bool minus) {
+    std::vector<std::pair<int64_t, int64_t>> dims;
+    for (int64_t i = 0; i < t.dim(); ++i)
+      if (t.size(i) > 1 && t.stride(i) != 0) dims.emplace_back(t.stride(i) * t.element_size(), t.size(i));
+    std::sort(dims.begin(), dims.end());
+    int64_t run = t.element_size();
+    for (const auto& [stride, size] : dims) {
+      if (stride == run) {
+        run *= size;
+        continue;
+      }
+      const auto at = std::find_if(of.begin(), of.end(), [s = stride](const auto& o) { return o[0] == s; });
+      auto& mine = at != of.end() ? *at : of.emplace_back(std::array<int64_t, 5>{stride, 0, 0, 0, 0});
+      mine[minus ? 1 : 2] += minus ? 1 - size : size - 1;
+    }
+    return run;
+  }
+  bool meet(size_t i, int64_t distance) {
+    if (i == of.size()) return distance > low && distance < high;
+    if (--tries < 0) return true;
+    const auto [stride, first, last, below, above] = of[i];
+    const int64_t rest_below = i + 1 < of.size() ? of[i + 1][3] : 0, rest_above = i + 1 < of.size() ? of[i + 1][4] : 0;
+    // low < distance + n * stride + rest < high
+    auto down = [](int64_t a, int64_t b) { return a >= 0 ? a / b : -((b - 1 - a) / b); };
+    const int64_t from = std::max(first, down(low - distance - rest_above, stride) + 1);
+    const int64_t to = std::min(last, -down(-(high - distance - rest_below), stride) - 1);
+    for (int64_t n = from; n <= to; ++n)
+      if (meet(i + 1, distance + n * stride)) return true;
+    return false;
+  }
+};
+
+bool shares_memory(const torch::Tensor& a, const torch::Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  Strides s;
+  s.high = s.add(b, true);
+  s.low = -s.add(a, false);
+  std::sort(s.of.begin(), s.of.end(), [](const auto& p, const auto& q) { return p[0] > q[0]; });
+  int64_t below = 0, above = 0;
+  for (size_t i = s.of.size(); i-- > 0;) {
+    s.of[i][3] = below += s.of[i][0] * s.of[i][1];
+    s.of[i][4] = above += s.of[i][0] * s.of[i][2];
+  }
+  return s.meet(0, static_cast<int64_t>(reinterpret_cast<intptr_t>(a.data_ptr()) - reinterpret_cast<intptr_t>(b.data_ptr())));
+}
+
+// What a kernel writes is nothing of what it reads.
+void check_apart(const torch::Tensor& out, const char* what, std::initializer_list<const torch::Tensor*> inputs) {
+  for (const torch::Tensor* in : inputs)
+    TORCH_CHECK(!in->defined() || !shares_memory(out, *in), what, " may not overlap the call's inputs");
+}
+
 // An output given by the caller: contiguous rows of any stride, or a new one.
-torch::Tensor output(const OptTensor& out, const std::vector<int64_t>& shape, const torch::Tensor& x) {
+torch::Tensor output(const OptTensor& out, const std::vector<int64_t>& shape, const torch::Tensor& x,
+                     std::initializer_list<const torch::Tensor*> others) {
   if (!out) return torch::empty(shape, x.options());
   TORCH_CHECK(out->device() == x.device() && out->scalar_type() == x.scalar_type() && out->sizes() == c10::IntArrayRef(shape),
               "out must have the product's shape and x's type and device");
   TORCH_CHECK(out->is_contiguous() || (out->dim() == 2 && out->stride(1) == 1 && out->stride(0) >= out->size(1)),
               "out must have contiguous rows");
-  at::assert_no_overlap(*out, x);
+  check_apart(*out, "out", {&x});
+  check_apart(*out, "out", others);
   return *out;
 }
 
@@ -677,7 +744,8 @@ std::tuple<torch::Tensor, OptTensor, OptTensor> w4a16_gemm(torch::Tensor packed,
   }
   const torch::Tensor xr = in_rows(x, w.K);
   const std::vector<int64_t> shape = shape_with(x, w.M);
-  torch::Tensor y = output(out, shape, x);
+  const torch::Tensor none;
+  torch::Tensor y = output(out, shape, x, {&packed, &scales, packed2 ? &*packed2 : &none, scales2 ? &*scales2 : &none});
   OptTensor g, u;
   if (keep) {  // kept for the gradient, whose product wants rows a multiple of 8 apart
     const int64_t wide = (w.M + 7) / 8 * 8;
@@ -715,7 +783,7 @@ torch::Tensor w4a16_gemm_t(torch::Tensor packed, torch::Tensor scales, OptTensor
   a.dtype = half_type(g, "g");
   check_rows(g, w.M, "g");
   const c10::cuda::CUDAGuard guard(g.device());
-  if (w.M == 0) return output(out, shape_with(g, w.K), g).zero_();
+  if (w.M == 0) return output(out, shape_with(g, w.K), g, {}).zero_();
   torch::Tensor gr = in_rows(g, w.M), gr2;
   std::optional<Weights> w2;
   if (packed2) {
@@ -732,7 +800,8 @@ torch::Tensor w4a16_gemm_t(torch::Tensor packed, torch::Tensor scales, OptTensor
     a.scales2 = w2->factors();
     a.g2 = gr2.data_ptr();
   }
-  torch::Tensor dx = output(out, shape_with(g, w.K), g);
+  const torch::Tensor none;
+  torch::Tensor dx = output(out, shape_with(g, w.K), g, {&packed, &scales, packed2 ? &*packed2 : &none, scales2 ? &*scales2 : &none, g2 ? &*g2 : &none});
   a.packed = w.words();
   a.scales = w.factors();
   a.g = gr.data_ptr();
@@ -835,12 +904,11 @@ std::tuple<torch::Tensor, OptTensor> rotary(torch::Tensor q, OptTensor k, torch:
   std::pair<torch::Tensor, torch::Tensor> ks;
   if (k) {
     ks = place(*k, q_bytes, a.k, a.k_out, a.k_token_stride, a.k_head_stride, a.k_out_token_stride, a.k_out_head_stride);
-    const at::MemOverlapStatus both = at::get_overlap_status(q, *k);
-    TORCH_CHECK(!inplace || tokens == 0 ||
-                    (k->data_ptr() != q.data_ptr() && both != at::MemOverlapStatus::Full && both != at::MemOverlapStatus::Partial),
-                "q and k that are turned in place must be two tensors");
+    TORCH_CHECK(!inplace || !shares_memory(q, *k), "q and k that are turned in place may not overlap each other");
+    if (inplace) check_apart(*k, "k", {&positions, &frequency});
     a.kv_heads = static_cast<int>(k->size(1));
   }
+  if (inplace) check_apart(q, "q", {&positions, &frequency});
   a.positions = at.data_ptr();
   a.positions_64 = at.scalar_type() == torch::kInt64;
   a.position_stride = at.dim() == 2 ? at.stride(0) : 0;
@@ -887,10 +955,11 @@ std::tuple<torch::Tensor, torch::Tensor> cache_read(const Cache8& cache, torch::
     TORCH_CHECK(t->stride(2) == 1 && (t->size(1) == 1 || t->stride(1) == t->size(2)) &&
                     (tokens <= 1 || (t->stride(0) % 8 == 0 && t->stride(0) >= t->size(1) * t->size(2))) && aligned16(*t),
                 what, " must have contiguous rows, a multiple of 8 values apart and 16-byte aligned");
+    check_apart(*t, what, {&cache.k, &cache.v, &cache.k_scale, &cache.v_scale, &block_table, &lengths, &starts});
     return *t;
   };
   const torch::Tensor ko = given(k, "k"), vo = given(v, "v");
-  TORCH_CHECK(tokens == 0 || ko.data_ptr() != vo.data_ptr(), "k and v must be two tensors");
+  TORCH_CHECK(!k || !v || !shares_memory(ko, vo), "k and v must be two tensors that do not overlap");
   dk_cache_read_args a{};
   a.cache = cache.c;
   a.block_table = block_table.data_ptr<int32_t>();
@@ -1043,6 +1112,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("act"));
   m.def("rotary", &turn, "Rotary positions of queries and keys", py::arg("q"), py::arg("k"), py::arg("positions"),
         py::arg("frequency"), py::arg("sections"), py::arg("paired"), py::arg("inverse"), py::arg("inplace"));
+  m.def("shares_memory", &shares_memory, "Whether two tensors have a byte in common", py::arg("a"), py::arg("b"));
   m.def("cache_read", &cache_read, "Keys and values of a paged 8-bit cache as rows", py::arg("cache"), py::arg("block_table"),
         py::arg("lengths"), py::arg("starts"), py::arg("tokens"), py::arg("dtype"), py::arg("k") = py::none(),
         py::arg("v") = py::none());

@@ -1,0 +1,57 @@
+"""Edges of the prompt operators that need no device: which tensors share memory."""
+
+from __future__ import annotations
+
+import random
+
+import pytest
+import torch
+
+from decode_kernel import _cuda
+
+
+def bytes_of(t):
+    """Every byte's address."""
+    at = torch.zeros((), dtype=torch.int64)
+    for size, stride in zip(t.shape, t.stride()):
+        at = at[..., None] + torch.arange(size) * stride * t.element_size()
+    at = at.reshape(-1, 1) + torch.arange(t.element_size()) + t.data_ptr()
+    return set(at.flatten().tolist())
+
+
+def any_tensor(rng, home):
+    t = home.view(rng.choice([torch.uint8, torch.float16, torch.float32]))
+    sizes, strides, room = [], [], t.numel() - 1
+    for _ in range(rng.randint(0, 4)):
+        sizes.append(rng.choice([0, 1, 2, 3, 5, 8, 13] if rng.random() < 0.2 else [1, 2, 3, 5, 8, 13]))
+        most = room // max(1, sizes[-1] - 1)
+        strides.append(rng.choice([0, 1, rng.randint(0, most), rng.randint(0, min(most, 20))]) if most else 0)
+        room -= (max(1, sizes[-1]) - 1) * strides[-1]
+        if room < 0:
+            return any_tensor(rng, home)
+    return t.as_strided(sizes, strides, rng.randint(0, room))
+
+
+def test_shared_memory_of_any_strides():
+    rng, home = random.Random(1), torch.zeros(600, dtype=torch.uint8)
+    seen = {True: 0, False: 0}
+    for _ in range(6000):
+        a, b = any_tensor(rng, home), any_tensor(rng, home)
+        want = bool(bytes_of(a) & bytes_of(b))
+        assert _cuda.shares_memory(a, b) == want, (a.dtype, a.shape, a.stride(), a.storage_offset(), b.dtype, b.shape, b.stride(), b.storage_offset())
+        seen[want] += 1
+    assert min(seen.values()) > 1000
+
+
+@pytest.mark.parametrize("heads", [5, 6, 48])
+def test_slices_of_a_projection(heads):
+    fused = torch.zeros(1 << 13, heads, 64, dtype=torch.float16)
+    share = _cuda.shares_memory
+    for i in range(heads):
+        assert not share(fused[:, :i], fused[:, i:]) and share(fused[:, :i + 1], fused[:, i:])
+    assert not share(fused[:, ::2], fused[:, 1::2]) and share(fused[:, ::2], fused[:, 4:5])
+    assert not share(fused[::2], fused[1::2]) and not share(fused[:100], fused[100:]) and share(fused[:101], fused[100:])
+    flat = fused.view(1 << 13, -1)
+    assert not share(flat[:, :100], flat[:, 100:]) and share(flat[:, :101], flat[:, 100:]) and share(flat[:, 5:6], flat.t()[5:7])
+    assert not share(fused[..., :32], fused[..., 32:]) and share(fused[..., :33], fused[..., 32:])
+    assert not share(fused, fused.clone()) and share(fused, fused.view(torch.int8)[..., 127:])

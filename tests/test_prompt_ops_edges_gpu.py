@@ -69,3 +69,47 @@ def test_rows_at_the_boxes_edges(mode, rows):
             check_product(got, x, values(v, x.dtype, T, 32).t(), depth=K)
         assert torch.equal(h, dk.gemm_gated(w, w2, x))
     assert (wide[T:] == 7).all()
+
+
+def test_outputs_over_inputs_are_refused_and_beside_them_are_not():
+    M, K, T = 192, 256, 40
+    w, w2 = weights(M, K, 1), weights(M, K, 2)
+    wide = rows_of(T, 1024, torch.float16, 3)
+    x, g = wide[:, :K], wide[:, :M]
+    fused = torch.randn(6, 9, 64, device="cuda")
+    positions, frequency = torch.arange(6, device="cuda"), torch.rand(32, device="cuda")
+    cache = dk.PagedCache8(4, 16, 2, 64)
+    ints = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    table, lengths, starts = ints([[0, 1]]), ints([20]), ints([0, 20])
+    rows = torch.zeros(41, 2, 64, dtype=torch.float16, device="cuda")
+    read = lambda k, v: dk.cache_read(cache, table, lengths, starts, 20, out=(k, v))  # noqa: E731
+    words = lambda t, n: t.view(torch.float16).view(-1)[:n]  # noqa: E731
+    bad = {
+        "gemm": lambda: dk.gemm(*w, x, out=wide[:, K - 64:K - 64 + M]), "gemm, few rows": lambda: dk.gemm(*w, x[:4], out=wide[:4, 8:8 + M]),
+        "gemm, rows": lambda: dk.gemm(*w, x[:20], out=wide[19:39, :M]), "gated": lambda: dk.gemm_gated(w, w2, x, out=wide[:, K - 1:K - 1 + M]),
+        "gemm_t": lambda: dk.gemm_t(*w, g, out=wide[:, M - 8:M - 8 + K]), "gemm_t, the second rows": lambda: _cuda.w4a16_gemm_t(*w, *w2, wide[:, 512:512 + M], g, wide[:, M - 8:M - 8 + K]),
+        "packed": lambda: dk.gemm(*w, x, out=words(w[0], T * M).view(T, M)), "scales": lambda: dk.gemm(*w, x[:2], out=words(w[1], 2 * M).view(2, M)),
+        "up": lambda: dk.gemm_gated(w, w2, x, out=words(w2[0], T * M).view(T, M)), "packed, transposed": lambda: dk.gemm_t(*w, g, out=words(w[0], T * K).view(T, K)),
+        "heads": lambda: dk.rotary(fused[:, :4], fused[:, 3:6], positions, frequency, inplace=True),
+        "frequency": lambda: dk.rotary(fused[:, :4], None, positions, fused.view(-1)[:32], inplace=True),
+        "k and v": lambda: read(rows[:20], rows[19:39]), "pool": lambda: read(cache.k.view(-1).view(torch.float16).view(-1, 2, 64)[:20], rows[:20]),
+        "heads of k and v": lambda: read(rows.view(41, 128)[:20].view(20, 2, 64), rows.view(-1)[64:64 + 20 * 128].view(20, 2, 64)),
+    }
+    before = [t.clone() for t in (wide, *w, *w2, fused, cache.k, rows)]
+    for name, call in bad.items():
+        with pytest.raises(RuntimeError, match="overlap"):
+            call()
+            pytest.fail(f"{name} was not refused")
+    assert all(torch.equal(a, b) for a, b in zip(before, (wide, *w, *w2, fused, cache.k, rows)))
+    # Beside one another in the same memory.
+    want = dk.gemm(*w, x)
+    assert torch.equal(dk.gemm(*w, x, out=wide[:, K:K + M]), want) and torch.equal(wide[:, K:K + M], want)
+    want = dk.gemm_gated(w, w2, x)
+    assert torch.equal(dk.gemm_gated(w, w2, x, out=wide[:, K + 1:K + 1 + M]), want)
+    assert torch.equal(dk.gemm(*w, x[::2], out=wide[1::2, :M]), dk.gemm(*w, before[0][::2, :K]))
+    q, k = fused[:, :4], fused[:, 4:6]
+    want = dk.rotary(q, k, positions, frequency)
+    assert all(torch.equal(a, b) for a, b in zip(dk.rotary(q, k, positions, frequency, inplace=True), want))
+    both = torch.zeros(20, 2, 2, 64, dtype=torch.float16, device="cuda")
+    want = dk.cache_read(cache, table, lengths, starts, 20)
+    assert all(torch.equal(a, b) for a, b in zip(read(both[:, 0], both[:, 1]), want))
