@@ -890,7 +890,8 @@ std::tuple<torch::Tensor, OptTensor> rotary(torch::Tensor q, OptTensor k, torch:
       TORCH_CHECK(t.stride(2) == 1, "q and k that are turned in place must have contiguous heads");
       for (int64_t i = 0; i < 2; ++i)
         TORCH_CHECK(t.size(i) == 1 || t.stride(i) >= dim, "q and k that are turned in place may not overlap themselves");
-      TORCH_CHECK(t.size(0) <= 1 || t.size(1) == 1 || t.stride(0) >= t.size(1) * t.stride(1) || t.stride(1) >= t.size(0) * t.stride(0),
+      TORCH_CHECK(t.size(0) <= 1 || t.size(1) == 1 || t.stride(0) >= (t.size(1) - 1) * t.stride(1) + dim ||
+                      t.stride(1) >= (t.size(0) - 1) * t.stride(0) + dim,
                   "q and k that are turned in place may not overlap themselves");
     }
     const torch::Tensor from = t.stride(2) == 1 ? t : t.contiguous();

@@ -113,3 +113,16 @@ def test_outputs_over_inputs_are_refused_and_beside_them_are_not():
     both = torch.zeros(20, 2, 2, 64, dtype=torch.float16, device="cuda")
     want = dk.cache_read(cache, table, lengths, starts, 20)
     assert all(torch.equal(a, b) for a, b in zip(read(both[:, 0], both[:, 1]), want))
+
+
+def test_every_second_head_is_turned_in_place():
+    """Heads that lie two apart, of an odd number: a token's last one ends before the next token's first."""
+    positions, frequency = torch.arange(6, device="cuda"), torch.rand(32, device="cuda")
+    fused = torch.randn(6, 9, 64, device="cuda")
+    for base in (fused, fused.transpose(0, 1).contiguous().transpose(0, 1)):
+        q, k = base[:, ::2], base[:, 1::2]
+        want = [t.clone() for t in dk.rotary(q, k, positions, frequency)]
+        assert all(torch.equal(a, b) for a, b in zip(dk.rotary(q, k, positions, frequency, inplace=True), want))
+    alike = torch.as_strided(fused, (6, 3, 64), (160, 64, 1))
+    with pytest.raises(RuntimeError, match="overlap themselves"):  # a token's last head begins before the next token's first
+        dk.rotary(alike, None, positions, frequency, inplace=True)
