@@ -707,10 +707,17 @@ bool shares_memory(const torch::Tensor& a, const torch::Tensor& b) {
   return s.meet(0, static_cast<int64_t>(reinterpret_cast<intptr_t>(a.data_ptr()) - reinterpret_cast<intptr_t>(b.data_ptr())));
 }
 
+// Forward-mode derivatives would be lost (or, of tensors written over, go stale).
+void check_no_tangent(std::initializer_list<const torch::Tensor*> tensors) {
+  for (const torch::Tensor* t : tensors)
+    TORCH_CHECK(!t || !t->defined() || !t->_fw_grad(0).defined(), "forward-mode derivatives are not supported");
+}
+const torch::Tensor* if_any(const OptTensor& t) { return t ? &*t : nullptr; }
+
 // What a kernel writes is nothing of what it reads.
 void check_apart(const torch::Tensor& out, const char* what, std::initializer_list<const torch::Tensor*> inputs) {
   for (const torch::Tensor* in : inputs)
-    TORCH_CHECK(!in->defined() || !shares_memory(out, *in), what, " may not overlap the call's inputs");
+    TORCH_CHECK(!in || !shares_memory(out, *in), what, " may not overlap the call's inputs");
 }
 
 // An output given by the caller: contiguous rows of any stride, or a new one.
@@ -729,6 +736,7 @@ torch::Tensor output(const OptTensor& out, const std::vector<int64_t>& shape, co
 std::tuple<torch::Tensor, OptTensor, OptTensor> w4a16_gemm(torch::Tensor packed, torch::Tensor scales, OptTensor packed2,
                                                            OptTensor scales2, torch::Tensor x, int act, bool keep,
                                                            OptTensor out) {
+  check_no_tangent({&x, &scales, if_any(scales2), if_any(out)});
   const Weights w(packed, scales, x);
   dk_gemm_args a{};
   a.dtype = half_type(x, "x");
@@ -744,8 +752,7 @@ std::tuple<torch::Tensor, OptTensor, OptTensor> w4a16_gemm(torch::Tensor packed,
   }
   const torch::Tensor xr = in_rows(x, w.K);
   const std::vector<int64_t> shape = shape_with(x, w.M);
-  const torch::Tensor none;
-  torch::Tensor y = output(out, shape, x, {&packed, &scales, packed2 ? &*packed2 : &none, scales2 ? &*scales2 : &none});
+  torch::Tensor y = output(out, shape, x, {&packed, &scales, if_any(packed2), if_any(scales2)});
   OptTensor g, u;
   if (keep) {  // kept for the gradient, whose product wants rows a multiple of 8 apart
     const int64_t wide = (w.M + 7) / 8 * 8;
@@ -778,6 +785,7 @@ std::tuple<torch::Tensor, OptTensor, OptTensor> w4a16_gemm(torch::Tensor packed,
 
 torch::Tensor w4a16_gemm_t(torch::Tensor packed, torch::Tensor scales, OptTensor packed2, OptTensor scales2,
                            torch::Tensor g, OptTensor g2, OptTensor out) {
+  check_no_tangent({&g, &scales, if_any(g2), if_any(scales2), if_any(out)});
   const Weights w(packed, scales, g);
   dk_gemm_t_args a{};
   a.dtype = half_type(g, "g");
@@ -800,8 +808,7 @@ torch::Tensor w4a16_gemm_t(torch::Tensor packed, torch::Tensor scales, OptTensor
     a.scales2 = w2->factors();
     a.g2 = gr2.data_ptr();
   }
-  const torch::Tensor none;
-  torch::Tensor dx = output(out, shape_with(g, w.K), g, {&packed, &scales, packed2 ? &*packed2 : &none, scales2 ? &*scales2 : &none, g2 ? &*g2 : &none});
+  torch::Tensor dx = output(out, shape_with(g, w.K), g, {&packed, &scales, if_any(packed2), if_any(scales2), if_any(g2)});
   a.packed = w.words();
   a.scales = w.factors();
   a.g = gr.data_ptr();
@@ -841,6 +848,7 @@ std::tuple<torch::Tensor, torch::Tensor> gated_grad(torch::Tensor dh, torch::Ten
 std::tuple<torch::Tensor, OptTensor> rotary(torch::Tensor q, OptTensor k, torch::Tensor positions, torch::Tensor frequency,
                                             std::optional<std::vector<int64_t>> sections, bool paired, bool inverse,
                                             bool inplace) {
+  check_no_tangent({&q, if_any(k), &frequency});
   TORCH_CHECK(q.is_cuda(), "q must be a CUDA tensor");
   TORCH_CHECK(q.dim() == 3, "q must be [tokens, q_heads, head_dim]");
   const torch::Device device = q.device();
@@ -933,6 +941,7 @@ std::tuple<torch::Tensor, OptTensor> rotary(torch::Tensor q, OptTensor k, torch:
 std::tuple<torch::Tensor, torch::Tensor> cache_read(const Cache8& cache, torch::Tensor block_table, torch::Tensor lengths,
                                                     torch::Tensor starts, int64_t tokens, torch::ScalarType type, OptTensor k,
                                                     OptTensor v) {
+  check_no_tangent({if_any(k), if_any(v)});
   const torch::Device device = cache.k.device();
   TORCH_CHECK(lengths.dim() == 1, "lengths must be [requests]");
   const int64_t n = lengths.size(0);

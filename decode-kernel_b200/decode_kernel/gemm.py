@@ -48,7 +48,7 @@ def gemm(packed: torch.Tensor, scales: torch.Tensor, x: torch.Tensor, *,
     results that are not finite; which of the two is the formula's answer for a
     single infinity in a group of 128.  x may be any view;
     rows that do not begin on 16-byte boundaries are copied first.  ``out`` is
-    contiguous or has contiguous rows.  Differentiable in x.
+    contiguous or has contiguous rows.  Differentiable in x (reverse mode).
     """
     return _extension().linear(False, packed, scales, x, out)
 
@@ -58,7 +58,7 @@ def gemm_t(packed: torch.Tensor, scales: torch.Tensor, g: torch.Tensor, *,
     """g . dequant(W): fp16 or bf16 [..., M] -> [..., K], the gradient of ``gemm``'s x.
 
     The types of ``gemm``; weights are rounded as for its many rows.  Differentiable
-    in g.
+    in g (reverse mode).
     """
     return _extension().linear(True, packed, scales, g, out)
 
@@ -70,8 +70,8 @@ def gemm_gated(gate: Tuple[torch.Tensor, torch.Tensor], up: Tuple[torch.Tensor, 
     ``gate`` and ``up``: ``(packed, scales)`` of two [M, K] matrices; ``act``:
     "silu" or "gelu" (its tanh form).  Everything between the products' fp32
     sums and the result is fp32, rounded once (``gemv_silu_mul`` rounds as the
-    unfused fp16 sequence does).  Differentiable in x: the two projections are
-    kept in x's type for that.
+    unfused fp16 sequence does).  Differentiable in x (reverse mode, once): the
+    two projections are kept in x's type for that.
     """
     if act not in _ACTS:
         raise ValueError("act is 'silu' or 'gelu'")

@@ -22,10 +22,16 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from .quantize import GROUP_SIZE, quantize_and_pack_cuda
 
 __all__ = ["W4A16GatedMLP", "W4A16Linear", "w4a16_linear_op", "w4a16_silu_mul_op"]
+
+
+def _no_tangent(x: torch.Tensor) -> None:
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None:
+        raise RuntimeError("forward-mode derivatives are not supported")
 
 
 @torch.library.custom_op("decode_kernel::w4a16_linear", mutates_args=())
@@ -33,6 +39,7 @@ def w4a16_linear_op(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor)
     """y[..., M] = x[..., K] . dequant(W)^T (fp16), any number of leading dims."""
     from . import gemv
 
+    _no_tangent(x)
     if not x.is_cuda:
         raise RuntimeError("decode_kernel::w4a16_linear runs on CUDA tensors only")
     lead = x.shape[:-1]
@@ -130,6 +137,7 @@ class W4A16Linear(torch.nn.Module):
         return cls(packed, s)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        _no_tangent(x)
         return torch.ops.decode_kernel.w4a16_linear(x, self.packed, self.scales)
 
     def extra_repr(self) -> str:

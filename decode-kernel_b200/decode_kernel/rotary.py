@@ -29,6 +29,6 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
 
     Angles are taken in fp64, so far positions are right; sines, cosines and the
     turning are fp32, rounded once.  ``inverse`` turns back.  ``inplace`` writes
-    over q and k.  Differentiable in q and k (not in place).
+    over q and k.  Differentiable in q and k (reverse mode, not in place).
     """
     return _extension().rotary(q, k, positions, frequency, sections, paired, inverse, inplace)

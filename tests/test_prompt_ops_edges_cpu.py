@@ -7,6 +7,7 @@ import random
 import pytest
 import torch
 
+import decode_kernel as dk
 from decode_kernel import _cuda
 
 
@@ -55,3 +56,27 @@ def test_slices_of_a_projection(heads):
     assert not share(flat[:, :100], flat[:, 100:]) and share(flat[:, :101], flat[:, 100:]) and share(flat[:, 5:6], flat.t()[5:7])
     assert not share(fused[..., :32], fused[..., 32:]) and share(fused[..., :33], fused[..., 32:])
     assert not share(fused, fused.clone()) and share(fused, fused.view(torch.int8)[..., 127:])
+
+
+PACKED, SCALES = torch.zeros(64, 32, dtype=torch.int32), torch.zeros(64, 2, dtype=torch.float16)
+PAIR = (PACKED, SCALES)
+DIFFERENTIABLE = {
+    "gemm": (lambda x: dk.gemm(*PAIR, x), (3, 256)), "gemm_t": (lambda x: dk.gemm_t(*PAIR, x), (3, 64)), "gemm_gated": (lambda x: dk.gemm_gated(PAIR, PAIR, x), (3, 256)),
+    "rotary": (lambda x: dk.rotary(x, None, torch.zeros(3, dtype=torch.int32), torch.ones(4)), (3, 2, 8)),
+    "rotary in place": (lambda x: dk.rotary(x, None, torch.zeros(3, dtype=torch.int32), torch.ones(4), inplace=True), (3, 2, 8)),
+    "linear": (lambda x: dk.W4A16Linear(*PAIR)(x), (3, 256)), "linear's op": (lambda x: torch.ops.decode_kernel.w4a16_linear(x, *PAIR), (3, 256)),
+}
+
+
+@pytest.mark.parametrize("which", list(DIFFERENTIABLE))
+def test_forward_mode_is_refused(which):
+    call, shape = DIFFERENTIABLE[which]
+    x = torch.zeros(shape, dtype=torch.float16)
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            call(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)))
+    if which == "linear":
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.func.jvp(call, (x,), (torch.ones_like(x),))
+    with pytest.raises(RuntimeError, match="CUDA"):  # without a tangent it is the device that is refused
+        call(x)
