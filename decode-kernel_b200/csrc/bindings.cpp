@@ -712,6 +712,12 @@ void check_no_tangent(std::initializer_list<const torch::Tensor*> tensors) {
   for (const torch::Tensor* t : tensors)
     TORCH_CHECK(!t || !t->defined() || !t->_fw_grad(0).defined(), "forward-mode derivatives are not supported");
 }
+// What is written over keeps no history: a gradient through it would be that of what
+// stood there.
+void check_no_history(const OptTensor& out) {
+  TORCH_CHECK(!out || !torch::GradMode::is_enabled() || !out->requires_grad(),
+              "out takes no part in a gradient: give one that requires none, or call under torch.no_grad()");
+}
 const torch::Tensor* if_any(const OptTensor& t) { return t ? &*t : nullptr; }
 
 // What a kernel writes is nothing of what it reads.
@@ -737,6 +743,7 @@ std::tuple<torch::Tensor, OptTensor, OptTensor> w4a16_gemm(torch::Tensor packed,
                                                            OptTensor scales2, torch::Tensor x, int act, bool keep,
                                                            OptTensor out) {
   check_no_tangent({&x, &scales, if_any(scales2), if_any(out)});
+  check_no_history(out);
   const Weights w(packed, scales, x);
   dk_gemm_args a{};
   a.dtype = half_type(x, "x");
@@ -786,6 +793,7 @@ std::tuple<torch::Tensor, OptTensor, OptTensor> w4a16_gemm(torch::Tensor packed,
 torch::Tensor w4a16_gemm_t(torch::Tensor packed, torch::Tensor scales, OptTensor packed2, OptTensor scales2,
                            torch::Tensor g, OptTensor g2, OptTensor out) {
   check_no_tangent({&g, &scales, if_any(g2), if_any(scales2), if_any(out)});
+  check_no_history(out);
   const Weights w(packed, scales, g);
   dk_gemm_t_args a{};
   a.dtype = half_type(g, "g");
@@ -942,6 +950,8 @@ std::tuple<torch::Tensor, torch::Tensor> cache_read(const Cache8& cache, torch::
                                                     torch::Tensor starts, int64_t tokens, torch::ScalarType type, OptTensor k,
                                                     OptTensor v) {
   check_no_tangent({if_any(k), if_any(v)});
+  check_no_history(k);
+  check_no_history(v);
   const torch::Device device = cache.k.device();
   TORCH_CHECK(lengths.dim() == 1, "lengths must be [requests]");
   const int64_t n = lengths.size(0);

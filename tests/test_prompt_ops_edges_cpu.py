@@ -80,3 +80,15 @@ def test_forward_mode_is_refused(which):
             torch.func.jvp(call, (x,), (torch.ones_like(x),))
     with pytest.raises(RuntimeError, match="CUDA"):  # without a tangent it is the device that is refused
         call(x)
+
+
+def test_outputs_that_require_a_gradient_are_refused():
+    x, g = torch.zeros(3, 256, dtype=torch.float16), torch.zeros(3, 64, dtype=torch.float16)
+    y, dx = torch.zeros(3, 64, dtype=torch.float16, requires_grad=True), torch.zeros(3, 256, dtype=torch.float16, requires_grad=True)
+    calls = (lambda out: dk.gemm(*PAIR, x, out=out), y), (lambda out: dk.gemm_gated(PAIR, PAIR, x, out=out), y), (lambda out: dk.gemm_t(*PAIR, g, out=out), dx)
+    for call, out in calls:
+        for given in (out, out * 2):
+            with pytest.raises(RuntimeError, match="out takes no part"):
+                call(given)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+                call(given)

@@ -126,3 +126,19 @@ def test_every_second_head_is_turned_in_place():
     alike = torch.as_strided(fused, (6, 3, 64), (160, 64, 1))
     with pytest.raises(RuntimeError, match="overlap themselves"):  # a token's last head begins before the next token's first
         dk.rotary(alike, None, positions, frequency, inplace=True)
+
+
+def test_outputs_of_a_graph_are_refused_but_under_no_grad():
+    w = weights(128, 256, 1)
+    x = rows_of(20, 256, torch.float16, 3)
+    leaf = torch.zeros(20, 128, dtype=torch.float16, device="cuda", requires_grad=True)
+    cache = dk.PagedCache8(4, 16, 2, 64)
+    ints = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    kv = [torch.zeros(20, 2, 64, dtype=torch.float16, device="cuda", requires_grad=i == 1) for i in range(2)]
+    calls = [lambda: dk.gemm(*w, x, out=leaf), lambda: dk.gemm_gated(w, w, x, out=leaf * 2), lambda: dk.cache_read(cache, ints([[0, 1]]), ints([20]), ints([0, 20]), 20, out=kv)]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="out takes no part"):
+            call()
+        with torch.no_grad():
+            call()
+    assert torch.equal(leaf.detach(), dk.gemm(*w, x))
