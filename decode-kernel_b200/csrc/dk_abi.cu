@@ -4,6 +4,8 @@
 #include <cstring>
 #include <mutex>
 
+#include <cudaTypedefs.h>
+
 #include "dk_host.h"
 
 namespace dk {
@@ -40,6 +42,30 @@ int sm_count(int device) {
     g_sm_cache[device] = sms;
   }
   return sms;
+}
+
+bool encode_tensor_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* at, const cuuint64_t* dims,
+                       const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle,
+                       CUtensorMapL2promotion promotion) {
+  static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  }();
+  if (!encode) return false;
+  const cuuint32_t steps[5] = {1, 1, 1, 1, 1};
+  auto encoded = [&] {
+    return encode(map, type, (cuuint32_t)rank, const_cast<void*>(at), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  swizzle, promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  if (encoded()) return true;
+  if (cudaSetDevice(current_device()) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return false;
+  }
+  return encoded();
 }
 
 }  // namespace dk

@@ -327,16 +327,12 @@ bool x_tensor_map(const void* x, int K, int B, CUtensorMap* out) {
     }
     if (e.stamp < victim->stamp) victim = &e;
   }
-  EncodeTiledFn enc = encode_fn();
-  if (!enc) return false;
   CUtensorMap map;
   cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)B};
   cuuint64_t strides[1] = {(cuuint64_t)K * 2};
   cuuint32_t box[2] = {(cuuint32_t)vb::kAtomK, (cuuint32_t)vb::kXRows};
-  cuuint32_t elem[2] = {1, 1};
-  if (enc(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(x), dims, strides, box, elem,
-          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-          CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+  if (!encode_tensor_map(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, x, dims, strides, box,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B))
     return false;
   *victim = Entry{x, K, B, ++clock, map};
   *out = map;
@@ -366,16 +362,12 @@ bool raw_tensor_map(const void* packed, int M, int K, int ntile, CUtensorMap* ou
     }
     if (e.stamp < victim->stamp) victim = &e;
   }
-  EncodeTiledFn enc = encode_fn();
-  if (!enc) return false;
   CUtensorMap map;
   cuuint64_t dims[2] = {(cuuint64_t)K / 2, (cuuint64_t)M};
   cuuint64_t strides[1] = {(cuuint64_t)K / 2};
   cuuint32_t box[2] = {(cuuint32_t)vb::kRawRowBytes, (cuuint32_t)ntile};
-  cuuint32_t elem[2] = {1, 1};
-  if (enc(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(packed), dims, strides, box,
-          elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
-          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+  if (!encode_tensor_map(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, packed, dims, strides, box,
+                         CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B))
     return false;
   *victim = Entry{packed, M, K, ntile, ++clock, map};
   *out = map;

@@ -33,7 +33,6 @@
 // of eight, A through tensor memory where possible, whole warps with uniform
 // operands around single-thread instructions (34 cycles an MMA instead of 80).
 #include <cuda.h>
-#include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -881,26 +880,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
-PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
-  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
-      f = nullptr;
-    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
-  }();
-  return fn;
-}
-
 // A matrix of `rows` rows, `stride` bytes apart, in boxes of `box` rows.
 bool tensor_map(CUtensorMap* map, const void* at, CUtensorMapDataType type, uint64_t width, uint64_t rows, uint64_t stride, uint32_t box_width,
                 uint32_t box, CUtensorMapSwizzle swizzle) {
-  const auto encode = tensor_map_encoder();
-  if (!encode) return false;
   const cuuint64_t dims[2] = {width, rows}, strides[1] = {stride};
-  const cuuint32_t boxes[2] = {box_width, box}, steps[2] = {1, 1};
-  return encode(map, type, 2, const_cast<void*>(at), dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  const cuuint32_t boxes[2] = {box_width, box};
+  return encode_tensor_map(map, type, 2, at, dims, strides, boxes, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
 }
 
 struct Product {

@@ -43,7 +43,6 @@
 #include <mutex>
 
 #include <cuda.h>
-#include <cudaTypedefs.h>
 
 #define DK_DEVICE_GLOBALS
 #include "dk_device.cuh"
@@ -1486,21 +1485,6 @@ dk_status ensure_smem(Kern kernel, size_t bytes, std::atomic<unsigned long long>
 // {128-byte strip, row, strip index} with strides {K/2, 128} bytes, boxes of
 // 16 rows x 16 strips (32 KB), 128-byte swizzle.  Encoded once per
 // (pointer, M, K) -- the map holds nothing else -- and kept in a small cache.
-using EncodeTiledFn = PFN_cuTensorMapEncodeTiled_v12000;
-
-EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = [] {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) !=
-            cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      return static_cast<EncodeTiledFn>(nullptr);
-    return reinterpret_cast<EncodeTiledFn>(f);
-  }();
-  return fn;
-}
-
 bool weight_tensor_map(const void* packed, int M, int K, CUtensorMap* out) {
   struct Entry {
     const void* ptr;
@@ -1521,16 +1505,12 @@ bool weight_tensor_map(const void* packed, int M, int K, CUtensorMap* out) {
     }
     if (e.stamp < victim->stamp) victim = &e;
   }
-  EncodeTiledFn enc = encode_fn();
-  if (!enc) return false;
   CUtensorMap map;
   cuuint64_t dims[3] = {(cuuint64_t)v5::kStrip, (cuuint64_t)M, (cuuint64_t)(K / 256)};
   cuuint64_t strides[2] = {(cuuint64_t)K / 2, (cuuint64_t)v5::kStrip};
   cuuint32_t box[3] = {(cuuint32_t)v5::kStrip, 16u, (cuuint32_t)v5::kStripsPerChunk};
-  cuuint32_t elem[3] = {1, 1, 1};
-  if (enc(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(packed), dims, strides, box,
-          elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+  if (!encode_tensor_map(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, packed, dims, strides, box,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B))
     return false;
   victim->ptr = packed;
   victim->M = M;

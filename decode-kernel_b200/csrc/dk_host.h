@@ -4,6 +4,7 @@
 #include <algorithm>
 #include <cstdint>
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include "dk_w4a16.h"
@@ -23,6 +24,14 @@ int current_device();
 // Device address of the device error word on the current device (defined in
 // dk_gemv.cu), for kernels of other translation units; nullptr on failure.
 int* device_error_address();
+
+// A tiled tensor map of steps of one, without interleaving, zeros outside; false
+// where the driver refuses it.  The driver wants a context that is current in the
+// calling thread, which a thread lacks until the runtime has done something there
+// (autograd's threads begin like that): the current device's is made current then.
+bool encode_tensor_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* at, const cuuint64_t* dims,
+                       const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle,
+                       CUtensorMapL2promotion promotion);
 
 // A gated pair of GEMVs for at most 8 contiguous fp16 rows, h rounded once
 // (defined in dk_gemv.cu).

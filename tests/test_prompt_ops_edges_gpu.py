@@ -142,3 +142,22 @@ def test_outputs_of_a_graph_are_refused_but_under_no_grad():
         with torch.no_grad():
             call()
     assert torch.equal(leaf.detach(), dk.gemm(*w, x))
+
+
+def test_calls_on_threads_of_their_own():
+    """A thread's first CUDA call may be one of the products, as in autograd's threads: nothing has made a context current there."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    w, w2 = weights(128, 256, 1), weights(128, 256, 2)
+    large = weights(16384, 256, 3)
+    xs = [rows_of(T, 256, torch.float16, T) for T in (1, 4, 12, 20, 300)]
+    gs = [rows_of(T, 128, torch.float16, T) for T in (4, 20, 300)]
+    calls = [lambda x=x: dk.gemm(*w, x) for x in xs] + [lambda x=x: dk.gemm_gated(w, w2, x) for x in xs] + [lambda g=g: dk.gemm_t(*w, g) for g in gs]
+    calls += [lambda x=x: dk.gemv(*large, x) for x in xs[:4]]
+    want = [call() for call in calls]
+    torch.cuda.synchronize()
+    for call, expected in zip(calls, want):
+        with ThreadPoolExecutor(1) as thread:
+            got = thread.submit(call).result()
+        torch.cuda.synchronize()
+        assert torch.equal(got, expected)
