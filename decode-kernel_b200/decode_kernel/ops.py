@@ -55,20 +55,40 @@ def _(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor) -> torch.Tens
     return x.new_empty((*x.shape[:-1], packed.shape[0]), dtype=torch.float16)
 
 
+@torch.library.custom_op("decode_kernel::w4a16_linear_grad", mutates_args=())
+def w4a16_linear_grad_op(dy: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """dx[..., K] = dy[..., M] . dequant(W): the gradient of w4a16_linear, an operator so that it can be traced."""
+    from . import gemm_t
+
+    return gemm_t(packed, scales, dy)
+
+
+@w4a16_linear_grad_op.register_fake
+def _(dy: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    return dy.new_empty((*dy.shape[:-1], packed.shape[1] * 8))
+
+
 def _linear_context(ctx, inputs, output) -> None:
     _, packed, scales = inputs
     ctx.save_for_backward(packed, scales)
 
 
 def _linear_backward(ctx, dy: torch.Tensor):
-    from . import gemm_t
+    if ctx.needs_input_grad[2]:
+        raise RuntimeError("the weights are frozen: scales must not require a gradient")
+    return (w4a16_linear_grad_op(dy, *ctx.saved_tensors) if ctx.needs_input_grad[0] else None), None, None
+
+
+def _linear_grad_backward(ctx, ddx: torch.Tensor):
+    from . import gemm
 
     if ctx.needs_input_grad[2]:
         raise RuntimeError("the weights are frozen: scales must not require a gradient")
-    return (gemm_t(*ctx.saved_tensors, dy) if ctx.needs_input_grad[0] else None), None, None
+    return (gemm(*ctx.saved_tensors, ddx) if ctx.needs_input_grad[0] else None), None, None
 
 
 w4a16_linear_op.register_autograd(_linear_backward, setup_context=_linear_context)
+w4a16_linear_grad_op.register_autograd(_linear_grad_backward, setup_context=_linear_context)
 
 
 @torch.library.custom_op("decode_kernel::w4a16_silu_mul", mutates_args=())

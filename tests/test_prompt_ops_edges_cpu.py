@@ -92,3 +92,21 @@ def test_outputs_that_require_a_gradient_are_refused():
                 call(given)
             with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
                 call(given)
+
+
+def test_the_linear_layers_gradient_is_traced():
+    """Forward and backward with tensors that have no data, as a compiler runs them."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    def step(x, dy, packed, scales):
+        x = x.detach().requires_grad_()
+        return torch.autograd.grad(torch.ops.decode_kernel.w4a16_linear(x, packed, scales), x, dy)[0]
+
+    for shape in ((3,), (2, 5), ()):
+        with FakeTensorMode():
+            args = (torch.empty(*shape, 256, dtype=torch.float16), torch.empty(*shape, 64, dtype=torch.float16), torch.empty(64, 32, dtype=torch.int32), torch.empty(64, 2, dtype=torch.float16))
+            dx = step(*args)
+            assert dx.shape == (*shape, 256) and dx.dtype == torch.float16
+    graph = make_fx(step, tracing_mode="fake")(torch.zeros(3, 256, dtype=torch.float16), torch.zeros(3, 64, dtype=torch.float16), PACKED, SCALES)
+    assert sum("w4a16_linear" in str(n.target) for n in graph.graph.nodes) == 2

@@ -161,3 +161,16 @@ def test_calls_on_threads_of_their_own():
             got = thread.submit(call).result()
         torch.cuda.synchronize()
         assert torch.equal(got, expected)
+
+
+def test_the_linear_layers_gradient_compiled_and_twice():
+    layer = dk.W4A16Linear(*weights(128, 256, 1))
+    x = rows_of(20, 256, torch.float16, 3).requires_grad_()
+    dy = rows_of(20, 128, torch.float16, 4).requires_grad_()
+    want, = torch.autograd.grad(layer(x), x, dy)
+    assert torch.equal(want, dk.gemm_t(layer.packed, layer.scales, dy.detach()))
+    got, = torch.autograd.grad(torch.compile(layer, backend="aot_eager", fullgraph=True)(x), x, dy)
+    assert torch.equal(got, want)
+    once, = torch.autograd.grad(layer(x), x, dy, create_graph=True)
+    twice, = torch.autograd.grad(once, dy, x.detach())
+    assert torch.equal(twice, dk.gemm(layer.packed, layer.scales, x.detach()))
