@@ -164,12 +164,21 @@ class W4A16Linear(torch.nn.Module):
         return f"in_features={self.in_features}, out_features={self.out_features}, bits=4, group={GROUP_SIZE}"
 
 
+def _plain(layer: torch.nn.Module) -> bool:
+    """Whether a call of the layer is its product and nothing else: no adapter in its place or round its forward, no hooks."""
+    return (type(layer) is W4A16Linear and "forward" not in layer.__dict__ and not layer._forward_hooks and not layer._forward_pre_hooks
+            and not layer._backward_hooks and not layer._backward_pre_hooks)
+
+
 class W4A16GatedMLP(torch.nn.Module):
     """A gated feed-forward block with frozen 4-bit weights: down(act(gate(x)) * up(x)).
 
     ``gate``, ``up`` and ``down`` are ``W4A16Linear`` layers; ``act`` is "silu"
-    or "gelu" (its tanh form).  Two launches for any number of rows, and
-    gradients for x.
+    or "gelu" (its tanh form).  Two products for any number of rows
+    (``gemm_gated`` and ``gemm``, fp16 or bf16), and gradients for x.  Layers
+    that have hooks, or that an adapter has taken the place of, are called as
+    modules, and the activation is torch's then: gate and up both where one of
+    them is, down by itself.
     """
 
     def __init__(self, gate: W4A16Linear, up: W4A16Linear, down: W4A16Linear, act: str = "silu"):
@@ -183,5 +192,9 @@ class W4A16GatedMLP(torch.nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         from . import gemm, gemm_gated
 
-        h = gemm_gated((self.gate.packed, self.gate.scales), (self.up.packed, self.up.scales), x, act=self.act)
-        return gemm(self.down.packed, self.down.scales, h)
+        if _plain(self.gate) and _plain(self.up):
+            h = gemm_gated((self.gate.packed, self.gate.scales), (self.up.packed, self.up.scales), x, act=self.act)
+        else:
+            g = self.gate(x)
+            h = (torch.nn.functional.silu(g) if self.act == "silu" else torch.nn.functional.gelu(g, approximate="tanh")) * self.up(x)
+        return gemm(self.down.packed, self.down.scales, h) if _plain(self.down) else self.down(h)

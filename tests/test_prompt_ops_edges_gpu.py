@@ -174,3 +174,40 @@ def test_the_linear_layers_gradient_compiled_and_twice():
     once, = torch.autograd.grad(layer(x), x, dy, create_graph=True)
     twice, = torch.autograd.grad(once, dy, x.detach())
     assert torch.equal(twice, dk.gemm(layer.packed, layer.scales, x.detach()))
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_hooks_and_adapters_of_a_gated_blocks_layers_count(act):
+    class Adapter(torch.nn.Module):
+        def __init__(self, layer):
+            super().__init__()
+            self.layer, self.more = layer, torch.nn.Parameter(torch.full((layer.out_features,), 0.5, dtype=torch.float16, device="cuda"))
+
+        def forward(self, x):
+            return self.layer(x) + self.more
+
+    def block():
+        return dk.W4A16GatedMLP(*(dk.W4A16Linear(*weights(m, k, s)) for m, k, s in ((384, 256, 1), (384, 256, 2), (256, 384, 3))), act=act)
+
+    x = rows_of(20, 256, torch.float16, 4)
+    bare = block()
+    want = bare(x)
+    f = torch.nn.functional.silu if act == "silu" else lambda g: torch.nn.functional.gelu(g, approximate="tanh")
+    for name in ("gate", "up", "down"):
+        mlp, seen = block(), []
+        handle = getattr(mlp, name).register_forward_hook(lambda m, args, out: seen.append(out.shape) or out * 0)
+        assert (mlp(x) == 0).all() and len(seen) == 1
+        handle.remove()
+        assert torch.equal(mlp(x), want)
+        adapter = Adapter(getattr(mlp, name))
+        setattr(mlp, name, adapter)
+        got = mlp(x)
+        parts = {n: getattr(mlp, n) for n in ("gate", "up", "down")}
+        if name == "down":
+            h = dk.gemm_gated((bare.gate.packed, bare.gate.scales), (bare.up.packed, bare.up.scales), x, act=act)
+            assert torch.equal(got, parts["down"](h))
+        else:
+            h = f(parts["gate"](x)) * parts["up"](x)
+            assert torch.equal(got, dk.gemm(bare.down.packed, bare.down.scales, h))
+        got.float().square().mean().backward()
+        assert adapter.more.grad.abs().max() > 0
