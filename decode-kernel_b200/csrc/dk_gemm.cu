@@ -302,7 +302,7 @@ __device__ __forceinline__ float gate_of(float g, int act, float& slope) {
   if (act == DK_MLP_GELU) {
     constexpr float c = 1.5957691216057308f;  // 2 sqrt(2 / pi)
     p = c * (g + 0.044715f * g * g * g);
-    slope = c * (1.f + 0.134145f * g * g);
+    slope = c * (1.f + 0.134145f * fminf(g * g, 1e30f));  // finite, where the sigmoid has long run out
   }
   // 1 / (1 + 2^(-p log2 e)); the two approximations are 2^-22 right.
   float e, y;
@@ -1185,8 +1185,11 @@ __global__ void __launch_bounds__(256) k_gated_grad(const __grid_constant__ Grad
     const float d = (float)dh.v[j], gv = (float)g.v[j];
     float slope;
     const float s = gate_of(gv, a.act, slope);
-    dg.v[j] = (T)(d * (float)u.v[j] * (s + gv * s * (1.f - s) * slope));
-    du.v[j] = (T)(d * gv * s);
+    // Where the sigmoid has run out to 0 or 1 a projection may be infinite: kept in
+    // 16 bits it is so past 65504 in fp16.
+    const float bend = s * (1.f - s) * slope;
+    dg.v[j] = (T)(d * (float)u.v[j] * (bend == 0.f ? s : s + gv * bend));
+    du.v[j] = (T)(d * (s == 0.f ? 0.f : gv * s));
   }
   *reinterpret_cast<P*>(static_cast<T*>(a.dg) + r * a.ldd + c) = dg;
   *reinterpret_cast<P*>(static_cast<T*>(a.du) + r * a.ldd + c) = du;

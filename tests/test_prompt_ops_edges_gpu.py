@@ -211,3 +211,31 @@ def test_hooks_and_adapters_of_a_gated_blocks_layers_count(act):
             assert torch.equal(got, dk.gemm(bare.down.packed, bare.down.scales, h))
         got.float().square().mean().backward()
         assert adapter.more.grad.abs().max() > 0
+
+
+@pytest.mark.parametrize("act", [0, 1], ids=["silu", "gelu"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+def test_gradients_of_projections_at_the_ends_of_the_range(dtype, act):
+    """act' is 1 far above zero and 0 far below, also where the kept projection has become infinite or its square would."""
+    far = torch.tensor([1e4, 6e4, 1e20, 3e38, float("inf")], device="cuda").to(dtype)
+    g = torch.cat([far, -far]).repeat(3, 1)
+    u = torch.tensor([[0.5], [-2.0], [0.0]], device="cuda").expand_as(g).to(dtype).contiguous()
+    dh = torch.tensor([[1.0], [0.25], [-3.0]], device="cuda").expand_as(g).to(dtype).contiguous()
+    dg, du = _cuda.gated_grad(dh, g, u, act)
+    high, low = slice(0, 5), slice(5, 10)
+    assert torch.equal(dg[:, high], (dh * u)[:, high]) and (dg[:, low] == 0).all()
+    assert torch.equal(du[:, high], (dh.float() * g.float())[:, high].to(dtype)) and (du[:, low] == 0).all()
+    nan = torch.full_like(g, float("nan"))
+    assert all(t.isnan().all() for t in _cuda.gated_grad(dh, nan, u, act) + _cuda.gated_grad(nan, g, u, act))
+
+
+@pytest.mark.parametrize("T", [3, 40, 300])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_gradient_where_gates_are_shut_past_the_range(T, act):
+    """Gates of -358400, which fp16 does not hold: the block's outputs are zeros and so are its gradients."""
+    gate = torch.full((64, 32), -0x66666667, dtype=torch.int32, device="cuda"), torch.ones((64, 2), dtype=torch.float16, device="cuda")  # every code -7
+    up = weights(64, 256, 5)
+    x = torch.full((T, 256), 200.0, dtype=torch.float16, device="cuda", requires_grad=True)
+    h = dk.gemm_gated(gate, up, x, act=act)
+    dx, = torch.autograd.grad(h, x, torch.ones_like(h))
+    assert (h == 0).all() and (dx == 0).all()
