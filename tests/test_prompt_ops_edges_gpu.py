@@ -9,7 +9,7 @@ import torch
 
 import decode_kernel as dk
 from decode_kernel import _cuda
-from test_prompt_ops_gpu import check_product, rows_of, values, weights
+from test_prompt_ops_gpu import check_product, half_step, rows_of, sum_error, values, weights
 
 pytestmark = pytest.mark.gpu
 
@@ -239,3 +239,59 @@ def test_gradient_where_gates_are_shut_past_the_range(T, act):
     h = dk.gemm_gated(gate, up, x, act=act)
     dx, = torch.autograd.grad(h, x, torch.ones_like(h))
     assert (h == 0).all() and (dx == 0).all()
+
+
+def against_weights_as_they_are(x, w, depth):
+    """(x @ w in 64 bits, what a sum of rounded weights may be off): each weight is half a step of the rows' type off, or half of
+    fp16's smallest step, and the sum has its own error."""
+    total = x.double().abs() @ w.abs()
+    smallest = 2.0 ** -25 * x.double().abs().sum(-1, keepdim=True) if x.dtype == torch.float16 else 0.0
+    return x.double() @ w, total * half_step(x.dtype) + smallest + sum_error(total, depth)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("T,M,K", [(17, 4096, 1408), (40, 1000, 384), (333, 1000, 2816), (1044, 640, 512)])
+def test_products_against_the_weights_as_they_are(T, M, K, dtype):
+    w, w2 = weights(M, K, T), weights(M, K, T + 1)
+    real, real2 = (values(v, torch.float64, 0) for v in (w, w2))
+    x, g = rows_of(T, K, dtype, T + 2), rows_of(T, M, dtype, T + 3)
+    half = half_step(dtype)
+    for got, rows, v, depth in ((dk.gemm(*w, x), x, real.t(), K), (dk.gemm_t(*w, g), g, real, M)):
+        want, off = against_weights_as_they_are(rows, v, depth)
+        assert ((got.double() - want).abs() <= want.abs() * half + off * (1 + half) + 2.0 ** -25).all()
+        # Roundings that go either way add up as their root: the whole stays below four times the result's own rounding.
+        assert (got.double() - want).norm() <= 4 * half * want.norm()
+    (a, ea), (b, eb) = (against_weights_as_they_are(x, v.t(), K) for v in (real, real2))
+    s, p = torch.sigmoid(a), a.abs()
+    want = a * s * b
+    # |act'| <= 1.13; the sigmoid is 2^-21 off times its argument.
+    off = want.abs() * (2 + p) * 2.0 ** -21 + 1.13 * ea * (b.abs() + eb) + (a * s).abs() * eb
+    got = dk.gemm_gated(w, w2, x)
+    assert ((got.double() - want).abs() <= want.abs() * half + off * (1 + half) + 2.0 ** -25).all()
+
+
+def test_boxed_results_on_streams_and_in_graphs():
+    M, K = 704, 1024
+    w, w2 = weights(M, K, 60), weights(M, K, 61)
+    xs = [rows_of(T, K, torch.float16, 62 + T) for T in (300, 1044, 2500)]
+    call = lambda x: (dk.gemm(*w, x), dk.gemm_gated(w, w2, x), dk.gemm_t(*w, dk.gemm(*w, x)))  # noqa: E731
+    want = [call(x) for x in xs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in xs], [[] for _ in xs]
+    for _ in range(10):
+        for s, x, out in zip(streams, xs, got):
+            with torch.cuda.stream(s):
+                out.append(call(x))
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(p, q) for out in b for p, q in zip(a, out))
+    held = [x.clone() for x in xs]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = [call(x) for x in held]
+    for scale in (1.0, -0.5):
+        for x, h in zip(xs, held):
+            h.copy_(x * scale)
+        graph.replay()
+        for h, b in zip(held, out):
+            assert all(torch.equal(p, q) for p, q in zip(call(h), b))
