@@ -88,7 +88,8 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatil
   }
 }
 // A warp's wait, without an answer: after the limit every wait ends at once and
-// the loops run out over whatever is there, without MMAs or results.  Nothing to
+// the loops run out over whatever is there.  What the CTA then writes means nothing,
+// as the device's error word says; it stays within the call's outputs.  Nothing to
 // vote on keeps a wait that need not wait short.
 template <bool SPIN = false>
 __device__ __forceinline__ void warp_wait(uint64_t* bar, uint32_t parity, volatile int* give_up, int* error) {
@@ -304,7 +305,8 @@ __device__ __forceinline__ float gate_of(float g, int act, float& slope) {
     p = c * (g + 0.044715f * g * g * g);
     slope = c * (1.f + 0.134145f * fminf(g * g, 1e30f));  // finite, where the sigmoid has long run out
   }
-  // 1 / (1 + 2^(-p log2 e)); the two approximations are 2^-22 right.
+  // 1 / (1 + 2^(-p log2 e)): the exponent is rounded, |p| 2^-24, and the two
+  // approximations are 2^-22 off; (2 + |p|) 2^-21 holds for all of it.
   float e, y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-1.4426950408889634f * p));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(1.f + e));

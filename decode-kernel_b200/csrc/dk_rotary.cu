@@ -82,8 +82,9 @@ __global__ void __launch_bounds__(kRotaryThreads) k_rotary(const __grid_constant
     const long long at = axis * a.position_stride + token0 + t;
     const double position = a.positions_64 ? (double)static_cast<const long long*>(a.positions)[at]
                                            : (double)static_cast<const int*>(a.positions)[at];
-    // Turns: the product of a 24-bit frequency and 1 / (2 pi) is rounded once,
-    // 2^-53 of the angle; the whole turns drop out without rounding.
+    // Turns: 1 / (2 pi), its product with the frequency and that with the position
+    // are rounded, 2^-53 of the angle each (7e-7 radians at 2^31); the whole turns
+    // drop out without rounding.
     const double turn = position * ((double)a.frequency[p] * 0.15915494309189533577);
     const float part = (float)(turn - rint(turn));
     float s, c;

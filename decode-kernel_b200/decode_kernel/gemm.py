@@ -1,8 +1,9 @@
 """Many rows through 4-bit weights, with gradients through the frozen weights.
 
 ``gemm`` is a layer's product for prompts and batches, ``gemm_gated`` the two
-projections, activation and product of a gated block in one launch, ``gemm_t``
-the transposed product.  The weights are frozen: gradients reach the rows, not
+projections, activation and product of a gated block in one kernel (calls of few
+rows have a small one before it that splits the rows), ``gemm_t`` the transposed
+product.  The weights are frozen: gradients reach the rows, not
 the packed weights or their scales.  There is no CPU fallback.
 """
 
@@ -43,8 +44,9 @@ def gemm(packed: torch.Tensor, scales: torch.Tensor, x: torch.Tensor, *,
 
     packed: int32 [M, K/8]; scales: fp16 [M, K/128].  Past 16 rows (32 of a
     gated pair) a weight q * scale is rounded once to x's type (past its range to
-    infinity), for fewer it is not; products and sums are fp32, and so is the
-    result until it is rounded once.  A row with an infinity or a NaN gives
+    infinity), for fewer it is not, so a row's last bits depend on how many stand
+    beside it (and, up to 8 rows in fp16, on the GEMV's order of sums); products
+    and sums are fp32, and so is the result until it is rounded once.  A row with an infinity or a NaN gives
     results that are not finite; which of the two is the formula's answer for a
     single infinity in a group of 128.  x may be any view;
     rows that do not begin on 16-byte boundaries are copied first.  ``out`` is
@@ -65,7 +67,7 @@ def gemm_t(packed: torch.Tensor, scales: torch.Tensor, g: torch.Tensor, *,
 
 def gemm_gated(gate: Tuple[torch.Tensor, torch.Tensor], up: Tuple[torch.Tensor, torch.Tensor], x: torch.Tensor, *,
                act: str = "silu", out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """act(x . Wg^T) * (x . Wu^T) in one launch: fp16 or bf16 [..., K] -> [..., M].
+    """act(x . Wg^T) * (x . Wu^T) in one kernel: fp16 or bf16 [..., K] -> [..., M].
 
     ``gate`` and ``up``: ``(packed, scales)`` of two [M, K] matrices; ``act``:
     "silu" or "gelu" (its tanh form).  Everything between the products' fp32

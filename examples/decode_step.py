@@ -3,7 +3,7 @@
     PYTHONPATH=decode-kernel_b200 python examples/decode_step.py [--steps 64] [--code int8|e4m3]
 
 Ragged prompts go in as one step (the products of many rows, the gated block in
-one launch), then every request decodes token by token with the whole step --
+one kernel), then every request decodes token by token with the whole step --
 plan, norms, W4A16 products, rotary positions, append, attention -- replayed as
 one CUDA graph: nothing in it waits for the host.  Half-way the requests move to
 a second server with other pages: their cache is read back and written into its.

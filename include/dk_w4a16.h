@@ -322,8 +322,8 @@ DK_API int dk_stream_recommended_blocks(int device);
 DK_API int dk_last_kernel_stamp(int device);
 
 /* Device-side error word of `device` (-1 = current): 0, or 1 when a bounded
- * wait inside a kernel ran out.  Synchronises the device; clears the word
- * when `clear` is non-zero.  (No counterpart in the reference.) */
+ * wait inside a kernel ran out; that call's outputs mean nothing then.
+ * Synchronises the device; clears the word when `clear` is non-zero.  (No counterpart in the reference.) */
 DK_API int dk_device_error(int device, int clear);
 
 /* Format helpers on the GPU, bit-exact with python/decode_kernel/quantize.py
