@@ -166,7 +166,8 @@ class W4A16Linear(torch.nn.Module):
 
 def _plain(layer: torch.nn.Module) -> bool:
     """Whether a call of the layer is its product and nothing else: no adapter in its place or round its forward, no hooks."""
-    return (type(layer) is W4A16Linear and "forward" not in layer.__dict__ and not layer._forward_hooks and not layer._forward_pre_hooks
+    return (isinstance(layer, W4A16Linear) and type(layer).forward is W4A16Linear.forward and "forward" not in layer.__dict__
+            and not layer._forward_hooks and not layer._forward_pre_hooks
             and not layer._backward_hooks and not layer._backward_pre_hooks)
 
 

@@ -189,9 +189,21 @@ def test_hooks_and_adapters_of_a_gated_blocks_layers_count(act):
     def block():
         return dk.W4A16GatedMLP(*(dk.W4A16Linear(*weights(m, k, s)) for m, k, s in ((384, 256, 1), (384, 256, 2), (256, 384, 3))), act=act)
 
+    class Named(dk.W4A16Linear):
+        pass
+
+    class Negative(dk.W4A16Linear):
+        def forward(self, x):
+            return -super().forward(x)
+
     x = rows_of(20, 256, torch.float16, 4)
     bare = block()
     want = bare(x)
+    named, negative = block(), block()
+    named.up = Named(bare.up.packed, bare.up.scales)  # a layer's own product under another name
+    assert torch.equal(named(x), want)
+    negative.down = Negative(bare.down.packed, bare.down.scales)
+    assert torch.equal(negative(x), -bare.down(dk.gemm_gated((bare.gate.packed, bare.gate.scales), (bare.up.packed, bare.up.scales), x, act=act)))
     f = torch.nn.functional.silu if act == "silu" else lambda g: torch.nn.functional.gelu(g, approximate="tanh")
     for name in ("gate", "up", "down"):
         mlp, seen = block(), []
