@@ -695,6 +695,13 @@ struct Strides {
 
 bool shares_memory(const torch::Tensor& a, const torch::Tensor& b) {
   if (a.numel() == 0 || b.numel() == 0) return false;
+  const int64_t distance = static_cast<int64_t>(reinterpret_cast<intptr_t>(a.data_ptr()) - reinterpret_cast<intptr_t>(b.data_ptr()));
+  auto reach = [](const torch::Tensor& t) {  // from the first byte to behind the last
+    int64_t values = 1;
+    for (int64_t i = 0; i < t.dim(); ++i) values += (t.size(i) - 1) * t.stride(i);
+    return values * t.element_size();
+  };
+  if (distance >= reach(b) || -distance >= reach(a)) return false;
   Strides s;
   s.high = s.add(b, true);
   s.low = -s.add(a, false);
@@ -704,7 +711,7 @@ bool shares_memory(const torch::Tensor& a, const torch::Tensor& b) {
     s.of[i][3] = below += s.of[i][0] * s.of[i][1];
     s.of[i][4] = above += s.of[i][0] * s.of[i][2];
   }
-  return s.meet(0, static_cast<int64_t>(reinterpret_cast<intptr_t>(a.data_ptr()) - reinterpret_cast<intptr_t>(b.data_ptr())));
+  return s.meet(0, distance);
 }
 
 // Forward-mode derivatives would be lost (or, of tensors written over, go stale).
